@@ -1,0 +1,395 @@
+// attention_packed.hip -- attention over packed sequences of different lengths with grouped heads,
+// forward and backward, with no scores in HBM.
+//
+//   s_ij = scale (q_i . k_j), lse_i = log sum_j exp(s_ij), out_i = sum_j exp(s_ij - lse_i) v_j
+//   p_ij = exp(s_ij - lse_i), delta_i = g_i . out_i, ds_ij = p_ij (g_i . v_j - delta_i)
+//   dv_j = sum_i p_ij g_i, dq_i = scale sum_j ds_ij k_j, dk_j = scale sum_i ds_ij q_i
+//
+// over the pairs (i, j) that the lengths and the causal mask let see each other. The offsets of the
+// sequences stay on the device: a launch has a block for every slot that a tile of rows could take
+// (find_tile), and a block without a tile ends at once.
+
+#include "common.hpp"
+
+#include <cmath>
+
+namespace ehip {
+namespace {
+
+constexpr int kMaxDim = 128;
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kRows = 64;  // rows (queries or keys) of one block
+
+struct Packed {
+    const float *q, *k, *v;
+    int64_t ld_q, ld_k, ld_v;
+    const int32_t *cu_q, *cu_k;
+    int sequences;
+    int total_q, total_k;
+    int heads, kv_heads, dim;
+    float scale;
+    int causal;
+    float* out;
+    int64_t ld_out;
+    float* lse;
+    const float* grad;
+    int64_t ld_grad;
+    float *dq, *dk, *dv;
+    int64_t ld_dq, ld_dk, ld_dv;
+    float* delta;  // (total_q, heads)
+};
+
+// A sequence's rows and the block's tile of them; rows == 0 where the block has none.
+struct Tile {
+    int q0, nq, k0, nk;  // first rows and lengths of the sequence
+    int first, rows;     // the tile, counted from the sequence's first row
+};
+
+__device__ __forceinline__ int offset_at(const int32_t* cu, int s, int total) {
+    const int x = cu[s];
+    return x < 0 ? 0 : (x > total ? total : x);
+}
+
+// The tile of slot `slot` when every sequence's rows (offsets cu) are cut into tiles of `size`.
+// Sequence s takes the slots from cu[s] / size + s on: that is at least one more for every
+// sequence before it than its tiles need, as ceil((b - a) / size) <= b / size - a / size + 1 in
+// whole numbers, so no sum over the sequences is needed to find a tile. The last s whose first
+// slot is not past `slot` is searched 64 candidates at a time, a lane each; every wave of the block
+// finds the same. Later tiles come first within a sequence: under a causal mask they are the
+// longest.
+__device__ __forceinline__ Tile find_tile(const Packed& a, bool keys, int slot, int size) {
+    const int32_t* cu = keys ? a.cu_k : a.cu_q;
+    const int total = keys ? a.total_k : a.total_q;
+    const int lane = int(threadIdx.x) & 63;
+    int lo = 0, n = a.sequences;  // the answer, if any, is in [lo, lo + n)
+    while (n > 0) {
+        const int step = (n + 63) / 64;
+        const int s = lo + lane * step;
+        const bool at = lane * step < n && offset_at(cu, s, total) / size + s <= slot;
+        const int c = __popcll(__ballot(at));
+        if (c == 0) break;
+        n = n - (c - 1) * step;
+        lo += (c - 1) * step;
+        n = n < step ? n : step;
+        if (step == 1) break;
+    }
+    Tile t{};
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    const int begin = offset_at(cu, lo, total);
+    int end = offset_at(cu, lo + 1, total);
+    end = end < begin ? begin : end;
+    const int tiles = (end - begin + size - 1) / size;
+    const int at = slot - (begin / size + lo);
+    if (at < 0 || at >= tiles) return t;
+    t.q0 = offset_at(a.cu_q, lo, a.total_q);
+    t.nq = offset_at(a.cu_q, lo + 1, a.total_q) - t.q0;
+    t.k0 = offset_at(a.cu_k, lo, a.total_k);
+    t.nk = offset_at(a.cu_k, lo + 1, a.total_k) - t.k0;
+    t.nq = t.nq < 0 ? 0 : t.nq;
+    t.nk = t.nk < 0 ? 0 : t.nk;
+    t.first = (tiles - 1 - at) * size;
+    t.rows = end - begin - t.first;
+    t.rows = t.rows < size ? t.rows : size;
+    return t;
+}
+
+// Keys that query i of the sequence sees: 0 .. count - 1.
+__device__ __forceinline__ int visible(const Packed& a, const Tile& t, int i) {
+    if (!a.causal) return t.nk;
+    const int64_t n = int64_t(i) + t.nk - t.nq + 1;
+    return n < 0 ? 0 : (n > t.nk ? t.nk : int(n));
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
+    return x;
+}
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+__device__ __forceinline__ float dot(const float* __restrict__ x, const float* __restrict__ y,
+                                     int n) {
+    float s = 0.0f;
+    for (int c = 0; c < n; ++c) s = __builtin_fmaf(x[c], y[c], s);
+    return s;
+}
+
+// ------------------------------------------------------- one row by one wave
+// The formulas as they stand, a lane for a key (or query) at a time and then a lane for a column;
+// only what the row sees is read.
+
+__device__ void forward_row(const Packed& a, const Tile& t, int h, int i) {
+    const int lane = int(threadIdx.x) & 63;
+    const int n = visible(a, t, i), c = h / (a.heads / a.kv_heads);
+    const float* q = a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim;
+    const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
+    const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
+    float m = -INFINITY;
+    bool bad = false;  // a score that is NaN: fmaxf passes over it
+    for (int j = lane; j < n; j += 64) {
+        const float s = dot(q, k + j * a.ld_k, a.dim) * a.scale;
+        m = fmaxf(m, s);
+        bad |= s != s;
+    }
+    m = wave_max(m);
+    if (__any(bad)) m = NAN;
+    float sum = 0.0f, acc[2] = {0.0f, 0.0f};
+    for (int j = lane; j < n; j += 64) sum += expf(dot(q, k + j * a.ld_k, a.dim) * a.scale - m);
+    sum = wave_sum(sum);
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        const int j = j0 + lane;
+        float p = 0.0f;  // divided here: the sums stay in range with v's values
+        if (j < n) p = expf(dot(q, k + j * a.ld_k, a.dim) * a.scale - m) / sum;
+        const int count = n - j0 < 64 ? n - j0 : 64;
+        for (int u = 0; u < count; ++u) {
+            const float w = __shfl(p, u);
+            const float* row = v + (j0 + u) * a.ld_v;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (lane + 64 * e < a.dim) acc[e] = __builtin_fmaf(w, row[lane + 64 * e], acc[e]);
+        }
+    }
+    float* out = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < a.dim) out[lane + 64 * e] = acc[e];
+    if (lane == 0)
+        a.lse[int64_t(t.q0 + i) * a.heads + h] = n == 0 ? -INFINITY : m + logf(sum);
+}
+
+__device__ float delta_of_row(const Packed& a, const Tile& t, int h, int i) {
+    const int lane = int(threadIdx.x) & 63;
+    const float* g = a.grad + int64_t(t.q0 + i) * a.ld_grad + int64_t(h) * a.dim;
+    const float* o = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
+    float s = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < a.dim) s = __builtin_fmaf(g[lane + 64 * e], o[lane + 64 * e], s);
+    return wave_sum(s);
+}
+
+// ds_ij, and p_ij through p.
+__device__ __forceinline__ float pair_gradient(const Packed& a, const float* q, const float* g,
+                                               const float* k, const float* v, float lse,
+                                               float delta, float& p) {
+    p = expf(dot(q, k, a.dim) * a.scale - lse);
+    return p * (dot(g, v, a.dim) - delta);
+}
+
+__device__ void dq_row(const Packed& a, const Tile& t, int h, int i, float delta) {
+    const int lane = int(threadIdx.x) & 63;
+    const int n = visible(a, t, i), c = h / (a.heads / a.kv_heads);
+    const int64_t row = t.q0 + i;
+    const float* q = a.q + row * a.ld_q + int64_t(h) * a.dim;
+    const float* g = a.grad + row * a.ld_grad + int64_t(h) * a.dim;
+    const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
+    const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
+    const float lse = a.lse[row * a.heads + h];
+    float acc[2] = {0.0f, 0.0f};
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        const int j = j0 + lane;
+        float p, ds = 0.0f;
+        if (j < n) ds = pair_gradient(a, q, g, k + j * a.ld_k, v + j * a.ld_v, lse, delta, p);
+        const int count = n - j0 < 64 ? n - j0 : 64;
+        for (int u = 0; u < count; ++u) {
+            const float w = __shfl(ds, u);
+            const float* x = k + (j0 + u) * a.ld_k;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (lane + 64 * e < a.dim) acc[e] = __builtin_fmaf(w, x[lane + 64 * e], acc[e]);
+        }
+    }
+    float* dq = a.dq + row * a.ld_dq + int64_t(h) * a.dim;
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < a.dim) dq[lane + 64 * e] = acc[e] * a.scale;
+}
+
+__device__ void dkv_row(const Packed& a, const Tile& t, int c, int j) {
+    const int lane = int(threadIdx.x) & 63, group = a.heads / a.kv_heads;
+    const int64_t row = t.k0 + j;
+    const float* k = a.k + row * a.ld_k + int64_t(c) * a.dim;
+    const float* v = a.v + row * a.ld_v + int64_t(c) * a.dim;
+    // The first query that sees key j.
+    int64_t start = a.causal ? int64_t(j) - t.nk + t.nq : 0;
+    start = start < 0 ? 0 : start;
+    float ak[2] = {0.0f, 0.0f}, av[2] = {0.0f, 0.0f};
+    for (int h = c * group; h < (c + 1) * group; ++h)
+        for (int64_t i0 = start; i0 < t.nq; i0 += 64) {
+            const int64_t i = i0 + lane;
+            float p = 0.0f, ds = 0.0f;
+            if (i < t.nq) {
+                const int64_t at = t.q0 + i;
+                ds = pair_gradient(a, a.q + at * a.ld_q + int64_t(h) * a.dim,
+                                   a.grad + at * a.ld_grad + int64_t(h) * a.dim, k, v,
+                                   a.lse[at * a.heads + h], a.delta[at * a.heads + h], p);
+            }
+            const int count = t.nq - i0 < 64 ? int(t.nq - i0) : 64;
+            for (int u = 0; u < count; ++u) {
+                const float wp = __shfl(p, u), wd = __shfl(ds, u);
+                const float* x = a.q + (t.q0 + i0 + u) * a.ld_q + int64_t(h) * a.dim;
+                const float* g = a.grad + (t.q0 + i0 + u) * a.ld_grad + int64_t(h) * a.dim;
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (lane + 64 * e < a.dim) {
+                        ak[e] = __builtin_fmaf(wd, x[lane + 64 * e], ak[e]);
+                        av[e] = __builtin_fmaf(wp, g[lane + 64 * e], av[e]);
+                    }
+            }
+        }
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        if (lane + 64 * e < a.dim) {
+            if (a.dk != nullptr)
+                a.dk[row * a.ld_dk + int64_t(c) * a.dim + lane + 64 * e] = ak[e] * a.scale;
+            if (a.dv != nullptr) a.dv[row * a.ld_dv + int64_t(c) * a.dim + lane + 64 * e] = av[e];
+        }
+}
+
+// ------------------------------------------------------------------- kernels
+// Block = slot * heads + head.
+
+__global__ __launch_bounds__(kThreads) void packed_forward(Packed a) {
+    const int h = int(blockIdx.x % a.heads);
+    const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kRows);
+    for (int i = int(threadIdx.x) / 64; i < t.rows; i += kWaves) forward_row(a, t, h, t.first + i);
+}
+
+__global__ __launch_bounds__(kThreads) void packed_backward_q(Packed a) {
+    const int h = int(blockIdx.x % a.heads);
+    const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kRows);
+    for (int r = int(threadIdx.x) / 64; r < t.rows; r += kWaves) {
+        const int i = t.first + r;
+        const float delta = delta_of_row(a, t, h, i);
+        if ((threadIdx.x & 63) == 0) a.delta[int64_t(t.q0 + i) * a.heads + h] = delta;
+        if (a.dq != nullptr) dq_row(a, t, h, i, delta);
+    }
+}
+
+__global__ __launch_bounds__(kThreads) void packed_backward_kv(Packed a) {
+    const int c = int(blockIdx.x % a.kv_heads);
+    const Tile t = find_tile(a, true, int(blockIdx.x / a.kv_heads), kRows);
+    for (int j = int(threadIdx.x) / 64; j < t.rows; j += kWaves) dkv_row(a, t, c, t.first + j);
+}
+
+// ---------------------------------------------------------------- host checks
+
+int64_t slots(int64_t total, int64_t sequences) { return total / kRows + sequences; }
+
+int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
+    if (d == nullptr) return fail(EHIP_EINVAL, "%s: null descriptor", name);
+    if (d->sequences < 0 || d->total_q < 0 || d->total_k < 0 || d->heads < 1 || d->kv_heads < 1 ||
+        d->heads % d->kv_heads != 0 || d->head_dim < 1 || d->head_dim > kMaxDim)
+        return fail(EHIP_EINVAL,
+                    "%s: %lld sequences, %lld and %lld rows, %lld heads over %lld of %lld values",
+                    name, (long long)d->sequences, (long long)d->total_q, (long long)d->total_k,
+                    (long long)d->heads, (long long)d->kv_heads, (long long)d->head_dim);
+    constexpr int64_t kBlocks = (int64_t(1) << 24) - 1;
+    if (d->heads > kBlocks || d->sequences > kBlocks || d->total_q > INT32_MAX ||
+        d->total_k > INT32_MAX ||
+        slots(d->total_q > d->total_k ? d->total_q : d->total_k, d->sequences) * d->heads > kBlocks)
+        return fail(EHIP_EINVAL, "%s: %lld x %lld rows of %lld heads are too many", name,
+                    (long long)d->total_q, (long long)d->total_k, (long long)d->heads);
+    const int64_t wide = d->heads * d->head_dim, narrow = d->kv_heads * d->head_dim;
+    if (d->ld_q < wide || d->ld_out < wide || d->ld_k < narrow || d->ld_v < narrow)
+        return fail(EHIP_EINVAL, "%s: leading dimension below the row's length", name);
+    if (d->sequences > 0 && (d->cu_q == nullptr || d->cu_k == nullptr))
+        return fail(EHIP_EINVAL, "%s: null offsets", name);
+    if ((d->total_q > 0 && (d->q == nullptr || d->out == nullptr || d->lse == nullptr)) ||
+        (d->total_k > 0 && (d->k == nullptr || d->v == nullptr)))
+        return fail(EHIP_EINVAL, "%s: null tensor", name);
+    a = Packed{};
+    a.q = d->q;
+    a.k = d->k;
+    a.v = d->v;
+    a.ld_q = d->ld_q;
+    a.ld_k = d->ld_k;
+    a.ld_v = d->ld_v;
+    a.cu_q = d->cu_q;
+    a.cu_k = d->cu_k;
+    a.sequences = int(d->sequences);
+    a.total_q = int(d->total_q);
+    a.total_k = int(d->total_k);
+    a.heads = int(d->heads);
+    a.kv_heads = int(d->kv_heads);
+    a.dim = int(d->head_dim);
+    a.scale = d->scale;
+    a.causal = d->causal != 0;
+    a.out = d->out;
+    a.ld_out = d->ld_out;
+    a.lse = d->lse;
+    return EHIP_OK;
+}
+
+}  // namespace
+}  // namespace ehip
+
+using namespace ehip;
+
+extern "C" {
+
+int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* stream) {
+    EHIP_READY();
+    Packed a;
+    if (int rc = fill("attention_packed", desc, a)) return rc;
+    if (a.sequences == 0 || a.total_q == 0) return EHIP_OK;
+    const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads);
+    EHIP_LAUNCH("attention_packed", packed_forward, dim3(blocks), dim3(kThreads), 0,
+                as_stream(stream), a);
+    return EHIP_OK;
+}
+
+int64_t ehip_attention_packed_backward_workspace(const ehip_attention_packed_t* desc) {
+    Packed a;
+    if (fill("attention_packed_backward", desc, a)) return -1;
+    return int64_t(a.total_q) * a.heads * int64_t(sizeof(float));
+}
+
+int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, const float* grad,
+                                       int64_t ld_grad, float* dq, int64_t ld_dq, float* dk,
+                                       int64_t ld_dk, float* dv, int64_t ld_dv, void* workspace,
+                                       size_t workspace_bytes, void* stream) {
+    EHIP_READY();
+    Packed a;
+    if (int rc = fill("attention_packed_backward", desc, a)) return rc;
+    if (a.sequences == 0) return EHIP_OK;
+    const int64_t wide = int64_t(a.heads) * a.dim, narrow = int64_t(a.kv_heads) * a.dim;
+    if (a.total_q > 0 && (grad == nullptr || ld_grad < wide))
+        return fail(EHIP_EINVAL, "attention_packed_backward: null gradient or a leading dimension "
+                                 "below the row's length");
+    if ((dq != nullptr && ld_dq < wide) || (dk != nullptr && ld_dk < narrow) ||
+        (dv != nullptr && ld_dv < narrow))
+        return fail(EHIP_EINVAL,
+                    "attention_packed_backward: leading dimension below the row's length");
+    const size_t need = size_t(a.total_q) * size_t(a.heads) * sizeof(float);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(EHIP_EINVAL,
+                    "attention_packed_backward: needs %zu bytes of 16-byte aligned workspace", need);
+    a.grad = grad;
+    a.ld_grad = ld_grad;
+    a.dq = dq;
+    a.dk = dk;
+    a.dv = dv;
+    a.ld_dq = ld_dq;
+    a.ld_dk = ld_dk;
+    a.ld_dv = ld_dv;
+    a.delta = static_cast<float*>(workspace);
+    if (a.total_q > 0 && (dq != nullptr || dk != nullptr)) {
+        const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads);
+        EHIP_LAUNCH("attention_packed_backward_q", packed_backward_q, dim3(blocks), dim3(kThreads),
+                    0, as_stream(stream), a);
+    }
+    if (a.total_k > 0 && (dk != nullptr || dv != nullptr)) {
+        const unsigned blocks = unsigned(slots(a.total_k, a.sequences) * a.kv_heads);
+        EHIP_LAUNCH("attention_packed_backward_kv", packed_backward_kv, dim3(blocks),
+                    dim3(kThreads), 0, as_stream(stream), a);
+    }
+    return EHIP_OK;
+}
+
+}  // extern "C"

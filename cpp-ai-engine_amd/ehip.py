@@ -81,6 +81,24 @@ class GemmEx(C.Structure):
                 ("residual", C.c_void_p), ("ld_residual", C.c_int64)]
 
 
+class AttentionPacked(C.Structure):
+    """ehip_attention_packed_t: packed sequences, grouped heads, and where the result goes."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("ld_q", C.c_int64),
+                ("ld_k", C.c_int64), ("ld_v", C.c_int64), ("cu_q", C.c_void_p),
+                ("cu_k", C.c_void_p), ("sequences", C.c_int64), ("total_q", C.c_int64),
+                ("total_k", C.c_int64), ("heads", C.c_int64), ("kv_heads", C.c_int64),
+                ("head_dim", C.c_int64), ("scale", C.c_float), ("causal", C.c_int),
+                ("out", C.c_void_p), ("ld_out", C.c_int64), ("lse", C.c_void_p)]
+
+
+class Cache(C.Structure):
+    """ehip_cache_t: the pools of a paged key-value cache and the sequences' page table."""
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("type", C.c_int),
+                ("pages", C.c_int64), ("page_size", C.c_int64), ("kv_heads", C.c_int64),
+                ("head_dim", C.c_int64), ("table", C.c_void_p), ("ld_table", C.c_int64),
+                ("table_width", C.c_int64), ("sequences", C.c_int64)]
+
+
 # name -> argtypes (all return int unless listed in _RESTYPES)
 _SIGS = {
     "ehip_init": [], "ehip_available": [], "ehip_enabled": [], "ehip_set_enabled": [_i],
@@ -179,9 +197,24 @@ _SIGS = {
     "ehip_cross_entropy_fused_supported": [_i64, _i64],
     "ehip_cross_entropy_fused_f32": [_vp] * 5 + [_i64, _i64, _vp],
     "ehip_softmax_xent_backward_f32": [_vp, _vp, _vp, _i64, _i64, _vp, _vp],
+    "ehip_attention_packed_f32": [C.POINTER(AttentionPacked), _vp],
+    "ehip_attention_packed_backward_workspace": [C.POINTER(AttentionPacked)],
+    "ehip_attention_packed_backward_f32": [C.POINTER(AttentionPacked)] + [_vp, _i64] * 4 +
+                                          [_vp, _sz, _vp],
+    "ehip_cache_append_f32": [C.POINTER(Cache), _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp],
+    "ehip_attention_paged_workspace": [C.POINTER(Cache), _i64, _i64],
+    "ehip_attention_paged_f32": [C.POINTER(Cache), _vp, _i64, _i64, _vp, _i64, _f, _vp, _i64,
+                                 _vp, _vp, _sz, _vp],
+    "ehip_token_logprobs_workspace": [_i64, _i64, _i64],
+    "ehip_token_logprobs_f32": [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp,
+                                _sz, _vp],
+    "ehip_token_logprobs_backward_f32": [_vp, _i64] + [_vp] * 6 + [_i64, _i64, _i64, _vp],
     "ehip_last_error": [],
 }
-_RESTYPES = {"ehip_last_error": C.c_char_p, "ehip_kernels_launched": C.c_uint64,
+_RESTYPES = {"ehip_last_error": C.c_char_p,
+             "ehip_attention_packed_backward_workspace": C.c_int64,
+             "ehip_attention_paged_workspace": C.c_int64,
+             "ehip_token_logprobs_workspace": C.c_int64, "ehip_kernels_launched": C.c_uint64,
              "ehip_conv2d_relu_maxpool_partials": C.c_int64,
              "ehip_layernorm_backward_partials": C.c_int64,
              "ehip_kernels_failed": C.c_uint64, "ehip_reset_counters": None,
@@ -737,3 +770,197 @@ class Backend:
                                                         self.p(dx), rows, cols, self.p(grad),
                                                         self.stream()), "softmax_xent_backward")
         return dx
+
+    # ------------------------------ packed sequences, a cache, token scores
+    def _here(self, *tensors):
+        """Refuses tensors that are not all on the current device (whose stream is used)."""
+        index = self.torch.cuda.current_device()
+        for t in tensors:
+            if t is not None and not (t.is_cuda and t.device.index == index):
+                raise ValueError(f"tensor on {t.device}, the current device is cuda:{index}")
+
+    def _rows(self, t, what, shape, dtype=None):
+        """The row pitch of a float32 tensor of this shape whose rows are dense (a column
+        range of a wider matrix may be passed), checked."""
+        if t.dtype != (dtype or self.torch.float32) or tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)}, expected "
+                             f"{dtype or self.torch.float32} {tuple(shape)}")
+        row = 1
+        for n, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            if n != 1 and stride != row:
+                raise ValueError(f"{what}: rows must be dense, strides are {t.stride()}")
+            row *= n
+        if t.shape[0] <= 1 or t.numel() == 0:
+            return row
+        if t.stride(0) < row:
+            raise ValueError(f"{what}: rows overlap, strides are {t.stride()}")
+        return t.stride(0)
+
+    def _index(self, t, what, *shape):
+        if t.dtype != self.torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)}, expected contiguous int32 "
+                             f"{shape}")
+        return _vp(t.data_ptr())
+
+    def _workspace(self, n, what):
+        """(tensor, pointer, bytes) of a call's own workspace of n bytes."""
+        if n < 0:
+            raise RuntimeError(f"{what} failed: {self.error()}")
+        if n == 0:
+            return None, None, 0
+        w = self.torch.empty(n, dtype=self.torch.uint8, device="cuda")
+        return w, _vp(w.data_ptr()), n
+
+    def _packed(self, q, k, v, cu_q, cu_k, scale, causal, out, lse):
+        if q.dim() != 3 or k.dim() != 3:
+            raise ValueError("q and k: expected (tokens, heads, head_dim)")
+        self._here(q, k, v, cu_q, cu_k, out, lse)
+        (tq, h, d), (tk, kv) = q.shape, k.shape[:2]
+        cu_k = cu_q if cu_k is None else cu_k
+        sequences = cu_q.numel() - 1
+        if sequences < 0:
+            raise ValueError("cu_q: expected one offset more than sequences")
+        return AttentionPacked(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), self._rows(q, "q", (tq, h, d)),
+            self._rows(k, "k", (tk, kv, d)), self._rows(v, "v", (tk, kv, d)),
+            self._index(cu_q, "cu_q", sequences + 1), self._index(cu_k, "cu_k", sequences + 1),
+            sequences, tq, tk, h, kv, d, d ** -0.5 if scale is None else scale, int(causal),
+            out.data_ptr(), self._rows(out, "out", (tq, h, d)), self._dense(lse, "lse", (tq, h)))
+
+    def _dense(self, t, what, shape, dtype=None):
+        if self._rows(t, what, shape, dtype) and not t.is_contiguous():
+            raise ValueError(f"{what}: expected a contiguous tensor")
+        return t.data_ptr()
+
+    def attention_packed(self, q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None,
+                         lse=None):
+        """Attention over packed sequences (ehip_attention_packed_f32): q (total_q, heads,
+        head_dim), k and v (total_k, kv_heads, head_dim), column ranges of a fused projection
+        allowed; cu_q, cu_k int32 offsets of the sequences on the device (cu_k: cu_q). scale:
+        head_dim ** -0.5. Returns (out, lse (total_q, heads)), written into `out` and `lse`
+        where given."""
+        out = self.f32(q.shape) if out is None else out
+        lse = self.f32(q.shape[:2]) if lse is None else lse
+        desc = self._packed(q, k, v, cu_q, cu_k, scale, causal, out, lse)
+        self.ok(self.lib.ehip_attention_packed_f32(C.byref(desc), self.stream()),
+                "attention_packed")
+        return out, lse
+
+    def attention_packed_backward(self, g, q, k, v, out, lse, cu_q, cu_k=None, scale=None,
+                                  causal=True, want=(True, True, True), grads=None):
+        """(dq, dk, dv) of attention_packed from its out and lse; None where `want` says so.
+        `grads`: tensors to write them into (rows may be column ranges)."""
+        desc = self._packed(q, k, v, cu_q, cu_k, scale, causal, out, lse)
+        if grads is None:
+            grads = [self.f32(t.shape) if w else None for t, w in zip((q, k, v), want)]
+        self._here(g, *grads)
+        args = []
+        for t, like, what in zip(grads, (q, k, v), ("dq", "dk", "dv")):
+            args += [None, 0] if t is None else [_vp(t.data_ptr()),
+                                                 self._rows(t, what, like.shape)]
+        need = self.lib.ehip_attention_packed_backward_workspace(C.byref(desc))
+        space, at, n = self._workspace(need, "attention_packed_backward")
+        self.ok(self.lib.ehip_attention_packed_backward_f32(
+            C.byref(desc), _vp(g.data_ptr()), self._rows(g, "g", q.shape), *args, at, n,
+            self.stream()), "attention_packed_backward")
+        return grads
+
+    def _cache(self, k_pages, v_pages, table):
+        self._here(k_pages, v_pages, table)
+        if k_pages.dim() != 4 or k_pages.dtype not in (self.torch.float32, self.torch.bfloat16):
+            raise ValueError("k_pages: expected float32 or bfloat16 (pages, page_size, kv_heads, "
+                             "head_dim)")
+        if (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype
+                or not k_pages.is_contiguous() or not v_pages.is_contiguous()):
+            raise ValueError("k_pages, v_pages: expected contiguous pools of one shape and type")
+        if table.dim() != 2:
+            raise ValueError("table: expected (sequences, pages of the longest)")
+        pages, size, kv, d = k_pages.shape
+        return Cache(k_pages.data_ptr(), v_pages.data_ptr(),
+                     int(k_pages.dtype == self.torch.bfloat16), pages, size, kv, d,
+                     table.data_ptr(), self._rows(table, "table", table.shape, self.torch.int32),
+                     table.shape[1], table.shape[0])
+
+    def cache_append(self, k, v, k_pages, v_pages, table, starts, cu=None):
+        """Writes tokens' keys and values (tokens, kv_heads, head_dim) into the pools
+        (pages, page_size, kv_heads, head_dim; float32 or bfloat16) at positions starts[s],
+        starts[s] + 1, ... of each sequence (ehip_cache_append_f32). cu: int32 offsets of the
+        sequences' tokens, None for one token each."""
+        cache = self._cache(k_pages, v_pages, table)
+        self._here(k, v, starts, cu)
+        tokens = k.shape[0]
+        if cu is None and tokens != cache.sequences:
+            raise ValueError(f"k: {tokens} tokens for {cache.sequences} sequences without cu")
+        shape = (tokens,) + tuple(k_pages.shape[2:])
+        self.ok(self.lib.ehip_cache_append_f32(
+            C.byref(cache), _vp(k.data_ptr()), self._rows(k, "k", shape), _vp(v.data_ptr()),
+            self._rows(v, "v", shape), self._index(starts, "starts", cache.sequences),
+            None if cu is None else self._index(cu, "cu", cache.sequences + 1), tokens,
+            self.stream()), "cache_append")
+
+    def attention_paged(self, q, k_pages, v_pages, table, lengths, longest=None, scale=None,
+                        out=None, lse=None):
+        """Attention of one new token per sequence over a paged cache
+        (ehip_attention_paged_f32): q (sequences, heads, head_dim); table int32 (sequences,
+        pages); lengths int32, at most `longest` (None: what the table holds). Returns
+        (out, lse (sequences, heads)), written into `out` and `lse` where given."""
+        if q.dim() != 3:
+            raise ValueError("q: expected (sequences, heads, head_dim)")
+        cache = self._cache(k_pages, v_pages, table)
+        out = self.f32(q.shape) if out is None else out
+        lse = self.f32(q.shape[:2]) if lse is None else lse
+        self._here(q, lengths, out, lse)
+        n, h, d = cache.sequences, q.shape[1], cache.head_dim
+        if longest is None:
+            longest = cache.table_width * cache.page_size
+        need = self.lib.ehip_attention_paged_workspace(C.byref(cache), h, longest)
+        space, at, size = self._workspace(need, "attention_paged")
+        self.ok(self.lib.ehip_attention_paged_f32(
+            C.byref(cache), _vp(q.data_ptr()), self._rows(q, "q", (n, h, d)), h,
+            self._index(lengths, "lengths", n), longest, d ** -0.5 if scale is None else scale,
+            _vp(out.data_ptr()), self._rows(out, "out", (n, h, d)),
+            _vp(self._dense(lse, "lse", (n, h))), at, size, self.stream()), "attention_paged")
+        return out, lse
+
+    def token_logprobs(self, logits, targets=None, top=0, want_entropy=True):
+        """Per row of logits (rows, vocab): (logprob of the int32 target, entropy, lse, the
+        `top` largest log probabilities, their int32 indices) (ehip_token_logprobs_f32); None
+        for what was not asked for."""
+        torch = self.torch
+        if logits.dim() != 2:
+            raise ValueError("logits: expected (rows, vocab)")
+        self._here(logits, targets)
+        rows, vocab = logits.shape
+        ld = self._rows(logits, "logits", (rows, vocab))
+        lse = self.f32((rows,))
+        logprob = None if targets is None else self.f32((rows,))
+        entropy = self.f32((rows,)) if want_entropy else None
+        best = self.f32((rows, top)) if top else None
+        index = torch.empty((rows, top), dtype=torch.int32, device="cuda") if top else None
+        need = self.lib.ehip_token_logprobs_workspace(rows, vocab, top)
+        space, at, size = self._workspace(need, "token_logprobs")
+        self.ok(self.lib.ehip_token_logprobs_f32(
+            _vp(logits.data_ptr()), ld,
+            None if targets is None else self._index(targets, "targets", rows), rows, vocab,
+            self.p(logprob), self.p(entropy), self.p(lse), top, self.p(best), self.p(index), at,
+            size, self.stream()), "token_logprobs")
+        return logprob, entropy, lse, best, index
+
+    def token_logprobs_backward(self, logits, targets, lse, entropy, g_logprob, g_entropy=None,
+                                dlogits=None):
+        """The logits' gradient from those of logprob and entropy and token_logprobs' lse and
+        entropy; `dlogits` may be `logits` itself."""
+        if logits.dim() != 2:
+            raise ValueError("logits: expected (rows, vocab)")
+        dlogits = self.f32(logits.shape) if dlogits is None else dlogits
+        entropy = None if g_entropy is None else entropy
+        self._here(logits, targets, lse, entropy, g_logprob, g_entropy, dlogits)
+        rows, vocab = logits.shape
+        part = lambda t, what: None if t is None else _vp(self._dense(t, what, (rows,)))
+        self.ok(self.lib.ehip_token_logprobs_backward_f32(
+            _vp(logits.data_ptr()), self._rows(logits, "logits", (rows, vocab)),
+            self._index(targets, "targets", rows), part(lse, "lse"), part(entropy, "entropy"),
+            part(g_logprob, "g_logprob"), part(g_entropy, "g_entropy"), _vp(dlogits.data_ptr()),
+            self._rows(dlogits, "dlogits", (rows, vocab)), rows, vocab, self.stream()),
+            "token_logprobs_backward")
+        return dlogits

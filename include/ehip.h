@@ -874,6 +874,148 @@ int ehip_cross_entropy_backward_f32(const float* probs, const int32_t* targets, 
 int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, float* dx,
                                    int64_t rows, int64_t cols, const float* grad, void* stream);
 
+/* ------------------------------- packed sequences, a cache, token scores */
+
+/* Attention over packed sequences of different lengths, with grouped heads,
+ * that stores no scores: beside the composition above (equal lengths, as many
+ * key heads as query heads, weights of seq x seq kept) for long or ragged
+ * batches. No counterpart in the reference.
+ *
+ * Sequence s owns rows [cu_q[s], cu_q[s + 1]) of q, out, lse (and of grad and
+ * dq) and rows [cu_k[s], cu_k[s + 1]) of k, v (dk, dv); the offsets are DEVICE
+ * arrays of sequences + 1 ascending int32 from 0 up, the last at most total_q
+ * or total_k. Query head h reads key head h / (heads / kv_heads). Query i of
+ * n_q sees key j of n_k when j < n_k and, with causal = 1, j <= i + n_k - n_q:
+ * the last query sees every key, so a prompt may come in pieces behind keys
+ * held from before.
+ *   s_ij = scale (q_i . k_j)    lse_i = log sum_j exp(s_ij)
+ *   out_i = sum_j exp(s_ij - lse_i) v_j
+ * over the keys seen. A row that sees none gets out = 0 and lse = -inf, and
+ * gives no gradient. Keys that a row does not see do not reach it, whatever
+ * they hold (NaN and infinities included). Rows of q past the last sequence
+ * leave out, lse and dq as they were, rows of k past it dk and dv.
+ *
+ * q, out, grad, dq are rows of heads * head_dim floats, ld_* floats apart (the
+ * queries of a fused projection are read and their gradient written in place);
+ * k, v, dk, dv rows of kv_heads * head_dim; lse is (total_q, heads), dense.
+ * Any alignment of a float. 1 <= head_dim <= 128; heads a multiple of
+ * kv_heads; at most 2^24 - 1 blocks of 64 rows and a head (else EHIP_EINVAL).
+ * Offsets out of range or descending are clamped, so nothing is read or
+ * written outside the tensors, but what the sequences they touch get is
+ * unspecified.
+ *
+ * The backward takes the forward's out and lse and writes (does not
+ * accumulate) each of dq, dk, dv that is not NULL:
+ *   p_ij = exp(s_ij - lse_i)    delta_i = grad_i . out_i
+ *   dv_j = sum_i p_ij grad_i    ds_ij = p_ij (grad_i . v_j - delta_i)
+ *   dq_i = scale sum_j ds_ij k_j    dk_j = scale sum_i ds_ij q_i
+ * dk and dv summed over the query heads of the group too. The outputs may not
+ * overlap the inputs or each other. `workspace` (device memory, 16-byte
+ * aligned) holds delta during the call: at least
+ * ehip_attention_packed_backward_workspace() bytes, of the call's own.
+ * Deterministic: no atomics, the sums' order goes by the lengths and sizes. */
+typedef struct {
+    const float *q, *k, *v;
+    int64_t ld_q, ld_k, ld_v;
+    const int32_t *cu_q, *cu_k;
+    int64_t sequences, total_q, total_k;
+    int64_t heads, kv_heads, head_dim;
+    float scale;
+    int causal;
+    float* out; /* written by the forward, read by the backward */
+    int64_t ld_out;
+    float* lse; /* likewise */
+} ehip_attention_packed_t;
+
+int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* stream);
+/* Bytes of workspace; -1 (with the error recorded) for a refused descriptor. */
+int64_t ehip_attention_packed_backward_workspace(const ehip_attention_packed_t* desc);
+int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, const float* grad,
+                                       int64_t ld_grad, float* dq, int64_t ld_dq, float* dk,
+                                       int64_t ld_dk, float* dv, int64_t ld_dv, void* workspace,
+                                       size_t workspace_bytes, void* stream);
+
+/* A cache of keys and values in pages, for producing one token at a time. The
+ * pools hold `pages` pages of page_size positions of (kv_heads, head_dim)
+ * values, dense, in fp32 or bf16; position p of sequence s is row p % page_size
+ * of page table[s * ld_table + p / page_size], table a DEVICE array of
+ * table_width int32 a sequence. Pages may be shared by sequences that only
+ * read them. The caller allots pages and keeps the lengths. No counterpart in
+ * the reference. */
+enum { EHIP_CACHE_F32 = 0, EHIP_CACHE_BF16 = 1 };
+
+typedef struct {
+    void *k_pages, *v_pages;
+    int type;
+    int64_t pages, page_size, kv_heads, head_dim;
+    const int32_t* table;
+    int64_t ld_table, table_width, sequences;
+} ehip_cache_t;
+
+/* Writes new keys and values into the pages: token t of sequence s, row
+ * cu[s] + t of k and v (rows of kv_heads * head_dim floats, ld_k and ld_v
+ * apart, `tokens` in all), goes to position starts[s] + t. cu (sequences + 1
+ * ascending int32) and starts (sequences) are DEVICE arrays; cu NULL is one
+ * token for each sequence (tokens = sequences). bf16 pools take the nearest
+ * bf16, ties to even. A token whose position is negative, past its table row or
+ * on a page outside the pool is not stored, nor are rows past the last
+ * sequence. Two tokens for one place leave either. */
+int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_k,
+                          const float* v, int64_t ld_v, const int32_t* starts,
+                          const int32_t* cu, int64_t tokens, void* stream);
+
+/* Attention of one new token per sequence over the cache: row s of q and out
+ * (heads * head_dim floats, ld_q and ld_out apart) sees positions 0 ..
+ * lengths[s] - 1 (a DEVICE array; write the new token's key and value first).
+ * out and lse (sequences, heads; may be NULL) as in
+ * ehip_attention_packed_f32. A length of zero gives out = 0, lse = -inf. A
+ * negative length, one past `longest` or its table row, or a page outside the
+ * pool makes the sequence's row NaN instead of a read out of bounds. `longest`,
+ * a host value, is what the work is split by: the same lengths under another
+ * `longest` may differ in the last bits.
+ * 1 <= head_dim <= 128, heads a multiple of kv_heads. `workspace` (16-byte
+ * aligned) holds the parts of a split length during the call: at least
+ * ehip_attention_paged_workspace() bytes, of the call's own (NULL where that is
+ * 0). Deterministic. */
+int64_t ehip_attention_paged_workspace(const ehip_cache_t* cache, int64_t heads,
+                                       int64_t longest);
+int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t ld_q,
+                             int64_t heads, const int32_t* lengths, int64_t longest,
+                             float scale, float* out, int64_t ld_out, float* lse,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens, one row of `vocab` logits each (rows ld
+ * floats apart), beside the mean loss of ehip_cross_entropy_f32: per row
+ *   lse = log sum_j exp(x_j)    logprob = x[target] - lse
+ *   entropy = lse - sum_j p_j x_j, p_j = exp(x_j - lse), a term of p_j = 0 is 0
+ * and the `top` largest logits' indices, by descending logit, equal ones by
+ * ascending index (-0 equals 0, NaN is above everything), with their log
+ * probabilities: top_logprob and top_index are (rows, top). logprob with
+ * targets, and entropy, may be NULL; 0 <= top <= min(vocab, 128). A target
+ * outside [0, vocab) makes its logprob NaN. Logits of -inf are tokens that
+ * cannot come. A row with nothing else has lse = -inf, entropy 0, every
+ * logprob -inf. A row with NaN or +inf has NaN for all but its indices.
+ * `workspace` (16-byte aligned) holds the parts of rows that are split over
+ * workgroups during the call: at least ehip_token_logprobs_workspace() bytes,
+ * of the call's own (NULL where that is 0). Deterministic. */
+int64_t ehip_token_logprobs_workspace(int64_t rows, int64_t vocab, int64_t top);
+int ehip_token_logprobs_f32(const float* logits, int64_t ld, const int32_t* targets,
+                            int64_t rows, int64_t vocab, float* logprob, float* entropy,
+                            float* lse, int64_t top, float* top_logprob, int32_t* top_index,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* The logits' gradient from the gradients of logprob and entropy (one per row;
+ * g_entropy, with entropy, may be NULL) and the forward's lse and entropy:
+ *   dx_j = g_logprob ([j = target] - p_j) - g_entropy p_j (x_j - lse + entropy)
+ * with p_j = 0 giving 0, so a row of -inf alone gives zeros. A target outside
+ * [0, vocab) makes its row NaN. dlogits, rows ld_dlogits apart, may be logits
+ * itself (with the same ld); no other overlap. */
+int ehip_token_logprobs_backward_f32(const float* logits, int64_t ld, const int32_t* targets,
+                                     const float* lse, const float* entropy,
+                                     const float* g_logprob, const float* g_entropy,
+                                     float* dlogits, int64_t ld_dlogits, int64_t rows,
+                                     int64_t vocab, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

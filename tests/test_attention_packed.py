@@ -1,0 +1,436 @@
+"""Attention over packed sequences with grouped heads, forward and backward, against the formula in
+64 bits with bounds from arithmetic (tests/_attention64.py), and what it refuses."""
+import ctypes as C
+import math
+
+import pytest
+
+import ehip as E
+from _attention64 import packed, within
+from _hip import print_case
+
+gpu = pytest.mark.gpu
+
+# (queries, keys) of each sequence.
+LENGTHS = {
+    "one": [(1, 1)],
+    "mixed": [(5, 5), (0, 3), (1, 1), (64, 64), (65, 65), (3, 0), (0, 0), (2, 130)],
+    "tiles": [(128, 128), (127, 127), (129, 129), (63, 191), (33, 32)],
+    "pieces": [(7, 100), (1, 300), (130, 450), (31, 31)],
+    "hidden": [(40, 25), (200, 70), (5, 1), (64, 1)],  # first queries that see no key
+    "long": [(600, 600), (1, 1), (257, 700)],
+}
+
+
+@pytest.fixture(scope="module")
+def hip():
+    import torch
+    if not torch.cuda.is_available():
+        pytest.fail("GPU test ran without a visible GPU")
+    return E.Backend()
+
+
+def offsets(lengths):
+    import torch
+    out = [0]
+    for n in lengths:
+        out.append(out[-1] + n)
+    return torch.tensor(out, dtype=torch.int32, device="cuda")
+
+
+def make(nq, nk, heads, kv, d, seed=0, fused=False, tail=0, spread=1.0):
+    """q, k, v, g on the GPU with `tail` rows past the last sequence."""
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen, device="cuda")
+    tq, tk = sum(nq) + tail, sum(nk) + tail
+    if fused and tq == tk:
+        rows = r(tq, heads + 2 * kv, d)
+        q, k, v = rows[:, :heads], rows[:, heads:heads + kv], rows[:, heads + kv:]
+    else:
+        q, k, v = r(tq, heads, d), r(tk, kv, d), r(tk, kv, d)
+    q.mul_(spread)
+    return q, k, v, r(tq, heads, d)
+
+
+def check(hip, nq, nk, heads, kv, d, causal, seed=0, fused=False, scale=None, spread=1.0):
+    print_case("packed", nq, nk, heads, kv, d, causal, seed, fused)
+    q, k, v, g = make(nq, nk, heads, kv, d, seed, fused, spread=spread)
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = hip.attention_packed(q, k, v, cq, ck, scale=scale, causal=causal)
+    grads = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck, scale=scale,
+                                          causal=causal)
+    value, bound = packed(q, k, v, nq, nk, d ** -0.5 if scale is None else scale, causal, g)
+    for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+        within(got, value[name], bound[name], name)
+
+
+@gpu
+@pytest.mark.parametrize("which", sorted(LENGTHS))
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("heads,kv,d", [(2, 2, 64), (6, 2, 32), (4, 1, 128), (3, 3, 24)])
+def test_lengths(hip, which, causal, heads, kv, d):
+    nq, nk = zip(*LENGTHS[which])
+    check(hip, nq, nk, heads, kv, d, causal, seed=hash((which, d)) % 1000)
+
+
+@gpu
+@pytest.mark.parametrize("d", [1, 2, 3, 7, 8, 16, 31, 33, 40, 63, 65, 72, 80, 95, 96, 97, 100, 112,
+                               127])
+def test_head_dims(hip, d):
+    check(hip, [70, 3, 129], [70, 40, 129], 4, 2, d, True, seed=d)
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv", [(1, 1), (8, 1), (5, 5), (9, 3), (16, 2), (12, 12)])
+def test_head_groups_in_a_fused_projection(hip, heads, kv):
+    check(hip, [50, 1, 0, 90], [50, 1, 0, 90], heads, kv, 48, True, seed=heads, fused=True)
+
+
+@gpu
+@pytest.mark.parametrize("scale,spread", [(1.0, 1.0), (0.0, 1.0), (-0.3, 2.0), (0.125, 40.0)])
+def test_scales_and_sharp_rows(hip, scale, spread):
+    """scale 0: even weights; spread 40: nearly one key a row, scores of some hundreds."""
+    check(hip, [100, 33], [100, 50], 2, 1, 64, True, seed=3, scale=scale, spread=spread)
+
+
+@gpu
+@pytest.mark.parametrize("count", [63, 64, 65, 200, 4097])
+def test_many_short_sequences(hip, count):
+    """More sequences than a wave has lanes, and than it has lanes times lanes, of 0 to 3 rows."""
+    nq = [(5 * i + i // 7) % 4 for i in range(count)]
+    check(hip, nq, nq, 2, 1, 16, True, seed=count)
+
+
+@gpu
+def test_one_offset_array_and_equal_heads(hip):
+    """cu_k left out; the same values as the framework's attention of equal lengths gives."""
+    import torch
+    print_case("packed against short")
+    b, s, h, d = 3, 48, 4, 24
+    q, k, v, g = make([s] * b, [s] * b, h, h, d, seed=8)
+    cu = offsets([s] * b)
+    out, lse = hip.attention_packed(q, k, v, cu)
+    grads = hip.attention_packed_backward(g, q, k, v, out, lse, cu)
+    flat = [t.reshape(b, s, h * d).contiguous() for t in (q, k, v, g)]
+    w, other = hip.attention_short(*flat[:3], h, d ** -0.5, True)
+    theirs = hip.attention_short_backward(*flat[:3], w, flat[3], h, d ** -0.5, True)
+    _, bound = packed(q, k, v, [s] * b, [s] * b, d ** -0.5, True, g)
+    for name, x, y in zip(("out", "dq", "dk", "dv"), (out, *grads), (other, *theirs)):
+        # Two results, each within the bound.
+        within(x, y.reshape(x.shape).cpu().double(), 2 * bound[name], name)
+
+
+@gpu
+@pytest.mark.parametrize("d", [32, 64, 100])
+def test_keys_that_are_not_seen_do_not_reach_a_row(hip, d):
+    """NaN and infinities in the keys and values past a row's own, and in other sequences."""
+    import torch
+    print_case("packed unseen", d)
+    nq, nk = [90, 70], [90, 130]
+    q, k, v, g = make(nq, nk, 4, 2, d, seed=d)
+    k[60:90], v[60:90] = math.nan, math.inf      # sequence 0: rows 60.. see them
+    k[90 + 100, 0], v[90 + 100, 1] = -math.inf, math.nan  # sequence 1: rows 40..
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = hip.attention_packed(q, k, v, cq, ck)
+    dq, _, _ = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck)
+    kz, vz = k.clone(), v.clone()
+    for t in (kz, vz):
+        t[60:90] = 0
+        t[90 + 100:] = 0
+    value, bound = packed(q, kz, vz, nq, nk, d ** -0.5, True, g)
+    for rows in (slice(0, 60), slice(90, 90 + 40)):
+        for name, got in (("out", out), ("lse", lse), ("dq", dq)):
+            within(got[rows], value[name][rows], bound[name][rows], f"{name} {rows}")
+    assert bool(torch.isnan(out[60:90]).all()) and bool(torch.isnan(lse[60:90]).all())
+
+
+@gpu
+def test_values_that_are_seen_and_not_finite(hip):
+    """As the formula has it: inf where a weight meets it, NaN where it has no value."""
+    import torch
+    print_case("packed not finite")
+    nq = [20]
+    q, k, v, _ = make(nq, nq, 2, 1, 64, seed=5)
+    v[10, 0, 3], v[12, 0, 4], v[14, 0, 5] = math.inf, -math.inf, math.nan
+    out, lse = hip.attention_packed(q, k, v, offsets(nq))
+    value, bound = packed(q, k, v, nq, nq, 0.125, True)
+    bound["out"] = torch.nan_to_num(bound["out"])
+    within(out, value["out"], bound["out"], "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e-38, 1e-30, 1e30, 2e38])
+def test_values_near_the_ends_of_the_range(hip, size):
+    """Values of 1e-38 keep an absolute 2^-126; larger ones their relative accuracy."""
+    import torch
+    print_case("packed range", size)
+    nq = [70, 9]
+    q, k, v, _ = make(nq, nq, 2, 2, 64, seed=6)
+    v.clamp_(-1, 1).mul_(size)
+    out, lse = hip.attention_packed(q, k, v, offsets(nq))
+    value, bound = packed(q, k, v, nq, nq, 0.125, True)
+    within(out, value["out"], bound["out"] + 2.0 ** -126, "out")
+
+
+@gpu
+def test_rows_past_the_last_sequence_are_left(hip):
+    import torch
+    print_case("packed tail")
+    nq, nk, tail = [30, 65], [30, 90], 70
+    q, k, v, g = make(nq, nk, 2, 1, 40, seed=7, tail=tail)
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    grads = [torch.full_like(t, 7.0) for t in (q, k, v)]
+    hip.attention_packed(q, k, v, cq, ck, out=out, lse=lse)
+    hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck, grads=grads)
+    for t in (out, lse, *grads):
+        assert bool((t[-tail:] == 7.0).all())
+    a, b = sum(nq), sum(nk)
+    value, bound = packed(q[:a], k[:b], v[:b], nq, nk, 40 ** -0.5, True, g[:a])
+    for name, x in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+        within(x[:-tail], value[name], bound[name], name)
+
+
+@gpu
+def test_gradients_into_a_fused_projection(hip):
+    """dq, dk, dv written as columns of one matrix; columns beside them stay."""
+    import torch
+    print_case("packed fused gradients")
+    nq, h, kv, d = [40, 77], 4, 2, 33
+    q, k, v, g = make(nq, nq, h, kv, d, seed=9)
+    cu = offsets(nq)
+    out, lse = hip.attention_packed(q, k, v, cu)
+    want = hip.attention_packed_backward(g, q, k, v, out, lse, cu)
+    rows = torch.full((sum(nq), h + 2 * kv + 1, d), 5.0, device="cuda")
+    into = [rows[:, :h], rows[:, h:h + kv], rows[:, h + kv:h + 2 * kv]]
+    hip.attention_packed_backward(g, q, k, v, out, lse, cu, grads=into)
+    for x, y in zip(into, want):
+        assert torch.equal(x, y)
+    assert bool((rows[:, -1] == 5.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("want", [(True, False, False), (False, True, False), (False, False, True),
+                                  (False, False, False)])
+def test_parts_of_the_backward(hip, want):
+    import torch
+    print_case("packed parts", want)
+    nq, nk = [40, 77], [50, 77]
+    q, k, v, g = make(nq, nk, 4, 2, 64, seed=10)
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = hip.attention_packed(q, k, v, cq, ck)
+    every = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck)
+    some = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck, want=want)
+    for w, x, y in zip(want, some, every):
+        assert (x is None) == (not w) and (x is None or torch.equal(x, y))
+
+
+@gpu
+def test_gradients_against_differences(hip):
+    """f = sum(out g): (f(x + e) - f(x - e)) / 2 e along a direction, f from the 64-bit forward of
+    the same inputs, against the kernel's gradient; e = 1e-4 leaves e^2 of the third derivative,
+    far below the 1e-4 of the gradient's norm that is allowed."""
+    import torch
+    print_case("packed differences")
+    nq, nk, d = [20, 9], [33, 9], 16
+    q, k, v, g = make(nq, nk, 4, 2, d, seed=11)
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = hip.attention_packed(q, k, v, cq, ck)
+    grads = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck)
+    base = [t.cpu().double() for t in (q, k, v)]
+    gen = torch.Generator().manual_seed(1)
+    for i, got in enumerate(grads):
+        step = torch.randn(base[i].shape, generator=gen, dtype=torch.float64)
+        f = []
+        for e in (1e-4, -1e-4):
+            x = [t + e * step if j == i else t for j, t in enumerate(base)]
+            f.append(float((packed(*x, nq, nk, d ** -0.5, True)[0]["out"] * g.cpu()).sum()))
+        slope = (f[0] - f[1]) / 2e-4
+        got = got.cpu().double()
+        assert abs(float((got * step).sum()) - slope) <= 1e-4 * float(got.norm() * step.norm())
+
+
+@gpu
+def test_same_bits_each_time_and_on_another_stream(hip):
+    import torch
+    print_case("packed repeat")
+    nq, nk = [300, 65, 1], [300, 300, 1]
+    q, k, v, g = make(nq, nk, 4, 2, 64, seed=12)
+    cq, ck = offsets(nq), offsets(nk)
+
+    def both():
+        out, lse = hip.attention_packed(q, k, v, cq, ck)
+        return [out, lse, *hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck)]
+
+    first = both()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    others = []
+    for s in streams:  # two calls at once
+        with torch.cuda.stream(s):
+            others.append(both())
+    torch.cuda.synchronize()
+    for other in others:
+        for x, y in zip(first, other):
+            assert torch.equal(x, y)
+
+
+@gpu
+def test_captured_and_replayed(hip):
+    import torch
+    print_case("packed graph")
+    nq, nk = [100, 33], [150, 33]
+    q, k, v, g = make(nq, nk, 4, 2, 64, seed=13)
+    cq, ck = offsets(nq), offsets(nk)
+
+    def both():
+        out, lse = hip.attention_packed(q, k, v, cq, ck)
+        return [out, lse, *hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck)]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # each with a workspace of its own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = both()
+        graphs.append((graph, outs))
+    for seed in range(3):
+        fresh = make(nq, nk, 4, 2, 64, seed=20 + seed)
+        for t, f in zip((q, k, v, g), fresh):
+            t.copy_(f)
+        want = both()
+        for graph, outs in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for graph, outs in graphs:
+            for x, y in zip(outs, want):
+                assert torch.equal(x, y)
+
+
+@gpu
+def test_offsets_out_of_range_stay_inside_the_tensors(hip):
+    """Negative, descending and too large offsets are clamped: rows around the tensors stay."""
+    import torch
+    print_case("packed offsets")
+    n, pad, h, d = 96, 64, 2, 32
+    big = [torch.full((n + 2 * pad, h, d), 3.0, device="cuda") for _ in range(7)]
+    q, k, v, g, dq, dk, dv = (t[pad:pad + n] for t in big)
+    out = torch.full((n + 2 * pad, h, d), 3.0, device="cuda")
+    lse = torch.full((n + 2 * pad, h), 3.0, device="cuda")
+    for bad in ([0, 200], [-5, 40], [0, 50, 20, 96], [90, 10], [2 ** 31 - 1, -2 ** 31, 96]):
+        cu = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        hip.attention_packed(q, k, v, cu, out=out[pad:pad + n], lse=lse[pad:pad + n])
+        hip.attention_packed_backward(g, q, k, v, out[pad:pad + n], lse[pad:pad + n], cu,
+                                      grads=[dq, dk, dv])
+        torch.cuda.synchronize()
+        for t in (*big, out, lse):
+            assert bool((t[:pad] == 3.0).all()) and bool((t[pad + n:] == 3.0).all())
+
+
+@gpu
+def test_empty_tensors(hip):
+    import torch
+    print_case("packed empty")
+    none = lambda h: torch.empty(0, h, 16, device="cuda")
+    some = torch.randn(9, 2, 16, device="cuda")
+    cu0 = torch.zeros(3, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 4, 9], dtype=torch.int32, device="cuda")
+    out, lse = hip.attention_packed(none(4), some, some, cu0, cu)
+    assert out.shape == (0, 4, 16)
+    grads = hip.attention_packed_backward(none(4), none(4), some, some, out, lse, cu0, cu)
+    assert bool((grads[1] == 0).all()) and bool((grads[2] == 0).all())
+    q = torch.randn(9, 4, 16, device="cuda")
+    out, lse = hip.attention_packed(q, none(2), none(2), cu, cu0)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    dq, dk, dv = hip.attention_packed_backward(q, q, none(2), none(2), out, lse, cu, cu0)
+    assert bool((dq == 0).all()) and dk.shape == (0, 2, 16)
+    hip.attention_packed(none(1), none(1), none(1), torch.zeros(1, dtype=torch.int32,
+                                                               device="cuda"))
+
+
+# ----------------------------------------------------------------- refusals
+
+def descriptor(**changes):
+    fields = dict(q=4096, k=4096, v=4096, ld_q=64, ld_k=32, ld_v=32, cu_q=4096, cu_k=4096,
+                  sequences=2, total_q=10, total_k=12, heads=4, kv_heads=2, head_dim=16, scale=1.0,
+                  causal=1, out=4096, ld_out=64, lse=4096)
+    fields.update(changes)
+    return E.AttentionPacked(**fields)
+
+
+def test_workspace_and_refused_descriptors():
+    """The checks that every call starts with, through the query that needs no device."""
+    lib = E.load_library()
+    size = lib.ehip_attention_packed_backward_workspace
+    assert size(C.byref(descriptor())) == 10 * 4 * 4
+    assert size(C.byref(descriptor(total_q=0, q=None, out=None, lse=None))) == 0
+    assert size(None) == -1
+    for bad in (dict(heads=3), dict(heads=0, kv_heads=0), dict(head_dim=0), dict(head_dim=129),
+                dict(ld_q=63), dict(ld_k=31), dict(ld_v=31), dict(ld_out=63), dict(q=None),
+                dict(k=None), dict(v=None), dict(out=None), dict(lse=None), dict(cu_q=None),
+                dict(cu_k=None), dict(sequences=-1), dict(total_q=-1), dict(total_k=-1),
+                dict(total_q=2 ** 31), dict(total_k=2 ** 31), dict(sequences=2 ** 24),
+                dict(total_q=2 ** 30), dict(kv_heads=-2, heads=-4)):
+        assert size(C.byref(descriptor(**bad))) == -1, bad
+        assert b"attention_packed" in lib.ehip_last_error()
+
+
+def binding():
+    """A Backend without a device: its argument checks only."""
+    import torch
+    b = E.Backend.__new__(E.Backend)
+    b.torch, b.lib = torch, E.load_library()
+    return b
+
+
+def test_binding_refuses_layouts():
+    import torch
+    b = binding()
+    rows = torch.zeros(6, 10, 8)
+    assert b._rows(rows[:, :4], "q", (6, 4, 8)) == 80
+    assert b._rows(rows[:1, 4:6], "q", (1, 2, 8)) == 16
+    for bad in (rows[:, ::2], rows[:, :, ::2], rows.transpose(0, 1), rows.double(),
+                rows[:, :, :1].expand(6, 10, 8), torch.zeros(1, 4, 8).expand(6, 4, 8)):
+        with pytest.raises(ValueError):
+            b._rows(bad, "q", tuple(bad.shape))
+    with pytest.raises(ValueError):
+        b._rows(rows, "q", (6, 10, 9))
+    with pytest.raises(ValueError):
+        b._index(torch.zeros(3), "cu", 3)
+    with pytest.raises(ValueError):
+        b._index(torch.zeros(6, dtype=torch.int32)[::2], "cu", 3)
+    with pytest.raises(ValueError):
+        b._dense(rows[:, :4, 0], "lse", (6, 4))
+
+
+@gpu
+def test_calls_are_refused(hip):
+    """Before anything is launched, with the reason."""
+    import torch
+    print_case("packed refusals")
+    q, k, v, g = make([4], [4], 2, 1, 16, seed=1)
+    cu = offsets([4])
+    out, lse = hip.attention_packed(q, k, v, cu)
+    launched = hip.launched()
+    for args in ((q, k, v[:3], cu), (q, k, v, cu.long()), (q[0], k, v, cu),
+                 (q.cpu(), k, v, cu), (q, k, v, cu, offsets([2, 2]))):
+        with pytest.raises(ValueError):
+            hip.attention_packed(*args)
+    with pytest.raises(RuntimeError, match="heads"):
+        hip.attention_packed(torch.zeros(4, 3, 16, device="cuda"), torch.zeros(4, 2, 16,
+                             device="cuda"), torch.zeros(4, 2, 16, device="cuda"), cu)
+    with pytest.raises(RuntimeError, match="129"):
+        hip.attention_packed(*[torch.zeros(4, 1, 129, device="cuda")] * 3, cu)
+    desc = hip._packed(q, k, v, cu, None, None, True, out, lse)
+    space = torch.empty(64, device="cuda")
+    call = lambda at, n: hip.lib.ehip_attention_packed_backward_f32(
+        C.byref(desc), g.data_ptr(), 32, out.data_ptr(), 32, None, 0, None, 0, at, n,
+        hip.stream())
+    assert call(None, 0) == 1 and call(space.data_ptr(), 31) == 1
+    assert call(space.data_ptr() + 4, 64) == 1 and "workspace" in hip.error()
+    assert hip.launched() == launched
