@@ -9,6 +9,7 @@
 // sequences stay on the device: a launch has a block for every slot that a tile of rows could take
 // (find_tile), and a block without a tile ends at once.
 
+#include "attention_tile.hpp"
 #include "common.hpp"
 
 #include <cmath>
@@ -19,7 +20,8 @@ namespace {
 constexpr int kMaxDim = 128;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kRows = 64;  // rows (queries or keys) of one block
+constexpr int kRows = 64;     // rows (queries or keys) of one block of the backward
+constexpr int kQueries = 128;  // queries of one block of the forward, 32 a wave
 
 struct Packed {
     const float *q, *k, *v;
@@ -252,12 +254,163 @@ __device__ void dkv_row(const Packed& a, const Tile& t, int c, int j) {
 }
 
 // ------------------------------------------------------------------- kernels
-// Block = slot * heads + head.
+// Block = slot * heads + head, the heads of one key head 8 (or any multiple of the key heads) apart:
+// with the dispatcher's round robin over the eight XCDs they meet their keys in one L2.
 
-__global__ __launch_bounds__(kThreads) void packed_forward(Packed a) {
-    const int h = int(blockIdx.x % a.heads);
-    const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kRows);
-    for (int i = int(threadIdx.x) / 64; i < t.rows; i += kWaves) forward_row(a, t, h, t.first + i);
+__device__ __forceinline__ int head_of(const Packed& a, int x) {
+    return x % a.kv_heads * (a.heads / a.kv_heads) + x / a.kv_heads;
+}
+
+template <int DP, int BN, bool VEC>
+__global__ __launch_bounds__(kThreads, 2) void packed_forward(Packed a) {
+    using namespace attention;
+    using KeyTile = RowTile<BN, DP, kThreads, VEC>;
+    using ValueTile = ColTile<BN, DP, kThreads>;
+    __shared__ __attribute__((aligned(16))) char lds[KeyTile::kBytes + ValueTile::kBytes];
+    char* const lds_v = lds + KeyTile::kBytes;
+    const int h = head_of(a, int(blockIdx.x % a.heads));
+    const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kQueries);
+    if (t.rows == 0) return;
+    const int c = h / (a.heads / a.kv_heads);
+    const int wave = int(threadIdx.x) / 64, lane = int(threadIdx.x) & 63;
+    const int mine = 32 * wave + (lane & 31);  // the lane's query, of the tile
+    const int i = t.first + (mine < t.rows ? mine : t.rows - 1);
+    const int limit = visible(a, t, i);
+    const int last = 32 * wave + 31 < t.rows ? 32 * wave + 31 : t.rows - 1;
+    const int end = visible(a, t, t.first + t.rows - 1);
+    const int wave_end = 32 * wave < t.rows ? visible(a, t, t.first + last) : 0;
+    const int wave_all = visible(a, t, t.first + 32 * wave);  // keys that all its queries see
+
+    // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q. Weights are 2^-24 of
+    // their value, so that sums over the values stay in their range.
+    const float c2 = fabsf(a.scale) * 1.44269504088896340736f;
+    bf16x8 q[DP / 16][3];
+    own_row<DP, VEC>(a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim, a.dim,
+                     a.scale < 0.0f ? -1.0f : 1.0f, q);
+    floatx16 o[DP / 32];
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) o[db] = zeros();
+    float top = -INFINITY, shift = 24.0f, sum = 0.0f;
+
+    const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
+    const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
+    const int ld_k = int(a.ld_k), ld_v = int(a.ld_v);
+    KeyTile kt;
+    ValueTile vt;
+    if (end > 0) {
+        kt.load(k, ld_k, t.nk, a.dim);
+        vt.load(v, ld_v, t.nk, a.dim);
+    }
+    for (int j0 = 0; j0 < end; j0 += BN) {
+        __syncthreads();
+        kt.store(lds, t.nk - j0, a.dim);
+        vt.store(lds_v, t.nk - j0, a.dim);
+        const int j1 = j0 + BN;
+        if (j1 < end) {
+            kt.load(k + int64_t(j1) * ld_k, ld_k, t.nk - j1, a.dim);
+            vt.load(v + int64_t(j1) * ld_v, ld_v, t.nk - j1, a.dim);
+        }
+        __syncthreads();
+        if (j0 >= wave_end) continue;
+        floatx16 s[BN / 32];
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b) s[b] = zeros();
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b) {
+                bf16x8 f[3];
+                KeyTile::block(lds, b, ks, f);
+                multiply(s[b], f, q[ks]);
+            }
+        if (j1 > wave_all) {
+#pragma unroll
+            for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (j0 + 32 * b + row_of(r) >= limit) s[b][r] = -INFINITY;
+        }
+        float m = top;
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
+        m = fmaxf(m, __shfl_xor(m, 32));
+        const float next = m == -INFINITY ? 24.0f : __builtin_fmaf(m, c2, 24.0f);
+        const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - next);
+        top = m;
+        shift = next;
+        float part = 0.0f;
+        bf16x8 p[BN / 16][3];
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b) {
+            float w[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], c2, -shift));
+                part += w[r];
+            }
+            split8(w, p[2 * b]);
+            split8(w + 8, p[2 * b + 1]);
+        }
+        sum = __builtin_fmaf(sum, keep, part);
+        // The tile's sum apart from the running one: that is rounded to nearest once a tile, where
+        // the instruction drops low bits towards minus infinity.
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+            floatx16 x = zeros();
+#pragma unroll
+            for (int u = 0; u < BN / 16; ++u) {
+                bf16x8 f[3];
+                ValueTile::block(lds_v, db, u, f);
+                multiply(x, f, p[u]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[db][r] = __builtin_fmaf(o[db][r], keep, x[r]);
+        }
+    }
+
+    // Rows that saw something and have no finite result are formed again by the formula: a NaN or
+    // an infinity where it counts, or one in a place of theirs that they do not see (0 times it).
+    sum += __shfl_xor(sum, 32);
+    const float inv = limit > 0 ? 1.0f / sum : 0.0f;
+    bool fine = sum > 0.0f && sum < INFINITY;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            o[db][r] *= inv;
+            fine = fine && fabsf(o[db][r]) < INFINITY;
+        }
+    fine = fine || limit == 0;
+    const uint64_t again = __ballot(!fine && mine < t.rows);
+    if (mine < t.rows) {
+        float* out = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int d = 32 * db + row_of(r);
+                if (VEC) {
+                    if (d < a.dim)
+                        *reinterpret_cast<floatx4u*>(out + d) =
+                            floatx4u{o[db][r], o[db][r + 1], o[db][r + 2], o[db][r + 3]};
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < a.dim) out[d + e] = o[db][r + e];
+                }
+            }
+        // shift ln 2 in two parts: ln 2 = hi + lo.
+        if (lane < 32)
+            a.lse[int64_t(t.q0 + i) * a.heads + h] =
+                limit == 0 ? -INFINITY
+                           : __builtin_fmaf(shift, 0.693147182464599609375f,
+                                            __builtin_fmaf(shift, -1.904654323148236017e-9f,
+                                                           logf(sum)));
+    }
+    for (uint32_t rows = uint32_t(again) | uint32_t(again >> 32); rows != 0; rows &= rows - 1)
+        forward_row(a, t, h, t.first + 32 * wave + __builtin_ctz(rows));
 }
 
 __global__ __launch_bounds__(kThreads) void packed_backward_q(Packed a) {
@@ -279,7 +432,12 @@ __global__ __launch_bounds__(kThreads) void packed_backward_kv(Packed a) {
 
 // ---------------------------------------------------------------- host checks
 
-int64_t slots(int64_t total, int64_t sequences) { return total / kRows + sequences; }
+int64_t slots(int64_t total, int64_t sequences, int rows = kRows) {
+    return total / rows + sequences;
+}
+
+// Tiles address their rows by 32-bit byte offsets from the first one.
+constexpr int64_t kMaxLd = int64_t(1) << 22;
 
 int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
     if (d == nullptr) return fail(EHIP_EINVAL, "%s: null descriptor", name);
@@ -296,8 +454,10 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
         return fail(EHIP_EINVAL, "%s: %lld x %lld rows of %lld heads are too many", name,
                     (long long)d->total_q, (long long)d->total_k, (long long)d->heads);
     const int64_t wide = d->heads * d->head_dim, narrow = d->kv_heads * d->head_dim;
-    if (d->ld_q < wide || d->ld_out < wide || d->ld_k < narrow || d->ld_v < narrow)
-        return fail(EHIP_EINVAL, "%s: leading dimension below the row's length", name);
+    if (d->ld_q < wide || d->ld_out < wide || d->ld_k < narrow || d->ld_v < narrow ||
+        d->ld_q > kMaxLd || d->ld_k > kMaxLd || d->ld_v > kMaxLd)
+        return fail(EHIP_EINVAL, "%s: leading dimension below the row's length or above 2^22",
+                    name);
     if (d->sequences > 0 && (d->cu_q == nullptr || d->cu_k == nullptr))
         return fail(EHIP_EINVAL, "%s: null offsets", name);
     if ((d->total_q > 0 && (d->q == nullptr || d->out == nullptr || d->lse == nullptr)) ||
@@ -326,6 +486,14 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
     return EHIP_OK;
 }
 
+template <int DP, int BN, bool VEC>
+int launch_forward(const Packed& a, hipStream_t s) {
+    const unsigned blocks = unsigned(slots(a.total_q, a.sequences, kQueries) * a.heads);
+    EHIP_LAUNCH("attention_packed", (packed_forward<DP, BN, VEC>), dim3(blocks), dim3(kThreads), 0,
+                s, a);
+    return EHIP_OK;
+}
+
 }  // namespace
 }  // namespace ehip
 
@@ -338,10 +506,15 @@ int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* stream)
     Packed a;
     if (int rc = fill("attention_packed", desc, a)) return rc;
     if (a.sequences == 0 || a.total_q == 0) return EHIP_OK;
-    const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads);
-    EHIP_LAUNCH("attention_packed", packed_forward, dim3(blocks), dim3(kThreads), 0,
-                as_stream(stream), a);
-    return EHIP_OK;
+    const bool vec = a.dim % 8 == 0;
+    if (a.dim <= 32) return vec ? launch_forward<32, 64, true>(a, as_stream(stream))
+                                : launch_forward<32, 64, false>(a, as_stream(stream));
+    if (a.dim <= 64) return vec ? launch_forward<64, 64, true>(a, as_stream(stream))
+                                : launch_forward<64, 64, false>(a, as_stream(stream));
+    if (a.dim <= 96) return vec ? launch_forward<96, 64, true>(a, as_stream(stream))
+                                : launch_forward<96, 64, false>(a, as_stream(stream));
+    return vec ? launch_forward<128, 32, true>(a, as_stream(stream))
+               : launch_forward<128, 32, false>(a, as_stream(stream));
 }
 
 int64_t ehip_attention_packed_backward_workspace(const ehip_attention_packed_t* desc) {

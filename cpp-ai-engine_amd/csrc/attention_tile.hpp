@@ -1,0 +1,233 @@
+// attention_tile.hpp -- the pieces of attention on the matrix instructions: rows of fp32 values in
+// three bf16 parts (gemm_split.hpp: 24 bits, six of the nine part products, fp32 sums), in
+// registers for the rows that a wave owns and in LDS for the rows that stream past.
+//
+// v_mfma_f32_32x32x16_bf16, D = A B + C: lane l holds A(l % 32, 8 (l / 32) + 0..7), B(8 (l / 32) +
+// 0..7, l % 32) and D(8 (r / 4) + 4 (l / 32) + r % 4, l % 32) in register r. A wave's own rows are
+// the columns of every product, so a lane has one of them throughout: row sums are sums over the
+// lane's registers and its partner's (l ^ 32), and a product's D is the next one's B as it stands,
+// but for the order of its 16 rows, which the next one's A follows (ColTile).
+#ifndef EHIP_ATTENTION_TILE_HPP
+#define EHIP_ATTENTION_TILE_HPP
+
+#include "gemm_split.hpp"
+
+namespace ehip {
+namespace attention {
+
+using gemm_detail::bf16x8;
+using gemm_detail::floatx4u;
+using gemm_detail::global_bytes;
+using gemm_detail::global_load;
+using gemm_detail::split_pair;
+using gemm_detail::uintx4;
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+
+// The six part products, the smallest first.
+constexpr int kPart[6][2] = {{1, 1}, {2, 0}, {0, 2}, {0, 1}, {1, 0}, {0, 0}};
+
+// Eight values in three parts, eight bf16 to a register quadruple. Unlike a product's tile they are not
+// scaled: values below 2^-110 lose what is below 2^-133.
+__device__ __forceinline__ void split8(const float* x, bf16x8 (&part)[3]) {
+    uintx4 h, m, l;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        uint32_t hj, mj, lj;
+        split_pair(x[2 * j], x[2 * j + 1], hj, mj, lj);
+        h[j] = hj;
+        m[j] = mj;
+        l[j] = lj;
+    }
+    part[0] = __builtin_bit_cast(bf16x8, h);
+    part[1] = __builtin_bit_cast(bf16x8, m);
+    part[2] = __builtin_bit_cast(bf16x8, l);
+}
+
+// d += the product of two blocks of 32 x 16.
+__device__ __forceinline__ void multiply(floatx16& d, const bf16x8 (&a)[3], const bf16x8 (&b)[3]) {
+#pragma unroll
+    for (int q = 0; q < 6; ++q)
+        d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[kPart[q][0]], b[kPart[q][1]], d, 0, 0, 0);
+}
+
+__device__ __forceinline__ floatx16 zeros() {
+    floatx16 z;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) z[r] = 0.0f;
+    return z;
+}
+
+// Row (of 32) of register r of a lane's D.
+__device__ __forceinline__ int row_of(int r) {
+    return 8 * (r / 4) + 4 * ((int(threadIdx.x) & 63) / 32) + r % 4;
+}
+
+// The lane's own row (a pointer to its `dim` values) as the B operand of products over the head's
+// values: DP / 16 blocks. VEC: dim is a multiple of 8.
+template <int DP, bool VEC>
+__device__ __forceinline__ void own_row(const float* row, int dim, float factor,
+                                        bf16x8 (&b)[DP / 16][3]) {
+    const int half = (int(threadIdx.x) & 63) / 32;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d0 = 16 * ks + 8 * half;
+        float x[8];
+        if (VEC) {
+            const bool in = d0 < dim;
+            const float* p = row + (in ? d0 : 0);
+            const floatx4u u = *reinterpret_cast<const floatx4u*>(p);
+            const floatx4u v = *reinterpret_cast<const floatx4u*>(p + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                x[j] = in ? u[j] * factor : 0.0f;
+                x[4 + j] = in ? v[j] * factor : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool in = d0 + j < dim;
+                const float v = row[in ? d0 + j : 0];
+                x[j] = in ? v * factor : 0.0f;
+            }
+        }
+        split8(x, b[ks]);
+    }
+}
+
+// ROWS streamed rows as the A operand of products over the head's values: LDS in three planes, each
+// in blocks of 32 rows x 16 values as the instruction takes them, 1 KiB, 16 bytes a lane: a
+// conflict-free ds_read_b128. The row's place within its half block is permuted by its group of
+// eight values, so that the writes of a row's groups, which neighbouring threads hold, fall on
+// different banks too. A thread stages kUnits units of one row by 8 values.
+template <int ROWS, int DP, int THREADS, bool VEC>
+struct RowTile {
+    static constexpr int kGroups = DP / 8;
+    static constexpr int kUnits = ROWS * kGroups / THREADS;
+    static constexpr int kPlane = ROWS * DP * 2;
+    static constexpr int kBytes = 3 * kPlane;
+    static_assert(kUnits >= 1 && kUnits * THREADS == ROWS * kGroups, "tile shape");
+
+    float v[kUnits][8];
+
+    __device__ __forceinline__ static int row(int u) {
+        return (int(threadIdx.x) + u * THREADS) / kGroups;
+    }
+    __device__ __forceinline__ static int group(int u) {
+        return (int(threadIdx.x) + u * THREADS) % kGroups;
+    }
+    __device__ __forceinline__ static int slot(int r, int g) {
+        return ((r / 32) * (DP / 16) + g / 2) * 1024 + (g & 1) * 512 + (((r & 31) ^ (g & 7)) << 4);
+    }
+    // The first `left` rows from `base`, ld floats apart (left >= 1; rows past them repeat the
+    // last). Offsets within the tile are below 2^31: ld is at most kMaxLd.
+    __device__ __forceinline__ void load(const float* base, int ld, int left, int dim) {
+        const auto at = (global_bytes)base;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const int r = row(u) < left ? row(u) : left - 1, d = 8 * group(u);
+            if (VEC) {
+                const uint32_t o = 4u * uint32_t(r * ld + (d < dim ? d : 0));
+                const floatx4u x = global_load<floatx4u>(at + o);
+                const floatx4u y = global_load<floatx4u>(at + o + 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    v[u][j] = x[j];
+                    v[u][4 + j] = y[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[u][j] = global_load<float>(
+                        at + 4u * uint32_t(r * ld + (d + j < dim ? d + j : 0)));
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char* lds, int left, int dim) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const bool in = row(u) < left;
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[j] = in && 8 * group(u) + (VEC ? 0 : j) < dim ? v[u][j] : 0.0f;
+            bf16x8 part[3];
+            split8(x, part);
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                *reinterpret_cast<bf16x8*>(lds + p * kPlane + slot(row(u), group(u))) = part[p];
+        }
+    }
+    // Block (rb, ks) of the tile.
+    __device__ __forceinline__ static void block(const char* lds, int rb, int ks, bf16x8 (&a)[3]) {
+        const int lane = int(threadIdx.x) & 63;
+        const char* at = lds + slot(32 * rb + (lane & 31), 2 * ks + lane / 32);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) a[p] = *reinterpret_cast<const bf16x8*>(at + p * kPlane);
+    }
+};
+
+// ROWS streamed rows as the A operand, transposed, of products over the rows: block (db, t) holds
+// values 32 db .. of rows 16 t .., the rows in the order that registers 8 (t % 2) .. of a D hold
+// them: half block h has rows 16 t + 4 h + {0..3, 8..11}. A thread stages kUnits units of one value
+// of the eight rows of a half block; a wave reads runs of a row.
+template <int ROWS, int DP, int THREADS>
+struct ColTile {
+    static constexpr int kUnits = ROWS * (DP / 8) / THREADS;
+    static constexpr int kPlane = ROWS * DP * 2;
+    static constexpr int kBytes = 3 * kPlane;
+    static_assert(kUnits >= 1 && kUnits * THREADS == ROWS * (DP / 8), "tile shape");
+
+    float v[kUnits][8];
+
+    __device__ __forceinline__ static int value(int u) {
+        return (int(threadIdx.x) + u * THREADS) % DP;
+    }
+    __device__ __forceinline__ static int octet(int u) {
+        return (int(threadIdx.x) + u * THREADS) / DP;
+    }
+    // Row j (of 8) of octet o.
+    __device__ __forceinline__ static int row(int o, int j) {
+        return 16 * (o / 2) + 4 * (o % 2) + (j < 4 ? j : j + 4);
+    }
+    __device__ __forceinline__ static int slot(int d, int o) {
+        return ((d / 32) * (ROWS / 16) + o / 2) * 1024 + (o % 2) * 512 + ((d & 31) << 4);
+    }
+    __device__ __forceinline__ void load(const float* base, int ld, int left, int dim) {
+        const auto at = (global_bytes)base;
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const int d = value(u) < dim ? value(u) : 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int r = row(octet(u), j);
+                v[u][j] = global_load<float>(at + 4u * uint32_t((r < left ? r : left - 1) * ld + d));
+            }
+        }
+    }
+    __device__ __forceinline__ void store(char* lds, int left, int dim) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[j] = row(octet(u), j) < left && value(u) < dim ? v[u][j] : 0.0f;
+            bf16x8 part[3];
+            split8(x, part);
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                *reinterpret_cast<bf16x8*>(lds + p * kPlane + slot(value(u), octet(u))) = part[p];
+        }
+    }
+    __device__ __forceinline__ static void block(const char* lds, int db, int t, bf16x8 (&a)[3]) {
+        const int lane = int(threadIdx.x) & 63;
+        const char* at = lds + slot(32 * db + (lane & 31), 2 * t + lane / 32);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) a[p] = *reinterpret_cast<const bf16x8*>(at + p * kPlane);
+    }
+};
+
+}  // namespace attention
+}  // namespace ehip
+
+#endif  // EHIP_ATTENTION_TILE_HPP
