@@ -19,9 +19,7 @@ namespace {
 
 constexpr int kMaxDim = 128;
 constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr int kRows = 64;     // rows (queries or keys) of one block of the backward
-constexpr int kQueries = 128;  // queries of one block of the forward, 32 a wave
+constexpr int kRows = 128;  // rows (queries or keys) of one block, 32 a wave
 
 struct Packed {
     const float *q, *k, *v;
@@ -58,8 +56,8 @@ __device__ __forceinline__ int offset_at(const int32_t* cu, int s, int total) {
 // sequence before it than its tiles need, as ceil((b - a) / size) <= b / size - a / size + 1 in
 // whole numbers, so no sum over the sequences is needed to find a tile. The last s whose first
 // slot is not past `slot` is searched 64 candidates at a time, a lane each; every wave of the block
-// finds the same. Later tiles come first within a sequence: under a causal mask they are the
-// longest.
+// finds the same. Later queries and earlier keys come first within a sequence: under a causal mask
+// they meet the most.
 __device__ __forceinline__ Tile find_tile(const Packed& a, bool keys, int slot, int size) {
     const int32_t* cu = keys ? a.cu_k : a.cu_q;
     const int total = keys ? a.total_k : a.total_q;
@@ -90,7 +88,7 @@ __device__ __forceinline__ Tile find_tile(const Packed& a, bool keys, int slot, 
     t.nk = offset_at(a.cu_k, lo + 1, a.total_k) - t.k0;
     t.nq = t.nq < 0 ? 0 : t.nq;
     t.nk = t.nk < 0 ? 0 : t.nk;
-    t.first = (tiles - 1 - at) * size;
+    t.first = (keys ? at : tiles - 1 - at) * size;
     t.rows = end - begin - t.first;
     t.rows = t.rows < size ? t.rows : size;
     return t;
@@ -162,17 +160,6 @@ __device__ void forward_row(const Packed& a, const Tile& t, int h, int i) {
         if (lane + 64 * e < a.dim) out[lane + 64 * e] = acc[e];
     if (lane == 0)
         a.lse[int64_t(t.q0 + i) * a.heads + h] = n == 0 ? -INFINITY : m + logf(sum);
-}
-
-__device__ float delta_of_row(const Packed& a, const Tile& t, int h, int i) {
-    const int lane = int(threadIdx.x) & 63;
-    const float* g = a.grad + int64_t(t.q0 + i) * a.ld_grad + int64_t(h) * a.dim;
-    const float* o = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
-    float s = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-        if (lane + 64 * e < a.dim) s = __builtin_fmaf(g[lane + 64 * e], o[lane + 64 * e], s);
-    return wave_sum(s);
 }
 
 // ds_ij, and p_ij through p.
@@ -269,7 +256,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward(Packed a) {
     __shared__ __attribute__((aligned(16))) char lds[KeyTile::kBytes + ValueTile::kBytes];
     char* const lds_v = lds + KeyTile::kBytes;
     const int h = head_of(a, int(blockIdx.x % a.heads));
-    const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kQueries);
+    const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kRows);
     if (t.rows == 0) return;
     const int c = h / (a.heads / a.kv_heads);
     const int wave = int(threadIdx.x) / 64, lane = int(threadIdx.x) & 63;
@@ -385,22 +372,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward(Packed a) {
     fine = fine || limit == 0;
     const uint64_t again = __ballot(!fine && mine < t.rows);
     if (mine < t.rows) {
-        float* out = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
-#pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int d = 32 * db + row_of(r);
-                if (VEC) {
-                    if (d < a.dim)
-                        *reinterpret_cast<floatx4u*>(out + d) =
-                            floatx4u{o[db][r], o[db][r + 1], o[db][r + 2], o[db][r + 3]};
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < a.dim) out[d + e] = o[db][r + e];
-                }
-            }
+        store_own<DP, VEC>(a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim, a.dim, o);
         // shift ln 2 in two parts: ln 2 = hi + lo.
         if (lane < 32)
             a.lse[int64_t(t.q0 + i) * a.heads + h] =
@@ -413,27 +385,256 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward(Packed a) {
         forward_row(a, t, h, t.first + 32 * wave + __builtin_ctz(rows));
 }
 
-__global__ __launch_bounds__(kThreads) void packed_backward_q(Packed a) {
-    const int h = int(blockIdx.x % a.heads);
+// s, and so p_ij, for the pairs of the lane's own row and a block of 32 streamed ones is formed
+// again from the inputs, dp likewise; then the block's share of the gradients. The queries' kernel
+// also leaves delta for the keys' one.
+template <int DP, int BN, bool VEC, int MINW>
+__global__ __launch_bounds__(kThreads, MINW) void packed_backward_q(Packed a) {
+    using namespace attention;
+    using KeyTile = RowTile<BN, DP, kThreads, VEC>;
+    using KeyColumns = ColTile<BN, DP, kThreads>;
+    __shared__ __attribute__((aligned(16))) char lds[2 * KeyTile::kBytes + KeyColumns::kBytes];
+    char* const lds_v = lds + KeyTile::kBytes;
+    char* const lds_c = lds_v + KeyTile::kBytes;
+    const int h = head_of(a, int(blockIdx.x % a.heads));
     const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kRows);
-    for (int r = int(threadIdx.x) / 64; r < t.rows; r += kWaves) {
-        const int i = t.first + r;
-        const float delta = delta_of_row(a, t, h, i);
-        if ((threadIdx.x & 63) == 0) a.delta[int64_t(t.q0 + i) * a.heads + h] = delta;
-        if (a.dq != nullptr) dq_row(a, t, h, i, delta);
+    if (t.rows == 0) return;
+    const int c = h / (a.heads / a.kv_heads);
+    const int wave = int(threadIdx.x) / 64, lane = int(threadIdx.x) & 63;
+    const int mine = 32 * wave + (lane & 31);  // the lane's query, of the tile
+    const int i = t.first + (mine < t.rows ? mine : t.rows - 1);
+    const int64_t row = t.q0 + i;
+    const int limit = visible(a, t, i);
+    const int last = 32 * wave + 31 < t.rows ? 32 * wave + 31 : t.rows - 1;
+    const int end = visible(a, t, t.first + t.rows - 1);
+    const int wave_end = 32 * wave < t.rows ? visible(a, t, t.first + last) : 0;
+    const int wave_all = visible(a, t, t.first + 32 * wave);  // keys that all its queries see
+
+    const float* gr = a.grad + row * a.ld_grad + int64_t(h) * a.dim;
+    const float delta = own_dot<DP, VEC>(gr, a.out + row * a.ld_out + int64_t(h) * a.dim, a.dim);
+    if (lane < 32 && mine < t.rows) a.delta[row * a.heads + h] = delta;
+    if (a.dq == nullptr) return;
+    const float c2 = a.scale * 1.44269504088896340736f;
+    const float shift = limit > 0 ? a.lse[row * a.heads + h] * 1.44269504088896340736f : 0.0f;
+    bf16x8 q[DP / 16][3], g[DP / 16][3];
+    own_row<DP, VEC>(a.q + row * a.ld_q + int64_t(h) * a.dim, a.dim, 1.0f, q);
+    own_row<DP, VEC>(gr, a.dim, 1.0f, g);
+    floatx16 dq[DP / 32];
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) dq[db] = zeros();
+
+    const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
+    const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
+    const int ld_k = int(a.ld_k), ld_v = int(a.ld_v);
+    KeyTile kt, vt;
+    KeyColumns ct;
+    if (end > 0) {
+        kt.load(k, ld_k, t.nk, a.dim);
+        vt.load(v, ld_v, t.nk, a.dim);
+        ct.load(k, ld_k, t.nk, a.dim);
+    }
+    for (int j0 = 0; j0 < end; j0 += BN) {
+        __syncthreads();
+        kt.store(lds, t.nk - j0, a.dim);
+        vt.store(lds_v, t.nk - j0, a.dim);
+        ct.store(lds_c, t.nk - j0, a.dim);
+        const int j1 = j0 + BN;
+        if (j1 < end) {
+            kt.load(k + int64_t(j1) * ld_k, ld_k, t.nk - j1, a.dim);
+            vt.load(v + int64_t(j1) * ld_v, ld_v, t.nk - j1, a.dim);
+            ct.load(k + int64_t(j1) * ld_k, ld_k, t.nk - j1, a.dim);
+        }
+        __syncthreads();
+        if (j0 >= wave_end) continue;
+        const bool edge = j1 > wave_all;
+        bf16x8 w[BN / 16][3];
+#pragma unroll
+        for (int b = 0; b < BN / 32; ++b) {
+            floatx16 s = zeros(), dp = zeros();
+#pragma unroll
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                bf16x8 f[3];
+                KeyTile::block(lds, b, ks, f);
+                multiply(s, f, q[ks]);
+                KeyTile::block(lds_v, b, ks, f);
+                multiply(dp, f, g[ks]);
+            }
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -shift)) * (dp[r] - delta);
+                if (edge && j0 + 32 * b + row_of(r) >= limit) ds[r] = 0.0f;
+            }
+            split8(ds, w[2 * b]);
+            split8(ds + 8, w[2 * b + 1]);
+        }
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+            floatx16 x = zeros();
+#pragma unroll
+            for (int u = 0; u < BN / 16; ++u) {
+                bf16x8 f[3];
+                KeyColumns::block(lds_c, db, u, f);
+                multiply(x, f, w[u]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) dq[db][r] += x[r];
+        }
+    }
+    bool fine = true;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            dq[db][r] = limit > 0 ? dq[db][r] * a.scale : 0.0f;
+            fine = fine && fabsf(dq[db][r]) < INFINITY;
+        }
+    const uint64_t again = __ballot(!fine && mine < t.rows);
+    if (mine < t.rows)
+        store_own<DP, VEC>(a.dq + row * a.ld_dq + int64_t(h) * a.dim, a.dim, dq);
+    for (uint32_t rows = uint32_t(again) | uint32_t(again >> 32); rows != 0; rows &= rows - 1) {
+        const int r = __builtin_ctz(rows);
+        dq_row(a, t, h, t.first + 32 * wave + r, __shfl(delta, r));
     }
 }
 
-__global__ __launch_bounds__(kThreads) void packed_backward_kv(Packed a) {
-    const int c = int(blockIdx.x % a.kv_heads);
+template <int DP, bool VEC, int MINW>
+__global__ __launch_bounds__(kThreads, MINW) void packed_backward_kv(Packed a) {
+    using namespace attention;
+    constexpr int BN = 32;
+    using QueryTile = RowTile<BN, DP, kThreads, VEC>;
+    using QueryColumns = ColTile<BN, DP, kThreads>;
+    __shared__ __attribute__((aligned(16))) char
+        lds[2 * QueryTile::kBytes + 2 * QueryColumns::kBytes + 2 * BN * sizeof(float)];
+    char* const lds_g = lds + QueryTile::kBytes;
+    char* const lds_qc = lds_g + QueryTile::kBytes;
+    char* const lds_gc = lds_qc + QueryColumns::kBytes;
+    float* const lds_shift = reinterpret_cast<float*>(lds_gc + QueryColumns::kBytes);
+    float* const lds_delta = lds_shift + BN;
+    const int c = int(blockIdx.x % a.kv_heads), group = a.heads / a.kv_heads;
     const Tile t = find_tile(a, true, int(blockIdx.x / a.kv_heads), kRows);
-    for (int j = int(threadIdx.x) / 64; j < t.rows; j += kWaves) dkv_row(a, t, c, t.first + j);
+    if (t.rows == 0) return;
+    const int wave = int(threadIdx.x) / 64, lane = int(threadIdx.x) & 63;
+    const int mine = 32 * wave + (lane & 31);  // the lane's key, of the tile
+    const int j = t.first + (mine < t.rows ? mine : t.rows - 1);
+    const int64_t row = t.k0 + j;
+    // The first query that sees a key, and the first ones of the block and of the wave.
+    const auto first_of = [&](int key) {
+        const int64_t n = a.causal ? int64_t(key) - t.nk + t.nq : 0;
+        return n < 0 ? 0 : int(n);
+    };
+    const int from = first_of(j), start = first_of(t.first);
+    const int wave_start = first_of(t.first + 32 * wave);
+    const int wave_all = first_of(t.first + 32 * wave + 31);
+
+    const float c2 = a.scale * 1.44269504088896340736f;
+    bf16x8 k[DP / 16][3], v[DP / 16][3];
+    own_row<DP, VEC>(a.k + row * a.ld_k + int64_t(c) * a.dim, a.dim, 1.0f, k);
+    own_row<DP, VEC>(a.v + row * a.ld_v + int64_t(c) * a.dim, a.dim, 1.0f, v);
+    floatx16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) {
+        dk[db] = zeros();
+        dv[db] = zeros();
+    }
+    const int ld_q = int(a.ld_q), ld_g = int(a.ld_grad);
+    const int steps = start < t.nq ? (t.nq - start + BN - 1) / BN : 0;
+    QueryTile qt, gt;
+    QueryColumns qc, gc;
+    float stat = 0.0f;  // of the thread's query: lse (threads 0..31), delta (32..63)
+    // Tile n: head n / steps of the group, its queries from start + n % steps * BN on.
+    const auto load = [&](int n) {
+        const int h = c * group + n / steps, i0 = start + n % steps * BN;
+        const int64_t at = t.q0 + i0;
+        const int left = t.nq - i0;
+        const float* q = a.q + at * a.ld_q + int64_t(h) * a.dim;
+        const float* g = a.grad + at * a.ld_grad + int64_t(h) * a.dim;
+        qt.load(q, ld_q, left, a.dim);
+        gt.load(g, ld_g, left, a.dim);
+        qc.load(q, ld_q, left, a.dim);
+        gc.load(g, ld_g, left, a.dim);
+        if (wave == 0) {
+            const int r = (lane & 31) < left ? lane & 31 : left - 1;
+            stat = (lane < 32 ? a.lse : a.delta)[(at + r) * a.heads + h];
+        }
+    };
+    const int count = steps * group;
+    if (count > 0) load(0);
+    for (int n = 0; n < count; ++n) {
+        const int i0 = start + n % steps * BN, left = t.nq - i0;
+        __syncthreads();
+        qt.store(lds, left, a.dim);
+        gt.store(lds_g, left, a.dim);
+        qc.store(lds_qc, left, a.dim);
+        gc.store(lds_gc, left, a.dim);
+        if (wave == 0) lds_shift[lane] = lane < 32 ? stat * 1.44269504088896340736f : stat;
+        if (n + 1 < count) load(n + 1);
+        __syncthreads();
+        if (i0 + BN <= wave_start) continue;
+        const bool edge = i0 < wave_all || left < BN;
+        floatx16 s = zeros(), dp = zeros();
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+            bf16x8 f[3];
+            QueryTile::block(lds, 0, ks, f);
+            multiply(s, f, k[ks]);
+            QueryTile::block(lds_g, 0, ks, f);
+            multiply(dp, f, v[ks]);
+        }
+        float p[16], ds[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int at = row_of(r);
+            p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -lds_shift[at]));
+            ds[r] = p[r] * (dp[r] - lds_delta[at]);
+            if (edge && (i0 + at < from || at >= left)) p[r] = ds[r] = 0.0f;
+        }
+        bf16x8 wp[2][3], wd[2][3];
+        split8(p, wp[0]);
+        split8(p + 8, wp[1]);
+        split8(ds, wd[0]);
+        split8(ds + 8, wd[1]);
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db) {
+            floatx16 x = zeros(), y = zeros();
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                bf16x8 f[3];
+                QueryColumns::block(lds_gc, db, u, f);
+                multiply(x, f, wp[u]);
+                QueryColumns::block(lds_qc, db, u, f);
+                multiply(y, f, wd[u]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                dv[db][r] += x[r];
+                dk[db][r] += y[r];
+            }
+        }
+    }
+    bool fine = true;
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            dk[db][r] *= a.scale;
+            fine = fine && fabsf(dk[db][r]) < INFINITY && fabsf(dv[db][r]) < INFINITY;
+        }
+    const uint64_t again = __ballot(!fine && mine < t.rows);
+    if (mine < t.rows) {
+        if (a.dk != nullptr)
+            store_own<DP, VEC>(a.dk + row * a.ld_dk + int64_t(c) * a.dim, a.dim, dk);
+        if (a.dv != nullptr)
+            store_own<DP, VEC>(a.dv + row * a.ld_dv + int64_t(c) * a.dim, a.dim, dv);
+    }
+    for (uint32_t rows = uint32_t(again) | uint32_t(again >> 32); rows != 0; rows &= rows - 1)
+        dkv_row(a, t, c, t.first + 32 * wave + __builtin_ctz(rows));
 }
 
 // ---------------------------------------------------------------- host checks
 
-int64_t slots(int64_t total, int64_t sequences, int rows = kRows) {
-    return total / rows + sequences;
+int64_t slots(int64_t total, int64_t sequences) {
+    return total / kRows + sequences;
 }
 
 // Tiles address their rows by 32-bit byte offsets from the first one.
@@ -488,9 +689,24 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
 
 template <int DP, int BN, bool VEC>
 int launch_forward(const Packed& a, hipStream_t s) {
-    const unsigned blocks = unsigned(slots(a.total_q, a.sequences, kQueries) * a.heads);
+    const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads);
     EHIP_LAUNCH("attention_packed", (packed_forward<DP, BN, VEC>), dim3(blocks), dim3(kThreads), 0,
                 s, a);
+    return EHIP_OK;
+}
+
+template <int DP, bool VEC>
+int launch_backward(const Packed& a, hipStream_t s) {
+    if (a.total_q > 0 && (a.dq != nullptr || a.dk != nullptr)) {
+        const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads);
+        EHIP_LAUNCH("attention_packed_backward_q", (packed_backward_q<DP, 32, VEC, DP <= 64 ? 2 : 1>),
+                    dim3(blocks), dim3(kThreads), 0, s, a);
+    }
+    if (a.total_k > 0 && (a.dk != nullptr || a.dv != nullptr)) {
+        const unsigned blocks = unsigned(slots(a.total_k, a.sequences) * a.kv_heads);
+        EHIP_LAUNCH("attention_packed_backward_kv", (packed_backward_kv<DP, VEC, DP <= 32 ? 2 : 1>),
+                    dim3(blocks), dim3(kThreads), 0, s, a);
+    }
     return EHIP_OK;
 }
 
@@ -532,9 +748,9 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
     if (int rc = fill("attention_packed_backward", desc, a)) return rc;
     if (a.sequences == 0) return EHIP_OK;
     const int64_t wide = int64_t(a.heads) * a.dim, narrow = int64_t(a.kv_heads) * a.dim;
-    if (a.total_q > 0 && (grad == nullptr || ld_grad < wide))
-        return fail(EHIP_EINVAL, "attention_packed_backward: null gradient or a leading dimension "
-                                 "below the row's length");
+    if (a.total_q > 0 && (grad == nullptr || ld_grad < wide || ld_grad > kMaxLd))
+        return fail(EHIP_EINVAL, "attention_packed_backward: null gradient, or its leading dimension "
+                                 "below the row's length or above 2^22");
     if ((dq != nullptr && ld_dq < wide) || (dk != nullptr && ld_dk < narrow) ||
         (dv != nullptr && ld_dv < narrow))
         return fail(EHIP_EINVAL,
@@ -552,17 +768,12 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
     a.ld_dk = ld_dk;
     a.ld_dv = ld_dv;
     a.delta = static_cast<float*>(workspace);
-    if (a.total_q > 0 && (dq != nullptr || dk != nullptr)) {
-        const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads);
-        EHIP_LAUNCH("attention_packed_backward_q", packed_backward_q, dim3(blocks), dim3(kThreads),
-                    0, as_stream(stream), a);
-    }
-    if (a.total_k > 0 && (dk != nullptr || dv != nullptr)) {
-        const unsigned blocks = unsigned(slots(a.total_k, a.sequences) * a.kv_heads);
-        EHIP_LAUNCH("attention_packed_backward_kv", packed_backward_kv, dim3(blocks),
-                    dim3(kThreads), 0, as_stream(stream), a);
-    }
-    return EHIP_OK;
+    hipStream_t s = as_stream(stream);
+    const bool vec = a.dim % 8 == 0;
+    if (a.dim <= 32) return vec ? launch_backward<32, true>(a, s) : launch_backward<32, false>(a, s);
+    if (a.dim <= 64) return vec ? launch_backward<64, true>(a, s) : launch_backward<64, false>(a, s);
+    if (a.dim <= 96) return vec ? launch_backward<96, true>(a, s) : launch_backward<96, false>(a, s);
+    return vec ? launch_backward<128, true>(a, s) : launch_backward<128, false>(a, s);
 }
 
 }  // extern "C"

@@ -95,18 +95,64 @@ __device__ __forceinline__ void own_row(const float* row, int dim, float factor,
     }
 }
 
+// The product of the lane's own rows of two tensors, each of the two lanes that hold it over half of
+// the values.
+template <int DP, bool VEC>
+__device__ __forceinline__ float own_dot(const float* x, const float* y, int dim) {
+    const int half = (int(threadIdx.x) & 63) / 32;
+    float s = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+        const int d0 = 16 * ks + 8 * half;
+        if (VEC) {
+            if (d0 >= dim) continue;
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                const floatx4u u = *reinterpret_cast<const floatx4u*>(x + d0 + j);
+                const floatx4u v = *reinterpret_cast<const floatx4u*>(y + d0 + j);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s = __builtin_fmaf(u[e], v[e], s);
+            }
+        } else {
+            for (int j = 0; j < 8; ++j)
+                if (d0 + j < dim) s = __builtin_fmaf(x[d0 + j], y[d0 + j], s);
+        }
+    }
+    return s + __shfl_xor(s, 32);
+}
+
+// The lane's own row of a result held as D blocks of 32 values.
+template <int DP, bool VEC>
+__device__ __forceinline__ void store_own(float* row, int dim, const floatx16 (&x)[DP / 32]) {
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const int d = 32 * db + row_of(r);
+            if (VEC) {
+                if (d < dim)
+                    *reinterpret_cast<floatx4u*>(row + d) =
+                        floatx4u{x[db][r], x[db][r + 1], x[db][r + 2], x[db][r + 3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < dim) row[d + e] = x[db][r + e];
+            }
+        }
+}
+
 // ROWS streamed rows as the A operand of products over the head's values: LDS in three planes, each
 // in blocks of 32 rows x 16 values as the instruction takes them, 1 KiB, 16 bytes a lane: a
 // conflict-free ds_read_b128. The row's place within its half block is permuted by its group of
 // eight values, so that the writes of a row's groups, which neighbouring threads hold, fall on
-// different banks too. A thread stages kUnits units of one row by 8 values.
+// different banks too. A thread stages up to kUnits units of one row by 8 values.
 template <int ROWS, int DP, int THREADS, bool VEC>
 struct RowTile {
     static constexpr int kGroups = DP / 8;
-    static constexpr int kUnits = ROWS * kGroups / THREADS;
+    static constexpr int kUnits = (ROWS * kGroups + THREADS - 1) / THREADS;
     static constexpr int kPlane = ROWS * DP * 2;
     static constexpr int kBytes = 3 * kPlane;
-    static_assert(kUnits >= 1 && kUnits * THREADS == ROWS * kGroups, "tile shape");
+    static_assert(ROWS % 32 == 0 && DP % 32 == 0, "tile shape");
 
     float v[kUnits][8];
 
@@ -146,6 +192,7 @@ struct RowTile {
     __device__ __forceinline__ void store(char* lds, int left, int dim) {
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
+            if ((u + 1) * THREADS > ROWS * kGroups && row(u) >= ROWS) continue;  // no unit
             const bool in = row(u) < left;
             float x[8];
 #pragma unroll
@@ -169,14 +216,14 @@ struct RowTile {
 
 // ROWS streamed rows as the A operand, transposed, of products over the rows: block (db, t) holds
 // values 32 db .. of rows 16 t .., the rows in the order that registers 8 (t % 2) .. of a D hold
-// them: half block h has rows 16 t + 4 h + {0..3, 8..11}. A thread stages kUnits units of one value
-// of the eight rows of a half block; a wave reads runs of a row.
+// them: half block h has rows 16 t + 4 h + {0..3, 8..11}. A thread stages up to kUnits units of one
+// value of the eight rows of a half block; a wave reads runs of a row.
 template <int ROWS, int DP, int THREADS>
 struct ColTile {
-    static constexpr int kUnits = ROWS * (DP / 8) / THREADS;
+    static constexpr int kUnits = (ROWS * (DP / 8) + THREADS - 1) / THREADS;
     static constexpr int kPlane = ROWS * DP * 2;
     static constexpr int kBytes = 3 * kPlane;
-    static_assert(kUnits >= 1 && kUnits * THREADS == ROWS * (DP / 8), "tile shape");
+    static_assert(ROWS % 32 == 0 && DP % 32 == 0, "tile shape");
 
     float v[kUnits][8];
 
@@ -208,6 +255,7 @@ struct ColTile {
     __device__ __forceinline__ void store(char* lds, int left, int dim) {
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
+            if ((u + 1) * THREADS > ROWS * (DP / 8) && octet(u) >= ROWS / 8) continue;  // no unit
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
