@@ -248,18 +248,19 @@ __device__ __forceinline__ int head_of(const Packed& a, int x) {
     return x % a.kv_heads * (a.heads / a.kv_heads) + x / a.kv_heads;
 }
 
-template <int DP, int BN, bool VEC>
-__global__ __launch_bounds__(kThreads, 2) void packed_forward(Packed a) {
+template <int DP, int BN, int WAVES, bool VEC>
+__global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     using namespace attention;
-    using KeyTile = RowTile<BN, DP, kThreads, VEC>;
-    using ValueTile = ColTile<BN, DP, kThreads>;
-    __shared__ __attribute__((aligned(16))) char lds[KeyTile::kBytes + ValueTile::kBytes];
-    char* const lds_v = lds + KeyTile::kBytes;
+    using KeyTile = RowTile<BN, DP, 64 * WAVES, VEC>;
+    using ValueTile = ColTile<BN, DP, 64 * WAVES>;
+    constexpr int kTile = KeyTile::kBytes + ValueTile::kBytes;
+    __shared__ __attribute__((aligned(16))) char lds[2][kTile];
     const int h = head_of(a, int(blockIdx.x % a.heads));
-    const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kRows);
+    const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), 32 * WAVES);
     if (t.rows == 0) return;
     const int c = h / (a.heads / a.kv_heads);
-    const int wave = int(threadIdx.x) / 64, lane = int(threadIdx.x) & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int lane = int(threadIdx.x) & 63;
     const int mine = 32 * wave + (lane & 31);  // the lane's query, of the tile
     const int i = t.first + (mine < t.rows ? mine : t.rows - 1);
     const int limit = visible(a, t, i);
@@ -282,79 +283,96 @@ __global__ __launch_bounds__(kThreads, 2) void packed_forward(Packed a) {
     const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
     const int ld_k = int(a.ld_k), ld_v = int(a.ld_v);
-    KeyTile kt;
-    ValueTile vt;
-    if (end > 0) {
-        kt.load(k, ld_k, t.nk, a.dim);
-        vt.load(v, ld_v, t.nk, a.dim);
-    }
+    KeyTile kt(ld_k, a.dim);
+    ValueTile vt(ld_v, a.dim);
+    // The tile of keys from j on: into registers, and from there into its half of the LDS.
+    const auto load = [&](int j) {
+        if (j >= end) return;
+        kt.load(k + int64_t(j) * ld_k, ld_k, t.nk - j, a.dim);
+        vt.load(v + int64_t(j) * ld_v, ld_v, t.nk - j, a.dim);
+    };
+    const auto stage = [&](int j) {
+        if (j >= end) return;
+        char* const at = lds[j / BN & 1];
+        kt.store(at, t.nk - j, a.dim);
+        vt.store(at + KeyTile::kBytes, t.nk - j, a.dim);
+    };
+    load(0);
+    stage(0);
+    load(BN);
+    __syncthreads();
     for (int j0 = 0; j0 < end; j0 += BN) {
-        __syncthreads();
-        kt.store(lds, t.nk - j0, a.dim);
-        vt.store(lds_v, t.nk - j0, a.dim);
-        const int j1 = j0 + BN;
-        if (j1 < end) {
-            kt.load(k + int64_t(j1) * ld_k, ld_k, t.nk - j1, a.dim);
-            vt.load(v + int64_t(j1) * ld_v, ld_v, t.nk - j1, a.dim);
+        // One wave of a SIMD stages the next tile before its products, the other one after them:
+        // one's conversions run beside the other's matrix instructions.
+        const char* const lds_k = lds[j0 / BN & 1];
+        const char* const lds_v = lds_k + KeyTile::kBytes;
+        if (wave < WAVES / 2) {
+            stage(j0 + BN);
+            load(j0 + 2 * BN);
         }
-        __syncthreads();
-        if (j0 >= wave_end) continue;
-        floatx16 s[BN / 32];
+        if (j0 < wave_end) {
+            floatx16 s[BN / 32];
 #pragma unroll
-        for (int b = 0; b < BN / 32; ++b) s[b] = zeros();
+            for (int b = 0; b < BN / 32; ++b) s[b] = zeros();
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks)
+            for (int ks = 0; ks < DP / 16; ++ks) {
+                bf16x8 f[BN / 32][3];
 #pragma unroll
-            for (int b = 0; b < BN / 32; ++b) {
-                bf16x8 f[3];
-                KeyTile::block(lds, b, ks, f);
-                multiply(s[b], f, q[ks]);
+                for (int b = 0; b < BN / 32; ++b) KeyTile::block(lds_k, b, ks, f[b]);
+                if constexpr (BN == 64) multiply_two(s[0], s[1], f[0], f[1], q[ks]);
+                else multiply(s[0], f[0], q[ks]);
             }
-        if (j1 > wave_all) {
+            if (j0 + BN > wave_all) {
+#pragma unroll
+                for (int b = 0; b < BN / 32; ++b)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (j0 + 32 * b + row_of(r) >= limit) s[b][r] = -INFINITY;
+            }
+            float m = top;
 #pragma unroll
             for (int b = 0; b < BN / 32; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (j0 + 32 * b + row_of(r) >= limit) s[b][r] = -INFINITY;
-        }
-        float m = top;
+                for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float next = m == -INFINITY ? 24.0f : __builtin_fmaf(m, c2, 24.0f);
+            const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - next);
+            top = m;
+            shift = next;
+            float part = 0.0f;
+            bf16x8 p[BN / 16][3];
 #pragma unroll
-        for (int b = 0; b < BN / 32; ++b)
+            for (int b = 0; b < BN / 32; ++b) {
+                float w[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
-        m = fmaxf(m, __shfl_xor(m, 32));
-        const float next = m == -INFINITY ? 24.0f : __builtin_fmaf(m, c2, 24.0f);
-        const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - next);
-        top = m;
-        shift = next;
-        float part = 0.0f;
-        bf16x8 p[BN / 16][3];
-#pragma unroll
-        for (int b = 0; b < BN / 32; ++b) {
-            float w[16];
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], c2, -shift));
-                part += w[r];
+                for (int r = 0; r < 16; ++r) {
+                    w[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r], c2, -shift));
+                    part += w[r];
+                }
+                split8(w, p[2 * b]);
+                split8(w + 8, p[2 * b + 1]);
             }
-            split8(w, p[2 * b]);
-            split8(w + 8, p[2 * b + 1]);
-        }
-        sum = __builtin_fmaf(sum, keep, part);
-        // The tile's sum apart from the running one: that is rounded to nearest once a tile, where
-        // the instruction drops low bits towards minus infinity.
+            sum = __builtin_fmaf(sum, keep, part);
+            // The tile's sum apart from the running one: that is rounded to nearest once a tile,
+            // where the instruction drops low bits towards minus infinity.
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-            floatx16 x = zeros();
+            for (int db = 0; db < DP / 32; ++db) {
+                floatx16 x = zeros();
 #pragma unroll
-            for (int u = 0; u < BN / 16; ++u) {
-                bf16x8 f[3];
-                ValueTile::block(lds_v, db, u, f);
-                multiply(x, f, p[u]);
+                for (int u = 0; u < BN / 16; ++u) {
+                    bf16x8 f[3];
+                    ValueTile::block(lds_v, db, u, f);
+                    multiply(x, f, p[u]);
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[db][r] = __builtin_fmaf(o[db][r], keep, x[r]);
             }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[db][r] = __builtin_fmaf(o[db][r], keep, x[r]);
         }
+        if (wave >= WAVES / 2) {
+            stage(j0 + BN);
+            load(j0 + 2 * BN);
+        }
+        __syncthreads();
     }
 
     // Rows that saw something and have no finite result are formed again by the formula: a NaN or
@@ -426,8 +444,8 @@ __global__ __launch_bounds__(kThreads, MINW) void packed_backward_q(Packed a) {
     const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
     const int ld_k = int(a.ld_k), ld_v = int(a.ld_v);
-    KeyTile kt, vt;
-    KeyColumns ct;
+    KeyTile kt(ld_k, a.dim), vt(ld_v, a.dim);
+    KeyColumns ct(ld_k, a.dim);
     if (end > 0) {
         kt.load(k, ld_k, t.nk, a.dim);
         vt.load(v, ld_v, t.nk, a.dim);
@@ -539,8 +557,8 @@ __global__ __launch_bounds__(kThreads, MINW) void packed_backward_kv(Packed a) {
     }
     const int ld_q = int(a.ld_q), ld_g = int(a.ld_grad);
     const int steps = start < t.nq ? (t.nq - start + BN - 1) / BN : 0;
-    QueryTile qt, gt;
-    QueryColumns qc, gc;
+    QueryTile qt(ld_q, a.dim), gt(ld_g, a.dim);
+    QueryColumns qc(ld_q, a.dim), gc(ld_g, a.dim);
     float stat = 0.0f;  // of the thread's query: lse (threads 0..31), delta (32..63)
     // Tile n: head n / steps of the group, its queries from start + n % steps * BN on.
     const auto load = [&](int n) {
@@ -633,8 +651,8 @@ __global__ __launch_bounds__(kThreads, MINW) void packed_backward_kv(Packed a) {
 
 // ---------------------------------------------------------------- host checks
 
-int64_t slots(int64_t total, int64_t sequences) {
-    return total / kRows + sequences;
+int64_t slots(int64_t total, int64_t sequences, int rows = kRows) {
+    return total / rows + sequences;
 }
 
 // Tiles address their rows by 32-bit byte offsets from the first one.
@@ -687,11 +705,11 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
     return EHIP_OK;
 }
 
-template <int DP, int BN, bool VEC>
+template <int DP, int BN, int WAVES, bool VEC>
 int launch_forward(const Packed& a, hipStream_t s) {
-    const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads);
-    EHIP_LAUNCH("attention_packed", (packed_forward<DP, BN, VEC>), dim3(blocks), dim3(kThreads), 0,
-                s, a);
+    const unsigned blocks = unsigned(slots(a.total_q, a.sequences, 32 * WAVES) * a.heads);
+    EHIP_LAUNCH("attention_packed", (packed_forward<DP, BN, WAVES, VEC>), dim3(blocks),
+                dim3(64 * WAVES), 0, s, a);
     return EHIP_OK;
 }
 
@@ -723,14 +741,14 @@ int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* stream)
     if (int rc = fill("attention_packed", desc, a)) return rc;
     if (a.sequences == 0 || a.total_q == 0) return EHIP_OK;
     const bool vec = a.dim % 8 == 0;
-    if (a.dim <= 32) return vec ? launch_forward<32, 64, true>(a, as_stream(stream))
-                                : launch_forward<32, 64, false>(a, as_stream(stream));
-    if (a.dim <= 64) return vec ? launch_forward<64, 64, true>(a, as_stream(stream))
-                                : launch_forward<64, 64, false>(a, as_stream(stream));
-    if (a.dim <= 96) return vec ? launch_forward<96, 64, true>(a, as_stream(stream))
-                                : launch_forward<96, 64, false>(a, as_stream(stream));
-    return vec ? launch_forward<128, 32, true>(a, as_stream(stream))
-               : launch_forward<128, 32, false>(a, as_stream(stream));
+    if (a.dim <= 32) return vec ? launch_forward<32, 64, 8, true>(a, as_stream(stream))
+                                : launch_forward<32, 64, 8, false>(a, as_stream(stream));
+    if (a.dim <= 64) return vec ? launch_forward<64, 64, 8, true>(a, as_stream(stream))
+                                : launch_forward<64, 64, 8, false>(a, as_stream(stream));
+    if (a.dim <= 96) return vec ? launch_forward<96, 32, 8, true>(a, as_stream(stream))
+                                : launch_forward<96, 32, 8, false>(a, as_stream(stream));
+    return vec ? launch_forward<128, 32, 8, true>(a, as_stream(stream))
+               : launch_forward<128, 32, 8, false>(a, as_stream(stream));
 }
 
 int64_t ehip_attention_packed_backward_workspace(const ehip_attention_packed_t* desc) {

@@ -44,6 +44,16 @@ __device__ __forceinline__ void split8(const float* x, bf16x8 (&part)[3]) {
     part[2] = __builtin_bit_cast(bf16x8, l);
 }
 
+// Two products with one B, their sums interleaved.
+__device__ __forceinline__ void multiply_two(floatx16& d0, floatx16& d1, const bf16x8 (&a0)[3],
+                                             const bf16x8 (&a1)[3], const bf16x8 (&b)[3]) {
+#pragma unroll
+    for (int q = 0; q < 6; ++q) {
+        d0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0[kPart[q][0]], b[kPart[q][1]], d0, 0, 0, 0);
+        d1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1[kPart[q][0]], b[kPart[q][1]], d1, 0, 0, 0);
+    }
+}
+
 // d += the product of two blocks of 32 x 16.
 __device__ __forceinline__ void multiply(floatx16& d, const bf16x8 (&a)[3], const bf16x8 (&b)[3]) {
 #pragma unroll
@@ -155,6 +165,7 @@ struct RowTile {
     static_assert(ROWS % 32 == 0 && DP % 32 == 0, "tile shape");
 
     float v[kUnits][8];
+    uint32_t o[kUnits];  // byte offsets of the units from the tile's first row
 
     __device__ __forceinline__ static int row(int u) {
         return (int(threadIdx.x) + u * THREADS) / kGroups;
@@ -165,23 +176,34 @@ struct RowTile {
     __device__ __forceinline__ static int slot(int r, int g) {
         return ((r / 32) * (DP / 16) + g / 2) * 1024 + (g & 1) * 512 + (((r & 31) ^ (g & 7)) << 4);
     }
-    // The first `left` rows from `base`, ld floats apart (left >= 1; rows past them repeat the
-    // last). Offsets within the tile are below 2^31: ld is at most kMaxLd.
+    // Rows are ld floats apart, at most kMaxLd: offsets within a tile are below 2^31.
+    __device__ __forceinline__ RowTile(int ld, int dim) {
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+            const int r = row(u) < ROWS ? row(u) : 0, d = 8 * group(u);
+            o[u] = 4u * uint32_t(r * ld + (d < dim ? d : 0));
+        }
+    }
+    // The first `left` rows from `base` (left >= 1; rows past them repeat the last).
     __device__ __forceinline__ void load(const float* base, int ld, int left, int dim) {
         const auto at = (global_bytes)base;
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
-            const int r = row(u) < left ? row(u) : left - 1, d = 8 * group(u);
             if (VEC) {
-                const uint32_t o = 4u * uint32_t(r * ld + (d < dim ? d : 0));
-                const floatx4u x = global_load<floatx4u>(at + o);
-                const floatx4u y = global_load<floatx4u>(at + o + 16);
+                uint32_t from = o[u];
+                if (left < ROWS) {
+                    const int r = row(u) < left ? row(u) : left - 1, d = 8 * group(u);
+                    from = 4u * uint32_t(r * ld + (d < dim ? d : 0));
+                }
+                const floatx4u x = global_load<floatx4u>(at + from);
+                const floatx4u y = global_load<floatx4u>(at + from + 16);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     v[u][j] = x[j];
                     v[u][4 + j] = y[j];
                 }
             } else {
+                const int r = row(u) < left ? row(u) : left - 1, d = 8 * group(u);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     v[u][j] = global_load<float>(
@@ -189,7 +211,9 @@ struct RowTile {
             }
         }
     }
-    __device__ __forceinline__ void store(char* lds, int left, int dim) {
+    // CLEAN: every row and value of the tile is there.
+    template <bool CLEAN>
+    __device__ __forceinline__ void store_as(char* lds, int left, int dim) const {
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
             if ((u + 1) * THREADS > ROWS * kGroups && row(u) >= ROWS) continue;  // no unit
@@ -197,13 +221,17 @@ struct RowTile {
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                x[j] = in && 8 * group(u) + (VEC ? 0 : j) < dim ? v[u][j] : 0.0f;
+                x[j] = CLEAN || (in && 8 * group(u) + (VEC ? 0 : j) < dim) ? v[u][j] : 0.0f;
             bf16x8 part[3];
             split8(x, part);
 #pragma unroll
             for (int p = 0; p < 3; ++p)
                 *reinterpret_cast<bf16x8*>(lds + p * kPlane + slot(row(u), group(u))) = part[p];
         }
+    }
+    __device__ __forceinline__ void store(char* lds, int left, int dim) const {
+        if (left >= ROWS && dim == DP) store_as<true>(lds, left, dim);
+        else store_as<false>(lds, left, dim);
     }
     // Block (rb, ks) of the tile.
     __device__ __forceinline__ static void block(const char* lds, int rb, int ks, bf16x8 (&a)[3]) {
@@ -226,6 +254,7 @@ struct ColTile {
     static_assert(ROWS % 32 == 0 && DP % 32 == 0, "tile shape");
 
     float v[kUnits][8];
+    uint32_t o[kUnits];  // byte offsets of the units' first rows
 
     __device__ __forceinline__ static int value(int u) {
         return (int(threadIdx.x) + u * THREADS) % DP;
@@ -240,32 +269,54 @@ struct ColTile {
     __device__ __forceinline__ static int slot(int d, int o) {
         return ((d / 32) * (ROWS / 16) + o / 2) * 1024 + (o % 2) * 512 + ((d & 31) << 4);
     }
-    __device__ __forceinline__ void load(const float* base, int ld, int left, int dim) {
-        const auto at = (global_bytes)base;
+    __device__ __forceinline__ ColTile(int ld, int dim) {
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
             const int d = value(u) < dim ? value(u) : 0;
+            o[u] = 4u * uint32_t(row(octet(u) < ROWS / 8 ? octet(u) : 0, 0) * ld + d);
+        }
+    }
+    __device__ __forceinline__ void load(const float* base, int ld, int left, int dim) {
+        const auto at = (global_bytes)base;
+        if (left >= ROWS) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int r = row(octet(u), j);
-                v[u][j] = global_load<float>(at + 4u * uint32_t((r < left ? r : left - 1) * ld + d));
+                const global_bytes row_j = at + 4 * int64_t(row(0, j)) * ld;
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u) v[u][j] = global_load<float>(row_j + o[u]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                const int d = value(u) < dim ? value(u) : 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int r = row(octet(u), j);
+                    v[u][j] =
+                        global_load<float>(at + 4u * uint32_t((r < left ? r : left - 1) * ld + d));
+                }
             }
         }
     }
-    __device__ __forceinline__ void store(char* lds, int left, int dim) {
+    template <bool CLEAN>
+    __device__ __forceinline__ void store_as(char* lds, int left, int dim) const {
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
             if ((u + 1) * THREADS > ROWS * (DP / 8) && octet(u) >= ROWS / 8) continue;  // no unit
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                x[j] = row(octet(u), j) < left && value(u) < dim ? v[u][j] : 0.0f;
+                x[j] = CLEAN || (row(octet(u), j) < left && value(u) < dim) ? v[u][j] : 0.0f;
             bf16x8 part[3];
             split8(x, part);
 #pragma unroll
             for (int p = 0; p < 3; ++p)
                 *reinterpret_cast<bf16x8*>(lds + p * kPlane + slot(value(u), octet(u))) = part[p];
         }
+    }
+    __device__ __forceinline__ void store(char* lds, int left, int dim) const {
+        if (left >= ROWS && dim == DP) store_as<true>(lds, left, dim);
+        else store_as<false>(lds, left, dim);
     }
     __device__ __forceinline__ static void block(const char* lds, int db, int t, bf16x8 (&a)[3]) {
         const int lane = int(threadIdx.x) & 63;
