@@ -254,7 +254,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     using KeyTile = RowTile<BN, DP, 64 * WAVES, VEC>;
     using ValueTile = ColTile<BN, DP, 64 * WAVES>;
     constexpr int kTile = KeyTile::kBytes + ValueTile::kBytes;
-    __shared__ __attribute__((aligned(16))) char lds[2][kTile];
+    // Wide heads leave the third parts of the queries, which one product in six takes, in LDS: all
+    // of them in registers spill.
+    constexpr bool kPark = DP > 64;
+    constexpr int kParked = kPark ? WAVES * (DP / 16) * 1024 : 0;
+    __shared__ __attribute__((aligned(16))) char lds[2 * kTile + kParked];
     const int h = head_of(a, int(blockIdx.x % a.heads));
     const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), 32 * WAVES);
     if (t.rows == 0) return;
@@ -275,6 +279,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     bf16x8 q[DP / 16][3];
     own_row<DP, VEC>(a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim, a.dim,
                      a.scale < 0.0f ? -1.0f : 1.0f, q);
+    char* const parked = lds + 2 * kTile + (wave * (DP / 16) * 64 + lane) * 16;
+    if constexpr (kPark) {
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks)
+            *reinterpret_cast<bf16x8*>(parked + 1024 * ks) = q[ks][2];
+    }
     floatx16 o[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) o[db] = zeros();
@@ -293,7 +303,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     };
     const auto stage = [&](int j) {
         if (j >= end) return;
-        char* const at = lds[j / BN & 1];
+        char* const at = lds + (j / BN & 1) * kTile;
         kt.store(at, t.nk - j, a.dim);
         vt.store(at + KeyTile::kBytes, t.nk - j, a.dim);
     };
@@ -304,7 +314,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     for (int j0 = 0; j0 < end; j0 += BN) {
         // One wave of a SIMD stages the next tile before its products, the other one after them:
         // one's conversions run beside the other's matrix instructions.
-        const char* const lds_k = lds[j0 / BN & 1];
+        const char* const lds_k = lds + (j0 / BN & 1) * kTile;
         const char* const lds_v = lds_k + KeyTile::kBytes;
         if (wave < WAVES / 2) {
             stage(j0 + BN);
@@ -314,13 +324,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
             floatx16 s[BN / 32];
 #pragma unroll
             for (int b = 0; b < BN / 32; ++b) s[b] = zeros();
+            constexpr int NB = BN / 32, kScores = NB * (DP / 16);
+            bf16x8 f[2][3];
+            KeyTile::block(lds_k, 0, 0, f[0]);
 #pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                bf16x8 f[BN / 32][3];
-#pragma unroll
-                for (int b = 0; b < BN / 32; ++b) KeyTile::block(lds_k, b, ks, f[b]);
-                if constexpr (BN == 64) multiply_two(s[0], s[1], f[0], f[1], q[ks]);
-                else multiply(s[0], f[0], q[ks]);
+            for (int n = 0; n < kScores; ++n) {
+                const int ks = n / NB;
+                if (kPark && n % NB == 0)
+                    q[ks][2] = *reinterpret_cast<const bf16x8*>(parked + 1024 * ks);
+                if (n + 1 < kScores)
+                    KeyTile::block(lds_k, (n + 1) % NB, (n + 1) / NB, f[(n + 1) & 1]);
+                keep_order();
+                multiply(s[n % NB], f[n & 1], q[ks]);
+                keep_order();
             }
             if (j0 + BN > wave_all) {
 #pragma unroll
@@ -355,17 +371,22 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
             sum = __builtin_fmaf(sum, keep, part);
             // The tile's sum apart from the running one: that is rounded to nearest once a tile,
             // where the instruction drops low bits towards minus infinity.
+            constexpr int NU = BN / 16, kSums = NU * (DP / 32);
+            floatx16 x = zeros();
+            ValueTile::block(lds_v, 0, 0, f[0]);
 #pragma unroll
-            for (int db = 0; db < DP / 32; ++db) {
-                floatx16 x = zeros();
+            for (int n = 0; n < kSums; ++n) {
+                if (n + 1 < kSums)
+                    ValueTile::block(lds_v, (n + 1) / NU, (n + 1) % NU, f[(n + 1) & 1]);
+                keep_order();
+                multiply(x, f[n & 1], p[n % NU]);
+                keep_order();
+                if (n % NU == NU - 1) {
 #pragma unroll
-                for (int u = 0; u < BN / 16; ++u) {
-                    bf16x8 f[3];
-                    ValueTile::block(lds_v, db, u, f);
-                    multiply(x, f, p[u]);
+                    for (int r = 0; r < 16; ++r)
+                        o[n / NU][r] = __builtin_fmaf(o[n / NU][r], keep, x[r]);
+                    x = zeros();
                 }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[db][r] = __builtin_fmaf(o[db][r], keep, x[r]);
             }
         }
         if (wave >= WAVES / 2) {

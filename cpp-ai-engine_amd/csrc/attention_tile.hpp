@@ -44,15 +44,10 @@ __device__ __forceinline__ void split8(const float* x, bf16x8 (&part)[3]) {
     part[2] = __builtin_bit_cast(bf16x8, l);
 }
 
-// Two products with one B, their sums interleaved.
-__device__ __forceinline__ void multiply_two(floatx16& d0, floatx16& d1, const bf16x8 (&a0)[3],
-                                             const bf16x8 (&a1)[3], const bf16x8 (&b)[3]) {
-#pragma unroll
-    for (int q = 0; q < 6; ++q) {
-        d0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0[kPart[q][0]], b[kPart[q][1]], d0, 0, 0, 0);
-        d1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1[kPart[q][0]], b[kPart[q][1]], d1, 0, 0, 0);
-    }
-}
+// Keeps LDS reads and matrix instructions in the order of the source: the next block's operands are
+// asked for before the products of this one, whose six instructions (192 cycles) cover an LDS read.
+// Left alone the compiler reads them one or two instructions ahead. Other instructions may cross.
+__device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x0216); }
 
 // d += the product of two blocks of 32 x 16.
 __device__ __forceinline__ void multiply(floatx16& d, const bf16x8 (&a)[3], const bf16x8 (&b)[3]) {
