@@ -126,24 +126,22 @@ __device__ __forceinline__ float own_dot(const float* x, const float* y, int dim
     return s + __shfl_xor(s, 32);
 }
 
-// The lane's own row of a result held as D blocks of 32 values.
-template <int DP, bool VEC>
-__device__ __forceinline__ void store_own(float* row, int dim, const floatx16 (&x)[DP / 32]) {
+// Block db (32 values) of the lane's own row of a result, held as a D.
+template <bool VEC>
+__device__ __forceinline__ void store_own(float* row, int dim, int db, const floatx16& x) {
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db)
+    for (int r = 0; r < 16; r += 4) {
+        const int d = 32 * db + row_of(r);
+        if (VEC) {
+            if (d < dim)
+                *reinterpret_cast<floatx4u*>(row + d) =
+                    floatx4u{x[r], x[r + 1], x[r + 2], x[r + 3]};
+        } else {
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const int d = 32 * db + row_of(r);
-            if (VEC) {
-                if (d < dim)
-                    *reinterpret_cast<floatx4u*>(row + d) =
-                        floatx4u{x[db][r], x[db][r + 1], x[db][r + 2], x[db][r + 3]};
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (d + e < dim) row[d + e] = x[db][r + e];
-            }
+            for (int e = 0; e < 4; ++e)
+                if (d + e < dim) row[d + e] = x[r + e];
         }
+    }
 }
 
 // ROWS streamed rows as the A operand of products over the head's values: LDS in three planes, each
