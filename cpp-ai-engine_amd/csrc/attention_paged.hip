@@ -5,9 +5,11 @@
 //
 // over the positions p below the sequence's length, each on the page that the table names.
 
+#include "attention_tile.hpp"
 #include "common.hpp"
 
 #include <cmath>
+#include <cstdlib>
 
 namespace ehip {
 namespace {
@@ -113,19 +115,42 @@ struct Paged {
     float* part_out;     // (sequences, heads, splits, dim)
 };
 
-// x + the values of the other lanes of its group of N (the low bits of the lane number).
+template <int CONTROL>
+__device__ __forceinline__ float moved(float x) {
+    return __builtin_bit_cast(
+        float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CONTROL, 15, 15, true));
+}
+__device__ __forceinline__ float with_row_pair(float x) {  // lanes 16 apart
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x),
+                                                    __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t x0 = r[0], x1 = r[1];  // a bit cast of a vector's element takes the first
+    return __builtin_bit_cast(float, x0) + __builtin_bit_cast(float, x1);
+}
+__device__ __forceinline__ float with_half(float x) {  // lanes 32 apart
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x),
+                                                    __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t x0 = r[0], x1 = r[1];  // a bit cast of a vector's element takes the first
+    return __builtin_bit_cast(float, x0) + __builtin_bit_cast(float, x1);
+}
+
+// The sum over the N lanes of a position (the low bits of the lane number), in each of them.
 template <int N>
 __device__ __forceinline__ float group_sum(float x) {
-    if (N > 1)  // quad_perm 1 0 3 2
-        x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0xb1, 15, 15, true));
-    if (N > 2)  // quad_perm 2 3 0 1
-        x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x4e, 15, 15, true));
-    if (N > 4)  // row_half_mirror
-        x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x141, 15, 15, true));
-    if (N > 8)  // row_mirror
-        x += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x140, 15, 15, true));
-    if (N > 16) x += __shfl_xor(x, 16);
+    if (N > 1) x += moved<0xb1>(x);    // quad_perm 1 0 3 2
+    if (N > 2) x += moved<0x4e>(x);    // quad_perm 2 3 0 1
+    if (N > 4) x += moved<0x141>(x);   // row_half_mirror
+    if (N > 8) x += moved<0x140>(x);   // row_mirror
+    if (N > 16) x = with_row_pair(x);
     return x;
+}
+
+// The sum over the lanes that hold the same values of the wave's 64 / N positions, in each of them.
+template <int N>
+__device__ __forceinline__ float across(float x) {
+    if (N < 16) x += moved<0x128>(x);  // row_ror 8
+    if (N < 8) x += moved<0x124>(x);   // row_ror 4
+    if (N < 32) x = with_row_pair(x);
+    return with_half(x);
 }
 
 // One lane's values of a row as they are stored: 16 bytes, and its own first ones again in lanes past
@@ -149,7 +174,7 @@ struct Values {
 };
 
 template <class T, int LPP, int G, bool VEC>
-__global__ __launch_bounds__(kPagedThreads) void paged_part(Paged a) {
+__global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void paged_part(Paged a) {
     constexpr int N = 16 / int(sizeof(T)), SUBS = 64 / LPP, TILE = SUBS * kUnroll;
     __shared__ float sh_m[kPagedWaves][G], sh_l[kPagedWaves][G], sh_o[kPagedWaves][G][LPP * N];
     const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) / 64;
@@ -209,39 +234,37 @@ __global__ __launch_bounds__(kPagedThreads) void paged_part(Paged a) {
             vs[u].load(v + at, d0, dim);
         }
         row = int(row_of(p0 + kPagedWaves * TILE));
-        float kx[kUnroll][N], vx[kUnroll][N];
+        float w[G][kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
+        for (int u = 0; u < kUnroll; ++u) {
+            float x[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) {
-                kx[u][e] = ks[u][e];
-                vx[u][e] = vs[u][e];
+            for (int e = 0; e < N; ++e) x[e] = ks[u][e];
+            if (dim < LPP * N) {  // a lane past the row's end read something else
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[e] = e < left ? x[e] : 0.0f;
             }
-        // What a lane does not have counts as 0, whatever was read in its place.
-        if (dim < LPP * N) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
+            for (int g = 0; g < G; ++g) {
+                float dot = q[g][0] * x[0];
 #pragma unroll
-                for (int e = 0; e < N; ++e) kx[u][e] = e < left ? kx[u][e] : 0.0f;
+                for (int e = 1; e < N; ++e) dot = __builtin_fmaf(q[g][e], x[e], dot);
+                w[g][u] = group_sum<LPP>(dot);
+            }
         }
-        if (p0 + TILE > end) {
+        const bool tail = p0 + TILE > end;
+        if (tail) {
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-                for (int e = 0; e < N; ++e) vx[u][e] = p0 + u * SUBS + sub < end ? vx[u][e] : 0.0f;
+                for (int g = 0; g < G; ++g)
+                    w[g][u] = p0 + u * SUBS + sub < end ? w[g][u] : -INFINITY;
         }
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            float w[kUnroll], top = m[g];
+            float top = m[g];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                float dot = 0.0f;
-#pragma unroll
-                for (int e = 0; e < N; ++e) dot = __builtin_fmaf(q[g][e], kx[u][e], dot);
-                dot = group_sum<LPP>(dot);
-                w[u] = p0 + u * SUBS + sub < end ? dot : -INFINITY;
-                top = fmaxf(top, w[u]);
-            }
+            for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, w[g][u]);
             // Weights of 2^-24 of their value: sums over the values stay in their range.
             const float shift = top == -INFINITY ? 24.0f : top + 24.0f;
             const float keep =
@@ -252,11 +275,23 @@ __global__ __launch_bounds__(kPagedThreads) void paged_part(Paged a) {
             for (int e = 0; e < N; ++e) o[g][e] *= keep;
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                w[u] = __builtin_amdgcn_exp2f(w[u] - shift);
-                l[g] += w[u];
-#pragma unroll
-                for (int e = 0; e < N; ++e) o[g][e] = __builtin_fmaf(w[u], vx[u][e], o[g][e]);
+                w[g][u] = __builtin_amdgcn_exp2f(w[g][u] - shift);
+                l[g] += w[g][u];
             }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float x[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = vs[u][e];
+            if (tail) {  // nor does a position past the length
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[e] = p0 + u * SUBS + sub < end ? x[e] : 0.0f;
+            }
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[g][e] = __builtin_fmaf(w[g][u], x[e], o[g][e]);
         }
     }
     bad = __syncthreads_or(bad);
@@ -270,8 +305,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_part(Paged a) {
         const float keep = m[g] == -INFINITY ? (l[g] != l[g] ? NAN : 0.0f)
                                              : __builtin_amdgcn_exp2f(m[g] - top);
         l[g] *= keep;
-#pragma unroll
-        for (int w = LPP; w < 64; w *= 2) l[g] += __shfl_xor(l[g], w);
+        l[g] = across<LPP>(l[g]);
         if (lane == 0) {
             sh_m[wave][g] = top;
             sh_l[wave][g] = l[g];
@@ -279,8 +313,7 @@ __global__ __launch_bounds__(kPagedThreads) void paged_part(Paged a) {
 #pragma unroll
         for (int e = 0; e < N; ++e) {
             float y = o[g][e] * keep;
-#pragma unroll
-            for (int w = LPP; w < 64; w *= 2) y += __shfl_xor(y, w);
+            y = across<LPP>(y);
             if (sub == 0) sh_o[wave][g][d0 + e] = y;
         }
     }
@@ -308,6 +341,275 @@ __global__ __launch_bounds__(kPagedThreads) void paged_part(Paged a) {
             for (int w = 0; w < kPagedWaves; ++w) y += sh_o[w][g][d] * keep[w];
             if (a.splits > 1) a.part_out[(at * a.splits + split) * dim + d] = y;
             else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = n == 0 ? 0.0f : y / sum;
+        }
+    }
+}
+
+// One head's share of a block by the formula, for those whose sums by parts are not finite: a part of
+// an infinity, or an infinity times the parts of a finite value, is NaN where the product is an
+// infinity or, its weight 0, nothing at all. One wave.
+template <class T>
+__device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int begin, int end,
+                                float& top, float& sum, float (&o)[2]) {
+    const int lane = int(threadIdx.x) & 63, dim = int(a.c.dim);
+    const int64_t pitch = a.c.kv_heads * dim;
+    const float* q = a.q + s * a.ld_q + int64_t(h) * dim;
+    const T* k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
+    const T* v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
+    const float c2 = a.scale * 1.44269504088896340736f;
+    const auto score = [&](int p) {
+        const T* row = k + pool_row(a.c, s, p) * pitch;
+        float dot = 0.0f;
+        for (int e = 0; e < dim; ++e) dot = __builtin_fmaf(q[e] * c2, widen(row[e]), dot);
+        return dot;
+    };
+    top = -INFINITY;
+    for (int p = begin + lane; p < end; p += 64) top = fmaxf(top, score(p));
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
+    sum = o[0] = o[1] = 0.0f;
+    for (int p0 = begin; p0 < end; p0 += 64) {
+        const int p = p0 + lane;
+        const float weight = p < end ? exp2f(score(p) - top) * 0x1p-24f : 0.0f;
+        sum += weight;
+        for (int u = 0; u < 64 && p0 + u < end; ++u) {
+            const T* row = v + pool_row(a.c, s, p0 + u) * pitch;
+            const float w = __shfl(weight, u);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (lane + 64 * e < dim)
+                    o[e] = __builtin_fmaf(w, widen(row[lane + 64 * e]), o[e]);
+        }
+    }
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
+}
+
+// A cache in bf16, up to 16 query heads of a key head at a time, on v_mfma_f32_16x16x32_bf16: the
+// cached values are operands as they are, q and the weights in three parts, so a score and a
+// weighted value take three products each, for any number of heads at one cost; by vector
+// instructions four heads ran at 4.3 TB/s of 5.4 and eight at 2.7. Lane l holds A(l % 16, 8 (l / 16) +
+// 0..7), B(8 (l / 16) + 0..7, l % 16) and D(4 (l / 16) + r, l % 16).
+//   scores:  A = 16 positions by 32 values of K, as 16-byte reads leave them; B = q; D's column = head
+//   weights: the D's of positions 0..15 and 16..31 are the B of 32 positions, in the order 4 h + 0..3,
+//            16 + 4 h + 0..3 for the lanes h = l / 16
+//   values:  A = 16 values by those 32 positions of V: rows in LDS, read transposed
+// A wave takes 32 positions at a time; the next ones' reads are out while it forms weights and sums.
+constexpr int kTilePositions = 32;
+
+template <int DP>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
+    using attention::bf16x8;
+    using attention::floatx4u;
+    using attention::uintx4;
+    typedef float floatx4 __attribute__((ext_vector_type(4)));
+    typedef short shortx4 __attribute__((ext_vector_type(4)));
+    constexpr int KS = DP / 32, NV = DP / 16, LANES = DP / 8;  // lanes of a row's reads
+    constexpr int kRows = 64 / LANES, kReads = (kTilePositions + kRows - 1) / kRows;
+    // Rows 32 bytes apart in banks: a transposed read's sixteen rows take all banks twice.
+    constexpr int kPitch = 2 * DP + 32;
+    constexpr int kWaveLds = kTilePositions * kPitch;
+    constexpr int kLds = kWaveLds > 16 * DP * 4 ? kWaveLds : 16 * DP * 4;
+    __shared__ __attribute__((aligned(16))) char lds[kPagedWaves][kLds];
+    __shared__ float sh_m[kPagedWaves][16], sh_l[kPagedWaves][16];
+    const int lane = int(threadIdx.x) & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int kv_heads = int(a.c.kv_heads), dim = int(a.c.dim);
+    const int group = a.heads / kv_heads, pieces = (group + 15) / 16;
+    uint32_t x = blockIdx.x;
+    const int kv = int(x % uint32_t(kv_heads));
+    x /= uint32_t(kv_heads);
+    const int h0 = kv * group + int(x % uint32_t(pieces)) * 16;
+    const int count = min(16, (kv + 1) * group - h0);  // the block's heads
+    x /= uint32_t(pieces);
+    const int split = int(x % uint32_t(a.splits));
+    const int64_t s = x / uint32_t(a.splits);
+    const int n = a.lengths[s];
+    const int64_t held = a.c.width * a.c.page_size;
+    bool bad = n < 0 || n > a.longest || n > held || (n > 0 && a.c.pages == 0);
+    const int begin = split * a.chunk;
+    const int end = bad ? begin : min(n, begin + a.chunk);
+    if (split > 0 && (bad || begin >= n)) return;
+
+    const int col = lane & 15, quarter = lane / 16;
+    const float c2 = a.scale * 1.44269504088896340736f;
+    bf16x8 q[KS][3];
+    {
+        const float* row = a.q + s * a.ld_q + int64_t(h0 + (col < count ? col : 0)) * dim;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d0 = 32 * ks + 8 * quarter;
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                y[e] = d0 < dim && col < count ? row[d0 < dim ? d0 + e : 0] * c2 : 0.0f;
+            attention::split8(y, q[ks]);
+        }
+    }
+    floatx4 o[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+
+    const Bf16* const k = static_cast<const Bf16*>(a.c.k) + int64_t(kv) * dim;
+    const Bf16* const v = static_cast<const Bf16*>(a.c.v) + int64_t(kv) * dim;
+    const int64_t pitch = int64_t(kv_heads) * dim;
+    bf16x8 kx[2][KS];
+    uintx4 vx[kReads];
+    const int v_lane = lane / LANES, v_d0 = lane % LANES * 8;
+    const auto load = [&](int p0) {
+        const int p = p0 + (lane & 31);
+        int64_t row = 0;
+        if (p < end) {
+            row = pool_row(a.c, s, p);
+            if (row < 0) {
+                bad = true;
+                row = 0;
+            }
+        }
+        const int r = int(row);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const Bf16* at = k + int64_t(__shfl(r, 16 * t + col)) * pitch;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int d0 = 32 * ks + 8 * quarter;
+                kx[t][ks] = *reinterpret_cast<const bf16x8*>(at + (d0 < dim ? d0 : 0));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) {
+            const int j = i * kRows + v_lane;
+            const Bf16* at = v + int64_t(__shfl(r, j < kTilePositions ? j : 0)) * pitch;
+            vx[i] = *reinterpret_cast<const uintx4*>(at + (v_d0 < dim ? v_d0 : 0));
+        }
+    };
+    char* const mine = lds[wave];
+    const int first = begin + wave * kTilePositions;
+    if (first < end) load(first);
+    for (int p0 = first; p0 < end; p0 += kPagedWaves * kTilePositions) {
+        const bool tail = p0 + kTilePositions > end;
+#pragma unroll
+        for (int i = 0; i < kReads; ++i) {
+            const int j = i * kRows + v_lane;
+            uintx4 y = vx[i];
+            if (tail && p0 + j >= end) y = uintx4{0, 0, 0, 0};  // nothing, whatever is there
+            if (v_lane < kRows && j < kTilePositions)
+                *reinterpret_cast<uintx4*>(mine + j * kPitch + 2 * v_d0) = y;
+        }
+        floatx4 sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            sc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int part = 2; part >= 0; --part)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    // Past the row's end q is 0 and K something else, which has to be finite.
+                    bf16x8 f = kx[t][ks];
+                    if (DP != dim && 32 * ks + 8 * quarter >= dim)
+                        f = __builtin_bit_cast(bf16x8, uintx4{0, 0, 0, 0});
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][part], sc[t], 0, 0, 0);
+                }
+        }
+        if (p0 + kPagedWaves * kTilePositions < end) load(p0 + kPagedWaves * kTilePositions);
+        if (tail) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (p0 + 16 * t + 4 * quarter + r >= end) sc[t][r] = -INFINITY;
+        }
+        float top = m;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float shift = top == -INFINITY ? 24.0f : top + 24.0f;
+        const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m + 24.0f - shift);
+        m = top;
+        float w[8], part_sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j % 4] - shift);
+            part_sum += w[j];
+        }
+        l = __builtin_fmaf(l, keep, part_sum);
+        bf16x8 p[3];
+        attention::split8(w, p);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            typedef __attribute__((address_space(3))) shortx4* Rows;
+            // Lane: row 4 quarter + col / 4 (and 16 rows on), four values from 16 i + 4 (col % 4).
+            const char* at = mine + (4 * quarter + col / 4) * kPitch + 32 * i + 8 * (col % 4);
+            struct {
+                shortx4 x, y;
+            } f = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)at),
+                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(at + 16 * kPitch))};
+            const bf16x8 vt = __builtin_bit_cast(bf16x8, f);
+            floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int part = 2; part >= 0; --part)
+                y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, p[part], y, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[i][r] = __builtin_fmaf(o[i][r], keep, y[r]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    bad = __syncthreads_or(bad);
+
+    // The waves of the block: sums of head `col`, value 16 i + 4 quarter + r.
+    l = with_half(with_row_pair(l));
+    if (quarter == 0) {
+        sh_m[wave][col] = m;
+        sh_l[wave][col] = l;
+    }
+    float* const sums = reinterpret_cast<float*>(mine);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        *reinterpret_cast<floatx4*>(sums + col * DP + 16 * i + 4 * quarter) = o[i];
+    __syncthreads();
+    for (int g = wave; g < count; g += kPagedWaves) {
+        float top = sh_m[0][g], sum = 0.0f, keep[kPagedWaves], y[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int u = 1; u < kPagedWaves; ++u) top = fmaxf(top, sh_m[u][g]);
+        bool fine = true;
+#pragma unroll
+        for (int u = 0; u < kPagedWaves; ++u) {
+            keep[u] = sh_m[u][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh_m[u][g] - top);
+            sum += sh_l[u][g] * keep[u];
+            fine = fine && fabsf(sh_l[u][g]) < INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int d = lane + 64 * e;
+            if (d >= dim) continue;
+#pragma unroll
+            for (int u = 0; u < kPagedWaves; ++u)
+                y[e] += reinterpret_cast<const float*>(lds[u])[g * DP + d] * keep[u];
+            fine = fine && fabsf(y[e]) < INFINITY;
+        }
+        if (!bad && begin < end && !(__all(fine) && sum > 0.0f))
+            part_by_formula<Bf16>(a, s, h0 + g, kv, begin, end, top, sum, y);
+        const int64_t at = s * a.heads + h0 + g;
+        if (bad) sum = NAN;
+        if (lane == 0) {
+            if (a.splits > 1) a.part_stats[at * a.splits + split] = float2{top, sum};
+            else if (a.lse != nullptr) a.lse[at] = n == 0 ? -INFINITY : lse_of(top, sum);
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int d = lane + 64 * e;
+            if (d >= dim) continue;
+            if (a.splits > 1) a.part_out[(at * a.splits + split) * dim + d] = y[e];
+            else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = n == 0 ? 0.0f : y[e] / sum;
         }
     }
 }
@@ -396,8 +698,11 @@ struct Split {
 Split split_of(const Cache& c, int64_t heads, int64_t longest) {
     const int64_t group = heads / c.kv_heads;
     const int64_t units = c.sequences * c.kv_heads * ceil_div(group, kMaxGroup);
-    const int64_t most = ceil_div(longest > 0 ? longest : 1, 256);
-    int64_t splits = ceil_div(4096, units > 0 ? units : 1);
+    
+    static const char* e1 = getenv("TARGET"); static const char* e2 = getenv("LEAST");
+    const int64_t T = e1 ? atoi(e1) : 4096, LE = e2 ? atoi(e2) : 256;
+    int64_t splits = ceil_div(T, units > 0 ? units : 1);
+    const int64_t most = ceil_div(longest > 0 ? longest : 1, LE);
     splits = splits < most ? splits : most;
     const int64_t chunk = ceil_div(ceil_div(longest > 0 ? longest : 1, splits), 64) * 64;
     return {int(ceil_div(longest > 0 ? longest : 1, chunk)), int(chunk)};
@@ -436,10 +741,25 @@ int launch_lanes(const Paged& a, hipStream_t s) {
 }
 
 // 16-byte reads where every head's row begins at 16 bytes.
-template <class T>
-int launch_parts(const Paged& a, bool aligned, hipStream_t s) {
-    return aligned && a.c.dim % int64_t(16 / sizeof(T)) == 0 ? launch_lanes<T, true>(a, s)
-                                                             : launch_lanes<T, false>(a, s);
+int launch_parts_f32(const Paged& a, bool aligned, hipStream_t s) {
+    return aligned && a.c.dim % 4 == 0 ? launch_lanes<float, true>(a, s)
+                                       : launch_lanes<float, false>(a, s);
+}
+
+template <int DP>
+int launch_part_bf16(const Paged& a, hipStream_t s) {
+    const int64_t group = a.heads / a.c.kv_heads;
+    const int64_t blocks = a.c.sequences * a.splits * ceil_div(group, 16) * a.c.kv_heads;
+    EHIP_LAUNCH("attention_paged", paged_part_bf16<DP>, dim3(unsigned(blocks)),
+                dim3(kPagedThreads), 0, s, a);
+    return EHIP_OK;
+}
+
+int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
+    if (!aligned || a.c.dim % 8 != 0) return launch_lanes<Bf16, false>(a, s);
+    if (a.c.dim <= 32) return launch_part_bf16<32>(a, s);
+    if (a.c.dim <= 64) return launch_part_bf16<64>(a, s);
+    return launch_part_bf16<128>(a, s);
 }
 
 }  // namespace
@@ -519,8 +839,8 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     }
     hipStream_t s = as_stream(stream);
     const bool aligned = aligned16(c.k) && aligned16(c.v);
-    const int rc = cache->type == EHIP_CACHE_F32 ? launch_parts<float>(a, aligned, s)
-                                                 : launch_parts<Bf16>(a, aligned, s);
+    const int rc = cache->type == EHIP_CACHE_F32 ? launch_parts_f32(a, aligned, s)
+                                                 : launch_parts_bf16(a, aligned, s);
     if (rc != EHIP_OK || p.splits == 1) return rc;
     EHIP_LAUNCH("attention_paged_join", paged_join, dim3(unsigned(c.sequences * heads)), dim3(256),
                 0, s, a);
