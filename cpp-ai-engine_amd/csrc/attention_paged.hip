@@ -8,8 +8,8 @@
 #include "attention_tile.hpp"
 #include "common.hpp"
 
+#include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 namespace ehip {
 namespace {
@@ -110,10 +110,119 @@ struct Paged {
     float* out;
     int64_t ld_out;
     float* lse;
-    int splits, chunk;   // a sequence's positions by blocks
-    float2* part_stats;  // (sequences, heads, splits): maximum (as 2^x), sum
-    float* part_out;     // (sequences, heads, splits, dim)
+    int workers;         // blocks of a key head (and piece of its query heads)
+    float2* part_stats;  // (heads, workers + sequences): maximum (as 2^x), sum
+    float* part_out;     // (heads, workers + sequences, dim)
+    int* first;          // (sequences + 1): the sequences' first tiles
 };
+
+// The work is cut evenly, whatever the lengths: the positions of all sequences in tiles of kTile, one
+// after the other, and a worker's blocks (one for each key head) take its share of them, which may
+// be part of a long sequence or several short ones. What a worker adds to a sequence is a segment.
+// Segment (worker w, sequence s) has place w + s of a head's parts, no other's: from one to the next
+// at least one of them grows.
+constexpr int kTile = 128;
+
+// Positions of a sequence, -1 for a length that is none.
+__device__ __forceinline__ int length_of(const Paged& a, int64_t s) {
+    const int n = a.lengths[s];
+    return n < 0 || n > a.longest || n > a.c.width * a.c.page_size || (n > 0 && a.c.pages == 0)
+               ? -1
+               : n;
+}
+__device__ __forceinline__ int tiles_of(int n) { return n > 0 ? (n - 1) / kTile + 1 : 0; }
+
+// The first tile of worker w of so many tiles, and the worker of tile t. With fewer tiles than workers
+// the last ones have none; every other one has one at least.
+__device__ __forceinline__ int first_tile(const Paged& a, int w, int tiles) {
+    const int workers = min(a.workers, tiles);
+    return w < workers ? int(int64_t(w) * tiles / workers) : tiles;
+}
+__device__ __forceinline__ int worker_of(const Paged& a, int t, int tiles) {
+    return int(((int64_t(t) + 1) * min(a.workers, tiles) - 1) / tiles);
+}
+
+struct Segment {
+    int64_t s;       // the sequence
+    int n;           // its length
+    int begin, end;  // positions
+    int t, t_end;    // the worker's tiles from here on
+    int t0;          // the sequence's first
+    bool whole;      // the sequence is this segment
+};
+
+__device__ __forceinline__ int wave_scan(int x) {  // inclusive
+    const int lane = int(threadIdx.x) & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(x, d);
+        x += lane >= d ? y : 0;
+    }
+    return x;
+}
+
+// Sequence, positions and last tile of a segment from its first tile g.t, s and t0 given.
+__device__ __forceinline__ void measure(const Paged& a, Segment& g) {
+    const int stop = min(g.t_end, g.t0 + tiles_of(g.n));
+    g.begin = (g.t - g.t0) * kTile;
+    g.end = stop - g.t0 == tiles_of(g.n) ? g.n : (stop - g.t0) * kTile;
+    g.whole = g.begin == 0 && g.end == g.n;
+}
+
+// The first segment of worker w (t == t_end: none). Every wave finds the same; block 0 leaves the
+// sequences' first tiles for the join.
+__device__ __forceinline__ Segment first_segment(const Paged& a, int w) {
+    const int lane = int(threadIdx.x) & 63;
+    const int sequences = int(a.c.sequences);
+    int tiles = 0;
+    for (int base = 0; base < sequences; base += 64) {
+        const int s = base + lane;
+        const int mine = s < sequences ? tiles_of(length_of(a, s)) : 0;
+        const int upto = wave_scan(mine);
+        if (blockIdx.x == 0 && threadIdx.x < 64 && a.first != nullptr && s < sequences)
+            a.first[s] = tiles + upto - mine;
+        tiles += __shfl(upto, 63);
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.first != nullptr) a.first[sequences] = tiles;
+    Segment g{};
+    g.t = first_tile(a, w, tiles);
+    g.t_end = first_tile(a, w + 1, tiles);
+    if (g.t == g.t_end) return g;
+    int before = 0;
+    for (int base = 0; base < sequences; base += 64) {
+        const int s = base + lane;
+        const int mine = s < sequences ? tiles_of(length_of(a, s)) : 0;
+        const int upto = before + wave_scan(mine);
+        const uint64_t past = __ballot(upto > g.t);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            g.s = base + at;
+            g.t0 = __shfl(upto - mine, at);
+            break;
+        }
+        before = __shfl(upto, 63);
+    }
+    g.s = __builtin_amdgcn_readfirstlane(int(g.s));
+    g.t0 = __builtin_amdgcn_readfirstlane(g.t0);
+    g.n = length_of(a, g.s);
+    measure(a, g);
+    return g;
+}
+
+__device__ __forceinline__ void next_segment(const Paged& a, Segment& g) {
+    const int stop = g.t0 + tiles_of(g.n);
+    g.t = min(g.t_end, stop);
+    if (g.t == g.t_end) return;
+    do {
+        if (++g.s >= a.c.sequences) {  // only where the lengths changed under the launch
+            g.t = g.t_end;
+            return;
+        }
+        g.n = length_of(a, g.s);
+    } while (tiles_of(g.n) == 0);
+    g.t0 = stop;
+    measure(a, g);
+}
 
 template <int CONTROL>
 __device__ __forceinline__ float moved(float x) {
@@ -186,15 +295,11 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
     const int h0 = kv * group + int(x % uint32_t(pieces)) * G;
     const int count = min(G, (kv + 1) * group - h0);  // the block's heads
     x /= uint32_t(pieces);
-    const int split = int(x % uint32_t(a.splits));
-    const int64_t s = x / uint32_t(a.splits);
-    const int n = a.lengths[s];
-    const int64_t held = a.c.width * a.c.page_size;
-    // A length that is none leaves NaN, by its first block.
-    bool bad = n < 0 || n > a.longest || n > held || (n > 0 && a.c.pages == 0);
-    const int begin = split * a.chunk;
-    const int end = bad ? begin : min(n, begin + a.chunk);
-    if (split > 0 && (bad || begin >= n)) return;
+    const int worker = int(x);
+    for (Segment seg = first_segment(a, worker); seg.t < seg.t_end; next_segment(a, seg)) {
+    const int64_t s = seg.s;
+    const int begin = seg.begin, end = seg.end;
+    bool bad = false;  // a page outside the pool
 
     const int sub = lane / LPP, d0 = (lane % LPP) * N, left = dim - d0;
     const float c2 = fabsf(a.scale) * 1.44269504088896340736f;
@@ -328,20 +433,21 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
             keep[w] = sh_m[w][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh_m[w][g] - top);
             sum += sh_l[w][g] * (sh_l[w][g] != sh_l[w][g] ? 1.0f : keep[w]);
         }
-        const int64_t at = s * a.heads + h0 + g;
+        const int64_t at = int64_t(h0 + g) * (a.workers + a.c.sequences) + worker + s;
         if (bad) sum = NAN;
-        if (a.splits > 1) {
-            if (threadIdx.x == 0) a.part_stats[at * a.splits + split] = float2{top, sum};
-        } else if (threadIdx.x == 0 && a.lse != nullptr) {
-            a.lse[at] = n == 0 ? -INFINITY : lse_of(top, sum);
+        if (threadIdx.x == 0) {
+            if (!seg.whole) a.part_stats[at] = float2{top, sum};
+            else if (a.lse != nullptr) a.lse[s * a.heads + h0 + g] = lse_of(top, sum);
         }
         for (int d = int(threadIdx.x); d < dim; d += kPagedThreads) {
             float y = 0.0f;
 #pragma unroll
             for (int w = 0; w < kPagedWaves; ++w) y += sh_o[w][g][d] * keep[w];
-            if (a.splits > 1) a.part_out[(at * a.splits + split) * dim + d] = y;
-            else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = n == 0 ? 0.0f : y / sum;
+            if (!seg.whole) a.part_out[at * dim + d] = y;
+            else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y / sum;
         }
+    }
+    __syncthreads();
     }
 }
 
@@ -422,14 +528,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
     const int h0 = kv * group + int(x % uint32_t(pieces)) * 16;
     const int count = min(16, (kv + 1) * group - h0);  // the block's heads
     x /= uint32_t(pieces);
-    const int split = int(x % uint32_t(a.splits));
-    const int64_t s = x / uint32_t(a.splits);
-    const int n = a.lengths[s];
-    const int64_t held = a.c.width * a.c.page_size;
-    bool bad = n < 0 || n > a.longest || n > held || (n > 0 && a.c.pages == 0);
-    const int begin = split * a.chunk;
-    const int end = bad ? begin : min(n, begin + a.chunk);
-    if (split > 0 && (bad || begin >= n)) return;
+    const int worker = int(x);
+    for (Segment seg = first_segment(a, worker); seg.t < seg.t_end; next_segment(a, seg)) {
+    const int64_t s = seg.s;
+    const int begin = seg.begin, end = seg.end;
+    bool bad = false;  // a page outside the pool
 
     const int col = lane & 15, quarter = lane / 16;
     const float c2 = a.scale * 1.44269504088896340736f;
@@ -596,48 +699,59 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
                 y[e] += reinterpret_cast<const float*>(lds[u])[g * DP + d] * keep[u];
             fine = fine && fabsf(y[e]) < INFINITY;
         }
-        if (!bad && begin < end && !(__all(fine) && sum > 0.0f))
+        if (!bad && !(__all(fine) && sum > 0.0f))
             part_by_formula<Bf16>(a, s, h0 + g, kv, begin, end, top, sum, y);
-        const int64_t at = s * a.heads + h0 + g;
+        const int64_t at = int64_t(h0 + g) * (a.workers + a.c.sequences) + worker + s;
         if (bad) sum = NAN;
         if (lane == 0) {
-            if (a.splits > 1) a.part_stats[at * a.splits + split] = float2{top, sum};
-            else if (a.lse != nullptr) a.lse[at] = n == 0 ? -INFINITY : lse_of(top, sum);
+            if (!seg.whole) a.part_stats[at] = float2{top, sum};
+            else if (a.lse != nullptr) a.lse[s * a.heads + h0 + g] = lse_of(top, sum);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int d = lane + 64 * e;
             if (d >= dim) continue;
-            if (a.splits > 1) a.part_out[(at * a.splits + split) * dim + d] = y[e];
-            else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = n == 0 ? 0.0f : y[e] / sum;
+            if (!seg.whole) a.part_out[at * dim + d] = y[e];
+            else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y[e] / sum;
         }
+    }
+    __syncthreads();
     }
 }
 
-// The blocks of a sequence and a head. Thread d % 128 has a value, two threads for alternate blocks.
+// The segments of a sequence and a head, where there are several, and the rows of sequences that
+// have no segment. Thread d % 128 has a value, two threads for alternate segments.
 __global__ __launch_bounds__(256) void paged_join(Paged a) {
     __shared__ float sh[2][kMaxDim], sh_l[2];
     const int64_t at = blockIdx.x, s = at / a.heads;
     const int h = int(at % a.heads), dim = int(a.c.dim);
-    const int n = a.lengths[s];
-    const bool bad = n < 0 || n > a.longest || n > a.c.width * a.c.page_size ||
-                     (n > 0 && a.c.pages == 0);
-    const int parts = bad ? 0 : (n + a.chunk - 1) / a.chunk;
     const int d = int(threadIdx.x) % kMaxDim, half = int(threadIdx.x) / kMaxDim;
-    const float2* stats = a.part_stats + at * a.splits;
+    const int n = length_of(a, s);
+    if (n <= 0) {
+        if (half == 0 && d < dim)
+            a.out[s * a.ld_out + int64_t(h) * dim + d] = n < 0 ? NAN : 0.0f;
+        if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at] = n < 0 ? NAN : -INFINITY;
+        return;
+    }
+    const int tiles = a.first[a.c.sequences];
+    const int w0 = worker_of(a, a.first[s], tiles);
+    const int parts = worker_of(a, a.first[s + 1] - 1, tiles) - w0 + 1;
+    if (parts == 1) return;  // the sequence was one segment
+    const int64_t from = int64_t(h) * (a.workers + a.c.sequences) + w0 + s;
+    const float2* stats = a.part_stats + from;
     float top = -INFINITY;
     for (int i = int(threadIdx.x) & 63; i < parts; i += 64) top = fmaxf(top, stats[i].x);
 #pragma unroll
     for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
     float sum = 0.0f, y = 0.0f;
-    const float* from = a.part_out + at * a.splits * dim + (d < dim ? d : 0);
-#pragma unroll 4
+    const float* values = a.part_out + from * dim + (d < dim ? d : 0);
+#pragma unroll 8
     for (int i = half; i < parts; i += 2) {
         const float2 z = stats[i];
         const float keep = z.x == -INFINITY ? (z.y != z.y ? NAN : 0.0f)
                                             : __builtin_amdgcn_exp2f(z.x - top);
         sum += z.y * keep;
-        y = __builtin_fmaf(from[int64_t(i) * dim], keep, y);
+        y = __builtin_fmaf(values[int64_t(i) * dim], keep, y);
     }
     sh[half][d] = y;
     if (d == 0) sh_l[half] = sum;
@@ -645,10 +759,8 @@ __global__ __launch_bounds__(256) void paged_join(Paged a) {
     if (half != 0) return;
     sum = sh_l[0] + sh_l[1];
     y += sh[1][d];
-    if (d < dim)
-        a.out[s * a.ld_out + int64_t(h) * dim + d] = bad ? NAN : (n == 0 ? 0.0f : y / sum);
-    if (d == 0 && a.lse != nullptr)
-        a.lse[at] = bad ? NAN : (n == 0 ? -INFINITY : lse_of(top, sum));
+    if (d < dim) a.out[s * a.ld_out + int64_t(h) * dim + d] = y / sum;
+    if (d == 0 && a.lse != nullptr) a.lse[at] = lse_of(top, sum);
 }
 
 // ---------------------------------------------------------------- host checks
@@ -682,42 +794,35 @@ int check_heads(const char* name, const Cache& c, int64_t heads, int64_t longest
     if (c.dim > kMaxDim || heads < 1 || heads % c.kv_heads != 0 || longest < 0)
         return fail(EHIP_EINVAL, "%s: %lld heads over %lld of %lld values, length %lld", name,
                     (long long)heads, (long long)c.kv_heads, (long long)c.dim, (long long)longest);
-    if (heads > kMaxBlocks || c.sequences * heads > kMaxBlocks || longest > INT32_MAX)
+    if (heads > kMaxBlocks || c.sequences * heads > kMaxBlocks || longest > INT32_MAX ||
+        c.sequences * ceil_div(longest, kTile) > INT32_MAX)
         return fail(EHIP_EINVAL, "%s: %lld sequences of %lld heads of length %lld are too many",
                     name, (long long)c.sequences, (long long)heads, (long long)longest);
     return EHIP_OK;
 }
 
-struct Split {
-    int splits, chunk;
-};
-
-// How many blocks a sequence's length is cut into, and the positions of each: enough for some
-// sixteen blocks a CU over all, of 256 positions at least (below that the join costs more than the
-// blocks gain).
-Split split_of(const Cache& c, int64_t heads, int64_t longest) {
+// Workers for 512 blocks in all, two a CU (64 sequences of 64 to 4096 positions in bf16: 75 us against
+// 85 with 1024 blocks and 101 with 2048; two of 131072 in fp32: 383, 388, 389), and no more than there
+// can be tiles.
+int workers_of(const Cache& c, int64_t heads, int64_t longest, int type) {
     const int64_t group = heads / c.kv_heads;
-    const int64_t units = c.sequences * c.kv_heads * ceil_div(group, kMaxGroup);
-    
-    static const char* e1 = getenv("TARGET"); static const char* e2 = getenv("LEAST");
-    const int64_t T = e1 ? atoi(e1) : 4096, LE = e2 ? atoi(e2) : 256;
-    int64_t splits = ceil_div(T, units > 0 ? units : 1);
-    const int64_t most = ceil_div(longest > 0 ? longest : 1, LE);
-    splits = splits < most ? splits : most;
-    const int64_t chunk = ceil_div(ceil_div(longest > 0 ? longest : 1, splits), 64) * 64;
-    return {int(ceil_div(longest > 0 ? longest : 1, chunk)), int(chunk)};
+    const int64_t units = c.kv_heads * ceil_div(group, type == EHIP_CACHE_F32 ? kMaxGroup : 16);
+    constexpr int64_t resident = 512;
+    const int64_t most = std::max<int64_t>(1, c.sequences * ceil_div(longest, kTile));
+    return int(std::min(most, std::max<int64_t>(1, resident / units)));
 }
 
-size_t part_bytes(const Cache& c, int64_t heads, int splits) {
-    return splits > 1 ? size_t(c.sequences) * size_t(heads) * size_t(splits) *
-                            (sizeof(float2) + size_t(c.dim) * sizeof(float))
-                      : 0;
+// Parts of a head, and the bytes of all heads' and of the sequences' first tiles.
+size_t part_bytes(const Cache& c, int64_t heads, int workers) {
+    return size_t(heads) * size_t(workers + c.sequences) *
+               (sizeof(float2) + size_t(c.dim) * sizeof(float)) +
+           size_t(c.sequences + 1) * sizeof(int);
 }
 
 template <class T, int LPP, int G, bool VEC>
 int launch_part(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
-    const int64_t blocks = a.c.sequences * a.splits * ceil_div(group, G) * a.c.kv_heads;
+    const int64_t blocks = a.workers * ceil_div(group, G) * a.c.kv_heads;
     EHIP_LAUNCH("attention_paged", (paged_part<T, LPP, G, VEC>), dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
@@ -749,7 +854,7 @@ int launch_parts_f32(const Paged& a, bool aligned, hipStream_t s) {
 template <int DP>
 int launch_part_bf16(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
-    const int64_t blocks = a.c.sequences * a.splits * ceil_div(group, 16) * a.c.kv_heads;
+    const int64_t blocks = a.workers * ceil_div(group, 16) * a.c.kv_heads;
     EHIP_LAUNCH("attention_paged", paged_part_bf16<DP>, dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
@@ -799,7 +904,9 @@ int64_t ehip_attention_paged_workspace(const ehip_cache_t* cache, int64_t heads,
     Cache c;
     if (check("attention_paged", cache, c) || check_heads("attention_paged", c, heads, longest))
         return -1;
-    return int64_t(part_bytes(c, heads, split_of(c, heads, longest).splits));
+    return c.sequences == 0
+               ? 0
+               : int64_t(part_bytes(c, heads, workers_of(c, heads, longest, cache->type)));
 }
 
 int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t ld_q,
@@ -815,9 +922,9 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     if (c.sequences == 0) return EHIP_OK;
     if (q == nullptr || lengths == nullptr || out == nullptr)
         return fail(EHIP_EINVAL, "attention_paged: null tensor");
-    const Split p = split_of(c, heads, longest);
-    const size_t need = part_bytes(c, heads, p.splits);
-    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+    const int workers = workers_of(c, heads, longest, cache->type);
+    const size_t need = part_bytes(c, heads, workers);
+    if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
         return fail(EHIP_EINVAL, "attention_paged: needs %zu bytes of 16-byte aligned workspace",
                     need);
     Paged a{};
@@ -831,17 +938,16 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     a.out = out;
     a.ld_out = ld_out;
     a.lse = lse;
-    a.splits = p.splits;
-    a.chunk = p.chunk;
-    if (need > 0) {
-        a.part_stats = static_cast<float2*>(workspace);
-        a.part_out = reinterpret_cast<float*>(a.part_stats + c.sequences * heads * p.splits);
-    }
+    a.workers = workers;
+    const int64_t parts = heads * (workers + c.sequences);
+    a.part_stats = static_cast<float2*>(workspace);
+    a.part_out = reinterpret_cast<float*>(a.part_stats + parts);
+    a.first = reinterpret_cast<int*>(a.part_out + parts * c.dim);
     hipStream_t s = as_stream(stream);
     const bool aligned = aligned16(c.k) && aligned16(c.v);
     const int rc = cache->type == EHIP_CACHE_F32 ? launch_parts_f32(a, aligned, s)
                                                  : launch_parts_bf16(a, aligned, s);
-    if (rc != EHIP_OK || p.splits == 1) return rc;
+    if (rc != EHIP_OK) return rc;
     EHIP_LAUNCH("attention_paged_join", paged_join, dim3(unsigned(c.sequences * heads)), dim3(256),
                 0, s, a);
     return EHIP_OK;
