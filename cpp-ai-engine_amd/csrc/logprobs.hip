@@ -128,6 +128,20 @@ struct Top {
     int count;
 };
 
+// list = the largest `top` of found[0 .. n), which all differ, 0 after them. Every thread calls it.
+__device__ __forceinline__ void list_found(Top& sh, int n, int top) {
+    for (int i = int(threadIdx.x); i < top; i += kThreads)
+        if (i >= n) sh.list[i] = 0;
+    for (int i = int(threadIdx.x); i < n; i += kThreads) {
+        const uint64_t k = sh.found[i];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += sh.found[j] > k;
+        if (rank < top) sh.list[rank] = k;  // the order of arrival does not matter
+    }
+    __syncthreads();
+}
+
 // Takes the kOffer keys key(0) .. of every thread (0: none; all others differ from each other and from
 // the list's) into the list of the `top` largest. Every thread calls it.
 template <class Key>
@@ -146,12 +160,27 @@ __device__ __forceinline__ void offer(Top& sh, int top, Key key) {
     // `top`-th of the threads' largest is a lower limit of the list, and as many threads reach it.
     uint64_t limit = 0;
     if (threads > top) {
-        sh.largest[threadIdx.x] = largest;
-        __syncthreads();
+        // The wave's order first: only its first `top` can be among the block's.
         int rank = 0;
 #pragma unroll 8
-        for (int i = 0; i < kThreads; ++i) rank += sh.largest[i] > largest;
-        if (rank == top - 1 && largest != 0) sh.limit = largest;
+        for (int i = 0; i < 64; ++i) {
+            const uint64_t other =
+                uint64_t(uint32_t(__builtin_amdgcn_readlane(int(largest >> 32), i))) << 32 |
+                uint32_t(__builtin_amdgcn_readlane(int(uint32_t(largest)), i));
+            rank += other > largest;
+        }
+        const int each = top < 64 ? top : 64;
+        const bool mine = rank < each && largest != 0;
+        sh.largest[threadIdx.x] = 0;
+        __syncthreads();
+        if (mine) sh.largest[int(threadIdx.x) / 64 * each + rank] = largest;
+        __syncthreads();
+        if (mine) {
+            rank = 0;
+#pragma unroll 4
+            for (int i = 0; i < kWaves * each; ++i) rank += sh.largest[i] > largest;
+            if (rank == top - 1) sh.limit = largest;
+        }
         __syncthreads();
         limit = sh.limit;
     }
@@ -171,15 +200,7 @@ __device__ __forceinline__ void offer(Top& sh, int top, Key key) {
     else
         for (int i = 0; i < top && sh.list[i] != 0; ++i) ++n;
     __syncthreads();
-    for (int i = int(threadIdx.x); i < top; i += kThreads)
-        if (i >= n) sh.list[i] = 0;
-    for (int i = int(threadIdx.x); i < n; i += kThreads) {
-        const uint64_t k = sh.found[i];
-        int rank = 0;
-        for (int j = 0; j < n; ++j) rank += sh.found[j] > k;
-        if (rank < top) sh.list[rank] = k;  // the order of arrival does not matter
-    }
-    __syncthreads();
+    list_found(sh, n, top);
 }
 
 // ------------------------------------------------------------------ forward
@@ -309,7 +330,16 @@ __global__ __launch_bounds__(kThreads) void logprob_join(RowOut o, Parts p) {
         __syncthreads();
         const uint64_t* keys = p.tops + r * p.per_row * o.top;
         const int n = p.per_row * o.top;
-        for (int base = 0; base < n; base += kThreads * kOffer)
+        if (n <= kThreads) {  // few enough to rank as they are
+            if (int(threadIdx.x) < n) {
+                const uint64_t key = keys[threadIdx.x];
+                // Parts shorter than the list leave zeros; made to differ, they come last.
+                st.found[threadIdx.x] = key != 0 ? key : uint64_t(threadIdx.x) + 1;
+            }
+            __syncthreads();
+            list_found(st, n, o.top);
+        }
+        for (int base = 0; n > kThreads && base < n; base += kThreads * kOffer)
             offer(st, o.top, [&](int i) {
                 const int at = base + i * kThreads + int(threadIdx.x);
                 return at < n ? keys[at] : 0;
