@@ -265,7 +265,8 @@ class Backend:
             raise RuntimeError(f"{what} failed ({rc}): {self.error()}")
 
     def stream(self):
-        return _vp(self.torch.cuda.current_stream().cuda_stream)
+        cuda = self.torch.cuda  # the handle alone: making a Stream object of it takes 2.7 us
+        return _vp(self.torch._C._cuda_getCurrentRawStream(cuda.current_device()))
 
     @staticmethod
     def p(t):
@@ -782,9 +783,11 @@ class Backend:
     def _rows(self, t, what, shape, dtype=None):
         """The row pitch of a float32 tensor of this shape whose rows are dense (a column
         range of a wider matrix may be passed), checked."""
-        if t.dtype != (dtype or self.torch.float32) or tuple(t.shape) != tuple(shape):
+        if t.dtype != (dtype or self.torch.float32) or t.shape != shape:
             raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)}, expected "
                              f"{dtype or self.torch.float32} {tuple(shape)}")
+        if t.is_contiguous() and t.shape[0] > 1:
+            return t.stride(0)
         row = 1
         for n, stride in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
             if n != 1 and stride != row:
@@ -797,7 +800,7 @@ class Backend:
         return t.stride(0)
 
     def _index(self, t, what, *shape):
-        if t.dtype != self.torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+        if t.dtype != self.torch.int32 or t.shape != shape or not t.is_contiguous():
             raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)}, expected contiguous int32 "
                              f"{shape}")
         return _vp(t.data_ptr())
@@ -827,9 +830,10 @@ class Backend:
             sequences, tq, tk, h, kv, d, d ** -0.5 if scale is None else scale, int(causal),
             out.data_ptr(), self._rows(out, "out", (tq, h, d)), self._dense(lse, "lse", (tq, h)))
 
-    def _dense(self, t, what, shape, dtype=None):
-        if self._rows(t, what, shape, dtype) and not t.is_contiguous():
-            raise ValueError(f"{what}: expected a contiguous tensor")
+    def _dense(self, t, what, shape):
+        if t.dtype != self.torch.float32 or t.shape != shape or not t.is_contiguous():
+            raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)}, expected contiguous float32 "
+                             f"{tuple(shape)}")
         return t.data_ptr()
 
     def attention_packed(self, q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None,

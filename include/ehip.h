@@ -898,8 +898,10 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  * q, out, grad, dq are rows of heads * head_dim floats, ld_* floats apart (the
  * queries of a fused projection are read and their gradient written in place);
  * k, v, dk, dv rows of kv_heads * head_dim; lse is (total_q, heads), dense.
- * Any alignment of a float. 1 <= head_dim <= 128; heads a multiple of
- * kv_heads; at most 2^24 - 1 blocks of 64 rows and a head (else EHIP_EINVAL).
+ * Any alignment of a float; ld_q, ld_k, ld_v and ld_grad at most 2^22.
+ * 1 <= head_dim <= 128; heads a multiple of kv_heads; at most 2^24 - 1 blocks
+ * of 128 rows and a head (else EHIP_EINVAL). Values keep 24 bits from 2^-110
+ * on, smaller ones what is above 2^-133.
  * Offsets out of range or descending are clamped, so nothing is read or
  * written outside the tensors, but what the sequences they touch get is
  * unspecified.
@@ -911,7 +913,8 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  *   dq_i = scale sum_j ds_ij k_j    dk_j = scale sum_i ds_ij q_i
  * dk and dv summed over the query heads of the group too. The outputs may not
  * overlap the inputs or each other. `workspace` (device memory, 16-byte
- * aligned) holds delta during the call: at least
+ * aligned) holds delta, and each query head's share of dk and dv where heads
+ * are grouped, during the call: at least
  * ehip_attention_packed_backward_workspace() bytes, of the call's own.
  * Deterministic: no atomics, the sums' order goes by the lengths and sizes. */
 typedef struct {
@@ -937,7 +940,8 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
 
 /* A cache of keys and values in pages, for producing one token at a time. The
  * pools hold `pages` pages of page_size positions of (kv_heads, head_dim)
- * values, dense, in fp32 or bf16; position p of sequence s is row p % page_size
+ * values, dense, in fp32 or bf16 (at most 2^31 - 1 positions in all); position
+ * p of sequence s is row p % page_size
  * of page table[s * ld_table + p / page_size], table a DEVICE array of
  * table_width int32 a sequence. Pages may be shared by sequences that only
  * read them. The caller allots pages and keeps the lengths. No counterpart in
@@ -974,9 +978,8 @@ int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_
  * a host value, is what the work is split by: the same lengths under another
  * `longest` may differ in the last bits.
  * 1 <= head_dim <= 128, heads a multiple of kv_heads. `workspace` (16-byte
- * aligned) holds the parts of a split length during the call: at least
- * ehip_attention_paged_workspace() bytes, of the call's own (NULL where that is
- * 0). Deterministic. */
+ * aligned) holds the parts of split lengths during the call: at least
+ * ehip_attention_paged_workspace() bytes, of the call's own. Deterministic. */
 int64_t ehip_attention_paged_workspace(const ehip_cache_t* cache, int64_t heads,
                                        int64_t longest);
 int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t ld_q,
