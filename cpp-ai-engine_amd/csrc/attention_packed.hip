@@ -277,8 +277,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     const int wave_end = 32 * wave < t.rows ? visible(a, t, t.first + last) : 0;
     const int wave_all = visible(a, t, t.first + 32 * wave);  // keys that all its queries see
 
-    // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q. Weights are 2^-24 of
-    // their value, so that sums over the values stay in their range.
+    // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q.
     const float c2 = fabsf(a.scale) * 1.44269504088896340736f;
     bf16x8 q[DP / 16][3];
     own_row<DP, VEC>(a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim, a.dim,
@@ -292,7 +291,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     floatx16 o[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) o[db] = zeros();
-    float top = -INFINITY, shift = 24.0f, sum = 0.0f;
+    float top = -INFINITY, shift = 0.0f, sum = 0.0f;
 
     const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
@@ -326,22 +325,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
         }
         if (j0 < wave_end) {
             floatx16 s[BN / 32];
-#pragma unroll
-            for (int b = 0; b < BN / 32; ++b) s[b] = zeros();
-            constexpr int NB = BN / 32, kScores = NB * (DP / 16);
-            bf16x8 f[2][3];
-            KeyTile::block(lds_k, 0, 0, f[0]);
-#pragma unroll
-            for (int n = 0; n < kScores; ++n) {
-                const int ks = n / NB;
-                if (kPark && n % NB == 0)
-                    q[ks][2] = *reinterpret_cast<const bf16x8*>(parked + 1024 * ks);
-                if (n + 1 < kScores)
-                    KeyTile::block(lds_k, (n + 1) % NB, (n + 1) / NB, f[(n + 1) & 1]);
-                keep_order();
-                multiply(s[n % NB], f[n & 1], q[ks]);
-                keep_order();
-            }
+            scores<KeyTile>(s, lds_k, q, [&](int ks) {
+                if (kPark) q[ks][2] = *reinterpret_cast<const bf16x8*>(parked + 1024 * ks);
+            });
             if (j0 + BN > wave_all) {
 #pragma unroll
                 for (int b = 0; b < BN / 32; ++b)
@@ -355,7 +341,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) m = fmaxf(m, s[b][r]);
             m = fmaxf(m, __shfl_xor(m, 32));
-            const float next = m == -INFINITY ? 24.0f : __builtin_fmaf(m, c2, 24.0f);
+            const float next = m == -INFINITY ? 0.0f : m * c2;
             const float keep = top == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(shift - next);
             top = m;
             shift = next;
@@ -373,25 +359,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
                 split8(w + 8, p[2 * b + 1]);
             }
             sum = __builtin_fmaf(sum, keep, part);
-            // The tile's sum apart from the running one: that is rounded to nearest once a tile,
-            // where the instruction drops low bits towards minus infinity.
-            constexpr int NU = BN / 16, kSums = NU * (DP / 32);
-            floatx16 x = zeros();
-            ValueTile::block(lds_v, 0, 0, f[0]);
+            // The tile's sum apart from the running one, which is rounded to nearest once a tile.
+            weighted<ValueTile, DP / 32, BN / 16>(
+                lds_v, 0, DP / 32, p, [&](int db, const floatx16& x) {
 #pragma unroll
-            for (int n = 0; n < kSums; ++n) {
-                if (n + 1 < kSums)
-                    ValueTile::block(lds_v, (n + 1) / NU, (n + 1) % NU, f[(n + 1) & 1]);
-                keep_order();
-                multiply(x, f[n & 1], p[n % NU]);
-                keep_order();
-                if (n % NU == NU - 1) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        o[n / NU][r] = __builtin_fmaf(o[n / NU][r], keep, x[r]);
-                    x = zeros();
-                }
-            }
+                    for (int r = 0; r < 16; ++r) o[db][r] = __builtin_fmaf(o[db][r], keep, x[r]);
+                });
         }
         if (BUFFERS == 1) __syncthreads();
         if (BUFFERS == 1 || wave >= WAVES / 2) {
@@ -498,36 +471,24 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
         bf16x8 w[BN / 16][3];
 #pragma unroll
         for (int b = 0; b < BN / 32; ++b) {
-            floatx16 s = zeros(), dp = zeros();
-#pragma unroll
-            for (int ks = 0; ks < DP / 16; ++ks) {
-                bf16x8 f[3];
-                KeyTile::block(lds, b, ks, f);
-                multiply(s, f, q[ks]);
-                KeyTile::block(lds_v, b, ks, f);
-                multiply(dp, f, g[ks]);
-            }
+            floatx16 s[1], dp[1];
+            scores<KeyTile>(s, lds, q, [](int) {});
+            scores<KeyTile>(dp, lds_v, g, [](int) {});
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c2, -shift)) * (dp[r] - delta);
+                ds[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[0][r], c2, -shift)) *
+                        (dp[0][r] - delta);
                 if (edge && j0 + 32 * b + row_of(r) >= limit) ds[r] = 0.0f;
             }
             split8(ds, w[2 * b]);
             split8(ds + 8, w[2 * b + 1]);
         }
+        weighted<KeyColumns, DP / 32, BN / 16>(lds_c, 0, DP / 32, w,
+                                               [&](int db, const floatx16& x) {
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) {
-            floatx16 x = zeros();
-#pragma unroll
-            for (int u = 0; u < BN / 16; ++u) {
-                bf16x8 f[3];
-                KeyColumns::block(lds_c, db, u, f);
-                multiply(x, f, w[u]);
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) dq[db][r] += x[r];
-        }
+                                                   for (int r = 0; r < 16; ++r) dq[db][r] += x[r];
+                                               });
     }
     bool fine = true;
 #pragma unroll
@@ -631,20 +592,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
         const bool active = j0 < wave_end;
         ct.load(k + int64_t(j0) * ld_k, ld_k, t.nk - j0, a.dim);
         floatx16 s[NB];
-        bf16x8 f[2][3];
         if (active) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b) s[b] = zeros();
-            constexpr int kScores = NB * (DP / 16);
-            KeyTile::block(scored, 0, 0, f[0]);
-#pragma unroll
-            for (int n = 0; n < kScores; ++n) {
-                if (n + 1 < kScores)
-                    KeyTile::block(scored, (n + 1) % NB, (n + 1) / NB, f[(n + 1) & 1]);
-                keep_order();
-                multiply(s[n % NB], f[n & 1], own[n / NB]);
-                keep_order();
-            }
+            scores<KeyTile>(s, scored, own, [](int) {});
             if (role == 0) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
@@ -690,23 +639,11 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
                 split8(ds + 8, w[2 * b + 1]);
             }
             const int mid = role * kHalf;  // the wave's first block of values
-            constexpr int kSums = NU * kHalf;
-            floatx16 x = zeros();
-            KeyColumns::block(lds_c, mid < kBlocks ? mid : 0, 0, f[0]);
+            weighted<KeyColumns, kHalf, NU>(lds_c, mid, min(kHalf, kBlocks - mid), w,
+                                            [&](int d, const floatx16& x) {
 #pragma unroll
-            for (int n = 0; n < kSums; ++n) {
-                if (mid + n / NU >= kBlocks) break;
-                if (n + 1 < kSums && mid + (n + 1) / NU < kBlocks)
-                    KeyColumns::block(lds_c, mid + (n + 1) / NU, (n + 1) % NU, f[(n + 1) & 1]);
-                keep_order();
-                multiply(x, f[n & 1], w[n % NU]);
-                keep_order();
-                if (n % NU == NU - 1) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) dq[n / NU][r] += x[r];
-                    x = zeros();
-                }
-            }
+                                                for (int r = 0; r < 16; ++r) dq[d][r] += x[r];
+                                            });
         }
         stage_rows(j0 + BN);
         __syncthreads();
@@ -816,20 +753,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
         gc.load(a.grad + at * a.ld_grad + int64_t(h) * a.dim, ld_g, left, a.dim);
         qc.load(a.q + at * a.ld_q + int64_t(h) * a.dim, ld_q, left, a.dim);
         floatx16 s[NB];
-        bf16x8 f[2][3];
         if (active) {
-#pragma unroll
-            for (int b = 0; b < NB; ++b) s[b] = zeros();
-            constexpr int kScores = NB * (DP / 16);
-            QueryTile::block(scored, 0, 0, f[0]);
-#pragma unroll
-            for (int u = 0; u < kScores; ++u) {
-                if (u + 1 < kScores)
-                    QueryTile::block(scored, (u + 1) % NB, (u + 1) / NB, f[(u + 1) & 1]);
-                keep_order();
-                multiply(s[u % NB], f[u & 1], own[u / NB]);
-                keep_order();
-            }
+            scores<QueryTile>(s, scored, own, [](int) {});
             const float* const stat_of = stats[n & 1][role] + 4 * half;
             if (role == 0) {
 #pragma unroll
@@ -897,22 +822,11 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
                 split8(y, w[2 * b]);
                 split8(y + 8, w[2 * b + 1]);
             }
-            constexpr int kSums = NU * kBlocks;
-            floatx16 x = zeros();
-            QueryColumns::block(summed, 0, 0, f[0]);
+            weighted<QueryColumns, kBlocks, NU>(summed, 0, kBlocks, w,
+                                                [&](int d, const floatx16& x) {
 #pragma unroll
-            for (int u = 0; u < kSums; ++u) {
-                if (u + 1 < kSums)
-                    QueryColumns::block(summed, (u + 1) / NU, (u + 1) % NU, f[(u + 1) & 1]);
-                keep_order();
-                multiply(x, f[u & 1], w[u % NU]);
-                keep_order();
-                if (u % NU == NU - 1) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) sum[u / NU][r] += x[r];
-                    x = zeros();
-                }
-            }
+                                                    for (int r = 0; r < 16; ++r) sum[d][r] += x[r];
+                                                });
         }
         stage_rows(n + 1);
         __syncthreads();

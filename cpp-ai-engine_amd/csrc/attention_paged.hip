@@ -370,17 +370,16 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
             float top = m[g];
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, w[g][u]);
-            // Weights of 2^-24 of their value: sums over the values stay in their range.
-            const float shift = top == -INFINITY ? 24.0f : top + 24.0f;
-            const float keep =
-                m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[g] + 24.0f - shift);
+            const float shift = top == -INFINITY ? 0.0f : top;
+            const float keep = m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[g] - shift);
             m[g] = top;
             l[g] *= keep;
 #pragma unroll
             for (int e = 0; e < N; ++e) o[g][e] *= keep;
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                w[g][u] = __builtin_amdgcn_exp2f(w[g][u] - shift);
+                // 2^-24 of the weight: sums over the values stay in their range.
+                w[g][u] = __builtin_amdgcn_exp2f(w[g][u] - shift) * 0x1p-24f;
                 l[g] += w[g][u];
             }
         }
@@ -630,13 +629,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
             for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float shift = top == -INFINITY ? 24.0f : top + 24.0f;
-        const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m + 24.0f - shift);
+        const float shift = top == -INFINITY ? 0.0f : top;
+        const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
         m = top;
         float w[8], part_sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j % 4] - shift);
+            w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j % 4] - shift) * 0x1p-24f;
             part_sum += w[j];
         }
         l = __builtin_fmaf(l, keep, part_sum);

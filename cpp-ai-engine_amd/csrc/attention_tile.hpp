@@ -49,11 +49,19 @@ __device__ __forceinline__ void split8(const float* x, bf16x8 (&part)[3]) {
 // Left alone the compiler reads them one or two instructions ahead. Other instructions may cross.
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x0216); }
 
-// d += the product of two blocks of 32 x 16.
-__device__ __forceinline__ void multiply(floatx16& d, const bf16x8 (&a)[3], const bf16x8 (&b)[3]) {
+// d += the five smaller part products of two blocks of 32 x 16, or the first parts' alone. The matrix
+// instruction drops the low bits of its sums towards minus infinity: of a chain of six products a
+// block each drops as much as the first parts' do, unless those come last, when the sum is still
+// small (scores of 64 values: 4 instructions at full size in place of 24; the outputs' error against
+// 64 bits, sequences of 64 to 1537, went down by a fifth, at no cost in time).
+__device__ __forceinline__ void multiply_small(floatx16& d, const bf16x8 (&a)[3],
+                                               const bf16x8 (&b)[3]) {
 #pragma unroll
-    for (int q = 0; q < 6; ++q)
+    for (int q = 0; q < 5; ++q)
         d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[kPart[q][0]], b[kPart[q][1]], d, 0, 0, 0);
+}
+__device__ __forceinline__ void multiply_first(floatx16& d, const bf16x8& a, const bf16x8& b) {
+    d = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, d, 0, 0, 0);
 }
 
 __device__ __forceinline__ floatx16 zeros() {
@@ -226,12 +234,11 @@ struct RowTile {
         if (left >= ROWS && dim == DP) store_as<true>(lds, left, dim);
         else store_as<false>(lds, left, dim);
     }
-    // Block (rb, ks) of the tile.
-    __device__ __forceinline__ static void block(const char* lds, int rb, int ks, bf16x8 (&a)[3]) {
+    // Part p of block (rb, ks) of the tile.
+    __device__ __forceinline__ static bf16x8 block(const char* lds, int rb, int ks, int p) {
         const int lane = int(threadIdx.x) & 63;
-        const char* at = lds + slot(32 * rb + (lane & 31), 2 * ks + lane / 32);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) a[p] = *reinterpret_cast<const bf16x8*>(at + p * kPlane);
+        return *reinterpret_cast<const bf16x8*>(
+            lds + slot(32 * rb + (lane & 31), 2 * ks + lane / 32) + p * kPlane);
     }
 };
 
@@ -311,13 +318,86 @@ struct ColTile {
         if (left >= ROWS && dim == DP) store_as<true>(lds, left, dim);
         else store_as<false>(lds, left, dim);
     }
-    __device__ __forceinline__ static void block(const char* lds, int db, int t, bf16x8 (&a)[3]) {
+    __device__ __forceinline__ static bf16x8 block(const char* lds, int db, int t, int p) {
         const int lane = int(threadIdx.x) & 63;
-        const char* at = lds + slot(32 * db + (lane & 31), 2 * t + lane / 32);
-#pragma unroll
-        for (int p = 0; p < 3; ++p) a[p] = *reinterpret_cast<const bf16x8*>(at + p * kPlane);
+        return *reinterpret_cast<const bf16x8*>(
+            lds + slot(32 * db + (lane & 31), 2 * t + lane / 32) + p * kPlane);
     }
 };
+
+// s[b] = rows 32 b .. of the tile times the lane's own row: NB x 32 scores. fetch(ks) is called before
+// own[ks] is used whole.
+template <class Tile, int NB, int KS, class Fetch>
+__device__ __forceinline__ void scores(floatx16 (&s)[NB], const char* lds, bf16x8 (&own)[KS][3],
+                                       Fetch fetch) {
+    constexpr int N = NB * KS;
+    bf16x8 f[2][3];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) s[b] = zeros();
+#pragma unroll
+    for (int p = 0; p < 3; ++p) f[0][p] = Tile::block(lds, 0, 0, p);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        if (n % NB == 0) fetch(n / NB);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            if (n + 1 < N) f[(n + 1) & 1][p] = Tile::block(lds, (n + 1) % NB, (n + 1) / NB, p);
+            else if (p < N) f[N & 1][p] = Tile::block(lds, p % NB, p / NB, 0);
+        }
+        keep_order();
+        multiply_small(s[n % NB], f[n & 1], own[n / NB]);
+        keep_order();
+    }
+    // The first parts once more, three blocks ahead.
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        const int at = 3 * (N & 1) + n, ahead = at + 3;
+        if (n + 3 < N)
+            f[ahead / 3 % 2][ahead % 3] = Tile::block(lds, (n + 3) % NB, (n + 3) / NB, 0);
+        keep_order();
+        multiply_first(s[n % NB], f[at / 3 % 2][at % 3], own[n / NB][0]);
+        keep_order();
+    }
+}
+
+// For blocks first .. first + count - 1 (at most DB) of values: add(block - first, the transposed
+// tile's block times the weights w of its rows, 16 NU of them).
+template <class Tile, int DB, int NU, class Add>
+__device__ __forceinline__ void weighted(const char* lds, int first, int count,
+                                         const bf16x8 (&w)[NU][3], Add add) {
+    bf16x8 h[NU], f[2][2];  // first parts, the others
+    const auto ask = [&](int n) {
+        const int db = n / NU, u = n % NU;
+        h[u] = Tile::block(lds, first + db, u, 0);
+#pragma unroll
+        for (int p = 1; p < 3; ++p) f[n & 1][p - 1] = Tile::block(lds, first + db, u, p);
+    };
+    if (count > 0) ask(0);
+#pragma unroll
+    for (int db = 0; db < DB; ++db) {
+        if (db >= count) break;
+        floatx16 x = zeros();
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int n = db * NU + u;
+            if (u + 1 < NU) ask(n + 1);
+            keep_order();
+            const bf16x8 a[3] = {h[u], f[n & 1][0], f[n & 1][1]};
+            multiply_small(x, a, w[u]);
+            keep_order();
+        }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            multiply_first(x, h[u], w[u][0]);
+            if (u == 0 && db + 1 < DB) {  // its h is free now
+                keep_order();
+                if (db + 1 < count) ask((db + 1) * NU);
+                keep_order();
+            }
+        }
+        add(db, x);
+    }
+}
 
 }  // namespace attention
 }  // namespace ehip
