@@ -256,8 +256,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     constexpr int BUFFERS = WAVES / 4;
     using namespace attention;
     using KeyTile = RowTile<BN, DP, 64 * WAVES, VEC>;
-    using ValueTile = ColTile<BN, DP, 64 * WAVES>;
-    constexpr int kTile = KeyTile::kBytes + ValueTile::kBytes;
+    constexpr int kTile = 2 * KeyTile::kBytes;
     // Wide heads leave the third parts of the queries, which one product in six takes, in LDS: all
     // of them in registers spill.
     constexpr bool kPark = DP > 64;
@@ -296,8 +295,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
     const int ld_k = int(a.ld_k), ld_v = int(a.ld_v);
-    KeyTile kt(ld_k, a.dim);
-    ValueTile vt(ld_v, a.dim);
+    KeyTile kt(ld_k, a.dim), vt(ld_v, a.dim);
     // The tile of keys from j on: into registers, and from there into its half of the LDS.
     const auto load = [&](int j) {
         if (j >= end) return;
@@ -360,7 +358,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
             }
             sum = __builtin_fmaf(sum, keep, part);
             // The tile's sum apart from the running one, which is rounded to nearest once a tile.
-            weighted<ValueTile, DP / 32, BN / 16>(
+            weighted<KeyTile, DP / 32, BN / 16>(
                 lds_v, 0, DP / 32, p, [&](int db, const floatx16& x) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r) o[db][r] = __builtin_fmaf(o[db][r], keep, x[r]);
@@ -413,10 +411,8 @@ template <int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     using namespace attention;
     using KeyTile = RowTile<BN, DP, kThreads, VEC>;
-    using KeyColumns = ColTile<BN, DP, kThreads>;
-    __shared__ __attribute__((aligned(16))) char lds[2 * KeyTile::kBytes + KeyColumns::kBytes];
+    __shared__ __attribute__((aligned(16))) char lds[2 * KeyTile::kBytes];
     char* const lds_v = lds + KeyTile::kBytes;
-    char* const lds_c = lds_v + KeyTile::kBytes;
     const int h = head_of(a, int(blockIdx.x % a.heads));
     const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kRows);
     if (t.rows == 0) return;
@@ -448,22 +444,18 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
     const int ld_k = int(a.ld_k), ld_v = int(a.ld_v);
     KeyTile kt(ld_k, a.dim), vt(ld_v, a.dim);
-    KeyColumns ct(ld_k, a.dim);
     if (end > 0) {
         kt.load(k, ld_k, t.nk, a.dim);
         vt.load(v, ld_v, t.nk, a.dim);
-        ct.load(k, ld_k, t.nk, a.dim);
     }
     for (int j0 = 0; j0 < end; j0 += BN) {
         __syncthreads();
         kt.store(lds, t.nk - j0, a.dim);
         vt.store(lds_v, t.nk - j0, a.dim);
-        ct.store(lds_c, t.nk - j0, a.dim);
         const int j1 = j0 + BN;
         if (j1 < end) {
             kt.load(k + int64_t(j1) * ld_k, ld_k, t.nk - j1, a.dim);
             vt.load(v + int64_t(j1) * ld_v, ld_v, t.nk - j1, a.dim);
-            ct.load(k + int64_t(j1) * ld_k, ld_k, t.nk - j1, a.dim);
         }
         __syncthreads();
         if (j0 >= wave_end) continue;
@@ -484,11 +476,10 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
             split8(ds, w[2 * b]);
             split8(ds + 8, w[2 * b + 1]);
         }
-        weighted<KeyColumns, DP / 32, BN / 16>(lds_c, 0, DP / 32, w,
-                                               [&](int db, const floatx16& x) {
+        weighted<KeyTile, DP / 32, BN / 16>(lds, 0, DP / 32, w, [&](int db, const floatx16& x) {
 #pragma unroll
-                                                   for (int r = 0; r < 16; ++r) dq[db][r] += x[r];
-                                               });
+            for (int r = 0; r < 16; ++r) dq[db][r] += x[r];
+        });
     }
     bool fine = true;
 #pragma unroll
@@ -514,8 +505,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
 // accumulates its share of the gradients. So a wave holds one own row and half of the results a
 // lane, which leaves room for two waves a SIMD at every head size: a lone wave issues a vector
 // instruction every eighth cycle only. A step is two phases with a barrier after each: the scores,
-// from the streamed rows, then the gradients, from their transposed tiles; the tiles of a phase are
-// replaced during the other one.
+// from the streamed rows, then the gradients, from the same rows read transposed.
 constexpr int kBackThreads = 512;
 
 // Gives the two waves of a group the rows either of them found without a finite result (a bit each).
@@ -532,13 +522,11 @@ template <int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed a) {
     using namespace attention;
     using KeyTile = RowTile<BN, DP, kBackThreads, VEC>;
-    using KeyColumns = ColTile<BN, DP, kBackThreads>;
     constexpr int NB = BN / 32, NU = BN / 16, kBlocks = DP / 32, kHalf = (kBlocks + 1) / 2;
     constexpr int kSwap = 4 * NB * 4096;  // one role's scores
     __shared__ __attribute__((aligned(16))) char
-        lds[2 * KeyTile::kBytes + KeyColumns::kBytes + 2 * kSwap];
-    char* const lds_c = lds + 2 * KeyTile::kBytes;
-    char* const lds_x = lds_c + KeyColumns::kBytes;
+        lds[4 * KeyTile::kBytes + 2 * kSwap];  // two tiles of both, by turns
+    char* const lds_x = lds + 4 * KeyTile::kBytes;
     const int h = head_of(a, int(blockIdx.x % a.heads));
     const Tile t = find_tile(a, false, int(blockIdx.x / a.heads), kRows);
     if (t.rows == 0) return;
@@ -571,7 +559,6 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
     const int ld_k = int(a.ld_k), ld_v = int(a.ld_v);
     KeyTile kt(ld_k, a.dim), vt(ld_v, a.dim);
-    KeyColumns ct(ld_k, a.dim);
     const auto load_rows = [&](int j) {
         if (j >= end) return;
         kt.load(k + int64_t(j) * ld_k, ld_k, t.nk - j, a.dim);
@@ -579,21 +566,26 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
     };
     const auto stage_rows = [&](int j) {
         if (j >= end) return;
-        kt.store(lds, t.nk - j, a.dim);
-        vt.store(lds + KeyTile::kBytes, t.nk - j, a.dim);
+        char* const at = lds + (j / BN & 1) * 2 * KeyTile::kBytes;
+        kt.store(at, t.nk - j, a.dim);
+        vt.store(at + KeyTile::kBytes, t.nk - j, a.dim);
     };
-    const char* const scored = lds + role * KeyTile::kBytes;
     char* const give = lds_x + role * kSwap + ((wave & 3) * NB * 256 + lane) * 16;
     const char* const take = lds_x + (1 - role) * kSwap + ((wave & 3) * NB * 256 + lane) * 16;
     load_rows(0);
     stage_rows(0);
+    load_rows(BN);
     __syncthreads();
     for (int j0 = 0; j0 < end; j0 += BN) {
         const bool active = j0 < wave_end;
-        ct.load(k + int64_t(j0) * ld_k, ld_k, t.nk - j0, a.dim);
+        const char* const tile = lds + (j0 / BN & 1) * 2 * KeyTile::kBytes;
+        if (role == 1) {  // the next tile: one wave of a SIMD before its products, the other after
+            stage_rows(j0 + BN);
+            load_rows(j0 + 2 * BN);
+        }
         floatx16 s[NB];
         if (active) {
-            scores<KeyTile>(s, scored, own, [](int) {});
+            scores<KeyTile>(s, tile + role * KeyTile::kBytes, own, [](int) {});
             if (role == 0) {
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
@@ -620,9 +612,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
                     *reinterpret_cast<floatx4u*>(give + (4 * b + r / 4) * 1024) =
                         floatx4u{s[b][r], s[b][r + 1], s[b][r + 2], s[b][r + 3]};
         }
-        ct.store(lds_c, t.nk - j0, a.dim);
         __syncthreads();
-        load_rows(j0 + BN);
         if (active) {
             bf16x8 w[NU][3];
 #pragma unroll
@@ -639,13 +629,16 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
                 split8(ds + 8, w[2 * b + 1]);
             }
             const int mid = role * kHalf;  // the wave's first block of values
-            weighted<KeyColumns, kHalf, NU>(lds_c, mid, min(kHalf, kBlocks - mid), w,
-                                            [&](int d, const floatx16& x) {
+            weighted<KeyTile, kHalf, NU>(tile, mid, min(kHalf, kBlocks - mid), w,
+                                         [&](int d, const floatx16& x) {
 #pragma unroll
-                                                for (int r = 0; r < 16; ++r) dq[d][r] += x[r];
-                                            });
+                                             for (int r = 0; r < 16; ++r) dq[d][r] += x[r];
+                                         });
         }
-        stage_rows(j0 + BN);
+        if (role == 0) {
+            stage_rows(j0 + BN);
+            load_rows(j0 + 2 * BN);
+        }
         __syncthreads();
     }
     bool fine = true;
@@ -677,14 +670,11 @@ template <int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) {
     using namespace attention;
     using QueryTile = RowTile<BN, DP, kBackThreads, VEC>;
-    using QueryColumns = ColTile<BN, DP, kBackThreads>;
     constexpr int NB = BN / 32, NU = BN / 16, kBlocks = DP / 32;
     constexpr int kSwap = 4 * NB * 4096;
-    __shared__ __attribute__((aligned(16))) char lds[2 * QueryTile::kBytes +
-                                                     2 * QueryColumns::kBytes + kSwap];
-    __shared__ __attribute__((aligned(16))) float stats[2][2][BN];  // of alternate tiles
-    char* const lds_c = lds + 2 * QueryTile::kBytes;
-    char* const lds_x = lds_c + 2 * QueryColumns::kBytes;
+    __shared__ __attribute__((aligned(16))) char lds[4 * QueryTile::kBytes + kSwap];
+    __shared__ __attribute__((aligned(16))) float stats[2][2][BN];  // as the tiles, by turns
+    char* const lds_x = lds + 4 * QueryTile::kBytes;
     const int group = a.heads / a.kv_heads, parts = a.part_k != nullptr ? group : 1;
     const int x = int(blockIdx.x % (a.kv_heads * parts)), c = x % a.kv_heads;
     const Tile t = find_tile(a, true, int(blockIdx.x / (a.kv_heads * parts)), kRows);
@@ -717,7 +707,6 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     const int steps = start < t.nq ? (t.nq - start + BN - 1) / BN : 0;
     const int count = steps * heads;
     QueryTile qt(ld_q, a.dim), gt(ld_g, a.dim);
-    QueryColumns qc(ld_q, a.dim), gc(ld_g, a.dim);
     float stat = 0.0f;  // a query's lse (threads 0 .. BN - 1) or delta (the next BN)
     // Tile n: head h0 + n / steps, its queries from start + n % steps * BN on.
     const auto load_rows = [&](int n) {
@@ -734,27 +723,29 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     const auto stage_rows = [&](int n) {
         if (n >= count) return;
         const int left = t.nq - (start + n % steps * BN);
-        qt.store(lds, left, a.dim);
-        gt.store(lds + QueryTile::kBytes, left, a.dim);
+        char* const at = lds + (n & 1) * 2 * QueryTile::kBytes;
+        qt.store(at, left, a.dim);
+        gt.store(at + QueryTile::kBytes, left, a.dim);
         if (threadIdx.x < BN) stats[n & 1][0][threadIdx.x] = stat * 1.44269504088896340736f;
         else if (threadIdx.x < 2 * BN) stats[n & 1][1][threadIdx.x - BN] = stat;
     };
-    const char* const scored = lds + role * QueryTile::kBytes;
-    const char* const summed = lds_c + role * QueryColumns::kBytes;
     char* const swap = lds_x + ((wave & 3) * NB * 256 + lane) * 16;
     const int half = lane / 32;
     load_rows(0);
     stage_rows(0);
+    load_rows(1);
     __syncthreads();
     for (int n = 0; n < count; ++n) {
-        const int h = h0 + n / steps, i0 = start + n % steps * BN, left = t.nq - i0;
-        const int64_t at = t.q0 + i0;
+        const int i0 = start + n % steps * BN, left = t.nq - i0;
         const bool active = i0 + BN > wave_start;
-        gc.load(a.grad + at * a.ld_grad + int64_t(h) * a.dim, ld_g, left, a.dim);
-        qc.load(a.q + at * a.ld_q + int64_t(h) * a.dim, ld_q, left, a.dim);
+        const char* const tile = lds + (n & 1) * 2 * QueryTile::kBytes;
+        if (role == 1) {  // the next tile: one wave of a SIMD before its products, the other after
+            stage_rows(n + 1);
+            load_rows(n + 2);
+        }
         floatx16 s[NB];
         if (active) {
-            scores<QueryTile>(s, scored, own, [](int) {});
+            scores<QueryTile>(s, tile + role * QueryTile::kBytes, own, [](int) {});
             const float* const stat_of = stats[n & 1][role] + 4 * half;
             if (role == 0) {
 #pragma unroll
@@ -797,10 +788,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
                             floatx4u{s[b][r], s[b][r + 1], s[b][r + 2], s[b][r + 3]};
             }
         }
-        gc.store(lds_c, left, a.dim);
-        qc.store(lds_c + QueryColumns::kBytes, left, a.dim);
         __syncthreads();
-        load_rows(n + 1);
         if (active) {
             if (role != 0) {
 #pragma unroll
@@ -822,13 +810,17 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
                 split8(y, w[2 * b]);
                 split8(y + 8, w[2 * b + 1]);
             }
-            weighted<QueryColumns, kBlocks, NU>(summed, 0, kBlocks, w,
-                                                [&](int d, const floatx16& x) {
+            // dv from the gradient's rows, dk from the queries'.
+            weighted<QueryTile, kBlocks, NU>(tile + (1 - role) * QueryTile::kBytes, 0, kBlocks, w,
+                                             [&](int d, const floatx16& x) {
 #pragma unroll
-                                                    for (int r = 0; r < 16; ++r) sum[d][r] += x[r];
-                                                });
+                                                 for (int r = 0; r < 16; ++r) sum[d][r] += x[r];
+                                             });
         }
-        stage_rows(n + 1);
+        if (role == 0) {
+            stage_rows(n + 1);
+            load_rows(n + 2);
+        }
         __syncthreads();
     }
     const float factor = role == 0 ? 1.0f : a.scale;

@@ -6,7 +6,7 @@
 // 0..7, l % 32) and D(8 (r / 4) + 4 (l / 32) + r % 4, l % 32) in register r. A wave's own rows are
 // the columns of every product, so a lane has one of them throughout: row sums are sums over the
 // lane's registers and its partner's (l ^ 32), and a product's D is the next one's B as it stands,
-// but for the order of its 16 rows, which the next one's A follows (ColTile).
+// but for the order of its 16 rows, which the next one's A follows (RowTile::columns).
 #ifndef EHIP_ATTENTION_TILE_HPP
 #define EHIP_ATTENTION_TILE_HPP
 
@@ -234,94 +234,28 @@ struct RowTile {
         if (left >= ROWS && dim == DP) store_as<true>(lds, left, dim);
         else store_as<false>(lds, left, dim);
     }
+    // Part p of the transposed block (db, t): values 32 db .. of rows 16 t .., as the A operand of
+    // products over the rows, the rows in the order that registers 8 (t % 2) .. of a D hold them: half
+    // h of the lanes has rows 16 t + 4 h + {0..3, 8..11}. A transposed read gives sixteen lanes one
+    // value each of four rows from the sixteen places of four values that they name.
+    __device__ __forceinline__ static bf16x8 columns(const char* lds, int db, int t, int p) {
+        typedef short shortx4 __attribute__((ext_vector_type(4)));
+        typedef __attribute__((address_space(3))) shortx4* Rows;
+        const int lane = int(threadIdx.x) & 63, i = lane & 15;
+        const int r = 16 * t + 4 * (lane / 32) + i / 4;
+        const int g = 4 * db + 2 * (lane / 16 % 2) + i % 4 / 2;
+        const char* at = lds + p * kPlane + slot(r, g) + 8 * (i & 1);
+        struct {
+            shortx4 x, y;
+        } f = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)at),
+               __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(at + 128))};  // 8 rows on
+        return __builtin_bit_cast(bf16x8, f);
+    }
     // Part p of block (rb, ks) of the tile.
     __device__ __forceinline__ static bf16x8 block(const char* lds, int rb, int ks, int p) {
         const int lane = int(threadIdx.x) & 63;
         return *reinterpret_cast<const bf16x8*>(
             lds + slot(32 * rb + (lane & 31), 2 * ks + lane / 32) + p * kPlane);
-    }
-};
-
-// ROWS streamed rows as the A operand, transposed, of products over the rows: block (db, t) holds
-// values 32 db .. of rows 16 t .., the rows in the order that registers 8 (t % 2) .. of a D hold
-// them: half block h has rows 16 t + 4 h + {0..3, 8..11}. A thread stages up to kUnits units of one
-// value of the eight rows of a half block; a wave reads runs of a row.
-template <int ROWS, int DP, int THREADS>
-struct ColTile {
-    static constexpr int kUnits = (ROWS * (DP / 8) + THREADS - 1) / THREADS;
-    static constexpr int kPlane = ROWS * DP * 2;
-    static constexpr int kBytes = 3 * kPlane;
-    static_assert(ROWS % 32 == 0 && DP % 32 == 0, "tile shape");
-
-    float v[kUnits][8];
-    uint32_t o[kUnits];  // byte offsets of the units' first rows
-
-    __device__ __forceinline__ static int value(int u) {
-        return (int(threadIdx.x) + u * THREADS) % DP;
-    }
-    __device__ __forceinline__ static int octet(int u) {
-        return (int(threadIdx.x) + u * THREADS) / DP;
-    }
-    // Row j (of 8) of octet o.
-    __device__ __forceinline__ static int row(int o, int j) {
-        return 16 * (o / 2) + 4 * (o % 2) + (j < 4 ? j : j + 4);
-    }
-    __device__ __forceinline__ static int slot(int d, int o) {
-        return ((d / 32) * (ROWS / 16) + o / 2) * 1024 + (o % 2) * 512 + ((d & 31) << 4);
-    }
-    __device__ __forceinline__ ColTile(int ld, int dim) {
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int d = value(u) < dim ? value(u) : 0;
-            o[u] = 4u * uint32_t(row(octet(u) < ROWS / 8 ? octet(u) : 0, 0) * ld + d);
-        }
-    }
-    __device__ __forceinline__ void load(const float* base, int ld, int left, int dim) {
-        const auto at = (global_bytes)base;
-        if (left >= ROWS) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const global_bytes row_j = at + 4 * int64_t(row(0, j)) * ld;
-#pragma unroll
-                for (int u = 0; u < kUnits; ++u) v[u][j] = global_load<float>(row_j + o[u]);
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < kUnits; ++u) {
-                const int d = value(u) < dim ? value(u) : 0;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int r = row(octet(u), j);
-                    v[u][j] =
-                        global_load<float>(at + 4u * uint32_t((r < left ? r : left - 1) * ld + d));
-                }
-            }
-        }
-    }
-    template <bool CLEAN>
-    __device__ __forceinline__ void store_as(char* lds, int left, int dim) const {
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            if ((u + 1) * THREADS > ROWS * (DP / 8) && octet(u) >= ROWS / 8) continue;  // no unit
-            float x[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                x[j] = CLEAN || (row(octet(u), j) < left && value(u) < dim) ? v[u][j] : 0.0f;
-            bf16x8 part[3];
-            split8(x, part);
-#pragma unroll
-            for (int p = 0; p < 3; ++p)
-                *reinterpret_cast<bf16x8*>(lds + p * kPlane + slot(value(u), octet(u))) = part[p];
-        }
-    }
-    __device__ __forceinline__ void store(char* lds, int left, int dim) const {
-        if (left >= ROWS && dim == DP) store_as<true>(lds, left, dim);
-        else store_as<false>(lds, left, dim);
-    }
-    __device__ __forceinline__ static bf16x8 block(const char* lds, int db, int t, int p) {
-        const int lane = int(threadIdx.x) & 63;
-        return *reinterpret_cast<const bf16x8*>(
-            lds + slot(32 * db + (lane & 31), 2 * t + lane / 32) + p * kPlane);
     }
 };
 
@@ -360,17 +294,17 @@ __device__ __forceinline__ void scores(floatx16 (&s)[NB], const char* lds, bf16x
     }
 }
 
-// For blocks first .. first + count - 1 (at most DB) of values: add(block - first, the transposed
-// tile's block times the weights w of its rows, 16 NU of them).
+// For blocks first .. first + count - 1 (at most DB) of values: add(block - first, the tile's
+// transposed block times the weights w of its rows, 16 NU of them).
 template <class Tile, int DB, int NU, class Add>
 __device__ __forceinline__ void weighted(const char* lds, int first, int count,
                                          const bf16x8 (&w)[NU][3], Add add) {
     bf16x8 h[NU], f[2][2];  // first parts, the others
     const auto ask = [&](int n) {
         const int db = n / NU, u = n % NU;
-        h[u] = Tile::block(lds, first + db, u, 0);
+        h[u] = Tile::columns(lds, first + db, u, 0);
 #pragma unroll
-        for (int p = 1; p < 3; ++p) f[n & 1][p - 1] = Tile::block(lds, first + db, u, p);
+        for (int p = 1; p < 3; ++p) f[n & 1][p - 1] = Tile::columns(lds, first + db, u, p);
     };
     if (count > 0) ask(0);
 #pragma unroll
