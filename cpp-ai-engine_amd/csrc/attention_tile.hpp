@@ -155,8 +155,10 @@ __device__ __forceinline__ void store_own(float* row, int dim, int db, const flo
 // ROWS streamed rows as the A operand of products over the head's values: LDS in three planes, each
 // in blocks of 32 rows x 16 values as the instruction takes them, 1 KiB, 16 bytes a lane: a
 // conflict-free ds_read_b128. The row's place within its half block is permuted by its group of
-// eight values, so that the writes of a row's groups, which neighbouring threads hold, fall on
-// different banks too. A thread stages up to kUnits units of one row by 8 values.
+// eight values, so that a transposed read's eight rows of two groups fall on all banks, twice, and the
+// writes of a row's groups, which neighbouring threads hold, on no bank more than twice either; few
+// address bits depend on the lane and the block both, so few addresses are kept. A thread stages up
+// to kUnits units of one row by 8 values.
 template <int ROWS, int DP, int THREADS, bool VEC>
 struct RowTile {
     static constexpr int kGroups = DP / 8;
@@ -175,7 +177,9 @@ struct RowTile {
         return (int(threadIdx.x) + u * THREADS) % kGroups;
     }
     __device__ __forceinline__ static int slot(int r, int g) {
-        return ((r / 32) * (DP / 16) + g / 2) * 1024 + (g & 1) * 512 + (((r & 31) ^ (g & 7)) << 4);
+        const int place = (r & 7) | (r >> 4 & 1) << 3 | (r >> 3 & 1) << 4;
+        return ((r / 32) * (DP / 16) + g / 2) * 1024 + (g & 1) * 512 +
+               ((place ^ (g & 3) ^ (g & 1) << 3) << 4);
     }
     // Rows are ld floats apart, at most kMaxLd: offsets within a tile are below 2^31.
     __device__ __forceinline__ RowTile(int ld, int dim) {
@@ -248,7 +252,7 @@ struct RowTile {
         struct {
             shortx4 x, y;
         } f = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)at),
-               __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(at + 128))};  // 8 rows on
+               __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(at + 256))};  // 8 rows on
         return __builtin_bit_cast(bf16x8, f);
     }
     // Part p of block (rb, ks) of the tile.
