@@ -114,29 +114,27 @@ __device__ __forceinline__ Tile find_tile_by_work(const Packed& a, bool keys, in
         const int begin = offset_at(cu, lane, total), end = offset_at(cu, lane + 1, total);
         tiles = end > begin ? (end - begin + size - 1) / size : 0;
     }
-    const auto count = [&](int w) {
-        int c = 0;
-        for (int s = 0; s < a.sequences; ++s) {
-            const int more = __builtin_amdgcn_readlane(tiles, s) - w + 1;
-            c += more > 0 ? more : 0;
-        }
-        return c;
-    };
-    int w = 1, n = total / size + 1;  // the answer, if any, is in [w, w + n)
-    while (true) {
+    int n = tiles;  // the answer, if any, is in [w, w + n)
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) n = max(n, __shfl_xor(n, o));
+    n = __builtin_amdgcn_readfirstlane(n);
+    int w = 1, above = 0;  // above: C(w + 1)
+    while (n > 0) {
         const int step = (n + 63) / 64;
-        const bool at = lane * step < n && count(w + lane * step) > slot;
-        const int c = __popcll(__ballot(at));
-        if (c == 0) return Tile{};
-        w += (c - 1) * step;
-        n -= (c - 1) * step;
-        n = n < step ? n : step;
+        const int mine = w + lane * step - 1;
+        int c = 0;
+        for (int s = 0; s < a.sequences; ++s)
+            c += max(0, __builtin_amdgcn_readlane(tiles, s) - mine);
+        const int last = __popcll(__ballot(lane * step < n && c > slot)) - 1;
+        if (last < 0) return Tile{};
+        if (last < 63) above = __builtin_amdgcn_readlane(c, last + 1);
+        w += last * step;
+        n = min(n - last * step, step);
         if (step == 1) break;
     }
-    w = __builtin_amdgcn_readfirstlane(w);
     uint64_t with = __ballot(tiles >= w);
-    for (int skip = slot - count(w + 1); skip > 0; --skip) with &= with - 1;
-    if (with == 0) return Tile{};
+    for (int skip = slot - above; skip > 0; --skip) with &= with - 1;
+    if (n == 0 || with == 0) return Tile{};
     const int s = __builtin_amdgcn_readfirstlane(__builtin_ctzll(with));
     return tile_of(a, keys, s, keys ? __builtin_amdgcn_readlane(tiles, s) - w : w - 1, size);
 }
@@ -993,10 +991,15 @@ int launch_forward(const Packed& a, hipStream_t s) {
 
 template <int DP, int BN, bool VEC>
 int forward_of(const Packed& a, hipStream_t s) {
-    // 256 queries a block, whose keys are converted once for all of them, for long sequences; 128 for
-    // batches of shorter ones, whose few blocks differ more in length (16384 queries: 2.82 ms
-    // against 3.90; 24 sequences of 64 to 1537: 260 us against 227; 16 of 512: 81 us either way).
-    const bool four = a.total_q < 1024 * int64_t(a.sequences);
+    // 256 queries a block convert their keys once and read them by turns of two tiles, 128 end with
+    // less between the last block and the others. Up to 96 values 128 it is, but for long sequences
+    // that fill the card twice over (64 values: 24 sequences of 64 to 1291, 16 heads, 147 us against
+    // 169; one of 4096, 8 heads, 211 : 274; 4 of 2048, 16 heads, 207 : 200); wider heads spill there,
+    // and take 256 unless most sequences are shorter (128 values: 335 : 303, 593 : 509, 525 : 398,
+    // and 64 sequences of 128 87 : 103).
+    const int64_t n = a.total_q, s_count = a.sequences;
+    const bool four = DP > 96 ? n < 256 * s_count
+                              : n < 2048 * s_count || n / 256 * a.heads < 512;
     return four ? launch_forward<DP, BN, 4, VEC>(a, s) : launch_forward<DP, BN, 8, VEC>(a, s);
 }
 
@@ -1050,7 +1053,7 @@ int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* stream)
     Packed a;
     if (int rc = fill("attention_packed", desc, a)) return rc;
     if (a.sequences == 0 || a.total_q == 0) return EHIP_OK;
-    const bool vec = a.dim % 8 == 0;
+    const bool vec = a.dim % 4 == 0;
     if (a.dim <= 32) return vec ? forward_of<32, 64, true>(a, as_stream(stream))
                                 : forward_of<32, 64, false>(a, as_stream(stream));
     if (a.dim <= 64) return vec ? forward_of<64, 64, true>(a, as_stream(stream))
@@ -1101,7 +1104,7 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
         a.part_v = a.part_k + part_bytes(a) / sizeof(float);
     }
     hipStream_t s = as_stream(stream);
-    const bool vec = a.dim % 8 == 0;
+    const bool vec = a.dim % 4 == 0;
     if (a.dim <= 32) return vec ? launch_backward<32, 64, true>(a, s) : launch_backward<32, 64, false>(a, s);
     if (a.dim <= 64) return vec ? launch_backward<64, 64, true>(a, s) : launch_backward<64, 64, false>(a, s);
     if (a.dim <= 96) return vec ? launch_backward<96, 32, true>(a, s) : launch_backward<96, 32, false>(a, s);

@@ -77,7 +77,7 @@ __device__ __forceinline__ int row_of(int r) {
 }
 
 // The lane's own row (a pointer to its `dim` values) as the B operand of products over the head's
-// values: DP / 16 blocks. VEC: dim is a multiple of 8.
+// values: DP / 16 blocks. VEC: dim is a multiple of 4.
 template <int DP, bool VEC>
 __device__ __forceinline__ void own_row(const float* row, int dim, float factor,
                                         bf16x8 (&b)[DP / 16][3]) {
@@ -87,14 +87,12 @@ __device__ __forceinline__ void own_row(const float* row, int dim, float factor,
         const int d0 = 16 * ks + 8 * half;
         float x[8];
         if (VEC) {
-            const bool in = d0 < dim;
-            const float* p = row + (in ? d0 : 0);
-            const floatx4u u = *reinterpret_cast<const floatx4u*>(p);
-            const floatx4u v = *reinterpret_cast<const floatx4u*>(p + 4);
+            const floatx4u u = *reinterpret_cast<const floatx4u*>(row + (d0 < dim ? d0 : 0));
+            const floatx4u v = *reinterpret_cast<const floatx4u*>(row + (d0 + 4 < dim ? d0 + 4 : 0));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                x[j] = in ? u[j] * factor : 0.0f;
-                x[4 + j] = in ? v[j] * factor : 0.0f;
+                x[j] = d0 < dim ? u[j] * factor : 0.0f;
+                x[4 + j] = d0 + 4 < dim ? v[j] * factor : 0.0f;
             }
         } else {
 #pragma unroll
@@ -118,9 +116,9 @@ __device__ __forceinline__ float own_dot(const float* x, const float* y, int dim
     for (int ks = 0; ks < DP / 16; ++ks) {
         const int d0 = 16 * ks + 8 * half;
         if (VEC) {
-            if (d0 >= dim) continue;
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {
+                if (d0 + j >= dim) continue;
                 const floatx4u u = *reinterpret_cast<const floatx4u*>(x + d0 + j);
                 const floatx4u v = *reinterpret_cast<const floatx4u*>(y + d0 + j);
 #pragma unroll
@@ -201,7 +199,8 @@ struct RowTile {
                     from = 4u * uint32_t(r * ld + (d < dim ? d : 0));
                 }
                 const floatx4u x = global_load<floatx4u>(at + from);
-                const floatx4u y = global_load<floatx4u>(at + from + 16);
+                const floatx4u y =
+                    global_load<floatx4u>(at + from + (8 * group(u) + 4 < dim ? 16 : 0));
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     v[u][j] = x[j];
@@ -226,7 +225,7 @@ struct RowTile {
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                x[j] = CLEAN || (in && 8 * group(u) + (VEC ? 0 : j) < dim) ? v[u][j] : 0.0f;
+                x[j] = CLEAN || (in && 8 * group(u) + (VEC ? j & 4 : j) < dim) ? v[u][j] : 0.0f;
             bf16x8 part[3];
             split8(x, part);
 #pragma unroll
