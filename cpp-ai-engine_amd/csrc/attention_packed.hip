@@ -991,15 +991,17 @@ int launch_forward(const Packed& a, hipStream_t s) {
 
 template <int DP, int BN, bool VEC>
 int forward_of(const Packed& a, hipStream_t s) {
-    // 256 queries a block convert their keys once and read them by turns of two tiles, 128 end with
-    // less between the last block and the others. Up to 96 values 128 it is, but for long sequences
-    // that fill the card twice over (64 values: 24 sequences of 64 to 1291, 16 heads, 147 us against
-    // 169; one of 4096, 8 heads, 211 : 274; 4 of 2048, 16 heads, 207 : 200); wider heads spill there,
-    // and take 256 unless most sequences are shorter (128 values: 335 : 303, 593 : 509, 525 : 398,
-    // and 64 sequences of 128 87 : 103).
-    const int64_t n = a.total_q, s_count = a.sequences;
-    const bool four = DP > 96 ? n < 256 * s_count
-                              : n < 2048 * s_count || n / 256 * a.heads < 512;
+    // 256 queries a block convert their keys once and read them by turns of two tiles; 128 leave less
+    // between the last block and the others. Without the causal mask all blocks of a sequence are
+    // alike, and 256 it is once they fill the card (us, 128 : 256 queries, heads of 64 values: one of
+    // 4096, 16 heads, 341 : 326, with 8 heads 216 : 275). With it, long sequences that fill the card
+    // twice over (4 of 2048, 16 heads, 207 : 200; 24 of 64 to 1291 147 : 169; one of 8192, 8 heads,
+    // 490 : 566). Heads over 96 values spill with 128, and take them for short causal ones alone
+    // (64 of 128 87 : 103; one of 4096 593 : 509; without the mask 64 of 128 136 : 82).
+    const int64_t n = a.total_q, s_count = a.sequences, blocks = n / 256 * a.heads;
+    const bool four = DP > 96   ? a.causal && n < 256 * s_count
+                      : a.causal ? n < 2048 * s_count || blocks < 512
+                                 : blocks < 256;
     return four ? launch_forward<DP, BN, 4, VEC>(a, s) : launch_forward<DP, BN, 8, VEC>(a, s);
 }
 
