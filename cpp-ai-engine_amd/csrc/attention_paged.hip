@@ -789,11 +789,15 @@ int check(const char* name, const ehip_cache_t* c, Cache& out) {
     return EHIP_OK;
 }
 
+// Positions count on past a length by less than that again in 32 bits; pages may repeat in a table, so
+// the pool's extent does not bound a length.
+constexpr int64_t kMaxLength = int64_t(1) << 30;
+
 int check_heads(const char* name, const Cache& c, int64_t heads, int64_t longest) {
     if (c.dim > kMaxDim || heads < 1 || heads % c.kv_heads != 0 || longest < 0)
         return fail(EHIP_EINVAL, "%s: %lld heads over %lld of %lld values, length %lld", name,
                     (long long)heads, (long long)c.kv_heads, (long long)c.dim, (long long)longest);
-    if (heads > kMaxBlocks || c.sequences * heads > kMaxBlocks || longest > INT32_MAX ||
+    if (heads > kMaxBlocks || c.sequences * heads > kMaxBlocks || longest > kMaxLength ||
         c.sequences * ceil_div(longest, kTile) > INT32_MAX)
         return fail(EHIP_EINVAL, "%s: %lld sequences of %lld heads of length %lld are too many",
                     name, (long long)c.sequences, (long long)heads, (long long)longest);

@@ -941,11 +941,11 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
 /* A cache of keys and values in pages, for producing one token at a time. The
  * pools hold `pages` pages of page_size positions of (kv_heads, head_dim)
  * values, dense, in fp32 or bf16 (at most 2^31 - 1 positions in all); position
- * p of sequence s is row p % page_size
- * of page table[s * ld_table + p / page_size], table a DEVICE array of
- * table_width int32 a sequence. Pages may be shared by sequences that only
- * read them. The caller allots pages and keeps the lengths. No counterpart in
- * the reference. */
+ * p of sequence s is row p % page_size of page
+ * table[s * ld_table + p / page_size], table a DEVICE array of table_width
+ * int32 a sequence. Pages may be shared by sequences that only read them. The
+ * caller allots pages and keeps the lengths. No counterpart in the
+ * reference. */
 enum { EHIP_CACHE_F32 = 0, EHIP_CACHE_BF16 = 1 };
 
 typedef struct {
@@ -975,8 +975,8 @@ int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_
  * ehip_attention_packed_f32. A length of zero gives out = 0, lse = -inf. A
  * negative length, one past `longest` or its table row, or a page outside the
  * pool makes the sequence's row NaN instead of a read out of bounds. `longest`,
- * a host value, is what the work is split by: the same lengths under another
- * `longest` may differ in the last bits.
+ * a host value of at most 2^30, is what the work is split by: the same lengths
+ * under another `longest` may differ in the last bits.
  * 1 <= head_dim <= 128, heads a multiple of kv_heads. `workspace` (16-byte
  * aligned) holds the parts of split lengths during the call: at least
  * ehip_attention_paged_workspace() bytes, of the call's own. Deterministic. */

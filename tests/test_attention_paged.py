@@ -430,6 +430,13 @@ def test_refused_caches_and_sizes():
         assert size(C.byref(cache()), heads, longest) == -1, (heads, longest)
 
 
+def test_lengths_end_where_positions_leave_their_range():
+    """2^30: positions are counted on past a length in 32 bits."""
+    size = E.load_library().ehip_attention_paged_workspace
+    assert size(C.byref(cache()), 4, 2 ** 30) >= 0
+    assert size(C.byref(cache()), 4, 2 ** 30 + 1) == -1
+
+
 @gpu
 def test_calls_are_refused(hip):
     import torch
