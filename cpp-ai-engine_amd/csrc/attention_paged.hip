@@ -33,8 +33,10 @@ __device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p
     return page * c.page_size + (p - int64_t(at) * c.page_size);
 }
 
-// log of a sum whose terms are 2^-24 of their value relative to 2^top; ln 2 in two parts.
+// log of a sum whose terms are 2^-24 of their value relative to 2^top; ln 2 in two parts, whose
+// products with an infinity would cancel to NaN.
 __device__ __forceinline__ float lse_of(float top, float sum) {
+    if (top == -INFINITY && sum == 0.0f) return -INFINITY;
     return __builtin_fmaf(top, 0.693147182464599609375f,
                           __builtin_fmaf(top, -1.904654323148236017e-9f, logf(sum * 0x1p24f)));
 }
@@ -179,11 +181,11 @@ __device__ __forceinline__ Segment first_segment(const Paged& a, int w) {
         const int s = base + lane;
         const int mine = s < sequences ? tiles_of(length_of(a, s)) : 0;
         const int upto = wave_scan(mine);
-        if (blockIdx.x == 0 && threadIdx.x < 64 && a.first != nullptr && s < sequences)
+        if (blockIdx.x == 0 && threadIdx.x < 64 && s < sequences)
             a.first[s] = tiles + upto - mine;
         tiles += __shfl(upto, 63);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0 && a.first != nullptr) a.first[sequences] = tiles;
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.first[sequences] = tiles;
     Segment g{};
     g.t = first_tile(a, w, tiles);
     g.t_end = first_tile(a, w + 1, tiles);
@@ -472,10 +474,11 @@ __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int be
     for (int p = begin + lane; p < end; p += 64) top = fmaxf(top, score(p));
 #pragma unroll
     for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
+    const float shift = top == -INFINITY ? 0.0f : top;  // scores of -inf alone weigh nothing
     sum = o[0] = o[1] = 0.0f;
     for (int p0 = begin; p0 < end; p0 += 64) {
         const int p = p0 + lane;
-        const float weight = p < end ? exp2f(score(p) - top) * 0x1p-24f : 0.0f;
+        const float weight = p < end ? exp2f(score(p) - shift) * 0x1p-24f : 0.0f;
         sum += weight;
         for (int u = 0; u < 64 && p0 + u < end; ++u) {
             const T* row = v + pool_row(a.c, s, p0 + u) * pitch;

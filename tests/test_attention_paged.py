@@ -211,6 +211,51 @@ def test_values_that_are_seen_and_not_finite(hip):
 
 
 @gpu
+def test_bf16_values_that_are_seen_and_not_finite(hip):
+    """Blocks of the matrix instructions' kernel whose sums are not finite."""
+    import torch
+    print_case("paged bf16 not finite")
+    lengths = [300, 40]
+    kp, vp, table, k, v = make(lengths, 2, 64, 16, torch.bfloat16, seed=10)
+    vp[table[0, 3].long(), 2, 0, 5] = math.inf
+    vp[table[0, 9].long(), 2, 0, 6] = math.nan
+    kp[table[1, 1].long(), 2, 0, 6] = math.nan
+    q = torch.randn(2, 6, 64, device="cuda")
+    out, lse = hip.attention_paged(q, kp, vp, table, ints(lengths))
+    assert bool((out[0, :3, 5] == math.inf).all()) and bool(torch.isnan(out[0, :3, 6]).all())
+    assert bool(torch.isfinite(out[0, :3, [0, 1, 31, 63]]).all())
+    assert bool(torch.isnan(out[1, :3]).all()) and bool(torch.isnan(lse[1, :3]).all())
+    value, bound = reference(q[:, 3:], [x[:, 1:] for x in k], [x[:, 1:] for x in v], lengths,
+                             64 ** -0.5)
+    within(out[:, 3:], value["out"], bound["out"], "out")
+    within(lse[:, 3:], value["lse"], bound["lse"], "lse")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_part_whose_scores_are_all_minus_infinity(hip, dtype):
+    """Weight 0 beside the other parts' positions, whichever blocks the length is split over; alone
+    no distribution, with lse = -inf."""
+    import torch
+    print_case("paged -inf scores", dtype)
+    lengths = [385, 7, 300]
+    kp, vp, table, k, v = make(lengths, 1, 64, 16, getattr(torch, dtype), seed=12)
+    q = torch.rand(3, 4, 64, device="cuda") + 0.5
+    kp[table[0, 24].long(), 0, 0, 9] = -math.inf              # the last tile's one position
+    for p in range(256, 300):                                 # all of a tile
+        kp[table[2, p // 16].long(), p % 16, 0, 3] = -math.inf
+    for p in range(7):                                        # all of a sequence
+        kp[table[1, 0].long(), p, 0, 0] = -math.inf
+    out, lse = hip.attention_paged(q, kp, vp, table, ints(lengths))
+    value, bound = reference(q, [k[0][:384], k[1], k[2][:256]], [v[0][:384], v[1], v[2][:256]],
+                             [384, 7, 256], 0.125)
+    for s in (0, 2):
+        within(out[s], value["out"][s], bound["out"][s], "out")
+        within(lse[s], value["lse"][s], bound["lse"][s], "lse")
+    assert bool(torch.isnan(out[1]).all()) and bool((lse[1] == -math.inf).all())
+
+
+@gpu
 def test_strides_and_outputs(hip):
     """q and out as columns of wider rows, a table that is part of a larger one."""
     import torch
