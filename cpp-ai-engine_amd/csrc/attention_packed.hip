@@ -187,13 +187,14 @@ __device__ void forward_row(const Packed& a, const Tile& t, int h, int i) {
     }
     m = wave_max(m);
     if (__any(bad)) m = NAN;
+    const float shift = m == -INFINITY ? 0.0f : m;  // scores of -inf alone: lse = -inf, out 0 / 0
     float sum = 0.0f, acc[2] = {0.0f, 0.0f};
-    for (int j = lane; j < n; j += 64) sum += expf(dot(q, k + j * a.ld_k, a.dim) * a.scale - m);
+    for (int j = lane; j < n; j += 64) sum += expf(dot(q, k + j * a.ld_k, a.dim) * a.scale - shift);
     sum = wave_sum(sum);
     for (int j0 = 0; j0 < n; j0 += 64) {
         const int j = j0 + lane;
         float p = 0.0f;  // divided here: the sums stay in range with v's values
-        if (j < n) p = expf(dot(q, k + j * a.ld_k, a.dim) * a.scale - m) / sum;
+        if (j < n) p = expf(dot(q, k + j * a.ld_k, a.dim) * a.scale - shift) / sum;
         const int count = n - j0 < 64 ? n - j0 : 64;
         for (int u = 0; u < count; ++u) {
             const float w = __shfl(p, u);

@@ -891,9 +891,11 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  *   s_ij = scale (q_i . k_j)    lse_i = log sum_j exp(s_ij)
  *   out_i = sum_j exp(s_ij - lse_i) v_j
  * over the keys seen. A row that sees none gets out = 0 and lse = -inf, and
- * gives no gradient. Keys that a row does not see do not reach it, whatever
- * they hold (NaN and infinities included). Rows of q past the last sequence
- * leave out, lse and dq as they were, rows of k past it dk and dv.
+ * gives no gradient; one whose scores are all -inf has lse = -inf and out NaN.
+ * out and lse may not overlap the inputs. Keys that a row does not see do not
+ * reach it, whatever they hold (NaN and infinities included). Rows of q past
+ * the last sequence leave out, lse and dq as they were, rows of k past it dk
+ * and dv.
  *
  * q, out, grad, dq are rows of heads * head_dim floats, ld_* floats apart (the
  * queries of a fused projection are read and their gradient written in place);
@@ -963,7 +965,7 @@ typedef struct {
  * token for each sequence (tokens = sequences). bf16 pools take the nearest
  * bf16, ties to even. A token whose position is negative, past its table row or
  * on a page outside the pool is not stored, nor are rows past the last
- * sequence. Two tokens for one place leave either. */
+ * sequence. Two tokens for one place leave values of either, in any mixture. */
 int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_k,
                           const float* v, int64_t ld_v, const int32_t* starts,
                           const int32_t* cu, int64_t tokens, void* stream);
@@ -971,12 +973,12 @@ int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_
 /* Attention of one new token per sequence over the cache: row s of q and out
  * (heads * head_dim floats, ld_q and ld_out apart) sees positions 0 ..
  * lengths[s] - 1 (a DEVICE array; write the new token's key and value first).
- * out and lse (sequences, heads; may be NULL) as in
- * ehip_attention_packed_f32. A length of zero gives out = 0, lse = -inf. A
- * negative length, one past `longest` or its table row, or a page outside the
- * pool makes the sequence's row NaN instead of a read out of bounds. `longest`,
- * a host value of at most 2^30, is what the work is split by: the same lengths
- * under another `longest` may differ in the last bits.
+ * out and lse (sequences, heads; may be NULL) as in ehip_attention_packed_f32;
+ * they may not overlap the inputs. A length of zero gives out = 0, lse = -inf.
+ * A negative length, one past `longest` or its table row, or a page outside
+ * the pool makes the sequence's row NaN instead of a read out of bounds.
+ * `longest`, a host value of at most 2^30, is what the work is split by: the
+ * same lengths under another `longest` may differ in the last bits.
  * 1 <= head_dim <= 128, heads a multiple of kv_heads. `workspace` (16-byte
  * aligned) holds the parts of split lengths during the call: at least
  * ehip_attention_paged_workspace() bytes, of the call's own. Deterministic. */

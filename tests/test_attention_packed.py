@@ -161,6 +161,24 @@ def test_values_that_are_seen_and_not_finite(hip):
 
 
 @gpu
+def test_rows_whose_scores_are_all_minus_infinity(hip):
+    """lse = -inf, the log of nothing, and no distribution to take values by; with other keys in
+    sight such a key weighs nothing."""
+    import torch
+    print_case("packed -inf scores")
+    nq = [80, 3]
+    q, k, v, _ = make(nq, nq, 2, 1, 64, seed=15)
+    q = q.abs() + 0.5
+    k[:5, 0, 7] = -math.inf
+    out, lse = hip.attention_packed(q, k, v, offsets(nq))
+    assert bool((lse[:5] == -math.inf).all()) and bool(torch.isnan(out[:5]).all())
+    # Rows 5 .. 79 over keys 5 .. 79: the last query sees every key, as before.
+    value, bound = packed(q[5:], k[5:], v[5:], [75, 3], [75, 3], 0.125, True)
+    within(out[5:], value["out"], bound["out"], "out")
+    within(lse[5:], value["lse"], bound["lse"], "lse")
+
+
+@gpu
 @pytest.mark.parametrize("size", [1e-38, 1e-30, 1e30, 2e38])
 def test_values_near_the_ends_of_the_range(hip, size):
     """Values of 1e-38 keep an absolute 2^-126; larger ones their relative accuracy."""
