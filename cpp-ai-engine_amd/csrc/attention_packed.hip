@@ -121,7 +121,7 @@ __device__ __forceinline__ Tile find_tile_by_work(const Packed& a, bool keys, in
     int w = 1, above = 0;  // above: C(w + 1)
     while (n > 0) {
         const int step = (n + 63) / 64;
-        const int mine = w + lane * step - 1;
+        const int mine = w + min(lane * step, n) - 1;
         int c = 0;
         for (int s = 0; s < a.sequences; ++s)
             c += max(0, __builtin_amdgcn_readlane(tiles, s) - mine);
@@ -249,9 +249,9 @@ __device__ void dq_row(const Packed& a, const Tile& t, int h, int i, float delta
         if (lane + 64 * e < a.dim) dq[lane + 64 * e] = acc[e] * a.scale;
 }
 
-// The sums over query heads [h0, h1), into rows dk and dv of `dim` values (either may be null).
-__device__ void dkv_row(const Packed& a, const Tile& t, int c, int h0, int h1, int j, float* dk,
-                        float* dv) {
+// Query head h's share, into rows dk and dv of `dim` values (either may be null).
+__device__ void dkv_row(const Packed& a, const Tile& t, int h, int j, float* dk, float* dv) {
+    const int c = h / (a.heads / a.kv_heads);
     const int lane = int(threadIdx.x) & 63;
     const int64_t row = t.k0 + j;
     const float* k = a.k + row * a.ld_k + int64_t(c) * a.dim;
@@ -260,29 +260,28 @@ __device__ void dkv_row(const Packed& a, const Tile& t, int c, int h0, int h1, i
     int64_t start = a.causal ? int64_t(j) - t.nk + t.nq : 0;
     start = start < 0 ? 0 : start;
     float ak[2] = {0.0f, 0.0f}, av[2] = {0.0f, 0.0f};
-    for (int h = h0; h < h1; ++h)
-        for (int64_t i0 = start; i0 < t.nq; i0 += 64) {
-            const int64_t i = i0 + lane;
-            float p = 0.0f, ds = 0.0f;
-            if (i < t.nq) {
-                const int64_t at = t.q0 + i;
-                ds = pair_gradient(a, a.q + at * a.ld_q + int64_t(h) * a.dim,
-                                   a.grad + at * a.ld_grad + int64_t(h) * a.dim, k, v,
-                                   a.lse[at * a.heads + h], a.delta[at * a.heads + h], p);
-            }
-            const int count = t.nq - i0 < 64 ? int(t.nq - i0) : 64;
-            for (int u = 0; u < count; ++u) {
-                const float wp = __shfl(p, u), wd = __shfl(ds, u);
-                const float* x = a.q + (t.q0 + i0 + u) * a.ld_q + int64_t(h) * a.dim;
-                const float* g = a.grad + (t.q0 + i0 + u) * a.ld_grad + int64_t(h) * a.dim;
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    if (lane + 64 * e < a.dim) {
-                        ak[e] = __builtin_fmaf(wd, x[lane + 64 * e], ak[e]);
-                        av[e] = __builtin_fmaf(wp, g[lane + 64 * e], av[e]);
-                    }
-            }
+    for (int64_t i0 = start; i0 < t.nq; i0 += 64) {
+        const int64_t i = i0 + lane;
+        float p = 0.0f, ds = 0.0f;
+        if (i < t.nq) {
+            const int64_t at = t.q0 + i;
+            ds = pair_gradient(a, a.q + at * a.ld_q + int64_t(h) * a.dim,
+                               a.grad + at * a.ld_grad + int64_t(h) * a.dim, k, v,
+                               a.lse[at * a.heads + h], a.delta[at * a.heads + h], p);
         }
+        const int count = t.nq - i0 < 64 ? int(t.nq - i0) : 64;
+        for (int u = 0; u < count; ++u) {
+            const float wp = __shfl(p, u), wd = __shfl(ds, u);
+            const float* x = a.q + (t.q0 + i0 + u) * a.ld_q + int64_t(h) * a.dim;
+            const float* g = a.grad + (t.q0 + i0 + u) * a.ld_grad + int64_t(h) * a.dim;
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (lane + 64 * e < a.dim) {
+                    ak[e] = __builtin_fmaf(wd, x[lane + 64 * e], ak[e]);
+                    av[e] = __builtin_fmaf(wp, g[lane + 64 * e], av[e]);
+                }
+        }
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e)
         if (lane + 64 * e < a.dim) {
@@ -450,8 +449,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
         forward_row(a, t, h, t.first + 32 * wave + __builtin_ctz(rows));
 }
 
-// The backward forms s, and so p_ij, again from the inputs, and dp likewise, for the pairs of a wave's
-// own rows and a block of 32 streamed ones, then the block's share of the gradients.
+// The backward forms s, and so p_ij, again from the inputs, and dp likewise, for the pairs of a
+// wave's own rows and a block of 32 streamed ones, then the block's share of the gradients.
 
 // dq_i = scale sum_j ds_ij k_j of heads of up to 64 values, with delta on the way (left in the
 // workspace for the keys' kernel): a wave has room for q and g both, and needs no partner.
@@ -548,10 +547,10 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     }
 }
 
-// Its larger kernels' blocks own 128 rows, as four groups of 32 and two waves a group: both form scores
-// for the same pairs, one wave s and the other dp = g . v, exchange them through LDS, and each
-// accumulates its share of the gradients. So a wave holds one own row and half of the results a
-// lane, which leaves room for two waves a SIMD at every head size: a lone wave issues a vector
+// Its larger kernels' blocks own 128 rows, as four groups of 32 and two waves a group: both form
+// scores for the same pairs, one wave s and the other dp = g . v, exchange them through LDS, and
+// each accumulates its share of the gradients. So a wave holds one own row and half of the results
+// a lane, which leaves room for two waves a SIMD at every head size: a lone wave issues a vector
 // instruction every eighth cycle only. A step is two phases with a barrier after each: the scores,
 // from the streamed rows, then the gradients, from the same rows read transposed.
 constexpr int kBackThreads = 512;
@@ -565,7 +564,8 @@ __device__ __forceinline__ uint32_t shared_rows(uint32_t* votes, bool bad) {
     return __builtin_amdgcn_readfirstlane(votes[wave & 3] | votes[(wave & 3) + 4]);
 }
 
-// dq and delta of wider heads. Wave role 0 forms s and p, role 1 dp - delta; both then have ds, and half of dq's values each.
+// dq and delta of wider heads. Wave role 0 forms s and p, role 1 dp - delta; both then have ds, and
+// half of dq's values each.
 template <int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed a) {
     using namespace attention;
@@ -723,12 +723,9 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     __shared__ __attribute__((aligned(16))) char lds[4 * QueryTile::kBytes + kSwap];
     __shared__ __attribute__((aligned(16))) float stats[2][2][BN];  // as the tiles, by turns
     char* const lds_x = lds + 4 * QueryTile::kBytes;
-    const int group = a.heads / a.kv_heads, parts = a.part_k != nullptr ? group : 1;
-    const int x = int(blockIdx.x % (a.kv_heads * parts)), c = x % a.kv_heads;
-    const Tile t = block_tile(a, true, int(blockIdx.x / (a.kv_heads * parts)), kRows);
+    const int h = head_of(a, int(blockIdx.x % a.heads)), c = h / (a.heads / a.kv_heads);
+    const Tile t = block_tile(a, true, int(blockIdx.x / a.heads), kRows);
     if (t.rows == 0) return;
-    const int h0 = c * group + (parts > 1 ? x / a.kv_heads : 0);
-    const int heads = parts > 1 ? 1 : group;  // from h0 on
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int role = wave / 4, w0 = 32 * (wave & 3), lane = int(threadIdx.x) & 63;
     const int mine = w0 + (lane & 31);  // the lane's key, of the tile
@@ -752,14 +749,13 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d) sum[d] = zeros();
     const int ld_q = int(a.ld_q), ld_g = int(a.ld_grad);
-    const int steps = start < t.nq ? (t.nq - start + BN - 1) / BN : 0;
-    const int count = steps * heads;
     QueryTile qt(ld_q, a.dim), gt(ld_g, a.dim);
     float stat = 0.0f;  // a query's lse (threads 0 .. BN - 1) or delta (the next BN)
-    // Tile n: head h0 + n / steps, its queries from start + n % steps * BN on.
+    // Tile n: the queries from start + n * BN on.
+    const int count = start < t.nq ? (t.nq - start + BN - 1) / BN : 0;
     const auto load_rows = [&](int n) {
         if (n >= count) return;
-        const int h = h0 + n / steps, i0 = start + n % steps * BN, left = t.nq - i0;
+        const int i0 = start + n * BN, left = t.nq - i0;
         const int64_t at = t.q0 + i0;
         qt.load(a.q + at * a.ld_q + int64_t(h) * a.dim, ld_q, left, a.dim);
         gt.load(a.grad + at * a.ld_grad + int64_t(h) * a.dim, ld_g, left, a.dim);
@@ -770,7 +766,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     };
     const auto stage_rows = [&](int n) {
         if (n >= count) return;
-        const int left = t.nq - (start + n % steps * BN);
+        const int left = t.nq - (start + n * BN);
         char* const at = lds + (n & 1) * 2 * QueryTile::kBytes;
         qt.store(at, left, a.dim);
         gt.store(at + QueryTile::kBytes, left, a.dim);
@@ -784,7 +780,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     load_rows(1);
     __syncthreads();
     for (int n = 0; n < count; ++n) {
-        const int i0 = start + n % steps * BN, left = t.nq - i0;
+        const int i0 = start + n * BN, left = t.nq - i0;
         const bool active = i0 + BN > wave_start;
         const char* const tile = lds + (n & 1) * 2 * QueryTile::kBytes;
         if (role == 1) {  // the next tile: one wave of a SIMD before its products, the other after
@@ -883,12 +879,14 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     const uint32_t again = shared_rows(reinterpret_cast<uint32_t*>(lds), !fine && mine < t.rows);
     // Where the rows of dk (or dv) of key j go.
     const auto row_dk = [&](int64_t at) {
-        return parts > 1 ? a.part_k + (at * a.heads + h0) * a.dim
-                         : (a.dk == nullptr ? nullptr : a.dk + at * a.ld_dk + int64_t(c) * a.dim);
+        return a.part_k != nullptr ? a.part_k + (at * a.heads + h) * a.dim
+               : a.dk == nullptr   ? nullptr
+                                   : a.dk + at * a.ld_dk + int64_t(c) * a.dim;
     };
     const auto row_dv = [&](int64_t at) {
-        return parts > 1 ? a.part_v + (at * a.heads + h0) * a.dim
-                         : (a.dv == nullptr ? nullptr : a.dv + at * a.ld_dv + int64_t(c) * a.dim);
+        return a.part_v != nullptr ? a.part_v + (at * a.heads + h) * a.dim
+               : a.dv == nullptr   ? nullptr
+                                   : a.dv + at * a.ld_dv + int64_t(c) * a.dim;
     };
     float* const out = role == 0 ? row_dv(row) : row_dk(row);
     if (out != nullptr && mine < t.rows && !(again >> (lane & 31) & 1)) {
@@ -898,7 +896,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     if (role == 0)
         for (uint32_t rows = again; rows != 0; rows &= rows - 1) {
             const int64_t key = t.first + w0 + __builtin_ctz(rows);
-            dkv_row(a, t, c, h0, h0 + heads, int(key), row_dk(t.k0 + key), row_dv(t.k0 + key));
+            dkv_row(a, t, h, int(key), row_dk(t.k0 + key), row_dv(t.k0 + key));
         }
 }
 
@@ -1030,12 +1028,10 @@ int launch_backward(const Packed& a, hipStream_t s) {
                         dim3(blocks), dim3(kBackThreads), 0, s, a);
     }
     if (a.total_k == 0 || (a.dk == nullptr && a.dv == nullptr)) return EHIP_OK;
-    const bool split = a.part_k != nullptr;
-    const unsigned blocks =
-        unsigned(slots(a.total_k, a.sequences) * (split ? a.heads : a.kv_heads));
+    const unsigned blocks = unsigned(slots(a.total_k, a.sequences) * a.heads);
     EHIP_LAUNCH("attention_packed_backward_kv", (packed_backward_kv<DP, BN, VEC>), dim3(blocks),
                 dim3(kBackThreads), 0, s, a);
-    if (split) {
+    if (a.part_k != nullptr) {
         const int64_t n = int64_t(a.total_k) * a.kv_heads * a.dim;
         EHIP_LAUNCH("attention_packed_backward_join", packed_backward_join,
                     dim3(unsigned(std::min<int64_t>(ceil_div(n, kThreads), 1 << 16))),
@@ -1108,9 +1104,15 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
     }
     hipStream_t s = as_stream(stream);
     const bool vec = a.dim % 4 == 0;
-    if (a.dim <= 32) return vec ? launch_backward<32, 64, true>(a, s) : launch_backward<32, 64, false>(a, s);
-    if (a.dim <= 64) return vec ? launch_backward<64, 64, true>(a, s) : launch_backward<64, 64, false>(a, s);
-    if (a.dim <= 96) return vec ? launch_backward<96, 32, true>(a, s) : launch_backward<96, 32, false>(a, s);
+    if (a.dim <= 32)
+        return vec ? launch_backward<32, 64, true>(a, s)
+                   : launch_backward<32, 64, false>(a, s);
+    if (a.dim <= 64)
+        return vec ? launch_backward<64, 64, true>(a, s)
+                   : launch_backward<64, 64, false>(a, s);
+    if (a.dim <= 96)
+        return vec ? launch_backward<96, 32, true>(a, s)
+                   : launch_backward<96, 32, false>(a, s);
     return vec ? launch_backward<128, 32, true>(a, s) : launch_backward<128, 32, false>(a, s);
 }
 
