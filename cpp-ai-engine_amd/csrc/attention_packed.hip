@@ -100,11 +100,11 @@ __device__ __forceinline__ Tile find_tile(const Packed& a, bool keys, int slot, 
     return tile_of(a, keys, lo, keys ? at : tiles - 1 - at, size);
 }
 
-// The same, under a causal mask and for up to 64 sequences, in the order of the tiles' work, the most
-// first: the last blocks to start are the shortest, whatever their sequences. A sequence of n tiles
-// has one of work w for every w from 1 to n, so C(w), the sum over the sequences of n - w + 1 where
-// that is positive, tiles have work w or more, and slot's has the largest w with C(w) > slot. A lane
-// has a sequence's n for all of them, and then a candidate w, 64 at a time.
+// The same, under a causal mask and for up to 64 sequences, in the order of the tiles' work, the
+// most first: the last blocks to start are the shortest, whatever their sequences. A sequence of n
+// tiles has one of work w for every w from 1 to n, so C(w), the sum over the sequences of n - w + 1
+// where that is positive, tiles have work w or more, and slot's has the largest w with C(w) > slot.
+// A lane has a sequence's n for all of them, and then a candidate w, 64 at a time.
 __device__ __forceinline__ Tile find_tile_by_work(const Packed& a, bool keys, int slot, int size) {
     const int32_t* cu = keys ? a.cu_k : a.cu_q;
     const int total = keys ? a.total_k : a.total_q;
@@ -291,8 +291,8 @@ __device__ void dkv_row(const Packed& a, const Tile& t, int h, int j, float* dk,
 }
 
 // ------------------------------------------------------------------- kernels
-// Block = slot * heads + head, the heads of one key head 8 (or any multiple of the key heads) apart:
-// with the dispatcher's round robin over the eight XCDs they meet their keys in one L2.
+// Block = slot * heads + head, the heads of one key head 8 (or any multiple of the key heads)
+// apart: with the dispatcher's round robin over the eight XCDs they meet their keys in one L2.
 
 __device__ __forceinline__ int head_of(const Packed& a, int x) {
     return x % a.kv_heads * (a.heads / a.kv_heads) + x / a.kv_heads;
@@ -555,7 +555,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
 // from the streamed rows, then the gradients, from the same rows read transposed.
 constexpr int kBackThreads = 512;
 
-// Gives the two waves of a group the rows either of them found without a finite result (a bit each).
+// Gives the two waves of a group the rows (a bit each) that either found without a finite result.
 __device__ __forceinline__ uint32_t shared_rows(uint32_t* votes, bool bad) {
     const uint64_t b = __ballot(bad);
     const int wave = int(threadIdx.x) / 64;
@@ -712,8 +712,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
         }
 }
 
-// dv_j = sum_i p_ij g_i by the waves of role 0, from s and p, and dk_j = scale sum_i ds_ij q_i by those
-// of role 1, from dp and the other's p.
+// dv_j = sum_i p_ij g_i by the waves of role 0, from s and p, and dk_j = scale sum_i ds_ij q_i by
+// those of role 1, from dp and the other's p.
 template <int DP, int BN, bool VEC>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) {
     using namespace attention;
@@ -990,13 +990,13 @@ int launch_forward(const Packed& a, hipStream_t s) {
 
 template <int DP, int BN, bool VEC>
 int forward_of(const Packed& a, hipStream_t s) {
-    // 256 queries a block convert their keys once and read them by turns of two tiles; 128 leave less
-    // between the last block and the others. Without the causal mask all blocks of a sequence are
-    // alike, and 256 it is once they fill the card (us, 128 : 256 queries, heads of 64 values: one of
-    // 4096, 16 heads, 341 : 326, with 8 heads 216 : 275). With it, long sequences that fill the card
-    // twice over (4 of 2048, 16 heads, 207 : 200; 24 of 64 to 1291 147 : 169; one of 8192, 8 heads,
-    // 490 : 566). Heads over 96 values spill with 128, and take them for short causal ones alone
-    // (64 of 128 87 : 103; one of 4096 593 : 509; without the mask 64 of 128 136 : 82).
+    // 256 queries a block convert their keys once and read them by turns of two tiles; 128 leave
+    // less between the last block and the others. Without the causal mask all blocks of a sequence
+    // are alike, and 256 it is once they fill the card (us, 128 : 256 queries, heads of 64 values:
+    // one of 4096, 16 heads, 341 : 326, with 8 heads 216 : 275). With it, long sequences that fill
+    // the card twice over (4 of 2048, 16 heads, 207 : 200; 24 of 64 to 1291 147 : 169; one of 8192,
+    // 8 heads, 490 : 566). Heads over 96 values spill with 128, and take them for short causal ones
+    // alone (64 of 128 87 : 103; one of 4096 593 : 509; without the mask 64 of 128 136 : 82).
     const int64_t n = a.total_q, s_count = a.sequences, blocks = n / 256 * a.heads;
     const bool four = DP > 96   ? a.causal && n < 256 * s_count
                       : a.causal ? n < 2048 * s_count || blocks < 512
@@ -1005,7 +1005,7 @@ int forward_of(const Packed& a, hipStream_t s) {
 }
 
 // dk and dv of grouped heads are formed head by head, for as many blocks as the queries have, and
-// summed afterwards (12 heads over 4, 5576 rows of 96: 352 us in place of 993 by one block a group).
+// summed afterwards (12 heads over 4, 5576 rows of 96: one block a group took 2.8 times as long).
 bool splits(const Packed& a) { return a.heads != a.kv_heads; }
 
 size_t delta_bytes(const Packed& a) {
@@ -1079,8 +1079,8 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
     if (a.sequences == 0) return EHIP_OK;
     const int64_t wide = int64_t(a.heads) * a.dim, narrow = int64_t(a.kv_heads) * a.dim;
     if (a.total_q > 0 && (grad == nullptr || ld_grad < wide || ld_grad > kMaxLd))
-        return fail(EHIP_EINVAL, "attention_packed_backward: null gradient, or its leading dimension "
-                                 "below the row's length or above 2^22");
+        return fail(EHIP_EINVAL, "attention_packed_backward: null gradient, or its leading "
+                                 "dimension below the row's length or above 2^22");
     if ((dq != nullptr && ld_dq < wide) || (dk != nullptr && ld_dk < narrow) ||
         (dv != nullptr && ld_dv < narrow))
         return fail(EHIP_EINVAL,
@@ -1088,7 +1088,8 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
     const size_t need = delta_bytes(a) + 2 * part_bytes(a);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
         return fail(EHIP_EINVAL,
-                    "attention_packed_backward: needs %zu bytes of 16-byte aligned workspace", need);
+                    "attention_packed_backward: needs %zu bytes of 16-byte aligned workspace",
+                    need);
     a.grad = grad;
     a.ld_grad = ld_grad;
     a.dq = dq;

@@ -90,12 +90,13 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append(
 
 // ----------------------------------------------------------------- attention
 
-// The cache is read once and bounds the time, so the kernel's shape is that of its reads: a position's
-// row of `dim` values takes LPP lanes, 16 bytes each, and a wave reads kUnroll x 64 / LPP
-// positions of keys and values at a time. A lane holds its values of up to G query heads that share
-// the keys. The lanes of a position add up its scores; each position's lanes keep their own running
-// maximum, sum and weighted values over the positions they meet, joined at the end: of the wave, the
-// block's four waves, and, where the length is split, the blocks of a sequence by a second launch.
+// The cache is read once and bounds the time, so the kernel's shape is that of its reads: a
+// position's row of `dim` values takes LPP lanes, 16 bytes each, and a wave reads kUnroll x 64 /
+// LPP positions of keys and values at a time. A lane holds its values of up to G query heads that
+// share the keys. The lanes of a position add up its scores; each position's lanes keep their own
+// running maximum, sum and weighted values over the positions they meet, joined at the end: of the
+// wave, the block's four waves, and, where the length is split, the blocks of a sequence by a
+// second launch.
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = kPagedThreads / 64;
 constexpr int kUnroll = 4;
@@ -118,11 +119,11 @@ struct Paged {
     int* first;          // (sequences + 1): the sequences' first tiles
 };
 
-// The work is cut evenly, whatever the lengths: the positions of all sequences in tiles of kTile, one
-// after the other, and a worker's blocks (one for each key head) take its share of them, which may
-// be part of a long sequence or several short ones. What a worker adds to a sequence is a segment.
-// Segment (worker w, sequence s) has place w + s of a head's parts, no other's: from one to the next
-// at least one of them grows.
+// The work is cut evenly, whatever the lengths: the positions of all sequences in tiles of kTile,
+// one after the other, and a worker's blocks (one for each key head) take its share of them, which
+// may be part of a long sequence or several short ones. What a worker adds to a sequence is a
+// segment. Segment (worker w, sequence s) has place w + s of a head's parts, no other's: from one
+// to the next at least one of them grows.
 constexpr int kTile = 128;
 
 // Positions of a sequence, -1 for a length that is none.
@@ -134,8 +135,8 @@ __device__ __forceinline__ int length_of(const Paged& a, int64_t s) {
 }
 __device__ __forceinline__ int tiles_of(int n) { return n > 0 ? (n - 1) / kTile + 1 : 0; }
 
-// The first tile of worker w of so many tiles, and the worker of tile t. With fewer tiles than workers
-// the last ones have none; every other one has one at least.
+// The first tile of worker w of so many tiles, and the worker of tile t. With fewer tiles than
+// workers the last ones have none; every other one has one at least.
 __device__ __forceinline__ int first_tile(const Paged& a, int w, int tiles) {
     const int workers = min(a.workers, tiles);
     return w < workers ? int(int64_t(w) * tiles / workers) : tiles;
@@ -264,8 +265,8 @@ __device__ __forceinline__ float across(float x) {
     return with_half(x);
 }
 
-// One lane's values of a row as they are stored: 16 bytes, and its own first ones again in lanes past
-// the row's end.
+// One lane's values of a row as they are stored: 16 bytes, and its own first ones again in lanes
+// past the row's end.
 template <class T, bool VEC>
 struct Values {
     static constexpr int N = 16 / int(sizeof(T));
@@ -299,161 +300,161 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
     x /= uint32_t(pieces);
     const int worker = int(x);
     for (Segment seg = first_segment(a, worker); seg.t < seg.t_end; next_segment(a, seg)) {
-    const int64_t s = seg.s;
-    const int begin = seg.begin, end = seg.end;
-    bool bad = false;  // a page outside the pool
+        const int64_t s = seg.s;
+        const int begin = seg.begin, end = seg.end;
+        bool bad = false;  // a page outside the pool
 
-    const int sub = lane / LPP, d0 = (lane % LPP) * N, left = dim - d0;
-    const float c2 = fabsf(a.scale) * 1.44269504088896340736f;
-    float q[G][N], o[G][N], m[G], l[G];
+        const int sub = lane / LPP, d0 = (lane % LPP) * N, left = dim - d0;
+        const float c2 = fabsf(a.scale) * 1.44269504088896340736f;
+        float q[G][N], o[G][N], m[G], l[G];
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        m[g] = -INFINITY;
-        l[g] = 0.0f;
-        const float* row = a.q + s * a.ld_q + int64_t(h0 + (g < count ? g : 0)) * dim + d0;
+        for (int g = 0; g < G; ++g) {
+            m[g] = -INFINITY;
+            l[g] = 0.0f;
+            const float* row = a.q + s * a.ld_q + int64_t(h0 + (g < count ? g : 0)) * dim + d0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            q[g][e] = e < left ? row[e] * (a.scale < 0.0f ? -c2 : c2) : 0.0f;
-            o[g][e] = 0.0f;
+            for (int e = 0; e < N; ++e) {
+                q[g][e] = e < left ? row[e] * (a.scale < 0.0f ? -c2 : c2) : 0.0f;
+                o[g][e] = 0.0f;
+            }
         }
-    }
-    const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
-    const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
-    const int64_t pitch = int64_t(kv_heads) * dim;
-    // The pool row of the tile's position `lane`.
-    const auto row_of = [&](int p0) {
-        const int p = p0 + lane;
-        if (lane >= TILE || p >= end) return int64_t(0);
-        const int64_t row = pool_row(a.c, s, p);
-        if (row < 0) {
-            bad = true;
-            return int64_t(0);
-        }
-        return row;
-    };
-    int row = int(row_of(begin + wave * TILE));
-    for (int p0 = begin + wave * TILE; p0 < end; p0 += kPagedWaves * TILE) {
-        Values<T, VEC> ks[kUnroll], vs[kUnroll];
+        const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
+        const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
+        const int64_t pitch = int64_t(kv_heads) * dim;
+        // The pool row of the tile's position `lane`.
+        const auto row_of = [&](int p0) {
+            const int p = p0 + lane;
+            if (lane >= TILE || p >= end) return int64_t(0);
+            const int64_t row = pool_row(a.c, s, p);
+            if (row < 0) {
+                bad = true;
+                return int64_t(0);
+            }
+            return row;
+        };
+        int row = int(row_of(begin + wave * TILE));
+        for (int p0 = begin + wave * TILE; p0 < end; p0 += kPagedWaves * TILE) {
+            Values<T, VEC> ks[kUnroll], vs[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t at = int64_t(__shfl(row, u * SUBS + sub)) * pitch;
-            ks[u].load(k + at, d0, dim);
-            vs[u].load(v + at, d0, dim);
-        }
-        row = int(row_of(p0 + kPagedWaves * TILE));
-        float w[G][kUnroll];
+            for (int u = 0; u < kUnroll; ++u) {
+                const int64_t at = int64_t(__shfl(row, u * SUBS + sub)) * pitch;
+                ks[u].load(k + at, d0, dim);
+                vs[u].load(v + at, d0, dim);
+            }
+            row = int(row_of(p0 + kPagedWaves * TILE));
+            float w[G][kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float x[N];
+            for (int u = 0; u < kUnroll; ++u) {
+                float x[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = ks[u][e];
-            if (dim < LPP * N) {  // a lane past the row's end read something else
+                for (int e = 0; e < N; ++e) x[e] = ks[u][e];
+                if (dim < LPP * N) {  // a lane past the row's end read something else
 #pragma unroll
-                for (int e = 0; e < N; ++e) x[e] = e < left ? x[e] : 0.0f;
+                    for (int e = 0; e < N; ++e) x[e] = e < left ? x[e] : 0.0f;
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    float dot = q[g][0] * x[0];
+#pragma unroll
+                    for (int e = 1; e < N; ++e) dot = __builtin_fmaf(q[g][e], x[e], dot);
+                    w[g][u] = group_sum<LPP>(dot);
+                }
+            }
+            const bool tail = p0 + TILE > end;
+            if (tail) {
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+                        w[g][u] = p0 + u * SUBS + sub < end ? w[g][u] : -INFINITY;
             }
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                float dot = q[g][0] * x[0];
+                float top = m[g];
 #pragma unroll
-                for (int e = 1; e < N; ++e) dot = __builtin_fmaf(q[g][e], x[e], dot);
-                w[g][u] = group_sum<LPP>(dot);
+                for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, w[g][u]);
+                const float shift = top == -INFINITY ? 0.0f : top;
+                const float keep = m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[g] - shift);
+                m[g] = top;
+                l[g] *= keep;
+#pragma unroll
+                for (int e = 0; e < N; ++e) o[g][e] *= keep;
+#pragma unroll
+                for (int u = 0; u < kUnroll; ++u) {
+                    // 2^-24 of the weight: sums over the values stay in their range.
+                    w[g][u] = __builtin_amdgcn_exp2f(w[g][u] - shift) * 0x1p-24f;
+                    l[g] += w[g][u];
+                }
             }
-        }
-        const bool tail = p0 + TILE > end;
-        if (tail) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
+            for (int u = 0; u < kUnroll; ++u) {
+                float x[N];
+#pragma unroll
+                for (int e = 0; e < N; ++e) x[e] = vs[u][e];
+                if (tail) {  // nor does a position past the length
+#pragma unroll
+                    for (int e = 0; e < N; ++e) x[e] = p0 + u * SUBS + sub < end ? x[e] : 0.0f;
+                }
 #pragma unroll
                 for (int g = 0; g < G; ++g)
-                    w[g][u] = p0 + u * SUBS + sub < end ? w[g][u] : -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < N; ++e) o[g][e] = __builtin_fmaf(w[g][u], x[e], o[g][e]);
+            }
         }
+        bad = __syncthreads_or(bad);
+
+        // The wave's positions, then the block's waves.
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             float top = m[g];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) top = fmaxf(top, w[g][u]);
-            const float shift = top == -INFINITY ? 0.0f : top;
-            const float keep = m[g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[g] - shift);
-            m[g] = top;
+            for (int w = LPP; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
+            const float keep = m[g] == -INFINITY ? (l[g] != l[g] ? NAN : 0.0f)
+                                                 : __builtin_amdgcn_exp2f(m[g] - top);
             l[g] *= keep;
-#pragma unroll
-            for (int e = 0; e < N; ++e) o[g][e] *= keep;
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                // 2^-24 of the weight: sums over the values stay in their range.
-                w[g][u] = __builtin_amdgcn_exp2f(w[g][u] - shift) * 0x1p-24f;
-                l[g] += w[g][u];
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float x[N];
-#pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = vs[u][e];
-            if (tail) {  // nor does a position past the length
-#pragma unroll
-                for (int e = 0; e < N; ++e) x[e] = p0 + u * SUBS + sub < end ? x[e] : 0.0f;
+            l[g] = across<LPP>(l[g]);
+            if (lane == 0) {
+                sh_m[wave][g] = top;
+                sh_l[wave][g] = l[g];
             }
 #pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int e = 0; e < N; ++e) o[g][e] = __builtin_fmaf(w[g][u], x[e], o[g][e]);
+            for (int e = 0; e < N; ++e) {
+                float y = o[g][e] * keep;
+                y = across<LPP>(y);
+                if (sub == 0) sh_o[wave][g][d0 + e] = y;
+            }
         }
-    }
-    bad = __syncthreads_or(bad);
-
-    // The wave's positions, then the block's waves.
+        __syncthreads();
+        for (int g = 0; g < count; ++g) {
+            float top = sh_m[0][g], sum = 0.0f;
 #pragma unroll
-    for (int g = 0; g < G; ++g) {
-        float top = m[g];
+            for (int w = 1; w < kPagedWaves; ++w) top = fmaxf(top, sh_m[w][g]);
+            float keep[kPagedWaves];
 #pragma unroll
-        for (int w = LPP; w < 64; w *= 2) top = fmaxf(top, __shfl_xor(top, w));
-        const float keep = m[g] == -INFINITY ? (l[g] != l[g] ? NAN : 0.0f)
-                                             : __builtin_amdgcn_exp2f(m[g] - top);
-        l[g] *= keep;
-        l[g] = across<LPP>(l[g]);
-        if (lane == 0) {
-            sh_m[wave][g] = top;
-            sh_l[wave][g] = l[g];
+            for (int w = 0; w < kPagedWaves; ++w) {
+                keep[w] = sh_m[w][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh_m[w][g] - top);
+                sum += sh_l[w][g] * (sh_l[w][g] != sh_l[w][g] ? 1.0f : keep[w]);
+            }
+            const int64_t at = int64_t(h0 + g) * (a.workers + a.c.sequences) + worker + s;
+            if (bad) sum = NAN;
+            if (threadIdx.x == 0) {
+                if (!seg.whole) a.part_stats[at] = float2{top, sum};
+                else if (a.lse != nullptr) a.lse[s * a.heads + h0 + g] = lse_of(top, sum);
+            }
+            for (int d = int(threadIdx.x); d < dim; d += kPagedThreads) {
+                float y = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kPagedWaves; ++w) y += sh_o[w][g][d] * keep[w];
+                if (!seg.whole) a.part_out[at * dim + d] = y;
+                else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y / sum;
+            }
         }
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            float y = o[g][e] * keep;
-            y = across<LPP>(y);
-            if (sub == 0) sh_o[wave][g][d0 + e] = y;
-        }
-    }
-    __syncthreads();
-    for (int g = 0; g < count; ++g) {
-        float top = sh_m[0][g], sum = 0.0f;
-#pragma unroll
-        for (int w = 1; w < kPagedWaves; ++w) top = fmaxf(top, sh_m[w][g]);
-        float keep[kPagedWaves];
-#pragma unroll
-        for (int w = 0; w < kPagedWaves; ++w) {
-            keep[w] = sh_m[w][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh_m[w][g] - top);
-            sum += sh_l[w][g] * (sh_l[w][g] != sh_l[w][g] ? 1.0f : keep[w]);
-        }
-        const int64_t at = int64_t(h0 + g) * (a.workers + a.c.sequences) + worker + s;
-        if (bad) sum = NAN;
-        if (threadIdx.x == 0) {
-            if (!seg.whole) a.part_stats[at] = float2{top, sum};
-            else if (a.lse != nullptr) a.lse[s * a.heads + h0 + g] = lse_of(top, sum);
-        }
-        for (int d = int(threadIdx.x); d < dim; d += kPagedThreads) {
-            float y = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kPagedWaves; ++w) y += sh_o[w][g][d] * keep[w];
-            if (!seg.whole) a.part_out[at * dim + d] = y;
-            else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y / sum;
-        }
-    }
-    __syncthreads();
+        __syncthreads();
     }
 }
 
-// One head's share of a block by the formula, for those whose sums by parts are not finite: a part of
-// an infinity, or an infinity times the parts of a finite value, is NaN where the product is an
+// One head's share of a block by the formula, for those whose sums by parts are not finite: a part
+// of an infinity, or an infinity times the parts of a finite value, is NaN where the product is an
 // infinity or, its weight 0, nothing at all. One wave.
 template <class T>
 __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int begin, int end,
@@ -496,13 +497,15 @@ __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int be
 // A cache in bf16, up to 16 query heads of a key head at a time, on v_mfma_f32_16x16x32_bf16: the
 // cached values are operands as they are, q and the weights in three parts, so a score and a
 // weighted value take three products each, for any number of heads at one cost; by vector
-// instructions four heads ran at 4.3 TB/s of 5.4 and eight at 2.7. Lane l holds A(l % 16, 8 (l / 16) +
-// 0..7), B(8 (l / 16) + 0..7, l % 16) and D(4 (l / 16) + r, l % 16).
-//   scores:  A = 16 positions by 32 values of K, as 16-byte reads leave them; B = q; D's column = head
-//   weights: the D's of positions 0..15 and 16..31 are the B of 32 positions, in the order 4 h + 0..3,
-//            16 + 4 h + 0..3 for the lanes h = l / 16
+// instructions four heads ran at 4.3 TB/s of 5.4 and eight at 2.7. Lane l holds A(l % 16, 8 (l /
+// 16) + 0..7), B(8 (l / 16) + 0..7, l % 16) and D(4 (l / 16) + r, l % 16).
+//   scores:  A = 16 positions by 32 values of K, as 16-byte reads leave them; B = q; D's columns
+//            are heads
+//   weights: the D's of positions 0..15 and 16..31 are the B of 32 positions, in the order
+//            4 h + 0..3, 16 + 4 h + 0..3 for the lanes h = l / 16
 //   values:  A = 16 values by those 32 positions of V: rows in LDS, read transposed
-// A wave takes 32 positions at a time; the next ones' reads are out while it forms weights and sums.
+// A wave takes 32 positions at a time; the next ones' reads are out while it forms weights and
+// sums.
 constexpr int kTilePositions = 32;
 
 template <int DP>
@@ -532,192 +535,193 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
     x /= uint32_t(pieces);
     const int worker = int(x);
     for (Segment seg = first_segment(a, worker); seg.t < seg.t_end; next_segment(a, seg)) {
-    const int64_t s = seg.s;
-    const int begin = seg.begin, end = seg.end;
-    bool bad = false;  // a page outside the pool
+        const int64_t s = seg.s;
+        const int begin = seg.begin, end = seg.end;
+        bool bad = false;  // a page outside the pool
 
-    const int col = lane & 15, quarter = lane / 16;
-    const float c2 = a.scale * 1.44269504088896340736f;
-    bf16x8 q[KS][3];
-    {
-        const float* row = a.q + s * a.ld_q + int64_t(h0 + (col < count ? col : 0)) * dim;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const int d0 = 32 * ks + 8 * quarter;
-            float y[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                y[e] = d0 < dim && col < count ? row[d0 < dim ? d0 + e : 0] * c2 : 0.0f;
-            attention::split8(y, q[ks]);
-        }
-    }
-    floatx4 o[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m = -INFINITY, l = 0.0f;
-
-    const Bf16* const k = static_cast<const Bf16*>(a.c.k) + int64_t(kv) * dim;
-    const Bf16* const v = static_cast<const Bf16*>(a.c.v) + int64_t(kv) * dim;
-    const int64_t pitch = int64_t(kv_heads) * dim;
-    bf16x8 kx[2][KS];
-    uintx4 vx[kReads];
-    const int v_lane = lane / LANES, v_d0 = lane % LANES * 8;
-    const auto load = [&](int p0) {
-        const int p = p0 + (lane & 31);
-        int64_t row = 0;
-        if (p < end) {
-            row = pool_row(a.c, s, p);
-            if (row < 0) {
-                bad = true;
-                row = 0;
-            }
-        }
-        const int r = int(row);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            const Bf16* at = k + int64_t(__shfl(r, 16 * t + col)) * pitch;
+        const int col = lane & 15, quarter = lane / 16;
+        const float c2 = a.scale * 1.44269504088896340736f;
+        bf16x8 q[KS][3];
+        {
+            const float* row = a.q + s * a.ld_q + int64_t(h0 + (col < count ? col : 0)) * dim;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const int d0 = 32 * ks + 8 * quarter;
-                kx[t][ks] = *reinterpret_cast<const bf16x8*>(at + (d0 < dim ? d0 : 0));
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    y[e] = d0 < dim && col < count ? row[d0 < dim ? d0 + e : 0] * c2 : 0.0f;
+                attention::split8(y, q[ks]);
             }
         }
+        floatx4 o[NV];
 #pragma unroll
-        for (int i = 0; i < kReads; ++i) {
-            const int j = i * kRows + v_lane;
-            const Bf16* at = v + int64_t(__shfl(r, j < kTilePositions ? j : 0)) * pitch;
-            vx[i] = *reinterpret_cast<const uintx4*>(at + (v_d0 < dim ? v_d0 : 0));
-        }
-    };
-    char* const mine = lds[wave];
-    const int first = begin + wave * kTilePositions;
-    if (first < end) load(first);
-    for (int p0 = first; p0 < end; p0 += kPagedWaves * kTilePositions) {
-        const bool tail = p0 + kTilePositions > end;
+        for (int i = 0; i < NV; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+
+        const Bf16* const k = static_cast<const Bf16*>(a.c.k) + int64_t(kv) * dim;
+        const Bf16* const v = static_cast<const Bf16*>(a.c.v) + int64_t(kv) * dim;
+        const int64_t pitch = int64_t(kv_heads) * dim;
+        bf16x8 kx[2][KS];
+        uintx4 vx[kReads];
+        const int v_lane = lane / LANES, v_d0 = lane % LANES * 8;
+        const auto load = [&](int p0) {
+            const int p = p0 + (lane & 31);
+            int64_t row = 0;
+            if (p < end) {
+                row = pool_row(a.c, s, p);
+                if (row < 0) {
+                    bad = true;
+                    row = 0;
+                }
+            }
+            const int r = int(row);
 #pragma unroll
-        for (int i = 0; i < kReads; ++i) {
-            const int j = i * kRows + v_lane;
-            uintx4 y = vx[i];
-            if (tail && p0 + j >= end) y = uintx4{0, 0, 0, 0};  // nothing, whatever is there
-            if (v_lane < kRows && j < kTilePositions)
-                *reinterpret_cast<uintx4*>(mine + j * kPitch + 2 * v_d0) = y;
-        }
-        floatx4 sc[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            sc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int part = 2; part >= 0; --part)
+            for (int t = 0; t < 2; ++t) {
+                const Bf16* at = k + int64_t(__shfl(r, 16 * t + col)) * pitch;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
-                    // Past the row's end q is 0 and K something else, which has to be finite.
-                    bf16x8 f = kx[t][ks];
-                    if (DP != dim && 32 * ks + 8 * quarter >= dim)
-                        f = __builtin_bit_cast(bf16x8, uintx4{0, 0, 0, 0});
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][part], sc[t], 0, 0, 0);
+                    const int d0 = 32 * ks + 8 * quarter;
+                    kx[t][ks] = *reinterpret_cast<const bf16x8*>(at + (d0 < dim ? d0 : 0));
                 }
-        }
-        if (p0 + kPagedWaves * kTilePositions < end) load(p0 + kPagedWaves * kTilePositions);
-        if (tail) {
+            }
+#pragma unroll
+            for (int i = 0; i < kReads; ++i) {
+                const int j = i * kRows + v_lane;
+                const Bf16* at = v + int64_t(__shfl(r, j < kTilePositions ? j : 0)) * pitch;
+                vx[i] = *reinterpret_cast<const uintx4*>(at + (v_d0 < dim ? v_d0 : 0));
+            }
+        };
+        char* const mine = lds[wave];
+        const int first = begin + wave * kTilePositions;
+        if (first < end) load(first);
+        for (int p0 = first; p0 < end; p0 += kPagedWaves * kTilePositions) {
+            const bool tail = p0 + kTilePositions > end;
+#pragma unroll
+            for (int i = 0; i < kReads; ++i) {
+                const int j = i * kRows + v_lane;
+                uintx4 y = vx[i];
+                if (tail && p0 + j >= end) y = uintx4{0, 0, 0, 0};  // nothing, whatever is there
+                if (v_lane < kRows && j < kTilePositions)
+                    *reinterpret_cast<uintx4*>(mine + j * kPitch + 2 * v_d0) = y;
+            }
+            floatx4 sc[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                sc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int part = 2; part >= 0; --part)
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        // Past the row's end q is 0 and K something else, which has to be finite.
+                        bf16x8 f = kx[t][ks];
+                        if (DP != dim && 32 * ks + 8 * quarter >= dim)
+                            f = __builtin_bit_cast(bf16x8, uintx4{0, 0, 0, 0});
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][part], sc[t], 0,
+                                                                        0, 0);
+                    }
+            }
+            if (p0 + kPagedWaves * kTilePositions < end) load(p0 + kPagedWaves * kTilePositions);
+            if (tail) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (p0 + 16 * t + 4 * quarter + r >= end) sc[t][r] = -INFINITY;
+            }
+            float top = m;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (p0 + 16 * t + 4 * quarter + r >= end) sc[t][r] = -INFINITY;
+                for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float shift = top == -INFINITY ? 0.0f : top;
+            const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
+            m = top;
+            float w[8], part_sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j % 4] - shift) * 0x1p-24f;
+                part_sum += w[j];
+            }
+            l = __builtin_fmaf(l, keep, part_sum);
+            bf16x8 p[3];
+            attention::split8(w, p);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                typedef __attribute__((address_space(3))) shortx4* Rows;
+                // Lane: row 4 quarter + col / 4 (and 16 rows on), values 16 i + 4 (col % 4) + 0..3.
+                const char* at = mine + (4 * quarter + col / 4) * kPitch + 32 * i + 8 * (col % 4);
+                struct {
+                    shortx4 x, y;
+                } f = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)at),
+                       __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(at + 16 * kPitch))};
+                const bf16x8 vt = __builtin_bit_cast(bf16x8, f);
+                floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int part = 2; part >= 0; --part)
+                    y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, p[part], y, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[i][r] = __builtin_fmaf(o[i][r], keep, y[r]);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
-        float top = m;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float shift = top == -INFINITY ? 0.0f : top;
-        const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
-        m = top;
-        float w[8], part_sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j % 4] - shift) * 0x1p-24f;
-            part_sum += w[j];
-        }
-        l = __builtin_fmaf(l, keep, part_sum);
-        bf16x8 p[3];
-        attention::split8(w, p);
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            typedef __attribute__((address_space(3))) shortx4* Rows;
-            // Lane: row 4 quarter + col / 4 (and 16 rows on), four values from 16 i + 4 (col % 4).
-            const char* at = mine + (4 * quarter + col / 4) * kPitch + 32 * i + 8 * (col % 4);
-            struct {
-                shortx4 x, y;
-            } f = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)at),
-                   __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(at + 16 * kPitch))};
-            const bf16x8 vt = __builtin_bit_cast(bf16x8, f);
-            floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int part = 2; part >= 0; --part)
-                y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vt, p[part], y, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[i][r] = __builtin_fmaf(o[i][r], keep, y[r]);
-        }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
-    bad = __syncthreads_or(bad);
+        bad = __syncthreads_or(bad);
 
-    // The waves of the block: sums of head `col`, value 16 i + 4 quarter + r.
-    l = with_half(with_row_pair(l));
-    if (quarter == 0) {
-        sh_m[wave][col] = m;
-        sh_l[wave][col] = l;
-    }
-    float* const sums = reinterpret_cast<float*>(mine);
-#pragma unroll
-    for (int i = 0; i < NV; ++i)
-        *reinterpret_cast<floatx4*>(sums + col * DP + 16 * i + 4 * quarter) = o[i];
-    __syncthreads();
-    for (int g = wave; g < count; g += kPagedWaves) {
-        float top = sh_m[0][g], sum = 0.0f, keep[kPagedWaves], y[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int u = 1; u < kPagedWaves; ++u) top = fmaxf(top, sh_m[u][g]);
-        bool fine = true;
-#pragma unroll
-        for (int u = 0; u < kPagedWaves; ++u) {
-            keep[u] = sh_m[u][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh_m[u][g] - top);
-            sum += sh_l[u][g] * keep[u];
-            fine = fine && fabsf(sh_l[u][g]) < INFINITY;
+        // The waves of the block: sums of head `col`, value 16 i + 4 quarter + r.
+        l = with_half(with_row_pair(l));
+        if (quarter == 0) {
+            sh_m[wave][col] = m;
+            sh_l[wave][col] = l;
         }
+        float* const sums = reinterpret_cast<float*>(mine);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int d = lane + 64 * e;
-            if (d >= dim) continue;
+        for (int i = 0; i < NV; ++i)
+            *reinterpret_cast<floatx4*>(sums + col * DP + 16 * i + 4 * quarter) = o[i];
+        __syncthreads();
+        for (int g = wave; g < count; g += kPagedWaves) {
+            float top = sh_m[0][g], sum = 0.0f, keep[kPagedWaves], y[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int u = 0; u < kPagedWaves; ++u)
-                y[e] += reinterpret_cast<const float*>(lds[u])[g * DP + d] * keep[u];
-            fine = fine && fabsf(y[e]) < INFINITY;
-        }
-        if (!bad && !(__all(fine) && sum > 0.0f))
-            part_by_formula<Bf16>(a, s, h0 + g, kv, begin, end, top, sum, y);
-        const int64_t at = int64_t(h0 + g) * (a.workers + a.c.sequences) + worker + s;
-        if (bad) sum = NAN;
-        if (lane == 0) {
-            if (!seg.whole) a.part_stats[at] = float2{top, sum};
-            else if (a.lse != nullptr) a.lse[s * a.heads + h0 + g] = lse_of(top, sum);
-        }
+            for (int u = 1; u < kPagedWaves; ++u) top = fmaxf(top, sh_m[u][g]);
+            bool fine = true;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int d = lane + 64 * e;
-            if (d >= dim) continue;
-            if (!seg.whole) a.part_out[at * dim + d] = y[e];
-            else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y[e] / sum;
+            for (int u = 0; u < kPagedWaves; ++u) {
+                keep[u] = sh_m[u][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh_m[u][g] - top);
+                sum += sh_l[u][g] * keep[u];
+                fine = fine && fabsf(sh_l[u][g]) < INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int d = lane + 64 * e;
+                if (d >= dim) continue;
+#pragma unroll
+                for (int u = 0; u < kPagedWaves; ++u)
+                    y[e] += reinterpret_cast<const float*>(lds[u])[g * DP + d] * keep[u];
+                fine = fine && fabsf(y[e]) < INFINITY;
+            }
+            if (!bad && !(__all(fine) && sum > 0.0f))
+                part_by_formula<Bf16>(a, s, h0 + g, kv, begin, end, top, sum, y);
+            const int64_t at = int64_t(h0 + g) * (a.workers + a.c.sequences) + worker + s;
+            if (bad) sum = NAN;
+            if (lane == 0) {
+                if (!seg.whole) a.part_stats[at] = float2{top, sum};
+                else if (a.lse != nullptr) a.lse[s * a.heads + h0 + g] = lse_of(top, sum);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int d = lane + 64 * e;
+                if (d >= dim) continue;
+                if (!seg.whole) a.part_out[at * dim + d] = y[e];
+                else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y[e] / sum;
+            }
         }
-    }
-    __syncthreads();
+        __syncthreads();
     }
 }
 
@@ -792,8 +796,8 @@ int check(const char* name, const ehip_cache_t* c, Cache& out) {
     return EHIP_OK;
 }
 
-// Positions count on past a length by less than that again in 32 bits; pages may repeat in a table, so
-// the pool's extent does not bound a length.
+// Positions count on past a length by less than that again in 32 bits; pages may repeat in a table,
+// so the pool's extent does not bound a length.
 constexpr int64_t kMaxLength = int64_t(1) << 30;
 
 int check_heads(const char* name, const Cache& c, int64_t heads, int64_t longest) {
@@ -807,9 +811,9 @@ int check_heads(const char* name, const Cache& c, int64_t heads, int64_t longest
     return EHIP_OK;
 }
 
-// Workers for 512 blocks in all, two a CU (64 sequences of 64 to 4096 positions in bf16: 75 us against
-// 85 with 1024 blocks and 101 with 2048; two of 131072 in fp32: 383, 388, 389), and no more than there
-// can be tiles.
+// Workers for 512 blocks in all, two a CU (64 sequences of 64 to 4096 positions in bf16: 75 us
+// against 85 with 1024 blocks and 101 with 2048; two of 131072 in fp32: 383, 388, 389), and no more
+// than there can be tiles.
 int workers_of(const Cache& c, int64_t heads, int64_t longest, int type) {
     const int64_t group = heads / c.kv_heads;
     const int64_t units = c.kv_heads * ceil_div(group, type == EHIP_CACHE_F32 ? kMaxGroup : 16);

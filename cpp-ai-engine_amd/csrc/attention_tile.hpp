@@ -27,8 +27,8 @@ typedef float floatx16 __attribute__((ext_vector_type(16)));
 // The six part products, the smallest first.
 constexpr int kPart[6][2] = {{1, 1}, {2, 0}, {0, 2}, {0, 1}, {1, 0}, {0, 0}};
 
-// Eight values in three parts, eight bf16 to a register quadruple. Unlike a product's tile they are not
-// scaled: values below 2^-110 lose what is below 2^-133.
+// Eight values in three parts, eight bf16 to a register quadruple. Unlike a product's tile they are
+// not scaled: values below 2^-110 lose what is below 2^-133.
 __device__ __forceinline__ void split8(const float* x, bf16x8 (&part)[3]) {
     uintx4 h, m, l;
 #pragma unroll
@@ -49,11 +49,11 @@ __device__ __forceinline__ void split8(const float* x, bf16x8 (&part)[3]) {
 // Left alone the compiler reads them one or two instructions ahead. Other instructions may cross.
 __device__ __forceinline__ void keep_order() { __builtin_amdgcn_sched_barrier(0x0216); }
 
-// d += the five smaller part products of two blocks of 32 x 16, or the first parts' alone. The matrix
-// instruction drops the low bits of its sums towards minus infinity: of a chain of six products a
-// block each drops as much as the first parts' do, unless those come last, when the sum is still
-// small (scores of 64 values: 4 instructions at full size in place of 24; the outputs' error against
-// 64 bits, sequences of 64 to 1537, went down by a fifth, at no cost in time).
+// d += the five smaller part products of two blocks of 32 x 16, or the first parts' alone. The
+// matrix instruction drops the low bits of its sums towards minus infinity: of a chain of six
+// products a block each drops as much as the first parts' do, unless those come last, when the sum
+// is still small (scores of 64 values: 4 instructions at full size in place of 24; the outputs'
+// error against 64 bits, sequences of 64 to 1537, went down by a fifth, at no cost in time).
 __device__ __forceinline__ void multiply_small(floatx16& d, const bf16x8 (&a)[3],
                                                const bf16x8 (&b)[3]) {
 #pragma unroll
@@ -88,7 +88,8 @@ __device__ __forceinline__ void own_row(const float* row, int dim, float factor,
         float x[8];
         if (VEC) {
             const floatx4u u = *reinterpret_cast<const floatx4u*>(row + (d0 < dim ? d0 : 0));
-            const floatx4u v = *reinterpret_cast<const floatx4u*>(row + (d0 + 4 < dim ? d0 + 4 : 0));
+            const floatx4u v =
+                *reinterpret_cast<const floatx4u*>(row + (d0 + 4 < dim ? d0 + 4 : 0));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 x[j] = d0 < dim ? u[j] * factor : 0.0f;
@@ -106,8 +107,8 @@ __device__ __forceinline__ void own_row(const float* row, int dim, float factor,
     }
 }
 
-// The product of the lane's own rows of two tensors, each of the two lanes that hold it over half of
-// the values.
+// The product of the lane's own rows of two tensors, each of the two lanes that hold it over half
+// of the values.
 template <int DP, bool VEC>
 __device__ __forceinline__ float own_dot(const float* x, const float* y, int dim) {
     const int half = (int(threadIdx.x) & 63) / 32;
@@ -153,10 +154,10 @@ __device__ __forceinline__ void store_own(float* row, int dim, int db, const flo
 // ROWS streamed rows as the A operand of products over the head's values: LDS in three planes, each
 // in blocks of 32 rows x 16 values as the instruction takes them, 1 KiB, 16 bytes a lane: a
 // conflict-free ds_read_b128. The row's place within its half block is permuted by its group of
-// eight values, so that a transposed read's eight rows of two groups fall on all banks, twice, and the
-// writes of a row's groups, which neighbouring threads hold, on no bank more than twice either; few
-// address bits depend on the lane and the block both, so few addresses are kept. A thread stages up
-// to kUnits units of one row by 8 values.
+// eight values, so that a transposed read's eight rows of two groups fall on all banks, twice, and
+// the writes of a row's groups, which neighbouring threads hold, on no bank more than twice either;
+// few address bits depend on the lane and the block both, so few addresses are kept. A thread
+// stages up to kUnits units of one row by 8 values.
 template <int ROWS, int DP, int THREADS, bool VEC>
 struct RowTile {
     static constexpr int kGroups = DP / 8;
@@ -238,9 +239,9 @@ struct RowTile {
         else store_as<false>(lds, left, dim);
     }
     // Part p of the transposed block (db, t): values 32 db .. of rows 16 t .., as the A operand of
-    // products over the rows, the rows in the order that registers 8 (t % 2) .. of a D hold them: half
-    // h of the lanes has rows 16 t + 4 h + {0..3, 8..11}. A transposed read gives sixteen lanes one
-    // value each of four rows from the sixteen places of four values that they name.
+    // products over the rows, the rows in the order that registers 8 (t % 2) .. of a D hold them:
+    // half h of the lanes has rows 16 t + 4 h + {0..3, 8..11}. A transposed read gives sixteen
+    // lanes one value each of four rows from the sixteen places of four values that they name.
     __device__ __forceinline__ static bf16x8 columns(const char* lds, int db, int t, int p) {
         typedef short shortx4 __attribute__((ext_vector_type(4)));
         typedef __attribute__((address_space(3))) shortx4* Rows;
@@ -262,8 +263,8 @@ struct RowTile {
     }
 };
 
-// s[b] = rows 32 b .. of the tile times the lane's own row: NB x 32 scores. fetch(ks) is called before
-// own[ks] is used whole.
+// s[b] = rows 32 b .. of the tile times the lane's own row: NB x 32 scores. fetch(ks) is called
+// before own[ks] is used whole.
 template <class Tile, int NB, int KS, class Fetch>
 __device__ __forceinline__ void scores(floatx16 (&s)[NB], const char* lds, bf16x8 (&own)[KS][3],
                                        Fetch fetch) {

@@ -106,8 +106,8 @@ __device__ __forceinline__ void finish_row(const RowOut& o, int64_t r, const Sum
 
 // ------------------------------------------------------------------ the top
 
-// A logit's place in the order (-0 as 0, NaN above all; 0 is none) and, with its index from above in
-// the low half, a key that no other of the row has: larger keys come first.
+// A logit's place in the order (-0 as 0, NaN above all; 0 is none) and, with its index from above
+// in the low half, a key that no other of the row has: larger keys come first.
 __device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
     const uint32_t y = b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
@@ -142,8 +142,8 @@ __device__ __forceinline__ void list_found(Top& sh, int n, int top) {
     __syncthreads();
 }
 
-// Takes the kOffer keys key(0) .. of every thread (0: none; all others differ from each other and from
-// the list's) into the list of the `top` largest. Every thread calls it.
+// Takes the kOffer keys key(0) .. of every thread (0: none; all others differ from each other and
+// from the list's) into the list of the `top` largest. Every thread calls it.
 template <class Key>
 __device__ __forceinline__ void offer(Top& sh, int top, Key key) {
     const uint64_t last = sh.list[top - 1];
@@ -156,8 +156,9 @@ __device__ __forceinline__ void offer(Top& sh, int top, Key key) {
     if (threadIdx.x == 0) sh.count = 0;
     const int threads = __syncthreads_count(largest > last);
     if (threads == 0) return;
-    // At most `top` threads hold keys of the new list. Where more of them have one above the last: the
-    // `top`-th of the threads' largest is a lower limit of the list, and as many threads reach it.
+    // At most `top` threads hold keys of the new list. Where more of them have one above the last:
+    // the `top`-th of the threads' largest is a lower limit of the list, and as many threads reach
+    // it.
     uint64_t limit = 0;
     if (threads > top) {
         // The wave's order first: only its first `top` can be among the block's.
