@@ -336,6 +336,35 @@ def test_append(hip, dtype, kv, d, page):
 
 @gpu
 @pytest.mark.parametrize("dtype", types())
+@pytest.mark.parametrize("kv,d", [(1, 30), (2, 260), (9, 135), (10, 120)])
+def test_append_to_many_sequences(hip, dtype, kv, d):
+    """More sequences than a wave has lanes, and than its square, many of them without a token; rows
+    of one wave and of four, in multiples of four values and not."""
+    import torch
+    print_case("append many", dtype, kv, d)
+    page = 4
+    for count in (65, 4200):
+        new = [(7 * s) % 4 if s % 3 else 0 for s in range(count)]
+        starts = [s % 9 for s in range(count)]
+        cu = [0]
+        for n in new:
+            cu.append(cu[-1] + n)
+        table = torch.randperm(count * 3, device="cuda").to(torch.int32).reshape(count, 3)
+        kp = torch.zeros(count * 3, page, kv, d, dtype=dtype, device="cuda")
+        vp = torch.zeros_like(kp)
+        want_k, want_v = torch.zeros_like(kp), torch.zeros_like(kp)
+        k, v = (torch.randn(cu[-1] + 2, kv, d, device="cuda") for _ in range(2))
+        hip.cache_append(k, v, kp, vp, table, ints(starts), ints(cu))
+        who = torch.repeat_interleave(torch.arange(count), torch.tensor(new))
+        at = torch.arange(cu[-1]) - torch.tensor(cu)[who] + torch.tensor(starts)[who]
+        row = table.cpu()[who, at // page].long() * page + at % page
+        for want, x in ((want_k, k), (want_v, v)):
+            want.view(-1, kv, d)[row.cuda()] = x[:cu[-1]].to(dtype)
+        assert torch.equal(kp, want_k) and torch.equal(vp, want_v), count
+
+
+@gpu
+@pytest.mark.parametrize("dtype", types())
 def test_append_one_token_each(hip, dtype):
     import torch
     print_case("append one each", dtype)
