@@ -35,6 +35,9 @@ struct Packed {
     float* out;
     int64_t ld_out;
     float* lse;
+    int pieces;          // of a tile's keys in the forward; 1: the kernel writes the results
+    float2* piece_stats;  // (total_q, heads, pieces): maximum (as 2^x), sum
+    float* piece_out;     // (total_q, heads, pieces, dim)
     const float* grad;
     int64_t ld_grad;
     float *dq, *dk, *dv;
@@ -298,6 +301,22 @@ __device__ __forceinline__ int head_of(const Packed& a, int x) {
     return x % a.kv_heads * (a.heads / a.kv_heads) + x / a.kv_heads;
 }
 
+// log of a sum of terms relative to 2^shift; ln 2 in two parts.
+__device__ __forceinline__ float lse_of(float shift, float sum) {
+    return __builtin_fmaf(shift, 0.693147182464599609375f,
+                          __builtin_fmaf(shift, -1.904654323148236017e-9f, logf(sum)));
+}
+
+// Keys of each of a tile's pieces: what a step takes at a time divides them.
+constexpr int kLeastPiece = 128;
+__device__ __forceinline__ int piece_length(const Packed& a, int keys) {
+    const int n = keys / a.pieces / 64 * 64 + 64;
+    return n > kLeastPiece ? n : kLeastPiece;
+}
+__device__ __forceinline__ int64_t piece_of(const Packed& a, int64_t row, int h, int piece) {
+    return (row * a.heads + h) * a.pieces + piece;
+}
+
 template <int DP, int BN, int WAVES, bool VEC>
 __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     constexpr int BUFFERS = WAVES / 4;
@@ -310,7 +329,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     constexpr int kParked = kPark ? WAVES * (DP / 16) * 1024 : 0;
     __shared__ __attribute__((aligned(16))) char lds[BUFFERS * kTile + kParked];
     const int h = head_of(a, int(blockIdx.x % a.heads));
-    const Tile t = block_tile(a, false, int(blockIdx.x / a.heads), 32 * WAVES);
+    const int slot = int(blockIdx.x / a.heads), piece = slot % a.pieces;
+    const Tile t = block_tile(a, false, slot / a.pieces, 32 * WAVES);
     if (t.rows == 0) return;
     const int c = h / (a.heads / a.kv_heads);
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
@@ -319,8 +339,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     const int i = t.first + (mine < t.rows ? mine : t.rows - 1);
     const int limit = visible(a, t, i);
     const int last = 32 * wave + 31 < t.rows ? 32 * wave + 31 : t.rows - 1;
-    const int end = visible(a, t, t.first + t.rows - 1);
-    const int wave_end = 32 * wave < t.rows ? visible(a, t, t.first + last) : 0;
+    // The block's keys.
+    const int tile_end = visible(a, t, t.first + t.rows - 1);
+    const int begin = piece * piece_length(a, tile_end);
+    const int end = a.pieces == 1 ? tile_end
+                                  : int(min(int64_t(begin) + piece_length(a, tile_end),
+                                            int64_t(tile_end)));
+    if (begin > 0 && begin >= end) {
+        if (mine < t.rows && lane < 32)
+            a.piece_stats[piece_of(a, t.q0 + i, h, piece)] = float2{-INFINITY, 0.0f};
+        return;
+    }
+    const int wave_end = 32 * wave < t.rows ? min(visible(a, t, t.first + last), end) : 0;
     const int wave_all = visible(a, t, t.first + 32 * wave);  // keys that all its queries see
 
     // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q.
@@ -355,11 +385,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
         kt.store(at, t.nk - j, a.dim);
         vt.store(at + KeyTile::kBytes, t.nk - j, a.dim);
     };
-    load(0);
-    stage(0);
-    load(BN);
+    load(begin);
+    stage(begin);
+    load(begin + BN);
     __syncthreads();
-    for (int j0 = 0; j0 < end; j0 += BN) {
+    for (int j0 = begin; j0 < end; j0 += BN) {
         // One wave of a SIMD stages the next tile before its products, the other one after them:
         // one's conversions run beside the other's matrix instructions.
         const char* const lds_k = lds + j0 / BN % BUFFERS * kTile;
@@ -419,9 +449,20 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
         __syncthreads();
     }
 
+    sum += __shfl_xor(sum, 32);
+    if (a.pieces > 1) {
+        const int64_t at = piece_of(a, t.q0 + i, h, piece);
+        if (mine < t.rows) {
+#pragma unroll
+            for (int db = 0; db < DP / 32; ++db)
+                store_own<VEC>(a.piece_out + at * a.dim, a.dim, db, o[db]);
+            if (lane < 32)
+                a.piece_stats[at] = float2{top == -INFINITY ? -INFINITY : shift, sum};
+        }
+        return;
+    }
     // Rows that saw something and have no finite result are formed again by the formula: a NaN or
     // an infinity where it counts, or one in a place of theirs that they do not see (0 times it).
-    sum += __shfl_xor(sum, 32);
     const float inv = limit > 0 ? 1.0f / sum : 0.0f;
     bool fine = sum > 0.0f && sum < INFINITY;
 #pragma unroll
@@ -437,16 +478,64 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
         float* out = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) store_own<VEC>(out, a.dim, db, o[db]);
-        // shift ln 2 in two parts: ln 2 = hi + lo.
         if (lane < 32)
             a.lse[int64_t(t.q0 + i) * a.heads + h] =
                 limit == 0 ? -INFINITY
-                           : __builtin_fmaf(shift, 0.693147182464599609375f,
-                                            __builtin_fmaf(shift, -1.904654323148236017e-9f,
-                                                           logf(sum)));
+                           : lse_of(shift, sum);
     }
     for (uint32_t rows = uint32_t(again) | uint32_t(again >> 32); rows != 0; rows &= rows - 1)
         forward_row(a, t, h, t.first + 32 * wave + __builtin_ctz(rows));
+}
+
+// The rows' pieces. One wave a row and head, two values a lane.
+__global__ __launch_bounds__(kThreads) void packed_forward_join(Packed a) {
+    const int lane = int(threadIdx.x) & 63;
+    const int64_t at = __builtin_amdgcn_readfirstlane(
+        int(blockIdx.x) * (kThreads / 64) + int(threadIdx.x) / 64);
+    const int row = int(at / a.heads), h = int(at % a.heads);
+    if (row < offset_at(a.cu_q, 0, a.total_q) ||
+        row >= offset_at(a.cu_q, a.sequences, a.total_q))
+        return;
+    const float2* const stats = a.piece_stats + at * a.pieces;
+    float top = -INFINITY;
+    for (int n = 0; n < a.pieces; ++n) top = fmaxf(top, stats[n].x);
+    float sum = 0.0f, o[2] = {0.0f, 0.0f};
+    for (int n = 0; n < a.pieces; ++n) {
+        const float2 x = stats[n];
+        if (x.x == -INFINITY && x.y == 0.0f) continue;  // saw nothing
+        const float keep = __builtin_amdgcn_exp2f(x.x - top);
+        const float* const values = a.piece_out + (at * a.pieces + n) * a.dim;
+        sum = __builtin_fmaf(x.y, keep, sum);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (lane + 64 * e < a.dim) o[e] = __builtin_fmaf(values[lane + 64 * e], keep, o[e]);
+    }
+    const float inv = 1.0f / sum;
+    bool fine = sum > 0.0f && sum < INFINITY;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        o[e] *= inv;
+        fine = fine && fabsf(o[e]) < INFINITY;
+    }
+    if (__all(fine)) {
+        float* const out = a.out + row * a.ld_out + int64_t(h) * a.dim;
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (lane + 64 * e < a.dim) out[lane + 64 * e] = o[e];
+        if (lane == 0) a.lse[at] = lse_of(top, sum);
+        return;
+    }
+    // A row that saw nothing, or not finite: by the formula, in its sequence, the last that begins
+    // at or before it.
+    int lo = 0, n = a.sequences;
+    while (n > 1) {
+        const int mid = lo + n / 2;
+        const bool in = offset_at(a.cu_q, mid, a.total_q) <= row;
+        lo = in ? mid : lo;
+        n = in ? n - n / 2 : n / 2;
+    }
+    const Tile t = tile_of(a, false, lo, 0, kRows);
+    if (row - t.q0 < t.nq) forward_row(a, t, h, row - t.q0);
 }
 
 // The backward forms s, and so p_ij, again from the inputs, and dp likewise, for the pairs of a
@@ -982,26 +1071,59 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
 
 template <int DP, int BN, int WAVES, bool VEC>
 int launch_forward(const Packed& a, hipStream_t s) {
-    const unsigned blocks = unsigned(slots(a.total_q, a.sequences, 32 * WAVES) * a.heads);
+    const unsigned blocks =
+        unsigned(slots(a.total_q, a.sequences, 32 * WAVES) * a.heads * a.pieces);
     EHIP_LAUNCH("attention_packed", (packed_forward<DP, BN, WAVES, VEC>), dim3(blocks),
                 dim3(64 * WAVES), 0, s, a);
+    if (a.pieces > 1)
+        EHIP_LAUNCH("attention_packed_join", packed_forward_join,
+                    dim3(unsigned(ceil_div(int64_t(a.total_q) * a.heads, kThreads / 64))),
+                    dim3(kThreads), 0, s, a);
     return EHIP_OK;
+}
+
+// 256 queries a block convert their keys once and read them by turns of two tiles; 128 leave
+// less between the last block and the others. Without the causal mask all blocks of a sequence
+// are alike, and 256 it is once they fill the card (us, 128 : 256 queries, heads of 64 values:
+// one of 4096, 16 heads, 341 : 326, with 8 heads 216 : 275). With it, long sequences that fill
+// the card twice over (4 of 2048, 16 heads, 207 : 200; 24 of 64 to 1291 147 : 169; one of 8192,
+// 8 heads, 490 : 566). Heads over 96 values spill with 128, and take them for short causal ones
+// alone (64 of 128 87 : 103; one of 4096 593 : 509; without the mask 64 of 128 136 : 82).
+bool narrow_blocks(const Packed& a) {
+    const int64_t n = a.total_q, s_count = a.sequences, blocks = n / 256 * a.heads;
+    return a.dim > 96 ? a.causal && n < 256 * s_count
+           : a.causal ? n < 2048 * s_count || blocks < 512
+                      : blocks < 256;
+}
+
+// Pieces of a tile's keys, where the tiles alone leave CUs without work: for 512 blocks in all, or
+// 1024 of those of 128 queries where a causal mask leaves them uneven and the tiles make 256 (us,
+// heads of 64: one of 2048, 8 heads, whole 107, for 512 53, for 1024 63; one of 4096 212, 145, 125;
+// heads of 128: 128 queries behind 16384 keys 2049, 105; one of 4096, 8 heads, 525, 216, 271), of
+// 128 keys or more (8 of 64 to 946, heads of 128, 127 whole and with 256 or more, 82 with 128).
+// Sequences that are shorter do not make up for the second launch (4 of 256, 4 heads of 64, 18.6
+// whole, 21.2 in two).
+int pieces_of(const Packed& a) {
+    const int64_t mean = a.sequences == 0 ? 0 : a.total_k / a.sequences;
+    if (mean < 384) return 1;
+    const bool narrow = narrow_blocks(a);
+    const int64_t blocks = slots(a.total_q, a.sequences, narrow ? 128 : 256) * a.heads;
+    const int64_t want = narrow && a.causal && blocks >= 256 ? 1024 : 512;
+    const int64_t most = std::min<int64_t>(mean / kLeastPiece, 32);
+    return int(std::max<int64_t>(1, std::min((want + blocks / 2) / blocks, most)));
+}
+
+size_t piece_bytes(const Packed& a) {
+    const int pieces = pieces_of(a);
+    return pieces == 1 ? 0
+                       : size_t(a.total_q) * size_t(a.heads) * size_t(pieces) *
+                             (sizeof(float2) + size_t(a.dim) * sizeof(float));
 }
 
 template <int DP, int BN, bool VEC>
 int forward_of(const Packed& a, hipStream_t s) {
-    // 256 queries a block convert their keys once and read them by turns of two tiles; 128 leave
-    // less between the last block and the others. Without the causal mask all blocks of a sequence
-    // are alike, and 256 it is once they fill the card (us, 128 : 256 queries, heads of 64 values:
-    // one of 4096, 16 heads, 341 : 326, with 8 heads 216 : 275). With it, long sequences that fill
-    // the card twice over (4 of 2048, 16 heads, 207 : 200; 24 of 64 to 1291 147 : 169; one of 8192,
-    // 8 heads, 490 : 566). Heads over 96 values spill with 128, and take them for short causal ones
-    // alone (64 of 128 87 : 103; one of 4096 593 : 509; without the mask 64 of 128 136 : 82).
-    const int64_t n = a.total_q, s_count = a.sequences, blocks = n / 256 * a.heads;
-    const bool four = DP > 96   ? a.causal && n < 256 * s_count
-                      : a.causal ? n < 2048 * s_count || blocks < 512
-                                 : blocks < 256;
-    return four ? launch_forward<DP, BN, 4, VEC>(a, s) : launch_forward<DP, BN, 8, VEC>(a, s);
+    return narrow_blocks(a) ? launch_forward<DP, BN, 4, VEC>(a, s)
+                            : launch_forward<DP, BN, 8, VEC>(a, s);
 }
 
 // dk and dv of grouped heads are formed head by head, for as many blocks as the queries have, and
@@ -1047,11 +1169,26 @@ using namespace ehip;
 
 extern "C" {
 
-int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* stream) {
+int64_t ehip_attention_packed_workspace(const ehip_attention_packed_t* desc) {
+    Packed a;
+    if (fill("attention_packed", desc, a)) return -1;
+    return int64_t(piece_bytes(a));
+}
+
+int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* workspace,
+                              size_t workspace_bytes, void* stream) {
     EHIP_READY();
     Packed a;
     if (int rc = fill("attention_packed", desc, a)) return rc;
     if (a.sequences == 0 || a.total_q == 0) return EHIP_OK;
+    const size_t need = piece_bytes(a);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
+        return fail(EHIP_EINVAL, "attention_packed: needs %zu bytes of 16-byte aligned workspace",
+                    need);
+    a.pieces = pieces_of(a);
+    a.piece_stats = static_cast<float2*>(workspace);
+    a.piece_out = reinterpret_cast<float*>(
+        a.piece_stats + int64_t(a.total_q) * a.heads * a.pieces);
     const bool vec = a.dim % 4 == 0;
     if (a.dim <= 32) return vec ? forward_of<32, 64, true>(a, as_stream(stream))
                                 : forward_of<32, 64, false>(a, as_stream(stream));

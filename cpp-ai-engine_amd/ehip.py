@@ -197,7 +197,8 @@ _SIGS = {
     "ehip_cross_entropy_fused_supported": [_i64, _i64],
     "ehip_cross_entropy_fused_f32": [_vp] * 5 + [_i64, _i64, _vp],
     "ehip_softmax_xent_backward_f32": [_vp, _vp, _vp, _i64, _i64, _vp, _vp],
-    "ehip_attention_packed_f32": [C.POINTER(AttentionPacked), _vp],
+    "ehip_attention_packed_workspace": [C.POINTER(AttentionPacked)],
+    "ehip_attention_packed_f32": [C.POINTER(AttentionPacked), _vp, _sz, _vp],
     "ehip_attention_packed_backward_workspace": [C.POINTER(AttentionPacked)],
     "ehip_attention_packed_backward_f32": [C.POINTER(AttentionPacked)] + [_vp, _i64] * 4 +
                                           [_vp, _sz, _vp],
@@ -212,6 +213,7 @@ _SIGS = {
     "ehip_last_error": [],
 }
 _RESTYPES = {"ehip_last_error": C.c_char_p,
+             "ehip_attention_packed_workspace": C.c_int64,
              "ehip_attention_packed_backward_workspace": C.c_int64,
              "ehip_attention_paged_workspace": C.c_int64,
              "ehip_token_logprobs_workspace": C.c_int64, "ehip_kernels_launched": C.c_uint64,
@@ -846,7 +848,9 @@ class Backend:
         out = self.f32(q.shape) if out is None else out
         lse = self.f32(q.shape[:2]) if lse is None else lse
         desc = self._packed(q, k, v, cu_q, cu_k, scale, causal, out, lse)
-        self.ok(self.lib.ehip_attention_packed_f32(C.byref(desc), self.stream()),
+        need = self.lib.ehip_attention_packed_workspace(C.byref(desc))
+        space, at, n = self._workspace(need, "attention_packed")
+        self.ok(self.lib.ehip_attention_packed_f32(C.byref(desc), at, n, self.stream()),
                 "attention_packed")
         return out, lse
 

@@ -932,8 +932,14 @@ typedef struct {
     float* lse; /* likewise */
 } ehip_attention_packed_t;
 
-int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* stream);
-/* Bytes of workspace; -1 (with the error recorded) for a refused descriptor. */
+/* `workspace` (device memory, 16-byte aligned) holds the parts of rows whose
+ * keys are split over workgroups during the call: at least
+ * ehip_attention_packed_workspace() bytes, of the call's own (NULL where that is
+ * 0). Both queries: bytes; -1 (with the error recorded) for a refused
+ * descriptor. */
+int64_t ehip_attention_packed_workspace(const ehip_attention_packed_t* desc);
+int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* workspace,
+                              size_t workspace_bytes, void* stream);
 int64_t ehip_attention_packed_backward_workspace(const ehip_attention_packed_t* desc);
 int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, const float* grad,
                                        int64_t ld_grad, float* dq, int64_t ld_dq, float* dk,

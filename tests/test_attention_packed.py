@@ -330,6 +330,114 @@ def test_captured_and_replayed(hip):
                 assert torch.equal(x, y)
 
 
+# ------------------------------------------ few rows of many keys: split and joined
+# The join adds a rounding for each of up to 32 pieces and a factor within 4 u for each, less than the
+# sums over the 384 keys or more that the bounds count one by one.
+
+def splits(hip, *args, **kw):
+    """attention_packed, and whether it took a second launch."""
+    before = hip.launched()
+    out = hip.attention_packed(*args, **kw)
+    return out, hip.launched() - before == 2
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("nq,nk,heads,kv,d", [
+    ([16], [2000], 2, 1, 64), ([130], [1027], 1, 1, 128), ([300], [900], 4, 2, 33),
+    ([700], [700], 3, 3, 96), ([1, 0, 260, 5], [1000, 900, 390, 64], 2, 1, 32),
+    ([600], [450], 2, 2, 100), ([1], [4000], 8, 1, 80), ([511, 2], [511, 513], 1, 1, 17)])
+def test_split_keys(hip, nq, nk, heads, kv, d, causal):
+    import torch
+    print_case("packed split", nq, nk, heads, kv, d, causal)
+    q, k, v, _ = make(nq, nk, heads, kv, d, seed=sum(nk) + d)
+    (out, lse), split = splits(hip, q, k, v, offsets(nq), offsets(nk), causal=causal)
+    assert split
+    value, bound = packed(q, k, v, nq, nk, d ** -0.5, causal)
+    within(out, value["out"], bound["out"], "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+    again = hip.attention_packed(q, k, v, offsets(nq), offsets(nk), causal=causal)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+@gpu
+def test_split_keys_not_finite_not_seen_and_past_the_last_sequence(hip):
+    import torch
+    print_case("packed split special")
+    nq, nk, tail = [100, 50], [1000, 700], 9
+    q, k, v, _ = make(nq, nk, 2, 1, 64, seed=31, tail=tail)
+    q = q.abs() + 0.5
+    k[:1000, 0, 3][::2] = -math.inf          # weighs nothing
+    k[940:960], v[940:960] = math.nan, math.inf  # sequence 0: rows 40.. see them, rows 0..39 do not
+    v[1000 + 20, 0, 5] = math.inf            # sequence 1: all rows see it
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    _, split = splits(hip, q, k, v, cq, ck, out=out, lse=lse)
+    assert split
+    assert bool((out[150:] == 7.0).all()) and bool((lse[150:] == 7.0).all())
+    assert bool(torch.isnan(out[40:100]).all()) and bool(torch.isnan(lse[40:100]).all())
+    assert bool((out[100:150, :, 5] == math.inf).all())
+    for i in (0, 7, 39):
+        seen = [j for j in range(900 + i + 1) if j % 2]
+        value, bound = packed(q[i:i + 1], k[seen], v[seen], [1], [len(seen)], 0.125, False)
+        # The bound's sums run over the positions that weigh nothing too.
+        within(out[i:i + 1], value["out"], 2.5 * bound["out"], "out")
+        within(lse[i:i + 1], value["lse"], 2.5 * bound["lse"], "lse")
+    vz = v.clone()
+    vz[1000 + 20, 0, 5] = 0
+    value, bound = packed(q[100:150], k[1000:1700], vz[1000:1700], [50], [700], 0.125, True)
+    others = [c for c in range(64) if c != 5]
+    within(out[100:150][..., others], value["out"][..., others], bound["out"][..., others], "out")
+    within(lse[100:150], value["lse"], bound["lse"], "lse")
+
+
+@gpu
+def test_split_rows_without_keys_and_with_nothing_but_minus_infinity(hip):
+    import torch
+    print_case("packed split empty")
+    q, k, v, _ = make([500], [400], 1, 1, 32, seed=33)
+    q = q.abs() + 0.5
+    k[:130, 0, 1] = -math.inf                # all that rows 100..229 see
+    (out, lse), split = splits(hip, q, k, v, offsets([500]), offsets([400]))
+    assert split
+    assert bool((out[:100] == 0).all()) and bool((lse[:230] == -math.inf).all())
+    assert bool(torch.isnan(out[100:230]).all())
+    value, bound = packed(q[230:], k[130:], v[130:], [270], [270], 32 ** -0.5, True)
+    # The bound's sums run over the positions that weigh nothing too.
+    factor = 400 / 270 + 1
+    within(out[230:], value["out"], factor * bound["out"], "out")
+    within(lse[230:], value["lse"], factor * bound["lse"], "lse")
+
+
+@gpu
+def test_split_keys_captured_and_replayed(hip):
+    import torch
+    print_case("packed split graph")
+    nq, nk = [40, 33], [1500, 600]
+    q, k, v, _ = make(nq, nk, 4, 2, 64, seed=34)
+    cq, ck = offsets(nq), offsets(nk)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        hip.attention_packed(q, k, v, cq, ck)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):  # each with a workspace of its own
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = hip.attention_packed(q, k, v, cq, ck)
+        graphs.append((graph, out))
+    for seed in range(3):
+        for t, f in zip((q, k, v), make(nq, nk, 4, 2, 64, seed=40 + seed)):
+            t.copy_(f)
+        want, split = splits(hip, q, k, v, cq, ck)
+        assert split
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
 @gpu
 def test_offsets_out_of_range_stay_inside_the_tensors(hip):
     """Negative, descending and too large offsets are clamped: rows around the tensors stay."""
@@ -398,6 +506,11 @@ def test_workspace_and_refused_descriptors():
                 dict(ld_k=2 ** 22 + 1), dict(ld_v=2 ** 22 + 1)):
         assert size(C.byref(descriptor(**bad))) == -1, bad
         assert b"attention_packed" in lib.ehip_last_error()
+        assert lib.ehip_attention_packed_workspace(C.byref(descriptor(**bad))) == -1, bad
+    forward = lib.ehip_attention_packed_workspace
+    assert forward(C.byref(descriptor())) == 0  # few keys
+    assert forward(C.byref(descriptor(total_k=9000))) >= 10 * 4 * (16 + 2) * 4 * 2
+    assert forward(C.byref(descriptor(sequences=0, total_q=0, q=None, cu_q=None, cu_k=None))) == 0
 
 
 def binding():
@@ -453,4 +566,11 @@ def test_calls_are_refused(hip):
         hip.stream())
     assert call(None, 0) == 1 and call(space.data_ptr(), 31) == 1
     assert call(space.data_ptr() + 4, 64) == 1 and "workspace" in hip.error()
+    q, k, v, _ = make([4], [900], 2, 1, 16, seed=1)
+    desc = hip._packed(q, k, v, offsets([4]), offsets([900]), None, True, out, lse)
+    need = hip.lib.ehip_attention_packed_workspace(C.byref(desc))
+    space = torch.empty(need, device="cuda")
+    call = lambda at, n: hip.lib.ehip_attention_packed_f32(C.byref(desc), at, n, hip.stream())
+    assert need > 0 and call(None, 0) == 1 and call(space.data_ptr(), need - 1) == 1
+    assert call(space.data_ptr() + 4, need) == 1 and "workspace" in hip.error()
     assert hip.launched() == launched
