@@ -1027,7 +1027,7 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
                     "%s: %lld sequences, %lld and %lld rows, %lld heads over %lld of %lld values",
                     name, (long long)d->sequences, (long long)d->total_q, (long long)d->total_k,
                     (long long)d->heads, (long long)d->kv_heads, (long long)d->head_dim);
-    constexpr int64_t kBlocks = (int64_t(1) << 24) - 1;
+    constexpr int64_t kBlocks = (int64_t(1) << 23) - 1;  // of 512 threads, 2^32 in all at most
     if (d->heads > kBlocks || d->sequences > kBlocks || d->total_q > INT32_MAX ||
         d->total_k > INT32_MAX ||
         slots(d->total_q > d->total_k ? d->total_q : d->total_k, d->sequences) * d->heads > kBlocks)

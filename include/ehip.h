@@ -901,8 +901,9 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  * queries of a fused projection are read and their gradient written in place);
  * k, v, dk, dv rows of kv_heads * head_dim; lse is (total_q, heads), dense.
  * Any alignment of a float; ld_q, ld_k, ld_v and ld_grad at most 2^22.
- * 1 <= head_dim <= 128; heads a multiple of kv_heads; at most 2^24 - 1 blocks
- * of 128 rows and a head (else EHIP_EINVAL). Values keep 24 bits from 2^-110
+ * 1 <= head_dim <= 128; heads a multiple of kv_heads; at most 2^23 - 1 blocks
+ * of 128 rows and a head, one more than it needs for each sequence (else
+ * EHIP_EINVAL). Values keep 24 bits from 2^-110
  * on, smaller ones what is above 2^-133.
  * Offsets out of range or descending are clamped, so nothing is read or
  * written outside the tensors, but what the sequences they touch get is

@@ -513,6 +513,13 @@ def test_workspace_and_refused_descriptors():
     assert forward(C.byref(descriptor(sequences=0, total_q=0, q=None, cu_q=None, cu_k=None))) == 0
 
 
+def test_blocks_fit_a_launch():
+    """2^32 threads: blocks of 512, so 2^23 - 1 of them."""
+    size = E.load_library().ehip_attention_packed_backward_workspace
+    assert size(C.byref(descriptor(sequences=2 ** 21 - 2))) >= 0
+    assert size(C.byref(descriptor(sequences=2 ** 21))) == -1
+
+
 def binding():
     """A Backend without a device: its argument checks only."""
     import torch
