@@ -168,6 +168,29 @@ def test_ties_go_to_the_lowest_index(hip, vocab):
 
 
 @gpu
+@pytest.mark.parametrize("top", [3, 50])
+def test_tops_of_rows_in_one_block(hip, top):
+    """Segments that come after the list is full: better ones at the end, none, a NaN or +inf in the
+    second or the last, thousands of equal ones, little but -inf."""
+    import torch
+    print_case("logprobs one block", top)
+    x, t, _, _ = make(520, 20001, seed=top)
+    x[0].copy_(torch.arange(20001, device="cuda") / 64)
+    x[1].copy_(torch.arange(20001, device="cuda").flip(0) / 64)
+    x[2, 9000], x[2, 20000] = math.nan, 50.0
+    x[3, 20000], x[3, 8191] = math.nan, math.inf
+    x[4, 8192:] = 4.0
+    x[5] = -math.inf
+    x[5, 17000:17002] = 1.0
+    x[6] = -math.inf
+    x[6, ::977] = torch.randn(21, device="cuda")
+    x[7, :8192] = -3.0e38
+    index = hip.token_logprobs(x, t, top=top)[4]
+    assert torch.equal(index[:12].cpu(), best(x[:12], top))
+    assert torch.equal(index[500:520].cpu(), best(x[500:], top))
+
+
+@gpu
 @pytest.mark.parametrize("vocab", [130, 2000, 33001])
 def test_masked_and_extreme_logits(hip, vocab):
     """-inf beside others, the lowest float as a mask, one token left, logits of 1e4 and 1e30."""
