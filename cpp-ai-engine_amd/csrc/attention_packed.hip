@@ -490,25 +490,43 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
 // The rows' pieces. One wave a row and head, two values a lane.
 __global__ __launch_bounds__(kThreads) void packed_forward_join(Packed a) {
     const int lane = int(threadIdx.x) & 63;
-    const int64_t at = __builtin_amdgcn_readfirstlane(
+    const int n_row = __builtin_amdgcn_readfirstlane(
         int(blockIdx.x) * (kThreads / 64) + int(threadIdx.x) / 64);
-    const int row = int(at / a.heads), h = int(at % a.heads);
+    const int row = n_row / a.heads, h = n_row - row * a.heads;
+    const int64_t at = n_row;
     if (row < offset_at(a.cu_q, 0, a.total_q) ||
         row >= offset_at(a.cu_q, a.sequences, a.total_q))
         return;
-    const float2* const stats = a.piece_stats + at * a.pieces;
-    float top = -INFINITY;
-    for (int n = 0; n < a.pieces; ++n) top = fmaxf(top, stats[n].x);
-    float sum = 0.0f, o[2] = {0.0f, 0.0f};
-    for (int n = 0; n < a.pieces; ++n) {
-        const float2 x = stats[n];
-        if (x.x == -INFINITY && x.y == 0.0f) continue;  // saw nothing
-        const float keep = __builtin_amdgcn_exp2f(x.x - top);
-        const float* const values = a.piece_out + (at * a.pieces + n) * a.dim;
-        sum = __builtin_fmaf(x.y, keep, sum);
+    // A lane has a piece's statistics, and then two values of every piece, four pieces asked for at a
+    // time; those that saw nothing left none.
+    const float2 x = lane < a.pieces ? a.piece_stats[at * a.pieces + lane]
+                                     : float2{-INFINITY, 0.0f};
+    const float top = wave_max(x.x);
+    const bool saw = x.x != -INFINITY || x.y != 0.0f;
+    const float mine = saw ? __builtin_amdgcn_exp2f(x.x - top) : 0.0f;
+    const float sum = wave_sum(saw ? x.y * mine : 0.0f);
+    const uint64_t seen = __ballot(saw);
+    const float* const values = a.piece_out + at * a.pieces * a.dim;
+    float o[2] = {0.0f, 0.0f};
+    for (int n0 = 0; n0 < a.pieces; n0 += 4) {
+        float y[4][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-            if (lane + 64 * e < a.dim) o[e] = __builtin_fmaf(values[lane + 64 * e], keep, o[e]);
+        for (int u = 0; u < 4; ++u) {
+            const int n = n0 + u < a.pieces ? n0 + u : 0;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int d = lane + 64 * e;
+                y[u][e] = values[int64_t(n) * a.dim + (d < a.dim ? d : 0)];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int n = n0 + u;
+            const float keep = __shfl(mine, n & 63);
+            if (n >= a.pieces || !(seen >> n & 1)) continue;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) o[e] = __builtin_fmaf(y[u][e], keep, o[e]);
+        }
     }
     const float inv = 1.0f / sum;
     bool fine = sum > 0.0f && sum < INFINITY;
