@@ -43,7 +43,11 @@ struct Packed {
     float *dq, *dk, *dv;
     int64_t ld_dq, ld_dk, ld_dv;
     float* delta;             // (total_q, heads)
-    float *part_k, *part_v;  // (total_k, heads, dim): each query head's share, or null
+    // Shares of the gradients: of a piece of the keys or queries that a block passes, and for dk
+    // and dv of a query head; or null.
+    int pieces_q, pieces_k;
+    float* part_q;            // (total_q, heads, pieces_q, dim)
+    float *part_k, *part_v;  // (total_k, heads, pieces_k, dim)
 };
 
 // A sequence's rows and the block's tile of them; rows == 0 where the block has none.
@@ -153,6 +157,22 @@ __device__ __forceinline__ int visible(const Packed& a, const Tile& t, int i) {
     return n < 0 ? 0 : (n > t.nk ? t.nk : int(n));
 }
 
+// Rows of each of so many pieces of n: what a step takes at a time divides them.
+constexpr int kLeastPiece = 128;
+__device__ __forceinline__ int piece_length(int n, int pieces) {
+    const int each = n / pieces / 64 * 64 + 64;
+    return each > kLeastPiece ? each : kLeastPiece;
+}
+
+// Piece `piece` of rows [first, end): its first row (end if it is empty), and the row after its
+// last.
+__device__ __forceinline__ void take_piece(int piece, int pieces, int& first, int& end) {
+    if (pieces == 1) return;
+    const int64_t each = piece_length(end - first, pieces), begin = first + piece * each;
+    first = int(min(begin, int64_t(end)));
+    end = int(min(begin + each, int64_t(end)));
+}
+
 __device__ __forceinline__ float wave_max(float x) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
@@ -223,9 +243,11 @@ __device__ __forceinline__ float pair_gradient(const Packed& a, const float* q, 
     return p * (dot(g, v, a.dim) - delta);
 }
 
-__device__ void dq_row(const Packed& a, const Tile& t, int h, int i, float delta) {
+// Of keys [begin, end).
+__device__ void dq_row(const Packed& a, const Tile& t, int h, int i, float delta, int begin,
+                       int end, float* dq) {
     const int lane = int(threadIdx.x) & 63;
-    const int n = visible(a, t, i), c = h / (a.heads / a.kv_heads);
+    const int n = min(visible(a, t, i), end), c = h / (a.heads / a.kv_heads);
     const int64_t row = t.q0 + i;
     const float* q = a.q + row * a.ld_q + int64_t(h) * a.dim;
     const float* g = a.grad + row * a.ld_grad + int64_t(h) * a.dim;
@@ -233,7 +255,7 @@ __device__ void dq_row(const Packed& a, const Tile& t, int h, int i, float delta
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
     const float lse = a.lse[row * a.heads + h];
     float acc[2] = {0.0f, 0.0f};
-    for (int j0 = 0; j0 < n; j0 += 64) {
+    for (int j0 = begin; j0 < n; j0 += 64) {
         const int j = j0 + lane;
         float p, ds = 0.0f;
         if (j < n) ds = pair_gradient(a, q, g, k + j * a.ld_k, v + j * a.ld_v, lse, delta, p);
@@ -246,14 +268,15 @@ __device__ void dq_row(const Packed& a, const Tile& t, int h, int i, float delta
                 if (lane + 64 * e < a.dim) acc[e] = __builtin_fmaf(w, x[lane + 64 * e], acc[e]);
         }
     }
-    float* dq = a.dq + row * a.ld_dq + int64_t(h) * a.dim;
 #pragma unroll
     for (int e = 0; e < 2; ++e)
         if (lane + 64 * e < a.dim) dq[lane + 64 * e] = acc[e] * a.scale;
 }
 
-// Query head h's share, into rows dk and dv of `dim` values (either may be null).
-__device__ void dkv_row(const Packed& a, const Tile& t, int h, int j, float* dk, float* dv) {
+// Query head h's share of queries [begin, end), into rows dk and dv of `dim` values (either may be
+// null).
+__device__ void dkv_row(const Packed& a, const Tile& t, int h, int j, int begin, int end, float* dk,
+                        float* dv) {
     const int c = h / (a.heads / a.kv_heads);
     const int lane = int(threadIdx.x) & 63;
     const int64_t row = t.k0 + j;
@@ -261,18 +284,18 @@ __device__ void dkv_row(const Packed& a, const Tile& t, int h, int j, float* dk,
     const float* v = a.v + row * a.ld_v + int64_t(c) * a.dim;
     // The first query that sees key j.
     int64_t start = a.causal ? int64_t(j) - t.nk + t.nq : 0;
-    start = start < 0 ? 0 : start;
+    start = start < begin ? begin : start;
     float ak[2] = {0.0f, 0.0f}, av[2] = {0.0f, 0.0f};
-    for (int64_t i0 = start; i0 < t.nq; i0 += 64) {
+    for (int64_t i0 = start; i0 < end; i0 += 64) {
         const int64_t i = i0 + lane;
         float p = 0.0f, ds = 0.0f;
-        if (i < t.nq) {
+        if (i < end) {
             const int64_t at = t.q0 + i;
             ds = pair_gradient(a, a.q + at * a.ld_q + int64_t(h) * a.dim,
                                a.grad + at * a.ld_grad + int64_t(h) * a.dim, k, v,
                                a.lse[at * a.heads + h], a.delta[at * a.heads + h], p);
         }
-        const int count = t.nq - i0 < 64 ? int(t.nq - i0) : 64;
+        const int count = end - i0 < 64 ? int(end - i0) : 64;
         for (int u = 0; u < count; ++u) {
             const float wp = __shfl(p, u), wd = __shfl(ds, u);
             const float* x = a.q + (t.q0 + i0 + u) * a.ld_q + int64_t(h) * a.dim;
@@ -307,12 +330,6 @@ __device__ __forceinline__ float lse_of(float shift, float sum) {
                           __builtin_fmaf(shift, -1.904654323148236017e-9f, logf(sum)));
 }
 
-// Keys of each of a tile's pieces: what a step takes at a time divides them.
-constexpr int kLeastPiece = 128;
-__device__ __forceinline__ int piece_length(const Packed& a, int keys) {
-    const int n = keys / a.pieces / 64 * 64 + 64;
-    return n > kLeastPiece ? n : kLeastPiece;
-}
 __device__ __forceinline__ int64_t piece_of(const Packed& a, int64_t row, int h, int piece) {
     return (row * a.heads + h) * a.pieces + piece;
 }
@@ -345,12 +362,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     const int limit = visible(a, t, i);
     const int last = 32 * wave + 31 < t.rows ? 32 * wave + 31 : t.rows - 1;
     // The block's keys.
-    const int tile_end = visible(a, t, t.first + t.rows - 1);
-    const int begin = piece * piece_length(a, tile_end);
-    const int end = a.pieces == 1 ? tile_end
-                                  : int(min(int64_t(begin) + piece_length(a, tile_end),
-                                            int64_t(tile_end)));
-    if (begin > 0 && begin >= end) {
+    int begin = 0, end = visible(a, t, t.first + t.rows - 1);
+    take_piece(piece, a.pieces, begin, end);
+    if (piece > 0 && begin == end) {
         if (mine < t.rows && lane < 32)
             a.piece_stats[piece_of(a, t.q0 + i, h, piece)] = float2{-INFINITY, 0.0f};
         return;
@@ -565,6 +579,13 @@ __global__ __launch_bounds__(kThreads) void packed_forward_join(Packed a) {
 // The backward forms s, and so p_ij, again from the inputs, and dp likewise, for the pairs of a
 // wave's own rows and a block of 32 streamed ones, then the block's share of the gradients.
 
+// Where a piece's share of dq goes.
+__device__ __forceinline__ float* row_dq(const Packed& a, int64_t row, int h, int piece) {
+    return a.part_q != nullptr
+               ? a.part_q + ((row * a.heads + h) * a.pieces_q + piece) * a.dim
+               : a.dq + row * a.ld_dq + int64_t(h) * a.dim;
+}
+
 // dq_i = scale sum_j ds_ij k_j of heads of up to 64 values, with delta on the way (left in the
 // workspace for the keys' kernel): a wave has room for q and g both, and needs no partner (16 of
 // 512 tokens, 16 heads of 64, causal: 98 to 112 us, bound as the forward).
@@ -575,7 +596,8 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     __shared__ __attribute__((aligned(16))) char lds[2 * KeyTile::kBytes];
     char* const lds_v = lds + KeyTile::kBytes;
     const int h = head_of(a, int(blockIdx.x % a.heads));
-    const Tile t = block_tile(a, false, int(blockIdx.x / a.heads), kRows);
+    const int slot = int(blockIdx.x / a.heads), piece = slot % a.pieces_q;
+    const Tile t = block_tile(a, false, slot / a.pieces_q, kRows);
     if (t.rows == 0) return;
     const int c = h / (a.heads / a.kv_heads);
     const int wave = int(threadIdx.x) / 64, lane = int(threadIdx.x) & 63;
@@ -584,13 +606,14 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     const int64_t row = t.q0 + i;
     const int limit = visible(a, t, i);
     const int last = 32 * wave + 31 < t.rows ? 32 * wave + 31 : t.rows - 1;
-    const int end = visible(a, t, t.first + t.rows - 1);
-    const int wave_end = 32 * wave < t.rows ? visible(a, t, t.first + last) : 0;
+    int begin = 0, end = visible(a, t, t.first + t.rows - 1);
+    take_piece(piece, a.pieces_q, begin, end);
+    const int wave_end = 32 * wave < t.rows ? min(visible(a, t, t.first + last), end) : 0;
     const int wave_all = visible(a, t, t.first + 32 * wave);  // keys that all its queries see
 
     const float* gr = a.grad + row * a.ld_grad + int64_t(h) * a.dim;
     const float delta = own_dot<DP, VEC>(gr, a.out + row * a.ld_out + int64_t(h) * a.dim, a.dim);
-    if (lane < 32 && mine < t.rows) a.delta[row * a.heads + h] = delta;
+    if (piece == 0 && lane < 32 && mine < t.rows) a.delta[row * a.heads + h] = delta;
     if (a.dq == nullptr) return;
     const float c2 = a.scale * 1.44269504088896340736f;
     const float shift = limit > 0 ? a.lse[row * a.heads + h] * 1.44269504088896340736f : 0.0f;
@@ -605,11 +628,11 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
     const int ld_k = int(a.ld_k), ld_v = int(a.ld_v);
     KeyTile kt(ld_k, a.dim), vt(ld_v, a.dim);
-    if (end > 0) {
-        kt.load(k, ld_k, t.nk, a.dim);
-        vt.load(v, ld_v, t.nk, a.dim);
+    if (begin < end) {
+        kt.load(k + int64_t(begin) * ld_k, ld_k, t.nk - begin, a.dim);
+        vt.load(v + int64_t(begin) * ld_v, ld_v, t.nk - begin, a.dim);
     }
-    for (int j0 = 0; j0 < end; j0 += BN) {
+    for (int j0 = begin; j0 < end; j0 += BN) {
         __syncthreads();
         kt.store(lds, t.nk - j0, a.dim);
         vt.store(lds_v, t.nk - j0, a.dim);
@@ -654,10 +677,11 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     if (mine < t.rows)
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
-            store_own<VEC>(a.dq + row * a.ld_dq + int64_t(h) * a.dim, a.dim, db, dq[db]);
+            store_own<VEC>(row_dq(a, row, h, piece), a.dim, db, dq[db]);
     for (uint32_t rows = uint32_t(again) | uint32_t(again >> 32); rows != 0; rows &= rows - 1) {
         const int r = __builtin_ctz(rows);
-        dq_row(a, t, h, t.first + 32 * wave + r, __shfl(delta, r));
+        dq_row(a, t, h, t.first + 32 * wave + r, __shfl(delta, r), begin, end,
+               row_dq(a, t.q0 + t.first + 32 * wave + r, h, piece));
     }
 }
 
@@ -690,7 +714,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
         lds[4 * KeyTile::kBytes + 2 * kSwap];  // two tiles of both, by turns
     char* const lds_x = lds + 4 * KeyTile::kBytes;
     const int h = head_of(a, int(blockIdx.x % a.heads));
-    const Tile t = block_tile(a, false, int(blockIdx.x / a.heads), kRows);
+    const int slot = int(blockIdx.x / a.heads), piece = slot % a.pieces_q;
+    const Tile t = block_tile(a, false, slot / a.pieces_q, kRows);
     if (t.rows == 0) return;
     const int c = h / (a.heads / a.kv_heads);
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
@@ -700,14 +725,15 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
     const int64_t row = t.q0 + i;
     const int limit = visible(a, t, i);
     const int last = w0 + 31 < t.rows ? w0 + 31 : t.rows - 1;
-    const int end = visible(a, t, t.first + t.rows - 1);
-    const int wave_end = w0 < t.rows ? visible(a, t, t.first + last) : 0;
+    int begin = 0, end = visible(a, t, t.first + t.rows - 1);
+    take_piece(piece, a.pieces_q, begin, end);
+    const int wave_end = w0 < t.rows ? min(visible(a, t, t.first + last), end) : 0;
     const int wave_all = visible(a, t, t.first + w0);  // keys that all its queries see
 
     const float* qr = a.q + row * a.ld_q + int64_t(h) * a.dim;
     const float* gr = a.grad + row * a.ld_grad + int64_t(h) * a.dim;
     const float delta = own_dot<DP, VEC>(gr, a.out + row * a.ld_out + int64_t(h) * a.dim, a.dim);
-    if (wave < 4 && lane < 32 && mine < t.rows) a.delta[row * a.heads + h] = delta;
+    if (piece == 0 && wave < 4 && lane < 32 && mine < t.rows) a.delta[row * a.heads + h] = delta;
     if (a.dq == nullptr) return;
     const float c2 = a.scale * 1.44269504088896340736f;
     const float shift = limit > 0 ? a.lse[row * a.heads + h] * 1.44269504088896340736f : 0.0f;
@@ -734,11 +760,11 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
     };
     char* const give = lds_x + role * kSwap + ((wave & 3) * NB * 256 + lane) * 16;
     const char* const take = lds_x + (1 - role) * kSwap + ((wave & 3) * NB * 256 + lane) * 16;
-    load_rows(0);
-    stage_rows(0);
-    load_rows(BN);
+    load_rows(begin);
+    stage_rows(begin);
+    load_rows(begin + BN);
     __syncthreads();
-    for (int j0 = 0; j0 < end; j0 += BN) {
+    for (int j0 = begin; j0 < end; j0 += BN) {
         const bool active = j0 < wave_end;
         const char* const tile = lds + (j0 / BN & 1) * 2 * KeyTile::kBytes;
         if (role == 1) {  // the next tile: one wave of a SIMD before its products, the other after
@@ -813,7 +839,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
         }
     const uint32_t again = shared_rows(reinterpret_cast<uint32_t*>(lds), !fine && mine < t.rows);
     if (mine < t.rows && !(again >> (lane & 31) & 1)) {
-        float* out = a.dq + row * a.ld_dq + int64_t(h) * a.dim;
+        float* out = row_dq(a, row, h, piece);
 #pragma unroll
         for (int d = 0; d < kHalf; ++d)
             if (role * kHalf + d < kBlocks)
@@ -822,7 +848,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
     if (role == 0)
         for (uint32_t rows = again; rows != 0; rows &= rows - 1) {
             const int r = __builtin_ctz(rows);
-            dq_row(a, t, h, t.first + w0 + r, __shfl(delta, r));
+            dq_row(a, t, h, t.first + w0 + r, __shfl(delta, r), begin, end,
+                   row_dq(a, t.q0 + t.first + w0 + r, h, piece));
         }
 }
 
@@ -839,7 +866,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     __shared__ __attribute__((aligned(16))) float stats[2][2][BN];  // as the tiles, by turns
     char* const lds_x = lds + 4 * QueryTile::kBytes;
     const int h = head_of(a, int(blockIdx.x % a.heads)), c = h / (a.heads / a.kv_heads);
-    const Tile t = block_tile(a, true, int(blockIdx.x / a.heads), kRows);
+    const int slot = int(blockIdx.x / a.heads), piece = slot % a.pieces_k;
+    const Tile t = block_tile(a, true, slot / a.pieces_k, kRows);
     if (t.rows == 0) return;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int role = wave / 4, w0 = 32 * (wave & 3), lane = int(threadIdx.x) & 63;
@@ -851,7 +879,9 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
         const int64_t n = a.causal ? int64_t(key) - t.nk + t.nq : 0;
         return n < 0 ? 0 : int(n);
     };
-    const int from = first_of(j), start = first_of(t.first);
+    const int from = first_of(j);
+    int start = first_of(t.first), end = t.nq;  // the block's queries
+    take_piece(piece, a.pieces_k, start, end);
     const int wave_start = w0 < t.rows ? first_of(t.first + w0) : t.nq;
     const int wave_all = first_of(t.first + w0 + 31);
 
@@ -867,10 +897,10 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     QueryTile qt(ld_q, a.dim), gt(ld_g, a.dim);
     float stat = 0.0f;  // a query's lse (threads 0 .. BN - 1) or delta (the next BN)
     // Tile n: the queries from start + n * BN on.
-    const int count = start < t.nq ? (t.nq - start + BN - 1) / BN : 0;
+    const int count = (end - start + BN - 1) / BN;
     const auto load_rows = [&](int n) {
         if (n >= count) return;
-        const int i0 = start + n * BN, left = t.nq - i0;
+        const int i0 = start + n * BN, left = end - i0;
         const int64_t at = t.q0 + i0;
         qt.load(a.q + at * a.ld_q + int64_t(h) * a.dim, ld_q, left, a.dim);
         gt.load(a.grad + at * a.ld_grad + int64_t(h) * a.dim, ld_g, left, a.dim);
@@ -881,7 +911,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     };
     const auto stage_rows = [&](int n) {
         if (n >= count) return;
-        const int left = t.nq - (start + n * BN);
+        const int left = end - (start + n * BN);
         char* const at = lds + (n & 1) * 2 * QueryTile::kBytes;
         qt.store(at, left, a.dim);
         gt.store(at + QueryTile::kBytes, left, a.dim);
@@ -895,7 +925,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     load_rows(1);
     __syncthreads();
     for (int n = 0; n < count; ++n) {
-        const int i0 = start + n * BN, left = t.nq - i0;
+        const int i0 = start + n * BN, left = end - i0;
         const bool active = i0 + BN > wave_start;
         const char* const tile = lds + (n & 1) * 2 * QueryTile::kBytes;
         if (role == 1) {  // the next tile: one wave of a SIMD before its products, the other after
@@ -983,6 +1013,8 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
         __syncthreads();
     }
     const float factor = role == 0 ? 1.0f : a.scale;
+    // Without dk there may be no delta either.
+    const bool wanted = (role == 0 ? a.dv : a.dk) != nullptr;
     bool fine = true;
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d)
@@ -991,49 +1023,61 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
             sum[d][r] *= factor;
             fine = fine && fabsf(sum[d][r]) < INFINITY;
         }
-    const uint32_t again = shared_rows(reinterpret_cast<uint32_t*>(lds), !fine && mine < t.rows);
+    const uint32_t again =
+        shared_rows(reinterpret_cast<uint32_t*>(lds), wanted && !fine && mine < t.rows);
     // Where the rows of dk (or dv) of key j go.
     const auto row_dk = [&](int64_t at) {
-        return a.part_k != nullptr ? a.part_k + (at * a.heads + h) * a.dim
+        return a.part_k != nullptr ? a.part_k + ((at * a.heads + h) * a.pieces_k + piece) * a.dim
                : a.dk == nullptr   ? nullptr
                                    : a.dk + at * a.ld_dk + int64_t(c) * a.dim;
     };
     const auto row_dv = [&](int64_t at) {
-        return a.part_v != nullptr ? a.part_v + (at * a.heads + h) * a.dim
+        return a.part_v != nullptr ? a.part_v + ((at * a.heads + h) * a.pieces_k + piece) * a.dim
                : a.dv == nullptr   ? nullptr
                                    : a.dv + at * a.ld_dv + int64_t(c) * a.dim;
     };
     float* const out = role == 0 ? row_dv(row) : row_dk(row);
-    if (out != nullptr && mine < t.rows && !(again >> (lane & 31) & 1)) {
+    if (wanted && mine < t.rows && !(again >> (lane & 31) & 1)) {
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) store_own<VEC>(out, a.dim, d, sum[d]);
     }
     if (role == 0)
         for (uint32_t rows = again; rows != 0; rows &= rows - 1) {
             const int64_t key = t.first + w0 + __builtin_ctz(rows);
-            dkv_row(a, t, h, int(key), row_dk(t.k0 + key), row_dv(t.k0 + key));
+            dkv_row(a, t, h, int(key), start, end, row_dk(t.k0 + key), row_dv(t.k0 + key));
         }
 }
 
-// The sums of the query heads' shares, in the order of the heads. Thread = row, key head, value.
-// HBM (5576 rows, 12 heads of 96 over 4: 13 us for 69 MB).
-__global__ __launch_bounds__(kThreads) void packed_backward_join(Packed a) {
-    const int64_t width = int64_t(a.kv_heads) * a.dim;
-    const int first = offset_at(a.cu_k, 0, a.total_k);
-    const int last = offset_at(a.cu_k, a.sequences, a.total_k);
-    const int group = a.heads / a.kv_heads;
+// Rows of one gradient, or of dk and dv, from `count` shares of each head's row one after the
+// other, in their order: the pieces', and for dk and dv the group's query heads'. Thread = row,
+// head, value. HBM (5576 rows, 12 heads of 96 over 4: 13 us for 69 MB).
+template <int N>
+struct Shares {
+    const int32_t* cu;
+    int sequences, total;
+    int heads, count, dim;
+    const float* from[N];
+    float* to[N];  // may be null
+    int64_t ld[N];
+};
+template <int N>
+__global__ __launch_bounds__(kThreads) void packed_backward_join(Shares<N> x) {
+    const int64_t width = int64_t(x.heads) * x.dim;
+    const int first = offset_at(x.cu, 0, x.total);
+    const int last = offset_at(x.cu, x.sequences, x.total);
     for (int64_t e = first * width + int64_t(blockIdx.x) * kThreads + threadIdx.x; e < last * width;
          e += int64_t(gridDim.x) * kThreads) {
         const int64_t row = e / width;
-        const int at = int(e - row * width), c = at / a.dim, d = at - c * a.dim;
-        const int64_t from = (row * a.heads + int64_t(c) * group) * a.dim + d;
-        float k = 0.0f, v = 0.0f;
-        for (int n = 0; n < group; ++n) {
-            k += a.part_k[from + int64_t(n) * a.dim];
-            v += a.part_v[from + int64_t(n) * a.dim];
-        }
-        if (a.dk != nullptr) a.dk[row * a.ld_dk + at] = k;
-        if (a.dv != nullptr) a.dv[row * a.ld_dv + at] = v;
+        const int at = int(e - row * width), c = at / x.dim, d = at - c * x.dim;
+        const int64_t from = (row * x.heads + c) * x.count * x.dim + d;
+        float y[N] = {};
+#pragma unroll 4
+        for (int n = 0; n < x.count; ++n)
+#pragma unroll
+            for (int g = 0; g < N; ++g) y[g] += x.from[g][from + int64_t(n) * x.dim];
+#pragma unroll
+        for (int g = 0; g < N; ++g)
+            if (x.to[g] != nullptr) x.to[g][row * x.ld[g] + at] = y[g];
     }
 }
 
@@ -1153,40 +1197,82 @@ int forward_of(const Packed& a, hipStream_t s) {
                             : launch_forward<DP, BN, 8, VEC>(a, s);
 }
 
-// dk and dv of grouped heads are formed head by head, for as many blocks as the queries have, and
-// summed afterwards (12 heads over 4, 5576 rows of 96: one block a group took 2.8 times as long).
-bool splits(const Packed& a) { return a.heads != a.kv_heads; }
-
-size_t delta_bytes(const Packed& a) {
-    return (size_t(a.total_q) * size_t(a.heads) * sizeof(float) + 15) & ~size_t(15);
+// The backward's pieces likewise, of the keys for dq and of the queries for dk and dv: for 512
+// blocks under a causal mask, else for 256, one a CU (us, whole : for 256 : for 512, 8 heads of 64
+// values: one sequence of 4096 584 : 572 : 416; 128 queries behind 4096 keys 327 : 78 : 76; without
+// the mask one of 2048 311 : 193 : 201, 8 of 512 117 : 113 : 136; heads of 96, 8 of 512 143 : 139 :
+// 208).
+int backward_pieces(const Packed& a, int64_t rows, int64_t passed) {
+    const int64_t mean = a.sequences == 0 ? 0 : passed / a.sequences;
+    if (mean < 384) return 1;
+    const int64_t blocks = slots(rows, a.sequences) * a.heads;
+    const int64_t want = a.causal ? 512 : 256;
+    const int64_t most = std::min<int64_t>(mean / kLeastPiece, 32);
+    return int(std::max<int64_t>(1, std::min((want + blocks / 2) / blocks, most)));
 }
 
-size_t part_bytes(const Packed& a) {
-    return splits(a) ? size_t(a.total_k) * size_t(a.heads) * size_t(a.dim) * sizeof(float) : 0;
+// Shares of dq, and of each of dk and dv. dk and dv of grouped heads are formed head by head, for
+// as many blocks as the queries have, and summed afterwards (12 heads over 4, 5576 rows of 96: one
+// block a group took 2.8 times as long).
+struct BackwardSpace {
+    int pieces_q, pieces_k;
+    size_t delta, part_q, part_k;  // bytes
+};
+BackwardSpace space_of(const Packed& a) {
+    BackwardSpace x;
+    x.pieces_q = backward_pieces(a, a.total_q, a.total_k);
+    x.pieces_k = backward_pieces(a, a.total_k, a.total_q);
+    const auto aligned = [](size_t n) { return (n + 15) & ~size_t(15); };
+    const size_t row = size_t(a.heads) * sizeof(float), dim = size_t(a.dim);
+    x.delta = aligned(size_t(a.total_q) * row);
+    x.part_q = x.pieces_q > 1 ? aligned(size_t(a.total_q) * row * dim * size_t(x.pieces_q)) : 0;
+    x.part_k = x.pieces_k > 1 || a.heads != a.kv_heads
+                   ? aligned(size_t(a.total_k) * row * dim * size_t(x.pieces_k))
+                   : 0;
+    return x;
+}
+size_t bytes_of(const BackwardSpace& x) { return x.delta + x.part_q + 2 * x.part_k; }
+
+template <int N>
+int join_shares(const Shares<N>& x, hipStream_t s) {
+    const int64_t n = int64_t(x.total) * x.heads * x.dim;
+    EHIP_LAUNCH("attention_packed_backward_join", packed_backward_join<N>,
+                dim3(unsigned(std::min<int64_t>(ceil_div(n, kThreads), 1 << 16))), dim3(kThreads),
+                0, s, x);
+    return EHIP_OK;
 }
 
 template <int DP, int BN, bool VEC>
 int launch_backward(const Packed& a, hipStream_t s) {
     if (a.total_q > 0 && (a.dq != nullptr || a.dk != nullptr)) {
-        const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads);
+        const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads * a.pieces_q);
         if constexpr (DP <= 64)
             EHIP_LAUNCH("attention_packed_backward_q", (packed_backward_q<DP, 32, VEC>),
                         dim3(blocks), dim3(kThreads), 0, s, a);
         else
             EHIP_LAUNCH("attention_packed_backward_q", (packed_backward_q_pair<DP, BN, VEC>),
                         dim3(blocks), dim3(kBackThreads), 0, s, a);
+        if (a.part_q != nullptr) {
+            const Shares<1> x{a.cu_q, a.sequences, a.total_q, a.heads,  a.pieces_q,
+                              a.dim,  {a.part_q},  {a.dq},    {a.ld_dq}};
+            if (int rc = join_shares(x, s)) return rc;
+        }
     }
     if (a.total_k == 0 || (a.dk == nullptr && a.dv == nullptr)) return EHIP_OK;
-    const unsigned blocks = unsigned(slots(a.total_k, a.sequences) * a.heads);
+    const unsigned blocks = unsigned(slots(a.total_k, a.sequences) * a.heads * a.pieces_k);
     EHIP_LAUNCH("attention_packed_backward_kv", (packed_backward_kv<DP, BN, VEC>), dim3(blocks),
                 dim3(kBackThreads), 0, s, a);
-    if (a.part_k != nullptr) {
-        const int64_t n = int64_t(a.total_k) * a.kv_heads * a.dim;
-        EHIP_LAUNCH("attention_packed_backward_join", packed_backward_join,
-                    dim3(unsigned(std::min<int64_t>(ceil_div(n, kThreads), 1 << 16))),
-                    dim3(kThreads), 0, s, a);
-    }
-    return EHIP_OK;
+    if (a.part_k == nullptr) return EHIP_OK;
+    const Shares<2> x{a.cu_k,
+                      a.sequences,
+                      a.total_k,
+                      a.kv_heads,
+                      a.heads / a.kv_heads * a.pieces_k,
+                      a.dim,
+                      {a.part_k, a.part_v},
+                      {a.dk, a.dv},
+                      {a.ld_dk, a.ld_dv}};
+    return join_shares(x, s);
 }
 
 }  // namespace
@@ -1230,7 +1316,7 @@ int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* workspa
 int64_t ehip_attention_packed_backward_workspace(const ehip_attention_packed_t* desc) {
     Packed a;
     if (fill("attention_packed_backward", desc, a)) return -1;
-    return int64_t(delta_bytes(a) + 2 * part_bytes(a));
+    return int64_t(bytes_of(space_of(a)));
 }
 
 int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, const float* grad,
@@ -1249,7 +1335,8 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
         (dv != nullptr && ld_dv < narrow))
         return fail(EHIP_EINVAL,
                     "attention_packed_backward: leading dimension below the row's length");
-    const size_t need = delta_bytes(a) + 2 * part_bytes(a);
+    const BackwardSpace space = space_of(a);
+    const size_t need = bytes_of(space);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace)))
         return fail(EHIP_EINVAL,
                     "attention_packed_backward: needs %zu bytes of 16-byte aligned workspace",
@@ -1263,9 +1350,15 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
     a.ld_dk = ld_dk;
     a.ld_dv = ld_dv;
     a.delta = static_cast<float*>(workspace);
-    if (part_bytes(a) != 0) {
-        a.part_k = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes(a));
-        a.part_v = a.part_k + part_bytes(a) / sizeof(float);
+    // Without dq its kernel leaves delta alone, for which one piece is enough.
+    a.pieces_q = dq != nullptr ? space.pieces_q : 1;
+    a.pieces_k = space.pieces_k;
+    char* at = static_cast<char*>(workspace) + space.delta;
+    if (a.pieces_q > 1) a.part_q = reinterpret_cast<float*>(at);
+    at += space.part_q;
+    if (space.part_k != 0) {
+        a.part_k = reinterpret_cast<float*>(at);
+        a.part_v = reinterpret_cast<float*>(at + space.part_k);
     }
     hipStream_t s = as_stream(stream);
     const bool vec = a.dim % 4 == 0;

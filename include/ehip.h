@@ -916,8 +916,8 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  *   dq_i = scale sum_j ds_ij k_j    dk_j = scale sum_i ds_ij q_i
  * dk and dv summed over the query heads of the group too. The outputs may not
  * overlap the inputs or each other. `workspace` (device memory, 16-byte
- * aligned) holds delta, and each query head's share of dk and dv where heads
- * are grouped, during the call: at least
+ * aligned) holds delta and, where heads are grouped or few rows pass many, the
+ * shares of the gradients, during the call: at least
  * ehip_attention_packed_backward_workspace() bytes, of the call's own.
  * Deterministic: no atomics, the sums' order goes by the lengths and sizes. */
 typedef struct {

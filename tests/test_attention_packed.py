@@ -360,6 +360,67 @@ def test_split_keys(hip, nq, nk, heads, kv, d, causal):
     assert torch.equal(again[0], out) and torch.equal(again[1], lse)
 
 
+# The gradients' shares are added one after the other, up to 32 for each head: the bounds' sums over
+# 384 rows or more count more roundings than those.
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("nq,nk,heads,kv,d", [
+    ([16], [2000], 2, 1, 64), ([1500], [40], 2, 2, 64), ([700], [700], 4, 2, 96),
+    ([1027], [1027], 1, 1, 128), ([1, 0, 260, 900], [1000, 900, 390, 64], 2, 1, 33),
+    ([600], [450], 2, 2, 100), ([450], [600], 3, 1, 17)])
+def test_split_gradients(hip, nq, nk, heads, kv, d, causal):
+    import torch
+    print_case("packed split gradients", nq, nk, heads, kv, d, causal)
+    q, k, v, g = make(nq, nk, heads, kv, d, seed=sum(nk) + d, tail=5)
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = hip.attention_packed(q, k, v, cq, ck, causal=causal)
+    grads = [torch.full_like(t, 7.0) for t in (q, k, v)]
+    hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck, causal=causal, grads=grads)
+    tq, tk = sum(nq), sum(nk)
+    value, bound = packed(q[:tq], k[:tk], v[:tk], nq, nk, d ** -0.5, causal, g[:tq])
+    for name, got, rows in zip(("dq", "dk", "dv"), grads, (tq, tk, tk)):
+        within(got[:rows], value[name], bound[name], name)
+        assert bool((got[rows:] == 7.0).all()), name
+    # Each alone, on the bits of all of them.
+    for n in range(3):
+        alone = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck, causal=causal,
+                                              want=tuple(m == n for m in range(3)))
+        rows = (tq, tk, tk)[n]
+        assert [t is None for t in alone] == [m != n for m in range(3)]
+        assert torch.equal(alone[n][:rows], grads[n][:rows])
+
+
+@gpu
+def test_split_gradients_not_finite_and_not_seen(hip):
+    """What only later rows see does not reach a row's gradients, whichever piece holds it."""
+    import torch
+    print_case("packed split gradients special")
+    nq, nk = [200], [900]
+    q, k, v, g = make(nq, nk, 2, 1, 64, seed=51)
+    cq, ck = offsets(nq), offsets(nk)
+    k[800:], v[830:] = math.nan, math.inf    # rows 100.. see them
+    out, lse = hip.attention_packed(q, k, v, cq, ck)
+    dq = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck, want=(True, False, False))[0]
+    kz, vz = k.clone(), v.clone()
+    kz[800:], vz[830:] = 0, 0
+    value, bound = packed(q, kz, vz, nq, nk, 0.125, True, g)
+    within(dq[:100], value["dq"][:100], bound["dq"][:100], "dq")
+    assert bool(torch.isnan(dq[100:]).all())
+    # And a query that is not finite reaches the keys it sees, not those after them.
+    q, k, v, g = make([900], [900], 2, 1, 64, seed=52)
+    cu = offsets([900])
+    g[700] = math.nan
+    out, lse = hip.attention_packed(q, k, v, cu)
+    _, dk, dv = hip.attention_packed_backward(g, q, k, v, out, lse, cu)
+    assert bool(torch.isnan(dk[:701]).all()) and bool(torch.isnan(dv[:701]).all())
+    gz = g.clone()
+    gz[700] = 0
+    value, bound = packed(q, k, v, [900], [900], 0.125, True, gz)
+    within(dk[701:], value["dk"][701:], bound["dk"][701:], "dk")
+    within(dv[701:], value["dv"][701:], bound["dv"][701:], "dv")
+
+
 @gpu
 def test_split_keys_not_finite_not_seen_and_past_the_last_sequence(hip):
     import torch
@@ -414,28 +475,34 @@ def test_split_keys_captured_and_replayed(hip):
     import torch
     print_case("packed split graph")
     nq, nk = [40, 33], [1500, 600]
-    q, k, v, _ = make(nq, nk, 4, 2, 64, seed=34)
+    q, k, v, g = make(nq, nk, 4, 2, 64, seed=34)
     cq, ck = offsets(nq), offsets(nk)
+
+    def both():
+        (out, lse), split = splits(hip, q, k, v, cq, ck)
+        assert split
+        return [out, lse, *hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck)]
+
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
-        hip.attention_packed(q, k, v, cq, ck)
+        both()
     torch.cuda.synchronize()
     graphs = []
     for _ in range(2):  # each with a workspace of its own
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            out = hip.attention_packed(q, k, v, cq, ck)
-        graphs.append((graph, out))
+            outs = both()
+        graphs.append((graph, outs))
     for seed in range(3):
-        for t, f in zip((q, k, v), make(nq, nk, 4, 2, 64, seed=40 + seed)):
+        for t, f in zip((q, k, v, g), make(nq, nk, 4, 2, 64, seed=40 + seed)):
             t.copy_(f)
-        want, split = splits(hip, q, k, v, cq, ck)
-        assert split
+        want = both()
         for graph, _ in graphs:
             graph.replay()
         torch.cuda.synchronize()
-        for _, out in graphs:
-            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        for _, outs in graphs:
+            for x, y in zip(outs, want):
+                assert torch.equal(x, y)
 
 
 @gpu
