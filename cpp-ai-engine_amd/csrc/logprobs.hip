@@ -218,7 +218,7 @@ __device__ __forceinline__ void offer(Top& sh, int top, Key key) {
 // The same for the logits x of a segment (all indices above the list's), `largest` each thread's
 // largest, special where the thread has met a NaN or +inf: a key is made for the few that may be in
 // the list only (155 rows of 91471, top 20: 32 us, 46 with keys for all). A lower limit of the
-// list's orders is the least over the waves of the ceil(top / 4)-th largest of their lanes'
+// list's orders is the least over the row's n waves of the ceil(top / n)-th largest of their lanes'
 // largest, its lowest 12 bits as 0: found by counting the lanes above it, a bit at a time. Where
 // that limit does not separate enough of them, as many are equal or the row has little but -inf,
 // all keys are offered.
@@ -237,7 +237,9 @@ __device__ __forceinline__ void offer_logits(Top& sh, int top, const float (&x)[
         if (threads == 0) return;
         uint32_t limit = floor + 1;
         if (threads > top) {
-            const int each = (top + kWaves - 1) / kWaves;
+            // Of a short row the waves that are full, or the first one.
+            const int waves = max(1, min(left / 4, kThreads) / 64);
+            const int each = (top + waves - 1) / waves;
             uint32_t upto = 0;
 #pragma unroll
             for (int b = 31; b >= 12; --b) {
@@ -248,7 +250,8 @@ __device__ __forceinline__ void offer_logits(Top& sh, int top, const float (&x)[
             __syncthreads();
             uint32_t least = sh.limits[0];
 #pragma unroll
-            for (int w = 1; w < kWaves; ++w) least = min(least, sh.limits[w]);
+            for (int w = 1; w < kWaves; ++w)
+                if (w < waves) least = min(least, sh.limits[w]);
             limit = max(limit, least);
         }
         if (limit > order_of(-INFINITY)) {
