@@ -339,11 +339,11 @@ __device__ __forceinline__ int64_t piece_of(const Packed& a, int64_t row, int h,
 // it (16384 tokens, 8 heads of 128 values, causal: 2.6 to 2.8 ms, 195 to 210 TFLOP/s of 201 that a
 // sixth of a bf16 product of 8192^3 reaches); shorter ones spend as long on exponents and on
 // splitting the weights (16 of 512, 16 heads of 64: 72 to 83 us, the matrix units busy 40 % of it).
-template <int DP, int BN, int WAVES, bool VEC>
+template <int DP, int BN, int WAVES, int READS>
 __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     constexpr int BUFFERS = WAVES / 4;
     using namespace attention;
-    using KeyTile = RowTile<BN, DP, 64 * WAVES, VEC>;
+    using KeyTile = RowTile<BN, DP, 64 * WAVES, READS>;
     constexpr int kTile = 2 * KeyTile::kBytes;
     // Wide heads leave the third parts of the queries, which one product in six takes, in LDS: all
     // of them in registers spill.
@@ -375,7 +375,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q.
     const float c2 = fabsf(a.scale) * 1.44269504088896340736f;
     bf16x8 q[DP / 16][3];
-    own_row<DP, VEC>(a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim, a.dim,
+    own_row<DP, READS>(a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim, a.dim,
                      a.scale < 0.0f ? -1.0f : 1.0f, q);
     char* const parked = lds + BUFFERS * kTile + (wave * (DP / 16) * 64 + lane) * 16;
     if constexpr (kPark) {
@@ -474,7 +474,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
         if (mine < t.rows) {
 #pragma unroll
             for (int db = 0; db < DP / 32; ++db)
-                store_own<VEC>(a.piece_out + at * a.dim, a.dim, db, o[db]);
+                store_own<READS>(a.piece_out + at * a.dim, a.dim, db, o[db]);
             if (lane < 32)
                 a.piece_stats[at] = float2{top == -INFINITY ? -INFINITY : shift, sum};
         }
@@ -496,7 +496,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     if (mine < t.rows) {
         float* out = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db) store_own<VEC>(out, a.dim, db, o[db]);
+        for (int db = 0; db < DP / 32; ++db) store_own<READS>(out, a.dim, db, o[db]);
         if (lane < 32)
             a.lse[int64_t(t.q0 + i) * a.heads + h] =
                 limit == 0 ? -INFINITY
@@ -589,10 +589,10 @@ __device__ __forceinline__ float* row_dq(const Packed& a, int64_t row, int h, in
 // dq_i = scale sum_j ds_ij k_j of heads of up to 64 values, with delta on the way (left in the
 // workspace for the keys' kernel): a wave has room for q and g both, and needs no partner (16 of
 // 512 tokens, 16 heads of 64, causal: 98 to 112 us, bound as the forward).
-template <int DP, int BN, bool VEC>
+template <int DP, int BN, int READS>
 __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     using namespace attention;
-    using KeyTile = RowTile<BN, DP, kThreads, VEC>;
+    using KeyTile = RowTile<BN, DP, kThreads, READS>;
     __shared__ __attribute__((aligned(16))) char lds[2 * KeyTile::kBytes];
     char* const lds_v = lds + KeyTile::kBytes;
     const int h = head_of(a, int(blockIdx.x % a.heads));
@@ -612,14 +612,14 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     const int wave_all = visible(a, t, t.first + 32 * wave);  // keys that all its queries see
 
     const float* gr = a.grad + row * a.ld_grad + int64_t(h) * a.dim;
-    const float delta = own_dot<DP, VEC>(gr, a.out + row * a.ld_out + int64_t(h) * a.dim, a.dim);
+    const float delta = own_dot<DP, READS>(gr, a.out + row * a.ld_out + int64_t(h) * a.dim, a.dim);
     if (piece == 0 && lane < 32 && mine < t.rows) a.delta[row * a.heads + h] = delta;
     if (a.dq == nullptr) return;
     const float c2 = a.scale * 1.44269504088896340736f;
     const float shift = limit > 0 ? a.lse[row * a.heads + h] * 1.44269504088896340736f : 0.0f;
     bf16x8 q[DP / 16][3], g[DP / 16][3];
-    own_row<DP, VEC>(a.q + row * a.ld_q + int64_t(h) * a.dim, a.dim, 1.0f, q);
-    own_row<DP, VEC>(gr, a.dim, 1.0f, g);
+    own_row<DP, READS>(a.q + row * a.ld_q + int64_t(h) * a.dim, a.dim, 1.0f, q);
+    own_row<DP, READS>(gr, a.dim, 1.0f, g);
     floatx16 dq[DP / 32];
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) dq[db] = zeros();
@@ -677,7 +677,7 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     if (mine < t.rows)
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
-            store_own<VEC>(row_dq(a, row, h, piece), a.dim, db, dq[db]);
+            store_own<READS>(row_dq(a, row, h, piece), a.dim, db, dq[db]);
     for (uint32_t rows = uint32_t(again) | uint32_t(again >> 32); rows != 0; rows &= rows - 1) {
         const int r = __builtin_ctz(rows);
         dq_row(a, t, h, t.first + 32 * wave + r, __shfl(delta, r), begin, end,
@@ -704,10 +704,10 @@ __device__ __forceinline__ uint32_t shared_rows(uint32_t* votes, bool bad) {
 
 // dq and delta of wider heads. Wave role 0 forms s and p, role 1 dp - delta; both then have ds, and
 // half of dq's values each (5576 tokens in 11 sequences, 12 heads of 96 over 4: 189 to 234 us).
-template <int DP, int BN, bool VEC>
+template <int DP, int BN, int READS>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed a) {
     using namespace attention;
-    using KeyTile = RowTile<BN, DP, kBackThreads, VEC>;
+    using KeyTile = RowTile<BN, DP, kBackThreads, READS>;
     constexpr int NB = BN / 32, NU = BN / 16, kBlocks = DP / 32, kHalf = (kBlocks + 1) / 2;
     constexpr int kSwap = 4 * NB * 4096;  // one role's scores
     __shared__ __attribute__((aligned(16))) char
@@ -732,13 +732,13 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
 
     const float* qr = a.q + row * a.ld_q + int64_t(h) * a.dim;
     const float* gr = a.grad + row * a.ld_grad + int64_t(h) * a.dim;
-    const float delta = own_dot<DP, VEC>(gr, a.out + row * a.ld_out + int64_t(h) * a.dim, a.dim);
+    const float delta = own_dot<DP, READS>(gr, a.out + row * a.ld_out + int64_t(h) * a.dim, a.dim);
     if (piece == 0 && wave < 4 && lane < 32 && mine < t.rows) a.delta[row * a.heads + h] = delta;
     if (a.dq == nullptr) return;
     const float c2 = a.scale * 1.44269504088896340736f;
     const float shift = limit > 0 ? a.lse[row * a.heads + h] * 1.44269504088896340736f : 0.0f;
     bf16x8 own[DP / 16][3];
-    own_row<DP, VEC>(role == 0 ? qr : gr, a.dim, 1.0f, own);
+    own_row<DP, READS>(role == 0 ? qr : gr, a.dim, 1.0f, own);
     floatx16 dq[kHalf];
 #pragma unroll
     for (int d = 0; d < kHalf; ++d) dq[d] = zeros();
@@ -843,7 +843,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
 #pragma unroll
         for (int d = 0; d < kHalf; ++d)
             if (role * kHalf + d < kBlocks)
-                store_own<VEC>(out, a.dim, role * kHalf + d, dq[d]);
+                store_own<READS>(out, a.dim, role * kHalf + d, dq[d]);
     }
     if (role == 0)
         for (uint32_t rows = again; rows != 0; rows &= rows - 1) {
@@ -856,10 +856,10 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
 // dv_j = sum_i p_ij g_i by the waves of role 0, from s and p, and dk_j = scale sum_i ds_ij q_i by
 // those of role 1, from dp and the other's p: 16 of 512 tokens, 16 heads of 64, 143 to 170 us; 5576
 // tokens, 12 heads of 96, 234 to 288. Vector work bounds it, the matrix units are busy 36 and 47 %.
-template <int DP, int BN, bool VEC>
+template <int DP, int BN, int READS>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) {
     using namespace attention;
-    using QueryTile = RowTile<BN, DP, kBackThreads, VEC>;
+    using QueryTile = RowTile<BN, DP, kBackThreads, READS>;
     constexpr int NB = BN / 32, NU = BN / 16, kBlocks = DP / 32;
     constexpr int kSwap = 4 * NB * 4096;
     __shared__ __attribute__((aligned(16))) char lds[4 * QueryTile::kBytes + kSwap];
@@ -887,7 +887,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
 
     const float c2 = a.scale * 1.44269504088896340736f;
     bf16x8 own[DP / 16][3];
-    own_row<DP, VEC>(role == 0 ? a.k + row * a.ld_k + int64_t(c) * a.dim
+    own_row<DP, READS>(role == 0 ? a.k + row * a.ld_k + int64_t(c) * a.dim
                                : a.v + row * a.ld_v + int64_t(c) * a.dim,
                      a.dim, 1.0f, own);
     floatx16 sum[kBlocks];  // dv or dk
@@ -1039,7 +1039,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
     float* const out = role == 0 ? row_dv(row) : row_dk(row);
     if (wanted && mine < t.rows && !(again >> (lane & 31) & 1)) {
 #pragma unroll
-        for (int d = 0; d < kBlocks; ++d) store_own<VEC>(out, a.dim, d, sum[d]);
+        for (int d = 0; d < kBlocks; ++d) store_own<READS>(out, a.dim, d, sum[d]);
     }
     if (role == 0)
         for (uint32_t rows = again; rows != 0; rows &= rows - 1) {
@@ -1140,11 +1140,11 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
     return EHIP_OK;
 }
 
-template <int DP, int BN, int WAVES, bool VEC>
+template <int DP, int BN, int WAVES, int READS>
 int launch_forward(const Packed& a, hipStream_t s) {
     const unsigned blocks =
         unsigned(slots(a.total_q, a.sequences, 32 * WAVES) * a.heads * a.pieces);
-    EHIP_LAUNCH("attention_packed", (packed_forward<DP, BN, WAVES, VEC>), dim3(blocks),
+    EHIP_LAUNCH("attention_packed", (packed_forward<DP, BN, WAVES, READS>), dim3(blocks),
                 dim3(64 * WAVES), 0, s, a);
     if (a.pieces > 1)
         EHIP_LAUNCH("attention_packed_join", packed_forward_join,
@@ -1191,10 +1191,10 @@ size_t piece_bytes(const Packed& a) {
                              (sizeof(float2) + size_t(a.dim) * sizeof(float));
 }
 
-template <int DP, int BN, bool VEC>
+template <int DP, int BN, int READS>
 int forward_of(const Packed& a, hipStream_t s) {
-    return narrow_blocks(a) ? launch_forward<DP, BN, 4, VEC>(a, s)
-                            : launch_forward<DP, BN, 8, VEC>(a, s);
+    return narrow_blocks(a) ? launch_forward<DP, BN, 4, READS>(a, s)
+                            : launch_forward<DP, BN, 8, READS>(a, s);
 }
 
 // The backward's pieces likewise, of the keys for dq and of the queries for dk and dv: for 512
@@ -1242,15 +1242,15 @@ int join_shares(const Shares<N>& x, hipStream_t s) {
     return EHIP_OK;
 }
 
-template <int DP, int BN, bool VEC>
+template <int DP, int BN, int READS>
 int launch_backward(const Packed& a, hipStream_t s) {
     if (a.total_q > 0 && (a.dq != nullptr || a.dk != nullptr)) {
         const unsigned blocks = unsigned(slots(a.total_q, a.sequences) * a.heads * a.pieces_q);
         if constexpr (DP <= 64)
-            EHIP_LAUNCH("attention_packed_backward_q", (packed_backward_q<DP, 32, VEC>),
+            EHIP_LAUNCH("attention_packed_backward_q", (packed_backward_q<DP, 32, READS>),
                         dim3(blocks), dim3(kThreads), 0, s, a);
         else
-            EHIP_LAUNCH("attention_packed_backward_q", (packed_backward_q_pair<DP, BN, VEC>),
+            EHIP_LAUNCH("attention_packed_backward_q", (packed_backward_q_pair<DP, BN, READS>),
                         dim3(blocks), dim3(kBackThreads), 0, s, a);
         if (a.part_q != nullptr) {
             const Shares<1> x{a.cu_q, a.sequences, a.total_q, a.heads,  a.pieces_q,
@@ -1260,7 +1260,7 @@ int launch_backward(const Packed& a, hipStream_t s) {
     }
     if (a.total_k == 0 || (a.dk == nullptr && a.dv == nullptr)) return EHIP_OK;
     const unsigned blocks = unsigned(slots(a.total_k, a.sequences) * a.heads * a.pieces_k);
-    EHIP_LAUNCH("attention_packed_backward_kv", (packed_backward_kv<DP, BN, VEC>), dim3(blocks),
+    EHIP_LAUNCH("attention_packed_backward_kv", (packed_backward_kv<DP, BN, READS>), dim3(blocks),
                 dim3(kBackThreads), 0, s, a);
     if (a.part_k == nullptr) return EHIP_OK;
     const Shares<2> x{a.cu_k,
@@ -1273,6 +1273,22 @@ int launch_backward(const Packed& a, hipStream_t s) {
                       {a.dk, a.dv},
                       {a.ld_dk, a.ld_dv}};
     return join_shares(x, s);
+}
+
+// A head's values in blocks of 32; wider heads take 32 rows of a tile at a time.
+template <int READS>
+int forward_dim(const Packed& a, hipStream_t s) {
+    if (a.dim <= 32) return forward_of<32, 64, READS>(a, s);
+    if (a.dim <= 64) return forward_of<64, 64, READS>(a, s);
+    if (a.dim <= 96) return forward_of<96, 32, READS>(a, s);
+    return forward_of<128, 32, READS>(a, s);
+}
+template <int READS>
+int backward_dim(const Packed& a, hipStream_t s) {
+    if (a.dim <= 32) return launch_backward<32, 64, READS>(a, s);
+    if (a.dim <= 64) return launch_backward<64, 64, READS>(a, s);
+    if (a.dim <= 96) return launch_backward<96, 32, READS>(a, s);
+    return launch_backward<128, 32, READS>(a, s);
 }
 
 }  // namespace
@@ -1302,15 +1318,10 @@ int ehip_attention_packed_f32(const ehip_attention_packed_t* desc, void* workspa
     a.piece_stats = static_cast<float2*>(workspace);
     a.piece_out = reinterpret_cast<float*>(
         a.piece_stats + int64_t(a.total_q) * a.heads * a.pieces);
-    const bool vec = a.dim % 4 == 0;
-    if (a.dim <= 32) return vec ? forward_of<32, 64, true>(a, as_stream(stream))
-                                : forward_of<32, 64, false>(a, as_stream(stream));
-    if (a.dim <= 64) return vec ? forward_of<64, 64, true>(a, as_stream(stream))
-                                : forward_of<64, 64, false>(a, as_stream(stream));
-    if (a.dim <= 96) return vec ? forward_of<96, 32, true>(a, as_stream(stream))
-                                : forward_of<96, 32, false>(a, as_stream(stream));
-    return vec ? forward_of<128, 32, true>(a, as_stream(stream))
-               : forward_of<128, 32, false>(a, as_stream(stream));
+    hipStream_t s = as_stream(stream);
+    using namespace attention;
+    if (a.dim < 4) return forward_of<32, 64, kSingle>(a, s);
+    return a.dim % 4 == 0 ? forward_dim<kFours>(a, s) : forward_dim<kClamped>(a, s);
 }
 
 int64_t ehip_attention_packed_backward_workspace(const ehip_attention_packed_t* desc) {
@@ -1361,17 +1372,9 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
         a.part_v = reinterpret_cast<float*>(at + space.part_k);
     }
     hipStream_t s = as_stream(stream);
-    const bool vec = a.dim % 4 == 0;
-    if (a.dim <= 32)
-        return vec ? launch_backward<32, 64, true>(a, s)
-                   : launch_backward<32, 64, false>(a, s);
-    if (a.dim <= 64)
-        return vec ? launch_backward<64, 64, true>(a, s)
-                   : launch_backward<64, 64, false>(a, s);
-    if (a.dim <= 96)
-        return vec ? launch_backward<96, 32, true>(a, s)
-                   : launch_backward<96, 32, false>(a, s);
-    return vec ? launch_backward<128, 32, true>(a, s) : launch_backward<128, 32, false>(a, s);
+    using namespace attention;
+    if (a.dim < 4) return launch_backward<32, 64, kSingle>(a, s);
+    return a.dim % 4 == 0 ? backward_dim<kFours>(a, s) : backward_dim<kClamped>(a, s);
 }
 
 }  // extern "C"

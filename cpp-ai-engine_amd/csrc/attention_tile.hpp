@@ -76,9 +76,31 @@ __device__ __forceinline__ int row_of(int r) {
     return 8 * (r / 4) + 4 * ((int(threadIdx.x) & 63) / 32) + r % 4;
 }
 
+// How a row's `dim` values are read: one by one (fewer than four), four at a time (a multiple of
+// four), or four at a time with the row's last four where a group of four passes its end, which are
+// put in their places afterwards (heads of 77 values, 25 sequences of 120: backward 314 us one by
+// one, 168 for heads of 80).
+enum Reads { kSingle, kFours, kClamped };
+
+// First of the four values that are read for those from d on.
+template <int READS>
+__device__ __forceinline__ int clamped(int d, int dim) {
+    return READS == kClamped ? (d < dim - 4 ? d : dim - 4) : (d < dim ? d : 0);
+}
+// Those from d on, of the four that were read for them; what is past the row's end is anything.
+template <int READS>
+__device__ __forceinline__ void in_place(float* x, int d, int dim) {
+    if (READS != kClamped) return;
+    const int over = d + 4 - dim;
+    const float x1 = x[1], x2 = x[2], x3 = x[3];
+    if (over == 1) x[0] = x1, x[1] = x2, x[2] = x3;
+    if (over == 2) x[0] = x2, x[1] = x3;
+    if (over == 3) x[0] = x3;
+}
+
 // The lane's own row (a pointer to its `dim` values) as the B operand of products over the head's
-// values: DP / 16 blocks. VEC: dim is a multiple of 4.
-template <int DP, bool VEC>
+// values: DP / 16 blocks.
+template <int DP, int READS>
 __device__ __forceinline__ void own_row(const float* row, int dim, float factor,
                                         bf16x8 (&b)[DP / 16][3]) {
     const int half = (int(threadIdx.x) & 63) / 32;
@@ -86,14 +108,18 @@ __device__ __forceinline__ void own_row(const float* row, int dim, float factor,
     for (int ks = 0; ks < DP / 16; ++ks) {
         const int d0 = 16 * ks + 8 * half;
         float x[8];
-        if (VEC) {
-            const floatx4u u = *reinterpret_cast<const floatx4u*>(row + (d0 < dim ? d0 : 0));
-            const floatx4u v =
-                *reinterpret_cast<const floatx4u*>(row + (d0 + 4 < dim ? d0 + 4 : 0));
+        if (READS != kSingle) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[j] = d0 < dim ? u[j] * factor : 0.0f;
-                x[4 + j] = d0 + 4 < dim ? v[j] * factor : 0.0f;
+            for (int g = 0; g < 8; g += 4) {
+                const int d = d0 + g;
+                const floatx4u u =
+                    *reinterpret_cast<const floatx4u*>(row + clamped<READS>(d, dim));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[g + j] = u[j];
+                in_place<READS>(x + g, d, dim);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    x[g + j] = d + (READS == kFours ? 0 : j) < dim ? x[g + j] * factor : 0.0f;
             }
         } else {
 #pragma unroll
@@ -109,14 +135,14 @@ __device__ __forceinline__ void own_row(const float* row, int dim, float factor,
 
 // The product of the lane's own rows of two tensors, each of the two lanes that hold it over half
 // of the values.
-template <int DP, bool VEC>
+template <int DP, int READS>
 __device__ __forceinline__ float own_dot(const float* x, const float* y, int dim) {
     const int half = (int(threadIdx.x) & 63) / 32;
     float s = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
         const int d0 = 16 * ks + 8 * half;
-        if (VEC) {
+        if (READS == kFours) {
 #pragma unroll
             for (int j = 0; j < 8; j += 4) {
                 if (d0 + j >= dim) continue;
@@ -124,6 +150,16 @@ __device__ __forceinline__ float own_dot(const float* x, const float* y, int dim
                 const floatx4u v = *reinterpret_cast<const floatx4u*>(y + d0 + j);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s = __builtin_fmaf(u[e], v[e], s);
+            }
+        } else if (READS == kClamped) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 4) {
+                const int d = d0 + j, first = clamped<READS>(d, dim);
+                const floatx4u u = *reinterpret_cast<const floatx4u*>(x + first);
+                const floatx4u v = *reinterpret_cast<const floatx4u*>(y + first);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)  // of those before d another group has the products
+                    if (first + e >= d) s = __builtin_fmaf(u[e], v[e], s);
             }
         } else {
             for (int j = 0; j < 8; ++j)
@@ -134,16 +170,14 @@ __device__ __forceinline__ float own_dot(const float* x, const float* y, int dim
 }
 
 // Block db (32 values) of the lane's own row of a result, held as a D.
-template <bool VEC>
+template <int READS>
 __device__ __forceinline__ void store_own(float* row, int dim, int db, const floatx16& x) {
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
         const int d = 32 * db + row_of(r);
-        if (VEC) {
-            if (d < dim)
-                *reinterpret_cast<floatx4u*>(row + d) =
-                    floatx4u{x[r], x[r + 1], x[r + 2], x[r + 3]};
-        } else {
+        if (READS == kFours ? d < dim : READS == kClamped && d + 4 <= dim) {
+            *reinterpret_cast<floatx4u*>(row + d) = floatx4u{x[r], x[r + 1], x[r + 2], x[r + 3]};
+        } else if (READS != kFours) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (d + e < dim) row[d + e] = x[r + e];
@@ -158,7 +192,7 @@ __device__ __forceinline__ void store_own(float* row, int dim, int db, const flo
 // the writes of a row's groups, which neighbouring threads hold, on no bank more than twice either;
 // few address bits depend on the lane and the block both, so few addresses are kept. A thread
 // stages up to kUnits units of one row by 8 values.
-template <int ROWS, int DP, int THREADS, bool VEC>
+template <int ROWS, int DP, int THREADS, int READS>
 struct RowTile {
     static constexpr int kGroups = DP / 8;
     static constexpr int kUnits = (ROWS * kGroups + THREADS - 1) / THREADS;
@@ -185,7 +219,7 @@ struct RowTile {
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
             const int r = row(u) < ROWS ? row(u) : 0, d = 8 * group(u);
-            o[u] = 4u * uint32_t(r * ld + (d < dim ? d : 0));
+            o[u] = 4u * uint32_t(r * ld + clamped<READS>(d, dim));
         }
     }
     // The first `left` rows from `base` (left >= 1; rows past them repeat the last).
@@ -193,15 +227,19 @@ struct RowTile {
         const auto at = (global_bytes)base;
 #pragma unroll
         for (int u = 0; u < kUnits; ++u) {
-            if (VEC) {
+            if (READS != kSingle) {
+                const int d = 8 * group(u);
                 uint32_t from = o[u];
                 if (left < ROWS) {
-                    const int r = row(u) < left ? row(u) : left - 1, d = 8 * group(u);
-                    from = 4u * uint32_t(r * ld + (d < dim ? d : 0));
+                    const int r = row(u) < left ? row(u) : left - 1;
+                    from = 4u * uint32_t(r * ld + clamped<READS>(d, dim));
                 }
                 const floatx4u x = global_load<floatx4u>(at + from);
-                const floatx4u y =
-                    global_load<floatx4u>(at + from + (8 * group(u) + 4 < dim ? 16 : 0));
+                const uint32_t next =
+                    READS == kFours
+                        ? (d + 4 < dim ? 16 : 0)
+                        : 4u * uint32_t(clamped<READS>(d + 4, dim) - clamped<READS>(d, dim));
+                const floatx4u y = global_load<floatx4u>(at + from + next);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     v[u][j] = x[j];
@@ -223,10 +261,15 @@ struct RowTile {
         for (int u = 0; u < kUnits; ++u) {
             if ((u + 1) * THREADS > ROWS * kGroups && row(u) >= ROWS) continue;  // no unit
             const bool in = row(u) < left;
+            const int d = 8 * group(u);
             float x[8];
 #pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = v[u][j];
+            in_place<READS>(x, d, dim);
+            in_place<READS>(x + 4, d + 4, dim);
+#pragma unroll
             for (int j = 0; j < 8; ++j)
-                x[j] = CLEAN || (in && 8 * group(u) + (VEC ? j & 4 : j) < dim) ? v[u][j] : 0.0f;
+                x[j] = CLEAN || (in && d + (READS == kFours ? j & 4 : j) < dim) ? x[j] : 0.0f;
             bf16x8 part[3];
             split8(x, part);
 #pragma unroll
