@@ -79,7 +79,7 @@ __device__ __forceinline__ int row_of(int r) {
 // How a row's `dim` values are read: one by one (fewer than four), four at a time (a multiple of
 // four), or four at a time with the row's last four where a group of four passes its end, which are
 // put in their places afterwards (heads of 77 values, 25 sequences of 120: backward 314 us one by
-// one, 168 for heads of 80).
+// one, 196 clamped, 168 for heads of 80).
 enum Reads { kSingle, kFours, kClamped };
 
 // First of the four values that are read for those from d on.

@@ -82,6 +82,15 @@ def test_head_dims(hip, d):
 
 
 @gpu
+@pytest.mark.parametrize("d", [4, 5, 6, 10, 34, 66, 98, 126])
+def test_head_dims_whose_last_four_values_overlap(hip, d):
+    """Every remainder by four, rows as wide as the heads and within a projection's, one row too."""
+    check(hip, [70, 3, 129], [70, 40, 129], 4, 2, d, True, seed=d)
+    check(hip, [33, 64], [33, 64], 2, 1, d, False, seed=d + 1, fused=True)
+    check(hip, [1], [1], 1, 1, d, True, seed=d + 2)
+
+
+@gpu
 @pytest.mark.parametrize("heads,kv", [(1, 1), (8, 1), (5, 5), (9, 3), (16, 2), (12, 12)])
 def test_head_groups_in_a_fused_projection(hip, heads, kv):
     check(hip, [50, 1, 0, 90], [50, 1, 0, 90], heads, kv, 48, True, seed=heads, fused=True)
