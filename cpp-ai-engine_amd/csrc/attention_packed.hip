@@ -338,7 +338,7 @@ __device__ __forceinline__ int64_t piece_of(const Packed& a, int64_t row, int h,
 // the running maximum, sum and weighted values beside them. For long sequences the products bound
 // it (16384 tokens, 8 heads of 128 values, causal: 2.6 to 2.8 ms, 195 to 210 TFLOP/s of 201 that a
 // sixth of a bf16 product of 8192^3 reaches); shorter ones spend as long on exponents and on
-// splitting the weights (16 of 512, 16 heads of 64: 72 to 83 us, the matrix units busy 40 % of it).
+// splitting the weights (16 of 512, 16 heads of 64: 72 to 85 us, the matrix units busy 40 % of it).
 template <int DP, int BN, int WAVES, int READS>
 __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     constexpr int BUFFERS = WAVES / 4;
@@ -588,7 +588,7 @@ __device__ __forceinline__ float* row_dq(const Packed& a, int64_t row, int h, in
 
 // dq_i = scale sum_j ds_ij k_j of heads of up to 64 values, with delta on the way (left in the
 // workspace for the keys' kernel): a wave has room for q and g both, and needs no partner (16 of
-// 512 tokens, 16 heads of 64, causal: 98 to 112 us, bound as the forward).
+// 512 tokens, 16 heads of 64, causal: 98 to 115 us, bound as the forward).
 template <int DP, int BN, int READS>
 __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
     using namespace attention;
@@ -703,7 +703,7 @@ __device__ __forceinline__ uint32_t shared_rows(uint32_t* votes, bool bad) {
 }
 
 // dq and delta of wider heads. Wave role 0 forms s and p, role 1 dp - delta; both then have ds, and
-// half of dq's values each (5576 tokens in 11 sequences, 12 heads of 96 over 4: 189 to 234 us).
+// half of dq's values each (5576 tokens in 11 sequences, 12 heads of 96 over 4: 189 to 238 us).
 template <int DP, int BN, int READS>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed a) {
     using namespace attention;
@@ -854,7 +854,7 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
 }
 
 // dv_j = sum_i p_ij g_i by the waves of role 0, from s and p, and dk_j = scale sum_i ds_ij q_i by
-// those of role 1, from dp and the other's p: 16 of 512 tokens, 16 heads of 64, 143 to 170 us; 5576
+// those of role 1, from dp and the other's p: 16 of 512 tokens, 16 heads of 64, 143 to 173 us; 5576
 // tokens, 12 heads of 96, 234 to 288. Vector work bounds it, the matrix units are busy 36 and 47 %.
 template <int DP, int BN, int READS>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) {
