@@ -482,13 +482,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     }
     // Rows that saw something and have no finite result are formed again by the formula: a NaN or
     // an infinity where it counts, or one in a place of theirs that they do not see (0 times it).
-    const float inv = limit > 0 ? 1.0f / sum : 0.0f;
+    // A row that saw nothing is 0, whatever the keys of its wave's other rows left in its sums.
+    const float inv = 1.0f / sum;
     bool fine = sum > 0.0f && sum < INFINITY;
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            o[db][r] *= inv;
+            o[db][r] = limit > 0 ? o[db][r] * inv : 0.0f;
             fine = fine && fabsf(o[db][r]) < INFINITY;
         }
     fine = fine || limit == 0;

@@ -555,6 +555,28 @@ def test_empty_tensors(hip):
                                                                device="cuda"))
 
 
+# ------------------------------------------- rows, scales and sizes of their own kind
+
+@gpu
+@pytest.mark.parametrize("d", [3, 24, 64, 67, 96, 128])
+def test_rows_without_keys_beside_keys_that_are_not_finite(hip, d):
+    """The first 30 queries see no key; the wave that holds them also has queries that do."""
+    import torch
+    print_case("packed keyless beside not finite", d)
+    q, k, v, g = make([70, 5], [40, 5], 2, 1, d, seed=60 + d)
+    cq, ck = offsets([70, 5]), offsets([40, 5])
+    for at, value in ((0, math.nan), (0, math.inf), (17, -math.inf)):
+        kx, vx = k.clone(), v.clone()
+        vx[at] = value
+        for keys in (k, kx):
+            out, lse = hip.attention_packed(q, keys, vx, cq, ck)
+            dq = hip.attention_packed_backward(g, q, keys, vx, out, lse, cq, ck,
+                                               want=(True, False, False))[0]
+            assert bool((out[:30] == 0).all()) and bool((lse[:30] == -math.inf).all())
+            assert bool((dq[:30] == 0).all())
+            kx[at] = value  # the second time the key itself too
+
+
 # ----------------------------------------------------------------- refusals
 
 def descriptor(**changes):
