@@ -372,11 +372,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     const int wave_end = 32 * wave < t.rows ? min(visible(a, t, t.first + last), end) : 0;
     const int wave_all = visible(a, t, t.first + 32 * wave);  // keys that all its queries see
 
-    // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q.
-    const float c2 = fabsf(a.scale) * 1.44269504088896340736f;
+    // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q, and so does a scale of
+    // 0, with which a masked score's -inf would be NaN.
+    const float c2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.44269504088896340736f;
     bf16x8 q[DP / 16][3];
     own_row<DP, READS>(a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim, a.dim,
-                     a.scale < 0.0f ? -1.0f : 1.0f, q);
+                       a.scale < 0.0f ? -1.0f : (a.scale > 0.0f ? 1.0f : a.scale), q);
     char* const parked = lds + BUFFERS * kTile + (wave * (DP / 16) * 64 + lane) * 16;
     if constexpr (kPark) {
 #pragma unroll

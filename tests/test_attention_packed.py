@@ -577,6 +577,28 @@ def test_rows_without_keys_beside_keys_that_are_not_finite(hip, d):
             kx[at] = value  # the second time the key itself too
 
 
+@gpu
+@pytest.mark.parametrize("nq,nk", [([70, 40], [40, 70]), ([300], [900]), ([900], [500])])
+def test_scale_of_zero(hip, nq, nk):
+    """Even weights over what a row sees, zeros where that is nothing, and the bits of a scale that
+    is too small to matter: the same arithmetic, but for lse of one key, which is scale times its
+    score: 0 or some 1e-30."""
+    import torch
+    print_case("packed scale 0", nq, nk)
+    q, k, v, g = make(nq, nk, 4, 2, 64, seed=61)
+    cq, ck = offsets(nq), offsets(nk)
+    got = []
+    for scale in (0.0, 1e-30):
+        out, lse = hip.attention_packed(q, k, v, cq, ck, scale=scale)
+        dv = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck, scale=scale)[2]
+        got.append((out, lse, dv))
+    for n in (0, 2):
+        assert bool(torch.equal(got[0][n], got[1][n])), ("out", "lse", "dv")[n]
+    value, bound = packed(q, k, v, nq, nk, 0.0, True, g)
+    for name, x in zip(("out", "lse", "dv"), got[0]):
+        within(x, value[name], bound[name], name)
+
+
 # ----------------------------------------------------------------- refusals
 
 def descriptor(**changes):
