@@ -184,136 +184,211 @@ __device__ __forceinline__ float wave_sum(float x) {
     return x;
 }
 
-__device__ __forceinline__ float dot(const float* __restrict__ x, const float* __restrict__ y,
-                                     int n) {
+// ------------------------------------------------------- one row by one wave
+// The formulas as they stand, for rows whose tiles gave no finite result; only what the row sees is
+// read. Sixteen lanes take one streamed row, its values 16 apart, so that a wave reads four rows at
+// a time and U times four ahead: a NaN or an infinity that every row sees has all rows formed here,
+// and then the reads' latency bounds a call (4 sequences of 512, 8 heads of 64, the first key
+// infinite: 168 us forward and 708 backward; without it 43 and 86; a lane for each key took 760 and
+// 4750). Where a score, lse or delta settles the row as NaN nothing else is read (first key NaN: 39
+// and 101 us, 767 and 4750 without that).
+
+constexpr int kRowLanes = 16, kRowColumns = kMaxDim / kRowLanes;
+
+// A lane's values of a row of `dim`, 0 past its end.
+struct Columns {
+    float x[kRowColumns];
+
+    __device__ __forceinline__ void load(const float* row, int dim) {
+        const int d = int(threadIdx.x) % kRowLanes;
+#pragma unroll
+        for (int e = 0; e < kRowColumns; ++e) {
+            x[e] = 0.0f;
+            if (kRowLanes * e < dim && d + kRowLanes * e < dim) x[e] = row[d + kRowLanes * e];
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int e = 0; e < kRowColumns; ++e) x[e] = 0.0f;
+    }
+    __device__ __forceinline__ void add(float w, const Columns& y) {
+#pragma unroll
+        for (int e = 0; e < kRowColumns; ++e) x[e] = __builtin_fmaf(w, y.x[e], x[e]);
+    }
+    // The four groups' sums, times `factor`, into a row; or one value for all of it.
+    __device__ __forceinline__ void store(float* row, int dim, float factor) {
+        const int d = int(threadIdx.x) % kRowLanes, group = (int(threadIdx.x) & 63) / kRowLanes;
+#pragma unroll
+        for (int e = 0; e < kRowColumns; ++e) {
+            if (kRowLanes * e >= dim) break;
+            float y = x[e];
+            y += __shfl_xor(y, 16);
+            y += __shfl_xor(y, 32);
+            if (group == 0 && d + kRowLanes * e < dim) row[d + kRowLanes * e] = y * factor;
+        }
+    }
+    __device__ __forceinline__ static void fill(float* row, int dim, float value) {
+        for (int d = int(threadIdx.x) & 63; d < dim; d += 64) row[d] = value;
+    }
+};
+
+// The product of two rows, in each of their sixteen lanes.
+__device__ __forceinline__ float dot(const Columns& x, const Columns& y) {
     float s = 0.0f;
-    for (int c = 0; c < n; ++c) s = __builtin_fmaf(x[c], y[c], s);
+#pragma unroll
+    for (int e = 0; e < kRowColumns; ++e) s = __builtin_fmaf(x.x[e], y.x[e], s);
+#pragma unroll
+    for (int o = kRowLanes / 2; o > 0; o >>= 1) s += __shfl_xor(s, o);
     return s;
 }
 
-// ------------------------------------------------------- one row by one wave
-// The formulas as they stand, a lane for a key (or query) at a time and then a lane for a column;
-// only what the row sees is read.
+// Rows j0 + the lane's group, and every fourth after it, of those before n (the last again past it).
+template <int U>
+__device__ __forceinline__ void load_rows(Columns (&x)[U], const float* base, int64_t ld,
+                                          int64_t j0, int64_t n, int dim) {
+    const int group = (int(threadIdx.x) & 63) / kRowLanes;
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u].load(base + min(j0 + 4 * u + group, n - 1) * ld, dim);
+}
+__device__ __forceinline__ bool row_is_there(int64_t j0, int u, int64_t n) {
+    return j0 + 4 * u + (int(threadIdx.x) & 63) / kRowLanes < n;
+}
 
+template <int U>
 __device__ void forward_row(const Packed& a, const Tile& t, int h, int i) {
-    const int lane = int(threadIdx.x) & 63;
     const int n = visible(a, t, i), c = h / (a.heads / a.kv_heads);
-    const float* q = a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim;
     const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
-    float m = -INFINITY;
-    bool bad = false;  // a score that is NaN: fmaxf passes over it
-    for (int j = lane; j < n; j += 64) {
-        const float s = dot(q, k + j * a.ld_k, a.dim) * a.scale;
-        m = fmaxf(m, s);
-        bad |= s != s;
-    }
-    m = wave_max(m);
-    if (__any(bad)) m = NAN;
-    const float shift = m == -INFINITY ? 0.0f : m;  // scores of -inf alone: lse = -inf, out 0 / 0
-    float sum = 0.0f, acc[2] = {0.0f, 0.0f};
-    for (int j = lane; j < n; j += 64) sum += expf(dot(q, k + j * a.ld_k, a.dim) * a.scale - shift);
-    sum = wave_sum(sum);
-    for (int j0 = 0; j0 < n; j0 += 64) {
-        const int j = j0 + lane;
-        float p = 0.0f;  // divided here: the sums stay in range with v's values
-        if (j < n) p = expf(dot(q, k + j * a.ld_k, a.dim) * a.scale - shift) / sum;
-        const int count = n - j0 < 64 ? n - j0 : 64;
-        for (int u = 0; u < count; ++u) {
-            const float w = __shfl(p, u);
-            const float* row = v + (j0 + u) * a.ld_v;
+    float* const out = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
+    Columns q;
+    q.load(a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim, a.dim);
+    // A group's running maximum and sum; a score of NaN or +inf settles the row.
+    float m = -INFINITY, sum = 0.0f;
+    bool settled = false;
+    for (int64_t j0 = 0; j0 < n && !settled; j0 += 4 * U) {
+        Columns x[U];
+        load_rows(x, k, a.ld_k, j0, n, a.dim);
+        float s[U], top = m;
+        bool bad = false;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (lane + 64 * e < a.dim) acc[e] = __builtin_fmaf(w, row[lane + 64 * e], acc[e]);
+        for (int u = 0; u < U; ++u) {
+            s[u] = dot(q, x[u]) * a.scale;
+            if (!row_is_there(j0, u, n)) s[u] = -INFINITY;
+            bad |= !(s[u] < INFINITY);
+            top = fmaxf(top, s[u]);
+        }
+        settled = __any(bad);
+        const float shift = top == -INFINITY ? 0.0f : top;
+        sum *= expf(m - shift);  // -inf - 0 where there was nothing yet
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum += expf(s[u] - shift);
+        m = top;
+    }
+    float top = fmaxf(m, __shfl_xor(m, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    sum *= expf(m - (top == -INFINITY ? 0.0f : top));
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if ((threadIdx.x & 63) == 0)
+        a.lse[int64_t(t.q0 + i) * a.heads + h] = settled            ? NAN
+                                                 : top == -INFINITY ? -INFINITY
+                                                                    : top + logf(sum);
+    if (settled || top == -INFINITY) {  // of scores of -inf alone: 0 / 0
+        Columns::fill(out, a.dim, n == 0 ? 0.0f : NAN);
+        return;
+    }
+    Columns o;
+    o.clear();
+    for (int64_t j0 = 0; j0 < n; j0 += 4 * U) {
+        Columns x[U], y[U];
+        load_rows(x, k, a.ld_k, j0, n, a.dim);
+        load_rows(y, v, a.ld_v, j0, n, a.dim);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // Divided here: the sums stay in range with v's values.
+            const float p = expf(dot(q, x[u]) * a.scale - top) / sum;
+            if (row_is_there(j0, u, n)) o.add(p, y[u]);
         }
     }
-    float* out = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-        if (lane + 64 * e < a.dim) out[lane + 64 * e] = acc[e];
-    if (lane == 0)
-        a.lse[int64_t(t.q0 + i) * a.heads + h] = n == 0 ? -INFINITY : m + logf(sum);
+    o.store(out, a.dim, 1.0f);
 }
 
-// ds_ij, and p_ij through p.
-__device__ __forceinline__ float pair_gradient(const Packed& a, const float* q, const float* g,
-                                               const float* k, const float* v, float lse,
-                                               float delta, float& p) {
-    p = expf(dot(q, k, a.dim) * a.scale - lse);
-    return p * (dot(g, v, a.dim) - delta);
-}
-
-// Of keys [begin, end).
+// The share of keys [begin, end).
 __device__ void dq_row(const Packed& a, const Tile& t, int h, int i, float delta, int begin,
                        int end, float* dq) {
-    const int lane = int(threadIdx.x) & 63;
+    constexpr int U = 4;
     const int n = min(visible(a, t, i), end), c = h / (a.heads / a.kv_heads);
     const int64_t row = t.q0 + i;
-    const float* q = a.q + row * a.ld_q + int64_t(h) * a.dim;
-    const float* g = a.grad + row * a.ld_grad + int64_t(h) * a.dim;
     const float* k = a.k + int64_t(t.k0) * a.ld_k + int64_t(c) * a.dim;
     const float* v = a.v + int64_t(t.k0) * a.ld_v + int64_t(c) * a.dim;
     const float lse = a.lse[row * a.heads + h];
-    float acc[2] = {0.0f, 0.0f};
-    for (int j0 = begin; j0 < n; j0 += 64) {
-        const int j = j0 + lane;
-        float p, ds = 0.0f;
-        if (j < n) ds = pair_gradient(a, q, g, k + j * a.ld_k, v + j * a.ld_v, lse, delta, p);
-        const int count = n - j0 < 64 ? n - j0 : 64;
-        for (int u = 0; u < count; ++u) {
-            const float w = __shfl(ds, u);
-            const float* x = k + (j0 + u) * a.ld_k;
+    if (begin < n && (lse != lse || delta != delta)) {  // every ds is
+        Columns::fill(dq, a.dim, NAN);
+        return;
+    }
+    Columns q, g, sum;
+    q.load(a.q + row * a.ld_q + int64_t(h) * a.dim, a.dim);
+    g.load(a.grad + row * a.ld_grad + int64_t(h) * a.dim, a.dim);
+    sum.clear();
+    for (int64_t j0 = begin; j0 < n; j0 += 4 * U) {
+        Columns x[U], y[U];
+        load_rows(x, k, a.ld_k, j0, n, a.dim);
+        load_rows(y, v, a.ld_v, j0, n, a.dim);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (lane + 64 * e < a.dim) acc[e] = __builtin_fmaf(w, x[lane + 64 * e], acc[e]);
+        for (int u = 0; u < U; ++u) {
+            const float ds = expf(dot(q, x[u]) * a.scale - lse) * (dot(g, y[u]) - delta);
+            if (row_is_there(j0, u, n)) sum.add(ds, x[u]);
         }
     }
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-        if (lane + 64 * e < a.dim) dq[lane + 64 * e] = acc[e] * a.scale;
+    sum.store(dq, a.dim, a.scale);
 }
 
-// Query head h's share of queries [begin, end), into rows dk and dv of `dim` values (either may be
-// null).
-__device__ void dkv_row(const Packed& a, const Tile& t, int h, int j, int begin, int end, float* dk,
-                        float* dv) {
-    const int c = h / (a.heads / a.kv_heads);
-    const int lane = int(threadIdx.x) & 63;
+// Query head h's share of queries [begin, end) in dk (KEYS) or dv of key j.
+template <bool KEYS>
+__device__ void dkv_row(const Packed& a, const Tile& t, int h, int j, int begin, int end,
+                        float* to) {
+    constexpr int U = 4;
+    const int c = h / (a.heads / a.kv_heads), lane = int(threadIdx.x) & 63;
     const int64_t row = t.k0 + j;
-    const float* k = a.k + row * a.ld_k + int64_t(c) * a.dim;
-    const float* v = a.v + row * a.ld_v + int64_t(c) * a.dim;
     // The first query that sees key j.
     int64_t start = a.causal ? int64_t(j) - t.nk + t.nq : 0;
     start = start < begin ? begin : start;
-    float ak[2] = {0.0f, 0.0f}, av[2] = {0.0f, 0.0f};
-    for (int64_t i0 = start; i0 < end; i0 += 64) {
-        const int64_t i = i0 + lane;
-        float p = 0.0f, ds = 0.0f;
-        if (i < end) {
-            const int64_t at = t.q0 + i;
-            ds = pair_gradient(a, a.q + at * a.ld_q + int64_t(h) * a.dim,
-                               a.grad + at * a.ld_grad + int64_t(h) * a.dim, k, v,
-                               a.lse[at * a.heads + h], a.delta[at * a.heads + h], p);
-        }
-        const int count = end - i0 < 64 ? int(end - i0) : 64;
-        for (int u = 0; u < count; ++u) {
-            const float wp = __shfl(p, u), wd = __shfl(ds, u);
-            const float* x = a.q + (t.q0 + i0 + u) * a.ld_q + int64_t(h) * a.dim;
-            const float* g = a.grad + (t.q0 + i0 + u) * a.ld_grad + int64_t(h) * a.dim;
+    const float* lse = a.lse + int64_t(t.q0) * a.heads + h;
+    const float* delta = a.delta + int64_t(t.q0) * a.heads + h;
+    bool settled = false;  // a query whose every p, or ds, is NaN
+    for (int64_t i0 = start; i0 < end && !settled; i0 += 64) {
+        const int64_t i = min(i0 + lane, int64_t(end) - 1) * a.heads;
+        settled = __any(lse[i] != lse[i] || (KEYS && delta[i] != delta[i]));
+    }
+    if (settled) {
+        Columns::fill(to, a.dim, NAN);
+        return;
+    }
+    const float* q = a.q + int64_t(t.q0) * a.ld_q + int64_t(h) * a.dim;
+    const float* g = a.grad + int64_t(t.q0) * a.ld_grad + int64_t(h) * a.dim;
+    Columns k, v, sum;
+    k.load(a.k + row * a.ld_k + int64_t(c) * a.dim, a.dim);
+    if (KEYS) v.load(a.v + row * a.ld_v + int64_t(c) * a.dim, a.dim);
+    sum.clear();
+    for (int64_t i0 = start; i0 < end; i0 += 4 * U) {
+        Columns x[U], y[U];
+        float z[U], d[U];
+        load_rows(x, q, a.ld_q, i0, end, a.dim);
+        load_rows(y, g, a.ld_grad, i0, end, a.dim);
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (lane + 64 * e < a.dim) {
-                    ak[e] = __builtin_fmaf(wd, x[lane + 64 * e], ak[e]);
-                    av[e] = __builtin_fmaf(wp, g[lane + 64 * e], av[e]);
-                }
+        for (int u = 0; u < U; ++u) {
+            const int64_t i = min(i0 + 4 * u + lane / kRowLanes, int64_t(end) - 1) * a.heads;
+            z[u] = lse[i];
+            d[u] = KEYS ? delta[i] : 0.0f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float w = expf(dot(k, x[u]) * a.scale - z[u]);
+            if (KEYS) w *= dot(v, y[u]) - d[u];
+            if (row_is_there(i0, u, end)) sum.add(w, KEYS ? x[u] : y[u]);
         }
     }
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-        if (lane + 64 * e < a.dim) {
-            if (dk != nullptr) dk[lane + 64 * e] = ak[e] * a.scale;
-            if (dv != nullptr) dv[lane + 64 * e] = av[e];
-        }
+    sum.store(to, a.dim, KEYS ? a.scale : 1.0f);
 }
 
 // ------------------------------------------------------------------- kernels
@@ -494,8 +569,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
             fine = fine && fabsf(o[db][r]) < INFINITY;
         }
     fine = fine || limit == 0;
-    const uint64_t again = __ballot(!fine && mine < t.rows);
-    if (mine < t.rows) {
+    const uint64_t votes = __ballot(!fine && mine < t.rows);
+    const uint32_t again = uint32_t(votes) | uint32_t(votes >> 32);
+    if (mine < t.rows && !(again >> (lane & 31) & 1)) {
         float* out = a.out + int64_t(t.q0 + i) * a.ld_out + int64_t(h) * a.dim;
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) store_own<READS>(out, a.dim, db, o[db]);
@@ -504,8 +580,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
                 limit == 0 ? -INFINITY
                            : lse_of(shift, sum);
     }
-    for (uint32_t rows = uint32_t(again) | uint32_t(again >> 32); rows != 0; rows &= rows - 1)
-        forward_row(a, t, h, t.first + 32 * wave + __builtin_ctz(rows));
+    for (uint32_t rows = again; rows != 0; rows &= rows - 1)
+        forward_row<4>(a, t, h, t.first + 32 * wave + __builtin_ctz(rows));
 }
 
 // The rows' pieces. One wave a row and head, two values a lane: latency (66912 rows of 96 values in
@@ -575,7 +651,8 @@ __global__ __launch_bounds__(kThreads) void packed_forward_join(Packed a) {
         n = in ? n - n / 2 : n / 2;
     }
     const Tile t = tile_of(a, false, lo, 0, kRows);
-    if (row - t.q0 < t.nq) forward_row(a, t, h, row - t.q0);
+    // One row ahead: more registers would leave fewer waves for the rows that are fine.
+    if (row - t.q0 < t.nq) forward_row<1>(a, t, h, row - t.q0);
 }
 
 // The backward forms s, and so p_ij, again from the inputs, and dp likewise, for the pairs of a
@@ -675,12 +752,13 @@ __global__ __launch_bounds__(kThreads, 2) void packed_backward_q(Packed a) {
             dq[db][r] = limit > 0 ? dq[db][r] * a.scale : 0.0f;
             fine = fine && fabsf(dq[db][r]) < INFINITY;
         }
-    const uint64_t again = __ballot(!fine && mine < t.rows);
-    if (mine < t.rows)
+    const uint64_t votes = __ballot(!fine && mine < t.rows);
+    const uint32_t again = uint32_t(votes) | uint32_t(votes >> 32);
+    if (mine < t.rows && !(again >> (lane & 31) & 1))
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db)
             store_own<READS>(row_dq(a, row, h, piece), a.dim, db, dq[db]);
-    for (uint32_t rows = uint32_t(again) | uint32_t(again >> 32); rows != 0; rows &= rows - 1) {
+    for (uint32_t rows = again; rows != 0; rows &= rows - 1) {
         const int r = __builtin_ctz(rows);
         dq_row(a, t, h, t.first + 32 * wave + r, __shfl(delta, r), begin, end,
                row_dq(a, t.q0 + t.first + 32 * wave + r, h, piece));
@@ -1025,29 +1103,27 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) 
             sum[d][r] *= factor;
             fine = fine && fabsf(sum[d][r]) < INFINITY;
         }
-    const uint32_t again =
-        shared_rows(reinterpret_cast<uint32_t*>(lds), wanted && !fine && mine < t.rows);
-    // Where the rows of dk (or dv) of key j go.
-    const auto row_dk = [&](int64_t at) {
-        return a.part_k != nullptr ? a.part_k + ((at * a.heads + h) * a.pieces_k + piece) * a.dim
-               : a.dk == nullptr   ? nullptr
-                                   : a.dk + at * a.ld_dk + int64_t(c) * a.dim;
+    const uint64_t votes = __ballot(wanted && !fine && mine < t.rows);
+    const uint32_t again = uint32_t(votes) | uint32_t(votes >> 32);
+    // Where the wave's gradient of key row `at` goes.
+    float* const part = role == 0 ? a.part_v : a.part_k;
+    float* const whole = role == 0 ? a.dv : a.dk;
+    const int64_t ld = role == 0 ? a.ld_dv : a.ld_dk;
+    const auto row_to = [&](int64_t at) {
+        return part != nullptr ? part + ((at * a.heads + h) * a.pieces_k + piece) * a.dim
+                               : whole + at * ld + int64_t(c) * a.dim;
     };
-    const auto row_dv = [&](int64_t at) {
-        return a.part_v != nullptr ? a.part_v + ((at * a.heads + h) * a.pieces_k + piece) * a.dim
-               : a.dv == nullptr   ? nullptr
-                                   : a.dv + at * a.ld_dv + int64_t(c) * a.dim;
-    };
-    float* const out = role == 0 ? row_dv(row) : row_dk(row);
     if (wanted && mine < t.rows && !(again >> (lane & 31) & 1)) {
+        float* const out = row_to(row);
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) store_own<READS>(out, a.dim, d, sum[d]);
     }
-    if (role == 0)
-        for (uint32_t rows = again; rows != 0; rows &= rows - 1) {
-            const int64_t key = t.first + w0 + __builtin_ctz(rows);
-            dkv_row(a, t, h, int(key), start, end, row_dk(t.k0 + key), row_dv(t.k0 + key));
-        }
+    for (uint32_t rows = again; rows != 0; rows &= rows - 1) {
+        const int key = t.first + w0 + __builtin_ctz(rows);
+        float* const out = row_to(t.k0 + key);
+        if (role == 0) dkv_row<false>(a, t, h, key, start, end, out);
+        else dkv_row<true>(a, t, h, key, start, end, out);
+    }
 }
 
 // Rows of one gradient, or of dk and dv, from `count` shares of each head's row one after the

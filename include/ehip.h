@@ -893,7 +893,9 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  * over the keys seen. A row that sees none gets out = 0 and lse = -inf, and
  * gives no gradient; one whose scores are all -inf has lse = -inf and out NaN.
  * out and lse may not overlap the inputs. Keys that a row does not see do not
- * reach it, whatever they hold (NaN and infinities included). Rows of q past
+ * reach it, whatever they hold (NaN and infinities included). Rows that meet an
+ * infinity, or a NaN that is not in a score, are formed a second time one by
+ * one: a call in which most do takes up to some 25 times as long. Rows of q past
  * the last sequence leave out, lse and dq as they were, rows of k past it dk
  * and dv.
  *

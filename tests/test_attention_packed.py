@@ -599,6 +599,65 @@ def test_scale_of_zero(hip, nq, nk):
         within(x, value[name], bound[name], name)
 
 
+@gpu
+@pytest.mark.parametrize("d", [33, 64, 128])
+@pytest.mark.parametrize("nq,nk", [([90, 40], [90, 60]), ([400, 3], [700, 500])])
+@pytest.mark.parametrize("which,value", [("q", math.nan), ("k", math.nan), ("v", math.nan),
+                                         ("v", math.inf), ("g", math.nan), ("g", -math.inf)])
+def test_gradients_of_what_is_not_finite(hip, which, value, nq, nk, d):
+    """NaN and infinities in one value of one row: they are where the formula has them, the gradients
+    of other heads and of rows that do not meet it are as ever."""
+    import torch
+    print_case("packed gradients not finite", which, value, nq, nk, d)
+    data = dict(zip("qkvg", make(nq, nk, 4, 2, d, seed=65 + d)))
+    data[which][50, 1, d - 2] = value
+    q, k, v, g = (data[n] for n in "qkvg")
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = hip.attention_packed(q, k, v, cq, ck)
+    grads = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck)
+    value, bound = packed(q, k, v, nq, nk, d ** -0.5, True, g)
+    for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+        within(got, value[name], bound[name], name)
+
+
+@gpu
+def test_a_step_that_is_not_finite_takes_no_longer(hip):
+    """A NaN that every row sees, in a key or everywhere, and not many times a finite call's time:
+    rows formed again one by one took 18 times the forward's and 55 times the backward's."""
+    import torch
+    print_case("packed time of NaN")
+    n = [512] * 4
+    q, k, v, g = make(n, n, 8, 8, 64, seed=66)
+    cu = offsets(n)
+
+    def took():
+        """The least of five, in ms, of the forward and of the backward."""
+        calls, best = [], [math.inf, math.inf]
+        out, lse = hip.attention_packed(q, k, v, cu)
+        calls.append(lambda: hip.attention_packed(q, k, v, cu))
+        calls.append(lambda: hip.attention_packed_backward(g, q, k, v, out, lse, cu))
+        for _ in range(5):
+            for i, call in enumerate(calls):
+                a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+                a.record()
+                call()
+                b.record()
+                torch.cuda.synchronize()
+                best[i] = min(best[i], a.elapsed_time(b))
+        return best
+
+    took()
+    finite = took()
+    k[0] = math.nan
+    one = took()
+    for t in (q, k, v, g):
+        t.fill_(math.nan)
+    every = took()
+    print(finite, one, every, flush=True)
+    for x in (one, every):
+        assert x[0] < 8 * finite[0] and x[1] < 8 * finite[1]
+
+
 # ----------------------------------------------------------------- refusals
 
 def descriptor(**changes):
