@@ -23,6 +23,8 @@ constexpr int kThreads = 256;
 constexpr int kRows = 128;  // rows (queries or keys) of one block, 32 a wave
 
 struct Packed {
+    // What the host shares out the work by: a sequence's rows, and how many such there are.
+    int64_t each_q, each_k, count_q, count_k;
     const float *q, *k, *v;
     int64_t ld_q, ld_k, ld_v;
     const int32_t *cu_q, *cu_k;
@@ -1165,6 +1167,13 @@ int64_t slots(int64_t total, int64_t sequences, int rows = kRows) {
     return total / rows + sequences;
 }
 
+// Rows are taken to be in sequences of the mean length, or, where the longest is known, in as many of
+// that length as they make: a long one among short or empty ones then counts as itself.
+void share(int64_t total, int64_t sequences, int64_t longest, int64_t& each, int64_t& count) {
+    each = longest > 0 ? std::min(longest, total) : sequences == 0 ? 0 : total / sequences;
+    count = longest > 0 ? std::min(sequences, ceil_div(total, longest)) : sequences;
+}
+
 // Tiles address their rows by 32-bit byte offsets from the first one.
 constexpr int64_t kMaxLd = int64_t(1) << 22;
 
@@ -1182,6 +1191,9 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
         slots(d->total_q > d->total_k ? d->total_q : d->total_k, d->sequences) * d->heads > kBlocks)
         return fail(EHIP_EINVAL, "%s: %lld x %lld rows of %lld heads are too many", name,
                     (long long)d->total_q, (long long)d->total_k, (long long)d->heads);
+    if (d->longest_q < 0 || d->longest_k < 0)
+        return fail(EHIP_EINVAL, "%s: longest sequences of %lld and %lld rows", name,
+                    (long long)d->longest_q, (long long)d->longest_k);
     const int64_t wide = d->heads * d->head_dim, narrow = d->kv_heads * d->head_dim;
     if (d->ld_q < wide || d->ld_out < wide || d->ld_k < narrow || d->ld_v < narrow ||
         d->ld_q > kMaxLd || d->ld_k > kMaxLd || d->ld_v > kMaxLd)
@@ -1193,6 +1205,8 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
         (d->total_k > 0 && (d->k == nullptr || d->v == nullptr)))
         return fail(EHIP_EINVAL, "%s: null tensor", name);
     a = Packed{};
+    share(d->total_q, d->sequences, d->longest_q, a.each_q, a.count_q);
+    share(d->total_k, d->sequences, d->longest_k, a.each_k, a.count_k);
     a.q = d->q;
     a.k = d->k;
     a.v = d->v;
@@ -1239,10 +1253,22 @@ int launch_forward(const Packed& a, hipStream_t s) {
 // 8 heads, 490 : 566). Heads over 96 values spill with 128, and take them for short causal ones
 // alone (64 of 128 87 : 103; one of 4096 593 : 509; without the mask 64 of 128 136 : 82).
 bool narrow_blocks(const Packed& a) {
-    const int64_t n = a.total_q, s_count = a.sequences, blocks = n / 256 * a.heads;
-    return a.dim > 96 ? a.causal && n < 256 * s_count
-           : a.causal ? n < 2048 * s_count || blocks < 512
+    const int64_t blocks = a.total_q / 256 * a.heads;
+    return a.dim > 96 ? a.causal && a.each_q < 256
+           : a.causal ? a.each_q < 2048 || blocks < 512
                       : blocks < 256;
+}
+
+// Pieces for `want` blocks in all where the tiles make `blocks` of them and pass `rows` rows, of
+// kLeastPiece rows or more; and no more than make kMostBlocks of those launched, most of which have
+// no tile where few of the sequences are long (8 heads of 128, 128 queries behind 16384 keys beside
+// 43 of one each, us whole 2052, for 4096 209, 8192 126, 16384 125; 500 behind 4000 beside 200 of
+// one 521, 369, 208, 249).
+constexpr int64_t kMostBlocks = 8192;
+int pieces_for(int64_t want, int64_t blocks, int64_t launched, int64_t rows) {
+    if (rows < 384) return 1;
+    const int64_t most = std::min({rows / kLeastPiece, int64_t(32), kMostBlocks / launched});
+    return int(std::max<int64_t>(1, std::min((want + blocks / 2) / blocks, most)));
 }
 
 // Pieces of a tile's keys, where the tiles alone leave CUs without work: for 512 blocks in all, or
@@ -1253,13 +1279,11 @@ bool narrow_blocks(const Packed& a) {
 // Sequences that are shorter do not make up for the second launch (4 of 256, 4 heads of 64, 18.6
 // whole, 21.2 in two).
 int pieces_of(const Packed& a) {
-    const int64_t mean = a.sequences == 0 ? 0 : a.total_k / a.sequences;
-    if (mean < 384) return 1;
     const bool narrow = narrow_blocks(a);
-    const int64_t blocks = slots(a.total_q, a.sequences, narrow ? 128 : 256) * a.heads;
-    const int64_t want = narrow && a.causal && blocks >= 256 ? 1024 : 512;
-    const int64_t most = std::min<int64_t>(mean / kLeastPiece, 32);
-    return int(std::max<int64_t>(1, std::min((want + blocks / 2) / blocks, most)));
+    const int rows = narrow ? 128 : 256;
+    const int64_t blocks = slots(a.total_q, a.count_k, rows) * a.heads;
+    return pieces_for(narrow && a.causal && blocks >= 256 ? 1024 : 512, blocks,
+                      slots(a.total_q, a.sequences, rows) * a.heads, a.each_k);
 }
 
 size_t piece_bytes(const Packed& a) {
@@ -1280,13 +1304,9 @@ int forward_of(const Packed& a, hipStream_t s) {
 // values: one sequence of 4096 584 : 572 : 416; 128 queries behind 4096 keys 327 : 78 : 76; without
 // the mask one of 2048 311 : 193 : 201, 8 of 512 117 : 113 : 136; heads of 96, 8 of 512 143 : 139 :
 // 208).
-int backward_pieces(const Packed& a, int64_t rows, int64_t passed) {
-    const int64_t mean = a.sequences == 0 ? 0 : passed / a.sequences;
-    if (mean < 384) return 1;
-    const int64_t blocks = slots(rows, a.sequences) * a.heads;
-    const int64_t want = a.causal ? 512 : 256;
-    const int64_t most = std::min<int64_t>(mean / kLeastPiece, 32);
-    return int(std::max<int64_t>(1, std::min((want + blocks / 2) / blocks, most)));
+int backward_pieces(const Packed& a, int64_t rows, int64_t each, int64_t count) {
+    return pieces_for(a.causal ? 512 : 256, slots(rows, count) * a.heads,
+                      slots(rows, a.sequences) * a.heads, each);
 }
 
 // Shares of dq, and of each of dk and dv. dk and dv of grouped heads are formed head by head, for
@@ -1298,8 +1318,8 @@ struct BackwardSpace {
 };
 BackwardSpace space_of(const Packed& a) {
     BackwardSpace x;
-    x.pieces_q = backward_pieces(a, a.total_q, a.total_k);
-    x.pieces_k = backward_pieces(a, a.total_k, a.total_q);
+    x.pieces_q = backward_pieces(a, a.total_q, a.each_k, a.count_k);
+    x.pieces_k = backward_pieces(a, a.total_k, a.each_q, a.count_q);
     const auto aligned = [](size_t n) { return (n + 15) & ~size_t(15); };
     const size_t row = size_t(a.heads) * sizeof(float), dim = size_t(a.dim);
     x.delta = aligned(size_t(a.total_q) * row);

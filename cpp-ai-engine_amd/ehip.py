@@ -88,7 +88,8 @@ class AttentionPacked(C.Structure):
                 ("cu_k", C.c_void_p), ("sequences", C.c_int64), ("total_q", C.c_int64),
                 ("total_k", C.c_int64), ("heads", C.c_int64), ("kv_heads", C.c_int64),
                 ("head_dim", C.c_int64), ("scale", C.c_float), ("causal", C.c_int),
-                ("out", C.c_void_p), ("ld_out", C.c_int64), ("lse", C.c_void_p)]
+                ("out", C.c_void_p), ("ld_out", C.c_int64), ("lse", C.c_void_p),
+                ("longest_q", C.c_int64), ("longest_k", C.c_int64)]
 
 
 class Cache(C.Structure):
@@ -816,12 +817,14 @@ class Backend:
         w = self.torch.empty(n, dtype=self.torch.uint8, device="cuda")
         return w, _vp(w.data_ptr()), n
 
-    def _packed(self, q, k, v, cu_q, cu_k, scale, causal, out, lse):
+    def _packed(self, q, k, v, cu_q, cu_k, scale, causal, out, lse, longest_q=None,
+                longest_k=None):
         if q.dim() != 3 or k.dim() != 3:
             raise ValueError("q and k: expected (tokens, heads, head_dim)")
         self._here(q, k, v, cu_q, cu_k, out, lse)
         (tq, h, d), (tk, kv) = q.shape, k.shape[:2]
-        cu_k = cu_q if cu_k is None else cu_k
+        if cu_k is None:
+            cu_k, longest_k = cu_q, longest_k or longest_q
         sequences = cu_q.numel() - 1
         if sequences < 0:
             raise ValueError("cu_q: expected one offset more than sequences")
@@ -830,7 +833,8 @@ class Backend:
             self._rows(k, "k", (tk, kv, d)), self._rows(v, "v", (tk, kv, d)),
             self._index(cu_q, "cu_q", sequences + 1), self._index(cu_k, "cu_k", sequences + 1),
             sequences, tq, tk, h, kv, d, d ** -0.5 if scale is None else scale, int(causal),
-            out.data_ptr(), self._rows(out, "out", (tq, h, d)), self._dense(lse, "lse", (tq, h)))
+            out.data_ptr(), self._rows(out, "out", (tq, h, d)), self._dense(lse, "lse", (tq, h)),
+            longest_q or 0, longest_k or 0)
 
     def _dense(self, t, what, shape):
         if t.dtype != self.torch.float32 or t.shape != shape or not t.is_contiguous():
@@ -839,15 +843,16 @@ class Backend:
         return t.data_ptr()
 
     def attention_packed(self, q, k, v, cu_q, cu_k=None, scale=None, causal=True, out=None,
-                         lse=None):
+                         lse=None, longest_q=None, longest_k=None):
         """Attention over packed sequences (ehip_attention_packed_f32): q (total_q, heads,
         head_dim), k and v (total_k, kv_heads, head_dim), column ranges of a fused projection
         allowed; cu_q, cu_k int32 offsets of the sequences on the device (cu_k: cu_q). scale:
-        head_dim ** -0.5. Returns (out, lse (total_q, heads)), written into `out` and `lse`
-        where given."""
+        head_dim ** -0.5. longest_q, longest_k: rows of the longest sequence, where known, for
+        batches of one long and many short or empty ones. Returns (out, lse (total_q, heads)),
+        written into `out` and `lse` where given."""
         out = self.f32(q.shape) if out is None else out
         lse = self.f32(q.shape[:2]) if lse is None else lse
-        desc = self._packed(q, k, v, cu_q, cu_k, scale, causal, out, lse)
+        desc = self._packed(q, k, v, cu_q, cu_k, scale, causal, out, lse, longest_q, longest_k)
         need = self.lib.ehip_attention_packed_workspace(C.byref(desc))
         space, at, n = self._workspace(need, "attention_packed")
         self.ok(self.lib.ehip_attention_packed_f32(C.byref(desc), at, n, self.stream()),
@@ -855,10 +860,11 @@ class Backend:
         return out, lse
 
     def attention_packed_backward(self, g, q, k, v, out, lse, cu_q, cu_k=None, scale=None,
-                                  causal=True, want=(True, True, True), grads=None):
+                                  causal=True, want=(True, True, True), grads=None,
+                                  longest_q=None, longest_k=None):
         """(dq, dk, dv) of attention_packed from its out and lse; None where `want` says so.
         `grads`: tensors to write them into (rows may be column ranges)."""
-        desc = self._packed(q, k, v, cu_q, cu_k, scale, causal, out, lse)
+        desc = self._packed(q, k, v, cu_q, cu_k, scale, causal, out, lse, longest_q, longest_k)
         if grads is None:
             grads = [self.f32(t.shape) if w else None for t, w in zip((q, k, v), want)]
         self._here(g, *grads)

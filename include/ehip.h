@@ -921,7 +921,14 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  * aligned) holds delta and, where heads are grouped or few rows pass many, the
  * shares of the gradients, during the call: at least
  * ehip_attention_packed_backward_workspace() bytes, of the call's own.
- * Deterministic: no atomics, the sums' order goes by the lengths and sizes. */
+ * Deterministic: no atomics, the sums' order goes by the lengths and sizes.
+ *
+ * longest_q and longest_k, where the caller knows them, say how the work is
+ * best shared out when a sequence is much longer than the mean of all
+ * (total / sequences), as beside many of one token or in offsets that are
+ * padded with empty sequences: without them no sequence is split where that
+ * mean is below 384. They are never relied on: a length past them is as right.
+ * The same rows under others may differ in the last bits. */
 typedef struct {
     const float *q, *k, *v;
     int64_t ld_q, ld_k, ld_v;
@@ -933,6 +940,7 @@ typedef struct {
     float* out; /* written by the forward, read by the backward */
     int64_t ld_out;
     float* lse; /* likewise */
+    int64_t longest_q, longest_k; /* rows of the longest sequence, 0: not known */
 } ehip_attention_packed_t;
 
 /* `workspace` (device memory, 16-byte aligned) holds the parts of rows whose

@@ -658,6 +658,48 @@ def test_a_step_that_is_not_finite_takes_no_longer(hip):
         assert x[0] < 8 * finite[0] and x[1] < 8 * finite[1]
 
 
+# One sequence of many keys among short or empty ones: offsets that are padded to a fixed count, a
+# prompt's piece beside answers that get one token each.
+SKEWED = [([128] + [1] * 43, [3000] + [1] * 43, 4, 2, 64), ([300] + [0] * 50, [900] + [0] * 50, 4, 1, 32),
+          ([5] * 9 + [700], [5] * 9 + [700], 2, 2, 96), ([1] * 70 + [40], [3] * 70 + [2000], 2, 1, 128)]
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("nq,nk,heads,kv,d", SKEWED)
+def test_one_long_sequence_among_short_ones(hip, nq, nk, heads, kv, d, causal):
+    """Split with the longest known; as right with lengths that are below or far above it."""
+    import torch
+    print_case("packed skewed", nq, nk, heads, kv, d, causal)
+    q, k, v, g = make(nq, nk, heads, kv, d, seed=sum(nk) + d)
+    cq, ck = offsets(nq), offsets(nk)
+    value, bound = packed(q, k, v, nq, nk, d ** -0.5, causal, g)
+    for longest in ((max(nq), max(nk)), (None, max(nk)), (1, 1), (2 ** 40, 2 ** 62), (7, None)):
+        kw = dict(causal=causal, longest_q=longest[0], longest_k=longest[1])
+        (out, lse), split = splits(hip, q, k, v, cq, ck, **kw)
+        assert split or longest[1] != max(nk)
+        grads = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck, **kw)
+        # A short sequence's sums count few roundings; the join adds one and a factor within 4 u.
+        for name, got in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads)):
+            within(got, value[name], bound[name] + 8 * 2.0 ** -24 * value[name].abs().nan_to_num(
+                posinf=0.0), name)
+        again = hip.attention_packed(q, k, v, cq, ck, **kw)
+        assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+@gpu
+def test_the_longest_of_one_offset_array(hip):
+    """cu_k left out: its longest is the queries'."""
+    import torch
+    print_case("packed longest")
+    n = [700] + [2] * 30
+    q, k, v, _ = make(n, n, 2, 1, 64, seed=67)
+    cu = offsets(n)
+    (out, _), split = splits(hip, q, k, v, cu, longest_q=700)
+    assert split
+    assert torch.equal(out, hip.attention_packed(q, k, v, cu, cu, longest_q=700, longest_k=700)[0])
+
+
 # ----------------------------------------------------------------- refusals
 
 def descriptor(**changes):
@@ -690,6 +732,24 @@ def test_workspace_and_refused_descriptors():
     assert forward(C.byref(descriptor())) == 0  # few keys
     assert forward(C.byref(descriptor(total_k=9000))) >= 10 * 4 * (16 + 2) * 4 * 2
     assert forward(C.byref(descriptor(sequences=0, total_q=0, q=None, cu_q=None, cu_k=None))) == 0
+
+
+def test_a_long_sequence_among_many_is_split():
+    """With the longest known a call's workspaces hold the parts of rows that the mean leaves whole."""
+    lib = E.load_library()
+    sizes = (lib.ehip_attention_packed_workspace, lib.ehip_attention_packed_backward_workspace)
+    for short in (0, 1, 300):
+        fields = dict(sequences=44, total_q=128 + 43 * min(short, 1), total_k=16384 + 43 * short)
+        long = descriptor(longest_q=128, longest_k=16384, **fields)
+        # Eight pieces or more of a maximum and a sum, and of 16 values, for each row and head.
+        assert sizes[0](C.byref(long)) >= 8 * long.total_q * 4 * 18 * 4
+        assert sizes[1](C.byref(long)) >= 8 * long.total_q * 4 * 16 * 4
+        for size in sizes:  # what fills the card without is not launched many times over
+            many = descriptor(**{**fields, "sequences": 10 ** 6}, longest_q=128, longest_k=16384)
+            assert 0 <= size(C.byref(many)) <= 4 * (long.total_q + 2 * long.total_k) * 4 * 17
+            for bad in (dict(longest_q=-1), dict(longest_k=-1)):
+                assert size(C.byref(descriptor(**fields, **bad))) == -1
+                assert b"longest" in lib.ehip_last_error()
 
 
 def test_blocks_fit_a_launch():
