@@ -514,39 +514,61 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
 
 // One head's share of a block by the formula, for those whose sums by parts are not finite: a part
 // of an infinity, or an infinity times the parts of a finite value, is NaN where the product is an
-// infinity or, its weight 0, nothing at all. One wave.
-template <class T>
+// infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time, of
+// rows of 16-byte units; a score of NaN or +inf settles the head as NaN (64 sequences of 1024, 32
+// heads over 8 of 128 values, us: finite 57, the first key NaN 61, the first value infinite 576;
+// value by value and to the end 1870 either way).
 __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int begin, int end,
                                 float& top, float& sum, float (&o)[2]) {
+    using attention::uintx4;
     const int lane = int(threadIdx.x) & 63, dim = int(a.c.dim);
     const int64_t pitch = a.c.kv_heads * dim;
     const float* q = a.q + s * a.ld_q + int64_t(h) * dim;
-    const T* k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
-    const T* v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
+    const Bf16* k = static_cast<const Bf16*>(a.c.k) + int64_t(kv) * dim;
+    const Bf16* v = static_cast<const Bf16*>(a.c.v) + int64_t(kv) * dim;
     const float c2 = a.scale * 1.44269504088896340736f;
-    const auto score = [&](int p) {
-        const T* row = k + pool_row(a.c, s, p) * pitch;
+    // The pool row of position p0 + lane, the last again past the end.
+    const auto row_of = [&](int p0) { return int(pool_row(a.c, s, min(p0 + lane, end - 1))); };
+    const auto score = [&](int row) {
+        const Bf16* at = k + int64_t(row) * pitch;
         float dot = 0.0f;
-        for (int e = 0; e < dim; ++e) dot = __builtin_fmaf(q[e] * c2, widen(row[e]), dot);
+        for (int e = 0; e < dim; e += 8) {
+            const uintx4 x = *reinterpret_cast<const uintx4*>(at + e);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t pair = x[j];
+                dot = __builtin_fmaf(q[e + 2 * j] * c2, __builtin_bit_cast(float, pair << 16), dot);
+                dot = __builtin_fmaf(q[e + 2 * j + 1] * c2,
+                                     __builtin_bit_cast(float, pair & 0xffff0000u), dot);
+            }
+        }
         return dot;
     };
     top = -INFINITY;
-    for (int p = begin + lane; p < end; p += 64) top = fmaxf(top, score(p));
+    for (int p0 = begin; p0 < end; p0 += 64) {
+        const float x = score(row_of(p0));
+        if (__any(!(x < INFINITY))) {
+            top = 0.0f;
+            sum = o[0] = o[1] = NAN;
+            return;
+        }
+        top = fmaxf(top, x);
+    }
 #pragma unroll
     for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
     const float shift = top == -INFINITY ? 0.0f : top;  // scores of -inf alone weigh nothing
     sum = o[0] = o[1] = 0.0f;
+    const int d0 = lane < dim ? lane : 0, d1 = lane + 64 < dim ? lane + 64 : 0;
     for (int p0 = begin; p0 < end; p0 += 64) {
-        const int p = p0 + lane;
-        const float weight = p < end ? exp2f(score(p) - shift) * 0x1p-24f : 0.0f;
+        const int row = row_of(p0), count = min(64, end - p0);
+        const float weight = lane < count ? exp2f(score(row) - shift) * 0x1p-24f : 0.0f;
         sum += weight;
-        for (int u = 0; u < 64 && p0 + u < end; ++u) {
-            const T* row = v + pool_row(a.c, s, p0 + u) * pitch;
+#pragma unroll 8
+        for (int u = 0; u < count; ++u) {
+            const Bf16* at = v + int64_t(__shfl(row, u)) * pitch;
             const float w = __shfl(weight, u);
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (lane + 64 * e < dim)
-                    o[e] = __builtin_fmaf(w, widen(row[lane + 64 * e]), o[e]);
+            o[0] = __builtin_fmaf(w, widen(at[d0]), o[0]);
+            o[1] = __builtin_fmaf(w, widen(at[d1]), o[1]);
         }
     }
 #pragma unroll
@@ -766,7 +788,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
                 fine = fine && fabsf(y[e]) < INFINITY;
             }
             if (!bad && !(__all(fine) && sum > 0.0f))
-                part_by_formula<Bf16>(a, s, h0 + g, kv, begin, end, top, sum, y);
+                part_by_formula(a, s, h0 + g, kv, begin, end, top, sum, y);
             const int64_t at = int64_t(h0 + g) * (a.workers + a.c.sequences) + worker + s;
             if (bad) sum = NAN;
             if (lane == 0) {

@@ -996,7 +996,9 @@ int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_
  * the pool makes the sequence's row NaN instead of a read out of bounds.
  * `longest`, a host value of at most 2^30, is what the work is split by: the
  * same lengths under another `longest` may differ in the last bits.
- * 1 <= head_dim <= 128, heads a multiple of kv_heads. `workspace` (16-byte
+ * 1 <= head_dim <= 128, heads a multiple of kv_heads. Heads of a bf16 cache
+ * that meet an infinity are formed a second time, at some ten times the
+ * cost. `workspace` (16-byte
  * aligned) holds the parts of split lengths during the call: at least
  * ehip_attention_paged_workspace() bytes, of the call's own. Deterministic. */
 int64_t ehip_attention_paged_workspace(const ehip_cache_t* cache, int64_t heads,

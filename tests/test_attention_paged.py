@@ -305,6 +305,71 @@ def test_same_bits_each_time_on_other_streams_and_in_a_graph(hip):
             assert torch.equal(outs[0], o) and torch.equal(outs[1], l)
 
 
+@gpu
+@pytest.mark.parametrize("dtype", types())
+@pytest.mark.parametrize("which,value", [("k", math.nan), ("k", math.inf), ("v", math.nan),
+                                         ("v", math.inf), ("v", -math.inf)])
+def test_a_value_that_is_not_finite_anywhere_in_a_length(hip, which, value, dtype):
+    """One of the first, middle or last positions of lengths that are one part and several: its key
+    head's heads are what the formula has, the others as ever."""
+    import torch
+    print_case("paged not finite anywhere", which, value, dtype)
+    lengths = [3000, 130, 70]
+    kp, vp, table, k, v = make(lengths, 2, 64, 16, dtype, seed=16)
+    q = torch.rand(3, 10, 64, device="cuda") + 0.5  # a key of inf is a score of inf
+    for at in ("first", "middle", "last"):
+        kx, vx = kp.clone(), vp.clone()
+        rows = {"k": [t.clone() for t in k], "v": [t.clone() for t in v]}
+        for s, n in enumerate(lengths):
+            p = {"first": 0, "middle": n // 2, "last": n - 1}[at]
+            pool = kx if which == "k" else vx
+            pool[table[s, p // 16].long(), p % 16, 0, 7] = value
+            rows[which][s][p, 0, 7] = value
+        out, lse = hip.attention_paged(q, kx, vx, table, ints(lengths))
+        if which == "k":  # no distribution
+            assert bool(torch.isnan(out[:, :5]).all()) and bool(torch.isnan(lse[:, :5]).all())
+        heads = slice(5 if which == "k" else 0, 10)
+        each = slice(1 if which == "k" else 0, 2)
+        want, bound = reference(q[:, heads], [t[:, each] for t in rows["k"]],
+                                [t[:, each] for t in rows["v"]], lengths, 0.125)
+        within(out[:, heads], want["out"], bound["out"], "out")
+        within(lse[:, heads], want["lse"], bound["lse"], "lse")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", types())
+def test_a_cache_that_is_not_finite_takes_no_longer(hip, dtype):
+    """A NaN in each sequence's first key, or nothing else: value by value it took 33 times as long."""
+    import torch
+    print_case("paged time of NaN", dtype)
+    lengths = [1024] * 64
+    kp, vp, table, _, _ = make(lengths, 8, 128, 16, dtype, seed=17)
+    q = torch.randn(64, 32, 128, device="cuda")
+    n = ints(lengths)
+
+    def took():
+        """The least of five, in ms."""
+        best = math.inf
+        for _ in range(5):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            hip.attention_paged(q, kp, vp, table, n)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        return best
+
+    took()
+    times = [took()]
+    kp[table[:, 0].long(), 0] = math.nan
+    times.append(took())
+    kp.fill_(math.nan)
+    vp.fill_(math.nan)
+    times.append(took())
+    print(times, flush=True)
+    assert max(times) < 8 * times[0]
+
+
 # ------------------------------------------------------------------- append
 
 @gpu
