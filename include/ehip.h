@@ -990,17 +990,19 @@ int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_
 /* Attention of one new token per sequence over the cache: row s of q and out
  * (heads * head_dim floats, ld_q and ld_out apart) sees positions 0 ..
  * lengths[s] - 1 (a DEVICE array; write the new token's key and value first).
- * out and lse (sequences, heads; may be NULL) as in ehip_attention_packed_f32;
- * they may not overlap the inputs. A length of zero gives out = 0, lse = -inf.
- * A negative length, one past `longest` or its table row, or a page outside
- * the pool makes the sequence's row NaN instead of a read out of bounds.
+ * out and lse (sequences, heads; may be NULL) as in ehip_attention_packed_f32,
+ * but that small values keep fewer bits: sums run on 2^-24 of a weight, and out
+ * may be off by another lengths[s] * 2^-123. They may not overlap the inputs. A
+ * length of zero gives out = 0, lse = -inf. A negative length, one past
+ * `longest` or its table row, or a page outside the pool makes the sequence's
+ * row NaN instead of a read out of bounds.
  * `longest`, a host value of at most 2^30, is what the work is split by: the
  * same lengths under another `longest` may differ in the last bits.
  * 1 <= head_dim <= 128, heads a multiple of kv_heads. Heads of a bf16 cache
- * that meet an infinity are formed a second time, at some ten times the
- * cost. `workspace` (16-byte
- * aligned) holds the parts of split lengths during the call: at least
- * ehip_attention_paged_workspace() bytes, of the call's own. Deterministic. */
+ * that meet an infinity are formed a second time, at some ten times the cost.
+ * `workspace` (16-byte aligned) holds the parts of split lengths during the
+ * call: at least ehip_attention_paged_workspace() bytes, of the call's own.
+ * Deterministic. */
 int64_t ehip_attention_paged_workspace(const ehip_cache_t* cache, int64_t heads,
                                        int64_t longest);
 int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t ld_q,

@@ -700,6 +700,48 @@ def test_the_longest_of_one_offset_array(hip):
     assert torch.equal(out, hip.attention_packed(q, k, v, cu, cu, longest_q=700, longest_k=700)[0])
 
 
+@gpu
+@pytest.mark.parametrize("d", [24, 64, 100])
+@pytest.mark.parametrize("power", [-100, -104, -108])
+def test_small_values_keep_24_bits(hip, power, d):
+    """Values from 2^-110 on are held whole in their three parts. Besides the relative bound there
+    is fp32's least step, 2^-149, for each of the at most 7 roundings a key (six part products and
+    the running sum), times weights and a divisor that are at most 1."""
+    import torch
+    print_case("packed small values", power, d)
+    nq, nk = [70, 9], [100, 9]
+    q, k, v, _ = make(nq, nk, 2, 1, d, seed=62)
+    v = (torch.rand_like(v) + 1) * v.sign() * 2.0 ** (power - 1)
+    out, _ = hip.attention_packed(q, k, v, offsets(nq), offsets(nk))
+    value, bound = packed(q, k, v, nq, nk, d ** -0.5, True)
+    bound = bound["out"] + 700 * 2.0 ** -149 - 1e-37  # the last is the reference's own allowance
+    assert float((value["out"].abs() > 100 * bound).double().mean()) > 0.9
+    within(out, value["out"], bound, "out")
+
+
+@gpu
+@pytest.mark.parametrize("d", [24, 64, 100])
+def test_gradients_of_small_values(hip, d):
+    """g near 2^-100. dv = sum p g as the forward's sums. ds is split like a value, and loses what is
+    below 2^-133: within that for each of a sum's terms, times the other factor (below 6) and the
+    scale (below 1)."""
+    import torch
+    print_case("packed small gradients", d)
+    nq, nk = [70, 9], [100, 9]
+    q, k, v, g = make(nq, nk, 2, 1, d, seed=64)
+    g = (torch.rand_like(g) + 1) * g.sign() * 2.0 ** -101
+    cq, ck = offsets(nq), offsets(nk)
+    out, lse = hip.attention_packed(q, k, v, cq, ck)
+    grads = hip.attention_packed_backward(g, q, k, v, out, lse, cq, ck)
+    value, bound = packed(q, k, v, nq, nk, d ** -0.5, True, g)
+    assert float(max(t.abs().max() for t in (q, k))) < 6
+    for name, got, loss in zip(("dq", "dk", "dv"), grads, (6 * 100, 6 * 140, 2.0 ** -6)):
+        # Two heads add to dk and dv.
+        bounds = bound[name] + loss * 2.0 ** -133 - (1 if name == "dq" else 2) * 1e-37
+        assert float((value[name].abs() > 10 * bounds).double().mean()) > 0.8
+        within(got, value[name], bounds, name)
+
+
 # ----------------------------------------------------------------- refusals
 
 def descriptor(**changes):

@@ -370,6 +370,33 @@ def test_a_cache_that_is_not_finite_takes_no_longer(hip, dtype):
     assert max(times) < 8 * times[0]
 
 
+@gpu
+@pytest.mark.parametrize("dtype", types())
+@pytest.mark.parametrize("d", [33, 64])
+@pytest.mark.parametrize("power", [-100, -104, -110])
+def test_small_values(hip, power, dtype, d):
+    """Sums run on 2^-24 of a weight, so fp32's least step is 2^-125 of what they stand for: besides
+    the relative bound there is that for each of the at most four roundings a position (three part
+    products and the running sum)."""
+    import torch
+    print_case("paged small values", power, dtype, d)
+    lengths = [300, 7]
+    kp, vp, table, k, v = make(lengths, 2, d, 16, torch.float32, seed=9)
+    vp = ((torch.rand_like(vp) + 1) * vp.sign() * 2.0 ** (power - 1)).to(dtype)
+    kp = kp.to(dtype)
+    rows = [[pool[table[s, :-(-n // 16)].long()].reshape(-1, 2, d)[:n].float()
+             for s, n in enumerate(lengths)] for pool in (kp, vp)]
+    q = torch.randn(2, 4, d, device="cuda")
+    out, lse = hip.attention_paged(q, kp, vp, table, ints(lengths))
+    value, bound = reference(q, *rows, lengths, d ** -0.5)
+    for s, n in enumerate(lengths):
+        # In place of the reference's own allowance.
+        bounds = bound["out"][s] - 1e-37 + n * 2.0 ** -123
+        within(out[s], value["out"][s], bounds, "out")
+    assert float((value["out"][1].abs() > 10 * bounds).double().mean()) > 0.9  # not zeros
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
 # ------------------------------------------------------------------- append
 
 @gpu
