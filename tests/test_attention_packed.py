@@ -742,6 +742,71 @@ def test_gradients_of_small_values(hip, d):
         within(got, value[name], bounds, name)
 
 
+@gpu
+@pytest.mark.parametrize("which", sorted(LENGTHS))
+@pytest.mark.parametrize("heads,kv,d", [(2, 2, 64), (4, 1, 128), (3, 3, 24)])
+def test_lengths_of_fixed_inputs(hip, which, heads, kv, d):
+    """The sets of lengths on inputs that are the same in every run."""
+    nq, nk = zip(*LENGTHS[which])
+    for causal in (True, False):
+        check(hip, nq, nk, heads, kv, d, causal, seed=1000 * sorted(LENGTHS).index(which) + d)
+
+
+# Blocks of 256 queries: without the mask from 256 of them on, with it from 512 and a mean of 2048
+# queries (heads of up to 96 values).
+
+@gpu
+@pytest.mark.parametrize("d", [3, 24, 31, 64, 67, 90, 96])
+def test_blocks_of_256_queries(hip, d):
+    import torch
+    print_case("packed 256 queries", d)
+    nq, nk, heads = [700, 1, 0, 323], [200, 77, 3, 130], 64
+    q, k, v, _ = make(nq, nk, heads, 4, d, seed=d)
+    out, lse = hip.attention_packed(q, k, v, offsets(nq), offsets(nk), causal=False)
+    value, bound = packed(q, k, v, nq, nk, d ** -0.5, False)
+    within(out, value["out"], bound["out"], "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
+@gpu
+@pytest.mark.parametrize("d", [3, 24, 64, 90])
+@pytest.mark.parametrize("n", [200, 2080])
+def test_causal_blocks_of_256_queries(hip, d, n):
+    """Of two heads in 64, the others the same rows in other places: as many keys as queries, or
+    keys for the last of them alone."""
+    import torch
+    print_case("packed 256 queries, causal", d, n)
+    q, k, v, _ = make([2080], [n], 64, 2, d, seed=d + n)
+    q = q[:, :2].repeat(1, 32, 1).reshape(2080, 32, 2, d).transpose(1, 2).reshape(2080, 64, d)
+    out, lse = hip.attention_packed(q.contiguous(), k, v, offsets([2080]), offsets([n]))
+    for x in (out, lse):
+        x = x.reshape(2080, 2, 32, -1)
+        assert torch.equal(x, x[:, :, :1].expand_as(x))
+    value, bound = packed(q[:, ::32], k, v, [2080], [n], d ** -0.5, True)
+    within(out[:, ::32], value["out"], bound["out"], "out")
+    within(lse[:, ::32], value["lse"], bound["lse"], "lse")
+
+
+@gpu
+def test_blocks_of_256_queries_not_finite_and_not_seen(hip):
+    import torch
+    print_case("packed 256 queries special")
+    q, k, v, _ = make([2100], [2050], 64, 2, 64, seed=63)
+    cq, ck = offsets([2100]), offsets([2050])
+    want, want_lse = hip.attention_packed(q, k, v, cq, ck)
+    k[1900], v[1900] = math.nan, math.inf  # queries 1950 .. see it
+    out, lse = hip.attention_packed(q, k, v, cq, ck)
+    assert bool((out[:50] == 0).all()) and bool((lse[:50] == -math.inf).all())
+    assert bool(torch.isnan(out[1950:]).all()) and bool(torch.isnan(lse[1950:]).all())
+    assert torch.equal(out[:1800], want[:1800]) and torch.equal(lse[:1800], want_lse[:1800])
+    kz, vz = k.clone(), v.clone()
+    kz[1900:], vz[1900:] = 0, 0
+    value, bound = packed(q[:, ::32], kz, vz, [2100], [2050], 0.125, True)
+    rows = slice(1800, 1950)
+    within(out[rows, ::32], value["out"][rows], bound["out"][rows], "out")
+    within(lse[rows, ::32], value["lse"][rows], bound["lse"][rows], "lse")
+
+
 # ----------------------------------------------------------------- refusals
 
 def descriptor(**changes):

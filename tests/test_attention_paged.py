@@ -397,6 +397,22 @@ def test_small_values(hip, power, dtype, d):
     within(lse, value["lse"], bound["lse"], "lse")
 
 
+@gpu
+@pytest.mark.parametrize("dtype", types())
+@pytest.mark.parametrize("heads,kv,d", [(17, 1, 64), (33, 1, 32), (40, 2, 128), (64, 2, 40)])
+def test_groups_over_several_blocks(hip, dtype, heads, kv, d):
+    """More query heads a key head than a block takes at a time."""
+    check(hip, [200, 0, 1, 33, 700], heads, kv, d, 16, dtype, seed=heads)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 100])
+@pytest.mark.parametrize("scale,spread", [(0.0, 1.0), (-0.2, 3.0), (0.125, 40.0)])
+def test_scales_and_sharp_rows_in_bf16(hip, scale, spread, d):
+    import torch
+    check(hip, [700, 33], 4, 2, d, 16, torch.bfloat16, seed=4, scale=scale, spread=spread)
+
+
 # ------------------------------------------------------------------- append
 
 @gpu

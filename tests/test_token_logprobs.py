@@ -346,6 +346,30 @@ def test_same_bits_on_other_streams_and_in_a_graph(hip, rows, vocab):
             assert all(torch.equal(a, b) for a, b in zip(outs, want))
 
 
+@gpu
+@pytest.mark.parametrize("vocab,top", [(32771, 0), (32771, 9), (40960, 5)])
+def test_more_logits_than_the_caches_hold(hip, vocab, top):
+    """2^26 logits and more are read past the caches: the bits of the same rows in two calls, which
+    are not, and some rows against 64 bits."""
+    import torch
+    rows = -(-2 ** 26 // vocab)
+    rows += rows % 2
+    x, t, _, _ = make(rows, vocab, seed=vocab + top)
+    got = hip.token_logprobs(x, t, top=top)
+    half = rows // 2
+    assert half >= 512  # whole rows a block, as in one call
+    parts = [hip.token_logprobs(x[at:at + half], t[at:at + half], top=top) for at in (0, half)]
+    for a, b, c in zip(got, *parts):
+        assert (a is None) == (b is None)
+        assert a is None or torch.equal(a, torch.cat([b, c]))
+    some = torch.arange(0, rows, rows // 6, device="cuda")
+    value, bound = exact(x[some], t[some])
+    for name, y in zip(("logprob", "entropy", "lse"), got):
+        near(y[some], value[name], bound[name], name)
+    if top:
+        assert torch.equal(got[4][some].cpu(), best(x[some], top))
+
+
 def test_refused_sizes():
     """The checks that every call starts with, through the query that needs no device."""
     lib = E.load_library()
