@@ -1170,7 +1170,7 @@ int64_t slots(int64_t total, int64_t sequences, int rows = kRows) {
 // Rows are taken to be in sequences of the mean length, or, where the longest is known, in as many of
 // that length as they make: a long one among short or empty ones then counts as itself.
 void share(int64_t total, int64_t sequences, int64_t longest, int64_t& each, int64_t& count) {
-    each = longest > 0 ? std::min(longest, total) : sequences == 0 ? 0 : total / sequences;
+    each = sequences == 0 ? 0 : longest > 0 ? std::min(longest, total) : total / sequences;
     count = longest > 0 ? std::min(sequences, ceil_div(total, longest)) : sequences;
 }
 

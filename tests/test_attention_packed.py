@@ -859,6 +859,17 @@ def test_a_long_sequence_among_many_is_split():
                 assert b"longest" in lib.ehip_last_error()
 
 
+def test_no_sequences_with_a_longest():
+    """Rows past the last sequence only, whatever the longest is said to be: nothing to split."""
+    lib = E.load_library()
+    for total_q, total_k in ((0, 0), (10, 10), (10, 5000), (5000, 10), (5000, 5000)):
+        for longest in (1, 5000, 2 ** 62):
+            desc = descriptor(sequences=0, total_q=total_q, total_k=total_k, longest_q=longest,
+                              longest_k=longest)
+            assert lib.ehip_attention_packed_workspace(C.byref(desc)) == 0
+            assert lib.ehip_attention_packed_backward_workspace(C.byref(desc)) >= 0
+
+
 def test_blocks_fit_a_launch():
     """2^32 threads: blocks of 512, so 2^23 - 1 of them."""
     size = E.load_library().ehip_attention_packed_backward_workspace
