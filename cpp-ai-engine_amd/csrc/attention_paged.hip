@@ -521,7 +521,9 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
 __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int begin, int end,
                                 float& top, float& sum, float (&o)[2]) {
     using attention::uintx4;
-    const int lane = int(threadIdx.x) & 63, dim = int(a.c.dim);
+    int lane = int(threadIdx.x) & 63;
+    asm volatile("" : "+v"(lane));  // else what follows from it is held all through the tiles
+    const int dim = int(a.c.dim);
     const int64_t pitch = a.c.kv_heads * dim;
     const float* q = a.q + s * a.ld_q + int64_t(h) * dim;
     const Bf16* k = static_cast<const Bf16*>(a.c.k) + int64_t(kv) * dim;
