@@ -187,13 +187,15 @@ __device__ __forceinline__ float wave_sum(float x) {
 }
 
 // ------------------------------------------------------- one row by one wave
+
 // The formulas as they stand, for rows whose tiles gave no finite result; only what the row sees is
 // read. Sixteen lanes take one streamed row, its values 16 apart, so that a wave reads four rows at
 // a time and U times four ahead: a NaN or an infinity that every row sees has all rows formed here,
 // and then the reads' latency bounds a call (4 sequences of 512, 8 heads of 64, the first key
 // infinite: 168 us forward and 708 backward; without it 43 and 86; a lane for each key took 760 and
-// 4750). Where a score, lse or delta settles the row as NaN nothing else is read (first key NaN: 39
-// and 101 us, 767 and 4750 without that).
+// 4750. One of 16384, 8 heads of 128 over 2: 104 ms and 110, without it 2.8 and 10.1). Where a
+// score, lse or delta settles the row as NaN nothing else is read (first key NaN: 39 and 101 us,
+// 767 and 4750 without that).
 
 constexpr int kRowLanes = 16, kRowColumns = kMaxDim / kRowLanes;
 
@@ -244,7 +246,8 @@ __device__ __forceinline__ float dot(const Columns& x, const Columns& y) {
     return s;
 }
 
-// Rows j0 + the lane's group, and every fourth after it, of those before n (the last again past it).
+// Rows j0 + the lane's group, and every fourth after it, of those before n (the last again past
+// it).
 template <int U>
 __device__ __forceinline__ void load_rows(Columns (&x)[U], const float* base, int64_t ld,
                                           int64_t j0, int64_t n, int dim) {
@@ -414,8 +417,9 @@ __device__ __forceinline__ int64_t piece_of(const Packed& a, int64_t row, int h,
 // A wave's 32 queries stay in registers; tiles of BN keys and their values pass through LDS with
 // the running maximum, sum and weighted values beside them. For long sequences the products bound
 // it (16384 tokens, 8 heads of 128 values, causal: 2.6 to 2.8 ms, 195 to 210 TFLOP/s of 201 that a
-// sixth of a bf16 product of 8192^3 reaches); shorter ones spend as long on exponents and on
-// splitting the weights (16 of 512, 16 heads of 64: 72 to 85 us, the matrix units busy 40 % of it).
+// sixth of a bf16 product of 8192^3 reaches, with 12 to 15 registers spilled); shorter ones spend
+// as long on exponents and on splitting the weights (16 of 512, 16 heads of 64: 72 to 85 us, the
+// matrix units busy 40 % of it).
 template <int DP, int BN, int WAVES, int READS>
 __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     constexpr int BUFFERS = WAVES / 4;
@@ -449,8 +453,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void packed_forward(Packed a) {
     const int wave_end = 32 * wave < t.rows ? min(visible(a, t, t.first + last), end) : 0;
     const int wave_all = visible(a, t, t.first + 32 * wave);  // keys that all its queries see
 
-    // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q, and so does a scale of
-    // 0, with which a masked score's -inf would be NaN.
+    // exp(scale s - m) as 2^(c2 s - m2); a negative scale's sign goes into q, and so does a scale
+    // of 0, with which a masked score's -inf would be NaN.
     const float c2 = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.44269504088896340736f;
     bf16x8 q[DP / 16][3];
     own_row<DP, READS>(a.q + int64_t(t.q0 + i) * a.ld_q + int64_t(h) * a.dim, a.dim,
@@ -785,7 +789,8 @@ __device__ __forceinline__ uint32_t shared_rows(uint32_t* votes, bool bad) {
 }
 
 // dq and delta of wider heads. Wave role 0 forms s and p, role 1 dp - delta; both then have ds, and
-// half of dq's values each (5576 tokens in 11 sequences, 12 heads of 96 over 4: 189 to 238 us).
+// half of dq's values each (5576 tokens in 11 sequences, 12 heads of 96 over 4: 189 to 238 us,
+// the matrix units busy 40 %, by turns as in the keys' kernel).
 template <int DP, int BN, int READS>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed a) {
     using namespace attention;
@@ -937,7 +942,9 @@ __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_q_pair(Packed
 
 // dv_j = sum_i p_ij g_i by the waves of role 0, from s and p, and dk_j = scale sum_i ds_ij q_i by
 // those of role 1, from dp and the other's p: 16 of 512 tokens, 16 heads of 64, 143 to 173 us; 5576
-// tokens, 12 heads of 96, 234 to 288. Vector work bounds it, the matrix units are busy 36 and 47 %.
+// tokens, 12 heads of 96, 228 to 288. The matrix units are busy 37 and 51 %: both waves of a SIMD
+// are in the phase of the scores, mostly vector work, or both in that of the gradients. Heads of
+// 128 values spill 37 to 40 registers, of 64 6 to 9.
 template <int DP, int BN, int READS>
 __global__ __launch_bounds__(kBackThreads, 2) void packed_backward_kv(Packed a) {
     using namespace attention;
@@ -1167,8 +1174,8 @@ int64_t slots(int64_t total, int64_t sequences, int rows = kRows) {
     return total / rows + sequences;
 }
 
-// Rows are taken to be in sequences of the mean length, or, where the longest is known, in as many of
-// that length as they make: a long one among short or empty ones then counts as itself.
+// Rows are taken to be in sequences of the mean length, or, where the longest is known, in as many
+// of that length as they make: a long one among short or empty ones then counts as itself.
 void share(int64_t total, int64_t sequences, int64_t longest, int64_t& each, int64_t& count) {
     each = sequences == 0 ? 0 : longest > 0 ? std::min(longest, total) : total / sequences;
     count = longest > 0 ? std::min(sequences, ceil_div(total, longest)) : sequences;
@@ -1223,8 +1230,8 @@ int fill(const char* name, const ehip_attention_packed_t* d, Packed& a) {
     a.dim = int(d->head_dim);
     a.scale = d->scale;
     a.causal = d->causal != 0;
-    // Under a causal mask by work (16 sequences of 512: forward 82 -> 70 us, dq 114 -> 97); more
-    // sequences than lanes have blocks enough to fill the gaps, and would take longer to order.
+    // Under a causal mask by work (16 sequences of 512: forward 82 -> 70 us, dq 114 -> 97), for as
+    // many sequences as a wave has lanes: find_tile_by_work has one in each.
     a.by_work = a.causal && a.sequences <= 64;
     a.out = d->out;
     a.ld_out = d->ld_out;

@@ -91,7 +91,7 @@ __device__ __forceinline__ int sequence_of(const int32_t* __restrict__ cu, int s
 
 // WAVES waves a token. Its first values are asked for before its place is known, which takes four
 // reads one after the other: the offsets (two, past 64 sequences), the start and the page. HBM
-// bounds it (5061 tokens, 1024 values of k and of v, fp32: 14.1 us, 5.9 TB/s).
+// bounds it (5061 tokens, 1024 values of k and of v, fp32: 13.9 us, 6.0 TB/s).
 template <class T, int WAVES, bool VEC>
 __global__ __launch_bounds__(kAppendThreads) void cache_append(
     Cache c, const float* __restrict__ k, int64_t ld_k, const float* __restrict__ v, int64_t ld_v,
@@ -514,9 +514,9 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
 
 // One head's share of a block by the formula, for those whose sums by parts are not finite: a part
 // of an infinity, or an infinity times the parts of a finite value, is NaN where the product is an
-// infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time, of
-// rows of 16-byte units; a score of NaN or +inf settles the head as NaN (64 sequences of 1024, 32
-// heads over 8 of 128 values, us: finite 57, the first key NaN 61, the first value infinite 576;
+// infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time,
+// of rows of 16-byte units; a score of NaN or +inf settles the head as NaN (64 sequences of 1024,
+// 32 heads over 8 of 128 values, us: finite 56, the first key NaN 59, the first value infinite 560;
 // value by value and to the end 1870 either way).
 __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int begin, int end,
                                 float& top, float& sum, float (&o)[2]) {
@@ -588,8 +588,8 @@ __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int be
 //            4 h + 0..3, 16 + 4 h + 0..3 for the lanes h = l / 16
 //   values:  A = 16 values by those 32 positions of V: rows in LDS, read transposed
 // A wave takes 32 positions at a time; the next ones' reads are out while it forms weights and
-// sums. 64 sequences of 4096, 32 heads over 8 of 128 values: 212 us, 5.1 TB/s; of 64 to 4096, 71
-// us, 3.7.
+// sums. 64 sequences of 4096, 32 heads over 8 of 128 values: 213 us, 5.0 TB/s; of 64 to 4096, 66
+// us, 4.0: a block passes parts of several there, and its loads run dry at each change.
 constexpr int kTilePositions = 32;
 
 template <int DP>

@@ -895,7 +895,7 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  * out and lse may not overlap the inputs. Keys that a row does not see do not
  * reach it, whatever they hold (NaN and infinities included). Rows that meet an
  * infinity, or a NaN that is not in a score, are formed a second time one by
- * one: a call in which most do takes up to some 25 times as long. Rows of q past
+ * one: a call in which most do takes up to some 50 times as long. Rows of q past
  * the last sequence leave out, lse and dq as they were, rows of k past it dk
  * and dv.
  *
@@ -920,7 +920,9 @@ int ehip_softmax_xent_backward_f32(const float* logits, const int32_t* targets, 
  * overlap the inputs or each other. `workspace` (device memory, 16-byte
  * aligned) holds delta and, where heads are grouped or few rows pass many, the
  * shares of the gradients, during the call: at least
- * ehip_attention_packed_backward_workspace() bytes, of the call's own.
+ * ehip_attention_packed_backward_workspace() bytes, of the call's own. With
+ * grouped heads that is 8 bytes for each of total_k * heads * head_dim values
+ * and more, whichever of dk and dv is asked for.
  * Deterministic: no atomics, the sums' order goes by the lengths and sizes.
  *
  * longest_q and longest_k, where the caller knows them, say how the work is
