@@ -1178,7 +1178,7 @@ int64_t slots(int64_t total, int64_t sequences, int rows = kRows) {
 // of that length as they make: a long one among short or empty ones then counts as itself.
 void share(int64_t total, int64_t sequences, int64_t longest, int64_t& each, int64_t& count) {
     each = sequences == 0 ? 0 : longest > 0 ? std::min(longest, total) : total / sequences;
-    count = longest > 0 ? std::min(sequences, ceil_div(total, longest)) : sequences;
+    count = longest > 0 && each > 0 ? std::min(sequences, ceil_div(total, each)) : sequences;
 }
 
 // Tiles address their rows by 32-bit byte offsets from the first one.

@@ -870,6 +870,17 @@ def test_no_sequences_with_a_longest():
             assert lib.ehip_attention_packed_backward_workspace(C.byref(desc)) >= 0
 
 
+def test_a_longest_past_everything():
+    """The largest number is as good as the rows there are."""
+    lib = E.load_library()
+    for total in (1, 10, 9000):
+        sizes = [(lib.ehip_attention_packed_workspace(C.byref(d)),
+                  lib.ehip_attention_packed_backward_workspace(C.byref(d)))
+                 for d in (descriptor(total_q=10, total_k=total, longest_q=q, longest_k=k)
+                           for q, k in ((10, total), (2 ** 63 - 1, 2 ** 63 - 1), (11, total + 1)))]
+        assert sizes[0] == sizes[1] == sizes[2] and min(sizes[0]) >= 0
+
+
 def test_blocks_fit_a_launch():
     """2^32 threads: blocks of 512, so 2^23 - 1 of them."""
     size = E.load_library().ehip_attention_packed_backward_workspace
