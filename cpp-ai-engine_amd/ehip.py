@@ -100,6 +100,15 @@ class Cache(C.Structure):
                 ("table_width", C.c_int64), ("sequences", C.c_int64)]
 
 
+class NormRotate(C.Structure):
+    """ehip_norm_rotate_t: query and key heads, their weights and rotation."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("ld_q", C.c_int64), ("ld_k", C.c_int64),
+                ("tokens", C.c_int64), ("heads", C.c_int64), ("kv_heads", C.c_int64),
+                ("head_dim", C.c_int64), ("rotary", C.c_int64), ("positions", C.c_void_p),
+                ("freqs", C.c_void_p), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+                ("eps", C.c_float), ("interleaved", C.c_int)]
+
+
 # name -> argtypes (all return int unless listed in _RESTYPES)
 _SIGS = {
     "ehip_init": [], "ehip_available": [], "ehip_enabled": [], "ehip_set_enabled": [_i],
@@ -211,13 +220,18 @@ _SIGS = {
     "ehip_token_logprobs_f32": [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp,
                                 _sz, _vp],
     "ehip_token_logprobs_backward_f32": [_vp, _i64] + [_vp] * 6 + [_i64, _i64, _i64, _vp],
+    "ehip_norm_rotate_f32": [C.POINTER(NormRotate), _vp, _i64, _vp, _i64, _vp],
+    "ehip_norm_rotate_backward_workspace": [C.POINTER(NormRotate)],
+    "ehip_norm_rotate_backward_f32": [C.POINTER(NormRotate)] + [_vp, _i64] * 4 +
+                                     [_vp, _vp, _vp, _sz, _vp],
     "ehip_last_error": [],
 }
 _RESTYPES = {"ehip_last_error": C.c_char_p,
              "ehip_attention_packed_workspace": C.c_int64,
              "ehip_attention_packed_backward_workspace": C.c_int64,
              "ehip_attention_paged_workspace": C.c_int64,
-             "ehip_token_logprobs_workspace": C.c_int64, "ehip_kernels_launched": C.c_uint64,
+             "ehip_token_logprobs_workspace": C.c_int64,
+             "ehip_norm_rotate_backward_workspace": C.c_int64, "ehip_kernels_launched": C.c_uint64,
              "ehip_conv2d_relu_maxpool_partials": C.c_int64,
              "ehip_layernorm_backward_partials": C.c_int64,
              "ehip_kernels_failed": C.c_uint64, "ehip_reset_counters": None,
@@ -978,3 +992,82 @@ class Backend:
             self._rows(dlogits, "dlogits", (rows, vocab)), rows, vocab, self.stream()),
             "token_logprobs_backward")
         return dlogits
+
+    # ----------------- answers sampled in groups, and training on them
+    def rotary_frequencies(self, rotary, base=10000.0):
+        """The angles of a step of one position, base ** (-2 i / rotary) for i < rotary / 2, in
+        64 bits on the device."""
+        i = self.torch.arange(rotary // 2, dtype=self.torch.float64, device="cuda")
+        return self.torch.pow(self.torch.full_like(i, base), -2.0 * i / max(1, rotary))
+
+    def _norm_rotate(self, q, k, positions, freqs, q_weight, k_weight, eps, interleaved):
+        if q.dim() != 3 or (k is not None and k.dim() != 3):
+            raise ValueError("q and k: expected (tokens, heads, head_dim)")
+        self._here(q, k, positions, freqs, q_weight, k_weight)
+        tokens, h, d = q.shape
+        kv = 0 if k is None else k.shape[1]
+        rotary = 0 if freqs is None else 2 * freqs.numel()
+        if rotary and (freqs.dtype != self.torch.float64 or freqs.dim() != 1
+                       or not freqs.is_contiguous()):
+            raise ValueError(f"freqs: {freqs.dtype} {tuple(freqs.shape)}, expected contiguous "
+                             f"float64 (rotary / 2,)")
+        if rotary and positions is None:
+            raise ValueError("positions: expected with freqs")
+        if k is None and k_weight is not None:
+            raise ValueError("k_weight: given without k")
+        weight = lambda w, what: None if w is None else self._dense(w, what, (d,))
+        return NormRotate(
+            q.data_ptr(), None if k is None else k.data_ptr(), self._rows(q, "q", (tokens, h, d)),
+            0 if k is None else self._rows(k, "k", (tokens, kv, d)), tokens, h, kv, d, rotary,
+            self._index(positions, "positions", tokens) if rotary else None,
+            freqs.data_ptr() if rotary else None, weight(q_weight, "q_weight"),
+            weight(k_weight, "k_weight"), eps, int(interleaved))
+
+    def _into(self, t, what, like):
+        """(pointer, row pitch) of a tensor of rows that is written, or of none."""
+        if t is None:
+            return None, 0
+        return _vp(t.data_ptr()), self._rows(t, what, like.shape)
+
+    def norm_rotate(self, q, k, positions, freqs, q_weight=None, k_weight=None, eps=1e-6,
+                    interleaved=False, out=None):
+        """The norm of each query and key head and its rotation by position
+        (ehip_norm_rotate_f32): q (tokens, heads, head_dim), k (tokens, kv_heads, head_dim) or
+        None, column ranges of a fused projection allowed; positions int32 (tokens,); freqs
+        float64 (rotary / 2,) as rotary_frequencies gives them, None for no rotation; weights
+        (head_dim,), None for no norm. Returns (q, k), written into the tensors `out` where
+        given, which may be q and k themselves."""
+        desc = self._norm_rotate(q, k, positions, freqs, q_weight, k_weight, eps, interleaved)
+        if out is None:
+            out = [self.f32(q.shape), None if k is None else self.f32(k.shape)]
+        self._here(*out)
+        self.ok(self.lib.ehip_norm_rotate_f32(
+            C.byref(desc), *self._into(out[0], "q_out", q),
+            *(self._into(out[1], "k_out", k) if k is not None else (None, 0)), self.stream()),
+            "norm_rotate")
+        return tuple(out)
+
+    def norm_rotate_backward(self, g_q, g_k, q, k, positions, freqs, q_weight=None,
+                             k_weight=None, eps=1e-6, interleaved=False,
+                             want=(True, True, True, True), grads=None):
+        """(dq, dk, dq_weight, dk_weight) of norm_rotate from the gradients of its outputs and its
+        inputs; None where `want` says so or there is no such input. `grads`: tensors to write dq
+        and dk into, which may be g_q and g_k themselves (None in place of one: not formed)."""
+        desc = self._norm_rotate(q, k, positions, freqs, q_weight, k_weight, eps, interleaved)
+        if grads is None:
+            grads = [self.f32(q.shape) if want[0] else None,
+                     self.f32(k.shape) if want[1] and k is not None else None]
+        dq_weight = self.f32(q_weight.shape) if want[2] and q_weight is not None else None
+        dk_weight = self.f32(k_weight.shape) if want[3] and k_weight is not None else None
+        self._here(g_q, g_k, *grads)
+        need = 0
+        if dq_weight is not None or dk_weight is not None:
+            need = self.lib.ehip_norm_rotate_backward_workspace(C.byref(desc))
+        space, at, n = self._workspace(need, "norm_rotate_backward")
+        self.ok(self.lib.ehip_norm_rotate_backward_f32(
+            C.byref(desc), *self._into(g_q, "g_q", q), *self._into(g_k if k is not None else None,
+                                                                   "g_k", k),
+            *self._into(grads[0], "dq", q), *self._into(grads[1] if k is not None else None, "dk",
+                                                        k),
+            self.p(dq_weight), self.p(dk_weight), at, n, self.stream()), "norm_rotate_backward")
+        return grads[0], grads[1], dq_weight, dk_weight

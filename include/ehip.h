@@ -1044,6 +1044,55 @@ int ehip_token_logprobs_backward_f32(const float* logits, int64_t ld, const int3
                                      float* dlogits, int64_t ld_dlogits, int64_t rows,
                                      int64_t vocab, void* stream);
 
+/* ------------------------- answers sampled in groups, and training on them */
+
+/* The norm of every query and key head and its rotation by the token's
+ * position, in one pass, before ehip_attention_packed_f32, ehip_cache_append_f32
+ * and ehip_attention_paged_f32. No counterpart in the reference, whose positions
+ * are added to the embeddings. For a head x of head_dim values:
+ *   r = 1 / sqrt(mean x^2 + eps)    y = x r weight    (weight NULL: y = x)
+ *   out_a = y_a cos t - y_b sin t    out_b = y_b cos t + y_a sin t
+ * for the pairs i < rotary / 2 of its first `rotary` values, (a, b) = (i, i +
+ * rotary / 2) or with interleaved (2 i, 2 i + 1), t = positions[token] freqs[i];
+ * the values past them are y. positions (tokens int32, any value) and freqs
+ * (rotary / 2 doubles) are DEVICE arrays; the angle's product and its turns are
+ * formed in 64 bits. With rotary = 0 both may be NULL. Squares are summed in
+ * fp32: of values of 2^63 and more the norm is not finite.
+ * q are rows of heads * head_dim floats, k of kv_heads * head_dim, ld_* apart
+ * (columns of a fused projection); either may have no heads (and be NULL).
+ * 1 <= head_dim <= 256, rotary even and at most head_dim. q_out may be q with
+ * ld_q_out = ld_q, likewise k_out; no other overlap. */
+typedef struct {
+    const float *q, *k;
+    int64_t ld_q, ld_k;
+    int64_t tokens, heads, kv_heads, head_dim, rotary;
+    const int32_t* positions;
+    const double* freqs;
+    const float *q_weight, *k_weight; /* head_dim floats, or NULL */
+    float eps;
+    int interleaved;
+} ehip_norm_rotate_t;
+
+int ehip_norm_rotate_f32(const ehip_norm_rotate_t* desc, float* q_out, int64_t ld_q_out,
+                         float* k_out, int64_t ld_k_out, void* stream);
+
+/* The gradients from those of q_out and k_out and the forward's inputs: with u
+ * the gradient turned back, dx = r (weight u - x r^2 mean(weight u x)) and the
+ * weight's gradient the sum of u x r over tokens and heads. Each of dq, dk,
+ * dq_weight, dk_weight is written (not accumulated) unless NULL; without tokens
+ * the weights' gradients are zeros. dq may be q or grad_q itself (with the same
+ * ld), likewise dk. `workspace` (device memory, 16-byte aligned) holds the
+ * weights' gradients' shares during the call: at least
+ * ehip_norm_rotate_backward_workspace() bytes, of the call's own (NULL where that
+ * is 0 or no weight's gradient is asked for; -1 with the error recorded for a
+ * refused descriptor). Deterministic. */
+int64_t ehip_norm_rotate_backward_workspace(const ehip_norm_rotate_t* desc);
+int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* grad_q,
+                                  int64_t ld_grad_q, const float* grad_k, int64_t ld_grad_k,
+                                  float* dq, int64_t ld_dq, float* dk, int64_t ld_dk,
+                                  float* dq_weight, float* dk_weight, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
