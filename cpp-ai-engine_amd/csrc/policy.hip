@@ -1,0 +1,407 @@
+// policy.hip -- the clipped policy loss of sampled tokens with a KL term and an entropy bonus, and
+// its gradient with respect to their log probabilities and entropies. For a token of log probability
+// p, under the sampling policy o and under a reference f, with advantage A and entropy H:
+//
+//   d = p - o, ratio = exp(d); surrogate = min(ratio, 1 + high) A, or max(ratio, 1 - low) A for A < 0
+//   kl = exp(f - p) - (f - p) - 1
+//   loss = sum_t w_t (-surrogate + beta kl - c H), w_t the mean's over tokens or over sequences
+//   dp = w (-[not clipped] ratio A + beta (1 - exp(f - p))), dH = -c w
+//
+// HBM bounds long batches, latency short ones. The flat tokens are cut into chunks of kChunk and a
+// wave takes what one sequence has of one chunk, a segment. The segment of chunk c and sequence s
+// has place c + s, no other's: from one to the next at least one of them grows. So a wave finds its
+// segment by searching the offsets, without a list of them.
+
+#include "common.hpp"
+
+#include <algorithm>
+#include <cmath>
+
+namespace ehip {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kChunk = 512;          // tokens of a wave
+constexpr int kJoinThreads = 1024;   // sequences of a joining block at a time
+constexpr int kOwn = 4;              // segments that a thread adds up by itself
+
+// Sums of a segment, a sequence or all, in 64 bits: up to 2^31 terms.
+struct Sums {
+    double loss, kl, ratio;
+    int clipped, tokens;
+};
+
+struct BlockSums {
+    double loss, kl, ratio, clipped, tokens, count;
+};
+
+struct Policy {
+    const float *logprob, *old, *advantage, *ref, *entropy;
+    const uint8_t* mask;
+    const int32_t* cu;
+    int sequences, tokens;
+    bool advantage_by_sequence, mean_by_sequence;
+    double log_low, log_high;  // clipped where d is below, above
+    float low, high;           // the ratio there
+    float kl_weight, entropy_weight;
+    int64_t places;
+};
+
+__device__ __forceinline__ int offset(const Policy& a, int s) {
+    return min(max(a.cu[s], 0), a.tokens);
+}
+
+struct Segment {
+    int s, begin, end;
+};
+
+// The segment of a place (begin == end: none). Every lane of the wave calls it.
+__device__ __forceinline__ Segment segment_of(const Policy& a, int64_t place) {
+    if (a.sequences == 0) return Segment{0, 0, 0};
+    // The last sequence whose first place is not past it: 64 candidates at a time, a lane each.
+    const int lane = int(threadIdx.x) & 63;
+    int lo = 0, n = a.sequences;
+    while (true) {
+        const int step = (n + 63) / 64, at = lane * step;
+        const int s = at < n ? lo + at : lo;
+        const int64_t first = int64_t(offset(a, s) / kChunk) + s;
+        const int c = __popcll(__ballot(at < n && first <= place));
+        if (c > 0) lo += (c - 1) * step;
+        n = c > 0 ? min(n - (c - 1) * step, step) : 1;
+        if (step == 1 || c == 0) break;
+    }
+    Segment g{lo, 0, 0};
+    const int64_t chunk = place - lo;
+    const int64_t begin = offset(a, lo), end = offset(a, lo + 1);
+    const int64_t from = std::max(begin, chunk * kChunk), to = std::min(end, (chunk + 1) * kChunk);
+    if (chunk >= 0 && from < to) {
+        g.begin = int(from);
+        g.end = int(to);
+    }
+    return g;
+}
+
+// exp(x) - x - 1 and exp(x) - 1. Below one in magnitude by the series of the first, whose next term
+// is 2^-36 of it, as the difference would have few digits.
+__device__ __forceinline__ void kl_terms(float x, float& kl, float& rise) {
+    float s = 1.0f;
+#pragma unroll
+    for (int n = 13; n >= 3; --n) s = __builtin_fmaf(x * (1.0f / float(n)), s, 1.0f);
+    const float e = expf(x);
+    const bool small = fabsf(x) < 1.0f;
+    kl = small ? 0.5f * x * x * s : e - 1.0f - x;
+    rise = small ? x + kl : e - 1.0f;
+    if (fabsf(x) == INFINITY) kl = INFINITY;
+}
+
+// A token's terms. Where the ratio stands against its limits goes by the difference in 64 bits.
+struct Token {
+    float loss, kl, ratio, slope;  // slope: of the loss by the log probability
+    bool clipped;
+};
+
+__device__ __forceinline__ Token token_of(const Policy& a, int t, float advantage) {
+    Token x;
+    const float p = a.logprob[t];
+    const double d = double(p) - double(a.old[t]);
+    x.ratio = expf(float(d));
+    x.clipped = advantage < 0.0f ? d < a.log_low : d > a.log_high;
+    const float limit = advantage < 0.0f ? a.low : a.high;
+    x.loss = -(x.clipped ? limit : x.ratio) * advantage;
+    x.slope = x.clipped ? 0.0f : -x.ratio * advantage;
+    x.kl = 0.0f;
+    if (a.ref != nullptr) {
+        float rise;
+        kl_terms(float(double(a.ref[t]) - double(p)), x.kl, rise);
+        if (a.kl_weight != 0.0f) {
+            x.loss = __builtin_fmaf(a.kl_weight, x.kl, x.loss);
+            x.slope = __builtin_fmaf(-a.kl_weight, rise, x.slope);
+        }
+    }
+    if (a.entropy != nullptr && a.entropy_weight != 0.0f)
+        x.loss = __builtin_fmaf(-a.entropy_weight, a.entropy[t], x.loss);
+    return x;
+}
+
+template <class T>
+__device__ __forceinline__ T wave_sum(T x) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o);
+    return x;
+}
+
+__global__ __launch_bounds__(kThreads) void policy_segments(Policy a, Sums* sums) {
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int lane = int(threadIdx.x) & 63;
+    const int64_t place = int64_t(blockIdx.x) * kWaves + wave;
+    if (place >= a.places) return;
+    const Segment g = segment_of(a, place);
+    if (g.begin == g.end) return;
+    Sums x{};
+#pragma unroll 4
+    for (int t = g.begin + lane; t < g.end; t += 64) {
+        if (a.mask != nullptr && a.mask[t] == 0) continue;
+        const Token y = token_of(a, t, a.advantage[a.advantage_by_sequence ? g.s : t]);
+        x.loss += double(y.loss);
+        x.kl += double(y.kl);
+        x.ratio += double(y.ratio);
+        x.clipped += y.clipped;
+        x.tokens += 1;
+    }
+    x.loss = wave_sum(x.loss);
+    x.kl = wave_sum(x.kl);
+    x.ratio = wave_sum(x.ratio);
+    x.clipped = wave_sum(x.clipped);
+    x.tokens = wave_sum(x.tokens);
+    if (lane == 0) sums[place] = x;
+}
+
+__device__ __forceinline__ void add(Sums& x, const Sums& y) {
+    x.loss += y.loss;
+    x.kl += y.kl;
+    x.ratio += y.ratio;
+    x.clipped += y.clipped;
+    x.tokens += y.tokens;
+}
+
+__device__ __forceinline__ void finish(const Policy& a, const BlockSums& x, float* loss,
+                                       float* stats, float* weights) {
+    const bool none = x.tokens == 0.0;
+    loss[0] = none ? 0.0f : float(x.loss / x.count);
+    if (stats != nullptr) {
+        stats[0] = none ? 0.0f : float(x.kl / x.tokens);
+        stats[1] = none ? 0.0f : float(x.clipped / x.tokens);
+        stats[2] = none ? 0.0f : float(x.ratio / x.tokens);
+    }
+    weights[a.sequences] = none ? 0.0f : float(1.0 / x.count);
+}
+
+// The sums of all threads of the block in thread 0. Every thread calls it.
+__device__ __forceinline__ BlockSums block_sums(const BlockSums& mine, BlockSums* sh) {
+    const BlockSums x{wave_sum(mine.loss),    wave_sum(mine.kl),     wave_sum(mine.ratio),
+                      wave_sum(mine.clipped), wave_sum(mine.tokens), wave_sum(mine.count)};
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x / 64] = x;
+    __syncthreads();
+    BlockSums all{};
+    if (threadIdx.x == 0)
+        for (int w = 0; w < kJoinThreads / 64; ++w) {
+            all.loss += sh[w].loss;
+            all.kl += sh[w].kl;
+            all.ratio += sh[w].ratio;
+            all.clipped += sh[w].clipped;
+            all.tokens += sh[w].tokens;
+            all.count += sh[w].count;
+        }
+    return all;
+}
+
+// The sequences' sums and weights, a thread each; a sequence of many segments by its wave. One
+// block writes the results, several their sums for policy_finish.
+__global__ __launch_bounds__(kJoinThreads) void policy_sequences(Policy a, const Sums* sums,
+                                                                 BlockSums* blocks, float* loss,
+                                                                 float* stats, float* weights) {
+    __shared__ BlockSums sh[kJoinThreads / 64];
+    const int lane = int(threadIdx.x) & 63;
+    const int s = int(blockIdx.x) * kJoinThreads + int(threadIdx.x);
+    int64_t first = 0;
+    int count = 0;
+    if (s < a.sequences) {
+        const int begin = offset(a, s), end = offset(a, s + 1);
+        first = int64_t(begin / kChunk) + s;
+        count = begin < end ? (end - 1) / kChunk - begin / kChunk + 1 : 0;
+    }
+    Sums x{};
+    if (count <= kOwn)
+        for (int i = 0; i < count; ++i) add(x, sums[first + i]);
+    for (uint64_t many = __ballot(count > kOwn); many != 0; many &= many - 1) {
+        const int from = __builtin_ctzll(many);
+        const int64_t at = __shfl(first, from);
+        const int n = __shfl(count, from);
+        Sums y{};
+        for (int i = lane; i < n; i += 64) add(y, sums[at + i]);
+        y.loss = wave_sum(y.loss);
+        y.kl = wave_sum(y.kl);
+        y.ratio = wave_sum(y.ratio);
+        y.clipped = wave_sum(y.clipped);
+        y.tokens = wave_sum(y.tokens);
+        if (lane == from) x = y;
+    }
+    const double n = double(x.tokens);
+    double w = 1.0;
+    if (a.mean_by_sequence) w = x.tokens > 0 ? 1.0 / n : 0.0;
+    if (s < a.sequences) weights[s] = float(w);
+    const BlockSums mine{x.tokens > 0 ? x.loss * w : 0.0,
+                         x.kl,
+                         x.ratio,
+                         double(x.clipped),
+                         n,
+                         a.mean_by_sequence ? double(x.tokens > 0) : n};
+    const BlockSums all = block_sums(mine, sh);
+    if (threadIdx.x != 0) return;
+    if (gridDim.x > 1) blocks[blockIdx.x] = all;
+    else finish(a, all, loss, stats, weights);
+}
+
+__global__ __launch_bounds__(kJoinThreads) void policy_finish(Policy a, const BlockSums* blocks,
+                                                              int count, float* loss, float* stats,
+                                                              float* weights) {
+    __shared__ BlockSums sh[kJoinThreads / 64];
+    BlockSums x{};
+    for (int i = int(threadIdx.x); i < count; i += kJoinThreads) {
+        const BlockSums y = blocks[i];
+        x.loss += y.loss;
+        x.kl += y.kl;
+        x.ratio += y.ratio;
+        x.clipped += y.clipped;
+        x.tokens += y.tokens;
+        x.count += y.count;
+    }
+    x = block_sums(x, sh);
+    if (threadIdx.x == 0) finish(a, x, loss, stats, weights);
+}
+
+__global__ __launch_bounds__(kThreads) void policy_backward(Policy a,
+                                                            const float* __restrict__ weights,
+                                                            const float* __restrict__ grad,
+                                                            float* g_logprob, float* g_entropy) {
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int lane = int(threadIdx.x) & 63;
+    const int64_t place = int64_t(blockIdx.x) * kWaves + wave;
+    if (place >= a.places) return;
+    // Tokens of the place's chunk that are of no sequence.
+    const int64_t base = place * kChunk, stop = std::min<int64_t>(base + kChunk, a.tokens);
+    const int begin = offset(a, 0), end = offset(a, a.sequences);
+    if (base < begin || stop > end) {
+        for (int64_t t = base + lane; t < stop; t += 64) {
+            if (t >= begin && t < end) continue;
+            if (g_logprob != nullptr) g_logprob[t] = 0.0f;
+            if (g_entropy != nullptr) g_entropy[t] = 0.0f;
+        }
+    }
+    const Segment g = segment_of(a, place);
+    if (g.begin == g.end) return;
+    const float w = grad[0] * (weights[g.s] * weights[a.sequences]);
+#pragma unroll 4
+    for (int t = g.begin + lane; t < g.end; t += 64) {
+        const bool counted = a.mask == nullptr || a.mask[t] != 0;
+        if (g_logprob != nullptr) {
+            float y = 0.0f;
+            if (counted)
+                y = w * token_of(a, t, a.advantage[a.advantage_by_sequence ? g.s : t]).slope;
+            g_logprob[t] = y;
+        }
+        if (g_entropy != nullptr) g_entropy[t] = counted ? -a.entropy_weight * w : 0.0f;
+    }
+}
+
+// ---------------------------------------------------------------- host checks
+
+constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
+
+int check(const char* name, const ehip_policy_t* d, Policy& a) {
+    if (d == nullptr) return fail(EHIP_EINVAL, "%s: null descriptor", name);
+    if (d->sequences < 0 || d->tokens < 0 || d->sequences > kMaxBlocks ||
+        d->tokens > INT32_MAX - kChunk)
+        return fail(EHIP_EINVAL, "%s: %lld sequences of %lld tokens", name,
+                    (long long)d->sequences, (long long)d->tokens);
+    if (!(d->clip_low >= 0.0) || !(d->clip_high >= 0.0))
+        return fail(EHIP_EINVAL, "%s: clipped by %g and %g", name, d->clip_low, d->clip_high);
+    if (!std::isfinite(d->kl_weight) || !std::isfinite(d->entropy_weight))
+        return fail(EHIP_EINVAL, "%s: weights %g and %g", name, double(d->kl_weight),
+                    double(d->entropy_weight));
+    if ((d->kl_weight != 0.0f && d->ref_logprob == nullptr && d->tokens > 0) ||
+        (d->entropy_weight != 0.0f && d->entropy == nullptr && d->tokens > 0))
+        return fail(EHIP_EINVAL, "%s: a weighted term without its tensor", name);
+    a = Policy{};
+    a.logprob = d->logprob;
+    a.old = d->old_logprob;
+    a.advantage = d->advantage;
+    a.ref = d->ref_logprob;
+    a.entropy = d->entropy;
+    a.mask = d->mask;
+    a.cu = d->cu;
+    a.sequences = int(d->sequences);
+    a.tokens = int(d->tokens);
+    a.advantage_by_sequence = d->advantage_by_sequence != 0;
+    a.mean_by_sequence = d->mean_by_sequence != 0;
+    a.log_low = d->clip_low < 1.0 ? std::log1p(-d->clip_low) : -INFINITY;
+    a.log_high = std::log1p(d->clip_high);
+    a.low = float(1.0 - d->clip_low);
+    a.high = float(1.0 + d->clip_high);
+    a.kl_weight = d->kl_weight;
+    a.entropy_weight = d->entropy_weight;
+    a.places = a.tokens / kChunk + 1 + a.sequences;
+    return EHIP_OK;
+}
+
+int check_tensors(const char* name, const Policy& a) {
+    if (a.cu == nullptr || (a.tokens > 0 && (a.logprob == nullptr || a.old == nullptr ||
+                                             a.advantage == nullptr)))
+        return fail(EHIP_EINVAL, "%s: null tensor", name);
+    return EHIP_OK;
+}
+
+int64_t join_blocks(const Policy& a) {
+    return std::max<int64_t>(1, ceil_div(a.sequences, kJoinThreads));
+}
+
+size_t part_bytes(const Policy& a) {
+    return size_t(a.places) * sizeof(Sums) + size_t(join_blocks(a)) * sizeof(BlockSums);
+}
+
+}  // namespace
+}  // namespace ehip
+
+using namespace ehip;
+
+extern "C" {
+
+int64_t ehip_policy_loss_workspace(const ehip_policy_t* desc) {
+    Policy a;
+    return check("policy_loss", desc, a) ? -1 : int64_t(part_bytes(a));
+}
+
+int ehip_policy_loss_f32(const ehip_policy_t* desc, float* loss, float* stats, float* weights,
+                         void* workspace, size_t workspace_bytes, void* stream) {
+    EHIP_READY();
+    Policy a;
+    if (int rc = check("policy_loss", desc, a)) return rc;
+    if (int rc = check_tensors("policy_loss", a)) return rc;
+    if (loss == nullptr || weights == nullptr)
+        return fail(EHIP_EINVAL, "policy_loss: null tensor");
+    const size_t need = part_bytes(a);
+    if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
+        return fail(EHIP_EINVAL, "policy_loss: needs %zu bytes of 16-byte aligned workspace", need);
+    BlockSums* const blocks = static_cast<BlockSums*>(workspace);
+    const int64_t joins = join_blocks(a);
+    Sums* const sums = reinterpret_cast<Sums*>(blocks + joins);
+    hipStream_t s = as_stream(stream);
+    if (a.tokens > 0 && a.sequences > 0)
+        EHIP_LAUNCH("policy_loss", policy_segments, dim3(unsigned(ceil_div(a.places, kWaves))),
+                    dim3(kThreads), 0, s, a, sums);
+    EHIP_LAUNCH("policy_loss_sequences", policy_sequences, dim3(unsigned(joins)),
+                dim3(kJoinThreads), 0, s, a, sums, blocks, loss, stats, weights);
+    if (joins > 1)
+        EHIP_LAUNCH("policy_loss_finish", policy_finish, dim3(1), dim3(kJoinThreads), 0, s, a,
+                    blocks, int(joins), loss, stats, weights);
+    return EHIP_OK;
+}
+
+int ehip_policy_loss_backward_f32(const ehip_policy_t* desc, const float* weights,
+                                  const float* grad, float* g_logprob, float* g_entropy,
+                                  void* stream) {
+    EHIP_READY();
+    Policy a;
+    if (int rc = check("policy_loss_backward", desc, a)) return rc;
+    if (int rc = check_tensors("policy_loss_backward", a)) return rc;
+    if (weights == nullptr || grad == nullptr)
+        return fail(EHIP_EINVAL, "policy_loss_backward: null tensor");
+    if (a.tokens == 0 || (g_logprob == nullptr && g_entropy == nullptr)) return EHIP_OK;
+    EHIP_LAUNCH("policy_loss_backward", policy_backward,
+                dim3(unsigned(ceil_div(a.places, kWaves))), dim3(kThreads), 0, as_stream(stream), a,
+                weights, grad, g_logprob, g_entropy);
+    return EHIP_OK;
+}
+
+}  // extern "C"

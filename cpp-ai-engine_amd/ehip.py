@@ -109,6 +109,16 @@ class NormRotate(C.Structure):
                 ("eps", C.c_float), ("interleaved", C.c_int)]
 
 
+class Policy(C.Structure):
+    """ehip_policy_t: sampled tokens, and how their loss is formed."""
+    _fields_ = [("logprob", C.c_void_p), ("old_logprob", C.c_void_p), ("advantage", C.c_void_p),
+                ("ref_logprob", C.c_void_p), ("entropy", C.c_void_p), ("mask", C.c_void_p),
+                ("cu", C.c_void_p), ("sequences", C.c_int64), ("tokens", C.c_int64),
+                ("advantage_by_sequence", C.c_int), ("mean_by_sequence", C.c_int),
+                ("clip_low", C.c_double), ("clip_high", C.c_double), ("kl_weight", C.c_float),
+                ("entropy_weight", C.c_float)]
+
+
 # name -> argtypes (all return int unless listed in _RESTYPES)
 _SIGS = {
     "ehip_init": [], "ehip_available": [], "ehip_enabled": [], "ehip_set_enabled": [_i],
@@ -224,6 +234,9 @@ _SIGS = {
     "ehip_norm_rotate_backward_workspace": [C.POINTER(NormRotate)],
     "ehip_norm_rotate_backward_f32": [C.POINTER(NormRotate)] + [_vp, _i64] * 4 +
                                      [_vp, _vp, _vp, _sz, _vp],
+    "ehip_policy_loss_workspace": [C.POINTER(Policy)],
+    "ehip_policy_loss_f32": [C.POINTER(Policy), _vp, _vp, _vp, _vp, _sz, _vp],
+    "ehip_policy_loss_backward_f32": [C.POINTER(Policy)] + [_vp] * 5,
     "ehip_last_error": [],
 }
 _RESTYPES = {"ehip_last_error": C.c_char_p,
@@ -231,7 +244,8 @@ _RESTYPES = {"ehip_last_error": C.c_char_p,
              "ehip_attention_packed_backward_workspace": C.c_int64,
              "ehip_attention_paged_workspace": C.c_int64,
              "ehip_token_logprobs_workspace": C.c_int64,
-             "ehip_norm_rotate_backward_workspace": C.c_int64, "ehip_kernels_launched": C.c_uint64,
+             "ehip_norm_rotate_backward_workspace": C.c_int64,
+             "ehip_policy_loss_workspace": C.c_int64, "ehip_kernels_launched": C.c_uint64,
              "ehip_conv2d_relu_maxpool_partials": C.c_int64,
              "ehip_layernorm_backward_partials": C.c_int64,
              "ehip_kernels_failed": C.c_uint64, "ehip_reset_counters": None,
@@ -1071,3 +1085,59 @@ class Backend:
                                                         k),
             self.p(dq_weight), self.p(dk_weight), at, n, self.stream()), "norm_rotate_backward")
         return grads[0], grads[1], dq_weight, dk_weight
+
+    def _policy(self, logprob, old, advantage, cu, clip_low, clip_high, ref, kl_weight, entropy,
+                entropy_weight, mask, by_sequence, mean_by_sequence):
+        torch = self.torch
+        if logprob.dim() != 1 or cu.dim() != 1 or cu.numel() < 1:
+            raise ValueError("logprob: expected (tokens,); cu: expected (sequences + 1,)")
+        self._here(logprob, old, advantage, cu, ref, entropy, mask)
+        tokens, sequences = logprob.numel(), cu.numel() - 1
+        if mask is not None and (mask.dtype not in (torch.bool, torch.uint8)
+                                 or mask.shape != (tokens,) or not mask.is_contiguous()):
+            raise ValueError(f"mask: {mask.dtype} {tuple(mask.shape)}, expected contiguous bool or "
+                             f"uint8 ({tokens},)")
+        part = lambda t, what: None if t is None else self._dense(t, what, (tokens,))
+        return Policy(
+            part(logprob, "logprob"), part(old, "old"),
+            self._dense(advantage, "advantage", (sequences if by_sequence else tokens,)),
+            part(ref, "ref"), part(entropy, "entropy"), None if mask is None else mask.data_ptr(),
+            self._index(cu, "cu", sequences + 1), sequences, tokens, int(by_sequence),
+            int(by_sequence if mean_by_sequence is None else mean_by_sequence), clip_low,
+            clip_high, kl_weight, entropy_weight)
+
+    def policy_loss(self, logprob, old, advantage, cu, clip_low=0.2, clip_high=0.2, ref=None,
+                    kl_weight=0.0, entropy=None, entropy_weight=0.0, mask=None,
+                    by_sequence=False, mean_by_sequence=None):
+        """The clipped policy loss of sampled tokens (ehip_policy_loss_f32): logprob, old, ref and
+        entropy (tokens,) of packed sequences with the int32 offsets cu; advantage (tokens,), or
+        (sequences,) with by_sequence; mask bool or uint8, the tokens that count. The mean is over
+        tokens, or over the sequences' means with mean_by_sequence (None: as by_sequence).
+        Returns (loss (1,), stats (3,): mean kl, share of clipped ratios, mean ratio, weights for
+        policy_loss_backward)."""
+        desc = self._policy(logprob, old, advantage, cu, clip_low, clip_high, ref, kl_weight,
+                            entropy, entropy_weight, mask, by_sequence, mean_by_sequence)
+        loss, stats, weights = self.f32((1,)), self.f32((3,)), self.f32((cu.numel(),))
+        need = self.lib.ehip_policy_loss_workspace(C.byref(desc))
+        space, at, n = self._workspace(need, "policy_loss")
+        self.ok(self.lib.ehip_policy_loss_f32(C.byref(desc), self.p(loss), self.p(stats),
+                                              self.p(weights), at, n, self.stream()),
+                "policy_loss")
+        return loss, stats, weights
+
+    def policy_loss_backward(self, grad, logprob, old, advantage, cu, weights, clip_low=0.2,
+                             clip_high=0.2, ref=None, kl_weight=0.0, entropy=None,
+                             entropy_weight=0.0, mask=None, by_sequence=False,
+                             mean_by_sequence=None):
+        """(g_logprob, g_entropy) of grad (1,) times policy_loss, from the weights that it returned
+        and its other arguments; g_entropy is None without entropy."""
+        desc = self._policy(logprob, old, advantage, cu, clip_low, clip_high, ref, kl_weight,
+                            entropy, entropy_weight, mask, by_sequence, mean_by_sequence)
+        self._here(grad, weights)
+        g_logprob = self.f32(logprob.shape)
+        g_entropy = None if entropy is None else self.f32(entropy.shape)
+        self.ok(self.lib.ehip_policy_loss_backward_f32(
+            C.byref(desc), _vp(self._dense(weights, "weights", (cu.numel(),))),
+            _vp(self._dense(grad, "grad", (1,))), self.p(g_logprob), self.p(g_entropy),
+            self.stream()), "policy_loss_backward")
+        return g_logprob, g_entropy

@@ -1093,6 +1093,55 @@ int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* g
                                   float* dq_weight, float* dk_weight, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
+/* The clipped policy loss of sampled tokens, with a KL term to a reference
+ * policy and an entropy bonus, over packed sequences; its inputs and gradients
+ * are ehip_token_logprobs_f32's outputs and its backward's inputs. No
+ * counterpart in the reference. Token t, of log probability p under the policy,
+ * o under the one that sampled it and f under the reference:
+ *   ratio = exp(p - o)    kl = exp(f - p) - (f - p) - 1
+ *   surrogate = min(ratio, 1 + clip_high) A, or for A < 0 max(ratio, 1 - clip_low) A
+ *   loss = mean of (-surrogate + kl_weight kl - entropy_weight entropy)
+ * Sequence s owns tokens [cu[s], cu[s + 1]), cu a DEVICE array of sequences + 1
+ * ascending int32. Of them those whose mask byte is not 0 count (mask NULL:
+ * all); what the others hold is not looked at. advantage has one value a token,
+ * or with advantage_by_sequence one a sequence. The mean is over the tokens that
+ * count, or with mean_by_sequence over the sequences that have such, of the means
+ * over theirs. ref_logprob and entropy may be NULL, with a weight of 0.
+ * A ratio that is clipped is one past its limit; whether it is goes by p - o in
+ * 64 bits. clip_low and clip_high of 0 and more. Offsets out of range or
+ * descending are clamped: nothing outside the tensors is read or written, but the
+ * results are unspecified.
+ *
+ * loss receives one float, stats (NULL to skip) the means over the tokens that
+ * count of kl and of whether the ratio was clipped, and of the ratio; weights
+ * (sequences + 1 floats) what the backward needs. All are 0 where no token counts.
+ * Sums in 64 bits, in a fixed order. `workspace` (device memory, 16-byte aligned)
+ * holds sums during the call: at least ehip_policy_loss_workspace() bytes, of the
+ * call's own (-1 with the error recorded for a refused descriptor). */
+typedef struct {
+    const float *logprob, *old_logprob, *advantage, *ref_logprob, *entropy;
+    const uint8_t* mask;
+    const int32_t* cu;
+    int64_t sequences, tokens;
+    int advantage_by_sequence, mean_by_sequence;
+    double clip_low, clip_high;
+    float kl_weight, entropy_weight;
+} ehip_policy_t;
+
+int64_t ehip_policy_loss_workspace(const ehip_policy_t* desc);
+int ehip_policy_loss_f32(const ehip_policy_t* desc, float* loss, float* stats, float* weights,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradients of grad[0] times the loss (grad a DEVICE scalar), from the
+ * forward's weights, w a token's share of the mean:
+ *   g_logprob = grad w (kl_weight (1 - exp(f - p)) - ratio A), without the last
+ *   where the ratio is clipped    g_entropy = -grad w entropy_weight
+ * Either may be NULL. Tokens that do not count, those of no sequence among them,
+ * get 0. No overlap with the inputs. */
+int ehip_policy_loss_backward_f32(const ehip_policy_t* desc, const float* weights,
+                                  const float* grad, float* g_logprob, float* g_entropy,
+                                  void* stream);
+
 #ifdef __cplusplus
 }
 #endif
