@@ -21,16 +21,25 @@ struct Cache {
     int64_t pages, page_size, kv_heads, dim;
     const int32_t* table;
     int64_t ld_table, width, sequences;
+    float *k_scales, *v_scales;  // (pages, kv_heads, page_size) of a cache in 8 bits
 };
 
-// The row of position p of sequence s in the pools, or -1 where the table does not hold it or
-// names a page outside the pool. 0 <= s < sequences.
-__device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p) {
+// The row of position p of sequence s in the pools and its page, or -1 where the table does not
+// hold it or names a page outside the pool. 0 <= s < sequences.
+__device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p, int64_t& page) {
     if (p < 0 || p > INT32_MAX || p >= c.width * c.page_size) return -1;
     const uint32_t at = uint32_t(p) / uint32_t(c.page_size);  // in 32 bits: a tenth of the steps
-    const int64_t page = c.table[s * c.ld_table + at];
+    page = c.table[s * c.ld_table + at];
     if (page < 0 || page >= c.pages) return -1;
     return page * c.page_size + (p - int64_t(at) * c.page_size);
+}
+__device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p) {
+    int64_t page;
+    return pool_row(c, s, p, page);
+}
+// Where the scale of a row's key head is.
+__device__ __forceinline__ int64_t scale_of(const Cache& c, int64_t row, int64_t page, int head) {
+    return row + (page * (c.kv_heads - 1) + head) * c.page_size;
 }
 
 // log of a sum whose terms are 2^-24 of their value relative to 2^top; ln 2 in two parts, whose
@@ -44,10 +53,15 @@ __device__ __forceinline__ float lse_of(float top, float sum) {
 struct Bf16 {
     uint16_t bits;
 };
+// A whole number from -127 to 127, of a scale that its position and key head have.
+struct Int8 {
+    int8_t n;
+};
 __device__ __forceinline__ float widen(float x) { return x; }
 __device__ __forceinline__ float widen(Bf16 x) {
     return __builtin_bit_cast(float, uint32_t(x.bits) << 16);
 }
+__device__ __forceinline__ float widen(Int8 x) { return float(x.n); }
 // The nearest value of the pool's type, ties to even.
 __device__ __forceinline__ void narrow(float x, float& out) { out = x; }
 __device__ __forceinline__ void narrow(float x, Bf16& out) {
@@ -142,6 +156,187 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append(
                 narrow(x[u][0], dk[e]);
                 narrow(y[u][0], dv[e]);
             }
+        }
+    }
+}
+
+// The nearest whole number of scales, ties to even. The quotient in fp32 may be one off next to a
+// half; what is left, exact in 64 bits, says so.
+__device__ __forceinline__ int quantised(float x, float scale, float lift, float inverse) {
+    float n = rintf(fminf(fmaxf(x * lift * inverse, -127.0f), 127.0f));
+    const double s = double(scale), left = 2.0 * __builtin_fma(-double(n), s, double(x));
+    const bool odd = int(n) & 1;
+    if (left > s || (left == s && odd)) n += 1.0f;
+    if (left < -s || (left == -s && odd)) n -= 1.0f;
+    return int(fminf(fmaxf(n, -127.0f), 127.0f));
+}
+
+template <int N>
+__device__ __forceinline__ float largest_of(float x) {
+#pragma unroll
+    for (int w = 1; w < N; w *= 2) x = fmaxf(x, __shfl_xor(x, w));
+    return x;
+}
+
+// The scale of a head's values (those of N lanes) and a lane's four as whole numbers. A NaN or an
+// infinity makes the scale NaN and so the whole head; where the scale rounds to 0 all are 0.
+template <int N>
+__device__ __forceinline__ float quantise(const float (&x)[4], uint32_t& codes) {
+    float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    bool fine = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) fine = fine && fabsf(x[e]) < INFINITY;
+    top = largest_of<N>(fine ? top : INFINITY);
+    codes = 0;
+    if (!(top < INFINITY)) return NAN;
+    float scale = top / 127.0f;
+    if (scale == 0.0f) return 0.0f;
+    if (scale * 127.0f == INFINITY)  // the next lower one: what is read back is finite
+        scale = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, scale) - 1);
+    const float lift = scale < 0x1p-100f ? 0x1p64f : 1.0f;  // the reciprocal is finite
+    const float inverse = 1.0f / (scale * lift);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        codes |= uint32_t(quantised(x[e], scale, lift, inverse) & 0xff) << (8 * e);
+    return scale;
+}
+
+// One of the four values that a lane has of a head, and where it has fewer.
+__device__ __forceinline__ void load_head(const float* row, int d0, int dim, float (&x)[4]) {
+    if (d0 + 4 <= dim) {
+        const floatx4u y = *reinterpret_cast<const floatx4u*>(row + d0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = y[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = d0 + e < dim ? row[d0 + e] : 0.0f;
+    }
+}
+__device__ __forceinline__ void store_codes(Int8* row, int d0, int dim, uint32_t codes) {
+    if (d0 + 4 <= dim) {
+        __builtin_memcpy(row + d0, &codes, 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+            if (d0 + e < dim) row[d0 + e].n = int8_t(codes >> (8 * e));
+    }
+}
+
+// In 8 bits: a wave a token, N lanes a key head, four values of k and of v each.
+template <int N>
+__global__ __launch_bounds__(kAppendThreads) void cache_append_i8(
+    Cache c, const float* __restrict__ k, int64_t ld_k, const float* __restrict__ v, int64_t ld_v,
+    const int32_t* __restrict__ starts, const int32_t* __restrict__ cu, int tokens) {
+    constexpr int kHeads = 64 / N;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int t = int(blockIdx.x) * (kAppendThreads / 64) + wave;
+    if (t >= tokens) return;
+    const int lane = int(threadIdx.x) & 63, d0 = lane % N * 4, dim = int(c.dim);
+    const int heads = int(c.kv_heads);
+    float x[4], y[4];
+    const auto load = [&](int h) {
+        load_head(k + t * ld_k + int64_t(h < heads ? h : 0) * dim, d0, dim, x);
+        load_head(v + t * ld_v + int64_t(h < heads ? h : 0) * dim, d0, dim, y);
+    };
+    load(lane / N);
+    int s = t, first = t;
+    if (cu != nullptr) {
+        s = sequence_of(cu, int(c.sequences), t);
+        first = cu[s];
+        if (t < first || t >= cu[s + 1]) return;
+    }
+    int64_t page;
+    const int64_t row = pool_row(c, s, int64_t(starts[s]) + (t - first), page);
+    if (row < 0) return;
+    for (int h0 = 0; h0 < heads; h0 += kHeads) {
+        const int h = h0 + lane / N;
+        if (h0 > 0) load(h);
+        uint32_t kx, vx;
+        const float ks = quantise<N>(x, kx), vs = quantise<N>(y, vx);
+        if (h >= heads) continue;
+        const int64_t at = row * heads + h;
+        store_codes(static_cast<Int8*>(c.k) + at * dim, d0, dim, kx);
+        store_codes(static_cast<Int8*>(c.v) + at * dim, d0, dim, vx);
+        if (d0 == 0) {
+            const int64_t place = scale_of(c, row, page, h);
+            c.k_scales[place] = ks;
+            c.v_scales[place] = vs;
+        }
+    }
+}
+
+// ---------------------------------------------------------------------- read
+
+__device__ __forceinline__ void load4(const float* from, float (&x)[4]) {
+    const floatx4u y = *reinterpret_cast<const floatx4u*>(from);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = y[e];
+}
+__device__ __forceinline__ void load4(const Bf16* from, float (&x)[4]) {
+    Bf16 y[4];
+    __builtin_memcpy(y, __builtin_assume_aligned(from, 8), 8);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = widen(y[e]);
+}
+__device__ __forceinline__ void load4(const Int8* from, float (&x)[4]) {
+    Int8 y[4];
+    __builtin_memcpy(y, __builtin_assume_aligned(from, 4), 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = widen(y[e]);
+}
+
+// Positions of the pools as rows: a wave a token. VEC: dim and the pools allow four values at a
+// time.
+template <class T, bool VEC>
+__global__ __launch_bounds__(kAppendThreads) void cache_read(
+    Cache c, const int32_t* __restrict__ starts, const int32_t* __restrict__ cu, int tokens,
+    float* __restrict__ k, int64_t ld_k, float* __restrict__ v, int64_t ld_v) {
+    constexpr bool kScaled = sizeof(T) == 1;
+    constexpr int N = VEC ? 4 : 1;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int t = int(blockIdx.x) * (kAppendThreads / 64) + wave;
+    if (t >= tokens) return;
+    int s = t, first = t;
+    if (cu != nullptr) {
+        s = sequence_of(cu, int(c.sequences), t);
+        first = cu[s];
+        if (t < first || t >= cu[s + 1]) return;
+    }
+    int64_t page = 0;
+    const int64_t row = pool_row(c, s, int64_t(starts[s]) + (t - first), page);
+    const int n = int(c.kv_heads * c.dim);
+    const T* const from_k = static_cast<const T*>(c.k) + row * n;
+    const T* const from_v = static_cast<const T*>(c.v) + row * n;
+#pragma unroll 2
+    for (int e = (int(threadIdx.x) & 63) * N; e < n; e += 64 * N) {
+        float x[4], y[4];
+        if (row < 0) {
+#pragma unroll
+            for (int j = 0; j < N; ++j) x[j] = y[j] = NAN;
+        } else {
+            if constexpr (VEC) {
+                load4(from_k + e, x);
+                load4(from_v + e, y);
+            } else {
+                x[0] = widen(from_k[e]);
+                y[0] = widen(from_v[e]);
+            }
+            if constexpr (kScaled) {
+                const int64_t place = scale_of(c, row, page, int(uint32_t(e) / uint32_t(c.dim)));
+                const float ks = c.k_scales[place], vs = c.v_scales[place];
+#pragma unroll
+                for (int j = 0; j < N; ++j) {
+                    x[j] *= ks;
+                    y[j] *= vs;
+                }
+            }
+        }
+        if (VEC) {
+            *reinterpret_cast<floatx4u*>(k + t * ld_k + e) = floatx4u{x[0], x[1], x[2], x[3]};
+            *reinterpret_cast<floatx4u*>(v + t * ld_v + e) = floatx4u{y[0], y[1], y[2], y[3]};
+        } else {
+            k[t * ld_k + e] = x[0];
+            v[t * ld_v + e] = y[0];
         }
     }
 }
@@ -518,6 +713,7 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
 // of rows of 16-byte units; a score of NaN or +inf settles the head as NaN (64 sequences of 1024,
 // 32 heads over 8 of 128 values, us: finite 56, the first key NaN 59, the first value infinite 560;
 // value by value and to the end 1870 either way).
+template <class T>
 __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int begin, int end,
                                 float& top, float& sum, float (&o)[2]) {
     using attention::uintx4;
@@ -526,14 +722,26 @@ __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int be
     const int dim = int(a.c.dim);
     const int64_t pitch = a.c.kv_heads * dim;
     const float* q = a.q + s * a.ld_q + int64_t(h) * dim;
-    const Bf16* k = static_cast<const Bf16*>(a.c.k) + int64_t(kv) * dim;
-    const Bf16* v = static_cast<const Bf16*>(a.c.v) + int64_t(kv) * dim;
+    const T* k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
+    const T* v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
     const float c2 = a.scale * 1.44269504088896340736f;
-    // The pool row of position p0 + lane, the last again past the end.
-    const auto row_of = [&](int p0) { return int(pool_row(a.c, s, min(p0 + lane, end - 1))); };
+    // The pool row of position p0 + lane, the last again past the end, and where its scales are.
+    int64_t place = 0;
+    const auto row_of = [&](int p0) {
+        int64_t page = 0;
+        const int64_t row = pool_row(a.c, s, min(p0 + lane, end - 1), page);
+        if constexpr (sizeof(T) == 1) place = scale_of(a.c, row, page, kv);
+        return int(row);
+    };
     const auto score = [&](int row) {
-        const Bf16* at = k + int64_t(row) * pitch;
+        const T* at = k + int64_t(row) * pitch;
         float dot = 0.0f;
+        if constexpr (sizeof(T) == 1) {
+            const float ks = a.c.k_scales[place];
+            for (int e = 0; e < dim; ++e)
+                dot = __builtin_fmaf(q[e] * c2, widen(at[e]) * ks, dot);
+            return dot;
+        }
         for (int e = 0; e < dim; e += 8) {
             const uintx4 x = *reinterpret_cast<const uintx4*>(at + e);
 #pragma unroll
@@ -564,13 +772,20 @@ __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int be
     for (int p0 = begin; p0 < end; p0 += 64) {
         const int row = row_of(p0), count = min(64, end - p0);
         const float weight = lane < count ? exp2f(score(row) - shift) * 0x1p-24f : 0.0f;
+        const float vs = sizeof(T) == 1 ? a.c.v_scales[place] : 1.0f;
         sum += weight;
 #pragma unroll 8
         for (int u = 0; u < count; ++u) {
-            const Bf16* at = v + int64_t(__shfl(row, u)) * pitch;
+            const T* at = v + int64_t(__shfl(row, u)) * pitch;
             const float w = __shfl(weight, u);
-            o[0] = __builtin_fmaf(w, widen(at[d0]), o[0]);
-            o[1] = __builtin_fmaf(w, widen(at[d1]), o[1]);
+            float x0 = widen(at[d0]), x1 = widen(at[d1]);
+            if constexpr (sizeof(T) == 1) {
+                const float scale = __shfl(vs, u);
+                x0 *= scale;
+                x1 *= scale;
+            }
+            o[0] = __builtin_fmaf(w, x0, o[0]);
+            o[1] = __builtin_fmaf(w, x1, o[1]);
         }
     }
 #pragma unroll
@@ -592,11 +807,59 @@ __device__ void part_by_formula(const Paged& a, int64_t s, int h, int kv, int be
 // us, 4.0: a block passes parts of several there, and its loads run dry at each change.
 constexpr int kTilePositions = 32;
 
-template <int DP>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
+// A cache in 8 bits goes the same way: whole numbers up to 127 are bf16 values, made of the bytes
+// in registers, a score is multiplied by its position's scale of K and a weight by that of V.
+using attention::uintx4;
+typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
+
+// Eight values of a row from d0 on, as they are read.
+template <class T>
+struct Eight;
+template <>
+struct Eight<Bf16> {
+    uintx4 x;
+    __device__ __forceinline__ void load(const Bf16* row, int d0, int dim) {
+        x = *reinterpret_cast<const uintx4*>(row + (d0 < dim ? d0 : 0));
+    }
+    __device__ __forceinline__ uintx4 bf16() const { return x; }
+};
+// Of rows of any length, at any address: the last eight where fewer are left, shifted to their
+// places.
+template <>
+struct Eight<Int8> {
+    uintx2 x;
+    __device__ __forceinline__ void load(const Int8* row, int d0, int dim) {
+        if (dim < 8) {
+            uint64_t y = 0;
+            for (int e = 0; e < dim; ++e) y |= uint64_t(uint8_t(row[e].n)) << (8 * e);
+            x = __builtin_bit_cast(uintx2, d0 == 0 ? y : uint64_t(0));
+            return;
+        }
+        const int from = min(d0, dim - 8);
+        uint64_t y;
+        __builtin_memcpy(&y, row + from, 8);
+        if (d0 > from) y = d0 < dim ? y >> (8 * (d0 - from)) : 0;
+        x = __builtin_bit_cast(uintx2, y);
+    }
+    __device__ __forceinline__ uintx4 bf16() const {
+        uintx4 r;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int32_t word = int32_t(x[j / 2]);
+            const float lo = float(int8_t(word >> (16 * (j & 1))));
+            const float hi = float(int8_t(word >> (16 * (j & 1) + 8)));
+            r[j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi),
+                                         __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+        }
+        return r;
+    }
+};
+
+template <class T, int DP>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
+    constexpr bool kScaled = sizeof(T) == 1;
     using attention::bf16x8;
     using attention::floatx4u;
-    using attention::uintx4;
     typedef float floatx4 __attribute__((ext_vector_type(4)));
     typedef short shortx4 __attribute__((ext_vector_type(4)));
     constexpr int KS = DP / 32, NV = DP / 16, LANES = DP / 8;  // lanes of a row's reads
@@ -607,6 +870,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
     constexpr int kLds = kWaveLds > 16 * DP * 4 ? kWaveLds : 16 * DP * 4;
     __shared__ __attribute__((aligned(16))) char lds[kPagedWaves][kLds];
     __shared__ float sh_m[kPagedWaves][16], sh_l[kPagedWaves][16];
+    __shared__ __attribute__((aligned(16)))
+    float sh_scales[kScaled ? kPagedWaves : 1][2][kTilePositions];
     const int lane = int(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int kv_heads = int(a.c.kv_heads), dim = int(a.c.dim);
@@ -633,8 +898,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
                 const int d0 = 32 * ks + 8 * quarter;
                 float y[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    y[e] = d0 < dim && col < count ? row[d0 < dim ? d0 + e : 0] * c2 : 0.0f;
+                for (int e = 0; e < 8; ++e) {
+                    // In bf16 a head is a multiple of eight values.
+                    const bool in = d0 + (kScaled ? e : 0) < dim;
+                    y[e] = in && col < count ? row[in ? d0 + e : 0] * c2 : 0.0f;
+                }
                 attention::split8(y, q[ks]);
             }
         }
@@ -643,37 +911,40 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
         for (int i = 0; i < NV; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
 
-        const Bf16* const k = static_cast<const Bf16*>(a.c.k) + int64_t(kv) * dim;
-        const Bf16* const v = static_cast<const Bf16*>(a.c.v) + int64_t(kv) * dim;
+        const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
+        const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
         const int64_t pitch = int64_t(kv_heads) * dim;
-        bf16x8 kx[2][KS];
-        uintx4 vx[kReads];
+        Eight<T> kx[2][KS], vx[kReads];
+        float k_scale = 0.0f, v_scale = 0.0f;  // of the tile's position lane % 32
         const int v_lane = lane / LANES, v_d0 = lane % LANES * 8;
         const auto load = [&](int p0) {
             const int p = p0 + (lane & 31);
-            int64_t row = 0;
+            int64_t row = 0, page = 0;
             if (p < end) {
-                row = pool_row(a.c, s, p);
+                row = pool_row(a.c, s, p, page);
                 if (row < 0) {
                     bad = true;
-                    row = 0;
+                    row = page = 0;
                 }
+            }
+            if constexpr (kScaled) {
+                const int64_t place = scale_of(a.c, row, page, kv);
+                k_scale = p < end ? a.c.k_scales[place] : 0.0f;
+                v_scale = p < end ? a.c.v_scales[place] : 0.0f;
             }
             const int r = int(row);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const Bf16* at = k + int64_t(__shfl(r, 16 * t + col)) * pitch;
+                const T* at = k + int64_t(__shfl(r, 16 * t + col)) * pitch;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const int d0 = 32 * ks + 8 * quarter;
-                    kx[t][ks] = *reinterpret_cast<const bf16x8*>(at + (d0 < dim ? d0 : 0));
-                }
+                for (int ks = 0; ks < KS; ++ks)
+                    kx[t][ks].load(at, 32 * ks + 8 * quarter, dim);
             }
 #pragma unroll
             for (int i = 0; i < kReads; ++i) {
                 const int j = i * kRows + v_lane;
-                const Bf16* at = v + int64_t(__shfl(r, j < kTilePositions ? j : 0)) * pitch;
-                vx[i] = *reinterpret_cast<const uintx4*>(at + (v_d0 < dim ? v_d0 : 0));
+                const T* at = v + int64_t(__shfl(r, j < kTilePositions ? j : 0)) * pitch;
+                vx[i].load(at, v_d0, dim);
             }
         };
         char* const mine = lds[wave];
@@ -684,10 +955,26 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
 #pragma unroll
             for (int i = 0; i < kReads; ++i) {
                 const int j = i * kRows + v_lane;
-                uintx4 y = vx[i];
+                uintx4 y = vx[i].bf16();
                 if (tail && p0 + j >= end) y = uintx4{0, 0, 0, 0};  // nothing, whatever is there
                 if (v_lane < kRows && j < kTilePositions)
                     *reinterpret_cast<uintx4*>(mine + j * kPitch + 2 * v_d0) = y;
+            }
+            floatx4 k_by[2], v_by[2];  // the scales of a lane's scores
+            if constexpr (kScaled) {
+                if (lane < kTilePositions) {
+                    sh_scales[wave][0][lane] = k_scale;
+                    sh_scales[wave][1][lane] = v_scale;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const int at = 16 * t + 4 * quarter;
+                    k_by[t] = *reinterpret_cast<const floatx4*>(&sh_scales[wave][0][at]);
+                    v_by[t] = *reinterpret_cast<const floatx4*>(&sh_scales[wave][1][at]);
+                }
             }
             floatx4 sc[2];
 #pragma unroll
@@ -698,14 +985,20 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
                         // Past the row's end q is 0 and K something else, which has to be finite.
-                        bf16x8 f = kx[t][ks];
-                        if (DP != dim && 32 * ks + 8 * quarter >= dim)
+                        bf16x8 f = __builtin_bit_cast(bf16x8, kx[t][ks].bf16());
+                        if (!kScaled && DP != dim && 32 * ks + 8 * quarter >= dim)
                             f = __builtin_bit_cast(bf16x8, uintx4{0, 0, 0, 0});
                         sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][part], sc[t], 0,
                                                                         0, 0);
                     }
             }
             if (p0 + kPagedWaves * kTilePositions < end) load(p0 + kPagedWaves * kTilePositions);
+            if constexpr (kScaled) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[t][r] *= k_by[t][r];
+            }
             if (tail) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -730,6 +1023,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
                 part_sum += w[j];
             }
             l = __builtin_fmaf(l, keep, part_sum);
+            if constexpr (kScaled) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] *= v_by[j / 4][j % 4];
+            }
             bf16x8 p[3];
             attention::split8(w, p);
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -790,7 +1087,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_bf16(Paged a) {
                 fine = fine && fabsf(y[e]) < INFINITY;
             }
             if (!bad && !(__all(fine) && sum > 0.0f))
-                part_by_formula(a, s, h0 + g, kv, begin, end, top, sum, y);
+                part_by_formula<T>(a, s, h0 + g, kv, begin, end, top, sum, y);
             const int64_t at = int64_t(h0 + g) * (a.workers + a.c.sequences) + worker + s;
             if (bad) sum = NAN;
             if (lane == 0) {
@@ -860,7 +1157,7 @@ constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
 
 int check(const char* name, const ehip_cache_t* c, Cache& out) {
     if (c == nullptr) return fail(EHIP_EINVAL, "%s: null cache", name);
-    if ((c->type != EHIP_CACHE_F32 && c->type != EHIP_CACHE_BF16) || c->pages < 0 ||
+    if (c->type < EHIP_CACHE_F32 || c->type > EHIP_CACHE_I8 || c->pages < 0 ||
         c->page_size < 1 || c->kv_heads < 1 || c->head_dim < 1 || c->sequences < 0 ||
         c->table_width < 0 || c->ld_table < c->table_width)
         return fail(EHIP_EINVAL,
@@ -876,8 +1173,17 @@ int check(const char* name, const ehip_cache_t* c, Cache& out) {
     if ((c->sequences > 0 && c->table_width > 0 && c->table == nullptr) ||
         (c->pages > 0 && (c->k_pages == nullptr || c->v_pages == nullptr)))
         return fail(EHIP_EINVAL, "%s: null pool or table", name);
-    out = Cache{c->k_pages, c->v_pages, c->pages, c->page_size, c->kv_heads, c->head_dim,
-                c->table,   c->ld_table, c->table_width, c->sequences};
+    out = Cache{c->k_pages,  c->v_pages,     c->pages,     c->page_size, c->kv_heads, c->head_dim,
+                c->table,    c->ld_table,    c->table_width, c->sequences, nullptr,     nullptr};
+    if (c->type == EHIP_CACHE_I8) {
+        if (c->head_dim > kMaxDim)
+            return fail(EHIP_EINVAL, "%s: heads of %lld values in 8 bits", name,
+                        (long long)c->head_dim);
+        if (c->pages > 0 && (c->k_scales == nullptr || c->v_scales == nullptr))
+            return fail(EHIP_EINVAL, "%s: null scales", name);
+        out.k_scales = c->k_scales;
+        out.v_scales = c->v_scales;
+    }
     return EHIP_OK;
 }
 
@@ -944,6 +1250,43 @@ int append(const Append& x, hipStream_t s) {
     return wide ? launch_append<T, 4, false>(x, s) : launch_append<T, 1, false>(x, s);
 }
 
+template <int N>
+int launch_append_i8(const Append& x, hipStream_t s) {
+    EHIP_LAUNCH("cache_append", cache_append_i8<N>,
+                dim3(unsigned(ceil_div(x.tokens, kAppendThreads / 64))), dim3(kAppendThreads), 0, s,
+                x.c, x.k, x.ld_k, x.v, x.ld_v, x.starts, x.cu, x.tokens);
+    return EHIP_OK;
+}
+
+int append_i8(const Append& x, hipStream_t s) {
+    if (x.c.dim <= 16) return launch_append_i8<4>(x, s);
+    if (x.c.dim <= 32) return launch_append_i8<8>(x, s);
+    if (x.c.dim <= 64) return launch_append_i8<16>(x, s);
+    return launch_append_i8<32>(x, s);
+}
+
+struct Read {
+    Cache c;
+    const int32_t *starts, *cu;
+    int tokens;
+    float* k;
+    int64_t ld_k;
+    float* v;
+    int64_t ld_v;
+};
+
+template <class T>
+int read(const Read& x, hipStream_t s) {
+    const dim3 grid{unsigned(ceil_div(x.tokens, kAppendThreads / 64))}, block{kAppendThreads};
+    if (x.c.dim % 4 == 0 && aligned16(x.c.k) && aligned16(x.c.v))
+        EHIP_LAUNCH("cache_read", (cache_read<T, true>), grid, block, 0, s, x.c, x.starts, x.cu,
+                    x.tokens, x.k, x.ld_k, x.v, x.ld_v);
+    else
+        EHIP_LAUNCH("cache_read", (cache_read<T, false>), grid, block, 0, s, x.c, x.starts, x.cu,
+                    x.tokens, x.k, x.ld_k, x.v, x.ld_v);
+    return EHIP_OK;
+}
+
 template <class T, int LPP, int G, bool VEC>
 int launch_part(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
@@ -976,20 +1319,24 @@ int launch_parts_f32(const Paged& a, bool aligned, hipStream_t s) {
                                        : launch_lanes<float, false>(a, s);
 }
 
-template <int DP>
-int launch_part_bf16(const Paged& a, hipStream_t s) {
+template <class T, int DP>
+int launch_part_mfma(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
     const int64_t blocks = a.workers * ceil_div(group, 16) * a.c.kv_heads;
-    EHIP_LAUNCH("attention_paged", paged_part_bf16<DP>, dim3(unsigned(blocks)),
+    EHIP_LAUNCH("attention_paged", (paged_part_mfma<T, DP>), dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 
+template <class T>
+int launch_mfma(const Paged& a, hipStream_t s) {
+    if (a.c.dim <= 32) return launch_part_mfma<T, 32>(a, s);
+    if (a.c.dim <= 64) return launch_part_mfma<T, 64>(a, s);
+    return launch_part_mfma<T, 128>(a, s);
+}
+
 int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
-    if (!aligned || a.c.dim % 8 != 0) return launch_lanes<Bf16, false>(a, s);
-    if (a.c.dim <= 32) return launch_part_bf16<32>(a, s);
-    if (a.c.dim <= 64) return launch_part_bf16<64>(a, s);
-    return launch_part_bf16<128>(a, s);
+    return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16>(a, s) : launch_lanes<Bf16, false>(a, s);
 }
 
 }  // namespace
@@ -1017,7 +1364,30 @@ int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_
         return fail(EHIP_EINVAL, "cache_append: null tensor");
     hipStream_t s = as_stream(stream);
     const Append x{c, k, ld_k, v, ld_v, starts, cu, int(tokens)};
+    if (cache->type == EHIP_CACHE_I8) return append_i8(x, s);
     return cache->type == EHIP_CACHE_F32 ? append<float>(x, s) : append<Bf16>(x, s);
+}
+
+int ehip_cache_read_f32(const ehip_cache_t* cache, const int32_t* starts, const int32_t* cu,
+                        int64_t tokens, float* k, int64_t ld_k, float* v, int64_t ld_v,
+                        void* stream) {
+    EHIP_READY();
+    Cache c;
+    if (int rc = check("cache_read", cache, c)) return rc;
+    const int64_t n = c.kv_heads * c.dim;
+    if (n > kMaxLength) return fail(EHIP_EINVAL, "cache_read: rows of %lld values", (long long)n);
+    if (tokens < 0 || tokens > kMaxBlocks || ld_k < n || ld_v < n ||
+        (cu == nullptr && tokens != c.sequences))
+        return fail(EHIP_EINVAL, "cache_read: %lld tokens of %lld sequences, rows %lld and %lld "
+                                 "apart",
+                    (long long)tokens, (long long)c.sequences, (long long)ld_k, (long long)ld_v);
+    if (tokens == 0 || c.sequences == 0) return EHIP_OK;
+    if (k == nullptr || v == nullptr || starts == nullptr)
+        return fail(EHIP_EINVAL, "cache_read: null tensor");
+    hipStream_t s = as_stream(stream);
+    const Read x{c, starts, cu, int(tokens), k, ld_k, v, ld_v};
+    if (cache->type == EHIP_CACHE_I8) return read<Int8>(x, s);
+    return cache->type == EHIP_CACHE_F32 ? read<float>(x, s) : read<Bf16>(x, s);
 }
 
 int64_t ehip_attention_paged_workspace(const ehip_cache_t* cache, int64_t heads,
@@ -1066,8 +1436,9 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     a.first = reinterpret_cast<int*>(a.part_out + parts * c.dim);
     hipStream_t s = as_stream(stream);
     const bool aligned = aligned16(c.k) && aligned16(c.v);
-    const int rc = cache->type == EHIP_CACHE_F32 ? launch_parts_f32(a, aligned, s)
-                                                 : launch_parts_bf16(a, aligned, s);
+    const int rc = cache->type == EHIP_CACHE_F32    ? launch_parts_f32(a, aligned, s)
+                   : cache->type == EHIP_CACHE_BF16 ? launch_parts_bf16(a, aligned, s)
+                                                    : launch_mfma<Int8>(a, s);
     if (rc != EHIP_OK) return rc;
     EHIP_LAUNCH("attention_paged_join", paged_join, dim3(unsigned(c.sequences * heads)), dim3(256),
                 0, s, a);

@@ -97,7 +97,8 @@ class Cache(C.Structure):
     _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("type", C.c_int),
                 ("pages", C.c_int64), ("page_size", C.c_int64), ("kv_heads", C.c_int64),
                 ("head_dim", C.c_int64), ("table", C.c_void_p), ("ld_table", C.c_int64),
-                ("table_width", C.c_int64), ("sequences", C.c_int64)]
+                ("table_width", C.c_int64), ("sequences", C.c_int64), ("k_scales", C.c_void_p),
+                ("v_scales", C.c_void_p)]
 
 
 class NormRotate(C.Structure):
@@ -223,6 +224,7 @@ _SIGS = {
     "ehip_attention_packed_backward_f32": [C.POINTER(AttentionPacked)] + [_vp, _i64] * 4 +
                                           [_vp, _sz, _vp],
     "ehip_cache_append_f32": [C.POINTER(Cache), _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp],
+    "ehip_cache_read_f32": [C.POINTER(Cache), _vp, _vp, _i64, _vp, _i64, _vp, _i64, _vp],
     "ehip_attention_paged_workspace": [C.POINTER(Cache), _i64, _i64],
     "ehip_attention_paged_f32": [C.POINTER(Cache), _vp, _i64, _i64, _vp, _i64, _f, _vp, _i64,
                                  _vp, _vp, _sz, _vp],
@@ -907,28 +909,35 @@ class Backend:
             self.stream()), "attention_packed_backward")
         return grads
 
-    def _cache(self, k_pages, v_pages, table):
-        self._here(k_pages, v_pages, table)
-        if k_pages.dim() != 4 or k_pages.dtype not in (self.torch.float32, self.torch.bfloat16):
-            raise ValueError("k_pages: expected float32 or bfloat16 (pages, page_size, kv_heads, "
-                             "head_dim)")
+    def _cache(self, k_pages, v_pages, table, scales=None):
+        torch = self.torch
+        self._here(k_pages, v_pages, table, *(scales or ()))
+        types = {torch.float32: 0, torch.bfloat16: 1, torch.int8: 2}
+        if k_pages.dim() != 4 or k_pages.dtype not in types:
+            raise ValueError("k_pages: expected float32, bfloat16 or int8 (pages, page_size, "
+                             "kv_heads, head_dim)")
         if (v_pages.shape != k_pages.shape or v_pages.dtype != k_pages.dtype
                 or not k_pages.is_contiguous() or not v_pages.is_contiguous()):
             raise ValueError("k_pages, v_pages: expected contiguous pools of one shape and type")
         if table.dim() != 2:
             raise ValueError("table: expected (sequences, pages of the longest)")
         pages, size, kv, d = k_pages.shape
-        return Cache(k_pages.data_ptr(), v_pages.data_ptr(),
-                     int(k_pages.dtype == self.torch.bfloat16), pages, size, kv, d,
-                     table.data_ptr(), self._rows(table, "table", table.shape, self.torch.int32),
-                     table.shape[1], table.shape[0])
+        if (k_pages.dtype == torch.int8) != (scales is not None):
+            raise ValueError("scales: expected (k_scales, v_scales) with pools of int8 alone")
+        k_scales, v_scales = (None, None) if scales is None else (
+            self._dense(t, what, (pages, kv, size)) for t, what in zip(scales, ("k_scales",
+                                                                                "v_scales")))
+        return Cache(k_pages.data_ptr(), v_pages.data_ptr(), types[k_pages.dtype], pages, size, kv,
+                     d, table.data_ptr(), self._rows(table, "table", table.shape, torch.int32),
+                     table.shape[1], table.shape[0], k_scales, v_scales)
 
-    def cache_append(self, k, v, k_pages, v_pages, table, starts, cu=None):
+    def cache_append(self, k, v, k_pages, v_pages, table, starts, cu=None, scales=None):
         """Writes tokens' keys and values (tokens, kv_heads, head_dim) into the pools
-        (pages, page_size, kv_heads, head_dim; float32 or bfloat16) at positions starts[s],
+        (pages, page_size, kv_heads, head_dim; float32, bfloat16, or int8 with `scales`, the
+        float32 pools (k_scales, v_scales) of (pages, kv_heads, page_size)) at positions starts[s],
         starts[s] + 1, ... of each sequence (ehip_cache_append_f32). cu: int32 offsets of the
         sequences' tokens, None for one token each."""
-        cache = self._cache(k_pages, v_pages, table)
+        cache = self._cache(k_pages, v_pages, table, scales)
         self._here(k, v, starts, cu)
         tokens = k.shape[0]
         if cu is None and tokens != cache.sequences:
@@ -940,15 +949,38 @@ class Backend:
             None if cu is None else self._index(cu, "cu", cache.sequences + 1), tokens,
             self.stream()), "cache_append")
 
+    def cache_read(self, k_pages, v_pages, table, starts, cu=None, tokens=None, scales=None,
+                   out=None):
+        """The reverse of cache_append (ehip_cache_read_f32): (k, v), float32 (tokens, kv_heads,
+        head_dim), of the positions from starts[s] on that the offsets cu give each sequence,
+        `tokens` rows in all (without cu one each). Written into the tensors `out` where given;
+        rows of no sequence stay as they were."""
+        cache = self._cache(k_pages, v_pages, table, scales)
+        if cu is None and tokens not in (None, cache.sequences):
+            raise ValueError(f"{tokens} tokens of {cache.sequences} sequences without cu")
+        if cu is not None and tokens is None:
+            raise ValueError("tokens: expected with cu")
+        tokens = cache.sequences if cu is None else tokens
+        shape = (tokens,) + tuple(k_pages.shape[2:])
+        k, v = (self.f32(shape), self.f32(shape)) if out is None else out
+        self._here(starts, cu, k, v)
+        self.ok(self.lib.ehip_cache_read_f32(
+            C.byref(cache), self._index(starts, "starts", cache.sequences),
+            None if cu is None else self._index(cu, "cu", cache.sequences + 1), tokens,
+            _vp(k.data_ptr()), self._rows(k, "k", shape), _vp(v.data_ptr()),
+            self._rows(v, "v", shape), self.stream()), "cache_read")
+        return k, v
+
     def attention_paged(self, q, k_pages, v_pages, table, lengths, longest=None, scale=None,
-                        out=None, lse=None):
+                        out=None, lse=None, scales=None):
         """Attention of one new token per sequence over a paged cache
         (ehip_attention_paged_f32): q (sequences, heads, head_dim); table int32 (sequences,
-        pages); lengths int32, at most `longest` (None: what the table holds). Returns
-        (out, lse (sequences, heads)), written into `out` and `lse` where given."""
+        pages); lengths int32, at most `longest` (None: what the table holds); scales as in
+        cache_append. Returns (out, lse (sequences, heads)), written into `out` and `lse` where
+        given."""
         if q.dim() != 3:
             raise ValueError("q: expected (sequences, heads, head_dim)")
-        cache = self._cache(k_pages, v_pages, table)
+        cache = self._cache(k_pages, v_pages, table, scales)
         out = self.f32(q.shape) if out is None else out
         lse = self.f32(q.shape[:2]) if lse is None else lse
         self._here(q, lengths, out, lse)

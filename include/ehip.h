@@ -961,13 +961,19 @@ int ehip_attention_packed_backward_f32(const ehip_attention_packed_t* desc, cons
 
 /* A cache of keys and values in pages, for producing one token at a time. The
  * pools hold `pages` pages of page_size positions of (kv_heads, head_dim)
- * values, dense, in fp32 or bf16 (at most 2^31 - 1 positions in all); position
+ * values, dense, in fp32, bf16 or 8 bits (at most 2^31 - 1 positions in all); position
  * p of sequence s is row p % page_size of page
  * table[s * ld_table + p / page_size], table a DEVICE array of table_width
  * int32 a sequence. Pages may be shared by sequences that only read them. The
  * caller allots pages and keeps the lengths. No counterpart in the
- * reference. */
-enum { EHIP_CACHE_F32 = 0, EHIP_CACHE_BF16 = 1 };
+ * reference.
+ * In 8 bits (heads of at most 128 values) a value is a whole number n from -127
+ * to 127 times the fp32 scale of its position and key head, in pools of their own
+ * of (pages, kv_heads, page_size): the scale is fl(max |x| / 127) over the head
+ * (the next lower number where 127 times that is past fp32), n the nearest to x /
+ * scale, ties to even, within +-127. A head with a NaN or an infinity has the
+ * scale NaN, and is NaN throughout. */
+enum { EHIP_CACHE_F32 = 0, EHIP_CACHE_BF16 = 1, EHIP_CACHE_I8 = 2 };
 
 typedef struct {
     void *k_pages, *v_pages;
@@ -975,6 +981,7 @@ typedef struct {
     int64_t pages, page_size, kv_heads, head_dim;
     const int32_t* table;
     int64_t ld_table, table_width, sequences;
+    float *k_scales, *v_scales; /* of EHIP_CACHE_I8; others do not look at them */
 } ehip_cache_t;
 
 /* Writes new keys and values into the pages: token t of sequence s, row
@@ -989,19 +996,28 @@ int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_
                           const float* v, int64_t ld_v, const int32_t* starts,
                           const int32_t* cu, int64_t tokens, void* stream);
 
+/* The reverse: positions starts[s], starts[s] + 1, ... of sequence s as fp32 rows
+ * [cu[s], cu[s + 1]) of k and v (ld_k and ld_v apart, `tokens` in all; cu NULL: one
+ * for each sequence), the keys that the next piece of a prompt attends to with
+ * ehip_attention_packed_f32. A position that is negative, past its table row or on
+ * a page outside the pool gives rows of NaN; rows of no sequence stay as they were. */
+int ehip_cache_read_f32(const ehip_cache_t* cache, const int32_t* starts, const int32_t* cu,
+                        int64_t tokens, float* k, int64_t ld_k, float* v, int64_t ld_v,
+                        void* stream);
+
 /* Attention of one new token per sequence over the cache: row s of q and out
  * (heads * head_dim floats, ld_q and ld_out apart) sees positions 0 ..
  * lengths[s] - 1 (a DEVICE array; write the new token's key and value first).
  * out and lse (sequences, heads; may be NULL) as in ehip_attention_packed_f32,
  * but that small values keep fewer bits: sums run on 2^-24 of a weight, and out
- * may be off by another lengths[s] * 2^-123. They may not overlap the inputs. A
+ * may be off by another lengths[s] * 2^-123 (in 8 bits 2^-100). They may not overlap the inputs. A
  * length of zero gives out = 0, lse = -inf. A negative length, one past
  * `longest` or its table row, or a page outside the pool makes the sequence's
  * row NaN instead of a read out of bounds.
  * `longest`, a host value of at most 2^30, is what the work is split by: the
  * same lengths under another `longest` may differ in the last bits.
- * 1 <= head_dim <= 128, heads a multiple of kv_heads. Heads of a bf16 cache
- * that meet an infinity are formed a second time, at some ten times the cost.
+ * 1 <= head_dim <= 128, heads a multiple of kv_heads. Heads of a cache in bf16
+ * or 8 bits that meet an infinity are formed a second time, at some ten times the cost.
  * `workspace` (16-byte aligned) holds the parts of split lengths during the
  * call: at least ehip_attention_paged_workspace() bytes, of the call's own.
  * Deterministic. */
