@@ -236,6 +236,9 @@ _SIGS = {
     "ehip_norm_rotate_backward_workspace": [C.POINTER(NormRotate)],
     "ehip_norm_rotate_backward_f32": [C.POINTER(NormRotate)] + [_vp, _i64] * 4 +
                                      [_vp, _vp, _vp, _sz, _vp],
+    "ehip_attention_shared_workspace": [C.POINTER(Cache)] + [_i64] * 4,
+    "ehip_attention_shared_f32": [C.POINTER(Cache), _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64,
+                                  _i64, _f, _vp, _i64, _vp, _vp, _sz, _vp],
     "ehip_policy_loss_workspace": [C.POINTER(Policy)],
     "ehip_policy_loss_f32": [C.POINTER(Policy), _vp, _vp, _vp, _vp, _sz, _vp],
     "ehip_policy_loss_backward_f32": [C.POINTER(Policy)] + [_vp] * 5,
@@ -247,7 +250,8 @@ _RESTYPES = {"ehip_last_error": C.c_char_p,
              "ehip_attention_paged_workspace": C.c_int64,
              "ehip_token_logprobs_workspace": C.c_int64,
              "ehip_norm_rotate_backward_workspace": C.c_int64,
-             "ehip_policy_loss_workspace": C.c_int64, "ehip_kernels_launched": C.c_uint64,
+             "ehip_policy_loss_workspace": C.c_int64,
+             "ehip_attention_shared_workspace": C.c_int64, "ehip_kernels_launched": C.c_uint64,
              "ehip_conv2d_relu_maxpool_partials": C.c_int64,
              "ehip_layernorm_backward_partials": C.c_int64,
              "ehip_kernels_failed": C.c_uint64, "ehip_reset_counters": None,
@@ -1117,6 +1121,39 @@ class Backend:
                                                         k),
             self.p(dq_weight), self.p(dk_weight), at, n, self.stream()), "norm_rotate_backward")
         return grads[0], grads[1], dq_weight, dk_weight
+
+    def attention_shared(self, q, k_pages, v_pages, table, lengths, group_cu, shared,
+                         longest=None, longest_shared=None, scale=None, out=None, lse=None,
+                         scales=None):
+        """attention_paged where the sequences of a group share their first positions
+        (ehip_attention_shared_f32): group_cu int32 (groups + 1,), the groups' sequences; shared
+        int32 (groups,), the positions that they share, at most `longest_shared` (None: `longest`),
+        read once through the table row of the group's first sequence. Returns (out, lse)."""
+        if q.dim() != 3:
+            raise ValueError("q: expected (sequences, heads, head_dim)")
+        if group_cu.dim() != 1 or group_cu.numel() < 1:
+            raise ValueError("group_cu: expected one offset more than groups")
+        cache = self._cache(k_pages, v_pages, table, scales)
+        out = self.f32(q.shape) if out is None else out
+        lse = self.f32(q.shape[:2]) if lse is None else lse
+        self._here(q, lengths, group_cu, shared, out, lse)
+        n, h, d = cache.sequences, q.shape[1], cache.head_dim
+        groups = group_cu.numel() - 1
+        if longest is None:
+            longest = cache.table_width * cache.page_size
+        if longest_shared is None:
+            longest_shared = longest
+        need = self.lib.ehip_attention_shared_workspace(C.byref(cache), h, longest, groups,
+                                                        longest_shared)
+        space, at, size = self._workspace(need, "attention_shared")
+        self.ok(self.lib.ehip_attention_shared_f32(
+            C.byref(cache), _vp(q.data_ptr()), self._rows(q, "q", (n, h, d)), h,
+            self._index(lengths, "lengths", n), longest,
+            self._index(group_cu, "group_cu", groups + 1), self._index(shared, "shared", groups),
+            groups, longest_shared, d ** -0.5 if scale is None else scale, _vp(out.data_ptr()),
+            self._rows(out, "out", (n, h, d)), _vp(self._dense(lse, "lse", (n, h))), at, size,
+            self.stream()), "attention_shared")
+        return out, lse
 
     def _policy(self, logprob, old, advantage, cu, clip_low, clip_high, ref, kl_weight, entropy,
                 entropy_weight, mask, by_sequence, mean_by_sequence):

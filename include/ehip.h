@@ -1109,6 +1109,32 @@ int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* g
                                   float* dq_weight, float* dk_weight, void* workspace,
                                   size_t workspace_bytes, void* stream);
 
+/* ehip_attention_paged_f32 where the sequences of a group share their first
+ * positions, as answers to one prompt do: those are read once for the group.
+ * Group g is sequences [group_cu[g], group_cu[g + 1]), group_cu a DEVICE array of
+ * groups + 1 ascending int32, and shares shared[g] positions (a DEVICE array; at
+ * most longest_shared, a host value that the work is split by): they are read
+ * through the table row of its first sequence, the others through each
+ * sequence's own, so what a page holds of both may be there twice. The result is
+ * that of ehip_attention_paged_f32 with the rest of its arguments, up to the last
+ * bits, if the table rows of a group lead to the same shared positions. Sequences
+ * of no group, in a group of their own or shorter than what their group shares are
+ * passed whole, as are the groups whose number is negative, past longest_shared or
+ * past the table row. A page outside the pool among the shared positions makes the
+ * rows of all that share them NaN. Group offsets out of range or descending are
+ * clamped: nothing outside the tensors is read or written, but what the sequences
+ * they touch get is unspecified.
+ * `workspace` (16-byte aligned) holds the parts during the call: at least
+ * ehip_attention_shared_workspace() bytes, of the call's own. Deterministic. No
+ * counterpart in the reference. */
+int64_t ehip_attention_shared_workspace(const ehip_cache_t* cache, int64_t heads, int64_t longest,
+                                        int64_t groups, int64_t longest_shared);
+int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t ld_q,
+                              int64_t heads, const int32_t* lengths, int64_t longest,
+                              const int32_t* group_cu, const int32_t* shared, int64_t groups,
+                              int64_t longest_shared, float scale, float* out, int64_t ld_out,
+                              float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
 /* The clipped policy loss of sampled tokens, with a KL term to a reference
  * policy and an entropy bonus, over packed sequences; its inputs and gradients
  * are ehip_token_logprobs_f32's outputs and its backward's inputs. No
