@@ -445,24 +445,30 @@ int launch_parts_f32(const Paged& a, bool aligned, hipStream_t s) {
                                        : launch_lanes<float, false>(a, s);
 }
 
-template <class T, int DP>
+template <class T, int DP, bool WIDE>
 int launch_part_mfma(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
     const int64_t blocks = a.workers * ceil_div(group, 16) * a.c.kv_heads;
-    EHIP_LAUNCH("attention_paged", (paged_part_mfma<T, DP, false>), dim3(unsigned(blocks)),
+    EHIP_LAUNCH("attention_paged", (paged_part_mfma<T, DP, WIDE, false>), dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 
-template <class T>
+template <class T, bool WIDE>
 int launch_mfma(const Paged& a, hipStream_t s) {
-    if (a.c.dim <= 32) return launch_part_mfma<T, 32>(a, s);
-    if (a.c.dim <= 64) return launch_part_mfma<T, 64>(a, s);
-    return launch_part_mfma<T, 128>(a, s);
+    if (a.c.dim <= 32) return launch_part_mfma<T, 32, WIDE>(a, s);
+    if (a.c.dim <= 64) return launch_part_mfma<T, 64, WIDE>(a, s);
+    return launch_part_mfma<T, 128, WIDE>(a, s);
+}
+
+// Reads of whole pieces in 8 bits: of 16 values, or of 8 in heads of up to 32.
+int launch_parts_i8(const Paged& a, bool aligned, hipStream_t s) {
+    return aligned && a.c.dim % (a.c.dim <= 32 ? 8 : 16) == 0 ? launch_mfma<Int8, true>(a, s)
+                                                              : launch_mfma<Int8, false>(a, s);
 }
 
 int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
-    return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16>(a, s) : launch_lanes<Bf16, false>(a, s);
+    return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16, true>(a, s) : launch_lanes<Bf16, false>(a, s);
 }
 
 }  // namespace
@@ -470,7 +476,7 @@ int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
 int paged::launch_parts(const Paged& a, int type, hipStream_t s) {
     const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
     if (type == EHIP_CACHE_F32) return launch_parts_f32(a, aligned, s);
-    return type == EHIP_CACHE_BF16 ? launch_parts_bf16(a, aligned, s) : launch_mfma<Int8>(a, s);
+    return type == EHIP_CACHE_BF16 ? launch_parts_bf16(a, aligned, s) : launch_parts_i8(a, aligned, s);
 }
 
 }  // namespace ehip

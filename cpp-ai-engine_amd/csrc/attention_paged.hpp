@@ -627,40 +627,56 @@ constexpr int kTilePositions = 32;
 using attention::uintx4;
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 
-// Eight values of a row from d0 on, as they are read.
-template <class T>
-struct Eight;
-template <>
-struct Eight<Bf16> {
+// A lane's N values of a row from d0 on, as they are read, and eight of them at a time as bf16.
+// WIDE: rows of whole groups of N values at N bytes in 8 bits, or of 8 values at 16 bytes in bf16.
+template <class T, int N, bool WIDE>
+struct Piece;
+template <int N, bool WIDE>
+struct Piece<Bf16, N, WIDE> {
+    static_assert(N == 8 && WIDE, "what is read at a time");
     uintx4 x;
     __device__ __forceinline__ void load(const Bf16* row, int d0, int dim) {
         x = *reinterpret_cast<const uintx4*>(row + (d0 < dim ? d0 : 0));
     }
-    __device__ __forceinline__ uintx4 bf16() const { return x; }
+    __device__ __forceinline__ uintx4 bf16(int, int, int) const { return x; }
 };
-// Of rows of any length, at any address: the last eight where fewer are left, shifted to their
-// places.
-template <>
-struct Eight<Int8> {
-    uintx2 x;
+// Other rows in 8 bits, of any length and at any address, are read eight at a time, the last eight
+// where fewer are left. Those are shifted to their places where they are used: earlier, the read
+// would be waited for a tile ahead (64 sequences up to 8192, 32 heads over 8 of 128 values: 202
+// us against 85).
+template <int N, bool WIDE>
+struct Piece<Int8, N, WIDE> {
+    uint32_t x[N / 4];
     __device__ __forceinline__ void load(const Int8* row, int d0, int dim) {
-        if (dim < 8) {
-            uint64_t y = 0;
-            for (int e = 0; e < dim; ++e) y |= uint64_t(uint8_t(row[e].n)) << (8 * e);
-            x = __builtin_bit_cast(uintx2, d0 == 0 ? y : uint64_t(0));
+        if (WIDE) {
+            __builtin_memcpy(x, __builtin_assume_aligned(row + (d0 < dim ? d0 : 0), N), N);
             return;
         }
-        const int from = min(d0, dim - 8);
-        uint64_t y;
-        __builtin_memcpy(&y, row + from, 8);
-        if (d0 > from) y = d0 < dim ? y >> (8 * (d0 - from)) : 0;
-        x = __builtin_bit_cast(uintx2, y);
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i) {
+            if (dim < 8) {
+                uint64_t y = 0;
+                for (int e = 0; e < dim; ++e) y |= uint64_t(uint8_t(row[e].n)) << (8 * e);
+                __builtin_memcpy(x + 2 * i, &y, 8);
+            } else {
+                __builtin_memcpy(x + 2 * i, row + min(d0 + 8 * i, dim - 8), 8);
+            }
+        }
     }
-    __device__ __forceinline__ uintx4 bf16() const {
+    // Values 8 i .. of the piece; past the row's end 0, or with WIDE anything.
+    __device__ __forceinline__ uintx4 bf16(int i, int d0, int dim) const {
+        uint32_t y[2] = {x[2 * i], x[2 * i + 1]};
+        if (!WIDE) {
+            uint64_t z;
+            __builtin_memcpy(&z, y, 8);
+            const int d = d0 + 8 * i, from = max(0, min(d, dim - 8));
+            z = d < dim ? z >> (8 * (d - from)) : 0;
+            __builtin_memcpy(y, &z, 8);
+        }
         uintx4 r;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int32_t word = int32_t(x[j / 2]);
+            const int32_t word = int32_t(y[j / 2]);
             const float lo = float(int8_t(word >> (16 * (j & 1))));
             const float hi = float(int8_t(word >> (16 * (j & 1) + 8)));
             r[j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi),
@@ -670,14 +686,16 @@ struct Eight<Int8> {
     }
 };
 
-template <class T, int DP, bool SHARED>
+template <class T, int DP, bool WIDE, bool SHARED>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
     constexpr bool kScaled = sizeof(T) == 1;
     using attention::bf16x8;
     using attention::floatx4u;
     typedef float floatx4 __attribute__((ext_vector_type(4)));
     typedef short shortx4 __attribute__((ext_vector_type(4)));
-    constexpr int KS = DP / 32, NV = DP / 16, LANES = DP / 8;  // lanes of a row's reads
+    constexpr int N = kScaled && DP > 32 ? 16 : 8;             // values of a piece
+    constexpr int KS = DP / 32, KP = DP / (4 * N), NV = DP / 16;
+    constexpr int LANES = DP / N;                              // of a row's reads
     constexpr int kRows = 64 / LANES, kReads = (kTilePositions + kRows - 1) / kRows;
     // Rows 32 bytes apart in banks: a transposed read's sixteen rows take all banks twice.
     constexpr int kPitch = 2 * DP + 32;
@@ -712,7 +730,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             const float* row = query_row<SHARED>(a, seg, kv, h0, col < count ? col : 0);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const int d0 = 32 * ks + 8 * quarter;
+                const int d0 = 4 * N * (8 * ks / N) + N * quarter + 8 * ks % N;
                 float y[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
@@ -731,9 +749,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
         const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
         const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
         const int64_t pitch = int64_t(kv_heads) * dim;
-        Eight<T> kx[2][KS], vx[kReads];
+        Piece<T, N, WIDE> kx[2][KP], vx[kReads];
         float k_scale = 0.0f, v_scale = 0.0f;  // of the tile's position lane % 32
-        const int v_lane = lane / LANES, v_d0 = lane % LANES * 8;
+        const int v_lane = lane / LANES, v_d0 = lane % LANES * N;
         const auto load = [&](int p0) {
             const int p = p0 + (lane & 31);
             int64_t row = 0, page = 0;
@@ -754,8 +772,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             for (int t = 0; t < 2; ++t) {
                 const T* at = k + int64_t(__shfl(r, 16 * t + col)) * pitch;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
-                    kx[t][ks].load(at, 32 * ks + 8 * quarter, dim);
+                for (int p = 0; p < KP; ++p)
+                    kx[t][p].load(at, 4 * N * p + N * quarter, dim);
             }
 #pragma unroll
             for (int i = 0; i < kReads; ++i) {
@@ -772,10 +790,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
 #pragma unroll
             for (int i = 0; i < kReads; ++i) {
                 const int j = i * kRows + v_lane;
-                uintx4 y = vx[i].bf16();
-                if (tail && p0 + j >= end) y = uintx4{0, 0, 0, 0};  // nothing, whatever is there
-                if (v_lane < kRows && j < kTilePositions)
-                    *reinterpret_cast<uintx4*>(mine + j * kPitch + 2 * v_d0) = y;
+#pragma unroll
+                for (int e = 0; e < N / 8; ++e) {
+                    uintx4 y = vx[i].bf16(e, v_d0, dim);
+                    if (tail && p0 + j >= end) y = uintx4{0, 0, 0, 0};  // nothing, whatever is there
+                    if (v_lane < kRows && j < kTilePositions)
+                        *reinterpret_cast<uintx4*>(mine + j * kPitch + 2 * v_d0 + 16 * e) = y;
+                }
             }
             floatx4 k_by[2], v_by[2];  // the scales of a lane's scores
             if constexpr (kScaled) {
@@ -802,7 +823,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
                         // Past the row's end q is 0 and K something else, which has to be finite.
-                        bf16x8 f = __builtin_bit_cast(bf16x8, kx[t][ks].bf16());
+                        const int d0 = 4 * N * (8 * ks / N) + N * quarter;
+                        bf16x8 f = __builtin_bit_cast(
+                            bf16x8, kx[t][8 * ks / N].bf16(ks % (N / 8), d0, dim));
                         if (!kScaled && DP != dim && 32 * ks + 8 * quarter >= dim)
                             f = __builtin_bit_cast(bf16x8, uintx4{0, 0, 0, 0});
                         sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][part], sc[t], 0,

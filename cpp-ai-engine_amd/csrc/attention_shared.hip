@@ -204,25 +204,31 @@ int launch_lanes(const Paged& a, hipStream_t s) {
     return launch_vector<T, 128 / N, VEC>(a, s);
 }
 
-template <class T, int DP>
+template <class T, int DP, bool WIDE>
 int launch_part_mfma(const Paged& a, hipStream_t s) {
-    EHIP_LAUNCH("attention_shared", (paged_part_mfma<T, DP, true>),
+    EHIP_LAUNCH("attention_shared", (paged_part_mfma<T, DP, WIDE, true>),
                 dim3(unsigned(a.workers * a.c.kv_heads)), dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 
-template <class T>
+template <class T, bool WIDE>
 int launch_mfma(const Paged& a, hipStream_t s) {
-    if (a.c.dim <= 32) return launch_part_mfma<T, 32>(a, s);
-    if (a.c.dim <= 64) return launch_part_mfma<T, 64>(a, s);
-    return launch_part_mfma<T, 128>(a, s);
+    if (a.c.dim <= 32) return launch_part_mfma<T, 32, WIDE>(a, s);
+    if (a.c.dim <= 64) return launch_part_mfma<T, 64, WIDE>(a, s);
+    return launch_part_mfma<T, 128, WIDE>(a, s);
+}
+
+// Reads of whole pieces in 8 bits: of 16 values, or of 8 in heads of up to 32.
+int launch_parts_i8(const Paged& a, bool aligned, hipStream_t s) {
+    return aligned && a.c.dim % (a.c.dim <= 32 ? 8 : 16) == 0 ? launch_mfma<Int8, true>(a, s)
+                                                              : launch_mfma<Int8, false>(a, s);
 }
 
 int launch_shared(const Paged& a, int type, hipStream_t s) {
     const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
-    if (type == EHIP_CACHE_I8) return launch_mfma<Int8>(a, s);
+    if (type == EHIP_CACHE_I8) return launch_parts_i8(a, aligned, s);
     if (type == EHIP_CACHE_BF16)
-        return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16>(a, s)
+        return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16, true>(a, s)
                                            : launch_lanes<Bf16, false>(a, s);
     return aligned && a.c.dim % 4 == 0 ? launch_lanes<float, true>(a, s)
                                        : launch_lanes<float, false>(a, s);
