@@ -336,12 +336,17 @@ __global__ __launch_bounds__(256) void paged_join(Paged a) {
 // Workers for 512 blocks in all, two a CU (64 sequences of 64 to 4096 positions in bf16: 75 us
 // against 85 with 1024 blocks and 101 with 2048; two of 131072 in fp32: 383, 388, 389), and no more
 // than there can be tiles.
-int paged::workers_of(const Cache& c, int64_t heads, int64_t longest, int type) {
+//
+// Of waves 2048, as many.
+Cut paged::cut_of(const Cache& c, int64_t heads, int64_t longest, int type) {
+    const bool waves = by_waves(c, type);
     const int64_t group = heads / c.kv_heads;
-    const int64_t units = c.kv_heads * ceil_div(group, type == EHIP_CACHE_F32 ? kMaxGroup : 16);
-    constexpr int64_t resident = 512;
-    const int64_t most = std::max<int64_t>(1, c.sequences * ceil_div(longest, kTile));
-    return int(std::min(most, std::max<int64_t>(1, resident / units)));
+    const int64_t units =
+        c.kv_heads * ceil_div(group, waves || type != EHIP_CACHE_F32 ? 16 : kMaxGroup);
+    const int64_t resident = waves ? 2048 : 512;
+    const int tile = tile_of(waves, c.sequences, longest);
+    const int64_t most = std::max<int64_t>(1, c.sequences * ceil_div(longest, tile));
+    return Cut{waves, tile, int(std::min(most, std::max<int64_t>(1, resident / units)))};
 }
 
 namespace {
@@ -448,7 +453,7 @@ int launch_parts_f32(const Paged& a, bool aligned, hipStream_t s) {
 template <class T, int DP, bool WIDE>
 int launch_part_mfma(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
-    const int64_t blocks = a.workers * ceil_div(group, 16) * a.c.kv_heads;
+    const int64_t blocks = ceil_div(a.workers * ceil_div(group, 16) * a.c.kv_heads, kPagedWaves);
     EHIP_LAUNCH("attention_paged", (paged_part_mfma<T, DP, WIDE, false>), dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
@@ -467,8 +472,9 @@ int launch_parts_i8(const Paged& a, bool aligned, hipStream_t s) {
                                                               : launch_mfma<Int8, false>(a, s);
 }
 
-int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
-    return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16, true>(a, s) : launch_lanes<Bf16, false>(a, s);
+int launch_parts_bf16(const Paged& a, hipStream_t s) {
+    return by_waves(a.c, EHIP_CACHE_BF16) ? launch_mfma<Bf16, true>(a, s)
+                                          : launch_lanes<Bf16, false>(a, s);
 }
 
 }  // namespace
@@ -476,7 +482,7 @@ int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
 int paged::launch_parts(const Paged& a, int type, hipStream_t s) {
     const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
     if (type == EHIP_CACHE_F32) return launch_parts_f32(a, aligned, s);
-    return type == EHIP_CACHE_BF16 ? launch_parts_bf16(a, aligned, s) : launch_parts_i8(a, aligned, s);
+    return type == EHIP_CACHE_BF16 ? launch_parts_bf16(a, s) : launch_parts_i8(a, aligned, s);
 }
 
 }  // namespace ehip
@@ -536,7 +542,7 @@ int64_t ehip_attention_paged_workspace(const ehip_cache_t* cache, int64_t heads,
         return -1;
     return c.sequences == 0
                ? 0
-               : int64_t(part_bytes(c, heads, workers_of(c, heads, longest, cache->type)));
+               : int64_t(part_bytes(c, heads, cut_of(c, heads, longest, cache->type).workers));
 }
 
 int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t ld_q,
@@ -552,8 +558,8 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     if (c.sequences == 0) return EHIP_OK;
     if (q == nullptr || lengths == nullptr || out == nullptr)
         return fail(EHIP_EINVAL, "attention_paged: null tensor");
-    const int workers = workers_of(c, heads, longest, cache->type);
-    const size_t need = part_bytes(c, heads, workers);
+    const Cut cut = cut_of(c, heads, longest, cache->type);
+    const size_t need = part_bytes(c, heads, cut.workers);
     if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
         return fail(EHIP_EINVAL, "attention_paged: needs %zu bytes of 16-byte aligned workspace",
                     need);
@@ -568,8 +574,9 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     a.out = out;
     a.ld_out = ld_out;
     a.lse = lse;
-    a.workers = workers;
-    const int64_t parts = heads * (workers + c.sequences);
+    a.tile = cut.tile;
+    a.workers = cut.workers;
+    const int64_t parts = heads * (cut.workers + c.sequences);
     a.part_stats = static_cast<float2*>(workspace);
     a.part_out = reinterpret_cast<float*>(a.part_stats + parts);
     a.first = reinterpret_cast<int*>(a.part_out + parts * c.dim);

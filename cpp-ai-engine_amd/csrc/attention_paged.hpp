@@ -94,7 +94,8 @@ struct Paged {
     float* out;
     int64_t ld_out;
     float* lse;
-    int workers;         // blocks of a key head (and piece of its query heads)
+    int tile;            // positions that the work is cut by
+    int workers;         // blocks, or waves, of a key head (and piece of its query heads)
     float2* part_stats;  // (heads, workers + sequences): maximum (as 2^x), sum
     float* part_out;     // (heads, workers + sequences, dim)
     int* first;          // (sequences + 1): the sequences' first tiles
@@ -106,12 +107,13 @@ struct Paged {
     int places;          // parts of a key head, `rows` rows each, in the layout (kv_heads, places)
 };
 
-// The work is cut evenly, whatever the lengths: the positions of all sequences in tiles of kTile,
-// one after the other, and a worker's blocks (one for each key head) take its share of them, which
-// may be part of a long sequence or several short ones. What a worker adds to a sequence is a
-// segment. Segment (worker w, sequence s) has place w + s of a head's parts, no other's: from one
-// to the next at least one of them grows.
-constexpr int kTile = 128;
+// The work is cut evenly, whatever the lengths: the positions of all sequences in tiles, one after
+// the other, and a worker (a block of the vector kernel, a wave of the other, for each key head)
+// takes its share of them, which may be part of a long sequence or several short ones. What a worker
+// adds to a sequence is a segment. Segment (worker w, sequence s) has place w + s of a head's parts,
+// no other's: from one to the next at least one of them grows.
+constexpr int kTile = 128;      // of blocks
+constexpr int kWaveTile = 32;   // of waves
 
 // Positions of a sequence, -1 for a length that is none.
 __device__ __forceinline__ int length_of(const Paged& a, int64_t s) {
@@ -120,7 +122,9 @@ __device__ __forceinline__ int length_of(const Paged& a, int64_t s) {
                ? -1
                : n;
 }
-__device__ __forceinline__ int tiles_of(int n) { return n > 0 ? (n - 1) / kTile + 1 : 0; }
+__device__ __forceinline__ int tiles_of(const Paged& a, int n) {
+    return n > 0 ? int(uint32_t(n - 1) / uint32_t(a.tile)) + 1 : 0;
+}
 
 // Positions of a sequence that are its own.
 __device__ __forceinline__ int start_of(const Paged& a, int64_t s) {
@@ -153,7 +157,7 @@ __device__ __forceinline__ int items(const Paged& a) {
 }
 template <bool SHARED>
 __device__ __forceinline__ int unit_tiles(const Paged& a, int i) {
-    return tiles_of(SHARED ? shared_of(a, i) : own_of(a, i));
+    return tiles_of(a, SHARED ? shared_of(a, i) : own_of(a, i));
 }
 template <bool SHARED>
 __device__ __forceinline__ int item_tiles(const Paged& a, int i) {
@@ -199,8 +203,8 @@ __device__ __forceinline__ void measure(const Paged& a, Segment& g) {
     const int start = SHARED ? 0 : start_of(a, g.item);
     const int end = SHARED ? shared_of(a, g.item) : length_of(a, g.item);
     g.s = SHARED ? group_begin(a, g.item) : g.item;
-    g.begin = start + (g.t - g.t0) * kTile;
-    g.end = stop - g.t0 == g.n ? end : start + (stop - g.t0) * kTile;
+    g.begin = start + (g.t - g.t0) * a.tile;
+    g.end = stop - g.t0 == g.n ? end : start + (stop - g.t0) * a.tile;
     g.whole = !SHARED && g.begin == 0 && g.end == end;
 }
 
@@ -617,9 +621,9 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int k
 //   weights: the D's of positions 0..15 and 16..31 are the B of 32 positions, in the order
 //            4 h + 0..3, 16 + 4 h + 0..3 for the lanes h = l / 16
 //   values:  A = 16 values by those 32 positions of V: rows in LDS, read transposed
-// A wave takes 32 positions at a time; the next ones' reads are out while it forms weights and
-// sums. 64 sequences of 4096, 32 heads over 8 of 128 values: 213 us, 5.0 TB/s; of 64 to 4096, 66
-// us, 4.0: a block passes parts of several there, and its loads run dry at each change.
+// A wave takes 32 positions at a time; the next ones' reads are out while it forms weights and sums,
+// and so across the end of a segment: the waves of a block have nothing in common but that they read
+// the key heads of the same positions, which lie next to each other.
 constexpr int kTilePositions = 32;
 
 // A cache in 8 bits goes the same way: whole numbers up to 127 are bf16 values, made of the bytes
@@ -699,23 +703,21 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
     constexpr int kRows = 64 / LANES, kReads = (kTilePositions + kRows - 1) / kRows;
     // Rows 32 bytes apart in banks: a transposed read's sixteen rows take all banks twice.
     constexpr int kPitch = 2 * DP + 32;
-    constexpr int kWaveLds = kTilePositions * kPitch;
-    constexpr int kLds = kWaveLds > 16 * DP * 4 ? kWaveLds : 16 * DP * 4;
-    __shared__ __attribute__((aligned(16))) char lds[kPagedWaves][kLds];
-    __shared__ float sh_m[kPagedWaves][16], sh_l[kPagedWaves][16];
+    __shared__ __attribute__((aligned(16))) char lds[kPagedWaves][kTilePositions * kPitch];
     __shared__ __attribute__((aligned(16)))
     float sh_scales[kScaled ? kPagedWaves : 1][2][kTilePositions];
     const int lane = int(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int kv_heads = int(a.c.kv_heads), dim = int(a.c.dim);
     const int group = a.heads / kv_heads, pieces = SHARED ? 1 : (group + 15) / 16;
-    uint32_t x = blockIdx.x;
+    uint32_t x = blockIdx.x * kPagedWaves + wave;
     const int kv = int(x % uint32_t(kv_heads));
     x /= uint32_t(kv_heads);
     const int h0 = kv * group + int(x % uint32_t(pieces)) * 16;
-    const int heads = min(16, (kv + 1) * group - h0);  // the block's
+    const int heads = min(16, (kv + 1) * group - h0);  // the wave's
     x /= uint32_t(pieces);
     const int worker = int(x);
+    if (worker >= a.workers) return;  // no barrier follows
     for (Segment seg = first_segment<SHARED>(a, worker); seg.t < seg.t_end;
          next_segment<SHARED>(a, seg)) {
         const int64_t s = seg.s;
@@ -752,7 +754,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
         Piece<T, N, WIDE> kx[2][KP], vx[kReads];
         float k_scale = 0.0f, v_scale = 0.0f;  // of the tile's position lane % 32
         const int v_lane = lane / LANES, v_d0 = lane % LANES * N;
-        const auto load = [&](int p0) {
+        // The pool row of position p0 + lane % 32 and where its scales are: found a tile before
+        // the reads of the rows, which would else wait for the table.
+        int r = 0;
+        int64_t place = 0;
+        const auto find = [&](int p0) {
             const int p = p0 + (lane & 31);
             int64_t row = 0, page = 0;
             if (p < end) {
@@ -762,12 +768,15 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
                     row = page = 0;
                 }
             }
+            if constexpr (kScaled) place = scale_of(a.c, row, page, kv);
+            r = int(row);
+        };
+        const auto load = [&](int p0) {
             if constexpr (kScaled) {
-                const int64_t place = scale_of(a.c, row, page, kv);
-                k_scale = p < end ? a.c.k_scales[place] : 0.0f;
-                v_scale = p < end ? a.c.v_scales[place] : 0.0f;
+                const bool in = p0 + (lane & 31) < end;
+                k_scale = in ? a.c.k_scales[place] : 0.0f;
+                v_scale = in ? a.c.v_scales[place] : 0.0f;
             }
-            const int r = int(row);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const T* at = k + int64_t(__shfl(r, 16 * t + col)) * pitch;
@@ -783,9 +792,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             }
         };
         char* const mine = lds[wave];
-        const int first = begin + wave * kTilePositions;
-        if (first < end) load(first);
-        for (int p0 = first; p0 < end; p0 += kPagedWaves * kTilePositions) {
+        find(begin);
+        load(begin);
+        find(begin + kTilePositions);
+        for (int p0 = begin; p0 < end; p0 += kTilePositions) {
             const bool tail = p0 + kTilePositions > end;
 #pragma unroll
             for (int i = 0; i < kReads; ++i) {
@@ -832,7 +842,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
                                                                         0, 0);
                     }
             }
-            if (p0 + kPagedWaves * kTilePositions < end) load(p0 + kPagedWaves * kTilePositions);
+            if (p0 + kTilePositions < end) {
+                load(p0 + kTilePositions);
+                find(p0 + 2 * kTilePositions);
+            }
             if constexpr (kScaled) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
@@ -893,57 +906,60 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
-        bad = __syncthreads_or(bad);
-
-        // The waves of the block: sums of head `col`, value 16 i + 4 quarter + r.
+        // Head `col`, values 16 i + 4 quarter + r.
+        bad = __any(bad);
         l = with_half(with_row_pair(l));
-        if (quarter == 0) {
-            sh_m[wave][col] = m;
-            sh_l[wave][col] = l;
-        }
-        float* const sums = reinterpret_cast<float*>(mine);
+        bool fine = l > 0.0f && l < INFINITY;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            *reinterpret_cast<floatx4*>(sums + col * DP + 16 * i + 4 * quarter) = o[i];
-        __syncthreads();
-        for (int g = wave; g < count; g += kPagedWaves) {
-            float top = sh_m[0][g], sum = 0.0f, keep[kPagedWaves], y[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int u = 1; u < kPagedWaves; ++u) top = fmaxf(top, sh_m[u][g]);
-            bool fine = true;
-#pragma unroll
-            for (int u = 0; u < kPagedWaves; ++u) {
-                keep[u] = sh_m[u][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh_m[u][g] - top);
-                sum += sh_l[u][g] * keep[u];
-                fine = fine && fabsf(sh_l[u][g]) < INFINITY;
+            for (int r = 0; r < 4; ++r) fine = fine && fabsf(o[i][r]) < INFINITY;
+        const uint64_t lanes = __ballot(!fine);
+        uint32_t again = uint32_t(lanes | lanes >> 32);
+        again = (again | again >> 16) & 0xffffu & ((1u << count) - 1u);
+        const int64_t at = part_of<SHARED>(a, seg, worker, kv, h0, col < count ? col : 0);
+        if (bad) l = NAN;
+        if (col < count && (bad || !(again >> col & 1))) {
+            if (quarter == 0) {
+                if (!seg.whole) a.part_stats[at] = float2{m, l};
+                else if (a.lse != nullptr) a.lse[s * a.heads + h0 + col] = lse_of(m, l);
             }
+            float* const to = seg.whole ? a.out + s * a.ld_out + int64_t(h0 + col) * dim
+                                        : a.part_out + at * dim;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int d = lane + 64 * e;
-                if (d >= dim) continue;
+            for (int i = 0; i < NV; ++i) {
+                const int d = 16 * i + 4 * quarter;
+                floatx4u y;
 #pragma unroll
-                for (int u = 0; u < kPagedWaves; ++u)
-                    y[e] += reinterpret_cast<const float*>(lds[u])[g * DP + d] * keep[u];
-                fine = fine && fabsf(y[e]) < INFINITY;
+                for (int r = 0; r < 4; ++r) y[r] = seg.whole ? o[i][r] / l : o[i][r];
+                if (d + 4 <= dim) {
+                    *reinterpret_cast<floatx4u*>(to + d) = y;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 3; ++r)
+                        if (d + r < dim) to[d + r] = y[r];
+                }
             }
-            if (!bad && !(__all(fine) && sum > 0.0f))
-                part_by_formula<T>(a, s, query_row<SHARED>(a, seg, kv, h0, g), kv, begin, end, top,
-                                   sum, y);
-            const int64_t at = part_of<SHARED>(a, seg, worker, kv, h0, g);
-            if (bad) sum = NAN;
+        }
+        if (bad) continue;
+        for (; again != 0; again &= again - 1) {
+            const int g = __builtin_ctz(again);
+            float top, sum, y[2];
+            part_by_formula<T>(a, s, query_row<SHARED>(a, seg, kv, h0, g), kv, begin, end, top, sum,
+                               y);
+            const int64_t place = part_of<SHARED>(a, seg, worker, kv, h0, g);
             if (lane == 0) {
-                if (!seg.whole) a.part_stats[at] = float2{top, sum};
+                if (!seg.whole) a.part_stats[place] = float2{top, sum};
                 else if (a.lse != nullptr) a.lse[s * a.heads + h0 + g] = lse_of(top, sum);
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int d = lane + 64 * e;
                 if (d >= dim) continue;
-                if (!seg.whole) a.part_out[at * dim + d] = y[e];
+                if (!seg.whole) a.part_out[place * dim + d] = y[e];
                 else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y[e] / sum;
             }
         }
-        __syncthreads();
     }
 }
 
@@ -1005,9 +1021,24 @@ inline size_t part_bytes(const Cache& c, int64_t heads, int workers) {
            size_t(c.sequences + 1) * sizeof(int);
 }
 
-// Blocks of a key head for these sequences, and the launch over their own positions
-// (attention_paged.hip).
-int workers_of(const Cache& c, int64_t heads, int64_t longest, int type);
+// How the work of a call is cut: by the matrix instructions' kernel, of waves, or the vector one.
+struct Cut {
+    bool waves;
+    int tile, workers;
+};
+
+// bf16 in rows of 16-byte units and 8 bits go by the matrix instructions.
+inline bool by_waves(const Cache& c, int type) {
+    return type == EHIP_CACHE_I8 || (type == EHIP_CACHE_BF16 && c.dim % 8 == 0 &&
+                                     aligned16(c.k) && aligned16(c.v));
+}
+// Positions that so many rows of work of at most `longest` are cut by.
+inline int tile_of(bool waves, int64_t rows, int64_t longest) {
+    return waves && rows * ceil_div(longest, kWaveTile) <= INT32_MAX ? kWaveTile : kTile;
+}
+
+// The cut of the sequences' own positions, and the launch over them (attention_paged.hip).
+Cut cut_of(const Cache& c, int64_t heads, int64_t longest, int type);
 int launch_parts(const Paged& a, int type, hipStream_t s);
 
 }  // namespace paged

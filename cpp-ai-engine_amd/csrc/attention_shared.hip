@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void shared_join(Paged own, Paged a) {
         const int lo = group_of(a.group_cu, a.groups, int(s));
         const int group = a.heads / int(a.c.kv_heads), kv = h / group;
         const int row = int(s - group_begin(a, lo)) * group + h % group;
-        const int tile = row / a.rows, each = tiles_of(shared_of(a, lo));
+        const int tile = row / a.rows, each = tiles_of(a, shared_of(a, lo));
         const int tiles = a.first[a.groups], t0 = a.first[lo] + tile * each;
         const int w0 = worker_of(a, t0, tiles);
         shared_parts = worker_of(a, t0 + each - 1, tiles) - w0 + 1;
@@ -155,15 +155,9 @@ int check_groups(const char* name, const Cache& c, int64_t heads, int64_t groups
     return EHIP_OK;
 }
 
-// The group's rows of a block, by what the kernel of a cache of that type takes.
-int rows_of(const Cache& c, int type) {
-    const bool aligned = aligned16(c.k) && aligned16(c.v);
-    if (type == EHIP_CACHE_I8 || (type == EHIP_CACHE_BF16 && aligned && c.dim % 8 == 0)) return 16;
-    return kMaxGroup;
-}
-
 struct Plan {
-    int rows, workers, places, own_workers;
+    Cut own, shared;
+    int rows, places;
     size_t own_bytes, part_bytes, first_bytes, bytes;
 };
 
@@ -172,14 +166,17 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t groups,
              int64_t longest_shared) {
     Plan p{};
-    p.rows = rows_of(c, type);
-    const int64_t group = heads / c.kv_heads;
-    const int64_t row_tiles = c.sequences * group / p.rows + groups;
-    const int64_t most = std::max<int64_t>(1, row_tiles * ceil_div(longest_shared, kTile));
-    p.workers = int(std::min(most, std::max<int64_t>(1, 512 / c.kv_heads)));
-    p.places = int(p.workers + row_tiles + 1);
-    p.own_workers = workers_of(c, heads, longest, type);
-    p.own_bytes = round16(part_bytes(c, heads, p.own_workers));
+    p.own = cut_of(c, heads, longest, type);
+    const bool waves = p.own.waves;
+    p.rows = waves ? 16 : kMaxGroup;
+    const int64_t row_tiles = c.sequences * (heads / c.kv_heads) / p.rows + groups;
+    const int tile = tile_of(waves, row_tiles, longest_shared);
+    const int64_t most = std::max<int64_t>(1, row_tiles * ceil_div(longest_shared, tile));
+    const int64_t resident = waves ? 2048 : 512;
+    p.shared = Cut{waves, tile,
+                   int(std::min(most, std::max<int64_t>(1, resident / c.kv_heads)))};
+    p.places = int(p.shared.workers + row_tiles + 1);
+    p.own_bytes = round16(part_bytes(c, heads, p.own.workers));
     p.part_bytes = round16(size_t(c.kv_heads) * size_t(p.places) * size_t(p.rows) *
                            (sizeof(float2) + size_t(c.dim) * sizeof(float)));
     // The parts of both; the groups' first tiles, offsets and shared positions, and the sequences'
@@ -207,7 +204,7 @@ int launch_lanes(const Paged& a, hipStream_t s) {
 template <class T, int DP, bool WIDE>
 int launch_part_mfma(const Paged& a, hipStream_t s) {
     EHIP_LAUNCH("attention_shared", (paged_part_mfma<T, DP, WIDE, true>),
-                dim3(unsigned(a.workers * a.c.kv_heads)), dim3(kPagedThreads), 0, s, a);
+                dim3(unsigned(ceil_div(a.workers * a.c.kv_heads, kPagedWaves))), dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 
@@ -228,8 +225,8 @@ int launch_shared(const Paged& a, int type, hipStream_t s) {
     const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
     if (type == EHIP_CACHE_I8) return launch_parts_i8(a, aligned, s);
     if (type == EHIP_CACHE_BF16)
-        return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16, true>(a, s)
-                                           : launch_lanes<Bf16, false>(a, s);
+        return by_waves(a.c, type) ? launch_mfma<Bf16, true>(a, s)
+                                   : launch_lanes<Bf16, false>(a, s);
     return aligned && a.c.dim % 4 == 0 ? launch_lanes<float, true>(a, s)
                                        : launch_lanes<float, false>(a, s);
 }
@@ -285,13 +282,15 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     a.lse = lse;
     Paged own = a;
     char* at = static_cast<char*>(workspace);
-    own.workers = p.own_workers;
+    own.tile = p.own.tile;
+    own.workers = p.own.workers;
     const int64_t parts = heads * (own.workers + c.sequences);
     own.part_stats = reinterpret_cast<float2*>(at);
     own.part_out = reinterpret_cast<float*>(own.part_stats + parts);
     own.first = reinterpret_cast<int*>(own.part_out + parts * c.dim);
     at += p.own_bytes;
-    a.workers = p.workers;
+    a.tile = p.shared.tile;
+    a.workers = p.shared.workers;
     a.rows = p.rows;
     a.places = p.places;
     a.groups = int(groups);
