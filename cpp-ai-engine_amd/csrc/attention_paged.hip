@@ -190,8 +190,8 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_i8(
         first = cu[s];
         if (t < first || t >= cu[s + 1]) return;
     }
-    int64_t page;
-    const int64_t row = pool_row(c, s, int64_t(starts[s]) + (t - first), page);
+    uint32_t off;
+    const int64_t row = pool_row(c, s, int64_t(starts[s]) + (t - first), off);
     if (row < 0) return;
     for (int h0 = 0; h0 < heads; h0 += kHeads) {
         const int h = h0 + lane / N;
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_i8(
         store_codes(static_cast<Int8*>(c.k) + at * dim, d0, dim, kx);
         store_codes(static_cast<Int8*>(c.v) + at * dim, d0, dim, vx);
         if (d0 == 0) {
-            const int64_t place = scale_of(c, row, page, h);
+            const int64_t place = scale_of(c, row, off, h);
             c.k_scales[place] = ks;
             c.v_scales[place] = vs;
         }
@@ -247,8 +247,8 @@ __global__ __launch_bounds__(kAppendThreads) void cache_read(
         first = cu[s];
         if (t < first || t >= cu[s + 1]) return;
     }
-    int64_t page = 0;
-    const int64_t row = pool_row(c, s, int64_t(starts[s]) + (t - first), page);
+    uint32_t off = 0;
+    const int64_t row = pool_row(c, s, int64_t(starts[s]) + (t - first), off);
     const int n = int(c.kv_heads * c.dim);
     const T* const from_k = static_cast<const T*>(c.k) + row * n;
     const T* const from_v = static_cast<const T*>(c.v) + row * n;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kAppendThreads) void cache_read(
                 y[0] = widen(from_v[e]);
             }
             if constexpr (kScaled) {
-                const int64_t place = scale_of(c, row, page, int(uint32_t(e) / uint32_t(c.dim)));
+                const int64_t place = scale_of(c, row, off, int(uint32_t(e) / uint32_t(c.dim)));
                 const float ks = c.k_scales[place], vs = c.v_scales[place];
 #pragma unroll
                 for (int j = 0; j < N; ++j) {

@@ -22,24 +22,30 @@ struct Cache {
     const int32_t* table;
     int64_t ld_table, width, sequences;
     float *k_scales, *v_scales;  // (pages, kv_heads, page_size) of a cache in 8 bits
+    int page_shift;              // where the page size is 2 to it, else -1
 };
 
-// The row of position p of sequence s in the pools and its page, or -1 where the table does not
-// hold it or names a page outside the pool. 0 <= s < sequences.
-__device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p, int64_t& page) {
+// The row of position p of sequence s in the pools and its place in the page, or -1 where the table
+// does not hold it or names a page outside the pool. 0 <= s < sequences. A position, a pool's rows
+// and a page's are below 2^31: in 32 bits the division takes a tenth of the steps.
+__device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p, uint32_t& off) {
     if (p < 0 || p > INT32_MAX || p >= c.width * c.page_size) return -1;
-    const uint32_t at = uint32_t(p) / uint32_t(c.page_size);  // in 32 bits: a tenth of the steps
-    page = c.table[s * c.ld_table + at];
+    const uint32_t size = uint32_t(c.page_size);
+    const uint32_t at = c.page_shift >= 0 ? uint32_t(p) >> c.page_shift : uint32_t(p) / size;
+    const int64_t page = c.table[s * c.ld_table + at];
     if (page < 0 || page >= c.pages) return -1;
-    return page * c.page_size + (p - int64_t(at) * c.page_size);
+    off = uint32_t(p) - at * size;
+    return int64_t(uint64_t(uint32_t(page)) * size + off);
 }
 __device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p) {
-    int64_t page;
-    return pool_row(c, s, p, page);
+    uint32_t off;
+    return pool_row(c, s, p, off);
 }
-// Where the scale of a row's key head is.
-__device__ __forceinline__ int64_t scale_of(const Cache& c, int64_t row, int64_t page, int head) {
-    return row + (page * (c.kv_heads - 1) + head) * c.page_size;
+// Where the scale of a row's key head is: (page kv_heads + head) page_size + off.
+__device__ __forceinline__ int64_t scale_of(const Cache& c, int64_t row, uint32_t off, int head) {
+    const uint32_t heads = uint32_t(c.kv_heads);  // below 2^24
+    return int64_t(uint64_t(uint32_t(row)) * heads - uint64_t(off) * (heads - 1)) +
+           int64_t(head) * c.page_size;
 }
 
 // log of a sum whose terms are 2^-24 of their value relative to 2^top; ln 2 in two parts, whose
@@ -547,9 +553,9 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int k
     // The pool row of position p0 + lane, the last again past the end, and where its scales are.
     int64_t place = 0;
     const auto row_of = [&](int p0) {
-        int64_t page = 0;
-        const int64_t row = pool_row(a.c, s, min(p0 + lane, end - 1), page);
-        if constexpr (sizeof(T) == 1) place = scale_of(a.c, row, page, kv);
+        uint32_t off = 0;
+        const int64_t row = pool_row(a.c, s, min(p0 + lane, end - 1), off);
+        if constexpr (sizeof(T) == 1) place = scale_of(a.c, row, off, kv);
         return int(row);
     };
     const auto score = [&](int row) {
@@ -750,7 +756,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
 
         const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
         const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
-        const int64_t pitch = int64_t(kv_heads) * dim;
+        const uint32_t pitch = uint32_t(kv_heads * dim);  // below 2^31, as the rows
         Piece<T, N, WIDE> kx[2][KP], vx[kReads];
         float k_scale = 0.0f, v_scale = 0.0f;  // of the tile's position lane % 32
         const int v_lane = lane / LANES, v_d0 = lane % LANES * N;
@@ -760,15 +766,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
         int64_t place = 0;
         const auto find = [&](int p0) {
             const int p = p0 + (lane & 31);
-            int64_t row = 0, page = 0;
+            int64_t row = 0;
+            uint32_t off = 0;
             if (p < end) {
-                row = pool_row(a.c, s, p, page);
+                row = pool_row(a.c, s, p, off);
                 if (row < 0) {
                     bad = true;
-                    row = page = 0;
+                    row = off = 0;
                 }
             }
-            if constexpr (kScaled) place = scale_of(a.c, row, page, kv);
+            if constexpr (kScaled) place = scale_of(a.c, row, off, kv);
             r = int(row);
         };
         const auto load = [&](int p0) {
@@ -779,7 +786,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const T* at = k + int64_t(__shfl(r, 16 * t + col)) * pitch;
+                const T* at = k + uint64_t(uint32_t(__shfl(r, 16 * t + col))) * pitch;
 #pragma unroll
                 for (int p = 0; p < KP; ++p)
                     kx[t][p].load(at, 4 * N * p + N * quarter, dim);
@@ -787,7 +794,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
 #pragma unroll
             for (int i = 0; i < kReads; ++i) {
                 const int j = i * kRows + v_lane;
-                const T* at = v + int64_t(__shfl(r, j < kTilePositions ? j : 0)) * pitch;
+                const T* at = v + uint64_t(uint32_t(__shfl(r, j < kTilePositions ? j : 0))) * pitch;
                 vx[i].load(at, v_d0, dim);
             }
         };
@@ -803,7 +810,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
 #pragma unroll
                 for (int e = 0; e < N / 8; ++e) {
                     uintx4 y = vx[i].bf16(e, v_d0, dim);
-                    if (tail && p0 + j >= end) y = uintx4{0, 0, 0, 0};  // nothing, whatever is there
+                    // Nothing, whatever is there; in 8 bits its scale is 0.
+                    if (!kScaled && tail && p0 + j >= end) y = uintx4{0, 0, 0, 0};
                     if (v_lane < kRows && j < kTilePositions)
                         *reinterpret_cast<uintx4*>(mine + j * kPitch + 2 * v_d0 + 16 * e) = y;
                 }
@@ -824,24 +832,30 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
                     v_by[t] = *reinterpret_cast<const floatx4*>(&sh_scales[wave][1][at]);
                 }
             }
-            floatx4 sc[2];
+            // The smaller parts' products and the first parts' apart, four chains of them: the
+            // matrix instruction drops the low bits of its sums, least where they are small.
+            floatx4 sc[2], small[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                sc[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < 2; ++t) sc[t] = small[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int part = 2; part >= 0; --part)
+            for (int ks = 0; ks < KS; ++ks) {
+                const int d0 = 4 * N * (8 * ks / N) + N * quarter;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        // Past the row's end q is 0 and K something else, which has to be finite.
-                        const int d0 = 4 * N * (8 * ks / N) + N * quarter;
-                        bf16x8 f = __builtin_bit_cast(
-                            bf16x8, kx[t][8 * ks / N].bf16(ks % (N / 8), d0, dim));
-                        if (!kScaled && DP != dim && 32 * ks + 8 * quarter >= dim)
-                            f = __builtin_bit_cast(bf16x8, uintx4{0, 0, 0, 0});
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][part], sc[t], 0,
-                                                                        0, 0);
-                    }
+                for (int t = 0; t < 2; ++t) {
+                    // Past the row's end q is 0 and K something else, which has to be finite.
+                    bf16x8 f = __builtin_bit_cast(
+                        bf16x8, kx[t][8 * ks / N].bf16(ks % (N / 8), d0, dim));
+                    if (!kScaled && DP != dim && 32 * ks + 8 * quarter >= dim)
+                        f = __builtin_bit_cast(bf16x8, uintx4{0, 0, 0, 0});
+                    small[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][2], small[t], 0, 0,
+                                                                       0);
+                    small[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][1], small[t], 0, 0,
+                                                                       0);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[ks][0], sc[t], 0, 0, 0);
+                }
             }
+#pragma unroll
+            for (int t = 0; t < 2; ++t) sc[t] += small[t];
             if (p0 + kTilePositions < end) {
                 load(p0 + kTilePositions);
                 find(p0 + 2 * kTilePositions);
@@ -986,7 +1000,9 @@ inline int check(const char* name, const ehip_cache_t* c, Cache& out) {
         (c->pages > 0 && (c->k_pages == nullptr || c->v_pages == nullptr)))
         return fail(EHIP_EINVAL, "%s: null pool or table", name);
     out = Cache{c->k_pages,  c->v_pages,     c->pages,     c->page_size, c->kv_heads, c->head_dim,
-                c->table,    c->ld_table,    c->table_width, c->sequences, nullptr,     nullptr};
+                c->table,    c->ld_table,    c->table_width, c->sequences, nullptr,     nullptr, -1};
+    if ((c->page_size & (c->page_size - 1)) == 0)
+        out.page_shift = __builtin_ctzll(uint64_t(c->page_size));
     if (c->type == EHIP_CACHE_I8) {
         if (c->head_dim > kMaxDim)
             return fail(EHIP_EINVAL, "%s: heads of %lld values in 8 bits", name,
