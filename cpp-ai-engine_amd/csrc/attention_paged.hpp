@@ -25,17 +25,29 @@ struct Cache {
     int page_shift;              // where the page size is 2 to it, else -1
 };
 
-// The row of position p of sequence s in the pools and its place in the page, or -1 where the table
-// does not hold it or names a page outside the pool. 0 <= s < sequences. A position, a pool's rows
-// and a page's are below 2^31: in 32 bits the division takes a tenth of the steps.
+// A position's table entry, and its place in the page: the read, and what is made of it.
+struct Entry {
+    int32_t page;
+    uint32_t off;
+};
+// Of position p of sequence s, both in range. A position, a pool's rows and a page's are below 2^31:
+// in 32 bits the division takes a tenth of the steps.
+__device__ __forceinline__ Entry entry_of(const Cache& c, int64_t s, uint32_t p) {
+    const uint32_t size = uint32_t(c.page_size);
+    const uint32_t at = c.page_shift >= 0 ? p >> c.page_shift : p / size;
+    return Entry{c.table[s * c.ld_table + at], p - at * size};
+}
+// The pools' row, or -1 where the entry names no page of theirs.
+__device__ __forceinline__ int64_t row_of_entry(const Cache& c, const Entry& e) {
+    if (e.page < 0 || e.page >= c.pages) return -1;
+    return int64_t(uint64_t(uint32_t(e.page)) * uint32_t(c.page_size) + e.off);
+}
+// Of any position, -1 too where the table does not hold it.
 __device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p, uint32_t& off) {
     if (p < 0 || p > INT32_MAX || p >= c.width * c.page_size) return -1;
-    const uint32_t size = uint32_t(c.page_size);
-    const uint32_t at = c.page_shift >= 0 ? uint32_t(p) >> c.page_shift : uint32_t(p) / size;
-    const int64_t page = c.table[s * c.ld_table + at];
-    if (page < 0 || page >= c.pages) return -1;
-    off = uint32_t(p) - at * size;
-    return int64_t(uint64_t(uint32_t(page)) * size + off);
+    const Entry e = entry_of(c, s, uint32_t(p));
+    off = e.off;
+    return row_of_entry(c, e);
 }
 __device__ __forceinline__ int64_t pool_row(const Cache& c, int64_t s, int64_t p) {
     uint32_t off;
@@ -110,7 +122,8 @@ struct Paged {
     // A block has `rows` of the group's rows, its sequences' query heads of the key head.
     const int32_t *group_cu, *shared;
     int groups, rows;
-    int places;          // parts of a key head, `rows` rows each, in the layout (kv_heads, places)
+    int places;          // parts of a key head, key_waves times `rows` rows each
+    int key_waves;
 };
 
 // The work is cut evenly, whatever the lengths: the positions of all sequences in tiles, one after
@@ -132,43 +145,57 @@ __device__ __forceinline__ int tiles_of(const Paged& a, int n) {
     return n > 0 ? int(uint32_t(n - 1) / uint32_t(a.tile)) + 1 : 0;
 }
 
-// Positions of a sequence that are its own.
+// The first of a sequence's positions that are its own.
 __device__ __forceinline__ int start_of(const Paged& a, int64_t s) {
     return a.starts != nullptr ? a.starts[s] : 0;
-}
-__device__ __forceinline__ int own_of(const Paged& a, int64_t s) {
-    return length_of(a, s) - start_of(a, s);
 }
 
 // A group's first sequence; the offsets ascend and are in range, and a group shares nothing that
 // its table row could not have: shared_plan has seen to it.
 __device__ __forceinline__ int group_begin(const Paged& a, int g) { return a.group_cu[g]; }
 __device__ __forceinline__ int shared_of(const Paged& a, int g) { return a.shared[g]; }
-__device__ __forceinline__ int row_tiles(const Paged& a, int g) {
-    const int group = a.heads / int(a.c.kv_heads);
-    const int64_t rows = int64_t(group_begin(a, g + 1) - group_begin(a, g)) * group;
-    return int((rows + a.rows - 1) / a.rows);
-}
 // Place of the first row tile of a group: every group before it has at most as many as that.
 __device__ __forceinline__ int row_tile_base(const Paged& a, int g) {
     const int group = a.heads / int(a.c.kv_heads);
     return int(int64_t(group_begin(a, g)) * group / a.rows) + g;
 }
 
-// What the tiles are counted over: the sequences, or with SHARED the groups, each row tile of which
-// passes all of the group's positions.
+// What the tiles are counted over, 64 at a time in the lanes of a wave: the sequences, or with SHARED
+// the groups, each row tile of which passes all of the group's positions.
+struct Items {
+    int base;        // of lane 0
+    int start, end;  // positions
+    int first;       // the sequence whose table row it goes by
+    int rows;        // with SHARED the group's
+};
+// Tiles of a sequence or row tile, and row tiles, of a lane.
+__device__ __forceinline__ int tiles_of(const Paged& a, const Items& x) {
+    return tiles_of(a, x.end - x.start);
+}
+template <bool SHARED>
+__device__ __forceinline__ int row_tiles_of(const Paged& a, int rows) {
+    return SHARED ? (rows + a.rows - 1) / a.rows : 1;
+}
 template <bool SHARED>
 __device__ __forceinline__ int items(const Paged& a) {
     return SHARED ? a.groups : int(a.c.sequences);
 }
 template <bool SHARED>
-__device__ __forceinline__ int unit_tiles(const Paged& a, int i) {
-    return tiles_of(a, SHARED ? shared_of(a, i) : own_of(a, i));
-}
-template <bool SHARED>
-__device__ __forceinline__ int item_tiles(const Paged& a, int i) {
-    const int n = unit_tiles<SHARED>(a, i);
-    return SHARED && n > 0 ? n * row_tiles(a, i) : n;
+__device__ __forceinline__ Items items_from(const Paged& a, int base) {
+    const int i = base + (int(threadIdx.x) & 63);
+    Items x{base, 0, 0, i, 0};
+    if (i < items<SHARED>(a)) {
+        if (SHARED) {
+            const int group = a.heads / int(a.c.kv_heads);
+            x.first = group_begin(a, i);
+            x.rows = (group_begin(a, i + 1) - x.first) * group;  // at most 2^24
+            x.end = shared_of(a, i);
+        } else {
+            x.start = start_of(a, i);
+            x.end = length_of(a, i);
+        }
+    }
+    return x;
 }
 
 // The first tile of worker w of so many tiles, and the worker of tile t. With fewer tiles than
@@ -185,8 +212,11 @@ struct Segment {
     int64_t s;       // the sequence whose table row it goes by
     int item;        // the sequence, or the group
     int row_tile;    // of the group
+    int rows;        // of the group
     int n;           // tiles of the sequence, or of the group's positions
-    int begin, end;  // positions
+    int row_tiles;   // of the group
+    int from, to;    // all of the positions
+    int begin, end;  // the segment's
     int t, t_end;    // the worker's tiles from here on
     int t0;          // the sequence's or the row tile's first
     bool whole;      // the sequence is this segment
@@ -202,54 +232,61 @@ __device__ __forceinline__ int wave_scan(int x) {  // inclusive
     return x;
 }
 
-// Sequence and positions of a segment from its first tile g.t, item, row tile, n and t0 given.
+// The segment's positions from its item, row tile, t and t0.
 template <bool SHARED>
 __device__ __forceinline__ void measure(const Paged& a, Segment& g) {
     const int stop = min(g.t_end, g.t0 + g.n);
-    const int start = SHARED ? 0 : start_of(a, g.item);
-    const int end = SHARED ? shared_of(a, g.item) : length_of(a, g.item);
-    g.s = SHARED ? group_begin(a, g.item) : g.item;
-    g.begin = start + (g.t - g.t0) * a.tile;
-    g.end = stop - g.t0 == g.n ? end : start + (stop - g.t0) * a.tile;
-    g.whole = !SHARED && g.begin == 0 && g.end == end;
+    g.begin = g.from + (g.t - g.t0) * a.tile;
+    g.end = stop - g.t0 == g.n ? g.to : g.from + (stop - g.t0) * a.tile;
+    g.whole = !SHARED && g.begin == 0 && g.end == g.to;
 }
 
-// The first segment of worker w (t == t_end: none). Every wave finds the same; block 0 leaves the
-// items' first tiles for the join.
+// Takes the item of a lane.
 template <bool SHARED>
-__device__ __forceinline__ Segment first_segment(const Paged& a, int w) {
+__device__ __forceinline__ void take(const Paged& a, const Items& x, int lane, Segment& g) {
+    const auto of = [&](int y) { return __builtin_amdgcn_readlane(y, lane); };
+    g.item = x.base + lane;
+    g.s = SHARED ? of(x.first) : g.item;
+    g.rows = SHARED ? of(x.rows) : 0;
+    g.row_tiles = row_tiles_of<SHARED>(a, g.rows);
+    g.from = SHARED ? 0 : of(x.start);
+    g.to = of(x.end);
+    g.n = tiles_of(a, g.to - g.from);
+}
+
+// The first segment of worker w (t == t_end: none), and the items that it is among. Every wave finds
+// the same; block 0 leaves the items' first tiles for the join.
+template <bool SHARED>
+__device__ __forceinline__ Segment first_segment(const Paged& a, int w, Items& x) {
     const int lane = int(threadIdx.x) & 63;
     const int count = items<SHARED>(a);
     int tiles = 0;
     for (int base = 0; base < count; base += 64) {
-        const int s = base + lane;
-        const int mine = s < count ? item_tiles<SHARED>(a, s) : 0;
-        const int upto = wave_scan(mine);
-        if (blockIdx.x == 0 && threadIdx.x < 64 && s < count) a.first[s] = tiles + upto - mine;
+        x = items_from<SHARED>(a, base);
+        const int mine = tiles_of(a, x) * row_tiles_of<SHARED>(a, x.rows), upto = wave_scan(mine);
+        if (blockIdx.x == 0 && threadIdx.x < 64 && base + lane < count)
+            a.first[base + lane] = tiles + upto - mine;
         tiles += __shfl(upto, 63);
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) a.first[count] = tiles;
     Segment g{};
-    g.t = first_tile(a, w, tiles);
-    g.t_end = first_tile(a, w + 1, tiles);
+    g.t = __builtin_amdgcn_readfirstlane(first_tile(a, w, tiles));
+    g.t_end = __builtin_amdgcn_readfirstlane(first_tile(a, w + 1, tiles));
     if (g.t == g.t_end) return g;
     int before = 0;
     for (int base = 0; base < count; base += 64) {
-        const int s = base + lane;
-        const int mine = s < count ? item_tiles<SHARED>(a, s) : 0;
-        const int upto = before + wave_scan(mine);
+        if (count > 64) x = items_from<SHARED>(a, base);
+        const int mine = tiles_of(a, x) * row_tiles_of<SHARED>(a, x.rows), upto = before + wave_scan(mine);
         const uint64_t past = __ballot(upto > g.t);
         if (past != 0) {
             const int at = __builtin_ctzll(past);
-            g.item = base + at;
-            g.t0 = __shfl(upto - mine, at);
+            take<SHARED>(a, x, at, g);
+            g.t0 = __builtin_amdgcn_readlane(upto - mine, at);
             break;
         }
-        before = __shfl(upto, 63);
+        before = __builtin_amdgcn_readlane(upto, 63);
     }
-    g.item = __builtin_amdgcn_readfirstlane(g.item);
-    g.t0 = __builtin_amdgcn_readfirstlane(g.t0);
-    g.n = max(1, unit_tiles<SHARED>(a, g.item));  // 0 only where lengths change under the launch
+    g.n = max(1, g.n);  // 0 only where lengths change under the launch
     if (SHARED) {
         g.row_tile = (g.t - g.t0) / g.n;
         g.t0 += g.row_tile * g.n;
@@ -259,23 +296,32 @@ __device__ __forceinline__ Segment first_segment(const Paged& a, int w) {
 }
 
 template <bool SHARED>
-__device__ __forceinline__ void next_segment(const Paged& a, Segment& g) {
+__device__ __forceinline__ void next_segment(const Paged& a, Segment& g, Items& x) {
     const int stop = g.t0 + g.n;
     g.t = min(g.t_end, stop);
     if (g.t == g.t_end) return;
     g.t0 = stop;
-    if (SHARED && g.row_tile + 1 < row_tiles(a, g.item)) {
+    if (SHARED && g.row_tile + 1 < g.row_tiles) {
         ++g.row_tile;
-    } else {
-        g.row_tile = 0;
-        do {
-            if (++g.item >= items<SHARED>(a)) {  // only where the lengths changed under the launch
-                g.t = g.t_end;
-                return;
-            }
-            g.n = unit_tiles<SHARED>(a, g.item);
-        } while (g.n == 0);
+        measure<SHARED>(a, g);
+        return;
     }
+    g.row_tile = 0;
+    int lane = g.item - x.base + 1;  // 64 at most
+    while (true) {
+        const uint64_t some = lane < 64 ? __ballot(x.end > x.start && (!SHARED || x.rows > 0)) >> lane : 0;
+        if (some != 0) {
+            lane += __builtin_ctzll(some);
+            break;
+        }
+        if (x.base + 64 >= items<SHARED>(a)) {  // only where the lengths changed under the launch
+            g.t = g.t_end;
+            return;
+        }
+        x = items_from<SHARED>(a, x.base + 64);
+        lane = 0;
+    }
+    take<SHARED>(a, x, lane, g);
     measure<SHARED>(a, g);
 }
 
@@ -283,10 +329,7 @@ __device__ __forceinline__ void next_segment(const Paged& a, Segment& g) {
 // of one of its sequences.
 template <bool SHARED>
 __device__ __forceinline__ int rows_of(const Paged& a, const Segment& g, int count) {
-    if (!SHARED) return count;
-    const int group = a.heads / int(a.c.kv_heads);
-    const int rows = (group_begin(a, g.item + 1) - int(g.s)) * group;
-    return min(a.rows, rows - g.row_tile * a.rows);
+    return SHARED ? min(a.rows, g.rows - g.row_tile * a.rows) : count;
 }
 template <bool SHARED>
 __device__ __forceinline__ const float* query_row(const Paged& a, const Segment& g, int kv, int h0,
@@ -377,8 +420,9 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
     const int heads = min(G, (kv + 1) * group - h0);  // the block's
     x /= uint32_t(pieces);
     const int worker = int(x);
-    for (Segment seg = first_segment<SHARED>(a, worker); seg.t < seg.t_end;
-         next_segment<SHARED>(a, seg)) {
+    Items among;
+    for (Segment seg = first_segment<SHARED>(a, worker, among); seg.t < seg.t_end;
+         next_segment<SHARED>(a, seg, among)) {
         const int64_t s = seg.s;
         const int count = rows_of<SHARED>(a, seg, heads);
         const int begin = seg.begin, end = seg.end;
@@ -561,6 +605,10 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int k
     const auto score = [&](int row) {
         const T* at = k + int64_t(row) * pitch;
         float dot = 0.0f;
+        if constexpr (sizeof(T) == 4) {
+            for (int e = 0; e < dim; ++e) dot = __builtin_fmaf(q[e] * c2, at[e], dot);
+            return dot;
+        }
         if constexpr (sizeof(T) == 1) {
             const float ks = a.c.k_scales[place];
             for (int e = 0; e < dim; ++e)
@@ -724,8 +772,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
     x /= uint32_t(pieces);
     const int worker = int(x);
     if (worker >= a.workers) return;  // no barrier follows
-    for (Segment seg = first_segment<SHARED>(a, worker); seg.t < seg.t_end;
-         next_segment<SHARED>(a, seg)) {
+    Items among;
+    for (Segment seg = first_segment<SHARED>(a, worker, among); seg.t < seg.t_end;
+         next_segment<SHARED>(a, seg, among)) {
         const int64_t s = seg.s;
         const int count = rows_of<SHARED>(a, seg, heads);
         const int begin = seg.begin, end = seg.end;
@@ -733,22 +782,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
 
         const int col = lane & 15, quarter = lane / 16;
         const float c2 = a.scale * 1.44269504088896340736f;
-        bf16x8 q[KS][3];
-        {
-            const float* row = query_row<SHARED>(a, seg, kv, h0, col < count ? col : 0);
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int d0 = 4 * N * (8 * ks / N) + N * quarter + 8 * ks % N;
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    // In bf16 a head is a multiple of eight values.
-                    const bool in = d0 + (kScaled ? e : 0) < dim;
-                    y[e] = in && col < count ? row[in ? d0 + e : 0] * c2 : 0.0f;
-                }
-                attention::split8(y, q[ks]);
-            }
-        }
         floatx4 o[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -760,22 +793,23 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
         Piece<T, N, WIDE> kx[2][KP], vx[kReads];
         float k_scale = 0.0f, v_scale = 0.0f;  // of the tile's position lane % 32
         const int v_lane = lane / LANES, v_d0 = lane % LANES * N;
-        // The pool row of position p0 + lane % 32 and where its scales are: found a tile before
-        // the reads of the rows, which would else wait for the table.
+        // The table's entry of position p0 + lane % 32, or the last, is asked for a tile before its
+        // row is read, and last of the tile's reads: what is made of it waits for those before it
+        // too. So would a choice that stands between the read and its use.
+        Entry entry;
         int r = 0;
         int64_t place = 0;
-        const auto find = [&](int p0) {
-            const int p = p0 + (lane & 31);
-            int64_t row = 0;
-            uint32_t off = 0;
-            if (p < end) {
-                row = pool_row(a.c, s, p, off);
-                if (row < 0) {
-                    bad = true;
-                    row = off = 0;
-                }
+        const auto ask = [&](int p0) {
+            entry = entry_of(a.c, s, uint32_t(min(p0 + (lane & 31), end - 1)));
+        };
+        const auto find = [&] {
+            int64_t row = row_of_entry(a.c, entry);
+            if (row < 0) {
+                bad = true;
+                row = 0;
+                entry.off = 0;
             }
-            if constexpr (kScaled) place = scale_of(a.c, row, off, kv);
+            if constexpr (kScaled) place = scale_of(a.c, row, entry.off, kv);
             r = int(row);
         };
         const auto load = [&](int p0) {
@@ -799,9 +833,47 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             }
         };
         char* const mine = lds[wave];
-        find(begin);
+        // q is asked for between the table and the rows that it names, and split while those are on
+        // their way; of wide heads in bf16, where that spills, before the table.
+        constexpr bool kFirst = !kScaled && DP > 64;
+        float qx[KS][8];
+        bf16x8 q[KS][3];
+        const auto ask_query = [&] {
+            const float* const row = query_row<SHARED>(a, seg, kv, h0, col < count ? col : 0);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int d0 = 4 * N * (8 * ks / N) + N * quarter + 8 * ks % N;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    // With WIDE a head is a multiple of eight values.
+                    const bool in = d0 + (WIDE ? 0 : e) < dim;
+                    qx[ks][e] = row[in ? d0 + e : 0];
+                }
+            }
+        };
+        const auto split_query = [&] {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int d0 = 4 * N * (8 * ks / N) + N * quarter + 8 * ks % N;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const bool in = d0 + (WIDE ? 0 : e) < dim;
+                    qx[ks][e] = in && col < count ? qx[ks][e] * c2 : 0.0f;
+                }
+                attention::split8(qx[ks], q[ks]);
+            }
+        };
+        if (kFirst) {
+            ask_query();
+            split_query();
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        ask(begin);
+        if (!kFirst) ask_query();
+        find();
         load(begin);
-        find(begin + kTilePositions);
+        ask(begin + kTilePositions);
+        if (!kFirst) split_query();
         for (int p0 = begin; p0 < end; p0 += kTilePositions) {
             const bool tail = p0 + kTilePositions > end;
 #pragma unroll
@@ -816,7 +888,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
                         *reinterpret_cast<uintx4*>(mine + j * kPitch + 2 * v_d0 + 16 * e) = y;
                 }
             }
-            floatx4 k_by[2], v_by[2];  // the scales of a lane's scores
             if constexpr (kScaled) {
                 if (lane < kTilePositions) {
                     sh_scales[wave][0][lane] = k_scale;
@@ -825,13 +896,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
                 __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    const int at = 16 * t + 4 * quarter;
-                    k_by[t] = *reinterpret_cast<const floatx4*>(&sh_scales[wave][0][at]);
-                    v_by[t] = *reinterpret_cast<const floatx4*>(&sh_scales[wave][1][at]);
-                }
             }
+            const auto scales = [&](int which, int t) {  // of a lane's scores
+                return *reinterpret_cast<const floatx4*>(
+                    &sh_scales[wave][which][16 * t + 4 * quarter]);
+            };
             // The smaller parts' products and the first parts' apart, four chains of them: the
             // matrix instruction drops the low bits of its sums, least where they are small.
             floatx4 sc[2], small[2];
@@ -856,15 +925,14 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             }
 #pragma unroll
             for (int t = 0; t < 2; ++t) sc[t] += small[t];
-            if (p0 + kTilePositions < end) {
-                load(p0 + kTilePositions);
-                find(p0 + 2 * kTilePositions);
-            }
+            // Past the end the last row again: on a condition the table's entry would be copied, and
+            // waited for, where the paths meet.
+            find();
+            load(p0 + kTilePositions);
+            ask(p0 + 2 * kTilePositions);
             if constexpr (kScaled) {
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) sc[t][r] *= k_by[t][r];
+                for (int t = 0; t < 2; ++t) sc[t] *= scales(0, t);
             }
             if (tail) {
 #pragma unroll
@@ -892,7 +960,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             l = __builtin_fmaf(l, keep, part_sum);
             if constexpr (kScaled) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] *= v_by[j / 4][j % 4];
+                for (int t = 0; t < 2; ++t) {
+                    const floatx4 by = scales(1, t);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) w[4 * t + r] *= by[r];
+                }
             }
             bf16x8 p[3];
             attention::split8(w, p);
@@ -946,9 +1018,9 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
                 floatx4u y;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) y[r] = seg.whole ? o[i][r] / l : o[i][r];
-                if (d + 4 <= dim) {
+                if (d + (WIDE ? 0 : 3) < dim) {
                     *reinterpret_cast<floatx4u*>(to + d) = y;
-                } else {
+                } else if (!WIDE) {
 #pragma unroll
                     for (int r = 0; r < 3; ++r)
                         if (d + r < dim) to[d + r] = y[r];

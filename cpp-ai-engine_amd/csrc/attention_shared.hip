@@ -4,12 +4,379 @@
 // the parts of both joined.
 
 #include "attention_paged.hpp"
+#include <cstdlib>
 
 namespace ehip {
 
 using namespace paged;
 
 namespace {
+
+using attention::bf16x8;
+using attention::floatx4u;
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+// ---------------------------------------------------------------- many rows
+
+// A thread's values of a row that is staged, in up to three bf16 parts of eight each.
+template <class T, int DP, bool WIDE>
+struct Staged {  // bf16 and 8 bits, exact in one part
+    static constexpr int kParts = 1;
+    static constexpr int N = sizeof(T) == 1 && DP > 64 ? 16 : 8;
+    Piece<T, N, WIDE> x;
+    __device__ __forceinline__ void load(const T* row, int d0, int dim) { x.load(row, d0, dim); }
+    // in: a position that is there; others are nothing, whatever was read.
+    __device__ __forceinline__ void parts(int i, int d0, int dim, bool in, bf16x8 (&p)[1]) const {
+        uintx4 y = x.bf16(i, d0, dim);
+        if (sizeof(T) == 2 && (!in || d0 + 8 * i >= dim)) y = uintx4{0, 0, 0, 0};
+        p[0] = __builtin_bit_cast(bf16x8, y);
+    }
+};
+template <int DP, bool WIDE>
+struct Staged<float, DP, WIDE> {
+    static constexpr int kParts = 3;
+    static constexpr int N = 8;
+    float x[8];
+    __device__ __forceinline__ void load(const float* row, int d0, int dim) {
+#pragma unroll
+        for (int g = 0; g < 8; g += 4) {
+            const int d = d0 + g;
+            if (WIDE) {
+                const floatx4u y = *reinterpret_cast<const floatx4u*>(row + (d < dim ? d : 0));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[g + e] = y[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[g + e] = row[d + e < dim ? d + e : 0];
+            }
+        }
+    }
+    __device__ __forceinline__ void parts(int, int d0, int dim, bool in, bf16x8 (&p)[3]) const {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = in && d0 + e < dim ? x[e] : 0.0f;
+        attention::split8(y, p);
+    }
+};
+
+// d += the products of a block of K or V in its parts with one of q or the weights in three, but for
+// the first parts', which go into a sum of their own: the matrix instruction drops the low bits of
+// its sums, least where they are small.
+template <int PARTS>
+__device__ __forceinline__ void multiply_small(floatx4& d, const bf16x8 (&x)[PARTS],
+                                               const bf16x8 (&y)[3]) {
+    if constexpr (PARTS == 3) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i)
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[attention::kPart[i][0]],
+                                                        y[attention::kPart[i][1]], d, 0, 0, 0);
+    } else {
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[2], d, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[1], d, 0, 0, 0);
+    }
+}
+
+// The shared positions of groups with many rows: a block takes 64 / KW of them, 16 a wave in its
+// registers as in paged_part_mfma, and stages 32 KW positions at a time for all in LDS, of which a
+// wave passes 32 with its rows. So the cache is read, and made bf16, once for 64 / KW rows in place
+// of 16. K lies in blocks of 16 positions by 32 values as the instruction takes them, 1 KiB, the
+// positions' places permuted by the values' so that neighbouring threads write to different banks;
+// V in rows as there.
+template <class T, int DP, int KW, bool WIDE>
+__global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
+    using Unit = Staged<T, DP, WIDE>;
+    constexpr bool kScaled = sizeof(T) == 1;
+    constexpr int kParts = Unit::kParts, N = Unit::N;
+    constexpr int kKeys = 32 * KW, KS = DP / 32, NV = DP / 16;
+    constexpr int kPieces = DP / N, kUnits = kKeys * kPieces / kPagedThreads;
+    constexpr int kBuffers = kParts == 1 ? 2 : 1;
+    constexpr int kPitch = 2 * DP + 32;  // of V
+    constexpr int kKeyPlane = kKeys * DP * 2, kValuePlane = kKeys * kPitch;
+    constexpr int kTile = kParts * (kKeyPlane + kValuePlane);
+    static_assert(kKeys * kPieces % kPagedThreads == 0, "whole units");
+    __shared__ __attribute__((aligned(16))) char lds[kBuffers][kTile];
+    __shared__ __attribute__((aligned(16))) float sh_scales[kScaled ? kBuffers : 1][2][kKeys];
+    __shared__ uint32_t sh_again[kPagedWaves];
+    const int lane = int(threadIdx.x) & 63, col = lane & 15, quarter = lane / 16;
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int rw = wave / KW, kw = wave % KW;
+    const int dim = int(a.c.dim), kv_heads = int(a.c.kv_heads);
+    const int kv = int(blockIdx.x % uint32_t(kv_heads));
+    const int worker = int(blockIdx.x / uint32_t(kv_heads));
+    const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
+    const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
+    const uint32_t pitch = uint32_t(kv_heads * dim);
+    const float c2 = a.scale * 1.44269504088896340736f;
+    Items among;
+    for (Segment seg = first_segment<true>(a, worker, among); seg.t < seg.t_end;
+         next_segment<true>(a, seg, among)) {
+        const int64_t s = seg.s;
+        const int begin = seg.begin, end = seg.end;
+        const int count = rows_of<true>(a, seg, 0);
+        const int mine = 16 * rw + col;  // the lane's row
+        const bool some = 16 * rw < count;
+        bool bad = false;  // a page outside the pool
+
+        // The table's entries of the thread's units, asked for a step before their rows are read,
+        // past the end the last again.
+        Entry entry[kUnits], scale_entry;
+        uint32_t row[kUnits];
+        int64_t place = 0;
+        Unit kx[kUnits], vx[kUnits];
+        float scale = 0.0f;
+        const auto ask = [&](int p0) {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                const int j = (int(threadIdx.x) + u * kPagedThreads) / kPieces;
+                entry[u] = entry_of(a.c, s, uint32_t(min(p0 + j, end - 1)));
+            }
+            if constexpr (kScaled)
+                scale_entry = entry_of(
+                    a.c, s, uint32_t(min(p0 + int(threadIdx.x) % kKeys, end - 1)));
+        };
+        const auto find = [&] {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                int64_t r = row_of_entry(a.c, entry[u]);
+                if (r < 0) {
+                    bad = true;
+                    r = 0;
+                }
+                row[u] = uint32_t(r);
+            }
+            if constexpr (kScaled) {
+                int64_t r = row_of_entry(a.c, scale_entry);
+                if (r < 0) {
+                    r = 0;
+                    scale_entry.off = 0;
+                }
+                place = scale_of(a.c, r, scale_entry.off, kv);
+            }
+        };
+        const auto load = [&](int p0) {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                const int d0 = (int(threadIdx.x) + u * kPagedThreads) % kPieces * N;
+                kx[u].load(k + uint64_t(row[u]) * pitch, d0, dim);
+                vx[u].load(v + uint64_t(row[u]) * pitch, d0, dim);
+            }
+            if constexpr (kScaled) {
+                const float* const from = int(threadIdx.x) < kKeys ? a.c.k_scales : a.c.v_scales;
+                scale = p0 + int(threadIdx.x) % kKeys < end ? from[place] : 0.0f;
+            }
+        };
+        const auto store = [&](int p0, char* to, float (*scales)[kKeys]) {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) {
+                const int unit = int(threadIdx.x) + u * kPagedThreads;
+                const int j = unit / kPieces, d0 = unit % kPieces * N;
+                const bool in = p0 + j < end;
+#pragma unroll
+                for (int i = 0; i < N / 8; ++i) {
+                    const int g = d0 / 8 + i;
+                    char* const at = to + (j / 16 * KS + g / 4) * 1024 + (g % 4) * 256 +
+                                     ((j % 16) ^ (g % 16)) * 16;
+                    bf16x8 part[kParts];
+                    kx[u].parts(i, d0, dim, in, part);
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)
+                        *reinterpret_cast<bf16x8*>(at + p * kKeyPlane) = part[p];
+                    vx[u].parts(i, d0, dim, in, part);
+#pragma unroll
+                    for (int p = 0; p < kParts; ++p)
+                        *reinterpret_cast<bf16x8*>(to + kParts * kKeyPlane + p * kValuePlane +
+                                                   j * kPitch + 16 * g) = part[p];
+                }
+            }
+            if constexpr (kScaled)
+                if (int(threadIdx.x) < 2 * kKeys)
+                    scales[int(threadIdx.x) / kKeys][int(threadIdx.x) % kKeys] = scale;
+        };
+        ask(begin);
+        bf16x8 q[KS][3];
+        {
+            const float* const from = query_row<true>(a, seg, kv, 0, mine < count ? mine : 0);
+            float y[KS][8];
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = 32 * ks + 8 * quarter + e;
+                    y[ks][e] = from[d < dim ? d : 0];
+                }
+            find();
+            load(begin);
+            ask(begin + kKeys);
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int d = 32 * ks + 8 * quarter + e;
+                    y[ks][e] = d < dim && mine < count ? y[ks][e] * c2 : 0.0f;
+                }
+                attention::split8(y[ks], q[ks]);
+            }
+        }
+        floatx4 o[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        store(begin, lds[0], sh_scales[0]);
+        int buffer = 0;
+        __syncthreads();
+        for (int p0 = begin; p0 < end; p0 += kKeys) {
+            find();
+            load(p0 + kKeys);
+            ask(p0 + 2 * kKeys);
+            if (some) {
+                const char* const keys = lds[buffer] + 2 * kw * KS * 1024;
+                const char* const values =
+                    lds[buffer] + kParts * kKeyPlane + 32 * kw * kPitch;
+                const auto scales = [&](int which, int t) {  // of a lane's scores
+                    return *reinterpret_cast<const floatx4*>(
+                        &sh_scales[buffer][which][32 * kw + 16 * t + 4 * quarter]);
+                };
+                floatx4 sc[2], small[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) sc[t] = small[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const char* const at = keys + (t * KS + ks) * 1024 + quarter * 256 +
+                                               (col ^ (4 * ks + quarter) % 16) * 16;
+                        bf16x8 f[kParts];
+#pragma unroll
+                        for (int p = 0; p < kParts; ++p)
+                            f[p] = *reinterpret_cast<const bf16x8*>(at + p * kKeyPlane);
+                        multiply_small<kParts>(small[t], f, q[ks]);
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0], q[ks][0], sc[t], 0, 0,
+                                                                        0);
+                    }
+                const int at = p0 + 32 * kw;
+                float w[8], top = m;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    sc[t] += small[t];
+                    if constexpr (kScaled) sc[t] *= scales(0, t);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool in = at + 16 * t + 4 * quarter + r < end;
+                        w[4 * t + r] = in ? sc[t][r] : -INFINITY;
+                        top = fmaxf(top, w[4 * t + r]);
+                    }
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float shift = top == -INFINITY ? 0.0f : top;
+                const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
+                m = top;
+                float sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    w[j] = __builtin_amdgcn_exp2f(w[j] - shift) * 0x1p-24f;
+                    sum += w[j];
+                }
+                l = __builtin_fmaf(l, keep, sum);
+                if constexpr (kScaled) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const floatx4 by = scales(1, t);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) w[4 * t + r] *= by[r];
+                    }
+                }
+                bf16x8 p[3];
+                attention::split8(w, p);
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    typedef __attribute__((address_space(3))) shortx4* Rows;
+                    bf16x8 f[kParts];
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) {
+                        const char* const from = values + part * kValuePlane +
+                                                 (4 * quarter + col / 4) * kPitch + 32 * i +
+                                                 8 * (col % 4);
+                        struct {
+                            shortx4 x, y;
+                        } g = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)from),
+                               __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(from + 16 * kPitch))};
+                        f[part] = __builtin_bit_cast(bf16x8, g);
+                    }
+                    floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+                    multiply_small<kParts>(y, f, p);
+                    y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0], p[0], y, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[i][r] = __builtin_fmaf(o[i][r], keep, y[r]);
+                }
+            }
+            if (kBuffers == 1) __syncthreads();  // all have read
+            if (kBuffers > 1) buffer ^= 1;
+            store(p0 + kKeys, lds[buffer], sh_scales[kScaled ? buffer : 0]);
+            __syncthreads();
+        }
+        // The lane's row, values 16 i + 4 quarter + r; rows whose sums are not finite by the formula,
+        // by the row's first wave.
+        bad = __syncthreads_or(bad);
+        l = with_half(with_row_pair(l));
+        bool fine = l > 0.0f && l < INFINITY;
+        if constexpr (KW > 1)  // a wave that met no position
+            fine = fine || begin + 32 * kw >= end;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) fine = fine && fabsf(o[i][r]) < INFINITY;
+        const uint64_t lanes = __ballot(!fine && mine < count);
+        uint32_t again = uint32_t(lanes | lanes >> 32);
+        again = (again | again >> 16) & 0xffffu;
+        if constexpr (KW > 1) {
+            if (lane == 0) sh_again[wave] = again;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < KW; ++w) again |= sh_again[rw * KW + w];
+            __syncthreads();  // before the next segment's
+        }
+        again = __builtin_amdgcn_readfirstlane(bad ? 0u : again);
+        const int64_t part0 =
+            ((int64_t(kv) * a.places + worker + row_tile_base(a, seg.item) + seg.row_tile) * KW +
+             kw) * a.rows;
+        const bool formed = again >> col & 1;
+        if (mine < count && !(formed && kw == 0)) {
+            const int64_t at = part0 + mine;
+            if (quarter == 0)
+                a.part_stats[at] = formed ? float2{-INFINITY, 0.0f} : float2{m, bad ? NAN : l};
+            float* const to = a.part_out + at * dim;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int d = 16 * i + 4 * quarter;
+                floatx4u y;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) y[r] = formed ? 0.0f : o[i][r];
+                if (d + 4 <= dim) {
+                    *reinterpret_cast<floatx4u*>(to + d) = y;
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 3; ++r)
+                        if (d + r < dim) to[d + r] = y[r];
+                }
+            }
+        }
+        if (kw != 0) continue;
+        for (; again != 0; again &= again - 1) {
+            const int i = 16 * rw + __builtin_ctz(again);
+            float top, sum, y[2];
+            part_by_formula<T>(a, s, query_row<true>(a, seg, kv, 0, i), kv, begin, end, top, sum,
+                               y);
+            if (lane == 0) a.part_stats[part0 + i] = float2{top, sum};
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (lane + 64 * e < dim) a.part_out[(part0 + i) * dim + lane + 64 * e] = y[e];
+        }
+    }
+}
+
+// --------------------------------------------------------------------- join
 
 constexpr int kPlanThreads = 1024;
 
@@ -58,9 +425,9 @@ __global__ __launch_bounds__(256) void shared_join(Paged own, Paged a) {
         const int tile = row / a.rows, each = tiles_of(a, shared_of(a, lo));
         const int tiles = a.first[a.groups], t0 = a.first[lo] + tile * each;
         const int w0 = worker_of(a, t0, tiles);
-        shared_parts = worker_of(a, t0 + each - 1, tiles) - w0 + 1;
+        shared_parts = (worker_of(a, t0 + each - 1, tiles) - w0 + 1) * a.key_waves;
         const int place = w0 + row_tile_base(a, lo) + tile;
-        shared_from = (int64_t(kv) * a.places + place) * a.rows + row % a.rows;
+        shared_from = (int64_t(kv) * a.places + place) * a.key_waves * a.rows + row % a.rows;
     }
     const float2* const stats = own.part_stats + from;
     const float2* const shared_stats = a.part_stats + shared_from;
@@ -155,9 +522,16 @@ int check_groups(const char* name, const Cache& c, int64_t heads, int64_t groups
     return EHIP_OK;
 }
 
+// Waves of shared_rows that pass the same rows, by the rows of a group in the mean.
+int key_waves_of(const Cache& c, int type, int64_t rows) {
+    if (type == EHIP_CACHE_BF16 && !by_waves(c, type)) return 0;
+    if (getenv("KW")) return type == EHIP_CACHE_F32 ? std::min(1, atoi(getenv("KW"))) : atoi(getenv("KW"));
+    return rows >= 96 ? 1 : 0;
+}
+
 struct Plan {
     Cut own, shared;
-    int rows, places;
+    int rows, places, key_waves;  // key_waves: of shared_rows, or 0 for attention_paged's kernels
     size_t own_bytes, part_bytes, first_bytes, bytes;
 };
 
@@ -168,16 +542,20 @@ Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t g
     Plan p{};
     p.own = cut_of(c, heads, longest, type);
     const bool waves = p.own.waves;
-    p.rows = waves ? 16 : kMaxGroup;
-    const int64_t row_tiles = c.sequences * (heads / c.kv_heads) / p.rows + groups;
-    const int tile = tile_of(waves, row_tiles, longest_shared);
+    const int64_t rows = c.sequences * (heads / c.kv_heads);
+    p.key_waves = key_waves_of(c, type, groups > 0 ? rows / groups : 0);
+    p.rows = p.key_waves > 0 ? 64 / p.key_waves : waves ? 16 : kMaxGroup;
+    const int64_t row_tiles = rows / p.rows + groups;
+    const int tile =
+        p.key_waves > 0 ? kTile : tile_of(waves, row_tiles, longest_shared);
     const int64_t most = std::max<int64_t>(1, row_tiles * ceil_div(longest_shared, tile));
-    const int64_t resident = waves ? 2048 : 512;
+    const int64_t resident = waves && p.key_waves == 0 ? 2048 : 512;
     p.shared = Cut{waves, tile,
                    int(std::min(most, std::max<int64_t>(1, resident / c.kv_heads)))};
     p.places = int(p.shared.workers + row_tiles + 1);
     p.own_bytes = round16(part_bytes(c, heads, p.own.workers));
     p.part_bytes = round16(size_t(c.kv_heads) * size_t(p.places) * size_t(p.rows) *
+                           size_t(std::max(1, p.key_waves)) *
                            (sizeof(float2) + size_t(c.dim) * sizeof(float)));
     // The parts of both; the groups' first tiles, offsets and shared positions, and the sequences'
     // own starts.
@@ -229,6 +607,34 @@ int launch_shared(const Paged& a, int type, hipStream_t s) {
                                    : launch_lanes<Bf16, false>(a, s);
     return aligned && a.c.dim % 4 == 0 ? launch_lanes<float, true>(a, s)
                                        : launch_lanes<float, false>(a, s);
+}
+
+template <class T, int DP, int KW, bool WIDE>
+int launch_shared_rows(const Paged& a, hipStream_t s) {
+    EHIP_LAUNCH("attention_shared", (shared_rows<T, DP, KW, WIDE>),
+                dim3(unsigned(a.workers * a.c.kv_heads)), dim3(kPagedThreads), 0, s, a);
+    return EHIP_OK;
+}
+
+template <class T, int KW, bool WIDE>
+int launch_rows_of(const Paged& a, hipStream_t s) {
+    if (a.c.dim <= 64) return launch_shared_rows<T, 64, KW, WIDE>(a, s);
+    return launch_shared_rows<T, 128, KW, WIDE>(a, s);
+}
+
+int launch_rows(const Paged& a, int type, int key_waves, hipStream_t s) {
+    const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
+    if (type == EHIP_CACHE_F32)
+        return aligned && a.c.dim % 4 == 0 ? launch_rows_of<float, 1, true>(a, s)
+                                           : launch_rows_of<float, 1, false>(a, s);
+    if (type == EHIP_CACHE_BF16)
+        return key_waves == 1 ? launch_rows_of<Bf16, 1, true>(a, s)
+                              : launch_rows_of<Bf16, 2, true>(a, s);
+    if (aligned && a.c.dim % (a.c.dim <= 64 ? 8 : 16) == 0)
+        return key_waves == 1 ? launch_rows_of<Int8, 1, true>(a, s)
+                              : launch_rows_of<Int8, 2, true>(a, s);
+    return key_waves == 1 ? launch_rows_of<Int8, 1, false>(a, s)
+                          : launch_rows_of<Int8, 2, false>(a, s);
 }
 
 }  // namespace
@@ -295,7 +701,9 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     a.places = p.places;
     a.groups = int(groups);
     a.part_stats = reinterpret_cast<float2*>(at);
-    a.part_out = reinterpret_cast<float*>(a.part_stats + c.kv_heads * int64_t(p.places) * p.rows);
+    a.key_waves = std::max(1, p.key_waves);
+    a.part_out = reinterpret_cast<float*>(a.part_stats + c.kv_heads * int64_t(p.places) * p.rows *
+                                                             a.key_waves);
     at += p.part_bytes;
     a.first = reinterpret_cast<int*>(at);
     int* const cu = reinterpret_cast<int*>(at + p.first_bytes);
@@ -308,7 +716,9 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     EHIP_LAUNCH("attention_shared_plan", shared_plan, dim3(1), dim3(kPlanThreads), 0, s, a,
                 group_cu, shared, int(longest_shared), cu, counts, starts);
     if (groups > 0)
-        if (int rc = launch_shared(a, cache->type, s)) return rc;
+        if (int rc = p.key_waves > 0 ? launch_rows(a, cache->type, p.key_waves, s)
+                                     : launch_shared(a, cache->type, s))
+            return rc;
     if (int rc = launch_parts(own, cache->type, s)) return rc;
     EHIP_LAUNCH("attention_shared_join", shared_join, dim3(unsigned(c.sequences * heads)),
                 dim3(256), 0, s, own, a);
