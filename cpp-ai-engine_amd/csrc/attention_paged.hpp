@@ -366,6 +366,18 @@ __device__ __forceinline__ float with_half(float x) {  // lanes 32 apart
     return __builtin_bit_cast(float, x0) + __builtin_bit_cast(float, x1);
 }
 
+// The largest of the four lanes 16 apart, in each of them.
+__device__ __forceinline__ float largest_of_rows(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x),
+                                                    __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t x0 = r[0], x1 = r[1];
+    x = fmaxf(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1));
+    const auto h = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x),
+                                                    __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t y0 = h[0], y1 = h[1];
+    return fmaxf(__builtin_bit_cast(float, y0), __builtin_bit_cast(float, y1));
+}
+
 // The sum over the N lanes of a position (the low bits of the lane number), in each of them.
 template <int N>
 __device__ __forceinline__ float group_sum(float x) {
@@ -946,8 +958,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
+            top = largest_of_rows(top);
             const float shift = top == -INFINITY ? 0.0f : top;
             const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
             m = top;

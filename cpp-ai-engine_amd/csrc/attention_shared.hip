@@ -14,6 +14,7 @@ namespace {
 
 using attention::bf16x8;
 using attention::floatx4u;
+using attention::keep_order;
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 
@@ -60,20 +61,20 @@ struct Staged<float, DP, WIDE> {
     }
 };
 
-// d += the products of a block of K or V in its parts with one of q or the weights in three, but for
+// d0, d1 += the products of a block each of K or V in its parts with one of q or the weights in three, but for
 // the first parts', which go into a sum of their own: the matrix instruction drops the low bits of
 // its sums, least where they are small.
+// Two chains at a time, as a product waits for the one before.
 template <int PARTS>
-__device__ __forceinline__ void multiply_small(floatx4& d, const bf16x8 (&x)[PARTS],
-                                               const bf16x8 (&y)[3]) {
-    if constexpr (PARTS == 3) {
+__device__ __forceinline__ void multiply_small(floatx4& d0, const bf16x8 (&x0)[PARTS], floatx4& d1,
+                                               const bf16x8 (&x1)[PARTS], const bf16x8 (&y0)[3],
+                                               const bf16x8 (&y1)[3]) {
+    using attention::kPart;
 #pragma unroll
-        for (int i = 0; i < 5; ++i)
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[attention::kPart[i][0]],
-                                                        y[attention::kPart[i][1]], d, 0, 0, 0);
-    } else {
-        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[2], d, 0, 0, 0);
-        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[1], d, 0, 0, 0);
+    for (int i = 0; i < (PARTS == 3 ? 5 : 2); ++i) {
+        const int a = PARTS == 3 ? kPart[i][0] : 0, b = PARTS == 3 ? kPart[i][1] : 2 - i;
+        d0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x0[a], y0[b], d0, 0, 0, 0);
+        d1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x1[a], y1[b], d1, 0, 0, 0);
     }
 }
 
@@ -240,20 +241,32 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
                 floatx4 sc[2], small[2];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) sc[t] = small[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks)
+                // LDS is read a block ahead of the products.
+                bf16x8 f[2][2][kParts];
+                const auto ask_keys = [&](int ks) {
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         const char* const at = keys + (t * KS + ks) * 1024 + quarter * 256 +
                                                (col ^ (4 * ks + quarter) % 16) * 16;
-                        bf16x8 f[kParts];
 #pragma unroll
                         for (int p = 0; p < kParts; ++p)
-                            f[p] = *reinterpret_cast<const bf16x8*>(at + p * kKeyPlane);
-                        multiply_small<kParts>(small[t], f, q[ks]);
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0], q[ks][0], sc[t], 0, 0,
-                                                                        0);
+                            f[ks & 1][t][p] =
+                                *reinterpret_cast<const bf16x8*>(at + p * kKeyPlane);
                     }
+                };
+                ask_keys(0);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (ks + 1 < KS) ask_keys(ks + 1);
+                    keep_order();
+                    multiply_small<kParts>(small[0], f[ks & 1][0], small[1], f[ks & 1][1], q[ks],
+                                           q[ks]);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[ks & 1][t][0], q[ks][0],
+                                                                        sc[t], 0, 0, 0);
+                    keep_order();
+                }
                 const int at = p0 + 32 * kw;
                 float w[8], top = m;
 #pragma unroll
@@ -261,14 +274,16 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
                     sc[t] += small[t];
                     if constexpr (kScaled) sc[t] *= scales(0, t);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool in = at + 16 * t + 4 * quarter + r < end;
-                        w[4 * t + r] = in ? sc[t][r] : -INFINITY;
-                        top = fmaxf(top, w[4 * t + r]);
-                    }
+                    for (int r = 0; r < 4; ++r) w[4 * t + r] = sc[t][r];
                 }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
+                if (at + 32 > end) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (at + 16 * (j / 4) + 4 * quarter + j % 4 >= end) w[j] = -INFINITY;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, w[j]);
+                top = largest_of_rows(top);
                 const float shift = top == -INFINITY ? 0.0f : top;
                 const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
                 m = top;
@@ -289,26 +304,44 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
                 }
                 bf16x8 p[3];
                 attention::split8(w, p);
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
+                // Two blocks of 16 values at a time.
+                const auto ask_values = [&](int i) {
                     typedef __attribute__((address_space(3))) shortx4* Rows;
-                    bf16x8 f[kParts];
 #pragma unroll
-                    for (int part = 0; part < kParts; ++part) {
-                        const char* const from = values + part * kValuePlane +
-                                                 (4 * quarter + col / 4) * kPitch + 32 * i +
-                                                 8 * (col % 4);
-                        struct {
-                            shortx4 x, y;
-                        } g = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)from),
-                               __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(from + 16 * kPitch))};
-                        f[part] = __builtin_bit_cast(bf16x8, g);
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int part = 0; part < kParts; ++part) {
+                            const char* const from = values + part * kValuePlane +
+                                                     (4 * quarter + col / 4) * kPitch +
+                                                     32 * (i + t) + 8 * (col % 4);
+                            struct {
+                                shortx4 x, y;
+                            } g = {
+                                __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)from),
+                                __builtin_amdgcn_ds_read_tr16_b64_v4i16((Rows)(from + 16 * kPitch))};
+                            f[i / 2 & 1][t][part] = __builtin_bit_cast(bf16x8, g);
+                        }
+                };
+                ask_values(0);
+#pragma unroll
+                for (int i = 0; i < NV; i += 2) {
+                    if (i + 2 < NV) ask_values(i + 2);
+                    keep_order();
+                    auto& x = f[i / 2 & 1];
+                    floatx4 y[2];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) y[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                    multiply_small<kParts>(y[0], x[0], y[1], x[1], p, p);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        y[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[t][0], p[0], y[t], 0, 0, 0);
                     }
-                    floatx4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-                    multiply_small<kParts>(y, f, p);
-                    y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0], p[0], y, 0, 0, 0);
+                    keep_order();
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) o[i][r] = __builtin_fmaf(o[i][r], keep, y[r]);
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            o[i + t][r] = __builtin_fmaf(o[i + t][r], keep, y[t][r]);
                 }
             }
             if (kBuffers == 1) __syncthreads();  // all have read
