@@ -287,48 +287,22 @@ __global__ __launch_bounds__(kAppendThreads) void cache_read(
 }
 
 // The segments of a sequence and a head, where there are several, and the rows of sequences that
-// have no segment. Thread d % 128 has a value, two threads for alternate segments. Latency: 3 to 6
-// us.
-__global__ __launch_bounds__(256) void paged_join(Paged a) {
-    __shared__ float sh[2][kMaxDim], sh_l[2];
-    const int64_t at = blockIdx.x, s = at / a.heads;
-    const int h = int(at % a.heads), dim = int(a.c.dim);
-    const int d = int(threadIdx.x) % kMaxDim, half = int(threadIdx.x) / kMaxDim;
-    const int n = length_of(a, s);
+// have no segment.
+template <int WAVES>
+__global__ __launch_bounds__(kPagedThreads) void paged_join(Paged a) {
+    __shared__ float sh[WAVES][kMaxDim + 1];
+    const int64_t at =
+        int64_t(blockIdx.x) * (kPagedWaves / WAVES) + int(threadIdx.x) / (64 * WAVES);
+    if (at >= a.c.sequences * a.heads) return;
+    const int64_t s = at / a.heads;
+    const int h = int(at % a.heads), n = length_of(a, s);
     if (n <= 0) {
-        if (half == 0 && d < dim)
-            a.out[s * a.ld_out + int64_t(h) * dim + d] = n < 0 ? NAN : 0.0f;
-        if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at] = n < 0 ? NAN : -INFINITY;
+        empty_row<WAVES>(a, s, h, n);
         return;
     }
-    const int tiles = a.first[a.c.sequences];
-    const int w0 = worker_of(a, a.first[s], tiles);
-    const int parts = worker_of(a, a.first[s + 1] - 1, tiles) - w0 + 1;
-    if (parts == 1) return;  // the sequence was one segment
-    const int64_t from = int64_t(h) * (a.workers + a.c.sequences) + w0 + s;
-    const float2* stats = a.part_stats + from;
-    float top = -INFINITY;
-    for (int i = int(threadIdx.x) & 63; i < parts; i += 64) top = fmaxf(top, stats[i].x);
-#pragma unroll
-    for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
-    float sum = 0.0f, y = 0.0f;
-    const float* values = a.part_out + from * dim + (d < dim ? d : 0);
-#pragma unroll 8
-    for (int i = half; i < parts; i += 2) {
-        const float2 z = stats[i];
-        const float keep = z.x == -INFINITY ? (z.y != z.y ? NAN : 0.0f)
-                                            : __builtin_amdgcn_exp2f(z.x - top);
-        sum += z.y * keep;
-        y = __builtin_fmaf(values[int64_t(i) * dim], keep, y);
-    }
-    sh[half][d] = y;
-    if (d == 0) sh_l[half] = sum;
-    __syncthreads();
-    if (half != 0) return;
-    sum = sh_l[0] + sh_l[1];
-    y += sh[1][d];
-    if (d < dim) a.out[s * a.ld_out + int64_t(h) * dim + d] = y / sum;
-    if (d == 0 && a.lse != nullptr) a.lse[at] = lse_of(top, sum);
+    const Parts p[2] = {own_parts(a, s, h), Parts{nullptr, nullptr, 0, 1}};
+    if (p[0].count == 1) return;  // the sequence was one segment
+    join_parts<WAVES>(a, s, h, p, sh);
 }
 
 }  // namespace
@@ -582,8 +556,13 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     a.first = reinterpret_cast<int*>(a.part_out + parts * c.dim);
     hipStream_t s = as_stream(stream);
     if (int rc = launch_parts(a, cache->type, s)) return rc;
-    EHIP_LAUNCH("attention_paged_join", paged_join, dim3(unsigned(c.sequences * heads)), dim3(256),
-                0, s, a);
+    const int64_t rows = c.sequences * heads;
+    if (join_waves(rows) == 1)
+        EHIP_LAUNCH("attention_paged_join", paged_join<1>,
+                    dim3(unsigned(ceil_div(rows, kPagedWaves))), dim3(kPagedThreads), 0, s, a);
+    else
+        EHIP_LAUNCH("attention_paged_join", paged_join<kPagedWaves>, dim3(unsigned(rows)),
+                    dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 

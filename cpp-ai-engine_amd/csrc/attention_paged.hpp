@@ -205,7 +205,9 @@ __device__ __forceinline__ int first_tile(const Paged& a, int w, int tiles) {
     return w < workers ? int(int64_t(w) * tiles / workers) : tiles;
 }
 __device__ __forceinline__ int worker_of(const Paged& a, int t, int tiles) {
-    return int(((int64_t(t) + 1) * min(a.workers, tiles) - 1) / tiles);
+    // Both numbers are whole and below 2^53, so the quotient's rounding does not pass a whole one; in
+    // whole numbers the division takes several times the steps.
+    return int(double((int64_t(t) + 1) * min(a.workers, tiles) - 1) / double(tiles));
 }
 
 struct Segment {
@@ -1060,6 +1062,83 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
     }
 }
 
+// Parts of a row, `stride` rows apart.
+struct Parts {
+    const float2* stats;
+    const float* out;
+    int count;
+    int64_t stride;
+};
+
+// The sequence's own parts of a head (stats null: of none). One that is its only one is whole.
+__device__ __forceinline__ Parts own_parts(const Paged& a, int64_t s, int h) {
+    const int tiles = a.first[a.c.sequences], t0 = a.first[s], t1 = a.first[s + 1];
+    if (t0 == t1) return Parts{nullptr, nullptr, 0, 1};
+    const int w0 = worker_of(a, t0, tiles);
+    const int64_t from = int64_t(h) * (a.workers + a.c.sequences) + w0 + s;
+    return Parts{a.part_stats + from, a.part_out + from * a.c.dim,
+                 worker_of(a, t1 - 1, tiles) - w0 + 1, 1};
+}
+
+// Row (s, h) of the results from its parts, by WAVES waves that take them in turn: one where the
+// rows fill the card, as each finds the parts' places by itself (2752 rows of some eleven parts: 9
+// us against 17 with four). Lane d has values d and d + 64. Every thread calls it.
+template <int WAVES>
+__device__ __forceinline__ void join_parts(const Paged& a, int64_t s, int h, const Parts (&p)[2],
+                                           float (*sh)[kMaxDim + 1]) {
+    const int lane = int(threadIdx.x) & 63, wave = WAVES > 1 ? int(threadIdx.x) / 64 : 0;
+    const int dim = int(a.c.dim);
+    const int d0 = lane < dim ? lane : 0, d1 = lane + 64 < dim ? lane + 64 : 0;
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+        for (int i = lane; i < p[k].count; i += 64)
+            top = fmaxf(top, p[k].stats[i * p[k].stride].x);
+#pragma unroll
+    for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
+    float sum = 0.0f, y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll 4
+        for (int i = wave; i < p[k].count; i += WAVES) {
+            const float2 z = p[k].stats[i * p[k].stride];
+            const float* const from = p[k].out + i * p[k].stride * dim;
+            const float x0 = from[d0], x1 = from[d1];
+            const float keep = z.x == -INFINITY ? (z.y != z.y ? NAN : 0.0f)
+                                                : __builtin_amdgcn_exp2f(z.x - top);
+            sum += z.y * keep;
+            y0 = __builtin_fmaf(x0, keep, y0);
+            y1 = __builtin_fmaf(x1, keep, y1);
+        }
+    }
+    if (WAVES > 1) {
+        sh[wave][lane] = y0;
+        sh[wave][lane + 64] = y1;
+        if (lane == 0) sh[wave][kMaxDim] = sum;
+        __syncthreads();
+        if (wave != 0) return;
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) {
+            sum += sh[w][kMaxDim];
+            y0 += sh[w][lane];
+            y1 += sh[w][lane + 64];
+        }
+    }
+    float* const out = a.out + s * a.ld_out + int64_t(h) * dim;
+    if (lane < dim) out[lane] = y0 / sum;
+    if (lane + 64 < dim) out[lane + 64] = y1 / sum;
+    if (lane == 0 && a.lse != nullptr) a.lse[s * a.heads + h] = lse_of(top, sum);
+}
+
+// The row of a sequence without positions, or of a length that is none.
+template <int WAVES>
+__device__ __forceinline__ void empty_row(const Paged& a, int64_t s, int h, int n) {
+    const int t = int(threadIdx.x) % (64 * WAVES);
+    float* const out = a.out + s * a.ld_out + int64_t(h) * a.c.dim;
+    for (int d = t; d < int(a.c.dim); d += 64 * WAVES) out[d] = n < 0 ? NAN : 0.0f;
+    if (t == 0 && a.lse != nullptr) a.lse[s * a.heads + h] = n < 0 ? NAN : -INFINITY;
+}
+
 // ---------------------------------------------------------------- host checks
 
 constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
@@ -1135,6 +1214,9 @@ inline bool by_waves(const Cache& c, int type) {
 inline int tile_of(bool waves, int64_t rows, int64_t longest) {
     return waves && rows * ceil_div(longest, kWaveTile) <= INT32_MAX ? kWaveTile : kTile;
 }
+
+// Waves of a row that is joined.
+inline int join_waves(int64_t rows) { return rows >= 1024 ? 1 : kPagedWaves; }
 
 // The cut of the sequences' own positions, and the launch over them (attention_paged.hip).
 Cut cut_of(const Cache& c, int64_t heads, int64_t longest, int type);

@@ -424,75 +424,36 @@ __device__ __forceinline__ int group_of(const int* cu, int groups, int s) {
     return lo;
 }
 
-// Whole answers for rows without a shared part, joined ones for the others. Thread d % 128 has a
-// value, two threads for alternate parts.
-__global__ __launch_bounds__(256) void shared_join(Paged own, Paged a) {
-    __shared__ float sh[2][kMaxDim], sh_l[2];
-    const int64_t at = blockIdx.x, s = at / a.heads;
-    const int h = int(at % a.heads), dim = int(a.c.dim);
-    const int d = int(threadIdx.x) % kMaxDim, half = int(threadIdx.x) / kMaxDim;
-    const int n = length_of(own, s), start = start_of(own, s);
+// The parts of rows, of their own and of the group's positions, where the row is not one part of its
+// own.
+template <int WAVES>
+__global__ __launch_bounds__(kPagedThreads) void shared_join(Paged own, Paged a) {
+    __shared__ float sh[WAVES][kMaxDim + 1];
+    const int64_t at =
+        int64_t(blockIdx.x) * (kPagedWaves / WAVES) + int(threadIdx.x) / (64 * WAVES);
+    if (at >= a.c.sequences * a.heads) return;
+    const int64_t s = at / a.heads;
+    const int h = int(at % a.heads), n = length_of(own, s), start = start_of(own, s);
     if (n <= 0) {
-        if (half == 0 && d < dim)
-            a.out[s * a.ld_out + int64_t(h) * dim + d] = n < 0 ? NAN : 0.0f;
-        if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at] = n < 0 ? NAN : -INFINITY;
+        empty_row<WAVES>(a, s, h, n);
         return;
     }
-    // The parts of the sequence's own positions.
-    int parts = 0;
-    int64_t from = 0;
-    if (n > start) {
-        const int tiles = own.first[a.c.sequences];
-        const int w0 = worker_of(own, own.first[s], tiles);
-        parts = worker_of(own, own.first[s + 1] - 1, tiles) - w0 + 1;
-        if (start == 0 && parts == 1) return;  // the sequence was one segment
-        from = int64_t(h) * (own.workers + a.c.sequences) + w0 + s;
-    }
-    // Those of the group's.
-    int shared_parts = 0;
-    int64_t shared_from = 0;
+    Parts p[2] = {own_parts(own, s, h), Parts{nullptr, nullptr, 0, 1}};
+    if (start == 0 && p[0].count == 1) return;  // the sequence was one segment
     if (start > 0) {
-        const int lo = group_of(a.group_cu, a.groups, int(s));
+        const int g = group_of(a.group_cu, a.groups, int(s));
         const int group = a.heads / int(a.c.kv_heads), kv = h / group;
-        const int row = int(s - group_begin(a, lo)) * group + h % group;
-        const int tile = row / a.rows, each = tiles_of(a, shared_of(a, lo));
-        const int tiles = a.first[a.groups], t0 = a.first[lo] + tile * each;
+        const int row = int(s - group_begin(a, g)) * group + h % group;
+        const int tile = row / a.rows, each = tiles_of(a, shared_of(a, g));
+        const int tiles = a.first[a.groups], t0 = a.first[g] + tile * each;
         const int w0 = worker_of(a, t0, tiles);
-        shared_parts = (worker_of(a, t0 + each - 1, tiles) - w0 + 1) * a.key_waves;
-        const int place = w0 + row_tile_base(a, lo) + tile;
-        shared_from = (int64_t(kv) * a.places + place) * a.key_waves * a.rows + row % a.rows;
+        const int place = w0 + row_tile_base(a, g) + tile;
+        const int64_t from =
+            (int64_t(kv) * a.places + place) * a.key_waves * a.rows + row % a.rows;
+        p[1] = Parts{a.part_stats + from, a.part_out + from * a.c.dim,
+                     (worker_of(a, t0 + each - 1, tiles) - w0 + 1) * a.key_waves, a.rows};
     }
-    const float2* const stats = own.part_stats + from;
-    const float2* const shared_stats = a.part_stats + shared_from;
-    float top = -INFINITY;
-    for (int i = int(threadIdx.x) & 63; i < parts; i += 64) top = fmaxf(top, stats[i].x);
-    for (int i = int(threadIdx.x) & 63; i < shared_parts; i += 64)
-        top = fmaxf(top, shared_stats[int64_t(i) * a.rows].x);
-#pragma unroll
-    for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
-    float sum = 0.0f, y = 0.0f;
-    const auto add = [&](const float2& z, float value) {
-        const float keep = z.x == -INFINITY ? (z.y != z.y ? NAN : 0.0f)
-                                            : __builtin_amdgcn_exp2f(z.x - top);
-        sum += z.y * keep;
-        y = __builtin_fmaf(value, keep, y);
-    };
-    const int column = d < dim ? d : 0;
-#pragma unroll 8
-    for (int i = half; i < parts; i += 2)
-        add(stats[i], own.part_out[(from + i) * dim + column]);
-#pragma unroll 8
-    for (int i = half; i < shared_parts; i += 2)
-        add(shared_stats[int64_t(i) * a.rows],
-            a.part_out[(shared_from + int64_t(i) * a.rows) * dim + column]);
-    sh[half][d] = y;
-    if (d == 0) sh_l[half] = sum;
-    __syncthreads();
-    if (half != 0) return;
-    sum = sh_l[0] + sh_l[1];
-    y += sh[1][d];
-    if (d < dim) a.out[s * a.ld_out + int64_t(h) * dim + d] = y / sum;
-    if (d == 0 && a.lse != nullptr) a.lse[at] = lse_of(top, sum);
+    join_parts<WAVES>(a, s, h, p, sh);
 }
 
 // One block. The groups' offsets, in range and ascending whatever came in; what each shares, nothing
@@ -753,8 +714,14 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
                                      : launch_shared(a, cache->type, s))
             return rc;
     if (int rc = launch_parts(own, cache->type, s)) return rc;
-    EHIP_LAUNCH("attention_shared_join", shared_join, dim3(unsigned(c.sequences * heads)),
-                dim3(256), 0, s, own, a);
+    const int64_t rows = c.sequences * heads;
+    if (join_waves(rows) == 1)
+        EHIP_LAUNCH("attention_shared_join", shared_join<1>,
+                    dim3(unsigned(ceil_div(rows, kPagedWaves))), dim3(kPagedThreads), 0, s, own,
+                    a);
+    else
+        EHIP_LAUNCH("attention_shared_join", shared_join<kPagedWaves>, dim3(unsigned(rows)),
+                    dim3(kPagedThreads), 0, s, own, a);
     return EHIP_OK;
 }
 
