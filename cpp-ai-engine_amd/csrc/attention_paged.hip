@@ -428,7 +428,7 @@ template <class T, int DP, bool WIDE>
 int launch_part_mfma(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
     const int64_t blocks = ceil_div(a.workers * ceil_div(group, 16) * a.c.kv_heads, kPagedWaves);
-    EHIP_LAUNCH("attention_paged", (paged_part_mfma<T, DP, WIDE, false>), dim3(unsigned(blocks)),
+    EHIP_LAUNCH("attention_paged", (paged_part_mfma<T, DP, WIDE>), dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }

@@ -122,8 +122,7 @@ struct Paged {
     // A block has `rows` of the group's rows, its sequences' query heads of the key head.
     const int32_t *group_cu, *shared;
     int groups, rows;
-    int places;          // parts of a key head, key_waves times `rows` rows each
-    int key_waves;
+    int places;          // parts of a key head, `rows` rows each
 };
 
 // The work is cut evenly, whatever the lengths: the positions of all sequences in tiles, one after
@@ -259,18 +258,18 @@ __device__ __forceinline__ void take(const Paged& a, const Items& x, int lane, S
 // The first segment of worker w (t == t_end: none), and the items that it is among. Every wave finds
 // the same; block 0 leaves the items' first tiles for the join.
 template <bool SHARED>
-__device__ __forceinline__ Segment first_segment(const Paged& a, int w, Items& x) {
+__device__ __forceinline__ Segment first_segment(const Paged& a, uint32_t block, int w, Items& x) {
     const int lane = int(threadIdx.x) & 63;
     const int count = items<SHARED>(a);
     int tiles = 0;
     for (int base = 0; base < count; base += 64) {
         x = items_from<SHARED>(a, base);
         const int mine = tiles_of(a, x) * row_tiles_of<SHARED>(a, x.rows), upto = wave_scan(mine);
-        if (blockIdx.x == 0 && threadIdx.x < 64 && base + lane < count)
+        if (block == 0 && threadIdx.x < 64 && base + lane < count)
             a.first[base + lane] = tiles + upto - mine;
         tiles += __shfl(upto, 63);
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.first[count] = tiles;
+    if (block == 0 && threadIdx.x == 0) a.first[count] = tiles;
     Segment g{};
     g.t = __builtin_amdgcn_readfirstlane(first_tile(a, w, tiles));
     g.t_end = __builtin_amdgcn_readfirstlane(first_tile(a, w + 1, tiles));
@@ -435,7 +434,7 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
     x /= uint32_t(pieces);
     const int worker = int(x);
     Items among;
-    for (Segment seg = first_segment<SHARED>(a, worker, among); seg.t < seg.t_end;
+    for (Segment seg = first_segment<SHARED>(a, blockIdx.x, worker, among); seg.t < seg.t_end;
          next_segment<SHARED>(a, seg, among)) {
         const int64_t s = seg.s;
         const int count = rows_of<SHARED>(a, seg, heads);
@@ -758,8 +757,15 @@ struct Piece<Int8, N, WIDE> {
     }
 };
 
+constexpr int value_pitch(int dp) { return 2 * dp + 32; }  // bytes of a row of V in LDS
+template <int DP>
+struct alignas(16) PartLds {
+    char values[kPagedWaves][kTilePositions * value_pitch(DP)];
+    float scales[kPagedWaves][2][kTilePositions];
+};
+
 template <class T, int DP, bool WIDE, bool SHARED>
-__global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
+__device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, PartLds<DP>& lds) {
     constexpr bool kScaled = sizeof(T) == 1;
     using attention::bf16x8;
     using attention::floatx4u;
@@ -770,15 +776,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
     constexpr int LANES = DP / N;                              // of a row's reads
     constexpr int kRows = 64 / LANES, kReads = (kTilePositions + kRows - 1) / kRows;
     // Rows 32 bytes apart in banks: a transposed read's sixteen rows take all banks twice.
-    constexpr int kPitch = 2 * DP + 32;
-    __shared__ __attribute__((aligned(16))) char lds[kPagedWaves][kTilePositions * kPitch];
-    __shared__ __attribute__((aligned(16)))
-    float sh_scales[kScaled ? kPagedWaves : 1][2][kTilePositions];
+    constexpr int kPitch = value_pitch(DP);
     const int lane = int(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int kv_heads = int(a.c.kv_heads), dim = int(a.c.dim);
     const int group = a.heads / kv_heads, pieces = SHARED ? 1 : (group + 15) / 16;
-    uint32_t x = blockIdx.x * kPagedWaves + wave;
+    uint32_t x = block * kPagedWaves + wave;
     const int kv = int(x % uint32_t(kv_heads));
     x /= uint32_t(kv_heads);
     const int h0 = kv * group + int(x % uint32_t(pieces)) * 16;
@@ -787,7 +790,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
     const int worker = int(x);
     if (worker >= a.workers) return;  // no barrier follows
     Items among;
-    for (Segment seg = first_segment<SHARED>(a, worker, among); seg.t < seg.t_end;
+    for (Segment seg = first_segment<SHARED>(a, block, worker, among); seg.t < seg.t_end;
          next_segment<SHARED>(a, seg, among)) {
         const int64_t s = seg.s;
         const int count = rows_of<SHARED>(a, seg, heads);
@@ -846,7 +849,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
                 vx[i].load(at, v_d0, dim);
             }
         };
-        char* const mine = lds[wave];
+        char* const mine = lds.values[wave];
         // q is asked for between the table and the rows that it names, and split while those are on
         // their way; of wide heads in bf16, where that spills, before the table.
         constexpr bool kFirst = !kScaled && DP > 64;
@@ -904,8 +907,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             }
             if constexpr (kScaled) {
                 if (lane < kTilePositions) {
-                    sh_scales[wave][0][lane] = k_scale;
-                    sh_scales[wave][1][lane] = v_scale;
+                    lds.scales[wave][0][lane] = k_scale;
+                    lds.scales[wave][1][lane] = v_scale;
                 }
                 __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
                 __builtin_amdgcn_wave_barrier();
@@ -913,7 +916,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             }
             const auto scales = [&](int which, int t) {  // of a lane's scores
                 return *reinterpret_cast<const floatx4*>(
-                    &sh_scales[wave][which][16 * t + 4 * quarter]);
+                    &lds.scales[wave][which][16 * t + 4 * quarter]);
             };
             // The smaller parts' products and the first parts' apart, four chains of them: the
             // matrix instruction drops the low bits of its sums, least where they are small.
@@ -1060,6 +1063,12 @@ __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
             }
         }
     }
+}
+
+template <class T, int DP, bool WIDE>
+__global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
+    __shared__ PartLds<DP> lds;
+    part_by_waves<T, DP, WIDE, false>(a, blockIdx.x, lds);
 }
 
 // Parts of a row, `stride` rows apart.

@@ -78,45 +78,49 @@ __device__ __forceinline__ void multiply_small(floatx4& d0, const bf16x8 (&x0)[P
     }
 }
 
-// The shared positions of groups with many rows: a block takes 64 / KW of them, 16 a wave in its
-// registers as in paged_part_mfma, and stages 32 KW positions at a time for all in LDS, of which a
-// wave passes 32 with its rows. So the cache is read, and made bf16, once for 64 / KW rows in place
-// of 16. K lies in blocks of 16 positions by 32 values as the instruction takes them, 1 KiB, the
+// The shared positions of groups with many rows: a block takes 64 of them, 16 a wave in its registers
+// as in part_by_waves, and stages 32 positions at a time for all in LDS. So the cache is read, and
+// made bf16, once for 64 rows in place of 16. K lies in blocks of 16 positions by 32 values as the instruction takes them, 1 KiB, the
 // positions' places permuted by the values' so that neighbouring threads write to different banks;
 // V in rows as there.
-template <class T, int DP, int KW, bool WIDE>
-__global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
+constexpr int kKeys = 32;  // positions of a step
+
+template <class T, int DP>
+struct alignas(16) RowsLds {
+    static constexpr int kParts = Staged<T, DP, true>::kParts, kBuffers = kParts == 1 ? 2 : 1;
+    static constexpr int kKeyPlane = kKeys * DP * 2, kValuePlane = kKeys * value_pitch(DP);
+    char tile[kBuffers][kParts * (kKeyPlane + kValuePlane)];
+    float scales[kBuffers][2][kKeys];
+};
+
+template <class T, int DP, bool WIDE>
+__device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
+                                             RowsLds<T, DP>& lds) {
     using Unit = Staged<T, DP, WIDE>;
+    using Lds = RowsLds<T, DP>;
     constexpr bool kScaled = sizeof(T) == 1;
-    constexpr int kParts = Unit::kParts, N = Unit::N;
-    constexpr int kKeys = 32 * KW, KS = DP / 32, NV = DP / 16;
+    constexpr int kParts = Unit::kParts, N = Unit::N, KS = DP / 32, NV = DP / 16;
     constexpr int kPieces = DP / N, kUnits = kKeys * kPieces / kPagedThreads;
-    constexpr int kBuffers = kParts == 1 ? 2 : 1;
-    constexpr int kPitch = 2 * DP + 32;  // of V
-    constexpr int kKeyPlane = kKeys * DP * 2, kValuePlane = kKeys * kPitch;
-    constexpr int kTile = kParts * (kKeyPlane + kValuePlane);
+    constexpr int kBuffers = Lds::kBuffers, kPitch = value_pitch(DP);
+    constexpr int kKeyPlane = Lds::kKeyPlane, kValuePlane = Lds::kValuePlane;
     static_assert(kKeys * kPieces % kPagedThreads == 0, "whole units");
-    __shared__ __attribute__((aligned(16))) char lds[kBuffers][kTile];
-    __shared__ __attribute__((aligned(16))) float sh_scales[kScaled ? kBuffers : 1][2][kKeys];
-    __shared__ uint32_t sh_again[kPagedWaves];
     const int lane = int(threadIdx.x) & 63, col = lane & 15, quarter = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
-    const int rw = wave / KW, kw = wave % KW;
     const int dim = int(a.c.dim), kv_heads = int(a.c.kv_heads);
-    const int kv = int(blockIdx.x % uint32_t(kv_heads));
-    const int worker = int(blockIdx.x / uint32_t(kv_heads));
+    const int kv = int(block % uint32_t(kv_heads));
+    const int worker = int(block / uint32_t(kv_heads));
     const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
     const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
     const uint32_t pitch = uint32_t(kv_heads * dim);
     const float c2 = a.scale * 1.44269504088896340736f;
     Items among;
-    for (Segment seg = first_segment<true>(a, worker, among); seg.t < seg.t_end;
+    for (Segment seg = first_segment<true>(a, block, worker, among); seg.t < seg.t_end;
          next_segment<true>(a, seg, among)) {
         const int64_t s = seg.s;
         const int begin = seg.begin, end = seg.end;
         const int count = rows_of<true>(a, seg, 0);
-        const int mine = 16 * rw + col;  // the lane's row
-        const bool some = 16 * rw < count;
+        const int mine = 16 * wave + col;  // the lane's row
+        const bool some = 16 * wave < count;
         bool bad = false;  // a page outside the pool
 
         // The table's entries of the thread's units, asked for a step before their rows are read,
@@ -223,7 +227,7 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
-        store(begin, lds[0], sh_scales[0]);
+        store(begin, lds.tile[0], lds.scales[0]);
         int buffer = 0;
         __syncthreads();
         for (int p0 = begin; p0 < end; p0 += kKeys) {
@@ -231,12 +235,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
             load(p0 + kKeys);
             ask(p0 + 2 * kKeys);
             if (some) {
-                const char* const keys = lds[buffer] + 2 * kw * KS * 1024;
-                const char* const values =
-                    lds[buffer] + kParts * kKeyPlane + 32 * kw * kPitch;
+                const char* const keys = lds.tile[buffer];
+                const char* const values = keys + kParts * kKeyPlane;
                 const auto scales = [&](int which, int t) {  // of a lane's scores
                     return *reinterpret_cast<const floatx4*>(
-                        &sh_scales[buffer][which][32 * kw + 16 * t + 4 * quarter]);
+                        &lds.scales[buffer][which][16 * t + 4 * quarter]);
                 };
                 floatx4 sc[2], small[2];
 #pragma unroll
@@ -267,7 +270,6 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
                                                                         sc[t], 0, 0, 0);
                     keep_order();
                 }
-                const int at = p0 + 32 * kw;
                 float w[8], top = m;
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
@@ -276,10 +278,10 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) w[4 * t + r] = sc[t][r];
                 }
-                if (at + 32 > end) {
+                if (p0 + kKeys > end) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        if (at + 16 * (j / 4) + 4 * quarter + j % 4 >= end) w[j] = -INFINITY;
+                        if (p0 + 16 * (j / 4) + 4 * quarter + j % 4 >= end) w[j] = -INFINITY;
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) top = fmaxf(top, w[j]);
@@ -346,16 +348,13 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
             }
             if (kBuffers == 1) __syncthreads();  // all have read
             if (kBuffers > 1) buffer ^= 1;
-            store(p0 + kKeys, lds[buffer], sh_scales[kScaled ? buffer : 0]);
+            store(p0 + kKeys, lds.tile[buffer], lds.scales[buffer]);
             __syncthreads();
         }
-        // The lane's row, values 16 i + 4 quarter + r; rows whose sums are not finite by the formula,
-        // by the row's first wave.
+        // The lane's row, values 16 i + 4 quarter + r; rows whose sums are not finite by the formula.
         bad = __syncthreads_or(bad);
         l = with_half(with_row_pair(l));
         bool fine = l > 0.0f && l < INFINITY;
-        if constexpr (KW > 1)  // a wave that met no position
-            fine = fine || begin + 32 * kw >= end;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -363,29 +362,18 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
         const uint64_t lanes = __ballot(!fine && mine < count);
         uint32_t again = uint32_t(lanes | lanes >> 32);
         again = (again | again >> 16) & 0xffffu;
-        if constexpr (KW > 1) {
-            if (lane == 0) sh_again[wave] = again;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < KW; ++w) again |= sh_again[rw * KW + w];
-            __syncthreads();  // before the next segment's
-        }
         again = __builtin_amdgcn_readfirstlane(bad ? 0u : again);
-        const int64_t part0 =
-            ((int64_t(kv) * a.places + worker + row_tile_base(a, seg.item) + seg.row_tile) * KW +
-             kw) * a.rows;
-        const bool formed = again >> col & 1;
-        if (mine < count && !(formed && kw == 0)) {
+        const int64_t part0 = part_of<true>(a, seg, worker, kv, 0, 0);
+        if (mine < count && !(again >> col & 1)) {
             const int64_t at = part0 + mine;
-            if (quarter == 0)
-                a.part_stats[at] = formed ? float2{-INFINITY, 0.0f} : float2{m, bad ? NAN : l};
+            if (quarter == 0) a.part_stats[at] = float2{m, bad ? NAN : l};
             float* const to = a.part_out + at * dim;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int d = 16 * i + 4 * quarter;
                 floatx4u y;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = formed ? 0.0f : o[i][r];
+                for (int r = 0; r < 4; ++r) y[r] = o[i][r];
                 if (d + 4 <= dim) {
                     *reinterpret_cast<floatx4u*>(to + d) = y;
                 } else {
@@ -395,9 +383,8 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
                 }
             }
         }
-        if (kw != 0) continue;
         for (; again != 0; again &= again - 1) {
-            const int i = 16 * rw + __builtin_ctz(again);
+            const int i = 16 * wave + __builtin_ctz(again);
             float top, sum, y[2];
             part_by_formula<T>(a, s, query_row<true>(a, seg, kv, 0, i), kv, begin, end, top, sum,
                                y);
@@ -407,6 +394,30 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
                 if (lane + 64 * e < dim) a.part_out[(part0 + i) * dim + lane + 64 * e] = y[e];
         }
     }
+}
+
+// The shared positions' parts, after those of the sequences' own: one launch, whose blocks of the one
+// kind begin where blocks of the other end. ROWS: part_by_rows.
+template <class T, int DP, bool WIDE, bool ROWS>
+__global__ __launch_bounds__(kPagedThreads, 2) void shared_parts(Paged own, Paged a,
+                                                                 uint32_t own_blocks) {
+    __shared__ union Lds {
+        PartLds<DP> part;
+        RowsLds<T, DP> rows;
+    } lds;
+    if (blockIdx.x < own_blocks)
+        part_by_waves<T, DP, WIDE, false>(own, blockIdx.x, lds.part);
+    else if constexpr (ROWS)
+        part_by_rows<T, DP, WIDE>(a, blockIdx.x - own_blocks, lds.rows);
+    else
+        part_by_waves<T, DP, WIDE, true>(a, blockIdx.x - own_blocks, lds.part);
+}
+
+// In fp32 apart: the own positions go by the vector kernel.
+template <int DP, bool WIDE>
+__global__ __launch_bounds__(kPagedThreads, 2) void shared_rows_f32(Paged a) {
+    __shared__ RowsLds<float, DP> lds;
+    part_by_rows<float, DP, WIDE>(a, blockIdx.x, lds);
 }
 
 // --------------------------------------------------------------------- join
@@ -448,10 +459,9 @@ __global__ __launch_bounds__(kPagedThreads) void shared_join(Paged own, Paged a)
         const int tiles = a.first[a.groups], t0 = a.first[g] + tile * each;
         const int w0 = worker_of(a, t0, tiles);
         const int place = w0 + row_tile_base(a, g) + tile;
-        const int64_t from =
-            (int64_t(kv) * a.places + place) * a.key_waves * a.rows + row % a.rows;
+        const int64_t from = (int64_t(kv) * a.places + place) * a.rows + row % a.rows;
         p[1] = Parts{a.part_stats + from, a.part_out + from * a.c.dim,
-                     (worker_of(a, t0 + each - 1, tiles) - w0 + 1) * a.key_waves, a.rows};
+                     worker_of(a, t0 + each - 1, tiles) - w0 + 1, a.rows};
     }
     join_parts<WAVES>(a, s, h, p, sh);
 }
@@ -516,16 +526,21 @@ int check_groups(const char* name, const Cache& c, int64_t heads, int64_t groups
     return EHIP_OK;
 }
 
-// Waves of shared_rows that pass the same rows, by the rows of a group in the mean.
-int key_waves_of(const Cache& c, int type, int64_t rows) {
-    if (type == EHIP_CACHE_BF16 && !by_waves(c, type)) return 0;
-    if (getenv("KW")) return type == EHIP_CACHE_F32 ? std::min(1, atoi(getenv("KW"))) : atoi(getenv("KW"));
-    return rows >= 96 ? 1 : 0;
+enum Kind { kVectorParts, kWaveParts, kRowParts };
+
+// What passes the shared positions: by the rows of a group in the mean.
+Kind kind_of(const Cache& c, int type, int64_t rows) {
+    if (getenv("KW") && (type == EHIP_CACHE_F32 || by_waves(c, type)))
+        return atoi(getenv("KW")) ? kRowParts : by_waves(c, type) ? kWaveParts : kVectorParts;
+    if (type == EHIP_CACHE_F32) return kRowParts;
+    if (!by_waves(c, type)) return kVectorParts;
+    return rows > 16 ? kRowParts : kWaveParts;
 }
 
 struct Plan {
     Cut own, shared;
-    int rows, places, key_waves;  // key_waves: of shared_rows, or 0 for attention_paged's kernels
+    Kind kind;
+    int rows, places;
     size_t own_bytes, part_bytes, first_bytes, bytes;
 };
 
@@ -535,21 +550,19 @@ Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t g
              int64_t longest_shared) {
     Plan p{};
     p.own = cut_of(c, heads, longest, type);
-    const bool waves = p.own.waves;
     const int64_t rows = c.sequences * (heads / c.kv_heads);
-    p.key_waves = key_waves_of(c, type, groups > 0 ? rows / groups : 0);
-    p.rows = p.key_waves > 0 ? 64 / p.key_waves : waves ? 16 : kMaxGroup;
+    p.kind = kind_of(c, type, groups > 0 ? rows / groups : 0);
+    p.rows = p.kind == kRowParts ? 64 : p.kind == kWaveParts ? 16 : kMaxGroup;
     const int64_t row_tiles = rows / p.rows + groups;
-    const int tile =
-        p.key_waves > 0 ? kTile : tile_of(waves, row_tiles, longest_shared);
+    const bool waves = p.kind == kWaveParts;
+    const int tile = tile_of(waves, row_tiles, longest_shared);
     const int64_t most = std::max<int64_t>(1, row_tiles * ceil_div(longest_shared, tile));
-    const int64_t resident = waves && p.key_waves == 0 ? 2048 : 512;
+    const int64_t resident = waves ? 2048 : 512;
     p.shared = Cut{waves, tile,
                    int(std::min(most, std::max<int64_t>(1, resident / c.kv_heads)))};
     p.places = int(p.shared.workers + row_tiles + 1);
     p.own_bytes = round16(part_bytes(c, heads, p.own.workers));
     p.part_bytes = round16(size_t(c.kv_heads) * size_t(p.places) * size_t(p.rows) *
-                           size_t(std::max(1, p.key_waves)) *
                            (sizeof(float2) + size_t(c.dim) * sizeof(float)));
     // The parts of both; the groups' first tiles, offsets and shared positions, and the sequences'
     // own starts.
@@ -565,70 +578,59 @@ int launch_vector(const Paged& a, hipStream_t s) {
     return EHIP_OK;
 }
 
-template <class T, bool VEC>
-int launch_lanes(const Paged& a, hipStream_t s) {
-    constexpr int N = 16 / sizeof(T);
-    if (a.c.dim <= 32) return launch_vector<T, 32 / N, VEC>(a, s);
-    if (a.c.dim <= 64) return launch_vector<T, 64 / N, VEC>(a, s);
-    return launch_vector<T, 128 / N, VEC>(a, s);
-}
-
-template <class T, int DP, bool WIDE>
-int launch_part_mfma(const Paged& a, hipStream_t s) {
-    EHIP_LAUNCH("attention_shared", (paged_part_mfma<T, DP, WIDE, true>),
-                dim3(unsigned(ceil_div(a.workers * a.c.kv_heads, kPagedWaves))), dim3(kPagedThreads), 0, s, a);
-    return EHIP_OK;
-}
-
-template <class T, bool WIDE>
-int launch_mfma(const Paged& a, hipStream_t s) {
-    if (a.c.dim <= 32) return launch_part_mfma<T, 32, WIDE>(a, s);
-    if (a.c.dim <= 64) return launch_part_mfma<T, 64, WIDE>(a, s);
-    return launch_part_mfma<T, 128, WIDE>(a, s);
-}
-
-// Reads of whole pieces in 8 bits: of 16 values, or of 8 in heads of up to 32.
-int launch_parts_i8(const Paged& a, bool aligned, hipStream_t s) {
-    return aligned && a.c.dim % (a.c.dim <= 32 ? 8 : 16) == 0 ? launch_mfma<Int8, true>(a, s)
-                                                              : launch_mfma<Int8, false>(a, s);
-}
-
-int launch_shared(const Paged& a, int type, hipStream_t s) {
-    const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
-    if (type == EHIP_CACHE_I8) return launch_parts_i8(a, aligned, s);
-    if (type == EHIP_CACHE_BF16)
-        return by_waves(a.c, type) ? launch_mfma<Bf16, true>(a, s)
-                                   : launch_lanes<Bf16, false>(a, s);
-    return aligned && a.c.dim % 4 == 0 ? launch_lanes<float, true>(a, s)
-                                       : launch_lanes<float, false>(a, s);
-}
-
-template <class T, int DP, int KW, bool WIDE>
-int launch_shared_rows(const Paged& a, hipStream_t s) {
-    EHIP_LAUNCH("attention_shared", (shared_rows<T, DP, KW, WIDE>),
+template <int DP, bool WIDE>
+int launch_rows_f32(const Paged& a, hipStream_t s) {
+    EHIP_LAUNCH("attention_shared", (shared_rows_f32<DP, WIDE>),
                 dim3(unsigned(a.workers * a.c.kv_heads)), dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 
-template <class T, int KW, bool WIDE>
-int launch_rows_of(const Paged& a, hipStream_t s) {
-    if (a.c.dim <= 64) return launch_shared_rows<T, 64, KW, WIDE>(a, s);
-    return launch_shared_rows<T, 128, KW, WIDE>(a, s);
+// The vector kernel and fp32: the shared positions, then the own ones.
+int launch_apart(const Paged& own, const Paged& a, int type, hipStream_t s) {
+    int rc;
+    if (type == EHIP_CACHE_F32) {
+        const bool wide = aligned16(a.c.k) && aligned16(a.c.v) && a.c.dim % 4 == 0;
+        if (a.c.dim <= 64)
+            rc = wide ? launch_rows_f32<64, true>(a, s) : launch_rows_f32<64, false>(a, s);
+        else
+            rc = wide ? launch_rows_f32<128, true>(a, s) : launch_rows_f32<128, false>(a, s);
+    } else {
+        rc = a.c.dim <= 32   ? launch_vector<Bf16, 4, false>(a, s)
+             : a.c.dim <= 64 ? launch_vector<Bf16, 8, false>(a, s)
+                             : launch_vector<Bf16, 16, false>(a, s);
+    }
+    return rc != EHIP_OK ? rc : launch_parts(own, type, s);
 }
 
-int launch_rows(const Paged& a, int type, int key_waves, hipStream_t s) {
-    const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
-    if (type == EHIP_CACHE_F32)
-        return aligned && a.c.dim % 4 == 0 ? launch_rows_of<float, 1, true>(a, s)
-                                           : launch_rows_of<float, 1, false>(a, s);
-    if (type == EHIP_CACHE_BF16)
-        return key_waves == 1 ? launch_rows_of<Bf16, 1, true>(a, s)
-                              : launch_rows_of<Bf16, 2, true>(a, s);
-    if (aligned && a.c.dim % (a.c.dim <= 64 ? 8 : 16) == 0)
-        return key_waves == 1 ? launch_rows_of<Int8, 1, true>(a, s)
-                              : launch_rows_of<Int8, 2, true>(a, s);
-    return key_waves == 1 ? launch_rows_of<Int8, 1, false>(a, s)
-                          : launch_rows_of<Int8, 2, false>(a, s);
+template <class T, int DP, bool WIDE, bool ROWS>
+int launch_both(const Paged& own, const Paged& a, hipStream_t s) {
+    const int64_t group = a.heads / a.c.kv_heads;
+    const int64_t own_blocks =
+        ceil_div(own.workers * ceil_div(group, 16) * a.c.kv_heads, kPagedWaves);
+    const int64_t units = a.workers * a.c.kv_heads;
+    EHIP_LAUNCH("attention_shared", (shared_parts<T, DP, WIDE, ROWS>),
+                dim3(unsigned(own_blocks + (ROWS ? units : ceil_div(units, kPagedWaves)))),
+                dim3(kPagedThreads), 0, s, own, a, uint32_t(own_blocks));
+    return EHIP_OK;
+}
+
+template <class T, int DP, bool WIDE>
+int launch_kind(const Paged& own, const Paged& a, Kind kind, hipStream_t s) {
+    return kind == kRowParts ? launch_both<T, DP, WIDE, true>(own, a, s)
+                             : launch_both<T, DP, WIDE, false>(own, a, s);
+}
+
+template <class T, bool WIDE>
+int launch_dim(const Paged& own, const Paged& a, Kind kind, hipStream_t s) {
+    return a.c.dim <= 64 ? launch_kind<T, 64, WIDE>(own, a, kind, s)
+                         : launch_kind<T, 128, WIDE>(own, a, kind, s);
+}
+
+int launch_shared(const Paged& own, const Paged& a, int type, Kind kind, hipStream_t s) {
+    if (type == EHIP_CACHE_F32 || !by_waves(a.c, type)) return launch_apart(own, a, type, s);
+    if (type == EHIP_CACHE_BF16) return launch_dim<Bf16, true>(own, a, kind, s);
+    const bool wide = aligned16(a.c.k) && aligned16(a.c.v) && a.c.dim % 16 == 0;
+    return wide ? launch_dim<Int8, true>(own, a, kind, s) : launch_dim<Int8, false>(own, a, kind, s);
 }
 
 }  // namespace
@@ -695,9 +697,7 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     a.places = p.places;
     a.groups = int(groups);
     a.part_stats = reinterpret_cast<float2*>(at);
-    a.key_waves = std::max(1, p.key_waves);
-    a.part_out = reinterpret_cast<float*>(a.part_stats + c.kv_heads * int64_t(p.places) * p.rows *
-                                                             a.key_waves);
+    a.part_out = reinterpret_cast<float*>(a.part_stats + c.kv_heads * int64_t(p.places) * p.rows);
     at += p.part_bytes;
     a.first = reinterpret_cast<int*>(at);
     int* const cu = reinterpret_cast<int*>(at + p.first_bytes);
@@ -709,11 +709,11 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     hipStream_t s = as_stream(stream);
     EHIP_LAUNCH("attention_shared_plan", shared_plan, dim3(1), dim3(kPlanThreads), 0, s, a,
                 group_cu, shared, int(longest_shared), cu, counts, starts);
-    if (groups > 0)
-        if (int rc = p.key_waves > 0 ? launch_rows(a, cache->type, p.key_waves, s)
-                                     : launch_shared(a, cache->type, s))
-            return rc;
-    if (int rc = launch_parts(own, cache->type, s)) return rc;
+    if (groups > 0) {
+        if (int rc = launch_shared(own, a, cache->type, p.kind, s)) return rc;
+    } else {
+        if (int rc = launch_parts(own, cache->type, s)) return rc;
+    }
     const int64_t rows = c.sequences * heads;
     if (join_waves(rows) == 1)
         EHIP_LAUNCH("attention_shared_join", shared_join<1>,
