@@ -396,7 +396,7 @@ template <class T, int LPP, int G, bool VEC>
 int launch_part(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
     const int64_t blocks = a.workers * ceil_div(group, G) * a.c.kv_heads;
-    EHIP_LAUNCH("attention_paged", (paged_part<T, LPP, G, VEC, false>), dim3(unsigned(blocks)),
+    EHIP_LAUNCH("attention_paged", (paged_part<T, LPP, G, VEC>), dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }

@@ -419,25 +419,24 @@ struct Values {
     __device__ __forceinline__ float operator[](int e) const { return widen(x.v[e]); }
 };
 
-template <class T, int LPP, int G, bool VEC, bool SHARED>
+template <class T, int LPP, int G, bool VEC>
 __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void paged_part(Paged a) {
     constexpr int N = 16 / int(sizeof(T)), SUBS = 64 / LPP, TILE = SUBS * kUnroll;
     __shared__ float sh_m[kPagedWaves][G], sh_l[kPagedWaves][G], sh_o[kPagedWaves][G][LPP * N];
     const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) / 64;
     const int kv_heads = int(a.c.kv_heads), dim = int(a.c.dim);
-    const int group = a.heads / kv_heads, pieces = SHARED ? 1 : (group + G - 1) / G;
+    const int group = a.heads / kv_heads, pieces = (group + G - 1) / G;
     uint32_t x = blockIdx.x;
     const int kv = int(x % uint32_t(kv_heads));
     x /= uint32_t(kv_heads);
     const int h0 = kv * group + int(x % uint32_t(pieces)) * G;
-    const int heads = min(G, (kv + 1) * group - h0);  // the block's
+    const int count = min(G, (kv + 1) * group - h0);  // the block's heads
     x /= uint32_t(pieces);
     const int worker = int(x);
     Items among;
-    for (Segment seg = first_segment<SHARED>(a, blockIdx.x, worker, among); seg.t < seg.t_end;
-         next_segment<SHARED>(a, seg, among)) {
+    for (Segment seg = first_segment<false>(a, blockIdx.x, worker, among); seg.t < seg.t_end;
+         next_segment<false>(a, seg, among)) {
         const int64_t s = seg.s;
-        const int count = rows_of<SHARED>(a, seg, heads);
         const int begin = seg.begin, end = seg.end;
         bool bad = false;  // a page outside the pool
 
@@ -448,7 +447,7 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
         for (int g = 0; g < G; ++g) {
             m[g] = -INFINITY;
             l[g] = 0.0f;
-            const float* row = query_row<SHARED>(a, seg, kv, h0, g < count ? g : 0) + d0;
+            const float* row = query_row<false>(a, seg, kv, h0, g < count ? g : 0) + d0;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 q[g][e] = e < left ? row[e] * (a.scale < 0.0f ? -c2 : c2) : 0.0f;
@@ -572,7 +571,7 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
                 keep[w] = sh_m[w][g] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sh_m[w][g] - top);
                 sum += sh_l[w][g] * (sh_l[w][g] != sh_l[w][g] ? 1.0f : keep[w]);
             }
-            const int64_t at = part_of<SHARED>(a, seg, worker, kv, h0, g);
+            const int64_t at = part_of<false>(a, seg, worker, kv, h0, g);
             if (bad) sum = NAN;
             if (threadIdx.x == 0) {
                 if (!seg.whole) a.part_stats[at] = float2{top, sum};
@@ -592,8 +591,8 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
 
 // One head's share of a block by the formula, for those whose sums by parts are not finite: a part
 // of an infinity, or an infinity times the parts of a finite value, is NaN where the product is an
-// infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time,
-// of rows of 16-byte units; a score of NaN or +inf settles the head as NaN (64 sequences of 1024,
+// infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time; a
+// score of NaN or +inf settles the head as NaN (64 sequences of 1024,
 // 32 heads over 8 of 128 values, us: finite 56, the first key NaN 59, the first value infinite 560;
 // value by value and to the end 1870 either way).
 template <class T>
@@ -615,29 +614,37 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int k
         if constexpr (sizeof(T) == 1) place = scale_of(a.c, row, off, kv);
         return int(row);
     };
+    // Rows of 16-byte units, or others four values at a time at any address.
+    const bool units = sizeof(T) == 2 && dim % 8 == 0 && aligned16(a.c.k);
     const auto score = [&](int row) {
         const T* at = k + int64_t(row) * pitch;
+        const float by = sizeof(T) == 1 ? a.c.k_scales[place] : 1.0f;
         float dot = 0.0f;
-        if constexpr (sizeof(T) == 4) {
-            for (int e = 0; e < dim; ++e) dot = __builtin_fmaf(q[e] * c2, at[e], dot);
-            return dot;
-        }
-        if constexpr (sizeof(T) == 1) {
-            const float ks = a.c.k_scales[place];
-            for (int e = 0; e < dim; ++e)
-                dot = __builtin_fmaf(q[e] * c2, widen(at[e]) * ks, dot);
-            return dot;
-        }
-        for (int e = 0; e < dim; e += 8) {
-            const uintx4 x = *reinterpret_cast<const uintx4*>(at + e);
+        int e = 0;
+        if (sizeof(T) == 2 && units) {
+            for (; e < dim; e += 8) {
+                const uintx4 x = *reinterpret_cast<const uintx4*>(at + e);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t pair = x[j];
-                dot = __builtin_fmaf(q[e + 2 * j] * c2, __builtin_bit_cast(float, pair << 16), dot);
-                dot = __builtin_fmaf(q[e + 2 * j + 1] * c2,
-                                     __builtin_bit_cast(float, pair & 0xffff0000u), dot);
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t pair = x[j];
+                    dot = __builtin_fmaf(q[e + 2 * j] * c2, __builtin_bit_cast(float, pair << 16),
+                                         dot);
+                    dot = __builtin_fmaf(q[e + 2 * j + 1] * c2,
+                                         __builtin_bit_cast(float, pair & 0xffff0000u), dot);
+                }
             }
+            return dot;
         }
+        for (; e + 4 <= dim; e += 4) {
+            T x[4];
+            __builtin_memcpy(x, at + e, sizeof(x));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                dot = __builtin_fmaf(q[e + j] * c2, sizeof(T) == 1 ? widen(x[j]) * by : widen(x[j]),
+                                     dot);
+        }
+        for (; e < dim; ++e)
+            dot = __builtin_fmaf(q[e] * c2, sizeof(T) == 1 ? widen(at[e]) * by : widen(at[e]), dot);
         return dot;
     };
     top = -INFINITY;
@@ -660,6 +667,9 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int k
         const float weight = lane < count ? exp2f(score(row) - shift) * 0x1p-24f : 0.0f;
         const float vs = sizeof(T) == 1 ? a.c.v_scales[place] : 1.0f;
         sum += weight;
+        // A scale that is not finite settles the values, whatever its weight.
+        if (sizeof(T) == 1 && __any(!(fabsf(vs) < INFINITY))) o[0] = o[1] = NAN;
+        if (sizeof(T) == 1 && o[0] != o[0]) continue;
 #pragma unroll 8
         for (int u = 0; u < count; ++u) {
             const T* at = v + int64_t(__shfl(row, u)) * pitch;
@@ -704,12 +714,29 @@ template <class T, int N, bool WIDE>
 struct Piece;
 template <int N, bool WIDE>
 struct Piece<Bf16, N, WIDE> {
-    static_assert(N == 8 && WIDE, "what is read at a time");
+    static_assert(N == 8, "what is read at a time");
     uintx4 x;
     __device__ __forceinline__ void load(const Bf16* row, int d0, int dim) {
-        x = *reinterpret_cast<const uintx4*>(row + (d0 < dim ? d0 : 0));
+        if (WIDE) {
+            x = *reinterpret_cast<const uintx4*>(row + (d0 < dim ? d0 : 0));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const uint32_t lo = row[d0 + e < dim ? d0 + e : 0].bits;
+                const uint32_t hi = row[d0 + e + 1 < dim ? d0 + e + 1 : 0].bits;
+                x[e / 2] = lo | hi << 16;
+            }
+        }
     }
-    __device__ __forceinline__ uintx4 bf16(int, int, int) const { return x; }
+    // With WIDE anything past the row's end.
+    __device__ __forceinline__ uintx4 bf16(int, int d0, int dim) const {
+        if (WIDE) return x;
+        uintx4 y;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2)
+            y[e / 2] = d0 + e + 1 < dim ? x[e / 2] : d0 + e < dim ? x[e / 2] & 0xffffu : 0;
+        return y;
+    }
 };
 // Other rows in 8 bits, of any length and at any address, are read eight at a time, the last eight
 // where fewer are left. Those are shifted to their places where they are used: earlier, the read

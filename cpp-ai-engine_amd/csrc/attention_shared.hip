@@ -4,7 +4,6 @@
 // the parts of both joined.
 
 #include "attention_paged.hpp"
-#include <cstdlib>
 
 namespace ehip {
 
@@ -413,11 +412,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_parts(Paged own, Page
         part_by_waves<T, DP, WIDE, true>(a, blockIdx.x - own_blocks, lds.part);
 }
 
-// In fp32 apart: the own positions go by the vector kernel.
-template <int DP, bool WIDE>
-__global__ __launch_bounds__(kPagedThreads, 2) void shared_rows_f32(Paged a) {
-    __shared__ RowsLds<float, DP> lds;
-    part_by_rows<float, DP, WIDE>(a, blockIdx.x, lds);
+// Apart where the own positions go by the vector kernel.
+template <class T, int DP, bool WIDE>
+__global__ __launch_bounds__(kPagedThreads, 2) void shared_rows(Paged a) {
+    __shared__ RowsLds<T, DP> lds;
+    part_by_rows<T, DP, WIDE>(a, blockIdx.x, lds);
 }
 
 // --------------------------------------------------------------------- join
@@ -526,20 +525,15 @@ int check_groups(const char* name, const Cache& c, int64_t heads, int64_t groups
     return EHIP_OK;
 }
 
-enum Kind { kVectorParts, kWaveParts, kRowParts };
-
-// What passes the shared positions: by the rows of a group in the mean.
-Kind kind_of(const Cache& c, int type, int64_t rows) {
-    if (getenv("KW") && (type == EHIP_CACHE_F32 || by_waves(c, type)))
-        return atoi(getenv("KW")) ? kRowParts : by_waves(c, type) ? kWaveParts : kVectorParts;
-    if (type == EHIP_CACHE_F32) return kRowParts;
-    if (!by_waves(c, type)) return kVectorParts;
-    return rows > 16 ? kRowParts : kWaveParts;
-}
+// Whether part_by_rows passes the shared positions: else, of groups of up to 16 rows in the mean, do
+// waves of their own (8 groups of 4000 shared positions and 100 own ones, 32 heads over 8 of 128,
+// us, waves : rows, for 8, 16, 32 and 64 rows; 8 bits 44 : 53, 49 : 52, 60 : 63, 82 : 72; bf16 54 :
+// 55, 63 : 56, 75 : 68, 98 : 81).
+bool by_rows(const Cache& c, int type, int64_t rows) { return !by_waves(c, type) || rows > 16; }
 
 struct Plan {
     Cut own, shared;
-    Kind kind;
+    bool by_rows;
     int rows, places;
     size_t own_bytes, part_bytes, first_bytes, bytes;
 };
@@ -551,10 +545,10 @@ Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t g
     Plan p{};
     p.own = cut_of(c, heads, longest, type);
     const int64_t rows = c.sequences * (heads / c.kv_heads);
-    p.kind = kind_of(c, type, groups > 0 ? rows / groups : 0);
-    p.rows = p.kind == kRowParts ? 64 : p.kind == kWaveParts ? 16 : kMaxGroup;
+    p.by_rows = by_rows(c, type, groups > 0 ? rows / groups : 0);
+    p.rows = p.by_rows ? 64 : 16;
     const int64_t row_tiles = rows / p.rows + groups;
-    const bool waves = p.kind == kWaveParts;
+    const bool waves = !p.by_rows;
     const int tile = tile_of(waves, row_tiles, longest_shared);
     const int64_t most = std::max<int64_t>(1, row_tiles * ceil_div(longest_shared, tile));
     const int64_t resident = waves ? 2048 : 512;
@@ -571,34 +565,24 @@ Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t g
     return p;
 }
 
-template <class T, int LPP, bool VEC>
-int launch_vector(const Paged& a, hipStream_t s) {
-    EHIP_LAUNCH("attention_shared", (paged_part<T, LPP, kMaxGroup, VEC, true>),
+template <class T, int DP, bool WIDE>
+int launch_rows(const Paged& a, hipStream_t s) {
+    EHIP_LAUNCH("attention_shared", (shared_rows<T, DP, WIDE>),
                 dim3(unsigned(a.workers * a.c.kv_heads)), dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 
-template <int DP, bool WIDE>
-int launch_rows_f32(const Paged& a, hipStream_t s) {
-    EHIP_LAUNCH("attention_shared", (shared_rows_f32<DP, WIDE>),
-                dim3(unsigned(a.workers * a.c.kv_heads)), dim3(kPagedThreads), 0, s, a);
-    return EHIP_OK;
+template <class T, bool WIDE>
+int launch_rows_dim(const Paged& a, hipStream_t s) {
+    return a.c.dim <= 64 ? launch_rows<T, 64, WIDE>(a, s) : launch_rows<T, 128, WIDE>(a, s);
 }
 
-// The vector kernel and fp32: the shared positions, then the own ones.
+// Where the vector kernel takes the own positions: the shared ones before them.
 int launch_apart(const Paged& own, const Paged& a, int type, hipStream_t s) {
-    int rc;
-    if (type == EHIP_CACHE_F32) {
-        const bool wide = aligned16(a.c.k) && aligned16(a.c.v) && a.c.dim % 4 == 0;
-        if (a.c.dim <= 64)
-            rc = wide ? launch_rows_f32<64, true>(a, s) : launch_rows_f32<64, false>(a, s);
-        else
-            rc = wide ? launch_rows_f32<128, true>(a, s) : launch_rows_f32<128, false>(a, s);
-    } else {
-        rc = a.c.dim <= 32   ? launch_vector<Bf16, 4, false>(a, s)
-             : a.c.dim <= 64 ? launch_vector<Bf16, 8, false>(a, s)
-                             : launch_vector<Bf16, 16, false>(a, s);
-    }
+    const bool wide = aligned16(a.c.k) && aligned16(a.c.v) && a.c.dim % 4 == 0;
+    const int rc = type == EHIP_CACHE_BF16 ? launch_rows_dim<Bf16, false>(a, s)
+                   : wide                  ? launch_rows_dim<float, true>(a, s)
+                                           : launch_rows_dim<float, false>(a, s);
     return rc != EHIP_OK ? rc : launch_parts(own, type, s);
 }
 
@@ -615,22 +599,22 @@ int launch_both(const Paged& own, const Paged& a, hipStream_t s) {
 }
 
 template <class T, int DP, bool WIDE>
-int launch_kind(const Paged& own, const Paged& a, Kind kind, hipStream_t s) {
-    return kind == kRowParts ? launch_both<T, DP, WIDE, true>(own, a, s)
-                             : launch_both<T, DP, WIDE, false>(own, a, s);
+int launch_kind(const Paged& own, const Paged& a, bool rows, hipStream_t s) {
+    return rows ? launch_both<T, DP, WIDE, true>(own, a, s)
+                : launch_both<T, DP, WIDE, false>(own, a, s);
 }
 
 template <class T, bool WIDE>
-int launch_dim(const Paged& own, const Paged& a, Kind kind, hipStream_t s) {
-    return a.c.dim <= 64 ? launch_kind<T, 64, WIDE>(own, a, kind, s)
-                         : launch_kind<T, 128, WIDE>(own, a, kind, s);
+int launch_dim(const Paged& own, const Paged& a, bool rows, hipStream_t s) {
+    return a.c.dim <= 64 ? launch_kind<T, 64, WIDE>(own, a, rows, s)
+                         : launch_kind<T, 128, WIDE>(own, a, rows, s);
 }
 
-int launch_shared(const Paged& own, const Paged& a, int type, Kind kind, hipStream_t s) {
-    if (type == EHIP_CACHE_F32 || !by_waves(a.c, type)) return launch_apart(own, a, type, s);
-    if (type == EHIP_CACHE_BF16) return launch_dim<Bf16, true>(own, a, kind, s);
+int launch_shared(const Paged& own, const Paged& a, int type, bool rows, hipStream_t s) {
+    if (!by_waves(a.c, type)) return launch_apart(own, a, type, s);
+    if (type == EHIP_CACHE_BF16) return launch_dim<Bf16, true>(own, a, rows, s);
     const bool wide = aligned16(a.c.k) && aligned16(a.c.v) && a.c.dim % 16 == 0;
-    return wide ? launch_dim<Int8, true>(own, a, kind, s) : launch_dim<Int8, false>(own, a, kind, s);
+    return wide ? launch_dim<Int8, true>(own, a, rows, s) : launch_dim<Int8, false>(own, a, rows, s);
 }
 
 }  // namespace
@@ -710,7 +694,7 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     EHIP_LAUNCH("attention_shared_plan", shared_plan, dim3(1), dim3(kPlanThreads), 0, s, a,
                 group_cu, shared, int(longest_shared), cu, counts, starts);
     if (groups > 0) {
-        if (int rc = launch_shared(own, a, cache->type, p.kind, s)) return rc;
+        if (int rc = launch_shared(own, a, cache->type, p.by_rows, s)) return rc;
     } else {
         if (int rc = launch_parts(own, cache->type, s)) return rc;
     }
