@@ -7,7 +7,10 @@
 //   loss = sum_t w_t (-surrogate + beta kl - c H), w_t the mean's over tokens or over sequences
 //   dp = w (-[not clipped] ratio A + beta (1 - exp(f - p))), dH = -c w
 //
-// HBM bounds long batches, latency short ones. The flat tokens are cut into chunks of kChunk and a
+// HBM bounds long batches, latency short ones. Over 2 million tokens of 2048 sequences with all
+// tensors the sums take 14 us (42 MB, 2.9 TB/s), joining them 7, the gradient 14 (50 MB, 3.5 TB/s);
+// a few short sequences 4, 3 and 4. The arithmetic of some 60 operations a token is not hidden by
+// the loads altogether. The flat tokens are cut into chunks of kChunk and a
 // wave takes what one sequence has of one chunk, a segment. The segment of chunk c and sequence s
 // has place c + s, no other's: from one to the next at least one of them grows. So a wave finds its
 // segment by searching the offsets, without a list of them.
@@ -23,8 +26,9 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kChunk = 512;          // tokens of a wave
-constexpr int kJoinThreads = 1024;   // sequences of a joining block at a time
-constexpr int kOwn = 4;              // segments that a thread adds up by itself
+constexpr int kBatch = 4;            // tokens of a lane that are read together
+constexpr int kJoinThreads = 256;    // sequences of a joining block
+constexpr int kOwn = 16;             // segments that a thread adds up by itself
 
 // Sums of a segment, a sequence or all, in 64 bits: up to 2^31 terms.
 struct Sums {
@@ -95,16 +99,41 @@ __device__ __forceinline__ void kl_terms(float x, float& kl, float& rise) {
     if (fabsf(x) == INFINITY) kl = INFINITY;
 }
 
+// Tokens t, t + 64, ... of a segment as they are read: all together, those that do not count too,
+// whose values are then not used (2 million tokens of 2048 sequences: 19 us
+// one by one, 14 like this, 15 by eight).
+struct Tokens {
+    float p[kBatch], old[kBatch], advantage[kBatch], ref[kBatch], entropy[kBatch];
+    bool counts[kBatch];
+};
+
+template <bool ENTROPY>
+__device__ __forceinline__ void load(const Policy& a, const Segment& g, int t, Tokens& x) {
+    uint8_t mask[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+        const int at = min(t + 64 * i, g.end - 1);
+        mask[i] = a.mask != nullptr ? a.mask[at] : 1;
+        x.p[i] = a.logprob[at];
+        x.old[i] = a.old[at];
+        x.advantage[i] = a.advantage[a.advantage_by_sequence ? g.s : at];
+        x.ref[i] = a.ref != nullptr ? a.ref[at] : 0.0f;
+        if (ENTROPY) x.entropy[i] = a.entropy != nullptr ? a.entropy[at] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) x.counts[i] = mask[i] != 0 && t + 64 * i < g.end;
+}
+
 // A token's terms. Where the ratio stands against its limits goes by the difference in 64 bits.
 struct Token {
     float loss, kl, ratio, slope;  // slope: of the loss by the log probability
     bool clipped;
 };
 
-__device__ __forceinline__ Token token_of(const Policy& a, int t, float advantage) {
+__device__ __forceinline__ Token token_of(const Policy& a, const Tokens& from, int i) {
     Token x;
-    const float p = a.logprob[t];
-    const double d = double(p) - double(a.old[t]);
+    const float p = from.p[i], advantage = from.advantage[i];
+    const double d = double(p) - double(from.old[i]);
     x.ratio = expf(float(d));
     x.clipped = advantage < 0.0f ? d < a.log_low : d > a.log_high;
     const float limit = advantage < 0.0f ? a.low : a.high;
@@ -113,14 +142,12 @@ __device__ __forceinline__ Token token_of(const Policy& a, int t, float advantag
     x.kl = 0.0f;
     if (a.ref != nullptr) {
         float rise;
-        kl_terms(float(double(a.ref[t]) - double(p)), x.kl, rise);
+        kl_terms(float(double(from.ref[i]) - double(p)), x.kl, rise);
         if (a.kl_weight != 0.0f) {
             x.loss = __builtin_fmaf(a.kl_weight, x.kl, x.loss);
             x.slope = __builtin_fmaf(-a.kl_weight, rise, x.slope);
         }
     }
-    if (a.entropy != nullptr && a.entropy_weight != 0.0f)
-        x.loss = __builtin_fmaf(-a.entropy_weight, a.entropy[t], x.loss);
     return x;
 }
 
@@ -139,15 +166,23 @@ __global__ __launch_bounds__(kThreads) void policy_segments(Policy a, Sums* sums
     const Segment g = segment_of(a, place);
     if (g.begin == g.end) return;
     Sums x{};
-#pragma unroll 4
-    for (int t = g.begin + lane; t < g.end; t += 64) {
-        if (a.mask != nullptr && a.mask[t] == 0) continue;
-        const Token y = token_of(a, t, a.advantage[a.advantage_by_sequence ? g.s : t]);
-        x.loss += double(y.loss);
-        x.kl += double(y.kl);
-        x.ratio += double(y.ratio);
-        x.clipped += y.clipped;
-        x.tokens += 1;
+    for (int t = g.begin; t < g.end; t += 64 * kBatch) {
+        Tokens all;
+        load<true>(a, g, t + lane, all);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            if (t + 64 * i >= g.end) break;
+            const Token y = token_of(a, all, i);
+            float loss = y.loss;
+            if (a.entropy_weight != 0.0f)
+                loss = __builtin_fmaf(-a.entropy_weight, all.entropy[i], loss);
+            const bool counts = all.counts[i];
+            x.loss += counts ? double(loss) : 0.0;
+            x.kl += counts ? double(y.kl) : 0.0;
+            x.ratio += counts ? double(y.ratio) : 0.0;
+            x.clipped += counts && y.clipped;
+            x.tokens += counts;
+        }
     }
     x.loss = wave_sum(x.loss);
     x.kl = wave_sum(x.kl);
@@ -212,8 +247,10 @@ __global__ __launch_bounds__(kJoinThreads) void policy_sequences(Policy a, const
         count = begin < end ? (end - 1) / kChunk - begin / kChunk + 1 : 0;
     }
     Sums x{};
-    if (count <= kOwn)
+    if (count <= kOwn) {
+#pragma unroll 4
         for (int i = 0; i < count; ++i) add(x, sums[first + i]);
+    }
     for (uint64_t many = __ballot(count > kOwn); many != 0; many &= many - 1) {
         const int from = __builtin_ctzll(many);
         const int64_t at = __shfl(first, from);
@@ -282,16 +319,19 @@ __global__ __launch_bounds__(kThreads) void policy_backward(Policy a,
     const Segment g = segment_of(a, place);
     if (g.begin == g.end) return;
     const float w = grad[0] * (weights[g.s] * weights[a.sequences]);
-#pragma unroll 4
-    for (int t = g.begin + lane; t < g.end; t += 64) {
-        const bool counted = a.mask == nullptr || a.mask[t] != 0;
-        if (g_logprob != nullptr) {
-            float y = 0.0f;
-            if (counted)
-                y = w * token_of(a, t, a.advantage[a.advantage_by_sequence ? g.s : t]).slope;
-            g_logprob[t] = y;
+    for (int t = g.begin; t < g.end; t += 64 * kBatch) {
+        Tokens all;
+        load<false>(a, g, t + lane, all);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int at = t + 64 * i + lane;
+            if (at - lane >= g.end) break;
+            if (at >= g.end) continue;
+            const float y = w * token_of(a, all, i).slope;
+            if (g_logprob != nullptr) g_logprob[at] = all.counts[i] ? y : 0.0f;
+            if (g_entropy != nullptr)
+                g_entropy[at] = all.counts[i] ? -a.entropy_weight * w : 0.0f;
         }
-        if (g_entropy != nullptr) g_entropy[t] = counted ? -a.entropy_weight * w : 0.0f;
     }
 }
 

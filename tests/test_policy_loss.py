@@ -139,7 +139,8 @@ def check(hip, what, how, grad=0.75):
 @gpu
 @pytest.mark.parametrize("by_sequence", [False, True])
 @pytest.mark.parametrize("lengths", [[1], [2, 0, 3], [511], [512], [513], [1024, 1025], [63, 64, 65],
-                                     [0, 0, 7, 0], [5000], [1] * 700, [100] * 70, [3000, 1, 1, 2500]])
+                                     [0, 0, 7, 0], [5000], [1] * 700, [100] * 70, [3000, 1, 1, 2500],
+                                     [8192], [8193, 9000], [255, 256, 257], [9] * 256, [9] * 257])
 def test_lengths(hip, lengths, by_sequence):
     for masked in (0.0, 0.4):
         check(hip, *make(lengths, by_sequence, masked=masked, seed=len(lengths)))
