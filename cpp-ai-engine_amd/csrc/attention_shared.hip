@@ -103,6 +103,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
     constexpr int kBuffers = Lds::kBuffers, kPitch = value_pitch(DP);
     constexpr int kKeyPlane = Lds::kKeyPlane, kValuePlane = Lds::kValuePlane;
     static_assert(kKeys * kPieces % kPagedThreads == 0, "whole units");
+    static_assert(!kScaled || kUnits == 1, "a thread has one position's scale");
     const int lane = int(threadIdx.x) & 63, col = lane & 15, quarter = lane / 16;
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int dim = int(a.c.dim), kv_heads = int(a.c.kv_heads);
@@ -124,7 +125,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
 
         // The table's entries of the thread's units, asked for a step before their rows are read,
         // past the end the last again.
-        Entry entry[kUnits], scale_entry;
+        Entry entry[kUnits];
         uint32_t row[kUnits];
         int64_t place = 0;
         Unit kx[kUnits], vx[kUnits];
@@ -135,9 +136,6 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                 const int j = (int(threadIdx.x) + u * kPagedThreads) / kPieces;
                 entry[u] = entry_of(a.c, s, uint32_t(min(p0 + j, end - 1)));
             }
-            if constexpr (kScaled)
-                scale_entry = entry_of(
-                    a.c, s, uint32_t(min(p0 + int(threadIdx.x) % kKeys, end - 1)));
         };
         const auto find = [&] {
 #pragma unroll
@@ -149,14 +147,9 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                 }
                 row[u] = uint32_t(r);
             }
-            if constexpr (kScaled) {
-                int64_t r = row_of_entry(a.c, scale_entry);
-                if (r < 0) {
-                    r = 0;
-                    scale_entry.off = 0;
-                }
-                place = scale_of(a.c, r, scale_entry.off, kv);
-            }
+            // Of its position's piece 0 a thread has the key's scale too, of piece 1 the value's.
+            if constexpr (kScaled)
+                place = scale_of(a.c, row[0], row[0] != 0 ? entry[0].off : 0, kv);
         };
         const auto load = [&](int p0) {
 #pragma unroll
@@ -166,8 +159,9 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                 vx[u].load(v + uint64_t(row[u]) * pitch, d0, dim);
             }
             if constexpr (kScaled) {
-                const float* const from = int(threadIdx.x) < kKeys ? a.c.k_scales : a.c.v_scales;
-                scale = p0 + int(threadIdx.x) % kKeys < end ? from[place] : 0.0f;
+                const float* const from =
+                    int(threadIdx.x) % kPieces == 0 ? a.c.k_scales : a.c.v_scales;
+                scale = p0 + int(threadIdx.x) / kPieces < end ? from[place] : 0.0f;
             }
         };
         const auto store = [&](int p0, char* to, float (*scales)[kKeys]) {
@@ -194,8 +188,8 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                 }
             }
             if constexpr (kScaled)
-                if (int(threadIdx.x) < 2 * kKeys)
-                    scales[int(threadIdx.x) / kKeys][int(threadIdx.x) % kKeys] = scale;
+                if (int(threadIdx.x) % kPieces < 2)
+                    scales[int(threadIdx.x) % kPieces][int(threadIdx.x) / kPieces] = scale;
         };
         ask(begin);
         bf16x8 q[KS][3];
@@ -278,6 +272,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                     for (int r = 0; r < 4; ++r) w[4 * t + r] = sc[t][r];
                 }
                 if (p0 + kKeys > end) {
+                    asm volatile("");  // a branch: as selects in every step, 16 instructions
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         if (p0 + 16 * (j / 4) + 4 * quarter + j % 4 >= end) w[j] = -INFINITY;
@@ -291,7 +286,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    w[j] = __builtin_amdgcn_exp2f(w[j] - shift) * 0x1p-24f;
+                    w[j] = __builtin_amdgcn_exp2f(w[j] - shift);
                     sum += w[j];
                 }
                 l = __builtin_fmaf(l, keep, sum);
@@ -324,30 +319,40 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                         }
                 };
                 ask_values(0);
+                if (kBuffers > 1) store(p0 + kKeys, lds.tile[buffer ^ 1], lds.scales[buffer ^ 1]);
+                floatx4 y[2][2];
+                const auto sum_up = [&](int i) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            o[i + t][r] = __builtin_fmaf(o[i + t][r], keep, y[i / 2 & 1][t][r]);
+                };
 #pragma unroll
                 for (int i = 0; i < NV; i += 2) {
                     if (i + 2 < NV) ask_values(i + 2);
                     keep_order();
                     auto& x = f[i / 2 & 1];
-                    floatx4 y[2];
+                    auto& z = y[i / 2 & 1];
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) y[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-                    multiply_small<kParts>(y[0], x[0], y[1], x[1], p, p);
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        y[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[t][0], p[0], y[t], 0, 0, 0);
-                    }
-                    keep_order();
+                    for (int t = 0; t < 2; ++t) z[t] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+                    multiply_small<kParts>(z[0], x[0], z[1], x[1], p, p);
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            o[i + t][r] = __builtin_fmaf(o[i + t][r], keep, y[t][r]);
+                        z[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[t][0], p[0], z[t], 0, 0, 0);
+                    if (i > 0) sum_up(i - 2);  // while these products are formed
+                    keep_order();
                 }
+                sum_up(NV - 2);
+            } else if (kBuffers > 1) {
+                store(p0 + kKeys, lds.tile[buffer ^ 1], lds.scales[buffer ^ 1]);
             }
-            if (kBuffers == 1) __syncthreads();  // all have read
-            if (kBuffers > 1) buffer ^= 1;
-            store(p0 + kKeys, lds.tile[buffer], lds.scales[buffer]);
+            if (kBuffers == 1) {
+                __syncthreads();  // all have read
+                store(p0 + kKeys, lds.tile[0], lds.scales[0]);
+            } else {
+                buffer ^= 1;
+            }
             __syncthreads();
         }
         // The lane's row, values 16 i + 4 quarter + r; rows whose sums are not finite by the formula.
@@ -365,14 +370,14 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
         const int64_t part0 = part_of<true>(a, seg, worker, kv, 0, 0);
         if (mine < count && !(again >> col & 1)) {
             const int64_t at = part0 + mine;
-            if (quarter == 0) a.part_stats[at] = float2{m, bad ? NAN : l};
+            if (quarter == 0) a.part_stats[at] = float2{m, bad ? NAN : l * 0x1p-24f};
             float* const to = a.part_out + at * dim;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int d = 16 * i + 4 * quarter;
                 floatx4u y;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = o[i][r];
+                for (int r = 0; r < 4; ++r) y[r] = o[i][r] * 0x1p-24f;  // as the other parts
                 if (d + 4 <= dim) {
                     *reinterpret_cast<floatx4u*>(to + d) = y;
                 } else {
