@@ -387,6 +387,108 @@ def test_pools_at_any_address(hip, kind):
 
 
 @gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kv", [(2, 2), (8, 1)])
+def test_many_groups(hip, kind, heads, kv):
+    """More groups, and more sequences, than a wave has lanes, of uneven lengths."""
+    groups = [((29 * i) % 70, [(11 * i + 5 * j) % 23 for j in range(1 + i % 5)])
+              for i in range(150)]
+    check(hip, groups, heads, kv, 32, 8, kind, seed=18)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("members", [3, 40])
+def test_values_next_to_the_largest(hip, kind, members):
+    """Weighted sums before their division by the weights' are past fp32, what comes out is not."""
+    print_case("shared large", kind, members)
+    b = Batch(hip, [(300, [2] * members), (40, [1, 1])], 4, 2, 64, 16, kind, seed=19)
+    if kind == "int8":
+        b.scales[1].fill_(2.0 ** 119)
+        b.vp.copy_(b.vp.abs())
+    else:
+        b.vp.copy_((b.vp.float().abs().clamp(max=1.9) * 2.0 ** 126).to(b.vp.dtype))
+    out, lse = b.run(hip)
+    value, bound = b.expect()
+    within(out, value["out"], bound["out"], "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
+@gpu
+@pytest.mark.parametrize("power", [-70, -80, 100])
+@pytest.mark.parametrize("members", [3, 40])
+def test_small_and_large_scales(hip, power, members):
+    """A weight times its scale runs in parts of at least 2^-133, of 2^-24 of it at the least: 2^-109
+    of a position, with codes of up to 127 2^-102 in what it stands for, and as much for the sums."""
+    print_case("shared scales", power, members)
+    b = Batch(hip, [(300, [2] * members), (40, [1, 1])], 4, 2, 64, 16, "int8", seed=20)
+    b.scales[1].mul_(2.0 ** power)
+    out, lse = b.run(hip)
+    value, bound = b.expect()
+    within(out, value["out"], bound["out"] + 302 * 2.0 ** -100, "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("members", [3, 40])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_odd_heads_that_are_not_finite(hip, kind, members, which):
+    """Heads whose rows begin at any address, formed a second time: a NaN key or scale of the shared
+    positions is its key head's in the group, one value's its column's."""
+    import torch
+    print_case("shared odd not finite", kind, members, which)
+    b, want, want_lse = check(hip, [(300, [2] * members), (40, [1, 1])], 4, 2, 33, 16, kind, seed=21)
+    page = int(b.table[0, 3])
+    if kind == "int8":
+        b.scales[which == "v"][page, 0, 2] = math.nan
+    else:
+        (b.kp if which == "k" else b.vp)[page, 2, 0, 7] = math.nan
+    out, lse = b.run(hip)
+    columns = [7] if which == "v" and kind != "int8" else list(range(33))
+    assert bool(torch.isnan(out[:members, :2][..., columns]).all())
+    rest = [c for c in range(33) if c not in columns]
+    value, bound = b.expect()
+    within(out[:members, :2][..., rest], value["out"][:members, :2][..., rest],
+           bound["out"][:members, :2][..., rest], "out")
+    if which == "k":
+        assert bool(torch.isnan(lse[:members, :2]).all())
+    else:
+        within(lse[:members, :2], value["lse"][:members, :2], bound["lse"][:members, :2], "lse")
+    assert torch.equal(out[:, 2:], want[:, 2:]) and torch.equal(lse[:, 2:], want_lse[:, 2:])
+    assert torch.equal(out[members:], want[members:])
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("members", [3, 20])
+def test_a_cache_past_32_bit_offsets(hip, kind, members):
+    """The same pages at the end of pools of 2^31 values and more: the same bits."""
+    import torch
+    print_case("shared large cache", kind, members)
+    b = Batch(hip, [(300, [2] * members), (40, [1, 1])], 8, 8, 128, 128, kind, seed=22)
+    want, want_lse = b.run(hip)
+    pages, count = 16400, b.kp.shape[0]
+    at = pages - 1 - torch.arange(count, device="cuda")
+    for name in ("kp", "vp"):
+        pool = getattr(b, name)
+        big = torch.zeros(pages, *pool.shape[1:], dtype=pool.dtype, device="cuda")
+        assert big.numel() > 2 ** 31
+        big[at] = pool
+        setattr(b, name, big)
+    if b.scales is not None:
+        scales = [torch.zeros(pages, *x.shape[1:], device="cuda") for x in b.scales]
+        for big, x in zip(scales, b.scales):
+            big[at] = x
+        b.scales = scales
+    b.table = (pages - 1 - b.table).to(torch.int32)
+    out, lse = b.run(hip)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    del b, big
+    torch.cuda.empty_cache()
+
+
+@gpu
 def test_no_sequences(hip):
     import torch
     print_case("shared no sequences")

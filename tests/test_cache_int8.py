@@ -415,6 +415,38 @@ def test_small_and_large_values(hip, power):
 
 
 @gpu
+@pytest.mark.parametrize("heads,kv,d", [(4, 4, 64), (8, 2, 128), (3, 1, 33)])
+def test_many_sequences(hip, heads, kv, d):
+    """More than a wave has lanes, of uneven lengths, some empty."""
+    check(hip, [(37 * i) % 90 if i % 7 else 0 for i in range(200)] + [3000] + [1] * 70, heads, kv, d,
+          16, seed=15)
+
+
+@gpu
+def test_a_cache_past_32_bit_offsets(hip):
+    """Written, read back and attended to at the end of pools of 2^31 values and more: the same bits
+    as in small ones."""
+    import torch
+    print_case("paged8 large")
+    pages, page, kv, d, lengths = 16400, 128, 8, 128, [300, 1, 40]
+    kp, vp, scales, table, k, v = fill(hip, lengths, kv, d, page, seed=16)
+    q = torch.randn(3, 16, d, device="cuda")
+    want = hip.attention_paged(q, kp, vp, table, ints(lengths), scales=scales)
+    held_k, held_v = hip.cache_read(kp, vp, table, ints([0] * 3), offsets(lengths), 341,
+                                    scales=scales)
+    kp, vp, scales = pools(pages, page, kv, d)
+    assert kp.numel() > 2 ** 31
+    table = (pages - 1 - table).to(torch.int32)
+    hip.cache_append(k, v, kp, vp, table, ints([0] * 3), offsets(lengths), scales=scales)
+    got = hip.cache_read(kp, vp, table, ints([0] * 3), offsets(lengths), 341, scales=scales)
+    assert torch.equal(got[0], held_k) and torch.equal(got[1], held_v)
+    out = hip.attention_paged(q, kp, vp, table, ints(lengths), scales=scales)
+    assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+    del kp, vp
+    torch.cuda.empty_cache()
+
+
+@gpu
 def test_strides_and_outputs(hip):
     import torch
     lengths = [100, 17]
