@@ -8,9 +8,8 @@
 //   dp = w (-[not clipped] ratio A + beta (1 - exp(f - p))), dH = -c w
 //
 // HBM bounds long batches, latency short ones. Over 2 million tokens of 2048 sequences with all
-// tensors the sums take 14 us (42 MB, 2.9 TB/s), joining them 7, the gradient 14 (50 MB, 3.5 TB/s);
-// a few short sequences 4, 3 and 4. The arithmetic of some 60 operations a token is not hidden by
-// the loads altogether. The flat tokens are cut into chunks of kChunk and a
+// tensors the sums take 17 us (42 MB, 2.4 TB/s), joining them 7, the gradient 14 (50 MB, 3.5 TB/s);
+// the arithmetic of some 60 to 80 operations a token is not hidden by the loads altogether. The flat tokens are cut into chunks of kChunk and a
 // wave takes what one sequence has of one chunk, a segment. The segment of chunk c and sequence s
 // has place c + s, no other's: from one to the next at least one of them grows. So a wave finds its
 // segment by searching the offsets, without a list of them.
@@ -29,6 +28,8 @@ constexpr int kChunk = 512;          // tokens of a wave
 constexpr int kBatch = 4;            // tokens of a lane that are read together
 constexpr int kJoinThreads = 256;    // sequences of a joining block
 constexpr int kOwn = 16;             // segments that a thread adds up by itself
+constexpr int kFewThreads = 1024;
+constexpr int kFew = 64;             // places that one block takes
 
 // Sums of a segment, a sequence or all, in 64 bits: up to 2^31 terms.
 struct Sums {
@@ -47,7 +48,7 @@ struct Policy {
     int sequences, tokens;
     bool advantage_by_sequence, mean_by_sequence;
     double log_low, log_high;  // clipped where d is below, above
-    float low, high;           // the ratio there
+    double low, high;          // the ratio there
     float kl_weight, entropy_weight;
     int64_t places;
 };
@@ -99,9 +100,21 @@ __device__ __forceinline__ void kl_terms(float x, float& kl, float& rise) {
     if (fabsf(x) == INFINITY) kl = INFINITY;
 }
 
+// exp(x): 2^n exp(f), |f| <= ln 2 / 2, by Taylor's series, whose next term is 2^-37 of it. A third of
+// the library's instructions, which has 53 bits.
+__device__ __forceinline__ double exp36(double x) {
+    x = x < -800.0 ? -800.0 : x > 800.0 ? 800.0 : x;  // 0 and infinity; NaN stays
+    const double n = rint(x * 1.44269504088896340736);
+    const double f = __builtin_fma(-n, 0.693147180559945309417, x);
+    double s = 1.0;
+#pragma unroll
+    for (int i = 9; i >= 1; --i) s = __builtin_fma(f * (1.0 / double(i)), s, 1.0);
+    return ldexp(s, x == x ? int(n) : 0);
+}
+
 // Tokens t, t + 64, ... of a segment as they are read: all together, those that do not count too,
-// whose values are then not used (2 million tokens of 2048 sequences: 19 us
-// one by one, 14 like this, 15 by eight).
+// whose values are then not used (2 million tokens of 2048 sequences, in
+// 32 bits: 19 us one by one, 14 like this, 15 by eight).
 struct Tokens {
     float p[kBatch], old[kBatch], advantage[kBatch], ref[kBatch], entropy[kBatch];
     bool counts[kBatch];
@@ -124,29 +137,33 @@ __device__ __forceinline__ void load(const Policy& a, const Segment& g, int t, T
     for (int i = 0; i < kBatch; ++i) x.counts[i] = mask[i] != 0 && t + 64 * i < g.end;
 }
 
-// A token's terms. Where the ratio stands against its limits goes by the difference in 64 bits.
+// A token's terms: T of the surrogate. The loss's sum takes 64 bits, as it has terms of both signs
+// (340 tokens' of about 1 have come to 10^-3; 17 us for the 14 of 32 bits), the gradient 32. Whether the ratio is clipped goes by
+// the difference in 64 bits.
+template <class T>
 struct Token {
-    float loss, kl, ratio, slope;  // slope: of the loss by the log probability
+    T ratio, surrogate, slope;  // slope: of the loss by the log probability
+    float kl;
     bool clipped;
 };
 
-__device__ __forceinline__ Token token_of(const Policy& a, const Tokens& from, int i) {
-    Token x;
+__device__ __forceinline__ float exp_of(double x, float) { return expf(float(x)); }
+__device__ __forceinline__ double exp_of(double x, double) { return exp36(x); }
+
+template <class T>
+__device__ __forceinline__ Token<T> token_of(const Policy& a, const Tokens& from, int i) {
+    Token<T> x;
     const float p = from.p[i], advantage = from.advantage[i];
     const double d = double(p) - double(from.old[i]);
-    x.ratio = expf(float(d));
+    x.ratio = exp_of(d, T());
     x.clipped = advantage < 0.0f ? d < a.log_low : d > a.log_high;
-    const float limit = advantage < 0.0f ? a.low : a.high;
-    x.loss = -(x.clipped ? limit : x.ratio) * advantage;
-    x.slope = x.clipped ? 0.0f : -x.ratio * advantage;
+    x.surrogate = (x.clipped ? T(advantage < 0.0f ? a.low : a.high) : x.ratio) * T(advantage);
+    x.slope = x.clipped ? T(0) : -x.ratio * T(advantage);
     x.kl = 0.0f;
     if (a.ref != nullptr) {
         float rise;
         kl_terms(float(double(from.ref[i]) - double(p)), x.kl, rise);
-        if (a.kl_weight != 0.0f) {
-            x.loss = __builtin_fmaf(a.kl_weight, x.kl, x.loss);
-            x.slope = __builtin_fmaf(-a.kl_weight, rise, x.slope);
-        }
+        if (a.kl_weight != 0.0f) x.slope -= T(a.kl_weight * rise);
     }
     return x;
 }
@@ -158,11 +175,9 @@ __device__ __forceinline__ T wave_sum(T x) {
     return x;
 }
 
-__global__ __launch_bounds__(kThreads) void policy_segments(Policy a, Sums* sums) {
-    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+// The sums of a place's segment. Every lane of the wave calls it.
+__device__ __forceinline__ void sum_segment(const Policy& a, int64_t place, Sums* sums) {
     const int lane = int(threadIdx.x) & 63;
-    const int64_t place = int64_t(blockIdx.x) * kWaves + wave;
-    if (place >= a.places) return;
     const Segment g = segment_of(a, place);
     if (g.begin == g.end) return;
     Sums x{};
@@ -172,14 +187,16 @@ __global__ __launch_bounds__(kThreads) void policy_segments(Policy a, Sums* sums
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             if (t + 64 * i >= g.end) break;
-            const Token y = token_of(a, all, i);
-            float loss = y.loss;
+            const Token<double> y = token_of<double>(a, all, i);
+            double loss = -y.surrogate;
+            if (a.kl_weight != 0.0f)
+                loss = __builtin_fma(double(a.kl_weight), double(y.kl), loss);
             if (a.entropy_weight != 0.0f)
-                loss = __builtin_fmaf(-a.entropy_weight, all.entropy[i], loss);
+                loss = __builtin_fma(-double(a.entropy_weight), double(all.entropy[i]), loss);
             const bool counts = all.counts[i];
-            x.loss += counts ? double(loss) : 0.0;
+            x.loss += counts ? loss : 0.0;
             x.kl += counts ? double(y.kl) : 0.0;
-            x.ratio += counts ? double(y.ratio) : 0.0;
+            x.ratio += counts ? y.ratio : 0.0;
             x.clipped += counts && y.clipped;
             x.tokens += counts;
         }
@@ -190,6 +207,12 @@ __global__ __launch_bounds__(kThreads) void policy_segments(Policy a, Sums* sums
     x.clipped = wave_sum(x.clipped);
     x.tokens = wave_sum(x.tokens);
     if (lane == 0) sums[place] = x;
+}
+
+__global__ __launch_bounds__(kThreads) void policy_segments(Policy a, Sums* sums) {
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    const int64_t place = int64_t(blockIdx.x) * kWaves + wave;
+    if (place < a.places) sum_segment(a, place, sums);
 }
 
 __device__ __forceinline__ void add(Sums& x, const Sums& y) {
@@ -213,6 +236,7 @@ __device__ __forceinline__ void finish(const Policy& a, const BlockSums& x, floa
 }
 
 // The sums of all threads of the block in thread 0. Every thread calls it.
+template <int THREADS>
 __device__ __forceinline__ BlockSums block_sums(const BlockSums& mine, BlockSums* sh) {
     const BlockSums x{wave_sum(mine.loss),    wave_sum(mine.kl),     wave_sum(mine.ratio),
                       wave_sum(mine.clipped), wave_sum(mine.tokens), wave_sum(mine.count)};
@@ -220,7 +244,7 @@ __device__ __forceinline__ BlockSums block_sums(const BlockSums& mine, BlockSums
     __syncthreads();
     BlockSums all{};
     if (threadIdx.x == 0)
-        for (int w = 0; w < kJoinThreads / 64; ++w) {
+        for (int w = 0; w < THREADS / 64; ++w) {
             all.loss += sh[w].loss;
             all.kl += sh[w].kl;
             all.ratio += sh[w].ratio;
@@ -231,14 +255,12 @@ __device__ __forceinline__ BlockSums block_sums(const BlockSums& mine, BlockSums
     return all;
 }
 
-// The sequences' sums and weights, a thread each; a sequence of many segments by its wave. One
-// block writes the results, several their sums for policy_finish.
-__global__ __launch_bounds__(kJoinThreads) void policy_sequences(Policy a, const Sums* sums,
-                                                                 BlockSums* blocks, float* loss,
-                                                                 float* stats, float* weights) {
-    __shared__ BlockSums sh[kJoinThreads / 64];
+// The sums and weights of a block's sequences, a thread each; a sequence of many segments by its
+// wave. Returns all sequences' sums in thread 0. Every thread of the block calls it.
+template <int THREADS>
+__device__ __forceinline__ BlockSums sum_sequences(const Policy& a, int s, const Sums* sums,
+                                                   float* weights, BlockSums* sh) {
     const int lane = int(threadIdx.x) & 63;
-    const int s = int(blockIdx.x) * kJoinThreads + int(threadIdx.x);
     int64_t first = 0;
     int count = 0;
     if (s < a.sequences) {
@@ -274,10 +296,32 @@ __global__ __launch_bounds__(kJoinThreads) void policy_sequences(Policy a, const
                          double(x.clipped),
                          n,
                          a.mean_by_sequence ? double(x.tokens > 0) : n};
-    const BlockSums all = block_sums(mine, sh);
+    return block_sums<THREADS>(mine, sh);
+}
+
+// One block writes the results, several their sums for policy_finish.
+__global__ __launch_bounds__(kJoinThreads) void policy_sequences(Policy a, const Sums* sums,
+                                                                 BlockSums* blocks, float* loss,
+                                                                 float* stats, float* weights) {
+    __shared__ BlockSums sh[kJoinThreads / 64];
+    const int s = int(blockIdx.x) * kJoinThreads + int(threadIdx.x);
+    const BlockSums all = sum_sequences<kJoinThreads>(a, s, sums, weights, sh);
     if (threadIdx.x != 0) return;
     if (gridDim.x > 1) blocks[blockIdx.x] = all;
     else finish(a, all, loss, stats, weights);
+}
+
+// All in one block, for up to kFew places: a launch less (32 sequences, 340 tokens in all, with the
+// gradient, from Python: 28 us with two, 22 like this, and with fewer tensors made).
+__global__ __launch_bounds__(kFewThreads) void policy_few(Policy a, Sums* sums, float* loss,
+                                                          float* stats, float* weights) {
+    __shared__ BlockSums sh[kFewThreads / 64];
+    const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
+    for (int64_t place = wave; place < a.places; place += kFewThreads / 64)
+        sum_segment(a, place, sums);
+    __syncthreads();
+    const BlockSums all = sum_sequences<kFewThreads>(a, int(threadIdx.x), sums, weights, sh);
+    if (threadIdx.x == 0) finish(a, all, loss, stats, weights);
 }
 
 __global__ __launch_bounds__(kJoinThreads) void policy_finish(Policy a, const BlockSums* blocks,
@@ -294,7 +338,7 @@ __global__ __launch_bounds__(kJoinThreads) void policy_finish(Policy a, const Bl
         x.tokens += y.tokens;
         x.count += y.count;
     }
-    x = block_sums(x, sh);
+    x = block_sums<kJoinThreads>(x, sh);
     if (threadIdx.x == 0) finish(a, x, loss, stats, weights);
 }
 
@@ -327,7 +371,7 @@ __global__ __launch_bounds__(kThreads) void policy_backward(Policy a,
             const int at = t + 64 * i + lane;
             if (at - lane >= g.end) break;
             if (at >= g.end) continue;
-            const float y = w * token_of(a, all, i).slope;
+            const float y = w * token_of<float>(a, all, i).slope;
             if (g_logprob != nullptr) g_logprob[at] = all.counts[i] ? y : 0.0f;
             if (g_entropy != nullptr)
                 g_entropy[at] = all.counts[i] ? -a.entropy_weight * w : 0.0f;
@@ -367,8 +411,8 @@ int check(const char* name, const ehip_policy_t* d, Policy& a) {
     a.mean_by_sequence = d->mean_by_sequence != 0;
     a.log_low = d->clip_low < 1.0 ? std::log1p(-d->clip_low) : -INFINITY;
     a.log_high = std::log1p(d->clip_high);
-    a.low = float(1.0 - d->clip_low);
-    a.high = float(1.0 + d->clip_high);
+    a.low = 1.0 - d->clip_low;
+    a.high = 1.0 + d->clip_high;
     a.kl_weight = d->kl_weight;
     a.entropy_weight = d->entropy_weight;
     a.places = a.tokens / kChunk + 1 + a.sequences;
@@ -376,8 +420,9 @@ int check(const char* name, const ehip_policy_t* d, Policy& a) {
 }
 
 int check_tensors(const char* name, const Policy& a) {
+    const bool advantages = !a.advantage_by_sequence || a.sequences > 0;
     if (a.cu == nullptr || (a.tokens > 0 && (a.logprob == nullptr || a.old == nullptr ||
-                                             a.advantage == nullptr)))
+                                             (advantages && a.advantage == nullptr))))
         return fail(EHIP_EINVAL, "%s: null tensor", name);
     return EHIP_OK;
 }
@@ -417,6 +462,11 @@ int ehip_policy_loss_f32(const ehip_policy_t* desc, float* loss, float* stats, f
     const int64_t joins = join_blocks(a);
     Sums* const sums = reinterpret_cast<Sums*>(blocks + joins);
     hipStream_t s = as_stream(stream);
+    if (a.places <= kFew) {
+        EHIP_LAUNCH("policy_loss", policy_few, dim3(1), dim3(kFewThreads), 0, s, a, sums, loss,
+                    stats, weights);
+        return EHIP_OK;
+    }
     if (a.tokens > 0 && a.sequences > 0)
         EHIP_LAUNCH("policy_loss", policy_segments, dim3(unsigned(ceil_div(a.places, kWaves))),
                     dim3(kThreads), 0, s, a, sums);

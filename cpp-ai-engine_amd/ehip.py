@@ -315,6 +315,11 @@ class Backend:
     def f32(self, shape):
         return self.torch.empty(shape, dtype=self.torch.float32, device="cuda")
 
+    def _like(self, t):
+        """A dense tensor of t's shape, type and device."""
+        torch = self.torch
+        return torch.empty_like(t, memory_format=torch.contiguous_format)
+
     def device_info(self):
         info = DeviceInfo()
         self.ok(self.lib.ehip_device_info(C.byref(info)), "device_info")
@@ -814,7 +819,7 @@ class Backend:
         """Refuses tensors that are not all on the current device (whose stream is used)."""
         index = self.torch.cuda.current_device()
         for t in tensors:
-            if t is not None and not (t.is_cuda and t.device.index == index):
+            if t is not None and t.get_device() != index:  # -1 in host memory
                 raise ValueError(f"tensor on {t.device}, the current device is cuda:{index}")
 
     def _rows(self, t, what, shape, dtype=None):
@@ -966,13 +971,17 @@ class Backend:
             raise ValueError("tokens: expected with cu")
         tokens = cache.sequences if cu is None else tokens
         shape = (tokens,) + tuple(k_pages.shape[2:])
-        k, v = (self.f32(shape), self.f32(shape)) if out is None else out
-        self._here(starts, cu, k, v)
+        self._here(starts, cu, *(out or ()))
+        if out is None:
+            k, v = self.f32(shape), self.f32(shape)
+            ld_k = ld_v = cache.kv_heads * cache.head_dim
+        else:
+            k, v = out
+            ld_k, ld_v = self._rows(k, "k", shape), self._rows(v, "v", shape)
         self.ok(self.lib.ehip_cache_read_f32(
             C.byref(cache), self._index(starts, "starts", cache.sequences),
             None if cu is None else self._index(cu, "cu", cache.sequences + 1), tokens,
-            _vp(k.data_ptr()), self._rows(k, "k", shape), _vp(v.data_ptr()),
-            self._rows(v, "v", shape), self.stream()), "cache_read")
+            k.data_ptr(), ld_k, v.data_ptr(), ld_v, self.stream()), "cache_read")
         return k, v
 
     def attention_paged(self, q, k_pages, v_pages, table, lengths, longest=None, scale=None,
@@ -985,19 +994,23 @@ class Backend:
         if q.dim() != 3:
             raise ValueError("q: expected (sequences, heads, head_dim)")
         cache = self._cache(k_pages, v_pages, table, scales)
-        out = self.f32(q.shape) if out is None else out
-        lse = self.f32(q.shape[:2]) if lse is None else lse
         self._here(q, lengths, out, lse)
         n, h, d = cache.sequences, q.shape[1], cache.head_dim
+        ld_q = self._rows(q, "q", (n, h, d))
+        if out is None:
+            out, ld_out = self._like(q), h * d
+        else:
+            ld_out = self._rows(out, "out", (n, h, d))
+        if lse is None:
+            lse = self.f32((n, h))
         if longest is None:
             longest = cache.table_width * cache.page_size
         need = self.lib.ehip_attention_paged_workspace(C.byref(cache), h, longest)
         space, at, size = self._workspace(need, "attention_paged")
         self.ok(self.lib.ehip_attention_paged_f32(
-            C.byref(cache), _vp(q.data_ptr()), self._rows(q, "q", (n, h, d)), h,
+            C.byref(cache), q.data_ptr(), ld_q, h,
             self._index(lengths, "lengths", n), longest, d ** -0.5 if scale is None else scale,
-            _vp(out.data_ptr()), self._rows(out, "out", (n, h, d)),
-            _vp(self._dense(lse, "lse", (n, h))), at, size, self.stream()), "attention_paged")
+            out.data_ptr(), ld_out, self._dense(lse, "lse", (n, h)), at, size, self.stream()), "attention_paged")
         return out, lse
 
     def token_logprobs(self, logits, targets=None, top=0, want_entropy=True):
@@ -1089,12 +1102,16 @@ class Backend:
         given, which may be q and k themselves."""
         desc = self._norm_rotate(q, k, positions, freqs, q_weight, k_weight, eps, interleaved)
         if out is None:
-            out = [self.f32(q.shape), None if k is None else self.f32(k.shape)]
-        self._here(*out)
-        self.ok(self.lib.ehip_norm_rotate_f32(
-            C.byref(desc), *self._into(out[0], "q_out", q),
-            *(self._into(out[1], "k_out", k) if k is not None else (None, 0)), self.stream()),
-            "norm_rotate")
+            out = self._like(q), None if k is None else self._like(k)
+            d = desc.head_dim
+            q_out, ld_q, ld_k = out[0].data_ptr(), desc.heads * d, desc.kv_heads * d
+            k_out = None if k is None else out[1].data_ptr()
+        else:
+            self._here(*out)
+            q_out, ld_q = self._into(out[0], "q_out", q)
+            k_out, ld_k = self._into(out[1], "k_out", k) if k is not None else (None, 0)
+        self.ok(self.lib.ehip_norm_rotate_f32(C.byref(desc), q_out, ld_q, k_out, ld_k,
+                                              self.stream()), "norm_rotate")
         return tuple(out)
 
     def norm_rotate_backward(self, g_q, g_k, q, k, positions, freqs, q_weight=None,
@@ -1105,8 +1122,8 @@ class Backend:
         and dk into, which may be g_q and g_k themselves (None in place of one: not formed)."""
         desc = self._norm_rotate(q, k, positions, freqs, q_weight, k_weight, eps, interleaved)
         if grads is None:
-            grads = [self.f32(q.shape) if want[0] else None,
-                     self.f32(k.shape) if want[1] and k is not None else None]
+            grads = [self._like(q) if want[0] else None,
+                     self._like(k) if want[1] and k is not None else None]
         dq_weight = self.f32(q_weight.shape) if want[2] and q_weight is not None else None
         dk_weight = self.f32(k_weight.shape) if want[3] and k_weight is not None else None
         self._here(g_q, g_k, *grads)
@@ -1134,10 +1151,15 @@ class Backend:
         if group_cu.dim() != 1 or group_cu.numel() < 1:
             raise ValueError("group_cu: expected one offset more than groups")
         cache = self._cache(k_pages, v_pages, table, scales)
-        out = self.f32(q.shape) if out is None else out
-        lse = self.f32(q.shape[:2]) if lse is None else lse
         self._here(q, lengths, group_cu, shared, out, lse)
         n, h, d = cache.sequences, q.shape[1], cache.head_dim
+        ld_q = self._rows(q, "q", (n, h, d))
+        if out is None:
+            out, ld_out = self._like(q), h * d
+        else:
+            ld_out = self._rows(out, "out", (n, h, d))
+        if lse is None:
+            lse = self.f32((n, h))
         groups = group_cu.numel() - 1
         if longest is None:
             longest = cache.table_width * cache.page_size
@@ -1147,12 +1169,11 @@ class Backend:
                                                         longest_shared)
         space, at, size = self._workspace(need, "attention_shared")
         self.ok(self.lib.ehip_attention_shared_f32(
-            C.byref(cache), _vp(q.data_ptr()), self._rows(q, "q", (n, h, d)), h,
+            C.byref(cache), q.data_ptr(), ld_q, h,
             self._index(lengths, "lengths", n), longest,
             self._index(group_cu, "group_cu", groups + 1), self._index(shared, "shared", groups),
-            groups, longest_shared, d ** -0.5 if scale is None else scale, _vp(out.data_ptr()),
-            self._rows(out, "out", (n, h, d)), _vp(self._dense(lse, "lse", (n, h))), at, size,
-            self.stream()), "attention_shared")
+            groups, longest_shared, d ** -0.5 if scale is None else scale, out.data_ptr(), ld_out,
+            self._dense(lse, "lse", (n, h)), at, size, self.stream()), "attention_shared")
         return out, lse
 
     def _policy(self, logprob, old, advantage, cu, clip_low, clip_high, ref, kl_weight, entropy,
@@ -1186,11 +1207,11 @@ class Backend:
         policy_loss_backward)."""
         desc = self._policy(logprob, old, advantage, cu, clip_low, clip_high, ref, kl_weight,
                             entropy, entropy_weight, mask, by_sequence, mean_by_sequence)
-        loss, stats, weights = self.f32((1,)), self.f32((3,)), self.f32((cu.numel(),))
+        loss, stats, weights = self.f32((4 + cu.numel(),)).split((1, 3, cu.numel()))
         need = self.lib.ehip_policy_loss_workspace(C.byref(desc))
         space, at, n = self._workspace(need, "policy_loss")
-        self.ok(self.lib.ehip_policy_loss_f32(C.byref(desc), self.p(loss), self.p(stats),
-                                              self.p(weights), at, n, self.stream()),
+        self.ok(self.lib.ehip_policy_loss_f32(C.byref(desc), loss.data_ptr(), stats.data_ptr(),
+                                              weights.data_ptr(), at, n, self.stream()),
                 "policy_loss")
         return loss, stats, weights
 
@@ -1203,8 +1224,8 @@ class Backend:
         desc = self._policy(logprob, old, advantage, cu, clip_low, clip_high, ref, kl_weight,
                             entropy, entropy_weight, mask, by_sequence, mean_by_sequence)
         self._here(grad, weights)
-        g_logprob = self.f32(logprob.shape)
-        g_entropy = None if entropy is None else self.f32(entropy.shape)
+        g_logprob = self._like(logprob)
+        g_entropy = None if entropy is None else self._like(entropy)
         self.ok(self.lib.ehip_policy_loss_backward_f32(
             C.byref(desc), _vp(self._dense(weights, "weights", (cu.numel(),))),
             _vp(self._dense(grad, "grad", (1,))), self.p(g_logprob), self.p(g_entropy),

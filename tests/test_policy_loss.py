@@ -147,6 +147,34 @@ def test_lengths(hip, lengths, by_sequence):
 
 
 @gpu
+@pytest.mark.parametrize("lengths", [[500], [30] * 40, [4000] * 3])
+def test_a_loss_of_terms_that_cancel(hip, lengths):
+    """Neighbours have the advantages a and -a and nearly the same ratio. A term is a product in 64
+    bits with a series that is 2^-37 off: 2^-36 of it with what is rounded, and the result 2^-24."""
+    import torch
+    what, how = make(lengths, ref=False, entropy=False, masked=0.0, seed=21, spread=0.05)
+    lp, old, a, cu = what
+    a = a.view(-1, 2)[:, :1].repeat(1, 2) * torch.tensor([1.0, -1.0], device="cuda")
+    a = a.reshape(-1)
+    d = (lp - old).view(-1, 2)
+    old = (lp.view(-1, 2) - d[:, :1] - torch.tensor([0.0, 1e-4], device="cuda")).reshape(-1)
+    print_case("policy cancel", lengths)
+    loss, _, _ = hip.policy_loss(lp, old, a.contiguous(), cu, 0.9, 9.0, **how)
+    term = (-(lp.double() - old.double()).exp() * a.double()).cpu()
+    want, size = float(term.mean()), float(term.abs().mean())
+    assert abs(want) < 1e-3 * size
+    assert abs(float(loss) - want) <= 2.0 ** -36 * size + 2.0 ** -24 * abs(want)
+
+
+@gpu
+@pytest.mark.parametrize("by_sequence", [False, True])
+@pytest.mark.parametrize("count", [1, 31, 32, 33, 63, 64, 65])
+def test_about_as_many_as_one_block_takes(hip, by_sequence, count):
+    check(hip, *make([1 + i % 9 for i in range(count)], by_sequence, seed=count))
+    check(hip, *make([520] * (count // 2), by_sequence, seed=count, entropy=False, before=3))
+
+
+@gpu
 @pytest.mark.parametrize("by_sequence", [False, True])
 def test_many_sequences(hip, by_sequence):
     """More than one joining block has, of which one block has more than its threads again."""
