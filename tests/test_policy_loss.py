@@ -46,9 +46,11 @@ def formula(lp, old, adv, cu, clip_low=0.2, clip_high=0.2, ref=None, kl_weight=0
     counts = which >= 0
     if mask is not None:
         counts = counts & (mask.cpu() != 0)
+    if by_sequence and len(offsets) == 1:
+        adv = torch.zeros(1, dtype=torch.float64)  # of no sequence: not used
     a = adv[which.clamp_min(0)] if by_sequence else adv
     if by_sequence if mean_by_sequence is None else mean_by_sequence:
-        size = torch.zeros(len(offsets) - 1, dtype=torch.float64).index_add_(
+        size = torch.zeros(max(1, len(offsets) - 1), dtype=torch.float64).index_add_(
             0, which[counts], torch.ones(int(counts.sum()), dtype=torch.float64))
         w = 1 / (size[which.clamp_min(0)] * max(1, int((size > 0).sum())))
     else:
