@@ -262,22 +262,24 @@ __global__ __launch_bounds__(kThreads) void norm_rotate(Args a) {
 }
 
 // The weights' gradients from the blocks' shares, in their order: sixteen columns a
-// block, sixteen threads of shares each.
-__global__ __launch_bounds__(kThreads) void norm_rotate_join(const float* __restrict__ parts,
+// block, sixty-four threads of shares each.
+constexpr int kJoinThreads = 1024;
+
+__global__ __launch_bounds__(kJoinThreads) void norm_rotate_join(const float* __restrict__ parts,
                                                              int count, int dim, float* dq,
                                                              float* dk) {
-    __shared__ float sh[kThreads];
+    __shared__ float sh[kJoinThreads];
     const int column = int(blockIdx.x) * 16 + int(threadIdx.x) % 16, share = int(threadIdx.x) / 16;
     float x = 0.0f;
     if (column < 2 * dim) {
 #pragma unroll 8
-        for (int b = share; b < count; b += 16) x += parts[int64_t(b) * 2 * dim + column];
+        for (int b = share; b < count; b += kJoinThreads / 16) x += parts[int64_t(b) * 2 * dim + column];
     }
     sh[threadIdx.x] = x;
     __syncthreads();
     if (share != 0 || column >= 2 * dim) return;
 #pragma unroll
-    for (int s = 1; s < 16; ++s) x += sh[s * 16 + int(threadIdx.x)];
+    for (int s = 1; s < kJoinThreads / 16; ++s) x += sh[s * 16 + int(threadIdx.x)];
     float* const out = column < dim ? dq : dk;
     if (out != nullptr) out[column < dim ? column : column - dim] = x;
 }
@@ -434,7 +436,7 @@ int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* g
     }
     if (weights)
         EHIP_LAUNCH("norm_rotate_backward_join", norm_rotate_join,
-                    dim3(unsigned(ceil_div(2 * a.dim, 16))), dim3(kThreads), 0, s, a.parts,
+                    dim3(unsigned(ceil_div(2 * a.dim, 16))), dim3(kJoinThreads), 0, s, a.parts,
                     desc->tokens > 0 ? int(blocks_of(a)) : 0, a.dim, dq_weight, dk_weight);
     return EHIP_OK;
 }
