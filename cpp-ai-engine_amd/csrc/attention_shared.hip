@@ -554,7 +554,7 @@ Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t g
     p.rows = p.by_rows ? 64 : 16;
     const int64_t row_tiles = rows / p.rows + groups;
     const bool waves = !p.by_rows;
-    const int tile = tile_of(waves, row_tiles, longest_shared);
+    const int tile = tile_of(true, row_tiles, longest_shared);
     const int64_t most = std::max<int64_t>(1, row_tiles * ceil_div(longest_shared, tile));
     const int64_t resident = waves ? 2048 : 512;
     p.shared = Cut{waves, tile,
