@@ -887,12 +887,12 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const int d0 = 4 * N * (8 * ks / N) + N * quarter + 8 * ks % N;
+                // With WIDE a head is a multiple of eight values, and one offset serves them all: those
+                // of each would be kept over the segments, in scratch.
+                const int from = WIDE && d0 < dim ? d0 : 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    // With WIDE a head is a multiple of eight values.
-                    const bool in = d0 + (WIDE ? 0 : e) < dim;
-                    qx[ks][e] = row[in ? d0 + e : 0];
-                }
+                for (int e = 0; e < 8; ++e)
+                    qx[ks][e] = row[WIDE ? from + e : d0 + e < dim ? d0 + e : 0];
             }
         };
         const auto split_query = [&] {

@@ -200,8 +200,9 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
             for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const int d = 32 * ks + 8 * quarter + e;
-                    y[ks][e] = from[d < dim ? d : 0];
+                    // With WIDE a head is a multiple of four values.
+                    const int d0 = 32 * ks + 8 * quarter + (WIDE ? e / 4 * 4 : e);
+                    y[ks][e] = from[(d0 < dim ? d0 : 0) + (WIDE ? e % 4 : 0)];
                 }
             find();
             load(begin);
