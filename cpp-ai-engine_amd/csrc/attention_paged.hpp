@@ -979,6 +979,7 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
                 for (int t = 0; t < 2; ++t) sc[t] *= scales(0, t);
             }
             if (tail) {
+                asm volatile("");  // a branch: as selects in every step, 16 instructions
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -997,7 +998,7 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
             float w[8], part_sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j % 4] - shift) * 0x1p-24f;
+                w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j % 4] - shift);
                 part_sum += w[j];
             }
             l = __builtin_fmaf(l, keep, part_sum);
@@ -1050,8 +1051,9 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
         if (bad) l = NAN;
         if (col < count && (bad || !(again >> col & 1))) {
             if (quarter == 0) {
-                if (!seg.whole) a.part_stats[at] = float2{m, l};
-                else if (a.lse != nullptr) a.lse[s * a.heads + h0 + col] = lse_of(m, l);
+                // As the other parts and sums, 2^-24 of what they are.
+                if (!seg.whole) a.part_stats[at] = float2{m, l * 0x1p-24f};
+                else if (a.lse != nullptr) a.lse[s * a.heads + h0 + col] = lse_of(m, l * 0x1p-24f);
             }
             float* const to = seg.whole ? a.out + s * a.ld_out + int64_t(h0 + col) * dim
                                         : a.part_out + at * dim;
@@ -1060,7 +1062,7 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
                 const int d = 16 * i + 4 * quarter;
                 floatx4u y;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[r] = seg.whole ? o[i][r] / l : o[i][r];
+                for (int r = 0; r < 4; ++r) y[r] = seg.whole ? o[i][r] / l : o[i][r] * 0x1p-24f;
                 if (d + (WIDE ? 0 : 3) < dim) {
                     *reinterpret_cast<floatx4u*>(to + d) = y;
                 } else if (!WIDE) {
