@@ -313,10 +313,10 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join(Paged a) {
 //
 // Of waves 2048, as many.
 Cut paged::cut_of(const Cache& c, int64_t heads, int64_t longest, int type) {
-    const bool waves = by_waves(c, type);
+    const bool waves = by_waves(type);
     const int64_t group = heads / c.kv_heads;
     const int64_t units =
-        c.kv_heads * ceil_div(group, waves || type != EHIP_CACHE_F32 ? 16 : kMaxGroup);
+        c.kv_heads * ceil_div(group, waves ? 16 : kMaxGroup);
     const int64_t resident = waves ? 2048 : 512;
     const int tile = tile_of(waves, c.sequences, longest);
     const int64_t most = std::max<int64_t>(1, c.sequences * ceil_div(longest, tile));
@@ -392,36 +392,35 @@ int read(const Read& x, hipStream_t s) {
     return EHIP_OK;
 }
 
-template <class T, int LPP, int G, bool VEC>
+template <int LPP, int G, bool VEC>
 int launch_part(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
     const int64_t blocks = a.workers * ceil_div(group, G) * a.c.kv_heads;
-    EHIP_LAUNCH("attention_paged", (paged_part<T, LPP, G, VEC>), dim3(unsigned(blocks)),
+    EHIP_LAUNCH("attention_paged", (paged_part<LPP, G, VEC>), dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 
-template <class T, int LPP, bool VEC>
+template <int LPP, bool VEC>
 int launch_group(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
-    if (group == 1) return launch_part<T, LPP, 1, VEC>(a, s);
-    if (group == 2) return launch_part<T, LPP, 2, VEC>(a, s);
-    if (group <= 4) return launch_part<T, LPP, 4, VEC>(a, s);
-    return launch_part<T, LPP, 8, VEC>(a, s);
+    if (group == 1) return launch_part<LPP, 1, VEC>(a, s);
+    if (group == 2) return launch_part<LPP, 2, VEC>(a, s);
+    if (group <= 4) return launch_part<LPP, 4, VEC>(a, s);
+    return launch_part<LPP, 8, VEC>(a, s);
 }
 
-template <class T, bool VEC>
+template <bool VEC>
 int launch_lanes(const Paged& a, hipStream_t s) {
-    constexpr int N = 16 / sizeof(T);
-    if (a.c.dim <= 32) return launch_group<T, 32 / N, VEC>(a, s);
-    if (a.c.dim <= 64) return launch_group<T, 64 / N, VEC>(a, s);
-    return launch_group<T, 128 / N, VEC>(a, s);
+    if (a.c.dim <= 32) return launch_group<8, VEC>(a, s);
+    if (a.c.dim <= 64) return launch_group<16, VEC>(a, s);
+    return launch_group<32, VEC>(a, s);
 }
 
 // 16-byte reads where every head's row begins at 16 bytes.
 int launch_parts_f32(const Paged& a, bool aligned, hipStream_t s) {
-    return aligned && a.c.dim % 4 == 0 ? launch_lanes<float, true>(a, s)
-                                       : launch_lanes<float, false>(a, s);
+    return aligned && a.c.dim % 4 == 0 ? launch_lanes<true>(a, s)
+                                       : launch_lanes<false>(a, s);
 }
 
 template <class T, int DP, bool WIDE>
@@ -446,9 +445,10 @@ int launch_parts_i8(const Paged& a, bool aligned, hipStream_t s) {
                                                               : launch_mfma<Int8, false>(a, s);
 }
 
-int launch_parts_bf16(const Paged& a, hipStream_t s) {
-    return by_waves(a.c, EHIP_CACHE_BF16) ? launch_mfma<Bf16, true>(a, s)
-                                          : launch_lanes<Bf16, false>(a, s);
+// Of 8 values in bf16.
+int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
+    return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16, true>(a, s)
+                                       : launch_mfma<Bf16, false>(a, s);
 }
 
 }  // namespace
@@ -456,7 +456,8 @@ int launch_parts_bf16(const Paged& a, hipStream_t s) {
 int paged::launch_parts(const Paged& a, int type, hipStream_t s) {
     const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
     if (type == EHIP_CACHE_F32) return launch_parts_f32(a, aligned, s);
-    return type == EHIP_CACHE_BF16 ? launch_parts_bf16(a, s) : launch_parts_i8(a, aligned, s);
+    return type == EHIP_CACHE_BF16 ? launch_parts_bf16(a, aligned, s)
+                                   : launch_parts_i8(a, aligned, s);
 }
 
 }  // namespace ehip

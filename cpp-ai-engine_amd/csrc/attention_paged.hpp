@@ -401,14 +401,14 @@ __device__ __forceinline__ float across(float x) {
 
 // One lane's values of a row as they are stored: 16 bytes, and its own first ones again in lanes
 // past the row's end.
-template <class T, bool VEC>
+template <bool VEC>
 struct Values {
-    static constexpr int N = 16 / int(sizeof(T));
+    static constexpr int N = 4;
     struct alignas(16) Pack {
-        T v[N];
+        float v[N];
     } x;
 
-    __device__ __forceinline__ void load(const T* row, int d0, int dim) {
+    __device__ __forceinline__ void load(const float* row, int d0, int dim) {
         if (VEC) {
             x = *reinterpret_cast<const Pack*>(row + (d0 < dim ? d0 : 0));
         } else {
@@ -416,12 +416,12 @@ struct Values {
             for (int e = 0; e < N; ++e) x.v[e] = row[d0 + e < dim ? d0 + e : 0];
         }
     }
-    __device__ __forceinline__ float operator[](int e) const { return widen(x.v[e]); }
+    __device__ __forceinline__ float operator[](int e) const { return x.v[e]; }
 };
 
-template <class T, int LPP, int G, bool VEC>
-__global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void paged_part(Paged a) {
-    constexpr int N = 16 / int(sizeof(T)), SUBS = 64 / LPP, TILE = SUBS * kUnroll;
+template <int LPP, int G, bool VEC>
+__global__ __launch_bounds__(kPagedThreads, G >= 4 ? 2 : 3) void paged_part(Paged a) {
+    constexpr int N = 4, SUBS = 64 / LPP, TILE = SUBS * kUnroll;
     __shared__ float sh_m[kPagedWaves][G], sh_l[kPagedWaves][G], sh_o[kPagedWaves][G][LPP * N];
     const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) / 64;
     const int kv_heads = int(a.c.kv_heads), dim = int(a.c.dim);
@@ -454,8 +454,8 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
                 o[g][e] = 0.0f;
             }
         }
-        const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
-        const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
+        const float* const k = static_cast<const float*>(a.c.k) + int64_t(kv) * dim;
+        const float* const v = static_cast<const float*>(a.c.v) + int64_t(kv) * dim;
         const int64_t pitch = int64_t(kv_heads) * dim;
         // The pool row of the tile's position `lane`.
         const auto row_of = [&](int p0) {
@@ -470,7 +470,7 @@ __global__ __launch_bounds__(kPagedThreads, G * sizeof(T) >= 16 ? 2 : 3) void pa
         };
         int row = int(row_of(begin + wave * TILE));
         for (int p0 = begin + wave * TILE; p0 < end; p0 += kPagedWaves * TILE) {
-            Values<T, VEC> ks[kUnroll], vs[kUnroll];
+            Values<VEC> ks[kUnroll], vs[kUnroll];
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const int64_t at = int64_t(__shfl(row, u * SUBS + sub)) * pitch;
@@ -719,29 +719,35 @@ struct Piece<Bf16, N, WIDE> {
     __device__ __forceinline__ void load(const Bf16* row, int d0, int dim) {
         if (WIDE) {
             x = *reinterpret_cast<const uintx4*>(row + (d0 < dim ? d0 : 0));
-        } else {
+        } else if (dim < 8) {
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
-                const uint32_t lo = row[d0 + e < dim ? d0 + e : 0].bits;
-                const uint32_t hi = row[d0 + e + 1 < dim ? d0 + e + 1 : 0].bits;
+                const uint32_t lo = d0 + e < dim ? row[d0 + e].bits : 0;
+                const uint32_t hi = d0 + e + 1 < dim ? row[d0 + e + 1].bits : 0;
                 x[e / 2] = lo | hi << 16;
             }
+        } else {
+            __builtin_memcpy(&x, row + min(d0, dim - 8), 16);
         }
     }
-    // With WIDE anything past the row's end.
+    // Past the row's end 0, or with WIDE anything.
     __device__ __forceinline__ uintx4 bf16(int, int d0, int dim) const {
-        if (WIDE) return x;
+        if (WIDE || dim < 8) return x;
+        uint64_t z[2];
+        __builtin_memcpy(z, &x, 16);
+        const int by = 16 * max(0, min(d0 - (dim - 8), 8)), low = by & 63;
+        const uint64_t both = z[0] >> low | z[1] << 1 << (63 - low), high = z[1] >> low;
+        z[0] = by < 64 ? both : by < 128 ? high : 0;
+        z[1] = by < 64 ? high : 0;
         uintx4 y;
-#pragma unroll
-        for (int e = 0; e < 8; e += 2)
-            y[e / 2] = d0 + e + 1 < dim ? x[e / 2] : d0 + e < dim ? x[e / 2] & 0xffffu : 0;
+        __builtin_memcpy(&y, z, 16);
         return y;
     }
 };
-// Other rows in 8 bits, of any length and at any address, are read eight at a time, the last eight
+// Other rows, of any length and at any address, are read eight values at a time, the last eight
 // where fewer are left. Those are shifted to their places where they are used: earlier, the read
-// would be waited for a tile ahead (64 sequences up to 8192, 32 heads over 8 of 128 values: 202
-// us against 85).
+// would be waited for a tile ahead (in 8 bits, 64 sequences up to 8192, 32 heads over 8 of 128
+// values, with reads like that: 202 us in place of 85).
 template <int N, bool WIDE>
 struct Piece<Int8, N, WIDE> {
     uint32_t x[N / 4];
@@ -1243,11 +1249,8 @@ struct Cut {
     int tile, workers;
 };
 
-// bf16 in rows of 16-byte units and 8 bits go by the matrix instructions.
-inline bool by_waves(const Cache& c, int type) {
-    return type == EHIP_CACHE_I8 || (type == EHIP_CACHE_BF16 && c.dim % 8 == 0 &&
-                                     aligned16(c.k) && aligned16(c.v));
-}
+// bf16 and 8 bits, exact in one part, go by the matrix instructions.
+inline bool by_waves(int type) { return type != EHIP_CACHE_F32; }
 // Positions that so many rows of work of at most `longest` are cut by.
 inline int tile_of(bool waves, int64_t rows, int64_t longest) {
     return waves && rows * ceil_div(longest, kWaveTile) <= INT32_MAX ? kWaveTile : kTile;

@@ -535,7 +535,7 @@ int check_groups(const char* name, const Cache& c, int64_t heads, int64_t groups
 // waves of their own (8 groups of 4000 shared positions and 100 own ones, 32 heads over 8 of 128,
 // us, waves : rows, for 8, 16, 32 and 64 rows; 8 bits 44 : 53, 49 : 52, 60 : 63, 82 : 72; bf16 54 :
 // 55, 63 : 56, 75 : 68, 98 : 81).
-bool by_rows(const Cache& c, int type, int64_t rows) { return !by_waves(c, type) || rows > 16; }
+bool by_rows(int type, int64_t rows) { return !by_waves(type) || rows > 16; }
 
 struct Plan {
     Cut own, shared;
@@ -551,7 +551,7 @@ Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t g
     Plan p{};
     p.own = cut_of(c, heads, longest, type);
     const int64_t rows = c.sequences * (heads / c.kv_heads);
-    p.by_rows = by_rows(c, type, groups > 0 ? rows / groups : 0);
+    p.by_rows = by_rows(type, groups > 0 ? rows / groups : 0);
     p.rows = p.by_rows ? 64 : 16;
     const int64_t row_tiles = rows / p.rows + groups;
     const bool waves = !p.by_rows;
@@ -584,12 +584,10 @@ int launch_rows_dim(const Paged& a, hipStream_t s) {
 }
 
 // Where the vector kernel takes the own positions: the shared ones before them.
-int launch_apart(const Paged& own, const Paged& a, int type, hipStream_t s) {
+int launch_apart(const Paged& own, const Paged& a, hipStream_t s) {
     const bool wide = aligned16(a.c.k) && aligned16(a.c.v) && a.c.dim % 4 == 0;
-    const int rc = type == EHIP_CACHE_BF16 ? launch_rows_dim<Bf16, false>(a, s)
-                   : wide                  ? launch_rows_dim<float, true>(a, s)
-                                           : launch_rows_dim<float, false>(a, s);
-    return rc != EHIP_OK ? rc : launch_parts(own, type, s);
+    const int rc = wide ? launch_rows_dim<float, true>(a, s) : launch_rows_dim<float, false>(a, s);
+    return rc != EHIP_OK ? rc : launch_parts(own, EHIP_CACHE_F32, s);
 }
 
 template <class T, int DP, bool WIDE, bool ROWS>
@@ -617,9 +615,12 @@ int launch_dim(const Paged& own, const Paged& a, bool rows, hipStream_t s) {
 }
 
 int launch_shared(const Paged& own, const Paged& a, int type, bool rows, hipStream_t s) {
-    if (!by_waves(a.c, type)) return launch_apart(own, a, type, s);
-    if (type == EHIP_CACHE_BF16) return launch_dim<Bf16, true>(own, a, rows, s);
-    const bool wide = aligned16(a.c.k) && aligned16(a.c.v) && a.c.dim % 16 == 0;
+    if (!by_waves(type)) return launch_apart(own, a, s);
+    const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
+    const bool wide = aligned && a.c.dim % (type == EHIP_CACHE_BF16 ? 8 : 16) == 0;
+    if (type == EHIP_CACHE_BF16)
+        return wide ? launch_dim<Bf16, true>(own, a, rows, s)
+                    : launch_dim<Bf16, false>(own, a, rows, s);
     return wide ? launch_dim<Int8, true>(own, a, rows, s) : launch_dim<Int8, false>(own, a, rows, s);
 }
 
