@@ -167,7 +167,8 @@ __device__ __forceinline__ void store_codes(Int8* row, int d0, int dim, uint32_t
     }
 }
 
-// In 8 bits: a wave a token, N lanes a key head, four values of k and of v each.
+// In 8 bits: a wave a token, N lanes a key head, four values of k and of v each (10060 tokens, 8
+// heads of 128: 39 us for 104 MB, 2.7 TB/s; vector instructions take 70 % of it).
 template <int N>
 __global__ __launch_bounds__(kAppendThreads) void cache_append_i8(
     Cache c, const float* __restrict__ k, int64_t ld_k, const float* __restrict__ v, int64_t ld_v,
@@ -231,7 +232,7 @@ __device__ __forceinline__ void load4(const Int8* from, float (&x)[4]) {
 }
 
 // Positions of the pools as rows: a wave a token. VEC: dim and the pools allow four values at a
-// time.
+// time (58430 positions, 8 heads of 128 in 8 bits: 122 us, 5.0 TB/s).
 template <class T, bool VEC>
 __global__ __launch_bounds__(kAppendThreads) void cache_read(
     Cache c, const int32_t* __restrict__ starts, const int32_t* __restrict__ cu, int tokens,
@@ -307,11 +308,8 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join(Paged a) {
 
 }  // namespace
 
-// Workers for 512 blocks in all, two a CU (64 sequences of 64 to 4096 positions in bf16: 75 us
-// against 85 with 1024 blocks and 101 with 2048; two of 131072 in fp32: 383, 388, 389), and no more
-// than there can be tiles.
-//
-// Of waves 2048, as many.
+// Workers for 512 blocks in all, two a CU (two sequences of 131072 in fp32: 383 us against 388 with
+// 1024 blocks and 389 with 2048), or as many of four waves, and no more than there can be tiles.
 Cut paged::cut_of(const Cache& c, int64_t heads, int64_t longest, int type) {
     const bool waves = by_waves(type);
     const int64_t group = heads / c.kv_heads;

@@ -593,8 +593,8 @@ __global__ __launch_bounds__(kPagedThreads, G >= 4 ? 2 : 3) void paged_part(Page
 // of an infinity, or an infinity times the parts of a finite value, is NaN where the product is an
 // infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time; a
 // score of NaN or +inf settles the head as NaN (64 sequences of 1024,
-// 32 heads over 8 of 128 values, us: finite 56, the first key NaN 59, the first value infinite 560;
-// value by value and to the end 1870 either way).
+// 32 heads over 8 of 128 values, us: finite 42, the first key NaN 105, the first value 557; value by
+// value and to the end 1870 either way).
 template <class T>
 __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int kv, int begin,
                                 int end, float& top, float& sum, float (&o)[2]) {
@@ -691,8 +691,9 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int k
 // A cache in bf16, up to 16 query heads of a key head at a time, on v_mfma_f32_16x16x32_bf16: the
 // cached values are operands as they are, q and the weights in three parts, so a score and a
 // weighted value take three products each, for any number of heads at one cost; by vector
-// instructions four heads ran at 4.3 TB/s of 5.4 and eight at 2.7. Lane l holds A(l % 16, 8 (l /
-// 16) + 0..7), B(8 (l / 16) + 0..7, l % 16) and D(4 (l / 16) + r, l % 16).
+// instructions four heads ran at 4.3 TB/s of 5.4 and eight at 2.7. HBM bounds it (64 sequences up
+// to 4096, 32 heads over 8 of 128: 265 MB in 49 us, 5.4 TB/s). Lane l holds A(l % 16, 8 (l / 16) +
+// 0..7), B(8 (l / 16) + 0..7, l % 16) and D(4 (l / 16) + r, l % 16).
 //   scores:  A = 16 positions by 32 values of K, as 16-byte reads leave them; B = q; D's columns
 //            are heads
 //   weights: the D's of positions 0..15 and 16..31 are the B of 32 positions, in the order
@@ -704,7 +705,9 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int k
 constexpr int kTilePositions = 32;
 
 // A cache in 8 bits goes the same way: whole numbers up to 127 are bf16 values, made of the bytes
-// in registers, a score is multiplied by its position's scale of K and a weight by that of V.
+// in registers, a score is multiplied by its position's scale of K and a weight by that of V. The
+// 1.5 instructions a value are a third of the kernel's (64 sequences up to 8192: 260 MB in 53 us, 4.9
+// TB/s).
 using attention::uintx4;
 typedef uint32_t uintx2 __attribute__((ext_vector_type(2)));
 
@@ -1125,7 +1128,7 @@ __device__ __forceinline__ Parts own_parts(const Paged& a, int64_t s, int h) {
 }
 
 // Row (s, h) of the results from its parts, by WAVES waves that take them in turn: one where the
-// rows fill the card, as each finds the parts' places by itself (2752 rows of some eleven parts: 9
+// rows fill the card, as each finds the parts' places by itself (2752 rows of some eleven parts: 10
 // us against 17 with four). Lane d has values d and d + 64. Every thread calls it.
 template <int WAVES>
 __device__ __forceinline__ void join_parts(const Paged& a, int64_t s, int h, const Parts (&p)[2],

@@ -8,7 +8,9 @@
 //
 // HBM bounds it: a head is read once, in registers of a few lanes, and written. The angles are
 // formed here, in 64 bits from the product to the quarter turn (a position of a million is some
-// 10^5 turns, whose fraction fp32 does not have), once for a wave's heads of a token.
+// 10^5 turns, whose fraction fp32 does not have), once for a wave's heads of a token. 369 MB of
+// query and key heads of 128 take 87 us, 4.2 TB/s; 134 MB of heads of 64 26 us, 5.2 TB/s, and back
+// 201 MB 44 us, 4.6 TB/s, with 5 for the weights' gradients.
 
 #include "common.hpp"
 
@@ -273,7 +275,8 @@ __global__ __launch_bounds__(kJoinThreads) void norm_rotate_join(const float* __
     float x = 0.0f;
     if (column < 2 * dim) {
 #pragma unroll 8
-        for (int b = share; b < count; b += kJoinThreads / 16) x += parts[int64_t(b) * 2 * dim + column];
+        for (int b = share; b < count; b += kJoinThreads / 16)
+            x += parts[int64_t(b) * 2 * dim + column];
     }
     sh[threadIdx.x] = x;
     __syncthreads();

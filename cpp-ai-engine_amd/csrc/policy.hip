@@ -9,10 +9,11 @@
 //
 // HBM bounds long batches, latency short ones. Over 2 million tokens of 2048 sequences with all
 // tensors the sums take 17 us (42 MB, 2.4 TB/s), joining them 7, the gradient 14 (50 MB, 3.5 TB/s);
-// the arithmetic of some 60 to 80 operations a token is not hidden by the loads altogether. The flat tokens are cut into chunks of kChunk and a
-// wave takes what one sequence has of one chunk, a segment. The segment of chunk c and sequence s
-// has place c + s, no other's: from one to the next at least one of them grows. So a wave finds its
-// segment by searching the offsets, without a list of them.
+// the arithmetic of some 60 to 80 operations a token is not hidden by the loads altogether. The
+// flat tokens are cut into chunks of kChunk and a wave takes what one sequence has of one chunk, a
+// segment. The segment of chunk c and sequence s has place c + s, no other's: from one to the next
+// at least one of them grows. So a wave finds its segment by searching the offsets, without a list
+// of them.
 
 #include "common.hpp"
 
@@ -138,8 +139,8 @@ __device__ __forceinline__ void load(const Policy& a, const Segment& g, int t, T
 }
 
 // A token's terms: T of the surrogate. The loss's sum takes 64 bits, as it has terms of both signs
-// (340 tokens' of about 1 have come to 10^-3; 17 us for the 14 of 32 bits), the gradient 32. Whether the ratio is clipped goes by
-// the difference in 64 bits.
+// (340 tokens' of about 1 have come to 10^-3; 17 us in place of the 14 in 32 bits), the gradient 32.
+// Whether the ratio is clipped goes by the difference in 64 bits.
 template <class T>
 struct Token {
     T ratio, surrogate, slope;  // slope: of the loss by the log probability
