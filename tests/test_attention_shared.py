@@ -152,6 +152,21 @@ def test_head_dims(hip, kind, d):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("d", [1, 2, 5, 8, 16, 31, 32, 40, 63, 65, 72, 96, 100, 127])
+def test_head_dims_of_many_rows(hip, kind, d):
+    check(hip, [(150, [3, 37] * 20), (97, [1] * 35)], 4, 2, d, 8, kind, seed=d)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [1, 3, 8, 64, 100])
+def test_pages_of_many_rows(hip, kind, page):
+    check(hip, [(n, [1, 2 * page] * 20) for n in (1, page + 1, 3 * page - 1, 129)], 4, 2, 64, page,
+          kind, seed=page)
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("groups", [[(5000, [1] * 3)], [(3000, [2000, 1] * 12), (1, [1, 1])],
                                     [(17, [1, 1])] * 40 + [(4096, [129] * 9)],
                                     [(1025, [1] * 100)]])
@@ -371,10 +386,11 @@ def test_strides_and_outputs(hip, kind):
 
 
 @gpu
-@pytest.mark.parametrize("kind", ["bfloat16", "int8"])
-def test_pools_at_any_address(hip, kind):
+@pytest.mark.parametrize("members", [3, 20, 80])
+@pytest.mark.parametrize("kind", KINDS)
+def test_pools_at_any_address(hip, kind, members):
     import torch
-    b, want, _ = check(hip, [(300, [3] * 20), (17, [1, 1])], 4, 2, 64, 16, kind, seed=15)
+    b, want, _ = check(hip, [(300, [3] * members), (17, [1, 1])], 4, 2, 64, 16, kind, seed=15)
     for name in ("kp", "vp"):
         pool = getattr(b, name)
         flat = torch.zeros(pool.numel() + 3, dtype=pool.dtype, device="cuda")
@@ -461,7 +477,7 @@ def test_odd_heads_that_are_not_finite(hip, kind, members, which):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("members", [3, 20])
+@pytest.mark.parametrize("members", [3, 80])
 def test_a_cache_past_32_bit_offsets(hip, kind, members):
     """The same pages at the end of pools of 2^31 values and more: the same bits."""
     import torch
