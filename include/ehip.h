@@ -1120,7 +1120,8 @@ int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* g
  * bits, if the table rows of a group lead to the same shared positions. Sequences
  * of no group, in a group of their own or shorter than what their group shares are
  * passed whole, as are the groups whose number is negative, past longest_shared or
- * past the table row. A page outside the pool among the shared positions makes the
+ * past the table row. Rows that meet an infinity, or a NaN among values, in shared
+ * positions are formed a second time, at some twenty times the cost. A page outside the pool among the shared positions makes the
  * rows of all that share them NaN. Group offsets out of range or descending are
  * clamped: nothing outside the tensors is read or written, but what the sequences
  * they touch get is unspecified.
