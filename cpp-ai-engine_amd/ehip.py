@@ -920,7 +920,7 @@ class Backend:
 
     def _cache(self, k_pages, v_pages, table, scales=None):
         torch = self.torch
-        self._here(k_pages, v_pages, table, *(scales or ()))
+        self._here(k_pages, v_pages, table, *(() if scales is None else scales))
         types = {torch.float32: 0, torch.bfloat16: 1, torch.int8: 2}
         if k_pages.dim() != 4 or k_pages.dtype not in types:
             raise ValueError("k_pages: expected float32, bfloat16 or int8 (pages, page_size, "
@@ -971,7 +971,7 @@ class Backend:
             raise ValueError("tokens: expected with cu")
         tokens = cache.sequences if cu is None else tokens
         shape = (tokens,) + tuple(k_pages.shape[2:])
-        self._here(starts, cu, *(out or ()))
+        self._here(starts, cu, *(() if out is None else out))
         if out is None:
             k, v = self.f32(shape), self.f32(shape)
             ld_k = ld_v = cache.kv_heads * cache.head_dim

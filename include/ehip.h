@@ -991,7 +991,8 @@ typedef struct {
  * token for each sequence (tokens = sequences). bf16 pools take the nearest
  * bf16, ties to even. A token whose position is negative, past its table row or
  * on a page outside the pool is not stored, nor are rows past the last
- * sequence. Two tokens for one place leave values of either, in any mixture. */
+ * sequence. Two tokens for one place leave values of either, in any mixture (in 8
+ * bits a number of one may be left with the scale of the other). */
 int ehip_cache_append_f32(const ehip_cache_t* cache, const float* k, int64_t ld_k,
                           const float* v, int64_t ld_v, const int32_t* starts,
                           const int32_t* cu, int64_t tokens, void* stream);

@@ -272,9 +272,11 @@ def test_group_offsets_that_are_none(hip, kind):
 
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
-def test_positions_past_the_lengths_do_not_reach_a_row(hip, kind):
+@pytest.mark.parametrize("d", [64, 33])
+@pytest.mark.parametrize("members", [2, 40])
+def test_positions_past_the_lengths_do_not_reach_a_row(hip, kind, d, members):
     import torch
-    b, want, _ = check(hip, [(40, [1, 2, 3]), (130, [5, 1])], 4, 2, 64, 16, kind, seed=10)
+    b, want, _ = check(hip, [(40, [1, 2, 3]), (130, [5, 1] * members)], 4, 2, d, 16, kind, seed=10)
     used = torch.zeros(b.kp.shape[:2], dtype=torch.bool, device="cuda")
     for s, n in enumerate(b.lengths):
         for p in range(n):

@@ -423,6 +423,22 @@ def test_many_sequences(hip, heads, kv, d):
 
 
 @gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_scales_and_outputs_in_one_tensor(hip, kind):
+    """A pair may be a tensor of two."""
+    import torch
+    print_case("cache pairs", kind)
+    lengths = [20, 3]
+    kp, vp, scales, table, k, v = fill(hip, lengths, 2, 32, 8, seed=17, kind=kind)
+    want = hip.cache_read(kp, vp, table, ints([0, 0]), offsets(lengths), 23, scales=scales)
+    both = torch.empty(2, 23, 2, 32, device="cuda")
+    got = hip.cache_read(kp, vp, table, ints([0, 0]), offsets(lengths), 23,
+                         scales=None if scales is None else torch.stack(scales), out=both)
+    assert torch.equal(both[0], want[0]) and torch.equal(both[1], want[1])
+    assert got[0].data_ptr() == both.data_ptr()
+
+
+@gpu
 def test_a_cache_past_32_bit_offsets(hip):
     """Written, read back and attended to at the end of pools of 2^31 values and more: the same bits
     as in small ones."""
