@@ -296,12 +296,13 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join(Paged a) {
         int64_t(blockIdx.x) * (kPagedWaves / WAVES) + int(threadIdx.x) / (64 * WAVES);
     if (at >= a.c.sequences * a.heads) return;
     const int64_t s = at / a.heads;
-    const int h = int(at % a.heads), n = length_of(a, s);
+    const Own own = own_of(a, s);
+    const int h = int(at % a.heads), n = length_from(a, own.length);
     if (n <= 0) {
         empty_row<WAVES>(a, s, h, n);
         return;
     }
-    const Parts p[2] = {own_parts(a, s, h), Parts{nullptr, nullptr, 0, 1}};
+    const Parts p[2] = {own_parts(a, own, s, h), Parts{nullptr, nullptr, 0, 1}};
     if (p[0].count == 1) return;  // the sequence was one segment
     join_parts<WAVES>(a, s, h, p, sh);
 }

@@ -134,11 +134,13 @@ constexpr int kTile = 128;      // of blocks
 constexpr int kWaveTile = 32;   // of waves
 
 // Positions of a sequence, -1 for a length that is none.
-__device__ __forceinline__ int length_of(const Paged& a, int64_t s) {
-    const int n = a.lengths[s];
+__device__ __forceinline__ int length_from(const Paged& a, int n) {
     return n < 0 || n > a.longest || n > a.c.width * a.c.page_size || (n > 0 && a.c.pages == 0)
                ? -1
                : n;
+}
+__device__ __forceinline__ int length_of(const Paged& a, int64_t s) {
+    return length_from(a, a.lengths[s]);
 }
 __device__ __forceinline__ int tiles_of(const Paged& a, int n) {
     return n > 0 ? int(uint32_t(n - 1) / uint32_t(a.tile)) + 1 : 0;
@@ -1117,14 +1119,22 @@ struct Parts {
     int64_t stride;
 };
 
+// What a sequence's own parts are found by, read at once, before any of it is used: a join is a
+// chain of reads.
+struct Own {
+    int length, start, tiles, first, end;
+};
+__device__ __forceinline__ Own own_of(const Paged& a, int64_t s) {
+    return Own{a.lengths[s], start_of(a, s), a.first[a.c.sequences], a.first[s], a.first[s + 1]};
+}
+
 // The sequence's own parts of a head (stats null: of none). One that is its only one is whole.
-__device__ __forceinline__ Parts own_parts(const Paged& a, int64_t s, int h) {
-    const int tiles = a.first[a.c.sequences], t0 = a.first[s], t1 = a.first[s + 1];
-    if (t0 == t1) return Parts{nullptr, nullptr, 0, 1};
-    const int w0 = worker_of(a, t0, tiles);
+__device__ __forceinline__ Parts own_parts(const Paged& a, const Own& x, int64_t s, int h) {
+    if (x.first == x.end) return Parts{nullptr, nullptr, 0, 1};
+    const int w0 = worker_of(a, x.first, x.tiles);
     const int64_t from = int64_t(h) * (a.workers + a.c.sequences) + w0 + s;
     return Parts{a.part_stats + from, a.part_out + from * a.c.dim,
-                 worker_of(a, t1 - 1, tiles) - w0 + 1, 1};
+                 worker_of(a, x.end - 1, x.tiles) - w0 + 1, 1};
 }
 
 // Row (s, h) of the results from its parts, by WAVES waves that take them in turn: one where the

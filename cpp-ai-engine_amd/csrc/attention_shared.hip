@@ -447,23 +447,25 @@ __device__ __forceinline__ int group_of(const int* cu, int groups, int s) {
 // The parts of rows, of their own and of the group's positions, where the row is not one part of its
 // own.
 template <int WAVES>
-__global__ __launch_bounds__(kPagedThreads) void shared_join(Paged own, Paged a) {
+__global__ __launch_bounds__(kPagedThreads) void shared_join(Paged own, Paged a,
+                                                             const int* __restrict__ group) {
     __shared__ float sh[WAVES][kMaxDim + 1];
     const int64_t at =
         int64_t(blockIdx.x) * (kPagedWaves / WAVES) + int(threadIdx.x) / (64 * WAVES);
     if (at >= a.c.sequences * a.heads) return;
     const int64_t s = at / a.heads;
-    const int h = int(at % a.heads), n = length_of(own, s), start = start_of(own, s);
+    const Own x = own_of(own, s);
+    const int g = group[s], group_rows = a.heads / int(a.c.kv_heads);
+    const int h = int(at % a.heads), n = length_from(own, x.length);
     if (n <= 0) {
         empty_row<WAVES>(a, s, h, n);
         return;
     }
-    Parts p[2] = {own_parts(own, s, h), Parts{nullptr, nullptr, 0, 1}};
-    if (start == 0 && p[0].count == 1) return;  // the sequence was one segment
-    if (start > 0) {
-        const int g = group_of(a.group_cu, a.groups, int(s));
-        const int group = a.heads / int(a.c.kv_heads), kv = h / group;
-        const int row = int(s - group_begin(a, g)) * group + h % group;
+    Parts p[2] = {own_parts(own, x, s, h), Parts{nullptr, nullptr, 0, 1}};
+    if (x.start == 0 && p[0].count == 1) return;  // the sequence was one segment
+    if (x.start > 0) {
+        const int kv = h / group_rows;
+        const int row = int(s - group_begin(a, g)) * group_rows + h % group_rows;
         const int tile = row / a.rows, each = tiles_of(a, shared_of(a, g));
         const int tiles = a.first[a.groups], t0 = a.first[g] + tile * each;
         const int w0 = worker_of(a, t0, tiles);
@@ -477,11 +479,12 @@ __global__ __launch_bounds__(kPagedThreads) void shared_join(Paged own, Paged a)
 
 // One block. The groups' offsets, in range and ascending whatever came in; what each shares, nothing
 // where it has no two sequences or the number is none that its table row could have; the sequences'
-// first own positions, 0 for those of no group or shorter than what theirs shares.
+// first own positions, 0 for those of no group or shorter than what theirs shares, and their groups.
 __global__ __launch_bounds__(kPlanThreads) void shared_plan(Paged a, const int32_t* group_cu,
                                                             const int32_t* shared,
                                                             int longest_shared, int* cu,
-                                                            int* counts, int* starts) {
+                                                            int* counts, int* starts,
+                                                            int* group) {
     __shared__ int sh[kPlanThreads / 64];
     const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) / 64;
     const int sequences = int(a.c.sequences);
@@ -511,12 +514,13 @@ __global__ __launch_bounds__(kPlanThreads) void shared_plan(Paged a, const int32
     }
     __syncthreads();
     for (int s = int(threadIdx.x); s < sequences; s += kPlanThreads) {
-        int start = 0;
+        int start = 0, g = 0;
         if (a.groups > 0) {
-            const int g = group_of(cu, a.groups, s);
+            g = group_of(cu, a.groups, s);
             if (cu[g] <= s && s < cu[g + 1] && length_of(a, s) >= counts[g]) start = counts[g];
         }
         starts[s] = start;
+        group[s] = g;
     }
 }
 
@@ -569,9 +573,9 @@ Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t g
     p.part_bytes = round16(size_t(c.kv_heads) * size_t(p.places) * size_t(p.rows) *
                            (sizeof(float2) + size_t(c.dim) * sizeof(float)));
     // The parts of both; the groups' first tiles, offsets and shared positions, and the sequences'
-    // own starts.
+    // own starts and groups.
     p.first_bytes = round16(size_t(groups + 1) * sizeof(int));
-    p.bytes = p.own_bytes + p.part_bytes + 3 * p.first_bytes + size_t(c.sequences) * sizeof(int);
+    p.bytes = p.own_bytes + p.part_bytes + 3 * p.first_bytes + 2 * size_t(c.sequences) * sizeof(int);
     return p;
 }
 
@@ -698,12 +702,13 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     int* const cu = reinterpret_cast<int*>(at + p.first_bytes);
     int* const counts = reinterpret_cast<int*>(at + 2 * p.first_bytes);
     int* const starts = reinterpret_cast<int*>(at + 3 * p.first_bytes);
+    int* const of = starts + c.sequences;
     a.group_cu = cu;
     a.shared = counts;
     own.starts = starts;
     hipStream_t s = as_stream(stream);
     EHIP_LAUNCH("attention_shared_plan", shared_plan, dim3(1), dim3(kPlanThreads), 0, s, a,
-                group_cu, shared, int(longest_shared), cu, counts, starts);
+                group_cu, shared, int(longest_shared), cu, counts, starts, of);
     if (groups > 0) {
         if (int rc = launch_shared(own, a, cache->type, p.by_rows, s)) return rc;
     } else {
@@ -713,10 +718,10 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     if (join_waves(rows) == 1)
         EHIP_LAUNCH("attention_shared_join", shared_join<1>,
                     dim3(unsigned(ceil_div(rows, kPagedWaves))), dim3(kPagedThreads), 0, s, own,
-                    a);
+                    a, of);
     else
         EHIP_LAUNCH("attention_shared_join", shared_join<kPagedWaves>, dim3(unsigned(rows)),
-                    dim3(kPagedThreads), 0, s, own, a);
+                    dim3(kPagedThreads), 0, s, own, a, of);
     return EHIP_OK;
 }
 
