@@ -42,8 +42,10 @@ struct Args {
     const int32_t* positions;
     const double* freqs;
     float eps;
+    int64_t tokens;
     int per, chunks;  // heads of a wave, shares of a token
-    int64_t units;    // tokens * chunks
+    int each;         // tokens of a wave, where it holds several tokens' heads at a time
+    int64_t units;    // waves' worth of work
     float* parts;     // (blocks, 2, dim): shares of the weights' gradients
 };
 
@@ -162,8 +164,9 @@ __device__ __forceinline__ float head_sum(float x) {
     return x;
 }
 
-// A wave has `per` heads of a token, 64 / G at a time, each in G lanes of eight values. The lanes
-// of a head read all of it before they write, so the output may be the input.
+// A wave has `per` heads of a token, 64 / G at a time, each in G lanes of eight values, or all heads
+// of several tokens. The lanes of a head read all of it before they write, so the output may be the
+// input.
 template <int G, bool BACK>
 __global__ __launch_bounds__(kThreads) void norm_rotate(Args a) {
     constexpr int kSlots = 64 / G;
@@ -171,27 +174,27 @@ __global__ __launch_bounds__(kThreads) void norm_rotate(Args a) {
     const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) / 64);
     const int slot = lane / G, u = lane % G;
     const Places p = places(a, u);
+    const int sub = a.each > 1 ? slot / a.total_heads : 0;  // the slot's token and head
+    const int head = slot - sub * a.total_heads;
     const float each = 1.0f / float(a.dim);
     float dw[2][8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) dw[0][e] = dw[1][e] = 0.0f;
     for (int64_t unit = int64_t(blockIdx.x) * kWaves + wave; unit < a.units;
          unit += int64_t(gridDim.x) * kWaves) {
-        const int64_t t = unit / a.chunks;
+        const int64_t t = unit / a.chunks * a.each + sub;
         const int first = int(unit % a.chunks) * a.per;
-        const int end = min(first + a.per, a.total_heads);
+        const int end = sub < a.each && t < a.tokens ? min(first + a.per, a.total_heads) : 0;
         float cosine[4], sine[4];
         if (a.half > 0) {
-            const double at = double(a.positions[t]);
+            const double at = double(a.positions[t < a.tokens ? t : a.tokens - 1]);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int i = 4 * u + j;
                 sine_cosine(at * a.freqs[i < a.half ? i : 0], sine[j], cosine[j]);
             }
         }
-        for (int h0 = first; h0 < end; h0 += kSlots) {
-            const int h = h0 + slot;
-            if (h >= end) continue;
+        for (int h = first + head; h < end; h += kSlots) {
             const bool key = h >= a.heads;
             // Chosen field by field: a reference to either would be read through memory.
             const Side side{key ? a.k.x : a.q.x,         key ? a.k.grad : a.q.grad,
@@ -339,7 +342,12 @@ Args arguments(const ehip_norm_rotate_t* d) {
     const int64_t want = std::min(most, ceil_div(4096, std::max<int64_t>(1, d->tokens)));
     a.per = int(ceil_div(most, want)) * slots;
     a.chunks = int(ceil_div(a.total_heads, a.per));
-    a.units = d->tokens * a.chunks;
+    // Tokens whose heads leave half of a wave or more without work share it (65536 tokens, us, a
+    // wave a token : like this; two heads of 24 values 43 : 13, of 64 44 : 17, of 128 44 : 29; four
+    // of 64 with the gradient 114 : 75).
+    a.each = std::max(1, slots / a.total_heads);
+    a.tokens = d->tokens;
+    a.units = ceil_div(d->tokens, a.each) * a.chunks;
     return a;
 }
 

@@ -261,13 +261,41 @@ def test_parts_that_are_not_asked_for(hip):
     alone, none = hip.norm_rotate(q, None, at, freqs, wq)
     assert none is None and torch.equal(alone, outs[0])
     part = hip.norm_rotate_backward(grads[0], None, q, None, at, freqs, wq)
-    assert torch.equal(part[0], got[0]) and torch.equal(part[2], got[2])
+    assert torch.equal(part[0], got[0])
     assert part[1] is None and part[3] is None
+    # How tokens are spread over waves goes by the heads of both, so a weight's gradient may be added
+    # up in another order: n numbers in any order are off by (n - 1) U of the sum of their sizes,
+    # which the formula's bound counts as (n + 8) U.
+    angle = at.cpu().double()[:, None] * freqs.cpu()[None, :]
+    value, bound = formula(q.cpu().double(), wq.cpu().double(), angle, 32, False, 1e-6,
+                           grads[0].cpu().double())
+    within(part[2], value["dw"], bound["dw"], "dq_weight")
     for skip in range(4):
         want = [i != skip for i in range(4)]
         part = hip.norm_rotate_backward(*grads, *what, want=want)
         assert part[skip] is None
         assert all(torch.equal(part[i], got[i]) for i in range(4) if i != skip)
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens", [1, 2, 7, 8, 9, 63, 65, 1000])
+@pytest.mark.parametrize("h,kv,d", [(1, 0, 8), (1, 1, 24), (2, 1, 64), (1, 2, 32), (3, 2, 16),
+                                    (1, 1, 128), (5, 3, 20), (1, 0, 256)])
+def test_tokens_that_share_a_wave(hip, h, kv, d, tokens, interleaved):
+    if kv > 0:
+        check(hip, tokens, h, kv, d, d // 2 * 2, interleaved, seed=tokens)
+        return
+    what, grads = make(tokens, h, 1, d, d // 2 * 2, seed=tokens)
+    q, _, at, freqs, wq, _ = what
+    out, _ = hip.norm_rotate(q, None, at, freqs, wq, interleaved=interleaved)
+    got = hip.norm_rotate_backward(grads[0], None, q, None, at, freqs, wq, interleaved=interleaved)
+    angle = at.cpu().double()[:, None] * freqs.cpu()[None, :]
+    value, bound = formula(q.cpu().double(), wq.cpu().double(), angle, d // 2 * 2, interleaved,
+                           1e-6, grads[0].cpu().double())
+    within(out, value["out"], bound["out"], "out")
+    within(got[0], value["dx"], bound["dx"], "dx")
+    within(got[2], value["dw"], bound["dw"], "dw")
 
 
 @gpu
