@@ -795,6 +795,15 @@ struct Piece<Int8, N, WIDE> {
     }
 };
 
+// The power of two that a query row's products run without, of its largest |value|. In 8 bits they are
+// sums of q times whole numbers of up to 127, which the position's scale multiplies only then: from
+// 2^113 on they could pass fp32 where the score does not. Scores are multiplied by it where the
+// maximum is taken and, in one step with the shift, before the exponential.
+template <class T>
+__device__ __forceinline__ float range_of(float largest) {
+    return sizeof(T) == 1 && largest > 0x1p100f ? 0x1p32f : 1.0f;
+}
+
 constexpr int value_pitch(int dp) { return 2 * dp + 32; }  // bytes of a row of V in LDS
 template <int DP>
 struct alignas(16) PartLds {
@@ -840,7 +849,7 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
         floatx4 o[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-        float m = -INFINITY, l = 0.0f;
+        float m = -INFINITY, l = 0.0f, range = 1.0f;
 
         const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
         const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
@@ -907,6 +916,7 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
             }
         };
         const auto split_query = [&] {
+            float largest = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const int d0 = 4 * N * (8 * ks / N) + N * quarter + 8 * ks % N;
@@ -914,7 +924,14 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
                 for (int e = 0; e < 8; ++e) {
                     const bool in = d0 + (WIDE ? 0 : e) < dim;
                     qx[ks][e] = in && col < count ? qx[ks][e] * c2 : 0.0f;
+                    largest = fmaxf(largest, fabsf(qx[ks][e]));
                 }
+            }
+            range = range_of<T>(largest_of_rows(largest));
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) qx[ks][e] *= 1.0f / range;
                 attention::split8(qx[ks], q[ks]);
             }
         };
@@ -997,19 +1014,19 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
                     for (int r = 0; r < 4; ++r)
                         if (p0 + 16 * t + 4 * quarter + r >= end) sc[t][r] = -INFINITY;
             }
-            float top = m;
+            float top = sc[0][0];
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) top = fmaxf(top, sc[t][r]);
-            top = largest_of_rows(top);
+            top = fmaxf(m, largest_of_rows(top) * range);
             const float shift = top == -INFINITY ? 0.0f : top;
             const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
             m = top;
             float w[8], part_sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                w[j] = __builtin_amdgcn_exp2f(sc[j / 4][j % 4] - shift);
+                w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j / 4][j % 4], range, -shift));
                 part_sum += w[j];
             }
             l = __builtin_fmaf(l, keep, part_sum);

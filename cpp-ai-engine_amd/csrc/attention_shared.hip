@@ -195,6 +195,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
         };
         ask(begin);
         bf16x8 q[KS][3];
+        float range = 1.0f;
         {
             const float* const from = query_row<true>(a, seg, kv, 0, mine < count ? mine : 0);
             float y[KS][8];
@@ -209,13 +210,21 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
             find();
             load(begin);
             ask(begin + kKeys);
+            float largest = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int d = 32 * ks + 8 * quarter + e;
                     y[ks][e] = d < dim && mine < count ? y[ks][e] * c2 : 0.0f;
+                    largest = fmaxf(largest, fabsf(y[ks][e]));
                 }
+            }
+            range = range_of<T>(largest_of_rows(largest));
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[ks][e] *= 1.0f / range;
                 attention::split8(y[ks], q[ks]);
             }
         }
@@ -266,7 +275,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                                                                         sc[t], 0, 0, 0);
                     keep_order();
                 }
-                float w[8], top = m;
+                float w[8];
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     sc[t] += small[t];
@@ -280,16 +289,17 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                     for (int j = 0; j < 8; ++j)
                         if (p0 + 16 * (j / 4) + 4 * quarter + j % 4 >= end) w[j] = -INFINITY;
                 }
+                float top = w[0];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) top = fmaxf(top, w[j]);
-                top = largest_of_rows(top);
+                for (int j = 1; j < 8; ++j) top = fmaxf(top, w[j]);
+                top = fmaxf(m, largest_of_rows(top) * range);
                 const float shift = top == -INFINITY ? 0.0f : top;
                 const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
                 m = top;
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    w[j] = __builtin_amdgcn_exp2f(w[j] - shift);
+                    w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[j], range, -shift));
                     sum += w[j];
                 }
                 l = __builtin_fmaf(l, keep, sum);

@@ -448,6 +448,23 @@ def test_small_and_large_scales(hip, power, members):
 
 
 @gpu
+@pytest.mark.parametrize("members", [3, 40])
+@pytest.mark.parametrize("power", [113, 118, 120, 122, 126])
+def test_large_queries_and_small_scales(hip, power, members):
+    """Queries times the whole numbers of a cache in 8 bits alone are past fp32, the scores are not."""
+    print_case("shared large q", power, members)
+    b = Batch(hip, [(300, [2] * members), (40, [1, 1])], 4, 2, 64, 16, "int8", seed=22)
+    b.scales[0].mul_(2.0 ** -power)
+    b.q.mul_(2.0 ** power)
+    b.kp[:, :, 0].abs_()
+    b.q[::2, 0] = -b.q[::2, 0].abs()  # sums far below zero alone
+    out, lse = b.run(hip)
+    value, bound = b.expect()
+    within(out, value["out"], bound["out"], "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
+@gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("members", [3, 40])
 @pytest.mark.parametrize("which", ["k", "v"])

@@ -415,6 +415,29 @@ def test_small_and_large_values(hip, power):
 
 
 @gpu
+@pytest.mark.parametrize("d", [24, 64, 100, 128])
+@pytest.mark.parametrize("power", [100, 113, 118, 120, 122, 126])
+def test_large_queries_and_small_scales(hip, power, d):
+    """Queries times the whole numbers alone are past fp32, the scores are not. The scales are taken as
+    they are held, of few bits where they are subnormal; powers of two add no rounding."""
+    import torch
+    print_case("paged8 large q", power, d)
+    lengths = [300, 7]
+    kp, vp, scales, table, _, _ = fill(hip, lengths, 2, d, 16, seed=9)
+    scales[0].mul_(2.0 ** -power)
+    gen = torch.Generator(device="cuda").manual_seed(power)
+    q = torch.randn(2, 4, d, generator=gen, device="cuda") * 2.0 ** power
+    q[1, 0].abs_()
+    kp[:, :, 0].abs_()
+    q[0, 0] = -q[0, 0].abs()  # sums far below zero alone
+    out, lse = hip.attention_paged(q, kp, vp, table, ints(lengths), scales=scales)
+    value, bound = reference(q, held(kp, scales[0], table, lengths),
+                             held(vp, scales[1], table, lengths), lengths, d ** -0.5)
+    within(out, value["out"], bound["out"], "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
+@gpu
 @pytest.mark.parametrize("heads,kv,d", [(4, 4, 64), (8, 2, 128), (3, 1, 33)])
 def test_many_sequences(hip, heads, kv, d):
     """More than a wave has lanes, of uneven lengths, some empty."""
