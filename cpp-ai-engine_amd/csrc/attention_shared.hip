@@ -195,7 +195,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
         };
         ask(begin);
         bf16x8 q[KS][3];
-        float range = 1.0f;
+        uint64_t apart = 0;  // rows for the formula
         {
             const float* const from = query_row<true>(a, seg, kv, 0, mine < count ? mine : 0);
             float y[KS][8];
@@ -216,15 +216,15 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int d = 32 * ks + 8 * quarter + e;
-                    y[ks][e] = d < dim && mine < count ? y[ks][e] * c2 : 0.0f;
+                    y[ks][e] = d < dim && mine < count ? y[ks][e] : 0.0f;
                     largest = fmaxf(largest, fabsf(y[ks][e]));
                 }
             }
-            range = range_of<T>(largest_of_rows(largest));
+            apart = __ballot(out_of_parts<T>(largest_of_rows(largest) * fabsf(c2)));
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[ks][e] *= 1.0f / range;
+                for (int e = 0; e < 8; ++e) y[ks][e] *= c2;
                 attention::split8(y[ks], q[ks]);
             }
         }
@@ -275,7 +275,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                                                                         sc[t], 0, 0, 0);
                     keep_order();
                 }
-                float w[8];
+                float w[8], top = m;
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
                     sc[t] += small[t];
@@ -289,17 +289,16 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                     for (int j = 0; j < 8; ++j)
                         if (p0 + 16 * (j / 4) + 4 * quarter + j % 4 >= end) w[j] = -INFINITY;
                 }
-                float top = w[0];
 #pragma unroll
-                for (int j = 1; j < 8; ++j) top = fmaxf(top, w[j]);
-                top = fmaxf(m, largest_of_rows(top) * range);
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, w[j]);
+                top = largest_of_rows(top);
                 const float shift = top == -INFINITY ? 0.0f : top;
                 const float keep = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - shift);
                 m = top;
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    w[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(w[j], range, -shift));
+                    w[j] = __builtin_amdgcn_exp2f(w[j] - shift);
                     sum += w[j];
                 }
                 l = __builtin_fmaf(l, keep, sum);
@@ -377,7 +376,7 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) fine = fine && fabsf(o[i][r]) < INFINITY;
-        const uint64_t lanes = __ballot(!fine && mine < count);
+        const uint64_t lanes = __ballot(!fine && mine < count) | apart;
         uint32_t again = uint32_t(lanes | lanes >> 32);
         again = (again | again >> 16) & 0xffffu;
         again = __builtin_amdgcn_readfirstlane(bad ? 0u : again);

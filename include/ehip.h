@@ -1011,14 +1011,17 @@ int ehip_cache_read_f32(const ehip_cache_t* cache, const int32_t* starts, const 
  * lengths[s] - 1 (a DEVICE array; write the new token's key and value first).
  * out and lse (sequences, heads; may be NULL) as in ehip_attention_packed_f32,
  * but that small values keep fewer bits: sums run on 2^-24 of a weight, and out
- * may be off by another lengths[s] * 2^-123 (in 8 bits 2^-100). They may not overlap the inputs. A
+ * may be off by another lengths[s] * 2^-123 (in 8 bits 2^-100); in bf16 and 8
+ * bits scale q is taken to 2^-134, and a score may be off by that times the sum
+ * of its |k|. They may not overlap the inputs. A
  * length of zero gives out = 0, lse = -inf. A negative length, one past
  * `longest` or its table row, or a page outside the pool makes the sequence's
  * row NaN instead of a read out of bounds.
  * `longest`, a host value of at most 2^30, is what the work is split by: the
  * same lengths under another `longest` may differ in the last bits.
  * 1 <= head_dim <= 128, heads a multiple of kv_heads. Heads of a cache in bf16
- * or 8 bits that meet an infinity are formed a second time, at some ten times the cost.
+ * or 8 bits that meet an infinity, whose |scale q| are all below 2^-101, or in 8
+ * bits one past 2^111, are formed a second time, at some ten times the cost.
  * `workspace` (16-byte aligned) holds the parts of split lengths during the
  * call: at least ehip_attention_paged_workspace() bytes, of the call's own.
  * Deterministic. */
@@ -1118,12 +1121,16 @@ int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* g
  * through the table row of its first sequence, the others through each
  * sequence's own, so what a page holds of both may be there twice. The result is
  * that of ehip_attention_paged_f32 with the rest of its arguments, up to the last
- * bits, if the table rows of a group lead to the same shared positions. Sequences
+ * bits, if the table rows of a group lead to the same shared positions (that of
+ * the first sequence also where that one's length is none or shorter). In fp32 too
+ * scale q is taken to 2^-134 there, as are the keys: a score may be off by that
+ * times the sums of its |k| and |scale q|. Sequences
  * of no group, in a group of their own or shorter than what their group shares are
  * passed whole, as are the groups whose number is negative, past longest_shared or
  * past the table row. Rows that meet an infinity, or a NaN among values, in shared
- * positions are formed a second time, at some twenty times the cost. A page outside the pool among the shared positions makes the
- * rows of all that share them NaN. Group offsets out of range or descending are
+ * positions, or whose q is as small or large as named there, are formed a second
+ * time, at some twenty times the cost. A page outside the pool among the shared
+ * positions makes the rows of all that share them NaN. Group offsets out of range or descending are
  * clamped: nothing outside the tensors is read or written, but what the sequences
  * they touch get is unspecified.
  * `workspace` (16-byte aligned) holds the parts during the call: at least

@@ -399,6 +399,28 @@ def test_small_values(hip, power, dtype, d):
 
 @gpu
 @pytest.mark.parametrize("dtype", types())
+@pytest.mark.parametrize("d", [33, 64, 100, 128])
+@pytest.mark.parametrize("power", [100, 104, 110, 118, 124])
+def test_small_queries_and_large_keys(hip, power, d, dtype):
+    """Scores of ordinary size from queries whose parts in bf16 would lose bits. Where q times the scale
+    and log2 e is subnormal it is off by 2^-150 a value; the bound has (d + 4) 2^-24 of |scale q|, at
+    2^-124 some (d + 4) 2^-151 on average: 18 times that for 33 values, more for others."""
+    import torch
+    print_case("paged small q", power, d, dtype)
+    lengths = [300, 7]
+    kp, vp, table, k, v = make(lengths, 2, d, 16, dtype, seed=12)
+    kp.mul_(2.0 ** power)
+    k = [x * 2.0 ** power for x in k]
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    q = torch.randn(2, 4, d, generator=gen, device="cuda") * 2.0 ** -power
+    out, lse = hip.attention_paged(q, kp, vp, table, ints(lengths), scale=0.125)
+    value, bound = reference(q, k, v, lengths, 0.125)
+    within(out, value["out"], bound["out"], "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", types())
 @pytest.mark.parametrize("heads,kv,d", [(17, 1, 64), (33, 1, 32), (40, 2, 128), (64, 2, 40)])
 def test_groups_over_several_blocks(hip, dtype, heads, kv, d):
     """More query heads a key head than a block takes at a time."""

@@ -467,6 +467,25 @@ def test_large_queries_and_small_scales(hip, power, members):
 @gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("members", [3, 40])
+@pytest.mark.parametrize("power", [100, 104, 110, 118, 124])
+def test_small_queries_and_large_keys(hip, power, members, kind):
+    """Scores of ordinary size from queries whose parts in bf16 would lose bits."""
+    print_case("shared small q", power, members, kind)
+    b = Batch(hip, [(300, [2] * members), (40, [1, 1])], 4, 2, 64, 16, kind, seed=23)
+    b.q.mul_(2.0 ** -power)
+    if kind == "int8":
+        b.scales[0].mul_(2.0 ** power)
+    else:
+        b.kp.mul_(2.0 ** power)
+    out, lse = b.run(hip)
+    value, bound = b.expect()
+    within(out, value["out"], bound["out"], "out")
+    within(lse, value["lse"], bound["lse"], "lse")
+
+
+@gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("members", [3, 40])
 @pytest.mark.parametrize("which", ["k", "v"])
 def test_odd_heads_that_are_not_finite(hip, kind, members, which):
     """Heads whose rows begin at any address, formed a second time: a NaN key or scale of the shared
