@@ -88,17 +88,20 @@ __device__ __forceinline__ Segment segment_of(const Policy& a, int64_t place) {
     return g;
 }
 
-// exp(x) - x - 1 and exp(x) - 1. Below one in magnitude by the series of the first, whose next term
-// is 2^-36 of it, as the difference would have few digits.
-__device__ __forceinline__ void kl_terms(float x, float& kl, float& rise) {
+// exp(x) - x - 1 below one in magnitude, by its series, whose next term is 2^-35 of it: the difference
+// would have few digits.
+__device__ __forceinline__ float kl_series(float x) {
     float s = 1.0f;
 #pragma unroll
     for (int n = 13; n >= 3; --n) s = __builtin_fmaf(x * (1.0f / float(n)), s, 1.0f);
-    const float e = expf(x);
-    const bool small = fabsf(x) < 1.0f;
-    kl = small ? 0.5f * x * x * s : e - 1.0f - x;
-    rise = small ? x + kl : e - 1.0f;
-    if (fabsf(x) == INFINITY) kl = INFINITY;
+    return 0.5f * x * x * s;
+}
+// The same of any x, past fp32 too, whose exponential is the square of that of its half.
+__device__ __forceinline__ double kl_of(float x) {
+    const double h = double(expf(0.5f * x));
+    const double kl = __builtin_fma(h, h, -1.0) - double(x);
+    if (fabsf(x) == INFINITY) return INFINITY;
+    return fabsf(x) < 1.0f ? double(kl_series(x)) : kl;
 }
 
 // exp(x): 2^n exp(f), |f| <= ln 2 / 2, by Taylor's series, whose next term is 2^-37 of it. A third of
@@ -138,35 +141,42 @@ __device__ __forceinline__ void load(const Policy& a, const Segment& g, int t, T
     for (int i = 0; i < kBatch; ++i) x.counts[i] = mask[i] != 0 && t + 64 * i < g.end;
 }
 
-// A token's terms: T of the surrogate. The loss's sum takes 64 bits, as it has terms of both signs
-// (340 tokens' of about 1 have come to 10^-3; 17 us in place of the 14 in 32 bits), the gradient 32.
 // Whether the ratio is clipped goes by the difference in 64 bits.
-template <class T>
+__device__ __forceinline__ bool clipped(const Policy& a, double d, float advantage) {
+    return advantage < 0.0f ? d < a.log_low : d > a.log_high;
+}
+
+// A token's terms. The loss's sum takes 64 bits, as it has terms of both signs (340 tokens' of about 1
+// have come to 10^-3; 17 us in place of the 14 in 32 bits).
 struct Token {
-    T ratio, surrogate, slope;  // slope: of the loss by the log probability
-    float kl;
+    double ratio, surrogate, kl;
     bool clipped;
 };
 
-__device__ __forceinline__ float exp_of(double x, float) { return expf(float(x)); }
-__device__ __forceinline__ double exp_of(double x, double) { return exp36(x); }
-
-template <class T>
-__device__ __forceinline__ Token<T> token_of(const Policy& a, const Tokens& from, int i) {
-    Token<T> x;
-    const float p = from.p[i], advantage = from.advantage[i];
-    const double d = double(p) - double(from.old[i]);
-    x.ratio = exp_of(d, T());
-    x.clipped = advantage < 0.0f ? d < a.log_low : d > a.log_high;
-    x.surrogate = (x.clipped ? T(advantage < 0.0f ? a.low : a.high) : x.ratio) * T(advantage);
-    x.slope = x.clipped ? T(0) : -x.ratio * T(advantage);
-    x.kl = 0.0f;
-    if (a.ref != nullptr) {
-        float rise;
-        kl_terms(float(double(from.ref[i]) - double(p)), x.kl, rise);
-        if (a.kl_weight != 0.0f) x.slope -= T(a.kl_weight * rise);
-    }
+__device__ __forceinline__ Token token_of(const Policy& a, const Tokens& from, int i) {
+    Token x;
+    const float advantage = from.advantage[i];
+    const double d = double(from.p[i]) - double(from.old[i]);
+    x.ratio = exp36(d);
+    x.clipped = clipped(a, d, advantage);
+    x.surrogate = (x.clipped ? (advantage < 0.0f ? a.low : a.high) : x.ratio) * double(advantage);
+    x.kl = a.ref != nullptr ? kl_of(float(double(from.ref[i]) - double(from.p[i]))) : 0.0;
     return x;
+}
+
+// The gradient of a token of weight w by its log probability, in 32 bits. An exponential past fp32, or
+// below its normal numbers, may not be once it has the weight: the weight takes the square root twice.
+__device__ __forceinline__ float gradient_of(const Policy& a, const Tokens& from, int i, float w) {
+    const float advantage = from.advantage[i];
+    const double d = double(from.p[i]) - double(from.old[i]);
+    const float h = expf(0.5f * float(d));
+    float y = clipped(a, d, advantage) ? 0.0f : -(w * advantage * h * h);
+    if (a.ref != nullptr && a.kl_weight != 0.0f) {
+        const float x = float(double(from.ref[i]) - double(from.p[i])), r = expf(0.5f * x);
+        const float by = w * a.kl_weight;
+        y -= fabsf(x) < 1.0f ? by * (x + kl_series(x)) : by * r * r - by;
+    }
+    return y;
 }
 
 template <class T>
@@ -188,15 +198,14 @@ __device__ __forceinline__ void sum_segment(const Policy& a, int64_t place, Sums
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
             if (t + 64 * i >= g.end) break;
-            const Token<double> y = token_of<double>(a, all, i);
+            const Token y = token_of(a, all, i);
             double loss = -y.surrogate;
-            if (a.kl_weight != 0.0f)
-                loss = __builtin_fma(double(a.kl_weight), double(y.kl), loss);
+            if (a.kl_weight != 0.0f) loss = __builtin_fma(double(a.kl_weight), y.kl, loss);
             if (a.entropy_weight != 0.0f)
                 loss = __builtin_fma(-double(a.entropy_weight), double(all.entropy[i]), loss);
             const bool counts = all.counts[i];
             x.loss += counts ? loss : 0.0;
-            x.kl += counts ? double(y.kl) : 0.0;
+            x.kl += counts ? y.kl : 0.0;
             x.ratio += counts ? y.ratio : 0.0;
             x.clipped += counts && y.clipped;
             x.tokens += counts;
@@ -372,7 +381,7 @@ __global__ __launch_bounds__(kThreads) void policy_backward(Policy a,
             const int at = t + 64 * i + lane;
             if (at - lane >= g.end) break;
             if (at >= g.end) continue;
-            const float y = w * token_of<float>(a, all, i).slope;
+            const float y = gradient_of(a, all, i, w);
             if (g_logprob != nullptr) g_logprob[at] = all.counts[i] ? y : 0.0f;
             if (g_entropy != nullptr)
                 g_entropy[at] = all.counts[i] ? -a.entropy_weight * w : 0.0f;

@@ -302,6 +302,32 @@ def test_what_is_not_finite(hip):
 
 
 @gpu
+@pytest.mark.parametrize("by_sequence", [False, True])
+@pytest.mark.parametrize("lengths", [[400] * 8, [3000] * 40])
+@pytest.mark.parametrize("far", [79.0, 81.0, 88.0, 90.0, 95.0])
+def test_terms_past_fp32_with_weights_that_bring_them_back(hip, far, lengths, by_sequence):
+    """exp(95) is 2^137; with a token's share of the mean it is in range again, in the loss, the means
+    and the gradients. Of a policy's token that the sampler or the reference held for certain, and the
+    other way round: ratios below fp32's normal numbers, times advantages of 10^30."""
+    import torch
+    print_case("policy far", far, len(lengths), by_sequence)
+    what, how = make(lengths, seed=13, masked=0.2)
+    how["mean_by_sequence"] = by_sequence
+    lp, old, adv, cu = what
+    n = lp.numel()
+    for i in (5, n // 2, n - 7):
+        old[i], adv[i] = lp[i] - far, -1e-3
+    for i in (9, n // 3):
+        how["ref"][i] = lp[i] + far
+    for i in (17, n - 3):
+        old[i], adv[i] = lp[i] + far, 1e30
+    how["mask"][[5, 9, 17, n // 3, n // 2, n - 7, n - 3]] = True
+    check(hip, what, how)
+    how.update(ref=None, kl_weight=0.0)
+    check(hip, what, how)
+
+
+@gpu
 def test_gradient_against_differences(hip):
     """Central differences of the formula in 64 bits, no token next to a limit."""
     import torch
