@@ -153,6 +153,36 @@ def test_many_tokens(hip):
 
 
 @gpu
+@pytest.mark.parametrize("tokens,h,kv,d", [(20011, 3, 1, 64), (4099, 16, 16, 24), (30000, 1, 1, 128),
+                                           (8192, 16, 4, 64), (65536, 2, 1, 16)])
+def test_weights_gradients_of_many_tokens(hip, tokens, h, kv, d):
+    """No share is lost on the way. The sums are no chain of all terms: a lane adds those of its wave's
+    turns, one in 4096 of the tokens with at most all heads each, the lanes of a wave join in 6 steps,
+    its waves in 4, up to 1024 blocks in 16 and 64. So many times u of the magnitudes' sum, beside
+    the terms' own errors, is what they may be off by. Without the terms of any eight tokens in a
+    row, a part of what a block has, the result would not pass."""
+    import torch
+    print_case("norm_rotate dw", tokens, h, kv, d)
+    what, grads = make(tokens, h, kv, d, d, seed=15)
+    got = hip.norm_rotate_backward(*grads, *what)
+    angle = what[2].cpu().double()[:, None] * what[3].cpu()[None, :]
+    cos, sin = torch.cos(angle), torch.sin(angle)
+    for i, name in enumerate("qk"):
+        x, g, w = what[i].cpu().double(), grads[i].cpu().double(), what[4 + i]
+        xr = x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6)
+        t = turned(g, cos, -sin, d, False)
+        e = 6 * U * turned(g.abs(), cos, sin, d, False, True)
+        terms, value = t * xr, (t * xr).sum((0, 1))
+        depth = -(-tokens // 4096) * x.shape[1] + 6 + 4 + 16 + 64
+        bound = 1.01 * ((xr.abs() * (e + 14 * U * t.abs())).sum((0, 1))
+                        + depth * U * terms.abs().sum((0, 1)))
+        within(got[2 + i], value, bound, f"d{name}_weight")
+        for at in range(0, tokens - 8, tokens // 7):
+            with pytest.raises(AssertionError):
+                within(value - terms[at:at + 8].sum((0, 1)), value, bound, "")
+
+
+@gpu
 @pytest.mark.parametrize("norm", [(True, True), (False, False), (True, False), (False, True)])
 @pytest.mark.parametrize("fused", [False, True])
 def test_norms_and_fused_rows(hip, norm, fused):
