@@ -290,10 +290,10 @@ __global__ __launch_bounds__(kAppendThreads) void cache_read(
 // The segments of a sequence and a head, where there are several, and the rows of sequences that
 // have no segment.
 template <int WAVES>
-__global__ __launch_bounds__(kPagedThreads) void paged_join(Paged a) {
+__global__ __launch_bounds__(join_threads(WAVES)) void paged_join(Paged a) {
     __shared__ float sh[WAVES][kMaxDim + 1];
-    const int64_t at =
-        int64_t(blockIdx.x) * (kPagedWaves / WAVES) + int(threadIdx.x) / (64 * WAVES);
+    const int64_t at = int64_t(blockIdx.x) * (join_threads(WAVES) / (64 * WAVES)) +
+                       int(threadIdx.x) / (64 * WAVES);
     if (at >= a.c.sequences * a.heads) return;
     const int64_t s = at / a.heads;
     const Own own = own_of(a, s);
@@ -310,7 +310,12 @@ __global__ __launch_bounds__(kPagedThreads) void paged_join(Paged a) {
 }  // namespace
 
 // Workers for 512 blocks in all, two a CU (two sequences of 131072 in fp32: 383 us against 388 with
-// 1024 blocks and 389 with 2048), or as many of four waves, and no more than there can be tiles.
+// 1024 blocks and 389 with 2048), or as many of four waves, and no more than there can be tiles. Few
+// sequences and key heads leave a wave few tiles, and a row as many parts as there are waves: a tile
+// takes some 0.9 us, a part of the join some 0.015, and their sum is least with 8 sqrt(tiles
+// sequences) waves, of as many tiles each (bf16, 8 heads of 128 over one, one sequence of 65536: 2048
+// waves 50 us, 1024 33, 512 27.6, 256 28.4; so 342, 27.4; four of up to 16384: 2048 24.9, 512 22.4,
+// 256 23.4; one of 4096, 16 heads of 64: 128 13.3, 90 14.0, 64 12.5).
 Cut paged::cut_of(const Cache& c, int64_t heads, int64_t longest, int type) {
     const bool waves = by_waves(type);
     const int64_t group = heads / c.kv_heads;
@@ -319,7 +324,12 @@ Cut paged::cut_of(const Cache& c, int64_t heads, int64_t longest, int type) {
     const int64_t resident = waves ? 2048 : 512;
     const int tile = tile_of(waves, c.sequences, longest);
     const int64_t most = std::max<int64_t>(1, c.sequences * ceil_div(longest, tile));
-    return Cut{waves, tile, int(std::min(most, std::max<int64_t>(1, resident / units)))};
+    int64_t workers = std::min(most, std::max<int64_t>(1, resident / units));
+    if (waves) {
+        const double even = 8.0 * std::sqrt(double(most) * double(c.sequences));
+        workers = std::min(workers, ceil_div(most, int64_t(std::ceil(double(most) / even))));
+    }
+    return Cut{waves, tile, int(workers)};
 }
 
 namespace {
@@ -450,6 +460,14 @@ int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
                                        : launch_mfma<Bf16, false>(a, s);
 }
 
+template <int WAVES>
+int launch_join(const Paged& a, int64_t rows, hipStream_t s) {
+    EHIP_LAUNCH("attention_paged_join", paged_join<WAVES>,
+                dim3(unsigned(ceil_div(rows, join_threads(WAVES) / (64 * WAVES)))),
+                dim3(join_threads(WAVES)), 0, s, a);
+    return EHIP_OK;
+}
+
 }  // namespace
 
 int paged::launch_parts(const Paged& a, int type, hipStream_t s) {
@@ -557,13 +575,11 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     hipStream_t s = as_stream(stream);
     if (int rc = launch_parts(a, cache->type, s)) return rc;
     const int64_t rows = c.sequences * heads;
-    if (join_waves(rows) == 1)
-        EHIP_LAUNCH("attention_paged_join", paged_join<1>,
-                    dim3(unsigned(ceil_div(rows, kPagedWaves))), dim3(kPagedThreads), 0, s, a);
-    else
-        EHIP_LAUNCH("attention_paged_join", paged_join<kPagedWaves>, dim3(unsigned(rows)),
-                    dim3(kPagedThreads), 0, s, a);
-    return EHIP_OK;
+    switch (join_waves(rows, cut.workers / c.sequences)) {
+        case 1: return launch_join<1>(a, rows, s);
+        case kPagedWaves: return launch_join<kPagedWaves>(a, rows, s);
+        default: return launch_join<kManyJoinWaves>(a, rows, s);
+    }
 }
 
 }  // extern "C"

@@ -1288,8 +1288,15 @@ inline int tile_of(bool waves, int64_t rows, int64_t longest) {
     return waves && rows * ceil_div(longest, kWaveTile) <= INT32_MAX ? kWaveTile : kTile;
 }
 
-// Waves of a row that is joined.
-inline int join_waves(int64_t rows) { return rows >= 1024 ? 1 : kPagedWaves; }
+// Waves of a row that is joined: one where the rows fill the card, many for few rows of many parts
+// (16 rows of 128 parts of 64 values: with the parts 14.3 us by 4 waves, 13.3 by 16; 128 of up to 128
+// 16.1 and 15.2; 16 of 16 10.1 and 10.9).
+constexpr int kManyJoinWaves = 16;
+constexpr int join_threads(int waves) { return waves > kPagedWaves ? 64 * waves : kPagedThreads; }
+inline int join_waves(int64_t rows, int64_t parts) {
+    if (rows >= 1024) return 1;
+    return rows <= 256 && parts >= 64 ? kManyJoinWaves : kPagedWaves;
+}
 
 // The cut of the sequences' own positions, and the launch over them (attention_paged.hip).
 Cut cut_of(const Cache& c, int64_t heads, int64_t longest, int type);

@@ -724,7 +724,7 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
         if (int rc = launch_parts(own, cache->type, s)) return rc;
     }
     const int64_t rows = c.sequences * heads;
-    if (join_waves(rows) == 1)
+    if (join_waves(rows, 0) == 1)
         EHIP_LAUNCH("attention_shared_join", shared_join<1>,
                     dim3(unsigned(ceil_div(rows, kPagedWaves))), dim3(kPagedThreads), 0, s, own,
                     a, of);

@@ -100,6 +100,14 @@ def test_lengths_that_are_split(hip, dtype, lengths):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", types())
+@pytest.mark.parametrize("lengths", [[9000], [20011, 3], [9001, 0, 12000]])
+@pytest.mark.parametrize("heads,kv,d", [(8, 1, 64), (4, 4, 33), (3, 1, 128)])
+def test_few_rows_of_many_parts(hip, dtype, lengths, heads, kv, d):
+    check(hip, lengths, heads, kv, d, 16, dtype, seed=heads)
+
+
+@gpu
 @pytest.mark.parametrize("scale,spread", [(0.0, 1.0), (-0.2, 3.0), (0.125, 40.0)])
 def test_scales_and_sharp_rows(hip, scale, spread):
     import torch
@@ -632,6 +640,23 @@ def test_refused_caches_and_sizes():
         assert b"attention_paged" in lib.ehip_last_error()
     for heads, longest in ((3, 64), (0, 64), (-2, 64), (4, -1), (4, 2 ** 31), (2 ** 24, 64)):
         assert size(C.byref(cache()), heads, longest) == -1, (heads, longest)
+
+
+@pytest.mark.parametrize("kind", [0, 1, 2])
+@pytest.mark.parametrize("sequences,longest,heads,kv,most", [
+    (1, 65536, 8, 1, 512), (1, 131072, 8, 1, 512), (1, 1 << 20, 16, 1, 2048), (4, 16384, 8, 1, 1024),
+    (1, 4096, 16, 16, 64), (1, 500, 16, 16, 16), (64, 4096, 32, 8, 256)])
+def test_few_rows_are_not_cut_into_more_parts_than_they_gain_by(kind, sequences, longest, heads, kv,
+                                                                most):
+    """A row of 2048 parts was joined for longer than its parts took. The workspace holds a maximum, a
+    sum and head_dim values for each head and part, of which there are as many as workers and
+    sequences, and an int a sequence."""
+    lib = E.load_library()
+    d = 128
+    c = cache(type=kind, kv_heads=kv, head_dim=d, sequences=sequences, k_scales=16, v_scales=16)
+    need = lib.ehip_attention_paged_workspace(C.byref(c), heads, longest)
+    parts, rest = divmod(need - 4 * (sequences + 1), heads * (8 + 4 * d))
+    assert rest == 0 and 0 < parts - sequences <= most
 
 
 def test_lengths_end_where_positions_leave_their_range():
