@@ -316,8 +316,7 @@ __global__ __launch_bounds__(join_threads(WAVES)) void paged_join(Paged a) {
 // sequences) waves, of as many tiles each (bf16, 8 heads of 128 over one, one sequence of 65536: 2048
 // waves 50 us, 1024 33, 512 27.6, 256 28.4; so 342, 27.4; four of up to 16384: 2048 24.9, 512 22.4,
 // 256 23.4; one of 4096, 16 heads of 64: 128 13.3, 90 14.0, 64 12.5).
-Cut paged::cut_of(const Cache& c, int64_t heads, int64_t longest, int type) {
-    const bool waves = by_waves(type);
+Cut paged::cut_of(const Cache& c, int64_t heads, int64_t longest, bool waves) {
     const int64_t group = heads / c.kv_heads;
     const int64_t units =
         c.kv_heads * ceil_div(group, waves ? 16 : kMaxGroup);
@@ -401,35 +400,30 @@ int read(const Read& x, hipStream_t s) {
     return EHIP_OK;
 }
 
-template <int LPP, int G, bool VEC>
+template <class T, int LPP, int G, bool VEC>
 int launch_part(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
     const int64_t blocks = a.workers * ceil_div(group, G) * a.c.kv_heads;
-    EHIP_LAUNCH("attention_paged", (paged_part<LPP, G, VEC>), dim3(unsigned(blocks)),
+    EHIP_LAUNCH("attention_paged", (paged_part<T, LPP, G, VEC>), dim3(unsigned(blocks)),
                 dim3(kPagedThreads), 0, s, a);
     return EHIP_OK;
 }
 
-template <int LPP, bool VEC>
+template <class T, int LPP, bool VEC>
 int launch_group(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
-    if (group == 1) return launch_part<LPP, 1, VEC>(a, s);
-    if (group == 2) return launch_part<LPP, 2, VEC>(a, s);
-    if (group <= 4) return launch_part<LPP, 4, VEC>(a, s);
-    return launch_part<LPP, 8, VEC>(a, s);
+    if (group == 1) return launch_part<T, LPP, 1, VEC>(a, s);
+    if (group == 2) return launch_part<T, LPP, 2, VEC>(a, s);
+    if (group <= 4) return launch_part<T, LPP, 4, VEC>(a, s);
+    return launch_part<T, LPP, 8, VEC>(a, s);
 }
 
-template <bool VEC>
+template <class T, bool VEC>
 int launch_lanes(const Paged& a, hipStream_t s) {
-    if (a.c.dim <= 32) return launch_group<8, VEC>(a, s);
-    if (a.c.dim <= 64) return launch_group<16, VEC>(a, s);
-    return launch_group<32, VEC>(a, s);
-}
-
-// 16-byte reads where every head's row begins at 16 bytes.
-int launch_parts_f32(const Paged& a, bool aligned, hipStream_t s) {
-    return aligned && a.c.dim % 4 == 0 ? launch_lanes<true>(a, s)
-                                       : launch_lanes<false>(a, s);
+    constexpr int N = 16 / int(sizeof(T));
+    if (a.c.dim <= 32) return launch_group<T, 32 / N, VEC>(a, s);
+    if (a.c.dim <= 64) return launch_group<T, 64 / N, VEC>(a, s);
+    return launch_group<T, 128 / N, VEC>(a, s);
 }
 
 template <class T, int DP, bool WIDE>
@@ -448,16 +442,20 @@ int launch_mfma(const Paged& a, hipStream_t s) {
     return launch_part_mfma<T, 128, WIDE>(a, s);
 }
 
-// Reads of whole pieces in 8 bits: of 16 values, or of 8 in heads of up to 32.
-int launch_parts_i8(const Paged& a, bool aligned, hipStream_t s) {
-    return aligned && a.c.dim % (a.c.dim <= 32 ? 8 : 16) == 0 ? launch_mfma<Int8, true>(a, s)
-                                                              : launch_mfma<Int8, false>(a, s);
-}
-
-// Of 8 values in bf16.
-int launch_parts_bf16(const Paged& a, bool aligned, hipStream_t s) {
-    return aligned && a.c.dim % 8 == 0 ? launch_mfma<Bf16, true>(a, s)
-                                       : launch_mfma<Bf16, false>(a, s);
+// Whether the positions go by waves and the matrix instructions. Two kinds of bf16 heads whose rows are
+// not whole units do not. Few of them: those kernels put the last values in place and spill, and what
+// they take before their first tile is more than the little work, unless many heads share it (us,
+// vector : matrix; one sequence of 64, 16 heads of 77 10.3 : 19.7, of 500 15.2 : 20.6, of 4096 22.9 :
+// 29.7; of 2048, 32 heads over 8 of 77 21.5 : 22.9, of 100 23.7 : 21.6; of 8192, 8 over one of 77 31.5
+// : 26.9; 4 of up to 4096, 32 over 8 of 77 50.8 : 38.2). And single ones of below eight values, which
+// both read one by one (256 of up to 300, 16 of 7, 75 : 95; of 33 101 : 67).
+bool waves_of(const Cache& c, int64_t heads, int64_t longest, int type) {
+    if (type == EHIP_CACHE_BF16 && !whole_rows(c, 8)) {
+        const int64_t group = heads / c.kv_heads;
+        const bool few = group <= 4 && c.sequences * heads * longest <= int64_t(1) << 16;
+        return !few && !(group == 1 && c.dim < 8);
+    }
+    return by_waves(type);
 }
 
 template <int WAVES>
@@ -470,11 +468,16 @@ int launch_join(const Paged& a, int64_t rows, hipStream_t s) {
 
 }  // namespace
 
-int paged::launch_parts(const Paged& a, int type, hipStream_t s) {
-    const bool aligned = aligned16(a.c.k) && aligned16(a.c.v);
-    if (type == EHIP_CACHE_F32) return launch_parts_f32(a, aligned, s);
-    return type == EHIP_CACHE_BF16 ? launch_parts_bf16(a, aligned, s)
-                                   : launch_parts_i8(a, aligned, s);
+int paged::launch_parts(const Paged& a, int type, bool waves, hipStream_t s) {
+    if (type == EHIP_CACHE_F32)
+        return whole_rows(a.c, 4) ? launch_lanes<float, true>(a, s)
+                                  : launch_lanes<float, false>(a, s);
+    if (!waves) return launch_lanes<Bf16, false>(a, s);
+    if (type == EHIP_CACHE_BF16)
+        return whole_rows(a.c, 8) ? launch_mfma<Bf16, true>(a, s) : launch_mfma<Bf16, false>(a, s);
+    // Reads of whole pieces in 8 bits: of 16 values, or of 8 in heads of up to 32.
+    return whole_rows(a.c, a.c.dim <= 32 ? 8 : 16) ? launch_mfma<Int8, true>(a, s)
+                                                   : launch_mfma<Int8, false>(a, s);
 }
 
 }  // namespace ehip
@@ -534,7 +537,8 @@ int64_t ehip_attention_paged_workspace(const ehip_cache_t* cache, int64_t heads,
         return -1;
     return c.sequences == 0
                ? 0
-               : int64_t(part_bytes(c, heads, cut_of(c, heads, longest, cache->type).workers));
+               : int64_t(part_bytes(c, heads, cut_of(c, heads, longest, waves_of(c, heads, longest, cache->type))
+                                        .workers));
 }
 
 int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t ld_q,
@@ -550,7 +554,7 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     if (c.sequences == 0) return EHIP_OK;
     if (q == nullptr || lengths == nullptr || out == nullptr)
         return fail(EHIP_EINVAL, "attention_paged: null tensor");
-    const Cut cut = cut_of(c, heads, longest, cache->type);
+    const Cut cut = cut_of(c, heads, longest, waves_of(c, heads, longest, cache->type));
     const size_t need = part_bytes(c, heads, cut.workers);
     if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
         return fail(EHIP_EINVAL, "attention_paged: needs %zu bytes of 16-byte aligned workspace",
@@ -573,7 +577,7 @@ int ehip_attention_paged_f32(const ehip_cache_t* cache, const float* q, int64_t 
     a.part_out = reinterpret_cast<float*>(a.part_stats + parts);
     a.first = reinterpret_cast<int*>(a.part_out + parts * c.dim);
     hipStream_t s = as_stream(stream);
-    if (int rc = launch_parts(a, cache->type, s)) return rc;
+    if (int rc = launch_parts(a, cache->type, cut.waves, s)) return rc;
     const int64_t rows = c.sequences * heads;
     switch (join_waves(rows, cut.workers / c.sequences)) {
         case 1: return launch_join<1>(a, rows, s);

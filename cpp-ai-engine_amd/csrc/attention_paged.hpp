@@ -95,7 +95,7 @@ __device__ __forceinline__ void narrow(float x, Bf16& out) {
 // running maximum, sum and weighted values over the positions they meet, joined at the end: of the
 // wave, the block's four waves, and, where the length is split, the blocks of a sequence by a
 // second launch. Two sequences of 131072 in fp32, 32 heads over 8 of 128 values: 356 us at best,
-// 6.0 TB/s.
+// 6.0 TB/s. It takes fp32, and what little there is of bf16 heads at any address (waves_of).
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = kPagedThreads / 64;
 constexpr int kUnroll = 4;
@@ -403,14 +403,14 @@ __device__ __forceinline__ float across(float x) {
 
 // One lane's values of a row as they are stored: 16 bytes, and its own first ones again in lanes
 // past the row's end.
-template <bool VEC>
+template <class T, bool VEC>
 struct Values {
-    static constexpr int N = 4;
+    static constexpr int N = 16 / int(sizeof(T));
     struct alignas(16) Pack {
-        float v[N];
+        T v[N];
     } x;
 
-    __device__ __forceinline__ void load(const float* row, int d0, int dim) {
+    __device__ __forceinline__ void load(const T* row, int d0, int dim) {
         if (VEC) {
             x = *reinterpret_cast<const Pack*>(row + (d0 < dim ? d0 : 0));
         } else {
@@ -418,12 +418,12 @@ struct Values {
             for (int e = 0; e < N; ++e) x.v[e] = row[d0 + e < dim ? d0 + e : 0];
         }
     }
-    __device__ __forceinline__ float operator[](int e) const { return x.v[e]; }
+    __device__ __forceinline__ float operator[](int e) const { return widen(x.v[e]); }
 };
 
-template <int LPP, int G, bool VEC>
+template <class T, int LPP, int G, bool VEC>
 __global__ __launch_bounds__(kPagedThreads, G >= 4 ? 2 : 3) void paged_part(Paged a) {
-    constexpr int N = 4, SUBS = 64 / LPP, TILE = SUBS * kUnroll;
+    constexpr int N = Values<T, VEC>::N, SUBS = 64 / LPP, TILE = SUBS * kUnroll;
     __shared__ float sh_m[kPagedWaves][G], sh_l[kPagedWaves][G], sh_o[kPagedWaves][G][LPP * N];
     const int lane = int(threadIdx.x) & 63, wave = int(threadIdx.x) / 64;
     const int kv_heads = int(a.c.kv_heads), dim = int(a.c.dim);
@@ -456,8 +456,8 @@ __global__ __launch_bounds__(kPagedThreads, G >= 4 ? 2 : 3) void paged_part(Page
                 o[g][e] = 0.0f;
             }
         }
-        const float* const k = static_cast<const float*>(a.c.k) + int64_t(kv) * dim;
-        const float* const v = static_cast<const float*>(a.c.v) + int64_t(kv) * dim;
+        const T* const k = static_cast<const T*>(a.c.k) + int64_t(kv) * dim;
+        const T* const v = static_cast<const T*>(a.c.v) + int64_t(kv) * dim;
         const int64_t pitch = int64_t(kv_heads) * dim;
         // The pool row of the tile's position `lane`.
         const auto row_of = [&](int p0) {
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(kPagedThreads, G >= 4 ? 2 : 3) void paged_part(Page
         };
         int row = int(row_of(begin + wave * TILE));
         for (int p0 = begin + wave * TILE; p0 < end; p0 += kPagedWaves * TILE) {
-            Values<VEC> ks[kUnroll], vs[kUnroll];
+            Values<T, VEC> ks[kUnroll], vs[kUnroll];
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 const int64_t at = int64_t(__shfl(row, u * SUBS + sub)) * pitch;
@@ -1283,6 +1283,10 @@ struct Cut {
 
 // bf16 and 8 bits, exact in one part, go by the matrix instructions.
 inline bool by_waves(int type) { return type != EHIP_CACHE_F32; }
+// Rows of whole units at 16 bytes.
+inline bool whole_rows(const Cache& c, int values) {
+    return c.dim % values == 0 && aligned16(c.k) && aligned16(c.v);
+}
 // Positions that so many rows of work of at most `longest` are cut by.
 inline int tile_of(bool waves, int64_t rows, int64_t longest) {
     return waves && rows * ceil_div(longest, kWaveTile) <= INT32_MAX ? kWaveTile : kTile;
@@ -1299,8 +1303,8 @@ inline int join_waves(int64_t rows, int64_t parts) {
 }
 
 // The cut of the sequences' own positions, and the launch over them (attention_paged.hip).
-Cut cut_of(const Cache& c, int64_t heads, int64_t longest, int type);
-int launch_parts(const Paged& a, int type, hipStream_t s);
+Cut cut_of(const Cache& c, int64_t heads, int64_t longest, bool waves);
+int launch_parts(const Paged& a, int type, bool waves, hipStream_t s);
 
 }  // namespace paged
 }  // namespace ehip

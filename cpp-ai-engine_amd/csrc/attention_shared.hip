@@ -566,7 +566,7 @@ size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 Plan plan_of(const Cache& c, int type, int64_t heads, int64_t longest, int64_t groups,
              int64_t longest_shared) {
     Plan p{};
-    p.own = cut_of(c, heads, longest, type);
+    p.own = cut_of(c, heads, longest, by_waves(type));
     const int64_t rows = c.sequences * (heads / c.kv_heads);
     p.by_rows = by_rows(type, groups > 0 ? rows / groups : 0);
     p.rows = p.by_rows ? 64 : 16;
@@ -604,7 +604,7 @@ int launch_rows_dim(const Paged& a, hipStream_t s) {
 int launch_apart(const Paged& own, const Paged& a, hipStream_t s) {
     const bool wide = aligned16(a.c.k) && aligned16(a.c.v) && a.c.dim % 4 == 0;
     const int rc = wide ? launch_rows_dim<float, true>(a, s) : launch_rows_dim<float, false>(a, s);
-    return rc != EHIP_OK ? rc : launch_parts(own, EHIP_CACHE_F32, s);
+    return rc != EHIP_OK ? rc : launch_parts(own, EHIP_CACHE_F32, false, s);
 }
 
 template <class T, int DP, bool WIDE, bool ROWS>
@@ -721,7 +721,7 @@ int ehip_attention_shared_f32(const ehip_cache_t* cache, const float* q, int64_t
     if (groups > 0) {
         if (int rc = launch_shared(own, a, cache->type, p.by_rows, s)) return rc;
     } else {
-        if (int rc = launch_parts(own, cache->type, s)) return rc;
+        if (int rc = launch_parts(own, cache->type, p.own.waves, s)) return rc;
     }
     const int64_t rows = c.sequences * heads;
     if (join_waves(rows, 0) == 1)

@@ -100,6 +100,43 @@ def test_lengths_that_are_split(hip, dtype, lengths):
 
 
 @gpu
+@pytest.mark.parametrize("longest", [130, 1 << 20])
+@pytest.mark.parametrize("heads,kv", [(6, 6), (8, 2), (10, 2), (17, 1)])
+@pytest.mark.parametrize("d", [1, 3, 4, 5, 7, 9, 12, 20, 31, 33, 50, 63, 65, 77, 100, 127])
+def test_odd_heads_in_bf16_of_little_and_much_work(hip, d, heads, kv, longest):
+    """The bound on the lengths says how much there may be, and with it which kernel passes them."""
+    import torch
+    check(hip, [37, 5, 0, 130, 64], heads, kv, d, 8, torch.bfloat16, seed=d, longest=longest)
+
+
+@gpu
+@pytest.mark.parametrize("longest", [130, 1 << 20])
+@pytest.mark.parametrize("which,value", [("k", math.nan), ("k", math.inf), ("v", math.nan),
+                                         ("v", -math.inf)])
+def test_odd_heads_in_bf16_that_are_not_finite(hip, which, value, longest):
+    import torch
+    print_case("paged odd not finite", which, value, longest)
+    lengths, d = [130, 40], 33
+    kp, vp, table, q, want, want_lse = check(hip, lengths, 4, 2, d, 16, torch.bfloat16, seed=31,
+                                             longest=longest)
+    pool = kp if which == "k" else vp
+    pool[int(table[0, 3]), 2, 0, 7] = value
+    q[0, :2, 7] = q[0, :2, 7].abs() + 1
+    out, lse = hip.attention_paged(q, kp, vp, table, ints(lengths), longest=longest)
+    columns = [7] if which == "v" else list(range(d))
+    hit = out[0, :2][:, columns]
+    if which == "v" and value == -math.inf:
+        assert bool((hit == value).all())
+    else:
+        assert bool(torch.isnan(hit).all())
+    rest = [c for c in range(d) if c not in columns]
+    if which == "v":
+        assert bool(torch.isfinite(out[0, :2][:, rest]).all())
+        assert bool(torch.isfinite(lse).all())
+    assert torch.equal(out[0, 2:], want[0, 2:]) and torch.equal(out[1], want[1])
+
+
+@gpu
 @pytest.mark.parametrize("dtype", types())
 @pytest.mark.parametrize("lengths", [[9000], [20011, 3], [9001, 0, 12000]])
 @pytest.mark.parametrize("heads,kv,d", [(8, 1, 64), (4, 4, 33), (3, 1, 128)])
