@@ -591,16 +591,21 @@ __global__ __launch_bounds__(kPagedThreads, G >= 4 ? 2 : 3) void paged_part(Page
     }
 }
 
-// One head's share of a block by the formula, for those whose sums by parts are not finite: a part
-// of an infinity, or an infinity times the parts of a finite value, is NaN where the product is an
-// infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time; a
-// score of NaN or +inf settles the head as NaN (64 sequences of 1024,
-// 32 heads over 8 of 128 values, us: finite 42, the first key NaN 105, the first value 557; value by
-// value and to the end 1870 either way).
-template <class T>
-__device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int kv, int begin,
-                                int end, float& top, float& sum, float (&o)[2]) {
+// Up to kAgain heads' share of a segment by the formula, for those whose sums by parts are not finite: a
+// part of an infinity, or an infinity times the parts of a finite value, is NaN where the product is
+// an infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time; a
+// score of NaN or +inf settles its head as NaN. Each segment's wave forms its own, so its reads are
+// several at a time and serve four heads (64 sequences of 1024, 32 heads over 8 of 128 values, us, bf16
+// and 8 bits: finite 52 and 37; the first key NaN 69 and 48, a head and a read at a time 82 and 98; the
+// first value infinite 274 and 130, and 623 and 555).
+constexpr int kAgain = 4;
+
+template <class T, int DP>
+__device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&q)[kAgain], int kv,
+                                int begin, int end, float (&top)[kAgain], float (&sum)[kAgain],
+                                float (&o)[kAgain][2]) {
     using attention::uintx4;
+    constexpr int kReads = DP > 64 ? 4 : 2;  // more than the tiles leave registers for hold up those
     int lane = int(threadIdx.x) & 63;
     asm volatile("" : "+v"(lane));  // else what follows from it is held all through the tiles
     const int dim = int(a.c.dim);
@@ -618,77 +623,140 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* q, int k
     };
     // Rows of 16-byte units, or others four values at a time at any address.
     const bool units = sizeof(T) == 2 && dim % 8 == 0 && aligned16(a.c.k);
-    const auto score = [&](int row) {
+    const auto scores = [&](int row, float (&dot)[kAgain]) {
         const T* at = k + int64_t(row) * pitch;
         const float by = sizeof(T) == 1 ? a.c.k_scales[place] : 1.0f;
-        float dot = 0.0f;
-        int e = 0;
-        if (sizeof(T) == 2 && units) {
-            for (; e < dim; e += 8) {
-                const uintx4 x = *reinterpret_cast<const uintx4*>(at + e);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t pair = x[j];
-                    dot = __builtin_fmaf(q[e + 2 * j] * c2, __builtin_bit_cast(float, pair << 16),
-                                         dot);
-                    dot = __builtin_fmaf(q[e + 2 * j + 1] * c2,
-                                         __builtin_bit_cast(float, pair & 0xffff0000u), dot);
+        for (int g = 0; g < kAgain; ++g) dot[g] = 0.0f;
+        const auto add = [&](int e, float x) {
+#pragma unroll
+            for (int g = 0; g < kAgain; ++g) dot[g] = __builtin_fmaf(q[g][e] * c2, x, dot[g]);
+        };
+        int e = 0;
+        if (units) {
+            for (; e < dim; e += 8 * kReads) {  // several at a time, past the end the first again
+                uintx4 x[kReads];
+#pragma unroll
+                for (int i = 0; i < kReads; ++i)
+                    x[i] = *reinterpret_cast<const uintx4*>(at + (e + 8 * i < dim ? e + 8 * i : 0));
+#pragma unroll
+                for (int i = 0; i < kReads; ++i) {
+                    __builtin_amdgcn_sched_barrier(0);  // the next eight of q are not held as well
+                    if (e + 8 * i >= dim) break;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t pair = x[i][j];
+                        add(e + 8 * i + 2 * j, __builtin_bit_cast(float, pair << 16));
+                        add(e + 8 * i + 2 * j + 1, __builtin_bit_cast(float, pair & 0xffff0000u));
+                    }
                 }
             }
-            return dot;
+            return;
+        }
+        for (; e + 16 <= dim; e += 16) {
+            T x[16];
+            __builtin_memcpy(x, at + e, sizeof(x));
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                if (j % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                add(e + j, sizeof(T) == 1 ? widen(x[j]) * by : widen(x[j]));
+            }
         }
         for (; e + 4 <= dim; e += 4) {
             T x[4];
             __builtin_memcpy(x, at + e, sizeof(x));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                dot = __builtin_fmaf(q[e + j] * c2, sizeof(T) == 1 ? widen(x[j]) * by : widen(x[j]),
-                                     dot);
+                add(e + j, sizeof(T) == 1 ? widen(x[j]) * by : widen(x[j]));
         }
-        for (; e < dim; ++e)
-            dot = __builtin_fmaf(q[e] * c2, sizeof(T) == 1 ? widen(at[e]) * by : widen(at[e]), dot);
-        return dot;
+        for (; e < dim; ++e) add(e, sizeof(T) == 1 ? widen(at[e]) * by : widen(at[e]));
     };
-    top = -INFINITY;
-    for (int p0 = begin; p0 < end; p0 += 64) {
-        const float x = score(row_of(p0));
-        if (__any(!(x < INFINITY))) {
-            top = 0.0f;
-            sum = o[0] = o[1] = NAN;
-            return;
+    float x[kAgain], shift[kAgain];
+    bool settled[kAgain], all = false;
+#pragma unroll
+    for (int g = 0; g < kAgain; ++g) {
+        top[g] = -INFINITY;
+        settled[g] = false;
+    }
+    for (int p0 = begin; p0 < end && !all; p0 += 64) {
+        scores(row_of(p0), x);
+        all = true;
+#pragma unroll
+        for (int g = 0; g < kAgain; ++g) {
+            settled[g] = settled[g] || __any(!(x[g] < INFINITY));
+            all = all && settled[g];
+            top[g] = fmaxf(top[g], x[g]);
         }
-        top = fmaxf(top, x);
     }
 #pragma unroll
-    for (int w = 32; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
-    const float shift = top == -INFINITY ? 0.0f : top;  // scores of -inf alone weigh nothing
-    sum = o[0] = o[1] = 0.0f;
+    for (int g = 0; g < kAgain; ++g) {
+#pragma unroll
+        for (int w = 32; w > 0; w >>= 1) top[g] = fmaxf(top[g], __shfl_xor(top[g], w));
+        shift[g] = top[g] == -INFINITY ? 0.0f : top[g];  // scores of -inf alone weigh nothing
+        sum[g] = o[g][0] = o[g][1] = 0.0f;
+    }
     const int d0 = lane < dim ? lane : 0, d1 = lane + 64 < dim ? lane + 64 : 0;
-    for (int p0 = begin; p0 < end; p0 += 64) {
+    bool none = false;  // a scale that is not finite settles the values, whatever its weight
+    for (int p0 = begin; p0 < end && !all; p0 += 64) {
         const int row = row_of(p0), count = min(64, end - p0);
-        const float weight = lane < count ? exp2f(score(row) - shift) * 0x1p-24f : 0.0f;
+        scores(row, x);
+#pragma unroll
+        for (int g = 0; g < kAgain; ++g) {
+            x[g] = lane < count ? exp2f(x[g] - shift[g]) * 0x1p-24f : 0.0f;
+            sum[g] += x[g];
+        }
         const float vs = sizeof(T) == 1 ? a.c.v_scales[place] : 1.0f;
-        sum += weight;
-        // A scale that is not finite settles the values, whatever its weight.
-        if (sizeof(T) == 1 && __any(!(fabsf(vs) < INFINITY))) o[0] = o[1] = NAN;
-        if (sizeof(T) == 1 && o[0] != o[0]) continue;
-#pragma unroll 8
-        for (int u = 0; u < count; ++u) {
-            const T* at = v + int64_t(__shfl(row, u)) * pitch;
-            const float w = __shfl(weight, u);
-            float x0 = widen(at[d0]), x1 = widen(at[d1]);
-            if constexpr (sizeof(T) == 1) {
-                const float scale = __shfl(vs, u);
-                x0 *= scale;
-                x1 *= scale;
+        if (sizeof(T) == 1) none = none || __any(!(fabsf(vs) < INFINITY));
+        if (none) continue;
+        for (int u0 = 0; u0 < count; u0 += 2 * kReads) {  // several positions' reads at a time
+            T from[2 * kReads][2];
+#pragma unroll
+            for (int i = 0; i < 2 * kReads; ++i) {
+                const T* at = v + int64_t(__shfl(row, u0 + i)) * pitch;
+                from[i][0] = at[d0];
+                from[i][1] = at[d1];
             }
-            o[0] = __builtin_fmaf(w, x0, o[0]);
-            o[1] = __builtin_fmaf(w, x1, o[1]);
+#pragma unroll
+            for (int i = 0; i < 2 * kReads; ++i) {
+                const int u = u0 + i;  // 63 at most; past the end the last again, for nothing
+                const float scale = sizeof(T) == 1 ? __shfl(vs, u) : 1.0f;
+                float y[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    y[e] = widen(from[i][e]);
+                    if (sizeof(T) == 1) y[e] *= scale;
+                    y[e] = u < count ? y[e] : 0.0f;
+                }
+#pragma unroll
+                for (int g = 0; g < kAgain; ++g) {
+                    const float w = __shfl(x[g], u);
+                    o[g][0] = __builtin_fmaf(w, y[0], o[g][0]);
+                    o[g][1] = __builtin_fmaf(w, y[1], o[g][1]);
+                }
+            }
         }
     }
 #pragma unroll
-    for (int w = 32; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
+    for (int g = 0; g < kAgain; ++g) {
+#pragma unroll
+        for (int w = 32; w > 0; w >>= 1) sum[g] += __shfl_xor(sum[g], w);
+        if (settled[g]) top[g] = 0.0f, sum[g] = NAN;
+        if (settled[g] || none) o[g][0] = o[g][1] = NAN;
+    }
 }
+
+// The next rows of a set, the last again past its end, which is cleared of them.
+struct Again {
+    int row[kAgain], count;
+    __device__ __forceinline__ explicit Again(uint32_t& rows) : count(0) {
+#pragma unroll
+        for (int g = 0; g < kAgain; ++g) {
+            row[g] = rows != 0 ? __builtin_ctz(rows) : row[g > 0 ? g - 1 : 0];
+            count += rows != 0;
+            rows &= rows - 1;
+        }
+    }
+};
 
 // A cache in bf16, up to 16 query heads of a key head at a time, on v_mfma_f32_16x16x32_bf16: the
 // cached values are operands as they are, q and the weights in three parts, so a score and a
@@ -805,6 +873,29 @@ __device__ __forceinline__ bool out_of_parts(float largest) {
     return (largest > 0.0f && largest < 0x1p-100f) || (sizeof(T) == 1 && largest > 0x1p112f);
 }
 
+// Eight values of a query row of any length at any address, four at a time, which are put in place where
+// they are used; one by one an address each is held, and with heads over 64 spilled (64 sequences up
+// to 1024, 32 heads over 8 of 100, bf16 65 us, like this 52; 256 up to 300, 16 of 33, 8 bits 63, 65).
+__device__ __forceinline__ void ask_eight(const float* row, int d0, int dim, float (&x)[8]) {
+    if (dim < 4) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = row[d0 + e < dim ? d0 + e : 0];
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e += 4) {
+        const auto y = *reinterpret_cast<const attention::floatx4u*>(
+            row + attention::clamped<attention::kClamped>(d0 + e, dim));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[e + j] = y[j];
+    }
+}
+__device__ __forceinline__ void eight_in_place(float (&x)[8], int d0, int dim) {
+    if (dim < 4) return;
+    attention::in_place<attention::kClamped>(x, d0, dim);
+    attention::in_place<attention::kClamped>(x + 4, d0 + 4, dim);
+}
+
 constexpr int value_pitch(int dp) { return 2 * dp + 32; }  // bytes of a row of V in LDS
 template <int DP>
 struct alignas(16) PartLds {
@@ -901,7 +992,7 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
         char* const mine = lds.values[wave];
         // q is asked for between the table and the rows that it names, and split while those are on
         // their way; of wide heads in bf16, where that spills, before the table.
-        constexpr bool kFirst = !kScaled && DP > 64;
+        constexpr bool kFirst = !kScaled && DP > 64, kFours = !WIDE && DP > 64;
         float qx[KS][8];
         bf16x8 q[KS][3];
         const auto ask_query = [&] {
@@ -911,6 +1002,10 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
                 const int d0 = 4 * N * (8 * ks / N) + N * quarter + 8 * ks % N;
                 // With WIDE a head is a multiple of eight values, and one offset serves them all: those
                 // of each would be kept over the segments, in scratch.
+                if (kFours) {
+                    ask_eight(row, d0, dim, qx[ks]);
+                    continue;
+                }
                 const int from = WIDE && d0 < dim ? d0 : 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -922,6 +1017,7 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const int d0 = 4 * N * (8 * ks / N) + N * quarter + 8 * ks % N;
+                if (kFours) eight_in_place(qx[ks], d0, dim);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const bool in = d0 + (WIDE ? 0 : e) < dim;
@@ -1103,22 +1199,29 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
             }
         }
         if (bad) continue;
-        for (; again != 0; again &= again - 1) {
-            const int g = __builtin_ctz(again);
-            float top, sum, y[2];
-            part_by_formula<T>(a, s, query_row<SHARED>(a, seg, kv, h0, g), kv, begin, end, top, sum,
-                               y);
-            const int64_t place = part_of<SHARED>(a, seg, worker, kv, h0, g);
-            if (lane == 0) {
-                if (!seg.whole) a.part_stats[place] = float2{top, sum};
-                else if (a.lse != nullptr) a.lse[s * a.heads + h0 + g] = lse_of(top, sum);
-            }
+        while (again != 0) {
+            const Again some(again);
+            const float* rows[kAgain];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int d = lane + 64 * e;
-                if (d >= dim) continue;
-                if (!seg.whole) a.part_out[place * dim + d] = y[e];
-                else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y[e] / sum;
+            for (int i = 0; i < kAgain; ++i) rows[i] = query_row<SHARED>(a, seg, kv, h0, some.row[i]);
+            float top[kAgain], sum[kAgain], y[kAgain][2];
+            part_by_formula<T, DP>(a, s, rows, kv, begin, end, top, sum, y);
+#pragma unroll
+            for (int i = 0; i < kAgain; ++i) {
+                const int g = some.row[i];
+                const int64_t place = part_of<SHARED>(a, seg, worker, kv, h0, g);
+                if (i < some.count && lane == 0) {
+                    if (!seg.whole) a.part_stats[place] = float2{top[i], sum[i]};
+                    else if (a.lse != nullptr)
+                        a.lse[s * a.heads + h0 + g] = lse_of(top[i], sum[i]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int d = lane + 64 * e;
+                    if (i >= some.count || d >= dim) continue;
+                    if (!seg.whole) a.part_out[place * dim + d] = y[i][e];
+                    else a.out[s * a.ld_out + int64_t(h0 + g) * dim + d] = y[i][e] / sum[i];
+                }
             }
         }
     }

@@ -200,19 +200,24 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
             const float* const from = query_row<true>(a, seg, kv, 0, mine < count ? mine : 0);
             float y[KS][8];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    // With WIDE a head is a multiple of four values.
-                    const int d0 = 32 * ks + 8 * quarter + (WIDE ? e / 4 * 4 : e);
-                    y[ks][e] = from[(d0 < dim ? d0 : 0) + (WIDE ? e % 4 : 0)];
+            for (int ks = 0; ks < KS; ++ks) {
+                if (!WIDE) {
+                    ask_eight(from, 32 * ks + 8 * quarter, dim, y[ks]);
+                    continue;
                 }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {  // a head is a multiple of four values
+                    const int d0 = 32 * ks + 8 * quarter + e / 4 * 4;
+                    y[ks][e] = from[(d0 < dim ? d0 : 0) + e % 4];
+                }
+            }
             find();
             load(begin);
             ask(begin + kKeys);
             float largest = 0.0f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
+                if (!WIDE) eight_in_place(y[ks], 32 * ks + 8 * quarter, dim);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int d = 32 * ks + 8 * quarter + e;
@@ -400,15 +405,23 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
                 }
             }
         }
-        for (; again != 0; again &= again - 1) {
-            const int i = 16 * wave + __builtin_ctz(again);
-            float top, sum, y[2];
-            part_by_formula<T>(a, s, query_row<true>(a, seg, kv, 0, i), kv, begin, end, top, sum,
-                               y);
-            if (lane == 0) a.part_stats[part0 + i] = float2{top, sum};
+        while (again != 0) {
+            const Again next(again);
+            const float* rows[kAgain];
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-                if (lane + 64 * e < dim) a.part_out[(part0 + i) * dim + lane + 64 * e] = y[e];
+            for (int i = 0; i < kAgain; ++i)
+                rows[i] = query_row<true>(a, seg, kv, 0, 16 * wave + next.row[i]);
+            float top[kAgain], sum[kAgain], y[kAgain][2];
+            part_by_formula<T, DP>(a, s, rows, kv, begin, end, top, sum, y);
+#pragma unroll
+            for (int i = 0; i < kAgain; ++i) {
+                const int64_t at = part0 + 16 * wave + next.row[i];
+                if (i < next.count && lane == 0) a.part_stats[at] = float2{top[i], sum[i]};
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    if (i < next.count && lane + 64 * e < dim)
+                        a.part_out[at * dim + lane + 64 * e] = y[i][e];
+            }
         }
     }
 }

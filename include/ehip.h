@@ -1021,7 +1021,7 @@ int ehip_cache_read_f32(const ehip_cache_t* cache, const int32_t* starts, const 
  * same lengths under another `longest` may differ in the last bits.
  * 1 <= head_dim <= 128, heads a multiple of kv_heads. Heads of a cache in bf16
  * or 8 bits that meet an infinity, whose |scale q| are all below 2^-101, or in 8
- * bits one past 2^111, are formed a second time, at some ten times the cost.
+ * bits one past 2^111, are formed a second time, at some six times the cost.
  * `workspace` (16-byte aligned) holds the parts of split lengths during the
  * call: at least ehip_attention_paged_workspace() bytes, of the call's own.
  * Deterministic. */
@@ -1129,7 +1129,7 @@ int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* g
  * passed whole, as are the groups whose number is negative, past longest_shared or
  * past the table row. Rows that meet an infinity, or a NaN among values, in shared
  * positions, or whose q is as small or large as named there, are formed a second
- * time, at some twenty times the cost. A page outside the pool among the shared
+ * time, at some twelve times the cost. A page outside the pool among the shared
  * positions makes the rows of all that share them NaN. Group offsets out of range or descending are
  * clamped: nothing outside the tensors is read or written, but what the sequences
  * they touch get is unspecified.
