@@ -442,20 +442,22 @@ int launch_mfma(const Paged& a, hipStream_t s) {
     return launch_part_mfma<T, 128, WIDE>(a, s);
 }
 
-// Whether the positions go by waves and the matrix instructions. Two kinds of bf16 heads whose rows are
-// not whole units do not. Few of them: those kernels put the last values in place and spill, and what
-// they take before their first tile is more than the little work, unless many heads share it (us,
-// vector : matrix; one sequence of 64, 16 heads of 77 10.3 : 19.7, of 500 15.2 : 20.6, of 4096 22.9 :
-// 29.7; of 2048, 32 heads over 8 of 77 21.5 : 22.9, of 100 23.7 : 21.6; of 8192, 8 over one of 77 31.5
-// : 26.9; 4 of up to 4096, 32 over 8 of 77 50.8 : 38.2). And single ones of below eight values, which
-// both read one by one (256 of up to 300, 16 of 7, 75 : 95; of 33 101 : 67).
+// Whether the positions go by waves and the matrix instructions. Three kinds of bf16 heads do not, whose
+// work is too little for what those kernels take before their first tile and for a join (us, vector :
+// matrix). Few whole rows, a head a key head: their products have one column of 16 (16 sequences of up
+// to 100, 8 heads of 64, 8.4 : 11.4; one of 4096, 16 heads 10.9 : 12.6; 64 of up to 64 12.5 : 11.5; two
+// heads over one, one sequence of 8192, 12.6 : 13.0, of 8 values 12.5 : 11.0). Few rows that are not
+// whole units: the last values are put in place there, and registers spilled (one sequence of 64, 16
+// heads of 77 10.3 : 19.7, of 4096 22.9 : 29.7; of 2048, 32 heads over 8 of 77 21.5 : 22.9, of 100 23.7
+// : 21.6; of 8192, 8 over one of 77 31.5 : 26.9; 4 of up to 4096, 32 over 8 of 77 50.8 : 38.2). And
+// single ones of below eight values, which both read one by one (256 of up to 300, 16 of 7, 75 : 95;
+// of 33 101 : 67).
 bool waves_of(const Cache& c, int64_t heads, int64_t longest, int type) {
-    if (type == EHIP_CACHE_BF16 && !whole_rows(c, 8)) {
-        const int64_t group = heads / c.kv_heads;
-        const bool few = group <= 4 && c.sequences * heads * longest <= int64_t(1) << 16;
-        return !few && !(group == 1 && c.dim < 8);
-    }
-    return by_waves(type);
+    if (type != EHIP_CACHE_BF16) return by_waves(type);
+    const int64_t group = heads / c.kv_heads;
+    const bool few = c.sequences * heads * longest <= int64_t(1) << 16;
+    if (whole_rows(c, 8)) return !(few && group == 1 && c.sequences <= 16);
+    return !(few && group <= 4) && !(group == 1 && c.dim < 8);
 }
 
 template <int WAVES>
@@ -472,7 +474,12 @@ int paged::launch_parts(const Paged& a, int type, bool waves, hipStream_t s) {
     if (type == EHIP_CACHE_F32)
         return whole_rows(a.c, 4) ? launch_lanes<float, true>(a, s)
                                   : launch_lanes<float, false>(a, s);
-    if (!waves) return launch_lanes<Bf16, false>(a, s);
+    if (!waves && !whole_rows(a.c, 8)) return launch_lanes<Bf16, false>(a, s);
+    if (!waves) {
+        if (a.c.dim <= 32) return launch_part<Bf16, 4, 1, true>(a, s);
+        if (a.c.dim <= 64) return launch_part<Bf16, 8, 1, true>(a, s);
+        return launch_part<Bf16, 16, 1, true>(a, s);
+    }
     if (type == EHIP_CACHE_BF16)
         return whole_rows(a.c, 8) ? launch_mfma<Bf16, true>(a, s) : launch_mfma<Bf16, false>(a, s);
     // Reads of whole pieces in 8 bits: of 16 values, or of 8 in heads of up to 32.

@@ -95,7 +95,7 @@ __device__ __forceinline__ void narrow(float x, Bf16& out) {
 // running maximum, sum and weighted values over the positions they meet, joined at the end: of the
 // wave, the block's four waves, and, where the length is split, the blocks of a sequence by a
 // second launch. Two sequences of 131072 in fp32, 32 heads over 8 of 128 values: 356 us at best,
-// 6.0 TB/s. It takes fp32, and what little there is of bf16 heads at any address (waves_of).
+// 6.0 TB/s. It takes fp32, and bf16 where there is little (waves_of).
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = kPagedThreads / 64;
 constexpr int kUnroll = 4;

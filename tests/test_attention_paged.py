@@ -111,6 +111,39 @@ def test_odd_heads_in_bf16_of_little_and_much_work(hip, d, heads, kv, longest):
 
 @gpu
 @pytest.mark.parametrize("longest", [130, 1 << 20])
+@pytest.mark.parametrize("heads,kv", [(6, 6), (1, 1), (8, 2)])
+@pytest.mark.parametrize("d", [8, 16, 24, 32, 40, 64, 72, 96, 112, 128])
+def test_whole_heads_in_bf16_of_little_and_much_work(hip, d, heads, kv, longest):
+    import torch
+    check(hip, [37, 5, 0, 130, 64], heads, kv, d, 8, torch.bfloat16, seed=d, longest=longest)
+
+
+@gpu
+@pytest.mark.parametrize("which,value", [("k", math.nan), ("k", -math.inf), ("v", math.nan),
+                                         ("v", math.inf)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_little_work_in_bf16_that_is_not_finite(hip, which, value, d):
+    """A key of -inf weighs nothing, whatever its value; an infinite value is its column's."""
+    import torch
+    print_case("paged little not finite", which, value, d)
+    lengths = [130, 40]
+    kp, vp, table, q, want, want_lse = check(hip, lengths, 4, 4, d, 16, torch.bfloat16, seed=32)
+    q[0, 0, 7] = 1.0
+    (kp if which == "k" else vp)[int(table[0, 3]), 2, 0, 7] = value
+    out, lse = hip.attention_paged(q, kp, vp, table, ints(lengths))
+    hit = out[0, 0]
+    if value == -math.inf:
+        assert bool(torch.isfinite(hit).all()) and bool(torch.isfinite(lse).all())
+    elif which == "k":
+        assert bool(torch.isnan(hit).all()) and bool(torch.isnan(lse[0, 0]))
+    else:
+        assert torch.equal(torch.isfinite(hit), torch.arange(d, device="cuda") != 7)
+        assert bool(torch.isnan(hit[7])) == math.isnan(value) and bool(torch.isfinite(lse).all())
+    assert torch.equal(out[0, 1:], want[0, 1:]) and torch.equal(out[1], want[1])
+
+
+@gpu
+@pytest.mark.parametrize("longest", [130, 1 << 20])
 @pytest.mark.parametrize("which,value", [("k", math.nan), ("k", math.inf), ("v", math.nan),
                                          ("v", -math.inf)])
 def test_odd_heads_in_bf16_that_are_not_finite(hip, which, value, longest):
