@@ -96,12 +96,14 @@ __device__ __forceinline__ float kl_series(float x) {
     for (int n = 13; n >= 3; --n) s = __builtin_fmaf(x * (1.0f / float(n)), s, 1.0f);
     return 0.5f * x * x * s;
 }
-// The same of any x, past fp32 too, whose exponential is the square of that of its half.
-__device__ __forceinline__ double kl_of(float x) {
-    const double h = double(expf(0.5f * x));
-    const double kl = __builtin_fma(h, h, -1.0) - double(x);
-    if (fabsf(x) == INFINITY) return INFINITY;
-    return fabsf(x) < 1.0f ? double(kl_series(x)) : kl;
+// 2^-40 of the same of any x: past fp32 up to x = 115, which is more than a mean over all the tokens that
+// there can be brings back. The exponential is the square of that of the half. (In 64 bits the kernel
+// of 2 million tokens took 19.2 us in place of 17.9.)
+constexpr float kKlUnit = 0x1p-40f;
+__device__ __forceinline__ float kl_of(float x) {
+    const float h = expf(0.5f * x) * 0x1p-20f;
+    const float kl = __builtin_fmaf(h, h, -kKlUnit) - fminf(x, 1e30f) * kKlUnit;  // not inf - inf
+    return fabsf(x) < 1.0f ? kl_series(x) * kKlUnit : kl;
 }
 
 // exp(x): 2^n exp(f), |f| <= ln 2 / 2, by Taylor's series, whose next term is 2^-37 of it. A third of
@@ -149,7 +151,8 @@ __device__ __forceinline__ bool clipped(const Policy& a, double d, float advanta
 // A token's terms. The loss's sum takes 64 bits, as it has terms of both signs (340 tokens' of about 1
 // have come to 10^-3; 17 us in place of the 14 in 32 bits).
 struct Token {
-    double ratio, surrogate, kl;
+    double ratio, surrogate;
+    float kl;  // kKlUnit of it
     bool clipped;
 };
 
@@ -160,7 +163,7 @@ __device__ __forceinline__ Token token_of(const Policy& a, const Tokens& from, i
     x.ratio = exp36(d);
     x.clipped = clipped(a, d, advantage);
     x.surrogate = (x.clipped ? (advantage < 0.0f ? a.low : a.high) : x.ratio) * double(advantage);
-    x.kl = a.ref != nullptr ? kl_of(float(double(from.ref[i]) - double(from.p[i]))) : 0.0;
+    x.kl = a.ref != nullptr ? kl_of(float(double(from.ref[i]) - double(from.p[i]))) : 0.0f;
     return x;
 }
 
@@ -200,12 +203,13 @@ __device__ __forceinline__ void sum_segment(const Policy& a, int64_t place, Sums
             if (t + 64 * i >= g.end) break;
             const Token y = token_of(a, all, i);
             double loss = -y.surrogate;
-            if (a.kl_weight != 0.0f) loss = __builtin_fma(double(a.kl_weight), y.kl, loss);
+            const double kl = double(y.kl) * (1.0 / kKlUnit);
+            if (a.kl_weight != 0.0f) loss = __builtin_fma(double(a.kl_weight), kl, loss);
             if (a.entropy_weight != 0.0f)
                 loss = __builtin_fma(-double(a.entropy_weight), double(all.entropy[i]), loss);
             const bool counts = all.counts[i];
             x.loss += counts ? loss : 0.0;
-            x.kl += counts ? y.kl : 0.0;
+            x.kl += counts ? kl : 0.0;
             x.ratio += counts ? y.ratio : 0.0;
             x.clipped += counts && y.clipped;
             x.tokens += counts;
