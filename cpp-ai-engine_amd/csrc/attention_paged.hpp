@@ -591,19 +591,17 @@ __global__ __launch_bounds__(kPagedThreads, G >= 4 ? 2 : 3) void paged_part(Page
     }
 }
 
-// Up to kAgain heads' share of a segment by the formula, for those whose sums by parts are not finite: a
+// Up to AGAIN heads' share of a segment by the formula, for those whose sums by parts are not finite: a
 // part of an infinity, or an infinity times the parts of a finite value, is NaN where the product is
 // an infinity or, its weight 0, nothing at all. One wave, a lane for each of 64 positions at a time; a
 // score of NaN or +inf settles its head as NaN. Each segment's wave forms its own, so its reads are
 // several at a time and serve four heads (64 sequences of 1024, 32 heads over 8 of 128 values, us, bf16
 // and 8 bits: finite 52 and 37; the first key NaN 69 and 48, a head and a read at a time 82 and 98; the
 // first value infinite 274 and 130, and 623 and 555).
-constexpr int kAgain = 4;
-
-template <class T, int DP>
-__device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&q)[kAgain], int kv,
-                                int begin, int end, float (&top)[kAgain], float (&sum)[kAgain],
-                                float (&o)[kAgain][2]) {
+template <class T, int DP, int AGAIN>
+__device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&q)[AGAIN], int kv,
+                                int begin, int end, float (&top)[AGAIN], float (&sum)[AGAIN],
+                                float (&o)[AGAIN][2]) {
     using attention::uintx4;
     constexpr int kReads = DP > 64 ? 4 : 2;  // more than the tiles leave registers for hold up those
     int lane = int(threadIdx.x) & 63;
@@ -623,14 +621,14 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&
     };
     // Rows of 16-byte units, or others four values at a time at any address.
     const bool units = sizeof(T) == 2 && dim % 8 == 0 && aligned16(a.c.k);
-    const auto scores = [&](int row, float (&dot)[kAgain]) {
+    const auto scores = [&](int row, float (&dot)[AGAIN]) {
         const T* at = k + int64_t(row) * pitch;
         const float by = sizeof(T) == 1 ? a.c.k_scales[place] : 1.0f;
 #pragma unroll
-        for (int g = 0; g < kAgain; ++g) dot[g] = 0.0f;
+        for (int g = 0; g < AGAIN; ++g) dot[g] = 0.0f;
         const auto add = [&](int e, float x) {
 #pragma unroll
-            for (int g = 0; g < kAgain; ++g) dot[g] = __builtin_fmaf(q[g][e] * c2, x, dot[g]);
+            for (int g = 0; g < AGAIN; ++g) dot[g] = __builtin_fmaf(q[g][e] * c2, x, dot[g]);
         };
         int e = 0;
         if (units) {
@@ -671,10 +669,10 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&
         }
         for (; e < dim; ++e) add(e, sizeof(T) == 1 ? widen(at[e]) * by : widen(at[e]));
     };
-    float x[kAgain], shift[kAgain];
-    bool settled[kAgain], all = false;
+    float x[AGAIN], shift[AGAIN];
+    bool settled[AGAIN], all = false;
 #pragma unroll
-    for (int g = 0; g < kAgain; ++g) {
+    for (int g = 0; g < AGAIN; ++g) {
         top[g] = -INFINITY;
         settled[g] = false;
     }
@@ -682,14 +680,14 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&
         scores(row_of(p0), x);
         all = true;
 #pragma unroll
-        for (int g = 0; g < kAgain; ++g) {
+        for (int g = 0; g < AGAIN; ++g) {
             settled[g] = settled[g] || __any(!(x[g] < INFINITY));
             all = all && settled[g];
             top[g] = fmaxf(top[g], x[g]);
         }
     }
 #pragma unroll
-    for (int g = 0; g < kAgain; ++g) {
+    for (int g = 0; g < AGAIN; ++g) {
 #pragma unroll
         for (int w = 32; w > 0; w >>= 1) top[g] = fmaxf(top[g], __shfl_xor(top[g], w));
         shift[g] = top[g] == -INFINITY ? 0.0f : top[g];  // scores of -inf alone weigh nothing
@@ -701,7 +699,7 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&
         const int row = row_of(p0), count = min(64, end - p0);
         scores(row, x);
 #pragma unroll
-        for (int g = 0; g < kAgain; ++g) {
+        for (int g = 0; g < AGAIN; ++g) {
             x[g] = lane < count ? exp2f(x[g] - shift[g]) * 0x1p-24f : 0.0f;
             sum[g] += x[g];
         }
@@ -728,7 +726,7 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&
                     y[e] = u < count ? y[e] : 0.0f;
                 }
 #pragma unroll
-                for (int g = 0; g < kAgain; ++g) {
+                for (int g = 0; g < AGAIN; ++g) {
                     const float w = __shfl(x[g], u);
                     o[g][0] = __builtin_fmaf(w, y[0], o[g][0]);
                     o[g][1] = __builtin_fmaf(w, y[1], o[g][1]);
@@ -737,7 +735,7 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&
         }
     }
 #pragma unroll
-    for (int g = 0; g < kAgain; ++g) {
+    for (int g = 0; g < AGAIN; ++g) {
 #pragma unroll
         for (int w = 32; w > 0; w >>= 1) sum[g] += __shfl_xor(sum[g], w);
         if (settled[g]) top[g] = 0.0f, sum[g] = NAN;
@@ -746,11 +744,12 @@ __device__ void part_by_formula(const Paged& a, int64_t s, const float* const (&
 }
 
 // The next rows of a set, the last again past its end, which is cleared of them.
+template <int AGAIN>
 struct Again {
-    int row[kAgain], count;
+    int row[AGAIN], count;
     __device__ __forceinline__ explicit Again(uint32_t& rows) : count(0) {
 #pragma unroll
-        for (int g = 0; g < kAgain; ++g) {
+        for (int g = 0; g < AGAIN; ++g) {
             row[g] = rows != 0 ? __builtin_ctz(rows) : row[g > 0 ? g - 1 : 0];
             count += rows != 0;
             rows &= rows - 1;
@@ -903,7 +902,7 @@ struct alignas(16) PartLds {
     float scales[kPagedWaves][2][kTilePositions];
 };
 
-template <class T, int DP, bool WIDE, bool SHARED>
+template <class T, int DP, bool WIDE, bool SHARED, int AGAIN>
 __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, PartLds<DP>& lds) {
     constexpr bool kScaled = sizeof(T) == 1;
     using attention::bf16x8;
@@ -1200,14 +1199,14 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
         }
         if (bad) continue;
         while (again != 0) {
-            const Again some(again);
-            const float* rows[kAgain];
+            const Again<AGAIN> some(again);
+            const float* rows[AGAIN];
 #pragma unroll
-            for (int i = 0; i < kAgain; ++i) rows[i] = query_row<SHARED>(a, seg, kv, h0, some.row[i]);
-            float top[kAgain], sum[kAgain], y[kAgain][2];
-            part_by_formula<T, DP>(a, s, rows, kv, begin, end, top, sum, y);
+            for (int i = 0; i < AGAIN; ++i) rows[i] = query_row<SHARED>(a, seg, kv, h0, some.row[i]);
+            float top[AGAIN], sum[AGAIN], y[AGAIN][2];
+            part_by_formula<T, DP, AGAIN>(a, s, rows, kv, begin, end, top, sum, y);
 #pragma unroll
-            for (int i = 0; i < kAgain; ++i) {
+            for (int i = 0; i < AGAIN; ++i) {
                 const int g = some.row[i];
                 const int64_t place = part_of<SHARED>(a, seg, worker, kv, h0, g);
                 if (i < some.count && lane == 0) {
@@ -1230,7 +1229,7 @@ __device__ __forceinline__ void part_by_waves(const Paged& a, uint32_t block, Pa
 template <class T, int DP, bool WIDE>
 __global__ __launch_bounds__(kPagedThreads, 2) void paged_part_mfma(Paged a) {
     __shared__ PartLds<DP> lds;
-    part_by_waves<T, DP, WIDE, false>(a, blockIdx.x, lds);
+    part_by_waves<T, DP, WIDE, false, 4>(a, blockIdx.x, lds);
 }
 
 // Parts of a row, `stride` rows apart.

@@ -85,6 +85,11 @@ __device__ __forceinline__ void multiply_small(floatx4& d0, const bf16x8 (&x0)[P
 // of 128 values in 8 bits, 130 us: 230 TFLOP/s of the 470 that three products for one leave; matrix
 // instructions take 35 % of the time and vector ones half of it, with two waves a SIMD.
 constexpr int kKeys = 32;  // positions of a step
+// Rows that are formed a second time together. Four want registers of the tiles (32 heads over 8 of 128, us:
+// 8 groups of up to 16 over up to 6000 positions in bf16, two 64.6, four 65.6; 64 over 30000 in 8 bits
+// 128 and 130; 64 over 16000, heads of 100, 91 and 94; an infinity in the first value, 2 groups of 32
+// over 4000 in 8 bits, 407 and 344).
+constexpr int kSharedAgain = 2;
 
 template <class T, int DP>
 struct alignas(16) RowsLds {
@@ -406,15 +411,15 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
             }
         }
         while (again != 0) {
-            const Again next(again);
-            const float* rows[kAgain];
+            const Again<kSharedAgain> next(again);
+            const float* rows[kSharedAgain];
 #pragma unroll
-            for (int i = 0; i < kAgain; ++i)
+            for (int i = 0; i < kSharedAgain; ++i)
                 rows[i] = query_row<true>(a, seg, kv, 0, 16 * wave + next.row[i]);
-            float top[kAgain], sum[kAgain], y[kAgain][2];
-            part_by_formula<T, DP>(a, s, rows, kv, begin, end, top, sum, y);
+            float top[kSharedAgain], sum[kSharedAgain], y[kSharedAgain][2];
+            part_by_formula<T, DP, kSharedAgain>(a, s, rows, kv, begin, end, top, sum, y);
 #pragma unroll
-            for (int i = 0; i < kAgain; ++i) {
+            for (int i = 0; i < kSharedAgain; ++i) {
                 const int64_t at = part0 + 16 * wave + next.row[i];
                 if (i < next.count && lane == 0) a.part_stats[at] = float2{top[i], sum[i]};
 #pragma unroll
@@ -437,11 +442,11 @@ __global__ __launch_bounds__(kPagedThreads, 2) void shared_parts(Paged own, Page
         RowsLds<T, DP> rows;
     } lds;
     if (blockIdx.x < own_blocks)
-        part_by_waves<T, DP, WIDE, false>(own, blockIdx.x, lds.part);
+        part_by_waves<T, DP, WIDE, false, kSharedAgain>(own, blockIdx.x, lds.part);
     else if constexpr (ROWS)
         part_by_rows<T, DP, WIDE>(a, blockIdx.x - own_blocks, lds.rows);
     else
-        part_by_waves<T, DP, WIDE, true>(a, blockIdx.x - own_blocks, lds.part);
+        part_by_waves<T, DP, WIDE, true, kSharedAgain>(a, blockIdx.x - own_blocks, lds.part);
 }
 
 // Apart where the own positions go by the vector kernel.

@@ -1129,7 +1129,7 @@ int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* g
  * passed whole, as are the groups whose number is negative, past longest_shared or
  * past the table row. Rows that meet an infinity, or a NaN among values, in shared
  * positions, or whose q is as small or large as named there, are formed a second
- * time, at some twelve times the cost. A page outside the pool among the shared
+ * time, at some twenty times the cost. A page outside the pool among the shared
  * positions makes the rows of all that share them NaN. Group offsets out of range or descending are
  * clamped: nothing outside the tensors is read or written, but what the sequences
  * they touch get is unspecified.
