@@ -414,8 +414,9 @@ int launch_group(const Paged& a, hipStream_t s) {
     const int64_t group = a.heads / a.c.kv_heads;
     if (group == 1) return launch_part<T, LPP, 1, VEC>(a, s);
     if (group == 2) return launch_part<T, LPP, 2, VEC>(a, s);
-    if (group <= 4) return launch_part<T, LPP, 4, VEC>(a, s);
-    return launch_part<T, LPP, 8, VEC>(a, s);
+    if constexpr (sizeof(T) == 4)  // bf16 comes with up to four
+        if (group > 4) return launch_part<T, LPP, kMaxGroup, VEC>(a, s);
+    return launch_part<T, LPP, 4, VEC>(a, s);
 }
 
 template <class T, bool VEC>
