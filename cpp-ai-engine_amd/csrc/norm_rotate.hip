@@ -9,7 +9,7 @@
 // HBM bounds it: a head is read once, in registers of a few lanes, and written. The angles are
 // formed here, in 64 bits from the product to the quarter turn (a position of a million is some
 // 10^5 turns, whose fraction fp32 does not have), once for a wave's heads of a token. 369 MB of
-// query and key heads of 128 take 87 us, 4.2 TB/s; 134 MB of heads of 64 26 us, 5.2 TB/s, and back
+// query and key heads of 96 take 87 us, 4.2 TB/s; 134 MB of heads of 64 26 us, 5.2 TB/s, and back
 // 201 MB 44 us, 4.6 TB/s, with 5 for the weights' gradients.
 
 #include "common.hpp"

@@ -8,7 +8,7 @@
 //   dp = w (-[not clipped] ratio A + beta (1 - exp(f - p))), dH = -c w
 //
 // HBM bounds long batches, latency short ones. Over 2 million tokens of 2048 sequences with all
-// tensors the sums take 17 us (42 MB, 2.4 TB/s), joining them 7, the gradient 14 (50 MB, 3.5 TB/s);
+// tensors the sums take 18 us (42 MB, 2.4 TB/s), joining them 7, the gradient 14 (50 MB, 3.7 TB/s);
 // the arithmetic of some 60 to 80 operations a token is not hidden by the loads altogether. The
 // flat tokens are cut into chunks of kChunk and a wave takes what one sequence has of one chunk, a
 // segment. The segment of chunk c and sequence s has place c + s, no other's: from one to the next

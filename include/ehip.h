@@ -1077,7 +1077,8 @@ int ehip_token_logprobs_backward_f32(const float* logits, int64_t ld, const int3
  * the values past them are y. positions (tokens int32, any value) and freqs
  * (rotary / 2 doubles) are DEVICE arrays; the angle's product and its turns are
  * formed in 64 bits. With rotary = 0 both may be NULL. Squares are summed in
- * fp32: of values of 2^63 and more the norm is not finite.
+ * fp32: with values of 2^63 and more the mean may be an infinity and the head
+ * zeros, and with an eps of 0 one whose values are all below 2^-63 is not exact.
  * q are rows of heads * head_dim floats, k of kv_heads * head_dim, ld_* apart
  * (columns of a fused projection); either may have no heads (and be NULL).
  * 1 <= head_dim <= 256, rotary even and at most head_dim. q_out may be q with
@@ -1119,7 +1120,11 @@ int ehip_norm_rotate_backward_f32(const ehip_norm_rotate_t* desc, const float* g
  * groups + 1 ascending int32, and shares shared[g] positions (a DEVICE array; at
  * most longest_shared, a host value that the work is split by): they are read
  * through the table row of its first sequence, the others through each
- * sequence's own, so what a page holds of both may be there twice. The result is
+ * sequence's own, so what a page holds of both may be there twice. It pays where
+ * (sequences - groups) shared positions are some 60000 and more (8 key heads of
+ * 128; 30000 in fp32); below, ehip_attention_paged_f32 takes up to 20 us less. How
+ * shared positions are passed goes by the mean of all sequences a group: sequences
+ * in groups of their own beside a large one can cost it a third. The result is
  * that of ehip_attention_paged_f32 with the rest of its arguments, up to the last
  * bits, if the table rows of a group lead to the same shared positions (that of
  * the first sequence also where that one's length is none or shorter). In fp32 too
