@@ -434,9 +434,12 @@ __device__ __forceinline__ void part_by_rows(const Paged& a, uint32_t block,
 // The shared positions' parts, after those of the sequences' own: one launch, whose blocks of the one
 // kind begin where blocks of the other end. ROWS: part_by_rows. (8 groups of up to 64 rows over up to
 // 6000 shared positions and 1024 own ones, 32 heads over 8 of 128, bf16: 171 MB in 52 us, 3.3 TB/s.)
+// bf16 heads of up to 64 are held to three waves a SIMD, a register or two below what they take (8 groups
+// of 16 over 4000, 32 heads over 8 of 64: 46.5 us, two waves 48.7; one of 64 over 16000 62.1, 60.2; 8 bits
+// have three as they are).
 template <class T, int DP, bool WIDE, bool ROWS>
-__global__ __launch_bounds__(kPagedThreads, 2) void shared_parts(Paged own, Paged a,
-                                                                 uint32_t own_blocks) {
+__global__ __launch_bounds__(kPagedThreads, sizeof(T) == 2 && DP <= 64 && WIDE ? 3 : 2) void
+shared_parts(Paged own, Paged a, uint32_t own_blocks) {
     __shared__ union Lds {
         PartLds<DP> part;
         RowsLds<T, DP> rows;
