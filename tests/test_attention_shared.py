@@ -484,6 +484,27 @@ def test_small_queries_and_large_keys(hip, power, members, kind):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["float32", "bfloat16"])
+@pytest.mark.parametrize("members", [3, 40])
+@pytest.mark.parametrize("power", [100, 110, 118, 124])
+def test_small_keys_and_large_queries(hip, power, members, kind):
+    """Shared fp32 keys are taken to 2^-134: a score is off by that times the sum of its |scale q|, the
+    weights by twice the largest of that, relative, and lse by it. bf16 keys are exact."""
+    print_case("shared small k", power, members, kind)
+    b = Batch(hip, [(300, [2] * members), (40, [1, 1])], 4, 2, 64, 16, kind, seed=24)
+    b.q.mul_(2.0 ** power)
+    b.kp = (b.kp.float() * 2.0 ** -power).to(b.kp.dtype)
+    out, lse = b.run(hip)
+    value, bound = b.expect()
+    off = 0.0 if kind == "bfloat16" else (
+        1.01 * 2.0 ** -134 * b.q.cpu().double().abs().sum(-1) * b.d ** -0.5)
+    largest = float(b.vp.float().abs().max())
+    within(out, value["out"], bound["out"] + (2 * off * largest)[..., None] if kind == "float32"
+           else bound["out"], "out")
+    within(lse, value["lse"], bound["lse"] + off, "lse")
+
+
+@gpu
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("members", [3, 40])
 @pytest.mark.parametrize("which", ["k", "v"])
